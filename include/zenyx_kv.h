@@ -458,6 +458,80 @@ int zx_paged_attention_ring_ws(const uint16_t *q, int64_t n_q, const int32_t *cu
 int zx_ring_shard_bounds(const int32_t *kv_len, int32_t n_seqs, int32_t degree, int32_t row_stride,
                          int32_t *kv_begin, int32_t *kv_end, zx_stream_t stream);
 
+/* ---------------------------------------------------------------------------
+ * Rotary positions (ABI version 9).  Pair (x1, x2) of a head's first rot_dim channels at
+ * position p becomes (x1 c - x2 s, x2 c + x1 s), c and s from row p of an fp32 table
+ * [n_pos][rot_dim]: rot_dim / 2 cosines, then as many sines.  Pair i is channels
+ * (i, i + rot_dim / 2), or (2 i, 2 i + 1) with ZX_ROPE_INTERLEAVED.  Products and sum are
+ * rounded to fp32 each, the result once to the tensor's type.  rot_dim is a multiple of 16.
+ */
+enum {
+  ZX_ROPE_INTERLEAVED = 16, /* pairs of neighbouring channels */
+  ZX_ROPE_TRANSPOSE = 32    /* the transposed rotation (s negated): the gradient's way back */
+};
+/* The table of angles p * inv_freq[i] (device, 64 bits; the angles are formed in 64 bits),
+ * cosines and sines times `scale`. */
+int zx_rope_table(const double *inv_freq, int32_t rot_dim, int64_t n_pos, double scale, float *out,
+                  zx_stream_t stream);
+/* Rows x[n_rows][n_heads][head_dim] of `dtype`, strides in elements (channels contiguous, rows
+ * of a head 16-byte aligned), row i at positions[i] (device int32).  Channels from rot_dim on
+ * are copied.  out may be x (then with its strides) and must not overlap it otherwise.  A row
+ * whose position is outside [0, n_pos) is copied and sets ZX_KERR_POS_RANGE in *err (may be
+ * NULL).  head_dim is a multiple of 8. */
+int zx_rope(const void *x, int dtype, int64_t n_rows, int32_t n_heads, int32_t head_dim, int64_t x_row_stride,
+            int64_t x_head_stride, const float *table, int64_t n_pos, int32_t rot_dim, const int32_t *positions,
+            int32_t flags, void *out, int64_t out_row_stride, int64_t out_head_stride, int32_t *err,
+            zx_stream_t stream);
+
+/* zx_kv_quant_append with the keys rotated by their positions on the way (rounded to bf16 as
+ * zx_rope rounds them, then quantised): the codes and scales of zx_rope followed by
+ * zx_kv_quant_append, without the rotated copy.  flags: ZX_APPEND_STATIC_SCALES,
+ * ZX_APPEND_SATURATE, ZX_ROPE_INTERLEAVED.  A token at or beyond n_pos is not stored and sets
+ * ZX_KERR_POS_RANGE; dynamic scales are taken over the tokens that have a position (rows
+ * outside [cu_seqlens[0], cu_seqlens[n_seqs]) have none).  workspace:
+ * zx_kv_rope_append_workspace_bytes() device bytes, 16-byte aligned. */
+size_t zx_kv_rope_append_workspace_bytes(int32_t n_layers, int64_t n_tok, int32_t n_heads, int32_t head_dim);
+int zx_kv_rope_append(const uint16_t *x, int64_t x_layer_stride, int32_t n_layers, int64_t n_tok, int32_t n_heads,
+                      int32_t head_dim, const float *table, int64_t n_pos, int32_t rot_dim,
+                      const int32_t *cu_seqlens, const int32_t *start_pos, int32_t n_seqs,
+                      const int32_t *block_tables, int32_t max_blocks, int32_t page_size, uint8_t *pool,
+                      int64_t pool_layer_stride, int64_t n_pages, float *scales, int32_t flags, int32_t *err,
+                      void *workspace, size_t workspace_bytes, zx_stream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * 4-bit KV pages (ABI version 9).  32 channels of a token, K or V, head are a block: e2m1 codes
+ * (0, 1/2, 1, 3/2, 2, 3, 4, 6 and their negatives; nearest, ties to the even code) times the
+ * smallest power of two 2^(byte - 127) >= 2^-125 that brings the block's largest magnitude to 6
+ * or below.  A block with a NaN, an infinity or a magnitude >= 1.75 x 2^127 is NaN (byte 255).
+ * Decoding is exact in bf16.  Pool layer [n_pages][2][H][P / 16][17 D / 2] bytes: tiles of 16
+ * tokens, codes [D / 32][16][16 bytes] (the even channel in a byte's low half), then power
+ * bytes [D / 32][16].  head_dim 64, 128 or 256, page_size a multiple of 16.
+ */
+/* Paged append of x[L][n_tok][2][H][D] bf16 (arguments as zx_kv_quant_append); with a table
+ * (may be NULL) the keys are rotated first, as zx_rope does.  flags: ZX_ROPE_INTERLEAVED.
+ * Tokens at bad pages or positions are not stored and set their bits in *err.  workspace:
+ * zx_kv4_append_workspace_bytes() device bytes, 16-byte aligned. */
+size_t zx_kv4_append_workspace_bytes(int64_t n_tok);
+int zx_kv4_append(const uint16_t *x, int64_t x_layer_stride, int32_t n_layers, int64_t n_tok, int32_t n_heads,
+                  int32_t head_dim, const float *table, int64_t n_pos, int32_t rot_dim, const int32_t *cu_seqlens,
+                  const int32_t *start_pos, int32_t n_seqs, const int32_t *block_tables, int32_t max_blocks,
+                  int32_t page_size, uint8_t *pool, int64_t pool_layer_stride, int64_t n_pages, int32_t flags,
+                  int32_t *err, void *workspace, size_t workspace_bytes, zx_stream_t stream);
+/* One layer's sequences as contiguous bf16 (k_out, v_out [n_seqs][H][out_len][D]; semantics as
+ * zx_kv_gather_dequant). */
+int zx_kv4_gather_dequant(const uint8_t *pool, int64_t n_pages, int32_t n_heads, int32_t head_dim, int32_t page_size,
+                          const int32_t *block_tables, int32_t max_blocks, const int32_t *seq_lens, int32_t n_seqs,
+                          int32_t out_len, uint16_t *k_out, uint16_t *v_out, int32_t *err, zx_stream_t stream);
+/* Decode attention from 4-bit pages: as zx_paged_attention_decode (softmax weights carried to
+ * 2^-17, sums in fp32, rounded once to bf16), any n_q_heads / n_kv_heads. */
+size_t zx_paged_attention4_decode_workspace_bytes(int32_t n_seqs, int32_t n_q_heads, int32_t n_kv_heads,
+                                                  int32_t head_dim, int32_t max_blocks, int32_t page_size);
+int zx_paged_attention4_decode(const uint16_t *q, int32_t n_q_heads, const uint8_t *pool, int64_t n_pages,
+                               int32_t n_kv_heads, int32_t head_dim, int32_t page_size, const int32_t *block_tables,
+                               int32_t max_blocks, const int32_t *seq_lens, int32_t n_seqs, float sm_scale,
+                               uint16_t *out, int32_t *err, void *workspace, size_t workspace_bytes,
+                               zx_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -33,7 +33,8 @@ ZX_PREFILL_FINAL = 64
 ZX_HEADS_TWO_PASS = 1
 ZX_HEADS_SINGLE_PASS = 2
 ZX_NEVER = 0x7FFFFFFF
-ABI_VERSION = 8
+ZX_ROPE_INTERLEAVED, ZX_ROPE_TRANSPOSE = 16, 32
+ABI_VERSION = 9
 
 _P = ctypes.c_void_p
 _I64, _I32, _SZ, _INT = ctypes.c_int64, ctypes.c_int32, ctypes.c_size_t, ctypes.c_int
@@ -85,6 +86,18 @@ SIGNATURES = {
                                           _P, _I32, _I32, _I32, _I32, ctypes.c_float, _I32, _P, _P, _P, _P, _P, _SZ,
                                           _P]),
     "zx_ring_shard_bounds": (_INT, [_P, _I32, _I32, _I32, _P, _P, _P]),
+    "zx_rope_table": (_INT, [_P, _I32, _I64, ctypes.c_double, _P, _P]),
+    "zx_rope": (_INT, [_P, _INT, _I64, _I32, _I32, _I64, _I64, _P, _I64, _I32, _P, _I32, _P, _I64, _I64, _P, _P]),
+    "zx_kv_rope_append_workspace_bytes": (_SZ, [_I32, _I64, _I32, _I32]),
+    "zx_kv_rope_append": (_INT, [_P, _I64, _I32, _I64, _I32, _I32, _P, _I64, _I32, _P, _P, _I32, _P, _I32, _I32, _P,
+                                 _I64, _I64, _P, _I32, _P, _P, _SZ, _P]),
+    "zx_kv4_append_workspace_bytes": (_SZ, [_I64]),
+    "zx_kv4_append": (_INT, [_P, _I64, _I32, _I64, _I32, _I32, _P, _I64, _I32, _P, _P, _I32, _P, _I32, _I32, _P,
+                             _I64, _I64, _I32, _P, _P, _SZ, _P]),
+    "zx_kv4_gather_dequant": (_INT, [_P, _I64, _I32, _I32, _I32, _P, _I32, _P, _I32, _I32, _P, _P, _P, _P]),
+    "zx_paged_attention4_decode_workspace_bytes": (_SZ, [_I32, _I32, _I32, _I32, _I32, _I32]),
+    "zx_paged_attention4_decode": (_INT, [_P, _I32, _P, _I64, _I32, _I32, _I32, _P, _I32, _P, _I32, ctypes.c_float,
+                                          _P, _P, _P, _SZ, _P]),
 }
 
 _lib = None

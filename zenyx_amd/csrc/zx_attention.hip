@@ -9,7 +9,7 @@
 //
 // Split-K flash decoding with the work dealt evenly.  The positions of all sequences are cut
 // into units (what the four waves of a block take per step), laid end to end, and every
-// block of a (kv head, group of query heads) takes an equal run of units (att_locate), so
+// block of a (kv head, group of query heads) takes an equal run of units (att_locate, zx_attn_deal.h), so
 // sequences of different lengths leave no block empty and none late.  A run may end one
 // sequence and begin the next: each part of it that lies in one sequence is a segment, with
 // its own running softmax.  A segment that is a whole sequence is finished by its block;
@@ -36,161 +36,12 @@
 // 64 x 512-4k 90 -> 59 us; 1,024 x 600 273 -> 225 us; 64 x 32k 673 -> 663 us (6.5 TB/s).
 #include <algorithm>
 
-#include "zx_attn_common.h"
+#include "zx_attn_deal.h"
 
 namespace zx {
 
-constexpr int ATT_THREADS = 256;  // 4 waves
-constexpr int ATT_WAVES = ATT_THREADS / 64;
 constexpr int ATT_U = 4;          // passes per online-softmax step
 constexpr int AM_ROWS = 16;  // query heads a block of the matrix-core variant can hold (the M rows of a tile)
-
-struct AttnGeom {
-  int32_t n_q_heads, n_kv_heads, head_dim, page_size, max_blocks, n_seqs;
-  int32_t n_run;        // equal runs, one block per head group each
-  uint32_t unit, cap;   // positions per unit (a power of two); positions a block table holds
-  uint32_t tail;        // see att_take_whole
-  int32_t whole;        // every sequence is taken whole: known to the host
-  int32_t group, n_group;       // query heads per block; groups of them
-  uint32_t p_magic;  // t / page_size = (t * p_magic) >> (31 + p_shift) for t < 2^31
-  int32_t p_shift;
-  int64_t n_pages;
-  float sm_scale;
-};
-
-__device__ __forceinline__ uint32_t page_of(const AttnGeom &g, uint32_t t) {
-  return (uint32_t)(((uint64_t)t * g.p_magic) >> (31 + g.p_shift));
-}
-
-// Positions of a sequence that are attended to (lengths are int32).
-__device__ __forceinline__ uint32_t att_live_len(const AttnGeom &g, int32_t len) {
-  return len > 0 ? min((uint32_t)len, g.cap) : 0u;
-}
-__device__ __forceinline__ uint32_t att_units(const AttnGeom &g, int32_t len) {
-  return (att_live_len(g, len) + (g.unit - 1)) / g.unit;  // unit: a power of two
-}
-
-// The U units of all sequences dealt to n_run runs: run x takes q = U / n_run of them, the
-// first r = U % n_run one more.  T: 32 bits where U fits.
-template <typename T> struct AttnDeal {
-  T q, r;
-  __device__ AttnDeal(T q_, T r_) : q(q_), r(r_) {}
-  __device__ T begin(T x) const { return x * q + min(x, r); }
-  __device__ T run_of(T u) const { return u < r * (q + 1) ? u / (q + 1) : r + (u - r * (q + 1)) / q; }
-};
-
-// Whole sequences instead of equal runs?  A run starts anew in every sequence that it touches
-// (q, the first page ids, K and V one after the other: about as long as four units) and its
-// parts are merged; whole sequences leave blocks idle while the longest one ends.  With as many
-// sequences as runs or more, where most runs would start anew anyway: if the longest one has
-// at most ATT_TAIL_MANY positions and an eighth of an equal share.  Else if it exceeds a share
-// by at most ATT_TAIL_ONE units.  (g.tail: that slack in units; a call whose longest sequence
-// is within it needs no sums.)  In a graph, Hq 32 / Hkv 8, D = 128, tables of 32k positions:
-// 512 x 100-500 139 us in runs, 90 whole; 4 x 100-500 10.9 in runs, 16.3 whole; 64 x 512-4k
-// 59 in runs, 73 whole.
-constexpr uint32_t ATT_TAIL_ONE = 2, ATT_TAIL_MANY = 1024;
-__device__ __forceinline__ bool att_take_whole(const AttnGeom &g, uint64_t most, uint64_t share) {
-  return most <= g.tail + (g.n_seqs < g.n_run ? share : share / 8);
-}
-
-// Inclusive sum over the lanes below n (n <= 64, uniform).
-__device__ __forceinline__ uint32_t att_scan(uint32_t v, int n) {
-  const int lane = threadIdx.x & 63;
-  for (int off = 1; off < n; off <<= 1) {
-    const uint32_t y = __shfl_up(v, off, 64);
-    if (lane >= off) v += y;
-  }
-  return v;
-}
-
-// More than 64 sequences: what every block needs to know, computed once by att_plan_kernel.
-struct AttnTable {
-  uint64_t *head;   // [4]: whole sequences?, q, r
-  uint64_t *first;  // [n_seqs] a sequence's first unit
-  int32_t *x0, *n_live;  // [n_seqs] the first run that holds a part of it, and how many do
-  int32_t *run_b;        // [n_run] the sequence in which a run begins
-  __host__ __device__ AttnTable(void *at, int64_t n_seqs) {
-    head = static_cast<uint64_t *>(at);
-    first = head + 4;
-    x0 = reinterpret_cast<int32_t *>(first + n_seqs);
-    n_live = x0 + n_seqs;
-    run_b = n_live + n_seqs;
-  }
-  static size_t bytes(int64_t n_seqs, int64_t n_run) {
-    return 4 * sizeof(uint64_t) + (size_t)n_seqs * (sizeof(uint64_t) + 2 * sizeof(int32_t)) +
-           (size_t)n_run * sizeof(int32_t);
-  }
-};
-
-// The run of block x: units [u, u_end), unit u in sequence b, whose first unit is b_first.
-// All block-uniform; an empty run has u == u_end.  Up to 64 sequences every lane keeps one
-// sequence's length, so that stepping to the next sequence reads no memory.
-struct AttnRun {
-  uint64_t u, u_end, b_first;
-  int32_t b, lane_len;
-  int32_t x, y;  // the run (or sequence) and the group of query heads
-};
-__device__ __forceinline__ int32_t att_len(const AttnGeom &g, const int32_t *seq_lens, const AttnRun &r) {
-  return g.n_seqs <= 64 ? __builtin_amdgcn_readlane(r.lane_len, r.b) : seq_lens[r.b];
-}
-// Lane b's units, and how up to 64 sequences are dealt: whole, or units [begin(x), begin(x +
-// 1)) to run x, where incl is the inclusive sum over the sequences.
-struct AttnLanes {
-  uint32_t n, incl = 0;
-  bool whole;
-  AttnDeal<uint32_t> deal;
-  __device__ AttnLanes(const AttnGeom &g, int32_t lane_len) : n(att_units(g, lane_len)), deal(0, 0) {
-    whole = __ballot(n > g.tail) == 0;
-    if (whole) return;
-    incl = att_scan(n, g.n_seqs);
-    const uint32_t all = __builtin_amdgcn_readlane(incl, g.n_seqs - 1);
-    deal = AttnDeal<uint32_t>(all / (uint32_t)g.n_run, all % (uint32_t)g.n_run);
-    whole = __ballot(!att_take_whole(g, n, deal.q)) == 0;
-  }
-};
-// Block `at` of a one-dimensional grid: the groups of a run (or sequence) are neighbours, so
-// that blocks that read the same pages run together, and the blocks without one come last
-// (between the others they left three quarters of the CUs idle).
-__device__ __forceinline__ AttnRun att_locate(const AttnGeom &g, const int32_t *seq_lens, const AttnTable &t,
-                                              uint32_t at) {
-  AttnRun r;
-  const int lane = threadIdx.x & 63;
-  r.lane_len = lane < g.n_seqs ? seq_lens[lane] : 0;
-  r.x = (int)(at / (uint32_t)g.n_group);
-  r.y = (int)(at - (uint32_t)r.x * (uint32_t)g.n_group);
-  const int x = r.x;
-  r.b = x;
-  r.u = r.u_end = r.b_first = 0;
-  bool whole = g.whole;
-  uint64_t q = 0, rem = 0;
-  if (!whole && g.n_seqs <= 64) {  // every wave by itself
-    const AttnLanes l(g, r.lane_len);
-    whole = l.whole;
-    if (!whole && x < g.n_run) {
-      const uint32_t u = l.deal.begin((uint32_t)x), u_end = l.deal.begin((uint32_t)x + 1);
-      r.u = u;
-      r.u_end = u_end;
-      const uint64_t after = __ballot(l.incl > u);  // sequences that end after u; the first holds it
-      r.b = after ? __ffsll((long long)after) - 1 : 0;
-      r.b_first = __builtin_amdgcn_readlane(l.incl - l.n, r.b);
-    }
-  } else if (!whole) {
-    whole = t.head[0] != 0;
-    q = t.head[1];
-    rem = t.head[2];
-    if (!whole && x < g.n_run) {
-      const AttnDeal<uint64_t> deal(q, rem);
-      r.u = deal.begin((uint64_t)x);
-      r.u_end = deal.begin((uint64_t)x + 1);
-      if (r.u < r.u_end) {
-        r.b = t.run_b[x];
-        r.b_first = t.first[r.b];
-      }
-    }
-  }
-  if (whole && x < g.n_seqs) r.u_end = __builtin_amdgcn_readfirstlane(att_units(g, att_len(g, seq_lens, r)));
-  return r;
-}
 
 // One block: the table of a call of more than 64 sequences.  (Each block of the two passes
 // scanned all lengths for itself before, work that grows with the square of the sequences:
@@ -262,46 +113,6 @@ paged_decode_plan_kernel(AttnGeom g, const int32_t *__restrict__ seq_lens, void 
     t.n_live[b] = (int32_t)(xz - xa + 1);
     for (uint64_t x = deal.begin(xa) < first ? xa + 1 : xa; x <= xz; ++x) t.run_b[x] = b;
   }
-}
-
-// Merges the block's four waves' (m, l, acc[G][D]) (in LDS, after a barrier) and stores the
-// segment's rows: bf16 rows when the segment is its whole sequence (zeros when no position
-// had a page), else partial x + b of the row's n_run + n_seqs (moving along the runs, x or
-// b or both grow from one segment to the next, so x + b names a segment).
-template <int D, int ROWS>
-__device__ __forceinline__ void att_store(const AttnGeom &g, const float (&sm_m)[ATT_WAVES][ROWS],
-                                          const float (&sm_l)[ATT_WAVES][ROWS], const float *const (&acc)[ATT_WAVES],
-                                          float *part, uint16_t *out, int G, int hq0, int b, int x, bool whole,
-                                          float sv) {
-  for (int idx = threadIdx.x; idx < G * D; idx += ATT_THREADS) {
-    const int j = idx / D, d = idx % D;
-    float M = sm_m[0][j];
-#pragma unroll
-    for (int w = 1; w < ATT_WAVES; ++w) M = fmaxf(M, sm_m[w][j]);
-    float a = 0.0f, ll = 0.0f;
-#pragma unroll
-    for (int w = 0; w < ATT_WAVES; ++w) {
-      const float f = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sm_m[w][j] - M);
-      a += f * acc[w][j * D + d];
-      ll += f * sm_l[w][j];
-    }
-    if (whole) {
-      const float o = ll == 0.0f ? 0.0f : a / ll * sv;
-      out[((int64_t)b * g.n_q_heads + hq0 + j) * D + d] = (uint16_t)(pack_bf16(o, 0.0f) & 0xFFFFu);
-    } else {
-      float *pp = part + ((int64_t)(hq0 + j) * ((int64_t)g.n_run + g.n_seqs) + x + b) * (2 + D);
-      pp[2 + d] = a;
-      if (d == 0) {
-        pp[0] = M;
-        pp[1] = ll;
-      }
-    }
-  }
-}
-
-// Zero rows of sequence b (a block that takes whole sequences meets an empty one).
-__device__ __forceinline__ void att_zero_rows(const AttnGeom &g, uint16_t *out, int G, int hq0, int b, int D) {
-  for (int i = threadIdx.x; i < G * D; i += ATT_THREADS) out[((int64_t)b * g.n_q_heads + hq0) * D + i] = 0;
 }
 
 // 16 e4m3 codes -> 16 fp32 values (exact).
@@ -875,7 +686,7 @@ paged_decode_mfma_kernel(const uint16_t *__restrict__ q, AttnGeom g, const uint8
   if (e && err) atomicOr(err, e);
 }
 
-// Pass 2: out[b][hq][:] = scale_v * sum_s 2^(m_s - M) acc_s / sum_s 2^(m_s - M) l_s over
+// Pass 2 (scales NULL: scale_v = 1): out[b][hq][:] = scale_v * sum_s 2^(m_s - M) acc_s / sum_s 2^(m_s - M) l_s over
 // the segments of sequence b.  A wave owns 64 channels of one row; its lanes hold the
 // maxima and sums of 64 segments at a time, whose weights reach the channels by readlane,
 // so there is no LDS and no barrier, and several segments' values are loaded
@@ -909,7 +720,7 @@ paged_decode_combine_kernel(const float *__restrict__ part, AttnGeom g, const fl
     n_live = t.n_live[b];
   }
   if (n_live == 1) return;  // the sequence was one segment: its block has written the row
-  const float sv = scales[g.n_kv_heads + h];
+  const float sv = scales ? scales[g.n_kv_heads + h] : 1.0f;
   const int64_t hq = row % g.n_q_heads;
   const float *pp = part + (hq * ((int64_t)g.n_run + g.n_seqs) + x0 + b) * (2 + D);
   float M = -INFINITY, L = 0.0f, A = 0.0f;
@@ -946,6 +757,20 @@ paged_decode_combine_kernel(const float *__restrict__ part, AttnGeom g, const fl
   out[row * D + d] = (uint16_t)(pack_bf16(o, 0.0f) & 0xFFFFu);
 }
 
+int att_make_table(const AttnGeom &g, const int32_t *seq_lens, void *table, hipStream_t st) {
+  if (g.n_seqs <= 64 || g.whole) return ZX_OK;
+  paged_decode_plan_kernel<<<1, AP_THREADS, 0, st>>>(g, seq_lens, table);
+  return check_launch("paged_decode_plan");
+}
+
+int att_combine(const float *part, const AttnGeom &g, const float *scales, const int32_t *seq_lens, uint16_t *out,
+                void *table, hipStream_t st) {
+  if (g.whole) return ZX_OK;  // every row is written
+  paged_decode_combine_kernel<<<(unsigned)((int64_t)g.n_seqs * g.n_q_heads), g.head_dim, 0, st>>>(part, g, scales,
+                                                                                                  seq_lens, out, table);
+  return check_launch("paged_decode_combine");
+}
+
 }  // namespace zx
 
 using namespace zx;
@@ -971,11 +796,9 @@ static bool att_mfma(int32_t grp, int32_t head_dim, int32_t page_size) {
 static bool att_dim_ok(int32_t head_dim) { return head_dim == 64 || head_dim == 128 || head_dim == 256; }
 
 // Blocks per group of query heads, and how the sequences are dealt to them.
-struct AttnPlan {
-  bool mfma, whole;
-  int32_t group, unit;
-  uint32_t tail;
-  int64_t n_run, n_blk;
+struct AttnPlan : AttnRuns {
+  bool mfma;
+  int32_t group;
 };
 static AttnPlan att_plan(int32_t n_seqs, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim, int32_t max_blocks,
                          int32_t page_size) {
@@ -983,36 +806,15 @@ static AttnPlan att_plan(int32_t n_seqs, int32_t n_q_heads, int32_t n_kv_heads, 
   const int32_t grp = n_q_heads / n_kv_heads;
   p.mfma = att_mfma(grp, head_dim, page_size);
   p.group = att_group(grp, p.mfma);
-  p.unit = ATT_WAVES * (p.mfma ? AM_STEP : ATT_U * 64 / (head_dim / 16));
-  const int64_t groups = n_q_heads / p.group;
-  // units of the longest sequence there can be (lengths are int32)
-  const int64_t seq_units = ceil_div(std::min((int64_t)max_blocks * page_size, (int64_t)INT32_MAX), p.unit);
-  // resident blocks per group, one equal run each: two per CU (registers, and LDS at D = 128),
-  // three where they fit (64 x 2k-8k, D = 64: 65 against 72 us; one head per block 64 against
+  // resident blocks: two per CU (registers, and LDS at D = 128), three where they fit
+  // (64 x 2k-8k, D = 64: 65 against 72 us; one head per block 64 against
   // 80, 71 heads on one kv head 297 against 337; at D = 256 1,412 against 1,326 the other way).
   // More runs than resident blocks leave a second, partly filled round: 16 x 1k-8k 37 against
-  // 31 us at three per CU.  A number of groups that leaves a part of the CUs without a run takes
-  // up to four rounds of shorter ones where those fill the chip by 5% more (152 groups: 3 runs
-  // on 456 of 512, or 10 in three rounds: 16 x 1k-8k, 19 heads per kv head, D = 128 371 -> 311
-  // us, D = 64 221 -> 164).
+  // 31 us at three per CU.
   const int64_t resident = ((p.mfma ? head_dim == 64 : p.group == 1 && head_dim < 256) ? 3LL : 2LL) * num_cus();
-  int64_t slots = std::max<int64_t>(1, resident / groups);
-  double per_round = (double)slots;
-  for (int64_t rounds = 2; rounds <= 4; ++rounds) {
-    const int64_t n = rounds * resident / groups;
-    if ((double)n / rounds > 1.05 * per_round) {
-      slots = n;
-      per_round = (double)n / rounds;
-    }
-  }
-  p.n_run = std::min(seq_units * n_seqs, slots);
-  p.tail = n_seqs >= p.n_run ? std::max<uint32_t>(1, ATT_TAIL_MANY / p.unit) : ATT_TAIL_ONE;
-  // Whole sequences whatever their lengths, without the merge's launch: one unit each, or at
-  // most 512 positions where they fill half the chip (32 x 100-500: 10.2 us, in runs 17), or
-  // so short that att_take_whole() says so anyway (128 x 100-600, 12 heads, D = 64: 26 -> 19).
-  p.whole = seq_units == 1 || (seq_units * p.unit <= 512 && n_seqs >= slots / 2) ||
-            seq_units <= p.tail;
-  p.n_blk = p.whole ? n_seqs : std::max<int64_t>(p.n_run, n_seqs);  // room for either way of dealing
+  static_cast<AttnRuns &>(p) = att_runs(n_seqs, n_q_heads / p.group, resident,
+                                        ATT_WAVES * (p.mfma ? AM_STEP : ATT_U * 64 / (head_dim / 16)), max_blocks,
+                                        page_size);
   return p;
 }
 
@@ -1022,9 +824,7 @@ extern "C" size_t zx_paged_attention_decode_workspace_bytes(int32_t n_seqs, int3
       max_blocks <= 0 || page_size <= 0)
     return 0;
   const AttnPlan p = att_plan(n_seqs, n_q_heads, n_kv_heads, head_dim, max_blocks, page_size);
-  // partials, then the table (read by 8 bytes: 2 + head_dim is even)
-  return (size_t)(n_q_heads * (p.n_run + n_seqs) * (2 + head_dim)) * sizeof(float) +
-         (n_seqs > 64 ? AttnTable::bytes(n_seqs, p.n_run) : 0);
+  return att_workspace_bytes(p, n_seqs, n_q_heads, head_dim);
 }
 
 template <int G, int D>
@@ -1077,27 +877,8 @@ extern "C" int zx_paged_attention_decode(const uint16_t *q, int32_t n_q_heads, c
   if (!workspace || workspace_bytes < need)
     return fail(ZX_ERR_WORKSPACE, "paged_attention_decode: workspace %zu < %zu bytes", workspace_bytes, need);
   const AttnPlan p = att_plan(n_seqs, n_q_heads, n_kv_heads, head_dim, max_blocks, page_size);
-  AttnGeom g;
-  g.n_q_heads = n_q_heads;
-  g.n_kv_heads = n_kv_heads;
-  g.head_dim = head_dim;
-  g.page_size = page_size;
-  g.max_blocks = max_blocks;
-  g.n_seqs = n_seqs;
-  g.n_run = (int32_t)p.n_run;
-  g.tail = p.tail;
-  g.unit = (uint32_t)p.unit;
-  g.cap = (uint32_t)std::min((int64_t)max_blocks * page_size, (int64_t)INT32_MAX);
-  g.whole = p.whole ? 1 : 0;
+  AttnGeom g = att_geom(p, n_seqs, n_q_heads, n_kv_heads, head_dim, max_blocks, page_size, n_pages, sm_scale);
   g.group = p.group;
-  g.n_pages = n_pages;
-  g.sm_scale = sm_scale;
-  {  // magic division by the page size for positions below 2^31
-    int sh = 0;
-    while ((1LL << sh) < page_size) ++sh;
-    g.p_shift = sh;
-    g.p_magic = (uint32_t)(((1ULL << (31 + sh)) + (uint64_t)page_size - 1) / (uint64_t)page_size);
-  }
   const int64_t gy = n_q_heads / p.group;
   if (gy > 65535) return fail(ZX_ERR_UNSUPPORTED, "paged_attention_decode: too many heads");
   ZX_REQUIRE(p.n_blk * gy < (1LL << 31), "paged_attention_decode: too many sequences or heads");
@@ -1105,20 +886,14 @@ extern "C" int zx_paged_attention_decode(const uint16_t *q, int32_t n_q_heads, c
   hipStream_t st = as_stream(stream);
   float *part = static_cast<float *>(workspace);
   void *table = part + n_q_heads * (p.n_run + n_seqs) * (2 + head_dim);
-  if (n_seqs > 64 && !p.whole) {
-    paged_decode_plan_kernel<<<1, AP_THREADS, 0, st>>>(g, seq_lens, table);
-    const int prc = check_launch("paged_decode_plan");
-    if (prc) return prc;
-  }
+  int rc = att_make_table(g, seq_lens, table, st);
+  if (rc) return rc;
   const dim3 grid((unsigned)(p.n_blk * gy));
-  int rc;
   switch (head_dim) {
     case 64: rc = launch_g<64>(p, grid, st, q, g, pool, scales, block_tables, seq_lens, part, out, err, table); break;
     case 128: rc = launch_g<128>(p, grid, st, q, g, pool, scales, block_tables, seq_lens, part, out, err, table); break;
     default: rc = launch_g<256>(p, grid, st, q, g, pool, scales, block_tables, seq_lens, part, out, err, table); break;
   }
-  if (rc || p.whole) return rc;  // every row is written
-  paged_decode_combine_kernel<<<(unsigned)((int64_t)n_seqs * n_q_heads), head_dim, 0, st>>>(part, g, scales, seq_lens,
-                                                                                            out, table);
-  return check_launch("paged_decode_combine");
+  if (rc) return rc;
+  return att_combine(part, g, scales, seq_lens, out, table, st);
 }

@@ -1,0 +1,280 @@
+// zx_attn_deal.h -- how decode attention deals the positions of all sequences to its blocks,
+// for 8-bit (zx_attention.hip) and 4-bit pages (zx_attention4.hip) alike: units of positions
+// laid end to end, equal runs of them, and the merge of a run's segments.
+#pragma once
+
+#include <algorithm>
+
+#include "zx_attn_common.h"
+
+namespace zx {
+
+constexpr int ATT_THREADS = 256;  // 4 waves
+constexpr int ATT_WAVES = ATT_THREADS / 64;
+
+struct AttnGeom {
+  int32_t n_q_heads, n_kv_heads, head_dim, page_size, max_blocks, n_seqs;
+  int32_t n_run;        // equal runs, one block per head group each
+  uint32_t unit, cap;   // positions per unit (a power of two); positions a block table holds
+  uint32_t tail;        // see att_take_whole
+  int32_t whole;        // every sequence is taken whole: known to the host
+  int32_t group, n_group;       // query heads per block; groups of them
+  uint32_t p_magic;  // t / page_size = (t * p_magic) >> (31 + p_shift) for t < 2^31
+  int32_t p_shift;
+  int64_t n_pages;
+  float sm_scale;
+};
+
+__device__ __forceinline__ uint32_t page_of(const AttnGeom &g, uint32_t t) {
+  return (uint32_t)(((uint64_t)t * g.p_magic) >> (31 + g.p_shift));
+}
+
+// Positions of a sequence that are attended to (lengths are int32).
+__device__ __forceinline__ uint32_t att_live_len(const AttnGeom &g, int32_t len) {
+  return len > 0 ? min((uint32_t)len, g.cap) : 0u;
+}
+__device__ __forceinline__ uint32_t att_units(const AttnGeom &g, int32_t len) {
+  return (att_live_len(g, len) + (g.unit - 1)) / g.unit;  // unit: a power of two
+}
+
+// The U units of all sequences dealt to n_run runs: run x takes q = U / n_run of them, the
+// first r = U % n_run one more.  T: 32 bits where U fits.
+template <typename T> struct AttnDeal {
+  T q, r;
+  __device__ AttnDeal(T q_, T r_) : q(q_), r(r_) {}
+  __device__ T begin(T x) const { return x * q + min(x, r); }
+  __device__ T run_of(T u) const { return u < r * (q + 1) ? u / (q + 1) : r + (u - r * (q + 1)) / q; }
+};
+
+// Whole sequences instead of equal runs?  A run starts anew in every sequence that it touches
+// (q, the first page ids, K and V one after the other: about as long as four units) and its
+// parts are merged; whole sequences leave blocks idle while the longest one ends.  With as many
+// sequences as runs or more, where most runs would start anew anyway: if the longest one has
+// at most ATT_TAIL_MANY positions and an eighth of an equal share.  Else if it exceeds a share
+// by at most ATT_TAIL_ONE units.  (g.tail: that slack in units; a call whose longest sequence
+// is within it needs no sums.)  In a graph, Hq 32 / Hkv 8, D = 128, tables of 32k positions:
+// 512 x 100-500 139 us in runs, 90 whole; 4 x 100-500 10.9 in runs, 16.3 whole; 64 x 512-4k
+// 59 in runs, 73 whole.
+constexpr uint32_t ATT_TAIL_ONE = 2, ATT_TAIL_MANY = 1024;
+__device__ __forceinline__ bool att_take_whole(const AttnGeom &g, uint64_t most, uint64_t share) {
+  return most <= g.tail + (g.n_seqs < g.n_run ? share : share / 8);
+}
+
+// Inclusive sum over the lanes below n (n <= 64, uniform).
+__device__ __forceinline__ uint32_t att_scan(uint32_t v, int n) {
+  const int lane = threadIdx.x & 63;
+  for (int off = 1; off < n; off <<= 1) {
+    const uint32_t y = __shfl_up(v, off, 64);
+    if (lane >= off) v += y;
+  }
+  return v;
+}
+
+// More than 64 sequences: what every block needs to know, computed once by att_plan_kernel.
+struct AttnTable {
+  uint64_t *head;   // [4]: whole sequences?, q, r
+  uint64_t *first;  // [n_seqs] a sequence's first unit
+  int32_t *x0, *n_live;  // [n_seqs] the first run that holds a part of it, and how many do
+  int32_t *run_b;        // [n_run] the sequence in which a run begins
+  __host__ __device__ AttnTable(void *at, int64_t n_seqs) {
+    head = static_cast<uint64_t *>(at);
+    first = head + 4;
+    x0 = reinterpret_cast<int32_t *>(first + n_seqs);
+    n_live = x0 + n_seqs;
+    run_b = n_live + n_seqs;
+  }
+  static size_t bytes(int64_t n_seqs, int64_t n_run) {
+    return 4 * sizeof(uint64_t) + (size_t)n_seqs * (sizeof(uint64_t) + 2 * sizeof(int32_t)) +
+           (size_t)n_run * sizeof(int32_t);
+  }
+};
+
+// The run of block x: units [u, u_end), unit u in sequence b, whose first unit is b_first.
+// All block-uniform; an empty run has u == u_end.  Up to 64 sequences every lane keeps one
+// sequence's length, so that stepping to the next sequence reads no memory.
+struct AttnRun {
+  uint64_t u, u_end, b_first;
+  int32_t b, lane_len;
+  int32_t x, y;  // the run (or sequence) and the group of query heads
+};
+__device__ __forceinline__ int32_t att_len(const AttnGeom &g, const int32_t *seq_lens, const AttnRun &r) {
+  return g.n_seqs <= 64 ? __builtin_amdgcn_readlane(r.lane_len, r.b) : seq_lens[r.b];
+}
+// Lane b's units, and how up to 64 sequences are dealt: whole, or units [begin(x), begin(x +
+// 1)) to run x, where incl is the inclusive sum over the sequences.
+struct AttnLanes {
+  uint32_t n, incl = 0;
+  bool whole;
+  AttnDeal<uint32_t> deal;
+  __device__ AttnLanes(const AttnGeom &g, int32_t lane_len) : n(att_units(g, lane_len)), deal(0, 0) {
+    whole = __ballot(n > g.tail) == 0;
+    if (whole) return;
+    incl = att_scan(n, g.n_seqs);
+    const uint32_t all = __builtin_amdgcn_readlane(incl, g.n_seqs - 1);
+    deal = AttnDeal<uint32_t>(all / (uint32_t)g.n_run, all % (uint32_t)g.n_run);
+    whole = __ballot(!att_take_whole(g, n, deal.q)) == 0;
+  }
+};
+// Block `at` of a one-dimensional grid: the groups of a run (or sequence) are neighbours, so
+// that blocks that read the same pages run together, and the blocks without one come last
+// (between the others they left three quarters of the CUs idle).
+__device__ __forceinline__ AttnRun att_locate(const AttnGeom &g, const int32_t *seq_lens, const AttnTable &t,
+                                              uint32_t at) {
+  AttnRun r;
+  const int lane = threadIdx.x & 63;
+  r.lane_len = lane < g.n_seqs ? seq_lens[lane] : 0;
+  r.x = (int)(at / (uint32_t)g.n_group);
+  r.y = (int)(at - (uint32_t)r.x * (uint32_t)g.n_group);
+  const int x = r.x;
+  r.b = x;
+  r.u = r.u_end = r.b_first = 0;
+  bool whole = g.whole;
+  uint64_t q = 0, rem = 0;
+  if (!whole && g.n_seqs <= 64) {  // every wave by itself
+    const AttnLanes l(g, r.lane_len);
+    whole = l.whole;
+    if (!whole && x < g.n_run) {
+      const uint32_t u = l.deal.begin((uint32_t)x), u_end = l.deal.begin((uint32_t)x + 1);
+      r.u = u;
+      r.u_end = u_end;
+      const uint64_t after = __ballot(l.incl > u);  // sequences that end after u; the first holds it
+      r.b = after ? __ffsll((long long)after) - 1 : 0;
+      r.b_first = __builtin_amdgcn_readlane(l.incl - l.n, r.b);
+    }
+  } else if (!whole) {
+    whole = t.head[0] != 0;
+    q = t.head[1];
+    rem = t.head[2];
+    if (!whole && x < g.n_run) {
+      const AttnDeal<uint64_t> deal(q, rem);
+      r.u = deal.begin((uint64_t)x);
+      r.u_end = deal.begin((uint64_t)x + 1);
+      if (r.u < r.u_end) {
+        r.b = t.run_b[x];
+        r.b_first = t.first[r.b];
+      }
+    }
+  }
+  if (whole && x < g.n_seqs) r.u_end = __builtin_amdgcn_readfirstlane(att_units(g, att_len(g, seq_lens, r)));
+  return r;
+}
+
+// Merges the block's four waves' (m, l, acc[G][D]) (in LDS, after a barrier) and stores the
+// segment's rows: bf16 rows when the segment is its whole sequence (zeros when no position
+// had a page), else partial x + b of the row's n_run + n_seqs (moving along the runs, x or
+// b or both grow from one segment to the next, so x + b names a segment).
+template <int D, int ROWS>
+__device__ __forceinline__ void att_store(const AttnGeom &g, const float (&sm_m)[ATT_WAVES][ROWS],
+                                          const float (&sm_l)[ATT_WAVES][ROWS], const float *const (&acc)[ATT_WAVES],
+                                          float *part, uint16_t *out, int G, int hq0, int b, int x, bool whole,
+                                          float sv) {
+  for (int idx = threadIdx.x; idx < G * D; idx += ATT_THREADS) {
+    const int j = idx / D, d = idx % D;
+    float M = sm_m[0][j];
+#pragma unroll
+    for (int w = 1; w < ATT_WAVES; ++w) M = fmaxf(M, sm_m[w][j]);
+    float a = 0.0f, ll = 0.0f;
+#pragma unroll
+    for (int w = 0; w < ATT_WAVES; ++w) {
+      const float f = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sm_m[w][j] - M);
+      a += f * acc[w][j * D + d];
+      ll += f * sm_l[w][j];
+    }
+    if (whole) {
+      const float o = ll == 0.0f ? 0.0f : a / ll * sv;
+      out[((int64_t)b * g.n_q_heads + hq0 + j) * D + d] = (uint16_t)(pack_bf16(o, 0.0f) & 0xFFFFu);
+    } else {
+      float *pp = part + ((int64_t)(hq0 + j) * ((int64_t)g.n_run + g.n_seqs) + x + b) * (2 + D);
+      pp[2 + d] = a;
+      if (d == 0) {
+        pp[0] = M;
+        pp[1] = ll;
+      }
+    }
+  }
+}
+
+// Zero rows of sequence b (a block that takes whole sequences meets an empty one).
+__device__ __forceinline__ void att_zero_rows(const AttnGeom &g, uint16_t *out, int G, int hq0, int b, int D) {
+  for (int i = threadIdx.x; i < G * D; i += ATT_THREADS) out[((int64_t)b * g.n_q_heads + hq0) * D + i] = 0;
+}
+
+// ------------------------------------------------------------------ host side
+
+// Blocks per group of query heads, and how the sequences are dealt to them.
+struct AttnRuns {
+  bool whole;
+  int32_t unit;
+  uint32_t tail;
+  int64_t n_run, n_blk;
+};
+// resident: blocks that the chip holds at once, one equal run each.  A number of groups that
+// leaves a part of the CUs without a run takes up to four rounds of shorter ones where those
+// fill the chip by 5% more (152 groups: 3 runs on 456 of 512, or 10 in three rounds: 16 x
+// 1k-8k, 19 heads per kv head, D = 128 371 -> 311 us, D = 64 221 -> 164).
+inline AttnRuns att_runs(int32_t n_seqs, int64_t groups, int64_t resident, int32_t unit, int32_t max_blocks,
+                         int32_t page_size) {
+  AttnRuns p;
+  p.unit = unit;
+  // units of the longest sequence there can be (lengths are int32)
+  const int64_t seq_units = ceil_div(std::min((int64_t)max_blocks * page_size, (int64_t)INT32_MAX), p.unit);
+  int64_t slots = std::max<int64_t>(1, resident / groups);
+  double per_round = (double)slots;
+  for (int64_t rounds = 2; rounds <= 4; ++rounds) {
+    const int64_t n = rounds * resident / groups;
+    if ((double)n / rounds > 1.05 * per_round) {
+      slots = n;
+      per_round = (double)n / rounds;
+    }
+  }
+  p.n_run = std::min(seq_units * n_seqs, slots);
+  p.tail = n_seqs >= p.n_run ? std::max<uint32_t>(1, ATT_TAIL_MANY / p.unit) : ATT_TAIL_ONE;
+  // Whole sequences whatever their lengths, without the merge's launch: one unit each, or at
+  // most 512 positions where they fill half the chip (32 x 100-500: 10.2 us, in runs 17), or
+  // so short that att_take_whole() says so anyway (128 x 100-600, 12 heads, D = 64: 26 -> 19).
+  p.whole = seq_units == 1 || (seq_units * p.unit <= 512 && n_seqs >= slots / 2) ||
+            seq_units <= p.tail;
+  p.n_blk = p.whole ? n_seqs : std::max<int64_t>(p.n_run, n_seqs);  // room for either way of dealing
+  return p;
+}
+
+// Partials, then the table (read by 8 bytes: 2 + head_dim is even).
+inline size_t att_workspace_bytes(const AttnRuns &p, int32_t n_seqs, int32_t n_q_heads, int32_t head_dim) {
+  return (size_t)(n_q_heads * (p.n_run + n_seqs) * (2 + head_dim)) * sizeof(float) +
+         (n_seqs > 64 ? AttnTable::bytes(n_seqs, p.n_run) : 0);
+}
+
+// (g.group and g.n_group are the caller's)
+inline AttnGeom att_geom(const AttnRuns &p, int32_t n_seqs, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim,
+                         int32_t max_blocks, int32_t page_size, int64_t n_pages, float sm_scale) {
+  AttnGeom g;
+  g.n_q_heads = n_q_heads;
+  g.n_kv_heads = n_kv_heads;
+  g.head_dim = head_dim;
+  g.page_size = page_size;
+  g.max_blocks = max_blocks;
+  g.n_seqs = n_seqs;
+  g.n_run = (int32_t)p.n_run;
+  g.tail = p.tail;
+  g.unit = (uint32_t)p.unit;
+  g.cap = (uint32_t)std::min((int64_t)max_blocks * page_size, (int64_t)INT32_MAX);
+  g.whole = p.whole ? 1 : 0;
+  g.group = g.n_group = 0;
+  g.n_pages = n_pages;
+  g.sm_scale = sm_scale;
+  {  // magic division by the page size for positions below 2^31
+    int sh = 0;
+    while ((1LL << sh) < page_size) ++sh;
+    g.p_shift = sh;
+    g.p_magic = (uint32_t)(((1ULL << (31 + sh)) + (uint64_t)page_size - 1) / (uint64_t)page_size);
+  }
+  return g;
+}
+
+// The table of a call of more than 64 sequences that is dealt in runs (otherwise nothing).
+int att_make_table(const AttnGeom &g, const int32_t *seq_lens, void *table, hipStream_t st);
+// Pass 2: merges the partials of sequences that were cut; scales NULL stands for ones.
+int att_combine(const float *part, const AttnGeom &g, const float *scales, const int32_t *seq_lens, uint16_t *out,
+                void *table, hipStream_t st);
+
+}  // namespace zx

@@ -10,6 +10,10 @@ inline size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
 // Sets n 32-bit words to v with a kernel (graph-capture safe, unlike hipMemsetAsync).
 int fill_u32(uint32_t *p, int64_t n, uint32_t v, hipStream_t st);
 
+// Scales from per-block maxima part[n_layers][gx][n_slabs] (fp32 bits; zx_quant.hip).
+int finalize_partials(const uint32_t *part, int32_t gx, int32_t n_slabs, int32_t n_layers, float *scales,
+                      hipStream_t st);
+
 // Single-pass paged append with dynamic scales (zx_append_fused.hip).  Returns
 // ZX_ERR_UNSUPPORTED when the device cannot run it (the caller then uses two passes).
 // append_fused_preferred: whether the single pass beats two passes for this call (a

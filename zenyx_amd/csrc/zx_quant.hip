@@ -7,6 +7,7 @@
 #include <algorithm>
 #include <mutex>
 
+#include "zx_append_common.h"
 #include "zx_internal.h"
 
 namespace zx {
@@ -536,12 +537,6 @@ struct RowGeom8 {
   int64_t row_bytes;
   int64_t x_layer_stride;  // elements
 };
-typedef unsigned int q_v4u __attribute__((ext_vector_type(4)));
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t q_rsrc(const void *base, int64_t bytes) {
-  const int n = bytes < 0 ? 0 : (bytes > 0x7FFFFFF0 ? 0x7FFFFFF0 : (int)bytes);
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(base), (short)0, n, 0x00020000);
-}
-
 // Pass 1: per-(layer, slab) amax.  Persistent grid sweeping the rows front to back with
 // default-policy loads; pass 2 runs back to front, so it starts on rows the memory-side
 // cache still holds (about 5% of pass 2 at 524,288-token layers on MI355X).  Each block
@@ -603,92 +598,6 @@ finalize_partials_kernel(const uint32_t *part, int32_t gx, int32_t n_slabs, floa
   __syncthreads();
   if (threadIdx.x == 0)
     scales[i] = scale_from_amax_bits(max(max(red[0], red[1]), max(red[2], red[3])));
-}
-
-// 0x80 in each byte of w whose low 7 bits are all set (an e4m3 NaN code), else 0.
-__device__ __forceinline__ uint32_t nan_code_bytes(uint32_t w) { return ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u; }
-
-// NaN codes of 8 inputs v under a finite static scale (sign bit s_sign, 0 or 0x80).  The
-// code is the NaN code S.1111.111 when the quotient x / s is NaN or rounds beyond the e4m3
-// range; its sign is that of the IEEE quotient: the sign of x for a NaN x, else
-// sign(x) ^ sign(s).  (div_by_scale's correction step turns an infinite quotient into a
-// NaN whose sign is the device's default, so the sign is set here.)  A finite x with a
-// NaN code overflowed: MODE 1 flags it, MODE 2 also stores +-448 (S.1111.110).  The
-// per-element look runs only when some code is a NaN code.
-template <int MODE>
-__device__ __forceinline__ uint2 static_overflow(uint4 v, uint2 cd, uint32_t s_sign, int32_t *err) {
-  if (!(nan_code_bytes(cd.x) | nan_code_bytes(cd.y))) return cd;
-  const uint32_t in[4] = {v.x, v.y, v.z, v.w};
-  uint32_t c[2] = {cd.x, cd.y};
-  bool hit = false;
-#pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    const uint32_t bits = (in[k >> 1] >> (16 * (k & 1))) & 0xFFFFu;
-    const uint32_t mag = bits & 0x7FFFu, x_sign = (bits >> 8) & 0x80u;
-    const int sh = 8 * (k & 3);
-    const uint32_t code = (c[k >> 2] >> sh) & 0xFFu;
-    if ((code & 0x7Fu) == 0x7Fu) {
-      const uint32_t sign = mag > 0x7F80u ? x_sign : (x_sign ^ s_sign);
-      uint32_t fixed = sign | 0x7Fu;
-      if (mag < 0x7F80u) {
-        hit = true;
-        if (MODE == 2) fixed = sign | 0x7Eu;
-      }
-      c[k >> 2] = (c[k >> 2] & ~(0xFFu << sh)) | (fixed << sh);
-    }
-  }
-  if (hit && err) atomicOr(err, ZX_KERR_OVERFLOW);
-  return make_uint2(c[0], c[1]);
-}
-
-// Where tokens go: the page tables of an append.
-struct TokGeom {
-  const int32_t *cu_seqlens, *start_pos, *block_tables;
-  int32_t n_seqs, max_blocks, page_size, head_dim;
-  int64_t n_pages, page_bytes;
-};
-
-// Pool offsets (bytes within one layer) of U tokens' (page, row) bases, or -1; *e collects
-// the error bits.  The U searches (last b with cu_seqlens[b] <= t) take their steps together,
-// so that a step waits for one load.
-template <int U>
-__device__ __forceinline__ void token_offsets(const TokGeom &g, const int64_t (&t)[U], int64_t n_tok,
-                                              int64_t (&off)[U], int32_t &e) {
-  int lo[U], hi[U];
-#pragma unroll
-  for (int k = 0; k < U; ++k) lo[k] = 0, hi[k] = g.n_seqs - 1;
-  for (int left = g.n_seqs - 1; left > 0; left >>= 1) {  // hi - lo <= left
-#pragma unroll
-    for (int k = 0; k < U; ++k) {
-      const int mid = (lo[k] + hi[k] + 1) >> 1;
-      const bool up = g.cu_seqlens[mid] <= t[k];
-      if (lo[k] < hi[k]) {
-        if (up) lo[k] = mid;
-        else hi[k] = mid - 1;
-      }
-    }
-  }
-  int32_t c0[U], c1[U], p0[U];
-#pragma unroll
-  for (int k = 0; k < U; ++k) {
-    c0[k] = g.cu_seqlens[lo[k]];
-    c1[k] = g.cu_seqlens[lo[k] + 1];
-    p0[k] = g.start_pos ? g.start_pos[lo[k]] : 0;
-  }
-#pragma unroll
-  for (int k = 0; k < U; ++k) {
-    off[k] = -1;
-    if (t[k] >= n_tok || t[k] < c0[k] || t[k] >= c1[k]) continue;
-    const int64_t pos = p0[k] + (t[k] - c0[k]);  // below 2^32
-    if (pos < 0 || pos >= (int64_t)g.max_blocks * g.page_size) {
-      e |= ZX_KERR_POS_RANGE;
-      continue;
-    }
-    const uint32_t bi = (uint32_t)pos / (uint32_t)g.page_size, row = (uint32_t)pos - bi * (uint32_t)g.page_size;
-    const int64_t page = g.block_tables[(int64_t)lo[k] * g.max_blocks + bi];
-    if (page < 0 || page >= g.n_pages) e |= ZX_KERR_PAGE_RANGE;
-    else off[k] = page * g.page_bytes + (int64_t)row * g.head_dim;
-  }
 }
 
 __global__ void kv_token_offsets_kernel(TokGeom g, int64_t n_tok, int64_t *tok_off, int32_t *err) {
@@ -753,6 +662,12 @@ kv_quant_rows_kernel(const uint16_t *x, RowGeom8 g, const int64_t *tok_off, TokG
   }
 }
 
+int finalize_partials(const uint32_t *part, int32_t gx, int32_t n_slabs, int32_t n_layers, float *scales,
+                      hipStream_t st) {
+  finalize_partials_kernel<<<(unsigned)((int64_t)n_layers * n_slabs), 256, 0, st>>>(part, gx, n_slabs, scales);
+  return check_launch("finalize_partials");
+}
+
 #ifndef KA_U
 #define KA_U 8  // rows per thread per step of the amax pass
 #endif
@@ -807,8 +722,7 @@ static int kv_scales_impl(const uint16_t *x, const RowGeom &g, int32_t n_layers,
     const unsigned gx = (unsigned)amax_grid_x(g.n_tok, r.rpb, n_layers);
     kv_amax_rows_kernel<KA_U><<<dim3(gx, n_layers), r.vpr8 * r.rpb, 0, st>>>(x, r, nullptr, part);
     if ((rc = check_launch("kv_amax_rows"))) return rc;
-    finalize_partials_kernel<<<(unsigned)n, 256, 0, st>>>(part, (int32_t)gx, g.n_slabs, scales);
-    return check_launch("finalize_partials");
+    return finalize_partials(part, (int32_t)gx, g.n_slabs, n_layers, scales, st);
   }
   if ((rc = fill_u32(reinterpret_cast<uint32_t *>(scales), n, 0, st))) return rc;
   if (g.n_tok > 0) {

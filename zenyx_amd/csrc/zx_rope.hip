@@ -1,0 +1,483 @@
+// zx_rope.hip -- rotary positions: the table of cosines and sines, the rotation of query or key
+// rows (and its transpose, the gradient), and the FP8 paged append that rotates the keys on the
+// way.  All of it is bound by HBM: a row is read and written once, the table's rows come from
+// the caches (every head of a row, and every layer of an append, reads the same one).
+#include <algorithm>
+
+#include "zx_append_common.h"
+#include "zx_internal.h"
+#include "zx_rope_common.h"
+
+namespace zx {
+
+// ------------------------------------------------------------------ the table
+
+// angle = position * inv_freq in 64 bits: in 32 the angle of position 100,000 is off by up to
+// 2^-8 radians.
+__global__ void __launch_bounds__(256)
+rope_table_kernel(const double *inv_freq, int32_t half, int64_t n_pos, double scale, float *out) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n_pos * half) return;
+  const int64_t pos = i / half;
+  const int32_t j = (int32_t)(i - pos * half);
+  double s, c;
+  sincos((double)pos * inv_freq[j], &s, &c);
+  out[pos * 2 * half + j] = (float)(c * scale);
+  out[pos * 2 * half + half + j] = (float)(s * scale);
+}
+
+// ------------------------------------------------------------------ the rotation
+
+template <int DT> struct RopeIo;  // 8 values as loaded and stored
+template <> struct RopeIo<ZX_BF16> {
+  using T = uint16_t;
+  static __device__ __forceinline__ void load(const T *p, float (&f)[8]) {
+    unpack_bf16x8(*reinterpret_cast<const uint4 *>(p), f);
+  }
+  static __device__ __forceinline__ void store(T *p, const float (&f)[8]) {
+    *reinterpret_cast<uint4 *>(p) = pack_bf16x8(f);
+  }
+};
+template <> struct RopeIo<ZX_F16> {
+  using T = uint16_t;
+  typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+  static __device__ __forceinline__ void load(const T *p, float (&f)[8]) {
+    const h8 v = *reinterpret_cast<const h8 *>(p);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = (float)v[i];
+  }
+  static __device__ __forceinline__ void store(T *p, const float (&f)[8]) {
+    h8 v;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = (_Float16)f[i];
+    *reinterpret_cast<h8 *>(p) = v;
+  }
+};
+template <> struct RopeIo<ZX_F32> {
+  using T = float;
+  static __device__ __forceinline__ void load(const T *p, float (&f)[8]) {
+    const float4 a = reinterpret_cast<const float4 *>(p)[0], b = reinterpret_cast<const float4 *>(p)[1];
+    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+  }
+  static __device__ __forceinline__ void store(T *p, const float (&f)[8]) {
+    reinterpret_cast<float4 *>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
+    reinterpret_cast<float4 *>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
+  }
+};
+
+struct RopeArgs {
+  const void *x;
+  void *out;
+  const int32_t *positions;
+  int32_t *err;
+  RopeTable r;
+  int64_t x_row, x_head, o_row, o_head;  // strides in elements
+  uint32_t n_rows;
+  int32_t n_heads, head_dim;
+  uint32_t units;    // of a head: rot / 16 that turn 8 pairs, then (copy) 8 channels each
+  uint32_t n_share;  // threads that share a row's unit; a thread takes every n_share-th head
+  int32_t transpose, copy;  // copy: out is another tensor (the channels past rot are written too)
+};
+
+// Unit u of a row for the heads h0, h0 + n_share, ...: the cosines and sines are loaded once for
+// all of them.  Neighbouring threads take neighbouring units, then heads: whole cache lines.
+template <int DT, bool INTER> __global__ void __launch_bounds__(256) rope_kernel(RopeArgs a) {
+  using Io = RopeIo<DT>;
+  using T = typename Io::T;
+  const uint32_t per_row = a.units * a.n_share;
+  const uint32_t at = blockIdx.x * 256u + threadIdx.x;
+  const uint32_t row = at / per_row;
+  if (row >= a.n_rows) return;
+  const uint32_t rest = at - row * per_row;
+  const uint32_t h0 = rest / a.units, u = rest - h0 * a.units;
+  const int32_t pos = a.positions[row];
+  const bool live = pos >= 0 && pos < a.r.n_pos;
+  if (!live && rest == 0 && a.err) atomicOr(a.err, ZX_KERR_POS_RANGE);
+  const T *x = static_cast<const T *>(a.x) + row * a.x_row;
+  T *out = static_cast<T *>(a.out) + row * a.o_row;
+  const uint32_t turning = (uint32_t)a.r.rot / 16;
+  if (u >= turning) {  // 8 channels past rot
+    const int c0 = a.r.rot + 8 * (int)(u - turning);
+    for (int h = h0; h < a.n_heads; h += a.n_share) {
+      float f[8];
+      Io::load(x + h * a.x_head + c0, f);
+      Io::store(out + h * a.o_head + c0, f);
+    }
+    return;
+  }
+  const int ca = INTER ? 16 * u : 8 * u, cb = INTER ? ca + 8 : ca + a.r.rot / 2;
+  if (!live) {  // no row of the table: as it is
+    if (a.copy)
+      for (int h = h0; h < a.n_heads; h += a.n_share) {
+        float f[8], g[8];
+        Io::load(x + h * a.x_head + ca, f);
+        Io::load(x + h * a.x_head + cb, g);
+        Io::store(out + h * a.o_head + ca, f);
+        Io::store(out + h * a.o_head + cb, g);
+      }
+    return;
+  }
+  float c[8], s[8];
+  rope_row(a.r, pos, u, c, s);
+  if (a.transpose) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s[i] = -s[i];
+  }
+  for (int h = h0; h < a.n_heads; h += a.n_share) {
+    float f[8], g[8];
+    Io::load(x + h * a.x_head + ca, f);
+    Io::load(x + h * a.x_head + cb, g);
+    rope_turn<INTER>(f, g, c, s);
+    Io::store(out + h * a.o_head + ca, f);
+    Io::store(out + h * a.o_head + cb, g);
+  }
+}
+
+// ------------------------------------------------------------------ FP8 append with rotation
+
+// Rows x[n_tok][2][H][D] bf16.  Thread t of a block owns unit t % n_unit of rows t / n_unit +
+// rpb * k: 16 channels of one (kv, head), as two 16-byte columns that hold whole pairs (K), so a
+// unit turns by itself and one scale, or one maximum, per thread suffices.
+struct RaGeom {
+  int32_t n_unit, rpb;  // n_unit = H * D / 8
+  int32_t upd;          // units per (kv, head) = D / 16
+  int32_t n_slabs, head_dim;
+  int64_t n_tok, row_bytes, x_layer_stride;
+};
+struct RaUnit {
+  int32_t slab, p;  // kv * H + head; its unit in the head
+  int32_t ca, cb;   // first channels of the two columns within the head
+  bool turns;
+};
+template <bool INTER> __device__ __forceinline__ RaUnit ra_unit(const RaGeom &g, int rot, int u) {
+  RaUnit n;
+  n.slab = u / g.upd;
+  n.p = u - n.slab * g.upd;
+  n.turns = n.slab < g.n_slabs / 2 && n.p < rot / 16;
+  const bool half = n.turns && !INTER;
+  n.ca = (half ? 8 : 16) * n.p;
+  n.cb = n.ca + (half ? rot / 2 : 8);
+  return n;
+}
+
+// A token's page (-1: none) and position (-1: none), found once per call when there are many.
+struct TokPlace {
+  int32_t page, pos;
+};
+__global__ void __launch_bounds__(256)
+ra_places_kernel(TokGeom g, int64_t limit, int64_t n_tok, TokPlace *places, int32_t *err) {
+  const int64_t t[1] = {(int64_t)blockIdx.x * 256 + threadIdx.x};
+  if (t[0] >= n_tok) return;
+  int64_t page[1], pos[1];
+  int32_t e = 0;
+  token_places<1>(g, limit, t, n_tok, page, pos, e);
+  if (e && err) atomicOr(err, e);
+  places[t[0]] = TokPlace{(int32_t)page[0], (int32_t)pos[0]};
+}
+
+template <int U, bool LOCATE>
+__device__ __forceinline__ void ra_find(const TokGeom &tg, int64_t limit, const TokPlace *places, const int64_t (&row)[U],
+                                        int64_t n_tok, int64_t (&page)[U], int64_t (&pos)[U], int32_t &e) {
+  if constexpr (LOCATE) {
+    token_places<U>(tg, limit, row, n_tok, page, pos, e);
+  } else {
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const TokPlace p = row[k] < n_tok ? places[row[k]] : TokPlace{-1, -1};
+      page[k] = p.page;
+      pos[k] = p.pos;
+    }
+  }
+}
+
+// Pass 1 (dynamic scales): maxima of |rotated K| and |V| of the tokens that have a position.
+template <int U, bool LOCATE, bool INTER>
+__global__ void __launch_bounds__(512)
+rope_append_amax_kernel(const uint16_t *x, RaGeom g, RopeTable r, TokGeom tg, int64_t limit, const TokPlace *places,
+                        uint32_t *part /* [L][gridDim.x][2H] */) {
+  const int t = threadIdx.x;
+  const int rs = t / g.n_unit;
+  const RaUnit n = ra_unit<INTER>(g, r.rot, t - rs * g.n_unit);
+  const int layer = blockIdx.y;
+  const char *xl = reinterpret_cast<const char *>(x + (int64_t)layer * g.x_layer_stride);
+  const int col = 2 * n.slab * g.head_dim;
+  const int64_t step = (int64_t)gridDim.x * U * g.rpb;
+  uint32_t m = 0;  // two packed 16-bit maxima
+  int32_t e = 0;
+  for (int64_t r0 = (int64_t)blockIdx.x * U * g.rpb; r0 < g.n_tok; r0 += step) {
+    const __amdgpu_buffer_rsrc_t rsrc = q_rsrc(xl + r0 * g.row_bytes, (g.n_tok - r0) * g.row_bytes);
+    uint4 a[U], b[U];
+    int64_t row[U], page[U], pos[U];
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const int off = (int)((k * g.rpb + rs) * g.row_bytes) + col;
+      const q_v4u v = __builtin_amdgcn_raw_buffer_load_b128(rsrc, off + 2 * n.ca, 0, 0);
+      const q_v4u w = __builtin_amdgcn_raw_buffer_load_b128(rsrc, off + 2 * n.cb, 0, 0);
+      a[k] = make_uint4(v.x, v.y, v.z, v.w);
+      b[k] = make_uint4(w.x, w.y, w.z, w.w);
+      row[k] = r0 + k * g.rpb + rs;
+    }
+    ra_find<U, LOCATE>(tg, limit, places, row, g.n_tok, page, pos, e);
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      if (n.turns) {
+        float c[8], s[8];
+        rope_row(r, pos[k] < 0 ? 0 : pos[k], n.p, c, s);
+        rope_turn_bf16<INTER>(a[k], b[k], c, s);
+      }
+      if (pos[k] >= 0) m = absmax_acc(absmax_acc(m, a[k]), b[k]);
+    }
+  }
+  const uint32_t mx = group_max(fold16(m), g.upd);
+  __shared__ uint32_t red[512];
+  red[t] = mx;
+  __syncthreads();
+  if (rs == 0 && n.p == 0) {
+    uint32_t v = mx;
+    for (int k = 1; k < g.rpb; ++k) v = max(v, red[k * g.n_unit + t]);
+    part[((int64_t)layer * gridDim.x + blockIdx.x) * g.n_slabs + n.slab] = v << 16;
+  }
+}
+
+// Pass 2: rotate, encode, scatter (tiles from the end of the batch first, where the first
+// pass has left the caches).  MODE as kv_quant_rows_kernel's: 0 dynamic scales, 1 static, 2 static and
+// saturating.
+template <int U, int MODE, bool LOCATE, bool INTER>
+__global__ void __launch_bounds__(512)
+rope_append_rows_kernel(const uint16_t *x, RaGeom g, RopeTable r, TokGeom tg, int64_t limit, const TokPlace *places,
+                        const float *scales, uint8_t *pool, int64_t pool_layer_stride, int32_t *err) {
+  const int t = threadIdx.x;
+  const int rs = t / g.n_unit;
+  const RaUnit n = ra_unit<INTER>(g, r.rot, t - rs * g.n_unit);
+  const int layer = blockIdx.y;
+  const float sc = scales[(int64_t)layer * g.n_slabs + n.slab];
+  const QuantScale q = quant_scale(sc);
+  const uint32_t s_sign = (__float_as_uint(sc) >> 24) & 0x80u;
+  const int64_t r0 = ((int64_t)gridDim.x - 1 - blockIdx.x) * U * g.rpb;
+  const char *xl = reinterpret_cast<const char *>(x + (int64_t)layer * g.x_layer_stride);
+  const __amdgpu_buffer_rsrc_t rsrc = q_rsrc(xl + r0 * g.row_bytes, (g.n_tok - r0) * g.row_bytes);
+  uint8_t *pl = pool + (int64_t)layer * pool_layer_stride + (int64_t)n.slab * tg.page_size * tg.head_dim;
+  uint4 a[U], b[U];
+  int64_t row[U], page[U], pos[U];
+#pragma unroll
+  for (int k = 0; k < U; ++k) {
+    const int off = (int)((k * g.rpb + rs) * g.row_bytes) + 2 * n.slab * g.head_dim;
+    const q_v4u v = __builtin_amdgcn_raw_buffer_load_b128(rsrc, off + 2 * n.ca, 0, 2 /* nontemporal: last read */);
+    const q_v4u w = __builtin_amdgcn_raw_buffer_load_b128(rsrc, off + 2 * n.cb, 0, 2);
+    a[k] = make_uint4(v.x, v.y, v.z, v.w);
+    b[k] = make_uint4(w.x, w.y, w.z, w.w);
+    row[k] = r0 + k * g.rpb + rs;
+  }
+  int32_t e = 0;
+  ra_find<U, LOCATE>(tg, limit, places, row, g.n_tok, page, pos, e);
+  if (LOCATE && e && err && layer == 0 && n.slab == 0 && n.p == 0) atomicOr(err, e);
+#pragma unroll
+  for (int k = 0; k < U; ++k) {
+    if (page[k] < 0) continue;
+    if (n.turns) {
+      float c[8], s[8];
+      rope_row(r, pos[k], n.p, c, s);
+      rope_turn_bf16<INTER>(a[k], b[k], c, s);
+    }
+    uint2 ea = quant8(a[k], q), eb = quant8(b[k], q);
+    if (MODE != 0 && q.nan_fix == 0) {
+      ea = static_overflow<MODE>(a[k], ea, s_sign, err);
+      eb = static_overflow<MODE>(b[k], eb, s_sign, err);
+    }
+    uint8_t *dst = pl + page[k] * tg.page_bytes + (int64_t)((uint32_t)pos[k] % (uint32_t)tg.page_size) * tg.head_dim;
+    typedef unsigned int v2u __attribute__((ext_vector_type(2)));
+    const v2u wa = {ea.x, ea.y}, wb = {eb.x, eb.y};
+    __builtin_nontemporal_store(wa, reinterpret_cast<v2u *>(dst + n.ca));
+    __builtin_nontemporal_store(wb, reinterpret_cast<v2u *>(dst + n.cb));
+  }
+}
+
+constexpr int RA_U = 4;        // rows per thread and step, both passes
+constexpr int RA_BPC = 4;      // blocks per CU of the first pass
+constexpr int64_t RA_LOCATE_BPC = 4;  // up to this many blocks per CU find the places themselves
+
+static int64_t ra_amax_grid_x(int64_t n_tok, int32_t rpb, int32_t n_layers) {
+  const int64_t tiles = ceil_div(n_tok, (int64_t)RA_U * rpb);
+  const int64_t want = std::max<int64_t>(1, ceil_div((int64_t)num_cus() * RA_BPC, n_layers));
+  return std::max<int64_t>(1, std::min(tiles, want));
+}
+
+}  // namespace zx
+
+using namespace zx;
+
+extern "C" int zx_rope_table(const double *inv_freq, int32_t rot_dim, int64_t n_pos, double scale, float *out,
+                             zx_stream_t stream) {
+  clear_error();
+  ZX_REQUIRE(inv_freq, "rope_table: null pointer");
+  const int rc = rope_check("rope_table", out, n_pos, rot_dim, rot_dim);
+  if (rc) return rc;
+  const int64_t blocks = ceil_div(n_pos * (rot_dim / 2), 256);
+  if (blocks >= (1LL << 31)) return fail(ZX_ERR_UNSUPPORTED, "rope_table: table too large");
+  rope_table_kernel<<<(unsigned)blocks, 256, 0, as_stream(stream)>>>(inv_freq, rot_dim / 2, n_pos, scale, out);
+  return check_launch("rope_table");
+}
+
+extern "C" int zx_rope(const void *x, int dtype, int64_t n_rows, int32_t n_heads, int32_t head_dim, int64_t x_row_stride,
+                       int64_t x_head_stride, const float *table, int64_t n_pos, int32_t rot_dim,
+                       const int32_t *positions, int32_t flags, void *out, int64_t out_row_stride,
+                       int64_t out_head_stride, int32_t *err, zx_stream_t stream) {
+  clear_error();
+  ZX_REQUIRE(dtype == ZX_BF16 || dtype == ZX_F16 || dtype == ZX_F32, "rope: unknown dtype %d", dtype);
+  ZX_REQUIRE(!(flags & ~(ZX_ROPE_INTERLEAVED | ZX_ROPE_TRANSPOSE)), "rope: unknown flag bits 0x%x", (unsigned)flags);
+  ZX_REQUIRE(n_rows >= 0 && n_rows < (1LL << 31) && n_heads > 0 && head_dim > 0, "rope: sizes must be positive");
+  if (head_dim % 8) return fail(ZX_ERR_UNSUPPORTED, "rope: head_dim %d is not a multiple of 8", head_dim);
+  const int rc = rope_check("rope", table, n_pos, rot_dim, head_dim);
+  if (rc) return rc;
+  if (n_rows == 0) return ZX_OK;
+  ZX_REQUIRE(x && out && positions, "rope: null pointer");
+  const int64_t vec = dtype == ZX_F32 ? 4 : 8;
+  ZX_REQUIRE(aligned16(x) && aligned16(out) && x_row_stride % vec == 0 && x_head_stride % vec == 0 &&
+                 out_row_stride % vec == 0 && out_head_stride % vec == 0,
+             "rope: every row of x and out must be 16-byte aligned");
+  ZX_REQUIRE(x_row_stride >= 0 && x_head_stride >= 0 && out_row_stride >= 0 && out_head_stride >= 0,
+             "rope: negative stride");
+  ZX_REQUIRE(x != out || (x_row_stride == out_row_stride && x_head_stride == out_head_stride),
+             "rope: in place, x and out must have the same strides");
+  RopeArgs a;
+  a.x = x;
+  a.out = out;
+  a.positions = positions;
+  a.err = err;
+  a.r = RopeTable{table, n_pos, rot_dim};
+  a.x_row = x_row_stride;
+  a.x_head = x_head_stride;
+  a.o_row = out_row_stride;
+  a.o_head = out_head_stride;
+  a.n_rows = (uint32_t)n_rows;
+  a.n_heads = n_heads;
+  a.head_dim = head_dim;
+  a.copy = x != out;
+  a.transpose = (flags & ZX_ROPE_TRANSPOSE) != 0;
+  a.units = (uint32_t)(rot_dim / 16 + (a.copy ? (head_dim - rot_dim) / 8 : 0));
+  // as many heads per thread as leave eight blocks per CU, at most 4
+  int64_t share = n_heads;
+  while (share > 1 && ceil_div(n_heads, share) < 4 &&
+         n_rows * ceil_div(share, 2) * a.units >= 8LL * 256 * num_cus())
+    share = ceil_div(share, 2);
+  a.n_share = (uint32_t)share;
+  const int64_t threads = n_rows * share * a.units;
+  if (threads >= (1LL << 32) - 256) return fail(ZX_ERR_UNSUPPORTED, "rope: too many rows");
+  const unsigned blocks = (unsigned)ceil_div(threads, 256);
+  const hipStream_t st = as_stream(stream);
+  const bool inter = flags & ZX_ROPE_INTERLEAVED;
+#define ZX_ROPE_LAUNCH(dt)                               \
+  if (inter)                                             \
+    rope_kernel<dt, true><<<blocks, 256, 0, st>>>(a);    \
+  else                                                   \
+    rope_kernel<dt, false><<<blocks, 256, 0, st>>>(a);
+  if (dtype == ZX_BF16) {
+    ZX_ROPE_LAUNCH(ZX_BF16)
+  } else if (dtype == ZX_F16) {
+    ZX_ROPE_LAUNCH(ZX_F16)
+  } else {
+    ZX_ROPE_LAUNCH(ZX_F32)
+  }
+#undef ZX_ROPE_LAUNCH
+  return check_launch("rope");
+}
+
+extern "C" size_t zx_kv_rope_append_workspace_bytes(int32_t n_layers, int64_t n_tok, int32_t n_heads,
+                                                    int32_t head_dim) {
+  (void)head_dim;
+  if (n_layers <= 0 || n_tok <= 0 || n_heads <= 0) return 0;
+  const int64_t gx = std::max<int64_t>(1, ceil_div((int64_t)num_cus() * RA_BPC, n_layers));
+  return align256((size_t)n_tok * sizeof(TokPlace)) + align256((size_t)gx * n_layers * 2 * n_heads * sizeof(uint32_t));
+}
+
+extern "C" int zx_kv_rope_append(const uint16_t *x, int64_t x_layer_stride, int32_t n_layers, int64_t n_tok,
+                                 int32_t n_heads, int32_t head_dim, const float *table, int64_t n_pos, int32_t rot_dim,
+                                 const int32_t *cu_seqlens, const int32_t *start_pos, int32_t n_seqs,
+                                 const int32_t *block_tables, int32_t max_blocks, int32_t page_size, uint8_t *pool,
+                                 int64_t pool_layer_stride, int64_t n_pages, float *scales, int32_t flags, int32_t *err,
+                                 void *workspace, size_t workspace_bytes, zx_stream_t stream) {
+  clear_error();
+  ZX_REQUIRE(!(flags & ~(ZX_APPEND_STATIC_SCALES | ZX_APPEND_SATURATE | ZX_ROPE_INTERLEAVED)),
+             "kv_rope_append: unknown flag bits 0x%x", (unsigned)flags);
+  const bool dynamic = !(flags & ZX_APPEND_STATIC_SCALES);
+  ZX_REQUIRE(!(dynamic && (flags & ZX_APPEND_SATURATE)), "kv_rope_append: ZX_APPEND_SATURATE needs static scales");
+  ZX_REQUIRE(scales && cu_seqlens && block_tables && pool && (x || n_tok == 0), "kv_rope_append: null pointer");
+  ZX_REQUIRE(n_layers > 0 && n_layers <= 65535, "kv_rope_append: n_layers out of range");
+  ZX_REQUIRE(n_seqs > 0 && max_blocks > 0 && page_size > 0 && n_pages > 0 && n_heads > 0,
+             "kv_rope_append: sizes must be positive");
+  ZX_REQUIRE(n_tok >= 0 && n_tok < (1LL << 31), "kv_rope_append: n_tok must be in [0, 2^31)");
+  ZX_REQUIRE(n_pages < (1LL << 31), "kv_rope_append: n_pages must be below 2^31");
+  if (!(head_dim == 64 || head_dim == 128 || head_dim == 256))
+    return fail(ZX_ERR_UNSUPPORTED, "kv_rope_append: head_dim %d not in {64, 128, 256}", head_dim);
+  const int64_t row = 2LL * n_heads * head_dim;
+  if (row > 8192) return fail(ZX_ERR_UNSUPPORTED, "kv_rope_append: 2*H*D = %lld exceeds 8192", (long long)row);
+  int rc = rope_check("kv_rope_append", table, n_pos, rot_dim, head_dim);
+  if (rc) return rc;
+  ZX_REQUIRE(aligned16(x) && aligned16(pool) &&
+                 (n_layers == 1 || (x_layer_stride % 8 == 0 && pool_layer_stride % 16 == 0)),
+             "kv_rope_append: x and pool (and every layer of them) must be 16-byte aligned");
+  const int64_t page_bytes = row * page_size;
+  ZX_REQUIRE(n_layers == 1 || x_layer_stride >= n_tok * row, "kv_rope_append: x layer stride smaller than a layer");
+  ZX_REQUIRE(n_layers == 1 || pool_layer_stride >= n_pages * page_bytes,
+             "kv_rope_append: pool layer stride smaller than a layer's pages");
+  const hipStream_t st = as_stream(stream);
+  if (n_tok == 0)  // no token: the scales of an empty batch
+    return dynamic ? zx_kv_scales(x, 0, n_layers, 0, n_heads, head_dim, scales, stream) : ZX_OK;
+  const size_t need = zx_kv_rope_append_workspace_bytes(n_layers, n_tok, n_heads, head_dim);
+  if (!workspace || workspace_bytes < need)
+    return fail(ZX_ERR_WORKSPACE, "kv_rope_append: workspace %zu < %zu bytes", workspace_bytes, need);
+  RaGeom g;
+  g.n_unit = (int32_t)(row / 16);
+  g.rpb = g.n_unit >= 256 ? 1 : 256 / g.n_unit;
+  g.upd = head_dim / 16;
+  g.n_slabs = 2 * n_heads;
+  g.head_dim = head_dim;
+  g.n_tok = n_tok;
+  g.row_bytes = 2 * row;
+  g.x_layer_stride = x_layer_stride;
+  const RopeTable r = {table, n_pos, rot_dim};
+  const TokGeom tg = {cu_seqlens, start_pos, block_tables, n_seqs, max_blocks, page_size, head_dim, n_pages, page_bytes};
+  const int64_t limit = std::min((int64_t)max_blocks * page_size, n_pos);
+  const int64_t tiles = ceil_div(n_tok, (int64_t)RA_U * g.rpb);
+  const bool locate = tiles * n_layers <= RA_LOCATE_BPC * num_cus();
+  TokPlace *places = static_cast<TokPlace *>(workspace);
+  uint32_t *part = reinterpret_cast<uint32_t *>(static_cast<char *>(workspace) + align256((size_t)n_tok * sizeof(TokPlace)));
+  if (!locate) {
+    ra_places_kernel<<<(unsigned)ceil_div(n_tok, 256), 256, 0, st>>>(tg, limit, n_tok, places, err);
+    if ((rc = check_launch("ra_places"))) return rc;
+  }
+  const bool inter = flags & ZX_ROPE_INTERLEAVED;
+  const int threads = g.n_unit * g.rpb;
+  if (dynamic) {
+    const unsigned gx = (unsigned)ra_amax_grid_x(n_tok, g.rpb, n_layers);
+    const dim3 grid(gx, n_layers);
+#define ZX_RA_AMAX(loc, il) \
+  rope_append_amax_kernel<RA_U, loc, il><<<grid, threads, 0, st>>>(x, g, r, tg, limit, places, part)
+    if (locate && inter) ZX_RA_AMAX(true, true);
+    else if (locate) ZX_RA_AMAX(true, false);
+    else if (inter) ZX_RA_AMAX(false, true);
+    else ZX_RA_AMAX(false, false);
+#undef ZX_RA_AMAX
+    if ((rc = check_launch("rope_append_amax"))) return rc;
+    if ((rc = finalize_partials(part, (int32_t)gx, g.n_slabs, n_layers, scales, st))) return rc;
+  }
+  const dim3 grid((unsigned)tiles, n_layers);
+#define ZX_RA_ROWS2(mode, loc, il) \
+  rope_append_rows_kernel<RA_U, mode, loc, il><<<grid, threads, 0, st>>>(x, g, r, tg, limit, places, scales, pool, \
+                                                                        pool_layer_stride, err)
+#define ZX_RA_ROWS(mode)                                   \
+  if (locate && inter) ZX_RA_ROWS2(mode, true, true);      \
+  else if (locate) ZX_RA_ROWS2(mode, true, false);         \
+  else if (inter) ZX_RA_ROWS2(mode, false, true);          \
+  else ZX_RA_ROWS2(mode, false, false);
+  if (dynamic) {
+    ZX_RA_ROWS(0)
+  } else if (flags & ZX_APPEND_SATURATE) {
+    ZX_RA_ROWS(2)
+  } else {
+    ZX_RA_ROWS(1)
+  }
+#undef ZX_RA_ROWS
+#undef ZX_RA_ROWS2
+  return check_launch("rope_append_rows");
+}

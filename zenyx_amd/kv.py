@@ -9,9 +9,11 @@ Layouts:
   * KV cache tensor (FP8KVQuantizer): ``[L, 2, B, H, T, D]`` bf16, scales ``[L, 2, H]``.
   * token-major append input: ``[L, n_tok, 2, H, D]`` (or one layer ``[n_tok, 2, H, D]``).
   * page pool: ``[L, n_pages, 2, H, P, D]`` uint8 e4m3fn codes (or one layer without L).
+  * 4-bit page pool: ``[L, n_pages, 2, H, P / 16, 17 D / 2]`` uint8 (``kv4_pool``; or one layer).
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 
 import torch
@@ -842,3 +844,289 @@ def tier_copy_runs(dst: torch.Tensor, src: torch.Tensor, dst_offs, src_offs, run
     lib = N.load()
     N.check(lib.zx_tier_copy_runs(N.ptr(dst), N.ptr(src), d.ctypes.data, s.ctypes.data, len(d), run_bytes,
                                   ctypes.c_void_p(st.cuda_stream), None), "tier_copy_runs")
+
+
+# ------------------------------------------------------------------ rotary positions
+
+_same_device = contextlib.nullcontext()
+
+
+def _on(device: torch.device):
+    """Makes ``device`` current for a launch (nothing to do where it already is)."""
+    return _same_device if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def _all_on(device: torch.device, **tensors) -> None:
+    for name, t in tensors.items():
+        if t is not None:
+            N.require_device(t, name)
+            if t.device != device:
+                raise ValueError(f"{name} must be on {device}, got {t.device}")
+
+
+def _rope_table_of(table: torch.Tensor, D: int) -> tuple[int, int]:
+    if table.dim() != 2 or table.dtype != torch.float32:
+        raise ValueError("table must be float32 [n_pos, rot_dim] (kv.rope_table)")
+    if table.shape[1] > D:
+        raise ValueError(f"the table rotates {table.shape[1]} channels, the heads have {D}")
+    return table.shape[0], table.shape[1]
+
+
+def rope_table(inv_freq: torch.Tensor, n_pos: int, scale: float = 1.0) -> torch.Tensor:
+    """Cosines and sines of the angles ``position * inv_freq[i]`` times ``scale``: float32
+    ``[n_pos, 2 * len(inv_freq)]``, cosines first.  ``inv_freq``: float64 ``[rot_dim / 2]`` on
+    the device; the angles are formed in 64 bits.  ``train.rotary.RotaryPositions`` makes the
+    usual frequencies, scaled ones for long contexts among them."""
+    N.need_gpu()
+    if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or not inv_freq.numel():
+        raise ValueError("inv_freq must be float64 [rot_dim / 2]")
+    N.require_device(inv_freq, "inv_freq")
+    out = torch.empty((int(n_pos), 2 * inv_freq.numel()), dtype=torch.float32, device=inv_freq.device)
+    with _on(out.device):
+        N.check(N.load().zx_rope_table(N.ptr(inv_freq), out.shape[1], out.shape[0], float(scale), N.ptr(out),
+                                       N.stream_ptr(out.device)), "rope_table")
+    return out
+
+
+def _rows_of(t: torch.Tensor, name: str) -> None:
+    vec = 16 // t.element_size()
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a HIP device tensor, got {t.device}")
+    if t.stride(2) != 1 or t.stride(0) % vec or t.stride(1) % vec or t.data_ptr() % 16:
+        raise ValueError(f"{name}: channels must be contiguous and every head's row 16-byte aligned")
+
+
+def rope(x: torch.Tensor, table: torch.Tensor, positions: torch.Tensor, interleaved: bool = False,
+         transpose: bool = False, out: torch.Tensor | None = None, check: bool = False) -> torch.Tensor:
+    """Rotary positions: rows ``x [n, H, D]`` (bf16, f16 or f32; a view into a larger tensor may
+    be given, e.g. the queries of a fused projection) at ``positions`` (int32 ``[n]``) of
+    ``table`` (``rope_table``).  Pair i of the first rot_dim channels is (i, i + rot_dim / 2),
+    or (2 i, 2 i + 1) when ``interleaved``; later channels are copied.  ``transpose`` applies
+    the transposed rotation, which takes a gradient back.  ``out`` may be ``x`` itself.  A row
+    at a position the table does not have is copied (``check`` synchronises and raises)."""
+    N.need_gpu()
+    if x.dim() != 3 or x.dtype not in _DT:
+        raise ValueError("x must be [n, n_heads, head_dim] in bf16, f16 or f32")
+    n, H, D = x.shape
+    n_pos, rot = _rope_table_of(table, D)
+    if positions.dtype != torch.int32 or positions.shape != (n,):
+        raise ValueError(f"positions must be int32 [{n}]")
+    if H == 0 or D == 0:
+        raise ValueError("x has no heads or no channels")
+    _rows_of(x, "x")
+    _all_on(x.device, table=table, positions=positions)
+    if out is None:
+        out = torch.empty((n, H, D), dtype=x.dtype, device=x.device)
+    else:
+        if out.shape != x.shape or out.dtype != x.dtype or out.device != x.device:
+            raise ValueError("out must be like x")
+        _rows_of(out, "out")
+        if n > 1 and out.stride(0) < D or H > 1 and out.stride(1) < D:
+            raise ValueError("out: rows must not overlap")
+        if n and not (out.data_ptr() == x.data_ptr() and out.stride() == x.stride()):
+            (a, z), (b, y) = ((t.data_ptr(), t.data_ptr() + t.element_size() * (
+                (n - 1) * t.stride(0) + (H - 1) * t.stride(1) + D)) for t in (x, out))
+            if a < y and b < z:
+                raise ValueError("out must be x itself or not overlap it")
+    err = _err_word_if(check, x.device)
+    flags = (N.ZX_ROPE_INTERLEAVED if interleaved else 0) | (N.ZX_ROPE_TRANSPOSE if transpose else 0)
+    with _on(x.device):
+        N.check(N.load().zx_rope(N.ptr(x), _DT[x.dtype], n, H, D, x.stride(0), x.stride(1), N.ptr(table), n_pos, rot,
+                                 N.ptr(positions), flags, N.ptr(out), out.stride(0), out.stride(1), N.ptr(err),
+                                 N.stream_ptr(x.device)), "rope")
+    if check:
+        _raise_kernel_error(err, "rope")
+    return out
+
+
+def _append_args(x, cu_seqlens, block_tables, start_pos, err):
+    for name, t in (("cu_seqlens", cu_seqlens), ("block_tables", block_tables)):
+        if t.dtype != torch.int32:
+            raise ValueError(f"{name} must be int32")
+    if block_tables.dim() != 2 or cu_seqlens.dim() != 1 or cu_seqlens.numel() != block_tables.shape[0] + 1:
+        raise ValueError("block_tables must be [B, max_blocks] and cu_seqlens [B+1]")
+    if start_pos is not None and (start_pos.dtype != torch.int32 or start_pos.numel() != block_tables.shape[0]):
+        raise ValueError("start_pos must be int32 [B]")
+    if err is not None and (err.dtype != torch.int32 or err.numel() < 1 or err.device != x.device):
+        raise ValueError("err must be an int32 tensor on x's device")
+
+
+def kv_rope_append(x: torch.Tensor, table: torch.Tensor, cu_seqlens: torch.Tensor, block_tables: torch.Tensor,
+                   pool: torch.Tensor, scales: torch.Tensor | None = None, start_pos: torch.Tensor | None = None,
+                   interleaved: bool = False, static_scales: bool = False, saturate: bool = False,
+                   check: bool = False, err: torch.Tensor | None = None) -> torch.Tensor:
+    """``kv_quant_append`` with the keys of ``x [L, n_tok, 2, H, D]`` rotated by their positions
+    on the way: the codes and scales of ``rope`` on the keys followed by ``kv_quant_append``.
+    ``table``: ``rope_table``; a token at a position it does not have is not stored (and
+    flagged).  Dynamic scales are taken over the tokens that belong to a sequence.  The other
+    arguments are ``kv_quant_append``'s."""
+    N.need_gpu()
+    x = _layers(x)
+    if pool.dim() == 5:
+        pool = pool.unsqueeze(0)
+    L, T, _, H, D = x.shape
+    if pool.dim() != 6 or pool.shape[0] != L or pool.shape[2:4] != (2, H) or pool.shape[5] != D or \
+            pool.dtype != torch.uint8:
+        raise ValueError(f"pool must be uint8 [L={L}, n_pages, 2, H={H}, P, D={D}]")
+    n_pages, P = pool.shape[1], pool.shape[4]
+    n_pos, rot = _rope_table_of(table, D)
+    _append_args(x, cu_seqlens, block_tables, start_pos, err)
+    if scales is None:
+        if static_scales:
+            raise ValueError("static_scales needs scales")
+        scales = torch.empty((L, 2, H), dtype=torch.float32, device=x.device)
+    if scales.shape != (L, 2, H) or scales.dtype != torch.float32:
+        raise ValueError(f"scales must be float32 [{L}, 2, {H}]")
+    if saturate and not static_scales:
+        raise ValueError("saturate applies to static scales (dynamic scales never overflow)")
+    _all_on(x.device, x=x, table=table, cu_seqlens=cu_seqlens, block_tables=block_tables, pool=pool, scales=scales,
+            start_pos=start_pos)
+    lib = N.load()
+    flags = (N.ZX_APPEND_STATIC_SCALES if static_scales else 0) | (N.ZX_APPEND_SATURATE if saturate else 0) | \
+        (N.ZX_ROPE_INTERLEAVED if interleaved else 0)
+    with _on(x.device):
+        ws = _workspace(lib.zx_kv_rope_append_workspace_bytes(L, T, H, D), x.device)
+        err = _err_word_if(check, x.device) if err is None else err
+        N.check(lib.zx_kv_rope_append(N.ptr(x), T * 2 * H * D, L, T, H, D, N.ptr(table), n_pos, rot, N.ptr(cu_seqlens),
+                                      N.ptr(start_pos), block_tables.shape[0], N.ptr(block_tables),
+                                      block_tables.shape[1], P, N.ptr(pool), pool[0].numel(), n_pages, N.ptr(scales),
+                                      flags, N.ptr(err), N.ptr(ws), ws.numel(), N.stream_ptr(x.device)),
+                "kv_rope_append")
+    if check:
+        _raise_kernel_error(err, "kv_rope_append")
+    return scales
+
+
+# ------------------------------------------------------------------ 4-bit pages
+
+def kv4_pool(n_layers: int, n_pages: int, n_heads: int, page_size: int, head_dim: int,
+             device: torch.device | None = None) -> torch.Tensor:
+    """An empty 4-bit page pool, uint8 ``[L, n_pages, 2, H, P / 16, 17 D / 2]``: per tile of 16
+    tokens their e2m1 codes ``[D / 32][16][16 bytes]`` and a power of two per 32 channels
+    ``[D / 32][16]``.  ``page_size`` is a multiple of 16, ``head_dim`` 64, 128 or 256."""
+    if head_dim not in (64, 128, 256) or page_size < 16 or page_size % 16:
+        raise ValueError("4-bit pages need a head_dim of 64, 128 or 256 and a page_size that is a multiple of 16")
+    return torch.zeros((n_layers, n_pages, 2, n_heads, page_size // 16, 17 * head_dim // 2), dtype=torch.uint8,
+                       device=device or N.ensure_gpu())
+
+
+def _pool4(pool_layer: torch.Tensor) -> tuple[int, int, int, int]:
+    """(n_pages, H, P, D) of one layer of 4-bit pages."""
+    if pool_layer.dim() != 5 or pool_layer.dtype != torch.uint8 or pool_layer.shape[1] != 2 or \
+            pool_layer.shape[4] not in (544, 1088, 2176):
+        raise ValueError("the layer's pool must be uint8 [n_pages, 2, H, P / 16, 17 D / 2] (kv4_pool)")
+    n_pages, _, H, tiles, nb = pool_layer.shape
+    return n_pages, H, 16 * tiles, nb * 2 // 17
+
+
+def kv4_append(x: torch.Tensor, cu_seqlens: torch.Tensor, block_tables: torch.Tensor, pool: torch.Tensor,
+               start_pos: torch.Tensor | None = None, table: torch.Tensor | None = None, interleaved: bool = False,
+               check: bool = False, err: torch.Tensor | None = None) -> None:
+    """Paged append into 4-bit pages (``kv4_pool``, written in place): every 32 channels of a
+    token, K or V, head become e2m1 codes times the smallest power of two that brings their
+    largest magnitude to 6 or below (a block with a NaN or an infinity becomes NaN).  With
+    ``table`` (``rope_table``) the keys are rotated by their positions first, as ``rope`` does
+    it.  The other arguments are ``kv_quant_append``'s; there are no scales to keep."""
+    N.need_gpu()
+    x = _layers(x)
+    if pool.dim() == 5:
+        pool = pool.unsqueeze(0)
+    L, T, _, H, D = x.shape
+    if pool.dim() != 6 or pool.shape[0] != L:
+        raise ValueError(f"pool must be uint8 [L={L}, n_pages, 2, H={H}, P / 16, {17 * D // 2}] (kv4_pool)")
+    n_pages, Hp, P, Dp = _pool4(pool[0])
+    if (Hp, Dp) != (H, D):
+        raise ValueError(f"pool holds {Hp} heads of {Dp}, x has {H} of {D}")
+    if interleaved and table is None:
+        raise ValueError("interleaved needs a table")
+    n_pos, rot = _rope_table_of(table, D) if table is not None else (0, 0)
+    _append_args(x, cu_seqlens, block_tables, start_pos, err)
+    _all_on(x.device, x=x, table=table, cu_seqlens=cu_seqlens, block_tables=block_tables, pool=pool,
+            start_pos=start_pos)
+    lib = N.load()
+    with _on(x.device):
+        ws = _workspace(lib.zx_kv4_append_workspace_bytes(T), x.device)
+        err = _err_word_if(check, x.device) if err is None else err
+        N.check(lib.zx_kv4_append(N.ptr(x), T * 2 * H * D, L, T, H, D, N.ptr(table), n_pos, rot, N.ptr(cu_seqlens),
+                                  N.ptr(start_pos), block_tables.shape[0], N.ptr(block_tables), block_tables.shape[1],
+                                  P, N.ptr(pool), pool[0].numel(), n_pages,
+                                  N.ZX_ROPE_INTERLEAVED if interleaved else 0, N.ptr(err), N.ptr(ws), ws.numel(),
+                                  N.stream_ptr(x.device)), "kv4_append")
+    if check:
+        _raise_kernel_error(err, "kv4_append")
+
+
+def kv4_gather_dequant(pool_layer: torch.Tensor, block_tables: torch.Tensor, seq_lens: torch.Tensor,
+                       out_len: int | None = None, check: bool = False,
+                       out: tuple[torch.Tensor, torch.Tensor] | None = None):
+    """One layer of 4-bit pages as contiguous bf16 ``(k, v)``, each ``[B, H, out_len, D]`` (exact:
+    every code times its power is a bf16 value); positions at or beyond ``seq_lens[b]`` are
+    zeros."""
+    N.need_gpu()
+    n_pages, H, P, D = _pool4(pool_layer)
+    if block_tables.dtype != torch.int32 or seq_lens.dtype != torch.int32 or block_tables.dim() != 2:
+        raise ValueError("block_tables [B, max_blocks] and seq_lens [B] must be int32")
+    B = block_tables.shape[0]
+    if seq_lens.numel() != B:
+        raise ValueError("seq_lens must have one entry per block-table row")
+    if out_len is None:
+        out_len = block_tables.shape[1] * P
+    dev = pool_layer.device
+    _all_on(dev, pool_layer=pool_layer, block_tables=block_tables, seq_lens=seq_lens)
+    if out is None:
+        k = torch.empty((B, H, out_len, D), dtype=torch.bfloat16, device=dev)
+        v = torch.empty_like(k)
+    else:
+        k, v = out
+        for t in (k, v):
+            if t.shape != (B, H, out_len, D) or t.dtype != torch.bfloat16:
+                raise ValueError(f"out tensors must be bf16 {(B, H, out_len, D)}")
+        _all_on(dev, out_k=k, out_v=v)
+    with _on(dev):
+        err = _err_word_if(check, dev)
+        N.check(N.load().zx_kv4_gather_dequant(N.ptr(pool_layer), n_pages, H, D, P, N.ptr(block_tables),
+                                               block_tables.shape[1], N.ptr(seq_lens), B, out_len, N.ptr(k), N.ptr(v),
+                                               N.ptr(err), N.stream_ptr(dev)), "kv4_gather_dequant")
+    if check:
+        _raise_kernel_error(err, "kv4_gather_dequant")
+    return k, v
+
+
+def _attention4_args(q, pool_layer, block_tables, out):
+    n_pages, Hkv, P, D = _pool4(pool_layer)
+    if q.dim() != 3 or q.dtype != torch.bfloat16 or q.shape[2] != D:
+        raise ValueError(f"q must be bf16 [rows, Hq, {D}]")
+    if q.shape[1] == 0 or q.shape[1] % Hkv:
+        raise ValueError("the number of query heads must be a multiple of the number of kv heads")
+    if block_tables.dtype != torch.int32 or block_tables.dim() != 2:
+        raise ValueError("block_tables must be int32 [B, max_blocks]")
+    if out is not None and (out.shape != q.shape or out.dtype != torch.bfloat16):
+        raise ValueError(f"out must be bf16 {tuple(q.shape)}")
+    return n_pages, Hkv, P, D
+
+
+def paged_attention4_decode(q: torch.Tensor, pool_layer: torch.Tensor, block_tables: torch.Tensor,
+                            seq_lens: torch.Tensor, sm_scale: float | None = None, out: torch.Tensor | None = None,
+                            check: bool = False) -> torch.Tensor:
+    """Decode attention straight from 4-bit pages: ``paged_attention_decode`` for a ``kv4_pool``
+    layer (which has no scales).  q ``[B, Hq, D]`` bf16 -> ``[B, Hq, D]`` bf16."""
+    N.need_gpu()
+    n_pages, Hkv, P, D = _attention4_args(q, pool_layer, block_tables, out)
+    B, Hq, _ = q.shape
+    if block_tables.shape[0] != B or seq_lens.numel() != B or seq_lens.dtype != torch.int32:
+        raise ValueError("block_tables and seq_lens (int32) need one row per sequence")
+    q = q.contiguous()
+    out = torch.empty((B, Hq, D), dtype=torch.bfloat16, device=q.device) if out is None else out
+    _all_on(q.device, q=q, pool_layer=pool_layer, block_tables=block_tables, seq_lens=seq_lens, out=out)
+    lib = N.load()
+    mb = block_tables.shape[1]
+    with _on(q.device):
+        ws = _workspace(lib.zx_paged_attention4_decode_workspace_bytes(B, Hq, Hkv, D, mb, P), q.device)
+        err = _err_word_if(check, q.device)
+        N.check(lib.zx_paged_attention4_decode(
+            N.ptr(q), Hq, N.ptr(pool_layer), n_pages, Hkv, D, P, N.ptr(block_tables), mb, N.ptr(seq_lens), B,
+            float(D ** -0.5 if sm_scale is None else sm_scale), N.ptr(out), N.ptr(err), N.ptr(ws), ws.numel(),
+            N.stream_ptr(q.device)), "paged_attention4_decode")
+    if check:
+        _raise_kernel_error(err, "paged_attention4_decode")
+    return out
