@@ -532,6 +532,26 @@ int zx_paged_attention4_decode(const uint16_t *q, int32_t n_q_heads, const uint8
                                uint16_t *out, int32_t *err, void *workspace, size_t workspace_bytes,
                                zx_stream_t stream);
 
+/* Blocks of queries over 4-bit pages: rows [cu_q[b], cu_q[b + 1]) of q [n_q][n_q_heads]
+ * [head_dim], row i of sequence b at position q_pos0[b] + i, attend to keys [0, kv_len[b]), when
+ * `causal` those up to their own position.  A row without a key gives zeros; rows beyond
+ * max_q_per_seq (host) or in no sequence are left unwritten (the former set
+ * ZX_KERR_POS_RANGE); kv_len beyond max_blocks * page_size is clipped and sets it too; keys on
+ * a page outside [0, n_pages) are left out and set ZX_KERR_PAGE_RANGE.  Softmax weights are
+ * rounded once to bf16 (the row sums use the same): |error| <= one bf16 ulp + 2^-7 max|V|; with
+ * ZX_PREFILL_EXACT_P they are carried as bf16 hi + lo: one ulp + 2^-15 max|V|.  workspace:
+ * zx_paged_attention4_prefill_workspace_bytes() device bytes let several blocks share a row's
+ * keys where the rows do not fill the chip; a smaller or NULL one runs the call uncut. */
+size_t zx_paged_attention4_prefill_workspace_bytes(int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim,
+                                                   int32_t page_size, int32_t max_blocks, int32_t n_seqs,
+                                                   int32_t max_q_per_seq);
+int zx_paged_attention4_prefill(const uint16_t *q, int64_t n_q, const int32_t *cu_q, const int32_t *q_pos0,
+                                int32_t n_q_heads, const uint8_t *pool, int64_t n_pages, int32_t n_kv_heads,
+                                int32_t head_dim, int32_t page_size, const int32_t *block_tables, int32_t max_blocks,
+                                const int32_t *kv_len, int32_t n_seqs, int32_t max_q_per_seq, int32_t causal,
+                                float sm_scale, int32_t flags, uint16_t *out, int32_t *err, void *workspace,
+                                size_t workspace_bytes, zx_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

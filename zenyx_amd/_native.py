@@ -98,6 +98,9 @@ SIGNATURES = {
     "zx_paged_attention4_decode_workspace_bytes": (_SZ, [_I32, _I32, _I32, _I32, _I32, _I32]),
     "zx_paged_attention4_decode": (_INT, [_P, _I32, _P, _I64, _I32, _I32, _I32, _P, _I32, _P, _I32, ctypes.c_float,
                                           _P, _P, _P, _SZ, _P]),
+    "zx_paged_attention4_prefill_workspace_bytes": (_SZ, [_I32, _I32, _I32, _I32, _I32, _I32, _I32]),
+    "zx_paged_attention4_prefill": (_INT, [_P, _I64, _P, _P, _I32, _P, _I64, _I32, _I32, _I32, _P, _I32, _P, _I32,
+                                           _I32, _I32, ctypes.c_float, _I32, _P, _P, _P, _SZ, _P]),
 }
 
 _lib = None

@@ -283,6 +283,352 @@ paged_decode4_kernel(const uint16_t *__restrict__ q, AttnGeom g, const uint8_t *
   if (e && err) atomicOr(err, e);
 }
 
+// Blocks of queries.  A column of the products is a (query row, head) of one KV head's group: a
+// block takes CT tiles of 16 columns, rows row0 .. of one sequence with all the group's heads,
+// and its four waves take every fourth step of 32 keys, each with a running softmax of its own,
+// merged at the end.  So no wave waits for another within the loop, K goes from memory to the
+// operand without LDS, every conversion serves CT products, and a K/V byte read serves 16 CT
+// columns: what a block reads is small, the pages have 4 bits.  Bound by the matrix cores and
+// the exponentials together for many rows, by the reads for few.
+//   EXACT: weights as bf16 hi + lo (2^-17); otherwise rounded once to bf16, and summed so rounded.
+// With few tiles the keys of a tile are shared by up to n_split blocks, whose parts
+// prefill4_combine_kernel merges.
+struct Prefill4Args {
+  const uint16_t *q;
+  const int32_t *cu_q, *q_pos0, *bt, *kv_len;
+  const uint8_t *pool;
+  uint16_t *out;
+  float *part;  // [tile][split][16 CT columns][2 + D]
+  int32_t *err;
+  int64_t n_pages;
+  int32_t n_q_heads, n_kv_heads, page_size, max_blocks, n_seqs, causal;
+  int32_t group, n_group;     // heads per block, groups of them
+  int32_t rows;               // query rows per tile: 16 CT / group
+  int32_t n_rt, n_split;      // row tiles per sequence, blocks per tile
+  int64_t max_rows;           // n_rt * rows
+  uint32_t p_magic;
+  int32_t p_shift;
+  float sm_log2e;
+};
+
+// A block's tile, and which steps of 32 keys are this split's.  All uniform.
+struct Prefill4Tile {
+  int64_t item;  // tile's number
+  int b, h, hq0, G, row0, n_rows, split, parts;
+  int64_t q_lo;
+  int32_t qpos0;    // position of row row0
+  int32_t len;      // keys there are
+  uint32_t t_begin, t_end;  // keys of this split
+};
+__device__ __forceinline__ bool p4_locate(const Prefill4Args &a, uint32_t at, Prefill4Tile &t, int32_t &e) {
+  // row tiles slowest and last ones first: under a causal mask they see the most keys
+  const uint32_t per_rt = (uint32_t)a.n_group * (uint32_t)a.n_seqs;
+  t.split = (int)(at % (uint32_t)a.n_split);
+  at /= (uint32_t)a.n_split;
+  t.item = at;
+  const uint32_t rt_rev = at / per_rt, rem = at - rt_rev * per_rt;
+  t.b = (int)(rem / (uint32_t)a.n_group);
+  const int y = (int)(rem - (uint32_t)t.b * (uint32_t)a.n_group);
+  const int grp = a.n_q_heads / a.n_kv_heads, per_kv = a.n_group / a.n_kv_heads;
+  t.h = y / per_kv;
+  const int first = (y - t.h * per_kv) * a.group;
+  t.G = min(a.group, grp - first);
+  t.hq0 = t.h * grp + first;
+  const int32_t lo = a.cu_q[t.b], hi = a.cu_q[t.b + 1];
+  if (rt_rev == 0 && (int64_t)hi - lo > a.max_rows) e |= ZX_KERR_POS_RANGE;
+  const int64_t row0 = ((int64_t)a.n_rt - 1 - rt_rev) * a.rows;
+  if (row0 >= (int64_t)hi - lo) return false;
+  t.row0 = (int)row0;
+  t.n_rows = min(a.rows, hi - lo - t.row0);
+  t.q_lo = lo;
+  int32_t len = a.kv_len[t.b];
+  const int64_t cap = (int64_t)a.max_blocks * a.page_size;  // below 2^31
+  if (len > cap) {
+    e |= ZX_KERR_POS_RANGE;
+    len = (int32_t)cap;
+  }
+  t.len = max(len, 0);
+  const int64_t qpos0 = (int64_t)a.q_pos0[t.b] + t.row0;
+  t.qpos0 = (int32_t)min(qpos0, (int64_t)INT32_MAX);
+  const int64_t end = a.causal ? min((int64_t)t.len, max((int64_t)0, qpos0 + t.n_rows)) : t.len;
+  const int64_t units = ceil_div(end, ATT_WAVES * A4_STEP);
+  t.parts = (int)max((int64_t)1, min((int64_t)a.n_split, units / 2));
+  if (t.split >= t.parts) return false;
+  t.t_begin = (uint32_t)(units * t.split / t.parts) * (ATT_WAVES * A4_STEP);
+  t.t_end = (uint32_t)min(end, units * (t.split + 1) / t.parts * (ATT_WAVES * A4_STEP));
+  return true;
+}
+
+// A row's running maximum is raised only when a score exceeds it by more than this (log2 units).
+constexpr float P4_LAZY = 8.0f;
+
+template <int D, int CT, bool EXACT>
+__global__ void __launch_bounds__(ATT_THREADS, CT * D > 256 ? 1 : 2) paged_prefill4_kernel(Prefill4Args a) {
+  using Lds = A4Lds<D>;
+  constexpr int NC = D / 32, NT = D / 16;
+  Prefill4Tile tl;
+  int32_t e = 0;
+  const bool work = p4_locate(a, blockIdx.x, tl, e);
+  if (!work) {  // block-uniform
+    if (e && a.err && threadIdx.x == 0) atomicOr(a.err, e);
+    return;
+  }
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n = lane & 15, kg = lane >> 4;
+  const int tiles = a.page_size / K4_TOK;
+  const int64_t page_bytes = 2LL * a.n_kv_heads * tiles * k4_tile_bytes(D);
+  const int64_t head_off = (int64_t)tl.h * tiles * k4_tile_bytes(D);
+  const int64_t v_off = (int64_t)a.n_kv_heads * tiles * k4_tile_bytes(D);
+  const float qs = a.sm_log2e;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[ATT_WAVES][Lds::WAVE];
+  __shared__ float sm_m[ATT_WAVES][A4_HEADS], sm_l[ATT_WAVES][A4_HEADS];
+  uint8_t *vt = lds[wave];
+  const int32_t *bt = a.bt + (int64_t)tl.b * a.max_blocks;
+
+  att_bf16x8 qa[CT][NC];
+  uint32_t lim[CT];  // keys below it count for the lane's column
+  uint32_t lim_all = 0xFFFFFFFFu;
+  const int cols = tl.n_rows * tl.G;
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    const int c = 16 * ct + n, row = c / tl.G;
+    const bool live = c < cols;
+    lim[ct] = (uint32_t)tl.len;
+    if (a.causal) lim[ct] = (uint32_t)min((int64_t)tl.len, max((int64_t)0, (int64_t)tl.qpos0 + row + 1));
+    const uint16_t *src = a.q + ((tl.q_lo + tl.row0 + row) * a.n_q_heads + tl.hq0 + (c - row * tl.G)) * (int64_t)D;
+#pragma unroll
+    for (int k = 0; k < NC; ++k) {
+      att_u32x4 w = {0u, 0u, 0u, 0u};
+      if (live) w = *reinterpret_cast<const att_u32x4 *>(src + a4_channel<D>(kg, k));
+      qa[ct][k] = __builtin_bit_cast(att_bf16x8, w);
+    }
+  }
+  // the lowest limit of the tile's rows (row 0's): steps below it need no mask
+  lim_all = a.causal ? (uint32_t)min((int64_t)tl.len, max((int64_t)0, (int64_t)tl.qpos0 + 1)) : (uint32_t)tl.len;
+
+  att_f32x4 o[CT][NT], ol[CT];
+  float m[CT], l[CT];
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) o[ct][t] = att_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    ol[ct] = att_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    m[ct] = -INFINITY;
+    l[ct] = 0.0f;
+  }
+  const att_bf16x8 ones = __builtin_bit_cast(att_bf16x8, att_u32x4{0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u});
+
+  const uint32_t t_end = tl.t_end, t_last = t_end ? t_end - 1 : 0;
+  auto page_of_pos = [&](uint32_t t) { return (uint32_t)(((uint64_t)t * a.p_magic) >> (31 + a.p_shift)); };
+  auto tile_page = [&](uint32_t tp) -> int32_t { return bt[page_of_pos(min(tp, t_last))]; };
+  auto load_tile = [&](uint32_t tp, int32_t page, A4Tile<D> &k, A4Tile<D> &v, int &rows) {
+    const int live = tp < t_end ? (int)min((uint32_t)K4_TOK, t_end - tp) : 0;
+    const uint32_t tc = min(tp, t_last);
+    const uint32_t in_page = tc - page_of_pos(tc) * (uint32_t)a.page_size;
+    const bool ok = page >= 0 && page < a.n_pages;
+    e |= (live > 0 && !ok) ? ZX_KERR_PAGE_RANGE : 0;
+    rows = ok ? live : 0;
+    const int nrec = rows ? k4_tile_bytes(D) : 0;
+    const uint8_t *src =
+        a.pool + (ok ? (int64_t)page * page_bytes + head_off + (int64_t)(in_page / K4_TOK) * k4_tile_bytes(D) : 0);
+    a4_load<D>(__builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(src), (short)0, nrec, 0x00020000), lane, k);
+    a4_load<D>(__builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(src + (ok ? v_off : 0)), (short)0, nrec,
+                                                 0x00020000), lane, v);
+  };
+  auto compute_step = [&](uint32_t t0, const A4Tile<D> (&k)[2], const A4Tile<D> (&v)[2], const int (&rows)[2]) {
+#pragma unroll
+    for (int T = 0; T < 2; ++T) {
+      A4Tile<D> t = v[T];
+      if (rows[T] < K4_TOK) {  // uniform
+#pragma unroll
+        for (int w = 0; w < A4Tile<D>::CW; ++w) t.c[w] = n < rows[T] ? t.c[w] : 0u;
+#pragma unroll
+        for (int i = 0; i < A4Tile<D>::NB; ++i) t.p[i] = n < rows[T] ? t.p[i] : 127u;
+      }
+#pragma unroll
+      for (int w = 0; w < A4Tile<D>::CW; ++w)
+        *reinterpret_cast<att_u32x4 *>(vt + (16 * T + n) * Lds::VROW + 2 * a4_channel<D>(kg, w)) = a4_word<D>(t, w);
+    }
+    float s[CT][8];
+#pragma unroll
+    for (int T = 0; T < 2; ++T) {
+      att_f32x4 sc[CT];
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) sc[ct] = att_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const att_bf16x8 kw = __builtin_bit_cast(att_bf16x8, a4_word<D>(k[T], c));
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct)
+          sc[ct] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kw, qa[ct][c], sc[ct], 0, 0, 0);
+      }
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[ct][4 * T + i] = sc[ct][i] * qs;
+    }
+    if (rows[0] < K4_TOK || rows[1] < K4_TOK || t0 + A4_STEP > lim_all) {  // uniform
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+        for (int T = 0; T < 2; ++T)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int j = 4 * kg + i;
+            if (j >= rows[T] || t0 + 16 * T + j >= lim[ct]) s[ct][4 * T + i] = -INFINITY;
+          }
+    }
+    att_bf16x8 ph[CT], pl[CT];
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      float mx = s[ct][0];
+#pragma unroll
+      for (int i = 1; i < 8; ++i) mx = fmaxf(mx, s[ct][i]);
+      mx = xrow_max(mx);
+      if (__builtin_amdgcn_ballot_w64(mx > m[ct] + P4_LAZY)) {  // (m = -inf: any score raises it)
+        const float m_new = fmaxf(m[ct], mx);
+        const float alpha = m_new == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[ct] - m_new);
+        m[ct] = m_new;
+        l[ct] *= alpha;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) ol[ct][i] *= alpha;
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[ct][t][i] *= alpha;
+      }
+      float p[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) p[i] = s[ct][i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s[ct][i] - m[ct]);
+      if constexpr (EXACT) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) l[ct] += p[i];
+        a4_split(p, ph[ct], pl[ct]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ph[ct][i] = (__bf16)p[i];
+        ol[ct] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, ph[ct], ol[ct], 0, 0, 0);
+      }
+    }
+    a4_wave_sync();
+#pragma unroll
+    for (int jt = 0; jt < NT; ++jt) {
+      const att_bf16x8 av = a4_vt<Lds::VROW>(vt, jt, n, kg);
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
+        o[ct][jt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, ph[ct], o[ct][jt], 0, 0, 0);
+        if constexpr (EXACT) o[ct][jt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, pl[ct], o[ct][jt], 0, 0, 0);
+      }
+    }
+    a4_wave_sync();
+  };
+
+  constexpr uint32_t stride = ATT_WAVES * A4_STEP;
+  uint32_t t0 = tl.t_begin + (uint32_t)wave * A4_STEP;
+  if (t0 < t_end) {  // (a wave without a step leaves its m at -inf)
+    A4Tile<D> k0[2], v0[2], k1[2], v1[2];
+    int r0[2], r1[2];
+    int32_t p0[2], p1[2];
+    auto pages_of_step = [&](uint32_t ts, int32_t (&p)[2]) {
+      p[0] = tile_page(ts);
+      p[1] = tile_page(ts + K4_TOK);
+    };
+    auto load_step = [&](uint32_t ts, const int32_t (&p)[2], A4Tile<D> (&k)[2], A4Tile<D> (&v)[2], int (&rows)[2]) {
+      load_tile(ts, p[0], k[0], v[0], rows[0]);
+      load_tile(ts + K4_TOK, p[1], k[1], v[1], rows[1]);
+    };
+    pages_of_step(t0, p0);
+    load_step(t0, p0, k0, v0, r0);
+    pages_of_step(t0 + stride, p1);
+    while (t0 < t_end) {
+      load_step(t0 + stride, p1, k1, v1, r1);
+      pages_of_step(t0 + 2 * stride, p0);
+      compute_step(t0, k0, v0, r0);
+      t0 += stride;
+      if (t0 >= t_end) break;
+      load_step(t0 + stride, p0, k0, v0, r0);
+      pages_of_step(t0 + 2 * stride, p1);
+      compute_step(t0, k1, v1, r1);
+      t0 += stride;
+    }
+  }
+
+  // the waves' columns meet in LDS, one tile of 16 after the other (O in the place of V)
+  float *acc_w = reinterpret_cast<float *>(vt);
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    if (EXACT) {
+      float x, y;
+      xrow_pair32(l[ct], x, y);
+      xrow_pair16(x + y, x, y);
+      l[ct] = x + y;
+    } else {
+      l[ct] = ol[ct][0];
+    }
+#pragma unroll
+    for (int jt = 0; jt < NT; ++jt) *reinterpret_cast<att_f32x4 *>(acc_w + n * D + 16 * jt + 4 * kg) = o[ct][jt];
+    if (kg == 0) {
+      sm_m[wave][n] = m[ct];
+      sm_l[wave][n] = l[ct];
+    }
+    __syncthreads();
+    for (int idx = threadIdx.x; idx < 16 * D; idx += ATT_THREADS) {
+      const int j = idx / D, d = idx % D, c = 16 * ct + j;
+      if (c >= cols) break;
+      float M = sm_m[0][j];
+#pragma unroll
+      for (int w = 1; w < ATT_WAVES; ++w) M = fmaxf(M, sm_m[w][j]);
+      float acc = 0.0f, ll = 0.0f;
+#pragma unroll
+      for (int w = 0; w < ATT_WAVES; ++w) {
+        const float f = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sm_m[w][j] - M);
+        acc += f * reinterpret_cast<const float *>(lds[w])[j * D + d];
+        ll += f * sm_l[w][j];
+      }
+      if (tl.parts == 1) {
+        const int row = c / tl.G;
+        const float v = ll == 0.0f ? 0.0f : acc / ll;
+        a.out[((tl.q_lo + tl.row0 + row) * a.n_q_heads + tl.hq0 + (c - row * tl.G)) * (int64_t)D + d] =
+            (uint16_t)(pack_bf16(v, 0.0f) & 0xFFFFu);
+      } else {
+        float *pp = a.part + ((tl.item * a.n_split + tl.split) * (16 * CT) + c) * (int64_t)(2 + D);
+        pp[2 + d] = acc;
+        if (d == 0) {
+          pp[0] = M;
+          pp[1] = ll;
+        }
+      }
+    }
+    __syncthreads();
+  }
+  if (e && a.err) atomicOr(a.err, e);
+}
+
+// Merges the parts of tiles that were cut: one block of D threads per column of a tile.
+template <int D>
+__global__ void __launch_bounds__(D) prefill4_combine_kernel(Prefill4Args a, int32_t columns) {
+  const uint32_t item = blockIdx.x / (uint32_t)columns;
+  const int c = (int)(blockIdx.x - item * (uint32_t)columns);
+  Prefill4Tile t;
+  int32_t e = 0;
+  if (!p4_locate(a, item * (uint32_t)a.n_split, t, e) || t.parts == 1 || c >= t.n_rows * t.G) return;
+  const int d = threadIdx.x;
+  const float *pp = a.part + (t.item * a.n_split * columns + c) * (int64_t)(2 + D);
+  const int64_t step = (int64_t)columns * (2 + D);
+  float M = -INFINITY, L = 0.0f, A = 0.0f;
+  for (int s = 0; s < t.parts; ++s) M = fmaxf(M, pp[s * step]);
+  for (int s = 0; s < t.parts; ++s) {
+    const float f = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(pp[s * step] - M);
+    A += f * pp[s * step + 2 + d];
+    L += f * pp[s * step + 1];
+  }
+  const int row = c / t.G;
+  const float v = L == 0.0f ? 0.0f : A / L;
+  a.out[((t.q_lo + t.row0 + row) * a.n_q_heads + t.hq0 + (c - row * t.G)) * (int64_t)D + d] =
+      (uint16_t)(pack_bf16(v, 0.0f) & 0xFFFFu);
+}
+
 }  // namespace zx
 
 using namespace zx;
@@ -342,4 +688,126 @@ extern "C" int zx_paged_attention4_decode(const uint16_t *q, int32_t n_q_heads, 
   }
   if ((rc = check_launch("paged_decode4"))) return rc;
   return att_combine(part, g, nullptr, seq_lens, out, table, st);
+}
+
+// Column tiles per block, by the columns that a sequence can have at most; with head_dim 256 four
+// would not fit the registers.
+static int a4_column_tiles(int64_t columns, int32_t head_dim) {
+  return columns <= 16 ? 1 : columns <= 32 || head_dim == 256 ? 2 : 4;
+}
+
+struct Prefill4Plan {
+  int ct;
+  int32_t group, n_group, rows;
+  int64_t n_rt, items, n_split;
+};
+static Prefill4Plan p4_plan(int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim, int32_t max_blocks,
+                            int32_t page_size, int32_t n_seqs, int32_t max_q) {
+  Prefill4Plan p;
+  const int32_t grp = n_q_heads / n_kv_heads;
+  p.group = (int32_t)ceil_div(grp, a4_groups(grp));
+  p.n_group = n_kv_heads * a4_groups(grp);
+  p.ct = a4_column_tiles((int64_t)max_q * p.group, head_dim);
+  p.rows = 16 * p.ct / p.group;
+  p.n_rt = ceil_div(max_q, p.rows);
+  p.items = p.n_rt * p.n_group * n_seqs;
+  // parts of a tile where the tiles do not fill the chip; none shorter than 256 keys
+  const int64_t units = ceil_div(std::min((int64_t)max_blocks * page_size, (int64_t)INT32_MAX), ATT_WAVES * A4_STEP);
+  const int64_t resident = (p.ct * head_dim > 256 ? 1LL : 2LL) * num_cus();
+  p.n_split = std::max<int64_t>(1, std::min(units / 2, resident / std::max<int64_t>(1, p.items)));
+  return p;
+}
+
+extern "C" size_t zx_paged_attention4_prefill_workspace_bytes(int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim,
+                                                              int32_t page_size, int32_t max_blocks, int32_t n_seqs,
+                                                              int32_t max_q_per_seq) {
+  if (n_seqs <= 0 || n_q_heads <= 0 || n_kv_heads <= 0 || n_q_heads % n_kv_heads || max_blocks <= 0 || page_size <= 0 ||
+      page_size % K4_TOK || max_q_per_seq <= 0 || !(head_dim == 64 || head_dim == 128 || head_dim == 256))
+    return 0;
+  const Prefill4Plan p = p4_plan(n_q_heads, n_kv_heads, head_dim, max_blocks, page_size, n_seqs, max_q_per_seq);
+  return p.n_split > 1 ? (size_t)p.items * p.n_split * 16 * p.ct * (2 + head_dim) * sizeof(float) : 0;
+}
+
+template <int D, int CT>
+static int p4_launch(const Prefill4Args &a, bool exact, unsigned grid, unsigned items, hipStream_t st) {
+  if (CT == 1 || exact)  // (bound by the reads with one tile of columns: the second product is free)
+    paged_prefill4_kernel<D, CT, true><<<grid, ATT_THREADS, 0, st>>>(a);
+  else if constexpr (CT > 1)
+    paged_prefill4_kernel<D, CT, false><<<grid, ATT_THREADS, 0, st>>>(a);
+  const int rc = check_launch("paged_prefill4");
+  if (rc || a.n_split == 1) return rc;
+  prefill4_combine_kernel<D><<<items * 16 * CT, D, 0, st>>>(a, 16 * CT);
+  return check_launch("prefill4_combine");
+}
+
+extern "C" int zx_paged_attention4_prefill(const uint16_t *q, int64_t n_q, const int32_t *cu_q, const int32_t *q_pos0,
+                                           int32_t n_q_heads, const uint8_t *pool, int64_t n_pages, int32_t n_kv_heads,
+                                           int32_t head_dim, int32_t page_size, const int32_t *block_tables,
+                                           int32_t max_blocks, const int32_t *kv_len, int32_t n_seqs,
+                                           int32_t max_q_per_seq, int32_t causal, float sm_scale, int32_t flags,
+                                           uint16_t *out, int32_t *err, void *workspace, size_t workspace_bytes,
+                                           zx_stream_t stream) {
+  clear_error();
+  ZX_REQUIRE(!(flags & ~ZX_PREFILL_EXACT_P), "paged_attention4_prefill: unknown flag bits 0x%x", (unsigned)flags);
+  int rc = k4_check("paged_attention4_prefill", n_pages, n_kv_heads, head_dim, page_size);
+  if (rc) return rc;
+  ZX_REQUIRE(n_q >= 0 && max_q_per_seq >= 0 && n_q_heads > 0 && max_blocks > 0 && n_seqs > 0,
+             "paged_attention4_prefill: sizes must be positive");
+  ZX_REQUIRE(n_q_heads % n_kv_heads == 0, "paged_attention4_prefill: n_q_heads must be a multiple of n_kv_heads");
+  ZX_REQUIRE((int64_t)max_blocks * page_size < (1LL << 31),
+             "paged_attention4_prefill: block tables of 2^31 positions and more");
+  if (n_q == 0 || max_q_per_seq == 0) return ZX_OK;
+  ZX_REQUIRE(q && cu_q && q_pos0 && pool && block_tables && kv_len && out, "paged_attention4_prefill: null pointer");
+  ZX_REQUIRE(aligned16(q) && aligned16(pool) && aligned16(out),
+             "paged_attention4_prefill: q, pool and out must be 16-byte aligned");
+  if (max_q_per_seq > n_q) max_q_per_seq = (int32_t)n_q;
+  const Prefill4Plan p = p4_plan(n_q_heads, n_kv_heads, head_dim, max_blocks, page_size, n_seqs, max_q_per_seq);
+  if (p.items * p.n_split * 16 * p.ct >= (1LL << 31))
+    return fail(ZX_ERR_UNSUPPORTED, "paged_attention4_prefill: too many rows");
+  Prefill4Args a;
+  a.q = q;
+  a.cu_q = cu_q;
+  a.q_pos0 = q_pos0;
+  a.bt = block_tables;
+  a.kv_len = kv_len;
+  a.pool = pool;
+  a.out = out;
+  a.part = static_cast<float *>(workspace);
+  a.err = err;
+  a.n_pages = n_pages;
+  a.n_q_heads = n_q_heads;
+  a.n_kv_heads = n_kv_heads;
+  a.page_size = page_size;
+  a.max_blocks = max_blocks;
+  a.n_seqs = n_seqs;
+  a.causal = causal ? 1 : 0;
+  a.group = p.group;
+  a.n_group = p.n_group;
+  a.rows = p.rows;
+  a.n_rt = (int32_t)p.n_rt;
+  a.max_rows = p.n_rt * p.rows;
+  a.sm_log2e = sm_scale * ATT_LOG2E;
+  const size_t need = zx_paged_attention4_prefill_workspace_bytes(n_q_heads, n_kv_heads, head_dim, page_size, max_blocks,
+                                                                  n_seqs, max_q_per_seq);
+  ZX_REQUIRE(!workspace || aligned16(workspace), "paged_attention4_prefill: workspace must be 16-byte aligned");
+  a.n_split = need && workspace && workspace_bytes >= need ? (int32_t)p.n_split : 1;
+  {
+    int sh = 0;
+    while ((1LL << sh) < page_size) ++sh;
+    a.p_shift = sh;
+    a.p_magic = (uint32_t)(((1ULL << (31 + sh)) + (uint64_t)page_size - 1) / (uint64_t)page_size);
+  }
+  const unsigned items = (unsigned)p.items, grid = items * (unsigned)a.n_split;
+  const hipStream_t st = as_stream(stream);
+  const bool exact = flags & ZX_PREFILL_EXACT_P;
+#define ZX_P4(D)                                                      \
+  p.ct == 1   ? p4_launch<D, 1>(a, exact, grid, items, st)            \
+  : p.ct == 2 ? p4_launch<D, 2>(a, exact, grid, items, st)            \
+              : p4_launch<D, D == 256 ? 2 : 4>(a, exact, grid, items, st)
+  switch (head_dim) {
+    case 64: return ZX_P4(64);
+    case 128: return ZX_P4(128);
+    default: return ZX_P4(256);
+  }
+#undef ZX_P4
 }

@@ -1130,3 +1130,53 @@ def paged_attention4_decode(q: torch.Tensor, pool_layer: torch.Tensor, block_tab
     if check:
         _raise_kernel_error(err, "paged_attention4_decode")
     return out
+
+
+PRECISIONS4 = ("bf16", "exact")
+
+
+def paged_attention4_prefill(q: torch.Tensor, cu_q: torch.Tensor, q_pos0: torch.Tensor, pool_layer: torch.Tensor,
+                             block_tables: torch.Tensor, kv_len: torch.Tensor, causal: bool = True,
+                             sm_scale: float | None = None, max_q_per_seq: int | None = None,
+                             precision: str = "bf16", out: torch.Tensor | None = None, check: bool = False,
+                             err: torch.Tensor | None = None) -> torch.Tensor:
+    """Blocks of queries over 4-bit pages: ``q [n_q, Hq, D]`` bf16 rows of all sequences
+    (``cu_q`` int32 ``[B + 1]`` offsets, ``q_pos0`` int32 ``[B]`` position of each sequence's
+    first row) attend to keys ``[0, kv_len[b])``, when ``causal`` those up to their own
+    position.  ``precision``: the softmax weights rounded once to bf16 (error within one ulp +
+    2^-7 max|V|), or ``"exact"``, carried to 2^-17 (one ulp + 2^-15 max|V|).  ``max_q_per_seq``
+    bounds every sequence's rows (read back from ``cu_q`` without it, which waits for the
+    device); rows beyond it, and rows in no sequence, are left as they are in ``out``.
+    ``err`` (device int32 ``[1]``) collects the kernels' error bits; ``check`` reads them and
+    raises."""
+    N.need_gpu()
+    if precision not in PRECISIONS4:
+        raise ValueError(f"precision must be one of {PRECISIONS4}, got {precision!r}")
+    n_pages, Hkv, P, D = _attention4_args(q, pool_layer, block_tables, out)
+    n_q, Hq, _ = q.shape
+    B = block_tables.shape[0]
+    for name, t, n in (("cu_q", cu_q, B + 1), ("q_pos0", q_pos0, B), ("kv_len", kv_len, B)):
+        if t.dtype != torch.int32 or t.numel() != n:
+            raise ValueError(f"{name} must be int32 [{n}]")
+    if err is not None and (err.dtype != torch.int32 or err.numel() < 1 or err.device != q.device):
+        raise ValueError("err must be an int32 tensor on q's device")
+    out = torch.empty_like(q) if out is None else out
+    _all_on(q.device, q=q, cu_q=cu_q, q_pos0=q_pos0, pool_layer=pool_layer, block_tables=block_tables, kv_len=kv_len,
+            out=out)
+    if max_q_per_seq is None:
+        max_q_per_seq = int((cu_q[1:] - cu_q[:-1]).max().item()) if B else 0
+    mq = max(0, min(int(max_q_per_seq), n_q))
+    lib = N.load()
+    mb = block_tables.shape[1]
+    with _on(q.device):
+        nb = lib.zx_paged_attention4_prefill_workspace_bytes(Hq, Hkv, D, P, mb, B, mq)
+        ws = _workspace(nb, q.device) if nb else None
+        err = _err_word_if(check, q.device) if err is None else err
+        N.check(lib.zx_paged_attention4_prefill(
+            N.ptr(q), n_q, N.ptr(cu_q), N.ptr(q_pos0), Hq, N.ptr(pool_layer), n_pages, Hkv, D, P, N.ptr(block_tables),
+            mb, N.ptr(kv_len), B, mq, int(bool(causal)), float(D ** -0.5 if sm_scale is None else sm_scale),
+            N.ZX_PREFILL_EXACT_P if precision == "exact" else 0, N.ptr(out), N.ptr(err), N.ptr(ws), nb,
+            N.stream_ptr(q.device)), "paged_attention4_prefill")
+    if check:
+        _raise_kernel_error(err, "paged_attention4_prefill")
+    return out
