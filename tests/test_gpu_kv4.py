@@ -1,0 +1,539 @@
+"""GPU 4-bit KV pages: append and gather to the bit against the oracle's search for the nearest
+code, decode and prefill attention against float64 on the decoded pages.
+
+Attention's tolerance, elementwise, beside half a bf16 step of the value (2^-8 of it) for the last
+rounding:
+
+* weights: hi + lo of bf16 carry a weight to 2^-16 of it, one bf16 to 2^-8; a row is a weighted
+  mean, so weights off by e move it by at most 2 e max|V|;
+* scores: a sum of D products in fp32 and its scaling by sm_scale log2(e) are off by at most
+  (D + 4) 2^-24 sum|q k|, the exponential by 2^-22 of a weight: each weight by
+  e = (D + 4) 2^-24 |sm| sum|q k| + 2^-21 (subtracting the maximum adds 2^-24 of a score, in it);
+* sums over keys in fp32: at most (n / 32 + 64) additions follow each other in an accumulator
+  and its merges, 2^-24 each, on numerator and denominator: 2 (n / 32 + 64) 2^-24 max|V|.
+"""
+import numpy as np
+import pytest
+import torch
+
+from oracle import kv4 as R
+from zenyx_amd import _native as N
+from zenyx_amd import kv
+from zenyx_amd.train.fp8_kv_quantization import PagedFP4KVCache, PagedFP8KVCache, QuantizedRingAttention
+from zenyx_amd.train.rotary import RotaryPositions, rotary_frequencies
+
+pytestmark = pytest.mark.gpu
+
+
+def bits(t):
+    return t.detach().cpu().contiguous().view(torch.int16).numpy()
+
+
+def tables(total, P, extra, seed):
+    rng = np.random.default_rng(seed)
+    need = [-(-t // P) for t in total]
+    n_pages = sum(need) + extra
+    perm = rng.permutation(n_pages).astype(np.int32)
+    bt = np.full((len(total), max(max(need), 1)), -1, np.int32)
+    k = 0
+    for b, n in enumerate(need):
+        bt[b, :n] = perm[k:k + n]
+        k += n
+    return bt, n_pages
+
+
+def i32(v, dev):
+    return torch.as_tensor(np.ascontiguousarray(v, np.int32), device=dev)
+
+
+# ------------------------------------------------------------------ codes
+
+def special_blocks():
+    """bf16 bit patterns [n, 32] that visit every power, the ties and what is not finite."""
+    rng = np.random.default_rng(0)
+    blocks = []
+    for e in list(range(0, 12)) + list(range(118, 136)) + list(range(244, 256)):  # exponent fields of the largest
+        for m in (0, 1, 63, 64, 65, 95, 96, 97, 127):
+            top = (e << 7) | m
+            other = rng.integers(0, top + 1, 31) if top else np.zeros(31, np.int64)
+            blocks.append(np.concatenate([[top], other]) | (rng.integers(0, 2, 32) << 15))
+    # every tie and its neighbours at several powers
+    for e in (-120, -3, 0, 5, 100):
+        for p in (0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 0.5, 1, 6):
+            v = np.float32(p * 2.0 ** e)
+            b = int(v.view(np.uint32)) >> 16
+            row = np.array([b, b - 1, b + 1, b | 0x8000, 0, 0x8000] + [b] * 26)
+            row[6] = int(np.float32(6 * 2.0 ** e).view(np.uint32)) >> 16
+            blocks.append(row)
+    for bad in (0x7F80, 0xFF80, 0x7FC0, 0xFFFF, 0x7F81):
+        row = rng.integers(0, 0x4100, 32)
+        row[rng.integers(32)] = bad
+        blocks.append(row)
+    return np.array(blocks, np.uint16)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_codes_of_special_blocks(dev, D):
+    b = special_blocks()
+    b = b[:len(b) // (D // 32) * (D // 32)].reshape(-1, D)
+    T, P, H = len(b), 32, 1
+    x = torch.from_numpy(np.stack([b, b[::-1]], 1).astype(np.int16).copy()).view(torch.bfloat16)  # [T, 2, D]
+    bt, n_pages = tables([T], P, 1, 0)
+    pool = kv.kv4_pool(1, n_pages, H, P, D)
+    kv.kv4_append(x[None, :, :, None].contiguous().to(dev), i32([0, T], dev), i32(bt, dev), pool, check=True)
+    want = np.zeros(pool.shape, np.uint8)
+    for kv_ in range(2):
+        vals = x[:, kv_].float().numpy()
+        for t in range(T):
+            R.store(want[0], bt[0, t // P], kv_, 0, t % P, vals[t])
+    assert np.array_equal(pool.cpu().numpy(), want)
+    k, v = kv.kv4_gather_dequant(pool[0], i32(bt, dev), i32([T], dev), T, check=True)
+    for got, kv_ in ((k, 0), (v, 1)):
+        w, ok = R.load(want[0], bt[0], T, kv_)
+        g = got[0].float().cpu().numpy()
+        assert ok.all() and np.array_equal(np.isnan(g), np.isnan(w))
+        assert np.array_equal(g[~np.isnan(g)], w[~np.isnan(w)].astype(np.float32))
+
+
+CASES = [  # lens, old, L, H, D, P, rot, rows behind the last sequence
+    ([1], [0], 1, 1, 64, 16, 0, 0), ([1, 1, 1], [5, 0, 33], 3, 8, 128, 16, 128, 0), ([0, 7, 0, 40], [3, 0, 9, 1], 2, 3, 64, 48, 32, 5),
+    ([70, 5, 33], [0, 100, 17], 1, 2, 128, 16, 64, 0), ([17], [0], 2, 1, 256, 16, 256, 3), ([64, 31], [0, 0], 1, 5, 128, 32, 112, 1),
+    ([20], [3], 1, 2, 256, 32, 16, 0), ([2500, 1, 1700], [0, 90, 11], 4, 8, 128, 16, 128, 2), ([9000], [0], 1, 12, 64, 64, 64, 0),
+    ([37], [0], 1, 71, 128, 16, 96, 0)]
+
+
+def oracle_append(x, bt, lens, old, pool):
+    """x [L, T, 2, H, D] torch bf16 (rotated) into pool (numpy): vectorised over tokens."""
+    L, _, _, H, D = x.shape
+    P = pool.shape[4] * 16
+    seq = np.repeat(np.arange(len(lens)), lens)
+    pos = np.concatenate([np.arange(a, a + n) for a, n in zip(old, lens)]) if sum(lens) else np.zeros(0, int)
+    page, row = bt[seq, pos // P], pos % P
+    f = x[:, :len(seq)].float().cpu().numpy()
+    for layer in range(L):
+        code, byte = R.encode_block(f[layer].reshape(len(seq), 2, H, D // 32, 32))
+        packed = code[..., 0::2] | (code[..., 1::2] << 4)  # [T, 2, H, D / 32, 16]
+        tiles = pool[layer][..., :8 * D].reshape(*pool.shape[1:5], D // 32, 16, 16).copy()
+        tiles[page, :, :, row // 16, :, row % 16] = packed
+        pw = pool[layer][..., 8 * D:].reshape(*pool.shape[1:5], D // 32, 16).copy()
+        pw[page, :, :, row // 16, :, row % 16] = byte
+        pool[layer][..., :8 * D] = tiles.reshape(*pool.shape[1:5], -1)
+        pool[layer][..., 8 * D:] = pw.reshape(*pool.shape[1:5], -1)
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("case", range(len(CASES)))
+def test_append_and_gather(dev, case, interleaved):
+    lens, old, L, H, D, P, rot, pad = CASES[case]
+    interleaved = interleaved and rot > 0
+    T = sum(lens)
+    total = [a + b for a, b in zip(lens, old)]
+    bt, n_pages = tables(total, P, 3, case)
+    g = torch.Generator(device=dev).manual_seed(case)
+    x = torch.randn((L, T + pad, 2, H, D), generator=g, device=dev).to(torch.bfloat16)
+    x *= torch.exp2(torch.randint(-6, 7, (1, 1, 1, 1, D), generator=g, device=dev).float()).to(torch.bfloat16)
+    cu, start = i32(np.concatenate([[0], np.cumsum(lens)]), dev), i32(old, dev)
+    turned, table = x, None
+    if rot:
+        table = kv.rope_table(rotary_frequencies(rot)[0].to(dev), max(total) + 1)
+        p = i32(np.concatenate([np.arange(a, a + n) for a, n in zip(old, lens)] + [np.zeros(pad)]), dev)
+        turned = x.clone()
+        for layer in range(L):
+            turned[layer, :, 0] = kv.rope(x[layer, :, 0].contiguous(), table, p, interleaved=interleaved)
+    pool = torch.randint(0, 256, tuple(kv.kv4_pool(L, n_pages, H, P, D).shape), generator=g, device=dev, dtype=torch.uint8)
+    want = pool.cpu().numpy()
+    oracle_append(turned, bt, lens, old, want)
+    kv.kv4_append(x, cu, i32(bt, dev), pool, start_pos=start, table=table, interleaved=interleaved, check=True)
+    assert np.array_equal(pool.cpu().numpy(), want)
+    # back: the whole sequences of the last layer, short of them and beyond them
+    layer = L - 1
+    for out_len in sorted({1, max(total) // 2 + 1, max(total) + 37}):
+        k, v = kv.kv4_gather_dequant(pool[layer], i32(bt, dev), i32(total, dev), out_len)
+        for got, kv_ in ((k, 0), (v, 1)):
+            got = got.float().cpu().numpy()
+            for b, n in enumerate(total):
+                m = min(n, out_len)
+                w, _ = R.load(want[layer], bt[b], m, kv_)
+                with np.errstate(over="ignore"):  # (random power bytes: 6 x 2^127 is an infinity in bf16 too)
+                    w = w.astype(np.float32)
+                np.testing.assert_array_equal(got[b, :, :m], w)
+                assert not got[b, :, m:].any()
+
+
+def test_append_bad_pages_and_positions(dev):
+    H, D, P = 2, 64, 16
+    bt = np.array([[0, 99, 2], [3, -1, 4]], np.int32)
+    x = torch.randn((2, 120, 2, H, D), device=dev).to(torch.bfloat16)
+    cu = i32([0, 60, 120], dev)  # 12 positions past each table
+    pool = torch.full((2, 5, 2, H, 1, 544), 3, dtype=torch.uint8, device=dev)
+    err = torch.zeros(1, dtype=torch.int32, device=dev)
+    kv.kv4_append(x, cu, i32(bt, dev), pool, err=err)
+    assert err.item() == N.ZX_KERR_PAGE_RANGE | N.ZX_KERR_POS_RANGE
+    assert torch.all(pool[:, 1] == 3)
+    good = torch.full_like(pool, 3)
+    for b, col, page in ((0, 0, 0), (0, 2, 2), (1, 0, 3), (1, 2, 4)):
+        one = x[:, 60 * b + 16 * col:60 * b + 16 * col + 16].contiguous()
+        kv.kv4_append(one, i32([0, 16], dev), i32([[page]], dev), good, check=True)
+    assert torch.equal(pool, good)
+    with pytest.raises(ValueError, match="block table"):
+        kv.kv4_append(x, cu, i32(bt, dev), pool, check=True)
+    # negative start positions and a table shorter than the sequence
+    kv.kv4_append(x[:, :4].contiguous(), i32([0, 4], dev), i32([[1]], dev), pool, start_pos=i32([-2], dev), err=err.zero_())
+    assert err.item() == N.ZX_KERR_POS_RANGE
+    table = kv.rope_table(rotary_frequencies(64)[0].to(dev), 5)
+    before = pool.clone()
+    kv.kv4_append(x[:, :9].contiguous(), i32([0, 9], dev), i32([[1]], dev), pool, table=table, err=err.zero_())
+    assert err.item() == N.ZX_KERR_POS_RANGE
+    changed = (pool != before)[:, 1, ..., :512].reshape(2, 2, H, 2, 16, 16).any(-1)
+    assert changed[:, :, :, :, :5].float().mean() > 0.9 and not changed[:, :, :, :, 5:].any()
+
+
+def test_gather_bad_pages(dev):
+    pool = torch.randint(0, 120, (4, 2, 3, 1, 1088), device=dev, dtype=torch.uint8)
+    bt = i32([[1, 7, 2], [0, 3, -1]], dev)
+    err_free = kv.kv4_gather_dequant(pool, i32([[1, 1, 2], [0, 3, 3]], dev), i32([48, 40], dev), 64)
+    k, v = kv.kv4_gather_dequant(pool, bt, i32([48, 40], dev), 64)
+    for got, want in zip((k, v), err_free):
+        want = want.clone()
+        want[0, :, 16:32] = 0
+        want[1, :, 32:] = 0
+        assert torch.equal(got, want)
+    with pytest.raises(ValueError, match="block table"):
+        kv.kv4_gather_dequant(pool, bt, i32([48, 40], dev), 64, check=True)
+    with pytest.raises(ValueError, match="position"):
+        kv.kv4_gather_dequant(pool, i32([[0, 1]], dev), i32([40], dev), 48, check=True)
+
+
+# ------------------------------------------------------------------ attention
+
+def random_pool(n_pages, H, P, D, seed, spread=3):
+    rng = np.random.default_rng(seed)
+    pool = rng.integers(0, 256, (n_pages, 2, H, P // 16, 17 * D // 2), dtype=np.uint8)
+    pool[..., 8 * D:] = rng.integers(126 - spread, 127, pool[..., 8 * D:].shape)
+    return pool
+
+
+def check_rows(got, want, qk, vm, n, D, sm, weight):
+    """got / want [rows, D], qk [rows], vm [D]; n keys; weight: what a weight's rounding costs."""
+    nan = np.isnan(want)
+    assert np.array_equal(np.isnan(got), nan)
+    e = (weight + (D + 4) * 2.0 ** -24 * abs(sm) * qk[:, None] + 2.0 ** -21 + (n / 32 + 64) * 2.0 ** -24)
+    with np.errstate(invalid="ignore"):
+        tol = 2.0 ** -8 * np.abs(want) + 2.1 * e * vm[None] + 2.0 ** -133
+        bad = ~nan & ~(np.abs(got - want) <= tol)
+    assert not bad.any(), (got[bad][:4], want[bad][:4], np.broadcast_to(tol, got.shape)[bad][:4])
+
+
+def check_attention(got, q, pool, bt, lens, sm, weight, rows=None, pos0=None, causal=False):
+    """got [n_q, Hq, D] against float64; rows[b] rows of sequence b from pos0[b] (decode: one)."""
+    n_pages, _, H, tiles, nb = pool.shape
+    D, P = nb * 2 // 17, tiles * 16
+    got, q = got.double().cpu().numpy(), q.double().cpu().numpy()
+    at = 0
+    for b, n in enumerate(lens):
+        r = 1 if rows is None else rows[b]
+        n = max(0, min(int(n), bt.shape[1] * P))
+        k, ok = R.load(pool, bt[b], n, 0)
+        v, _ = R.load(pool, bt[b], n, 1)
+        seen = np.broadcast_to(ok, (r, n))
+        if causal:
+            seen = seen & (np.arange(n) <= pos0[b] + np.arange(r)[:, None])
+        grp = q.shape[1] // H
+        for hq in range(q.shape[1]):
+            want, qk, vm = R.attend(q[at:at + r, hq], k[hq // grp], v[hq // grp], seen, sm)
+            check_rows(got[at:at + r, hq], want, qk, vm, n, D, sm, weight)
+        at += r
+
+
+DECODE = [  # lens, Hq, Hkv, D, P, spare table columns
+    ([1], 1, 1, 64, 16, 0), ([0, 5, 16], 8, 2, 128, 16, 1), ([15, 17, 31, 32, 33], 6, 2, 128, 16, 0),
+    ([127, 128, 129, 1, 0, 300], 32, 8, 128, 16, 40), ([700], 32, 8, 128, 16, 200), ([2000, 3], 17, 1, 64, 48, 0),
+    ([90, 1000], 71, 1, 64, 16, 3), ([333, 64], 12, 12, 64, 32, 0), ([500, 77, 1], 16, 2, 256, 16, 9), ([250] * 5, 3, 1, 256, 64, 0),
+    (list(range(1, 100)), 4, 2, 64, 16, 0), ([40] * 70 + [0, 3000], 4, 2, 128, 16, 5), ([4100], 8, 8, 128, 112, 0)]
+
+
+@pytest.mark.parametrize("case", range(len(DECODE)))
+def test_decode(dev, case):
+    lens, Hq, H, D, P, spare = DECODE[case]
+    bt, n_pages = tables(lens, P, 2, case)
+    bt = np.concatenate([bt, np.full((len(lens), spare), -1, np.int32)], 1)
+    pool = random_pool(n_pages, H, P, D, case)
+    # beyond a sequence's end a page holds what is not a number: it must not be seen
+    for b, n in enumerate(lens):
+        if n % 16:
+            tile = pool[bt[b, n // P], :, :, (n % P) // 16]
+            tile[..., 8 * D:].reshape(2, H, D // 32, 16)[..., n % 16:] = 255
+    q = torch.randn((len(lens), Hq, D), device=dev).mul(1.5).to(torch.bfloat16)
+    pd, btd, ld = torch.from_numpy(pool).to(dev), i32(bt, dev), i32(lens, dev)
+    got = kv.paged_attention4_decode(q, pd, btd, ld, check=True)
+    check_attention(got, q, pool, bt, lens, D ** -0.5, 2.0 ** -16)
+    out = torch.full_like(q, 3.0)
+    assert kv.paged_attention4_decode(q, pd, btd, ld, sm_scale=-0.3, out=out) is out
+    check_attention(out, q, pool, bt, lens, -0.3, 2.0 ** -16) if case < 4 else None
+    again = kv.paged_attention4_decode(q, pd, btd, ld)
+    assert np.array_equal(bits(again), bits(got))
+
+
+def test_decode_equals_the_gathered_pages(dev):
+    """The kernel reads what the gather writes: its error against the gathered bf16 is the same."""
+    lens = [100, 37]
+    bt, n_pages = tables(lens, 16, 0, 3)
+    pool = random_pool(n_pages, 2, 16, 128, 3)
+    pd = torch.from_numpy(pool).to(dev)
+    k, v = kv.kv4_gather_dequant(pd, i32(bt, dev), i32(lens, dev), 112)
+    q = torch.randn((2, 4, 128), device=dev).to(torch.bfloat16)
+    got = kv.paged_attention4_decode(q, pd, i32(bt, dev), i32(lens, dev)).double().cpu()
+    for b, n in enumerate(lens):
+        for hq in range(4):
+            s = (q[b, hq].double().cpu() @ k[b, hq // 2, :n].double().cpu().T) * 128 ** -0.5
+            want = torch.softmax(s, -1) @ v[b, hq // 2, :n].double().cpu()
+            assert torch.all((got[b, hq] - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -14 * 6)
+
+
+def test_decode_nan_and_bad_pages(dev):
+    H, Hq, D, P = 2, 4, 128, 16
+    lens = [40, 33, 20, 60]
+    bt, n_pages = tables(lens, P, 1, 5)
+    pool = random_pool(n_pages, H, P, D, 5)
+    pool[bt[0, 1], 0, 0, 0, 8 * D + 3] = 255       # a key's block of (sequence 0, head 0)
+    pool[bt[1, 0], 1, 1, 0, 8 * D + 16 * 2 + 5] = 255  # channels 64..96 of a value of (1, head 1)
+    bt[2, :] = [n_pages, -1, -7, 2 ** 31 - 1][:1] * bt.shape[1]  # no good page: as an empty sequence
+    bt[3, 1] = -1
+    q = torch.randn((4, Hq, D), device=dev).to(torch.bfloat16)
+    args = (q, torch.from_numpy(pool).to(dev), i32(bt, dev), i32(lens, dev))
+    got = kv.paged_attention4_decode(*args)
+    assert not got[2].any() and torch.isnan(got[0, :2]).all() and not torch.isnan(got[0, 2:]).any()
+    n = torch.isnan(got[1])
+    assert n[2:, 64:96].all() and n.sum() == 2 * 32
+    with pytest.raises(ValueError, match="block table"):
+        kv.paged_attention4_decode(*args, check=True)
+    keep = [3]
+    check_attention(got[keep], q[keep], pool, bt[keep], [60], D ** -0.5, 2.0 ** -16)
+    with pytest.raises(ValueError, match="position"):
+        kv.paged_attention4_decode(q[:1], args[1], i32([[0, 1]], dev), i32([33], dev), check=True)
+    # a single NaN key makes its row NaN, not zero
+    pool[:, 0, :, :, 8 * D:] = 255
+    got = kv.paged_attention4_decode(q[:1], torch.from_numpy(pool).to(dev), i32(bt[:1], dev), i32([1], dev))
+    assert torch.isnan(got).all()
+
+
+PREFILL = [  # rows, tokens before, Hq, Hkv, D, P, causal
+    ([1], [0], 1, 1, 64, 16, True), ([3, 0, 5], [10, 4, 0], 4, 2, 128, 16, True), ([4, 1, 2], [500, 1000, 31], 32, 8, 128, 16, True),
+    ([40, 17], [0, 90], 4, 1, 128, 32, True), ([130], [60], 8, 8, 64, 16, True), ([33, 64], [100, 0], 6, 2, 256, 16, True),
+    ([20, 7], [40, 200], 4, 2, 128, 16, False), ([100, 3], [3, 900], 17, 1, 64, 48, True), ([8], [3000], 8, 1, 128, 16, True),
+    ([70, 1], [0, 0], 71, 1, 64, 16, True), ([5], [1500], 4, 4, 256, 16, False), ([200], [0], 3, 1, 128, 112, True)]
+
+
+@pytest.mark.parametrize("precision", ["bf16", "exact"])
+@pytest.mark.parametrize("case", range(len(PREFILL)))
+def test_prefill(dev, case, precision):
+    rows, old, Hq, H, D, P, causal = PREFILL[case]
+    lens = [a + b for a, b in zip(rows, old)]
+    bt, n_pages = tables(lens, P, 2, case + 50)
+    pool = random_pool(n_pages, H, P, D, case)
+    for b, n in enumerate(lens):
+        if n % 16:
+            tile = pool[bt[b, n // P], :, :, (n % P) // 16]
+            tile[..., 8 * D:].reshape(2, H, D // 32, 16)[..., n % 16:] = 255
+    pad = 3  # rows behind the last sequence
+    q = torch.randn((sum(rows) + pad, Hq, D), device=dev).mul(1.5).to(torch.bfloat16)
+    cu = i32(np.concatenate([[0], np.cumsum(rows)]), dev)
+    args = (q, cu, i32(old, dev), torch.from_numpy(pool).to(dev), i32(bt, dev), i32(lens, dev))
+    out = torch.full_like(q, 5.0)
+    kv.paged_attention4_prefill(*args, causal=causal, precision=precision, out=out, check=True)
+    assert torch.all(out[sum(rows):] == 5)
+    weight = 2.0 ** -16 if precision == "exact" else 2.0 ** -8
+    check_attention(out[:sum(rows)], q, pool, bt, lens, D ** -0.5, weight, rows, old, causal)
+    # a loose bound on the rows changes tiles, not results; nor does running uncut
+    loose = torch.full_like(q, 5.0)
+    kv.paged_attention4_prefill(*args, causal=causal, precision=precision, out=loose, max_q_per_seq=max(rows) + 100, check=True)
+    check_attention(loose[:sum(rows)], q, pool, bt, lens, D ** -0.5, weight, rows, old, causal)
+    uncut = torch.full_like(q, 5.0)
+    lib = N.load()
+    N.check(lib.zx_paged_attention4_prefill(
+        q.data_ptr(), q.shape[0], cu.data_ptr(), args[2].data_ptr(), Hq, args[3].data_ptr(), n_pages, H, D, P,
+        args[4].data_ptr(), bt.shape[1], args[5].data_ptr(), len(rows), max(rows), int(causal), D ** -0.5,
+        N.ZX_PREFILL_EXACT_P if precision == "exact" else 0, uncut.data_ptr(), None, None, 0, N.stream_ptr(dev)), "uncut")
+    check_attention(uncut[:sum(rows)], q, pool, bt, lens, D ** -0.5, weight, rows, old, causal)
+    assert torch.all(uncut[sum(rows):] == 5)
+
+
+def test_prefill_rows_without_keys_and_errors(dev):
+    H, Hq, D, P = 2, 4, 64, 16
+    bt, n_pages = tables([64, 64, 64], P, 0, 9)
+    pool = random_pool(n_pages, H, P, D, 9)
+    q = torch.randn((30, Hq, D), device=dev).to(torch.bfloat16)
+    cu, pd, btd = i32([0, 10, 20, 30], dev), torch.from_numpy(pool).to(dev), i32(bt, dev)
+    # positions below 0 see nothing, a sequence without keys neither; rows past the keys see them all
+    pos0, lens = [-5, 0, 100], [40, 0, 30]
+    got = kv.paged_attention4_prefill(q, cu, i32(pos0, dev), pd, btd, i32(lens, dev), check=True)
+    assert not got[:5].any() and not got[10:20].any() and got[5:10].any()
+    check_attention(got, q, pool, bt, lens, D ** -0.5, 2.0 ** -8, [10, 10, 10], pos0, True)
+    out = torch.full_like(q, 5.0)
+    err = torch.zeros(1, dtype=torch.int32, device=dev)
+    kv.paged_attention4_prefill(q, cu, i32([20, 20, 20], dev), pd, btd, i32([30, 30, 30], dev), max_q_per_seq=8, out=out, err=err)
+    assert err.item() == N.ZX_KERR_POS_RANGE  # two rows of each sequence are not computed
+    rows = out.view(3, 10, Hq, D)
+    assert torch.all(rows[:, 8:] == 5) and not (rows[:, :8] == 5).all(-1).any()
+    bad = bt.copy()
+    bad[1, 1] = n_pages
+    with pytest.raises(ValueError, match="block table"):
+        kv.paged_attention4_prefill(q, cu, i32([20] * 3, dev), pd, i32(bad, dev), i32([30] * 3, dev), check=True)
+    with pytest.raises(ValueError, match="position"):
+        kv.paged_attention4_prefill(q, cu, i32([60] * 3, dev), pd, btd, i32([70] * 3, dev), check=True)
+    empty = kv.paged_attention4_prefill(q[:0], i32([0, 0, 0, 0], dev), i32(pos0, dev), pd, btd, i32(lens, dev))
+    assert empty.shape == (0, Hq, D)
+
+
+def test_prefill_nan_reaches_only_rows_that_see_it(dev):
+    """A NaN key or value at position 25 of 40: rows before it are as without it."""
+    H, Hq, D, P, n = 1, 2, 128, 16, 40
+    bt, n_pages = tables([n], P, 0, 4)
+    clean = random_pool(n_pages, H, P, D, 4)
+    q = torch.randn((n, Hq, D), device=dev).to(torch.bfloat16)
+
+    def run(pool):
+        return kv.paged_attention4_prefill(q, i32([0, n], dev), i32([0], dev), torch.from_numpy(pool).to(dev), i32(bt, dev),
+                                           i32([n], dev), precision="exact")
+    want = run(clean)
+    for kv_ in range(2):
+        pool = clean.copy()
+        pool[bt[0, 1], kv_, 0, 0, 8 * D + 16 * 3 + 9] = 255  # block 3 (channels 96..128) of position 25
+        got = run(pool)
+        assert torch.isnan(got[25:]).any(-1).all()
+        if kv_ == 0:
+            assert torch.equal(got[:25], want[:25])
+        else:  # weights of 0 times NaN may reach earlier rows of the same 32 keys, in its channels only
+            assert torch.equal(got[..., :96], want[..., :96]) and not torch.isnan(got[..., :96]).any()
+
+
+def test_refusals(dev):
+    pool, bt, lens = kv.kv4_pool(1, 4, 2, 16, 64), i32([[0, 1]], dev), i32([5], dev)
+    q = torch.zeros((1, 4, 64), dtype=torch.bfloat16, device=dev)
+    x = torch.zeros((1, 5, 2, 2, 64), dtype=torch.bfloat16, device=dev)
+    cu = i32([0, 5], dev)
+    table = kv.rope_table(rotary_frequencies(128)[0].to(dev), 5)
+    for bad in (lambda: kv.kv4_pool(1, 4, 2, 24, 64), lambda: kv.kv4_pool(1, 4, 2, 16, 96), lambda: kv.kv4_pool(1, 4, 2, 0, 64),
+                lambda: kv.kv4_append(x.half(), cu, bt, pool), lambda: kv.kv4_append(x, cu, bt, pool[..., :500]),
+                lambda: kv.kv4_append(x, cu, bt, kv.kv4_pool(1, 4, 3, 16, 64)), lambda: kv.kv4_append(x, cu, bt, pool, table=table),
+                lambda: kv.kv4_append(x, cu, bt, pool, interleaved=True), lambda: kv.kv4_append(x, cu.long(), bt, pool),
+                lambda: kv.kv4_append(x, cu, bt.cpu(), pool), lambda: kv.kv4_append(x[..., :32], cu, bt, pool),
+                lambda: kv.kv4_gather_dequant(pool, bt, lens), lambda: kv.kv4_gather_dequant(pool[0], bt, lens.long()),
+                lambda: kv.kv4_gather_dequant(pool[0], bt, i32([1, 2], dev)),
+                lambda: kv.paged_attention4_decode(q.float(), pool[0], bt, lens),
+                lambda: kv.paged_attention4_decode(q[:, :3], pool[0], bt, lens),
+                lambda: kv.paged_attention4_decode(q[..., :32], pool[0], bt, lens),
+                lambda: kv.paged_attention4_decode(q, pool[0], bt, i32([1, 2], dev)),
+                lambda: kv.paged_attention4_decode(q, pool[0], bt, lens, out=q.float()),
+                lambda: kv.paged_attention4_prefill(q, cu, lens, pool[0], bt, lens, precision="f16"),
+                lambda: kv.paged_attention4_prefill(q, lens, lens, pool[0], bt, lens),
+                lambda: kv.paged_attention4_prefill(q, cu, lens.long(), pool[0], bt, lens),
+                lambda: PagedFP4KVCache(1, 2, 64, 4, page_size=8), lambda: PagedFP4KVCache(1, 2, 80, 4)):
+        with pytest.raises(ValueError):
+            bad()
+
+
+def test_streams_and_graphs(dev):
+    """On another stream, and two captured graphs replayed in turn with eager work between."""
+    lens, Hq, H, D, P = [700, 20, 333], 8, 2, 128, 16
+    bt, n_pages = tables(lens, P, 0, 8)
+    pd, btd, ld = torch.from_numpy(random_pool(n_pages, H, P, D, 8)).to(dev), i32(bt, dev), i32(lens, dev)
+    q = torch.randn((3, Hq, D), device=dev).to(torch.bfloat16)
+    cu, pos0 = i32([0, 1, 2, 3], dev), i32([n - 1 for n in lens], dev)
+
+    def both():
+        return (kv.paged_attention4_decode(q, pd, btd, ld),
+                kv.paged_attention4_prefill(q, cu, pos0, pd, btd, ld, max_q_per_seq=1))
+    want = both()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = both()
+    torch.cuda.current_stream().wait_stream(s)
+    assert all(np.array_equal(bits(a), bits(b)) for a, b in zip(got, want))
+    graphs, outs = [], []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(both())
+        graphs.append(g)
+    for i in range(4):
+        q.copy_(torch.randn(q.shape, device=dev))
+        for g in graphs:
+            g.replay()
+        want = both()
+        torch.cuda.synchronize()
+        for o in outs:
+            assert all(np.array_equal(bits(a), bits(b)) for a, b in zip(o, want))
+
+
+# ------------------------------------------------------------------ together
+
+@pytest.mark.parametrize("four", [False, True])
+@pytest.mark.parametrize("interleaved, rot", [(False, 128), (True, 64)])
+def test_a_cache_that_rotates(dev, four, interleaved, rot):
+    """Prompts, a chunk on top, decode steps, a freed sequence: keys rotated while stored and
+    queries on their way, against the same cache given rotated keys and queries."""
+    L, H, Hq, D = 2, 2, 8, 128
+    rope = RotaryPositions(D, 400, rotary_dim=rot, interleaved=interleaved)
+    make = (lambda r: PagedFP4KVCache(L, H, D, 60, rope=r)) if four else (lambda r: PagedFP8KVCache(L, H, D, 60, rope=r))
+    cache, plain = make(rope), make(None)
+    att, ref = QuantizedRingAttention(cache, ring_degree=2), QuantizedRingAttention(plain, ring_degree=2)
+    g = torch.Generator(device=dev).manual_seed(rot)
+
+    def step(seqs, lens, decode):
+        x = torch.randn((L, sum(lens), 2, H, D), generator=g, device=dev).clamp(-3, 3).to(torch.bfloat16)
+        start = [cache.lengths.get(s, 0) for s in seqs]
+        p = torch.cat([torch.arange(a, a + n, dtype=torch.int32) for a, n in zip(start, lens)]).to(dev)
+        turned = x.clone()
+        for layer in range(L):
+            turned[layer, :, 0] = rope(x[layer, :, 0].contiguous(), p)
+        if four:
+            cache.append(x, seqs, lens, check=True)
+            plain.append(turned, seqs, lens, check=True)
+        else:
+            cache.overflow = plain.overflow = "saturate"
+            cache.append(x, seqs, lens, check=True)
+            plain.append(turned, seqs, lens, check=True)
+        assert torch.equal(cache.pool, plain.pool)
+        q = torch.randn((sum(lens), Hq, D), generator=g, device=dev).to(torch.bfloat16)
+        for layer in range(L):
+            got = att.decode(q, layer, seqs) if decode else att(q, layer, seqs, lens)
+            want = ref.decode(rope(q, p), layer, seqs) if decode else ref(rope(q, p), layer, seqs, lens)
+            assert np.array_equal(bits(got), bits(want))
+    step(["a", "b"], [100, 33], False)
+    step(["b"], [50], False)
+    for _ in range(3):
+        step(["b", "a"], [1, 1], True)
+    cache.free("a")
+    plain.free("a")
+    step(["c", "b"], [1, 17], False)
+    k, v = cache.gather(1, ["b", "c"])
+    assert k.shape == (2, H, cache.lengths["b"], D) and not k[1, :, 1:].any()
+    with pytest.raises(ValueError, match="positions"):
+        cache.append(torch.zeros((L, 400, 2, H, D), dtype=torch.bfloat16, device=dev), ["c"], [400])
+    assert cache.lengths["c"] == 1
+
+
+def test_4_bit_attention_against_float64_end_to_end(dev):
+    """Append, then attend: every row against float64 on what the oracle says the pages hold."""
+    L, H, Hq, D = 1, 2, 6, 64
+    cache = PagedFP4KVCache(L, H, D, 20, page_size=32)
+    att = QuantizedRingAttention(cache, precision="exact")
+    x = torch.randn((L, 150, 2, H, D), device=dev).to(torch.bfloat16)
+    cache.append(x, [0, 1], [100, 50], check=True)
+    q = torch.randn((150, Hq, D), device=dev).to(torch.bfloat16)
+    got = att(q, 0, [0, 1], [100, 50])
+    code, byte = R.encode_block(x[0].float().cpu().numpy().reshape(150, 2, H, 2, 32))
+    held = R.decode_block(code, byte).reshape(150, 2, H, D)
+    for lo, hi in ((0, 100), (100, 150)):
+        n = hi - lo
+        seen = np.arange(n) <= np.arange(n)[:, None]
+        for hq in range(Hq):
+            want, qk, vm = R.attend(q[lo:hi, hq].double().cpu().numpy(), held[lo:hi, 0, hq // 3], held[lo:hi, 1, hq // 3], seen,
+                                    D ** -0.5)
+            check_rows(got[lo:hi, hq].double().cpu().numpy(), want, qk, vm, n, D, D ** -0.5, 2.0 ** -16)
+    one = att.decode(q[:2], 0, [1, 0])
+    assert one.shape == (2, Hq, D) and torch.isfinite(one).all()
+    with pytest.raises(ValueError):
+        cache.append(x, [0], [10])

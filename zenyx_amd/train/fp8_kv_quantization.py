@@ -7,8 +7,12 @@ its behaviour is defined here and in include/zenyx_kv.h).
 * ``PagedFP8KVCache`` -- a paged FP8 KV cache: page pool ``[L, n_pages, 2, H, P, D]``,
   host-side page allocator and block tables, fused quantize+append of new tokens and
   gather+dequant of whole sequences for decode.
-* ``QuantizedRingAttention`` -- ring attention (and decode) over that cache, reading the
-  FP8 pages directly.
+* ``PagedFP4KVCache`` -- the same cache with 4-bit pages (e2m1 codes, a power of two per 32
+  channels): 17/32 byte per element, no scales to keep.
+* ``QuantizedRingAttention`` -- ring attention (and decode) over either cache, reading the
+  pages directly.
+A cache made with ``rope`` (train.rotary.RotaryPositions) takes unrotated keys, rotates them by
+their positions while it stores them, and the attention rotates the queries.
 All arithmetic runs in libzenyx_kv.so on the HIP device.
 """
 from __future__ import annotations
@@ -74,17 +78,17 @@ class PagedFP8KVCache:
     _ERR_WORDS = 64
 
     def __init__(self, num_layers: int, num_kv_heads: int, head_dim: int, num_pages: int,
-                 page_size: int = 16, device: torch.device | None = None, overflow: str = "raise"):
+                 page_size: int = 16, device: torch.device | None = None, overflow: str = "raise", rope=None):
         if overflow not in ("raise", "saturate"):
             raise ValueError('overflow must be "raise" or "saturate"')
+        if rope is not None and rope.head_dim != head_dim:
+            raise ValueError(f"rope is for heads of {rope.head_dim}, the cache has {head_dim}")
         self.device = device or ensure_gpu()
         self.L, self.H, self.D, self.P = num_layers, num_kv_heads, head_dim, page_size
         self.num_pages = num_pages
         self.overflow = overflow
-        self.pool = torch.zeros((num_layers, num_pages, 2, num_kv_heads, page_size, head_dim),
-                                dtype=torch.uint8, device=self.device)
-        self.scales = torch.ones((num_layers, 2, num_kv_heads), dtype=torch.float32, device=self.device)
-        self.has_scales = False
+        self.rope = rope
+        self._make_pool()
         # one error word per append since the last check (a ring; a full ring is checked
         # before it is reused), so saturation is counted per append
         self._err = torch.zeros(self._ERR_WORDS, dtype=torch.int32, device=self.device)
@@ -103,6 +107,35 @@ class PagedFP8KVCache:
         self._len = torch.zeros(16, dtype=torch.int32, device=self.device)
         self._rows_cache: tuple = ((), None)  # (seq_ids, device int64 rows) of the last call
         self._ones_cache: dict = {}  # n -> device int32 ones [n] / arange [n + 1] (one-token steps)
+
+    # ---------------------------------------------------------------- the pages' format
+
+    def _make_pool(self) -> None:
+        self.pool = torch.zeros((self.L, self.num_pages, 2, self.H, self.P, self.D), dtype=torch.uint8,
+                                device=self.device)
+        self.scales = torch.ones((self.L, 2, self.H), dtype=torch.float32, device=self.device)
+        self.has_scales = False
+
+    def _store(self, x, cu, tables, start_pos, dyn: bool, word, single_pass: bool) -> None:
+        saturate = (not dyn) and self.overflow == "saturate"
+        if self.rope is not None:
+            kv.kv_rope_append(x, self.rope.table, cu, tables, self.pool, scales=self.scales, start_pos=start_pos,
+                              interleaved=self.rope.interleaved, static_scales=not dyn, saturate=saturate, err=word)
+        else:
+            kv.kv_quant_append(x, cu, tables, self.pool, scales=self.scales, start_pos=start_pos,
+                               static_scales=not dyn, saturate=saturate, err=word, single_pass=single_pass and dyn)
+
+    def _attend(self, q, layer: int, tables, cu, q_pos0, lens, att, max_q: int) -> torch.Tensor:
+        return kv.ring_attention_fp8(q, cu, q_pos0, self.pool[layer], self.scales[layer], tables, lens,
+                                     ring_degree=att.ring_degree, causal=att.causal, sm_scale=att.sm_scale,
+                                     check=att.check, precision=att.precision, max_q_per_seq=max_q)
+
+    def _attend_step(self, q, layer: int, tables, lens, att) -> torch.Tensor:
+        return kv.paged_attention_decode(q, self.pool[layer], self.scales[layer], tables, lens, sm_scale=att.sm_scale,
+                                         check=att.check)
+
+    def _gather(self, layer: int, tables, lens, out_len: int):
+        return kv.kv_gather_dequant(self.pool[layer], self.scales[layer], tables, lens, out_len)
 
     # ---------------------------------------------------------------- block tables
 
@@ -232,6 +265,11 @@ class PagedFP8KVCache:
         if check or self._n_err == self._ERR_WORDS:
             self.check_errors()  # earlier appends first, so the word read below is this call's own
         start = [self.lengths.get(s, 0) for s in seq_ids]
+        if self.rope is not None:
+            if single_pass:
+                raise ValueError("single_pass is for appends that do not rotate their keys")
+            if any(st + n > self.rope.max_positions for st, n in zip(start, lengths)):
+                raise ValueError(f"a sequence would pass the {self.rope.max_positions} positions of the cache's rope")
         word = self._err[self._n_err:self._n_err + 1]
         had_scales = self.has_scales
         taken: list = []
@@ -242,10 +280,8 @@ class PagedFP8KVCache:
             self._write_entries(entries)
             counts, cu = self._counts(lengths)
             rows = self._rows(seq_ids)
-            kv.kv_quant_append(x.to(self.device), cu, self._tables(seq_ids), self.pool, scales=self.scales,
-                               start_pos=self._len.index_select(0, rows),
-                               static_scales=not dyn, saturate=(not dyn) and self.overflow == "saturate",
-                               err=word, single_pass=single_pass and dyn)
+            self._store(x.to(self.device), cu, self._tables(seq_ids), self._len.index_select(0, rows), dyn, word,
+                        single_pass)
         except BaseException:
             self._release(taken)
             raise
@@ -296,14 +332,49 @@ class PagedFP8KVCache:
         sequence's length are zeros."""
         if out_len is None:
             out_len = max(1, max(self.lengths.get(s, 0) for s in seq_ids))
-        return kv.kv_gather_dequant(self.pool[layer], self.scales[layer], self._tables(seq_ids),
-                                    self._lengths(seq_ids), out_len)
+        return self._gather(layer, self._tables(seq_ids), self._lengths(seq_ids), out_len)
 
     def free(self, seq_id) -> None:
         for p in self.pages.pop(seq_id, []):
             self._free.append(p)
         self.lengths.pop(seq_id, None)
         self._drop_row(seq_id)
+
+
+class PagedFP4KVCache(PagedFP8KVCache):
+    """``PagedFP8KVCache`` with 4-bit pages: every 32 channels of a token, K or V, head are e2m1
+    codes times a power of two of their own, so tokens do not share scales: nothing overflows,
+    and an append needs no earlier one.  A block of 32 that holds a NaN or an infinity is NaN.
+    ``head_dim`` 64, 128 or 256, ``page_size`` a multiple of 16.  ``scales`` is None."""
+
+    def __init__(self, num_layers: int, num_kv_heads: int, head_dim: int, num_pages: int, page_size: int = 16,
+                 device: torch.device | None = None, rope=None):
+        super().__init__(num_layers, num_kv_heads, head_dim, num_pages, page_size=page_size, device=device, rope=rope)
+
+    def _make_pool(self) -> None:
+        self.pool = kv.kv4_pool(self.L, self.num_pages, self.H, self.P, self.D, device=self.device)
+        self.scales = None
+        self.has_scales = True  # none to be computed: every append is like any other
+
+    def append(self, x: torch.Tensor, seq_ids: list, lengths: list[int], check: bool = False) -> None:
+        """``PagedFP8KVCache.append`` without its choices of scales and passes."""
+        super().append(x, seq_ids, lengths, check=check)
+
+    def _store(self, x, cu, tables, start_pos, dyn: bool, word, single_pass: bool) -> None:
+        rope = self.rope
+        kv.kv4_append(x, cu, tables, self.pool, start_pos=start_pos, table=rope.table if rope else None,
+                      interleaved=rope.interleaved if rope else False, err=word)
+
+    def _attend(self, q, layer: int, tables, cu, q_pos0, lens, att, max_q: int) -> torch.Tensor:
+        return kv.paged_attention4_prefill(q, cu, q_pos0, self.pool[layer], tables, lens, causal=att.causal,
+                                           sm_scale=att.sm_scale, max_q_per_seq=max_q, check=att.check,
+                                           precision="exact" if att.precision == "exact" else "bf16")
+
+    def _attend_step(self, q, layer: int, tables, lens, att) -> torch.Tensor:
+        return kv.paged_attention4_decode(q, self.pool[layer], tables, lens, sm_scale=att.sm_scale, check=att.check)
+
+    def _gather(self, layer: int, tables, lens, out_len: int):
+        return kv.kv4_gather_dequant(self.pool[layer], tables, lens, out_len)
 
 
 class QuantizedRingAttention:
@@ -314,7 +385,12 @@ class QuantizedRingAttention:
     queries to it straight from the FP8 pages (no bf16 copy of K/V) and merges by
     log-sum-exp into a running fp32 output, so the result is softmax(sm_scale q K^T) V over
     all cached keys (causal: keys up to each query's position).  On one GPU the steps run
-    in sequence.  ``decode`` is the one-token case (split-K decode kernel)."""
+    in sequence.  ``decode`` is the one-token case (split-K decode kernel).
+
+    With a ``PagedFP4KVCache`` one launch takes all keys, whatever ``ring_degree`` (the union
+    of a ring's shards), and ``precision`` is "exact" or, for the others, weights rounded once
+    to bf16.  A cache with ``rope`` has rotated its keys: the queries are rotated here, by the
+    positions of the tokens they stand for."""
 
     def __init__(self, cache: PagedFP8KVCache, ring_degree: int = 8, causal: bool = True,
                  sm_scale: float | None = None, precision: str = "f16", check: bool = True):
@@ -343,10 +419,11 @@ class QuantizedRingAttention:
             raise ValueError("a sequence has more query rows than cached tokens")
         counts, cu = c._counts(q_lens)
         lens = c._lengths(seq_ids)
-        out = kv.ring_attention_fp8(
-            q.to(c.device).contiguous(), cu, lens - counts, c.pool[layer], c.scales[layer], c._tables(seq_ids), lens,
-            ring_degree=self.ring_degree, causal=self.causal, sm_scale=self.sm_scale, check=self.check,
-            precision=self.precision, max_q_per_seq=max(q_lens, default=0))
+        q, q_pos0 = q.to(c.device).contiguous(), lens - counts
+        if c.rope is not None:
+            shift = torch.repeat_interleave(q_pos0 - cu[:-1], counts, output_size=q.shape[0])
+            q = c.rope(q, shift + torch.arange(q.shape[0], dtype=torch.int32, device=q.device))
+        out = c._attend(q, layer, c._tables(seq_ids), cu, q_pos0, lens, self, max(q_lens, default=0))
         if self.check:
             c.check_errors()  # the appends behind these pages (the check above has synchronised)
         return out
@@ -354,12 +431,13 @@ class QuantizedRingAttention:
     def decode(self, q: torch.Tensor, layer: int, seq_ids: list) -> torch.Tensor:
         """q ``[B, Hq, D]`` bf16, one query token per sequence over all its cached tokens."""
         c = self.cache
-        out = kv.paged_attention_decode(q.to(c.device).contiguous(), c.pool[layer], c.scales[layer],
-                                        c._tables(seq_ids), c._lengths(seq_ids), sm_scale=self.sm_scale,
-                                        check=self.check)
+        q, lens = q.to(c.device).contiguous(), c._lengths(seq_ids)
+        if c.rope is not None:
+            q = c.rope(q, lens - 1)
+        out = c._attend_step(q, layer, c._tables(seq_ids), lens, self)
         if self.check:
             c.check_errors()
         return out
 
 
-__all__ = ["FP8KVQuantizer", "PagedFP8KVCache", "QuantizedRingAttention"]
+__all__ = ["FP8KVQuantizer", "PagedFP4KVCache", "PagedFP8KVCache", "QuantizedRingAttention"]
