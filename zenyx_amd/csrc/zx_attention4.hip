@@ -64,6 +64,31 @@ template <int D> __device__ __forceinline__ att_u32x4 a4_word(const A4Tile<D> &t
   return att_u32x4{a, b, c, d};
 }
 
+// The scores' factor sm_scale log2(e) as a positive number: a negative one turns q's signs, 0
+// makes q zero (then the running maximum is that of the products, and a product masked with
+// -infinity stays that).
+struct A4Scale {
+  float f;
+  uint32_t flip, keep;
+  __device__ __forceinline__ explicit A4Scale(float s)
+      : f(s == 0.0f ? 1.0f : fabsf(s)), flip(s < 0.0f ? 0x80008000u : 0u), keep(s == 0.0f ? 0u : 0xFFFFFFFFu) {}
+  __device__ __forceinline__ att_bf16x8 operand(att_u32x4 w) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = (w[i] ^ flip) & keep;
+    return __builtin_bit_cast(att_bf16x8, w);
+  }
+};
+// A running maximum before the first key.  Finite, so that exp2(-inf - m) is 0 without a case of
+// its own; below every finite score.
+constexpr float A4_NONE = -3.402823466e38f;
+// A running maximum is raised only when a score exceeds it by more than this (log2 units), so
+// weights stay at or below 2^8 and the accumulators are rarely rescaled.
+constexpr float A4_LAZY = 8.0f;
+
+__device__ __forceinline__ float a4_max8(const float (&s)[8]) {
+  return fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
+}
+
 template <int D> struct A4Lds {
   static constexpr int VROW = 2 * D + 32;  // bytes of a token's row of V (D = 128: the rows that a
                                            // transposing read touches lie on distinct banks)
@@ -98,7 +123,7 @@ template <int VROW> __device__ __forceinline__ att_bf16x8 a4_vt(const uint8_t *v
 
 // g.group heads per block at most; the last group of a KV head may have fewer.
 template <int D>
-__global__ void __launch_bounds__(ATT_THREADS, 2)
+__global__ void __launch_bounds__(ATT_THREADS, D == 256 ? 2 : 3)
 paged_decode4_kernel(const uint16_t *__restrict__ q, AttnGeom g, const uint8_t *__restrict__ pool,
                      const int32_t *__restrict__ block_tables, const int32_t *__restrict__ seq_lens,
                      float *__restrict__ part, uint16_t *__restrict__ out, int32_t *err, void *table) {
@@ -118,7 +143,7 @@ paged_decode4_kernel(const uint16_t *__restrict__ q, AttnGeom g, const uint8_t *
   const int64_t page_bytes = 2LL * g.n_kv_heads * tiles * k4_tile_bytes(D);
   const int64_t head_off = (int64_t)h * tiles * k4_tile_bytes(D);
   const int64_t v_off = (int64_t)g.n_kv_heads * tiles * k4_tile_bytes(D);
-  const float qs = g.sm_scale * ATT_LOG2E;
+  const A4Scale qs(g.sm_scale * ATT_LOG2E);
   __shared__ __attribute__((aligned(16))) uint8_t lds[ATT_WAVES][Lds::WAVE];
   __shared__ float sm_m[ATT_WAVES][A4_HEADS], sm_l[ATT_WAVES][A4_HEADS];
   uint8_t *vt = lds[wave];
@@ -143,12 +168,12 @@ paged_decode4_kernel(const uint16_t *__restrict__ q, AttnGeom g, const uint8_t *
         att_u32x4 w = {0u, 0u, 0u, 0u};
         if (n < G)
           w = *reinterpret_cast<const att_u32x4 *>(q + ((int64_t)b * g.n_q_heads + hq0 + n) * D + a4_channel<D>(kg, c));
-        qa[c] = __builtin_bit_cast(att_bf16x8, w);
+        qa[c] = qs.operand(w);
       }
       att_f32x4 o[NT];
 #pragma unroll
       for (int t = 0; t < NT; ++t) o[t] = att_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-      float m = -INFINITY, l = 0.0f;  // of head n; l over this lane's keys
+      float m = A4_NONE, l = 0.0f;  // of head n; l over this lane's keys
 
       // Branch-free as in the 8-bit kernel: a page id is read for a position clamped into the
       // segment, a tile past the end or on a bad page loads through an empty resource.
@@ -183,7 +208,7 @@ paged_decode4_kernel(const uint16_t *__restrict__ q, AttnGeom g, const uint8_t *
           for (int w = 0; w < A4Tile<D>::CW; ++w)
             *reinterpret_cast<att_u32x4 *>(vt + (16 * T + n) * Lds::VROW + 2 * a4_channel<D>(kg, w)) = a4_word<D>(t, w);
         }
-        float s[8];  // of head n with keys 16 T + 4 kg + i, log2 units
+        float s[8];  // q . K of head n with keys 16 T + 4 kg + i
 #pragma unroll
         for (int T = 0; T < 2; ++T) {
           att_f32x4 sc = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -192,15 +217,11 @@ paged_decode4_kernel(const uint16_t *__restrict__ q, AttnGeom g, const uint8_t *
             sc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(att_bf16x8, a4_word<D>(k[T], c)), qa[c], sc,
                                                          0, 0, 0);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) s[4 * T + i] = 4 * kg + i < rows[T] ? sc[i] * qs : -INFINITY;
+          for (int i = 0; i < 4; ++i) s[4 * T + i] = 4 * kg + i < rows[T] ? sc[i] : -INFINITY;
         }
-        float mx = s[0];
-#pragma unroll
-        for (int i = 1; i < 8; ++i) mx = fmaxf(mx, s[i]);
-        const float m_new = fmaxf(m, xrow_max(mx));
-        // the accumulators are rescaled only on the steps where some head's maximum grew
-        if (__builtin_amdgcn_ballot_w64(m_new > m)) {
-          const float alpha = m_new == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - m_new);
+        const float mx = xrow_max(a4_max8(s)) * qs.f;
+        if (__builtin_amdgcn_ballot_w64(mx > m + A4_LAZY)) {
+          const float m_new = fmaxf(m, mx), alpha = __builtin_amdgcn_exp2f(m - m_new);
           m = m_new;
           l *= alpha;
 #pragma unroll
@@ -211,7 +232,7 @@ paged_decode4_kernel(const uint16_t *__restrict__ q, AttnGeom g, const uint8_t *
         float p[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          p[i] = s[i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s[i] - m);  // (a NaN score stays one)
+          p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], qs.f, -m));
           l += p[i];
         }
         att_bf16x8 ph, pl;
@@ -359,11 +380,15 @@ __device__ __forceinline__ bool p4_locate(const Prefill4Args &a, uint32_t at, Pr
   return true;
 }
 
-// A row's running maximum is raised only when a score exceeds it by more than this (log2 units).
-constexpr float P4_LAZY = 8.0f;
+// Tiles of 16 columns a block can hold: what leaves two waves per SIMD.
+__host__ __device__ constexpr int a4_most_tiles(int D) { return D == 64 ? 4 : D == 128 ? 3 : 1; }
+// Blocks per CU (waves per SIMD), by the registers of the tiles' accumulators and queries.
+__host__ __device__ constexpr int a4_per_cu(int D, int CT) {
+  return D * CT <= 128 ? 4 : D * CT <= 256 && D < 256 ? 3 : 2;
+}
 
 template <int D, int CT, bool EXACT>
-__global__ void __launch_bounds__(ATT_THREADS, CT * D > 256 ? 1 : 2) paged_prefill4_kernel(Prefill4Args a) {
+__global__ void __launch_bounds__(ATT_THREADS, a4_per_cu(D, CT)) paged_prefill4_kernel(Prefill4Args a) {
   using Lds = A4Lds<D>;
   constexpr int NC = D / 32, NT = D / 16;
   Prefill4Tile tl;
@@ -380,7 +405,7 @@ __global__ void __launch_bounds__(ATT_THREADS, CT * D > 256 ? 1 : 2) paged_prefi
   const int64_t page_bytes = 2LL * a.n_kv_heads * tiles * k4_tile_bytes(D);
   const int64_t head_off = (int64_t)tl.h * tiles * k4_tile_bytes(D);
   const int64_t v_off = (int64_t)a.n_kv_heads * tiles * k4_tile_bytes(D);
-  const float qs = a.sm_log2e;
+  const A4Scale qs(a.sm_log2e);
   __shared__ __attribute__((aligned(16))) uint8_t lds[ATT_WAVES][Lds::WAVE];
   __shared__ float sm_m[ATT_WAVES][A4_HEADS], sm_l[ATT_WAVES][A4_HEADS];
   uint8_t *vt = lds[wave];
@@ -401,7 +426,7 @@ __global__ void __launch_bounds__(ATT_THREADS, CT * D > 256 ? 1 : 2) paged_prefi
     for (int k = 0; k < NC; ++k) {
       att_u32x4 w = {0u, 0u, 0u, 0u};
       if (live) w = *reinterpret_cast<const att_u32x4 *>(src + a4_channel<D>(kg, k));
-      qa[ct][k] = __builtin_bit_cast(att_bf16x8, w);
+      qa[ct][k] = qs.operand(w);
     }
   }
   // the lowest limit of the tile's rows (row 0's): steps below it need no mask
@@ -414,7 +439,7 @@ __global__ void __launch_bounds__(ATT_THREADS, CT * D > 256 ? 1 : 2) paged_prefi
 #pragma unroll
     for (int t = 0; t < NT; ++t) o[ct][t] = att_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     ol[ct] = att_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    m[ct] = -INFINITY;
+    m[ct] = A4_NONE;
     l[ct] = 0.0f;
   }
   const att_bf16x8 ones = __builtin_bit_cast(att_bf16x8, att_u32x4{0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u});
@@ -436,7 +461,8 @@ __global__ void __launch_bounds__(ATT_THREADS, CT * D > 256 ? 1 : 2) paged_prefi
     a4_load<D>(__builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(src + (ok ? v_off : 0)), (short)0, nrec,
                                                  0x00020000), lane, v);
   };
-  auto compute_step = [&](uint32_t t0, const A4Tile<D> (&k)[2], const A4Tile<D> (&v)[2], const int (&rows)[2]) {
+  // V rows into LDS, then S^T of both tiles
+  auto scores = [&](uint32_t t0, const A4Tile<D> (&k)[2], const A4Tile<D> (&v)[2], const int (&rows)[2], float (&s)[CT][8]) {
 #pragma unroll
     for (int T = 0; T < 2; ++T) {
       A4Tile<D> t = v[T];
@@ -450,7 +476,7 @@ __global__ void __launch_bounds__(ATT_THREADS, CT * D > 256 ? 1 : 2) paged_prefi
       for (int w = 0; w < A4Tile<D>::CW; ++w)
         *reinterpret_cast<att_u32x4 *>(vt + (16 * T + n) * Lds::VROW + 2 * a4_channel<D>(kg, w)) = a4_word<D>(t, w);
     }
-    float s[CT][8];
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int T = 0; T < 2; ++T) {
       att_f32x4 sc[CT];
@@ -466,7 +492,7 @@ __global__ void __launch_bounds__(ATT_THREADS, CT * D > 256 ? 1 : 2) paged_prefi
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[ct][4 * T + i] = sc[ct][i] * qs;
+        for (int i = 0; i < 4; ++i) s[ct][4 * T + i] = sc[ct][i];
     }
     if (rows[0] < K4_TOK || rows[1] < K4_TOK || t0 + A4_STEP > lim_all) {  // uniform
 #pragma unroll
@@ -479,16 +505,20 @@ __global__ void __launch_bounds__(ATT_THREADS, CT * D > 256 ? 1 : 2) paged_prefi
             if (j >= rows[T] || t0 + 16 * T + j >= lim[ct]) s[ct][4 * T + i] = -INFINITY;
           }
     }
-    att_bf16x8 ph[CT], pl[CT];
+  };
+  // softmax and O^T += V^T P^T
+  auto weigh = [&](const float (&s)[CT][8]) {
+    float mx[CT];
+    bool grew = false;
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
-      float mx = s[ct][0];
+      mx[ct] = xrow_max(a4_max8(s[ct])) * qs.f;
+      grew = grew || mx[ct] > m[ct] + A4_LAZY;
+    }
+    if (__builtin_amdgcn_ballot_w64(grew)) {
 #pragma unroll
-      for (int i = 1; i < 8; ++i) mx = fmaxf(mx, s[ct][i]);
-      mx = xrow_max(mx);
-      if (__builtin_amdgcn_ballot_w64(mx > m[ct] + P4_LAZY)) {  // (m = -inf: any score raises it)
-        const float m_new = fmaxf(m[ct], mx);
-        const float alpha = m_new == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[ct] - m_new);
+      for (int ct = 0; ct < CT; ++ct) {
+        const float m_new = fmaxf(m[ct], mx[ct]), alpha = __builtin_amdgcn_exp2f(m[ct] - m_new);
         m[ct] = m_new;
         l[ct] *= alpha;
 #pragma unroll
@@ -498,9 +528,13 @@ __global__ void __launch_bounds__(ATT_THREADS, CT * D > 256 ? 1 : 2) paged_prefi
 #pragma unroll
           for (int i = 0; i < 4; ++i) o[ct][t][i] *= alpha;
       }
+    }
+    att_bf16x8 ph[CT], pl[CT];
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
       float p[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) p[i] = s[ct][i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s[ct][i] - m[ct]);
+      for (int i = 0; i < 8; ++i) p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[ct][i], qs.f, -m[ct]));
       if constexpr (EXACT) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) l[ct] += p[i];
@@ -511,6 +545,7 @@ __global__ void __launch_bounds__(ATT_THREADS, CT * D > 256 ? 1 : 2) paged_prefi
         ol[ct] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, ph[ct], ol[ct], 0, 0, 0);
       }
     }
+    __builtin_amdgcn_sched_barrier(0);
     a4_wave_sync();
 #pragma unroll
     for (int jt = 0; jt < NT; ++jt) {
@@ -526,31 +561,31 @@ __global__ void __launch_bounds__(ATT_THREADS, CT * D > 256 ? 1 : 2) paged_prefi
 
   constexpr uint32_t stride = ATT_WAVES * A4_STEP;
   uint32_t t0 = tl.t_begin + (uint32_t)wave * A4_STEP;
-  if (t0 < t_end) {  // (a wave without a step leaves its m at -inf)
-    A4Tile<D> k0[2], v0[2], k1[2], v1[2];
-    int r0[2], r1[2];
-    int32_t p0[2], p1[2];
-    auto pages_of_step = [&](uint32_t ts, int32_t (&p)[2]) {
-      p[0] = tile_page(ts);
-      p[1] = tile_page(ts + K4_TOK);
+  if (t0 < t_end) {
+    // the next step's loads go out once this one's codes are converted (a second set of
+    // registers for them would cost the second wave per SIMD), its page ids one step before
+    A4Tile<D> k[2], v[2];
+    int rows[2];
+    int32_t page[2];
+    auto pages_of_step = [&](uint32_t ts) {
+      page[0] = tile_page(ts);
+      page[1] = tile_page(ts + K4_TOK);
     };
-    auto load_step = [&](uint32_t ts, const int32_t (&p)[2], A4Tile<D> (&k)[2], A4Tile<D> (&v)[2], int (&rows)[2]) {
-      load_tile(ts, p[0], k[0], v[0], rows[0]);
-      load_tile(ts + K4_TOK, p[1], k[1], v[1], rows[1]);
+    auto load_step = [&](uint32_t ts) {
+      load_tile(ts, page[0], k[0], v[0], rows[0]);
+      load_tile(ts + K4_TOK, page[1], k[1], v[1], rows[1]);
     };
-    pages_of_step(t0, p0);
-    load_step(t0, p0, k0, v0, r0);
-    pages_of_step(t0 + stride, p1);
+    pages_of_step(t0);
+    load_step(t0);
+    pages_of_step(t0 + stride);
     while (t0 < t_end) {
-      load_step(t0 + stride, p1, k1, v1, r1);
-      pages_of_step(t0 + 2 * stride, p0);
-      compute_step(t0, k0, v0, r0);
+      float s[CT][8];
+      scores(t0, k, v, rows, s);
+      __builtin_amdgcn_sched_barrier(0);
       t0 += stride;
-      if (t0 >= t_end) break;
-      load_step(t0 + stride, p0, k0, v0, r0);
-      pages_of_step(t0 + 2 * stride, p1);
-      compute_step(t0, k1, v1, r1);
-      t0 += stride;
+      load_step(t0);
+      pages_of_step(t0 + stride);
+      weigh(s);
     }
   }
 
@@ -639,7 +674,7 @@ static int32_t a4_groups(int32_t grp) { return (int32_t)ceil_div(grp, A4_HEADS);
 static AttnRuns a4_plan(int32_t n_seqs, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim, int32_t max_blocks,
                         int32_t page_size) {
   const int64_t groups = (int64_t)n_kv_heads * a4_groups(n_q_heads / n_kv_heads);
-  return att_runs(n_seqs, groups, 2LL * num_cus(), ATT_WAVES * A4_STEP, max_blocks, page_size);
+  return att_runs(n_seqs, groups, (head_dim == 256 ? 2LL : 3LL) * num_cus(), ATT_WAVES * A4_STEP, max_blocks, page_size);
 }
 
 extern "C" size_t zx_paged_attention4_decode_workspace_bytes(int32_t n_seqs, int32_t n_q_heads, int32_t n_kv_heads,
@@ -690,10 +725,10 @@ extern "C" int zx_paged_attention4_decode(const uint16_t *q, int32_t n_q_heads, 
   return att_combine(part, g, nullptr, seq_lens, out, table, st);
 }
 
-// Column tiles per block, by the columns that a sequence can have at most; with head_dim 256 four
-// would not fit the registers.
+// Column tiles per block, by the columns that a sequence can have at most.
 static int a4_column_tiles(int64_t columns, int32_t head_dim) {
-  return columns <= 16 ? 1 : columns <= 32 || head_dim == 256 ? 2 : 4;
+  const int most = a4_most_tiles(head_dim);
+  return columns <= 16 || most == 1 ? 1 : columns <= 32 ? 2 : most;
 }
 
 struct Prefill4Plan {
@@ -713,7 +748,7 @@ static Prefill4Plan p4_plan(int32_t n_q_heads, int32_t n_kv_heads, int32_t head_
   p.items = p.n_rt * p.n_group * n_seqs;
   // parts of a tile where the tiles do not fill the chip; none shorter than 256 keys
   const int64_t units = ceil_div(std::min((int64_t)max_blocks * page_size, (int64_t)INT32_MAX), ATT_WAVES * A4_STEP);
-  const int64_t resident = (p.ct * head_dim > 256 ? 1LL : 2LL) * num_cus();
+  const int64_t resident = (int64_t)a4_per_cu(head_dim, p.ct) * num_cus();
   p.n_split = std::max<int64_t>(1, std::min(units / 2, resident / std::max<int64_t>(1, p.items)));
   return p;
 }
@@ -800,14 +835,16 @@ extern "C" int zx_paged_attention4_prefill(const uint16_t *q, int64_t n_q, const
   const unsigned items = (unsigned)p.items, grid = items * (unsigned)a.n_split;
   const hipStream_t st = as_stream(stream);
   const bool exact = flags & ZX_PREFILL_EXACT_P;
-#define ZX_P4(D)                                                      \
-  p.ct == 1   ? p4_launch<D, 1>(a, exact, grid, items, st)            \
-  : p.ct == 2 ? p4_launch<D, 2>(a, exact, grid, items, st)            \
-              : p4_launch<D, D == 256 ? 2 : 4>(a, exact, grid, items, st)
+  constexpr int M64 = a4_most_tiles(64), M128 = a4_most_tiles(128);
   switch (head_dim) {
-    case 64: return ZX_P4(64);
-    case 128: return ZX_P4(128);
-    default: return ZX_P4(256);
+    case 64:
+      return p.ct == 1   ? p4_launch<64, 1>(a, exact, grid, items, st)
+             : p.ct == 2 ? p4_launch<64, 2>(a, exact, grid, items, st)
+                         : p4_launch<64, M64>(a, exact, grid, items, st);
+    case 128:
+      return p.ct == 1   ? p4_launch<128, 1>(a, exact, grid, items, st)
+             : p.ct == 2 ? p4_launch<128, 2>(a, exact, grid, items, st)
+                         : p4_launch<128, M128>(a, exact, grid, items, st);
+    default: return p4_launch<256, 1>(a, exact, grid, items, st);
   }
-#undef ZX_P4
 }
