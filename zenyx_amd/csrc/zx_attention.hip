@@ -686,75 +686,21 @@ paged_decode_mfma_kernel(const uint16_t *__restrict__ q, AttnGeom g, const uint8
   if (e && err) atomicOr(err, e);
 }
 
-// Pass 2 (scales NULL: scale_v = 1): out[b][hq][:] = scale_v * sum_s 2^(m_s - M) acc_s / sum_s 2^(m_s - M) l_s over
-// the segments of sequence b.  A wave owns 64 channels of one row; its lanes hold the
-// maxima and sums of 64 segments at a time, whose weights reach the channels by readlane,
-// so there is no LDS and no barrier, and several segments' values are loaded
-// before the first is used (1 x 2,048 positions, both passes: 20.4 -> 9.5 us, this one's
-// share 4.0 -> 3.0; before, a block-wide table and one load at a time).
-constexpr int CB_U = 8;  // segments whose values are loaded together
+// Pass 2 (scales NULL: scale_v = 1): out[b][hq][:] = scale_v * sum_s 2^(m_s - M) acc_s / sum_s
+// 2^(m_s - M) l_s over the segments of sequence b.
 __global__ void __launch_bounds__(256)
 paged_decode_combine_kernel(const float *__restrict__ part, AttnGeom g, const float *__restrict__ scales,
                             const int32_t *__restrict__ seq_lens, uint16_t *__restrict__ out, void *table) {
   const int D = g.head_dim;
-  const int lane = threadIdx.x & 63;
   const int64_t row = blockIdx.x;  // b * Hq + hq
-  const int d = threadIdx.x;
   const int b = (int)(row / g.n_q_heads);
   const int h = (int)(row % g.n_q_heads) / (g.n_q_heads / g.n_kv_heads);
-  // the sequence's first run, and how many hold a part of it
-  int32_t x0 = 0, n_live = 0;
-  if (g.n_seqs <= 64) {
-    const AttnLanes l(g, lane < g.n_seqs ? seq_lens[lane] : 0);
-    const uint32_t nb = __builtin_amdgcn_readlane(l.n, b);
-    if (l.whole) {
-      n_live = nb != 0;
-    } else if (nb) {
-      const uint32_t last = __builtin_amdgcn_readlane(l.incl, b) - 1;
-      x0 = (int32_t)l.deal.run_of(last + 1 - nb);
-      n_live = (int32_t)l.deal.run_of(last) - x0 + 1;
-    }
-  } else {
-    const AttnTable t(table, g.n_seqs);
-    x0 = t.x0[b];
-    n_live = t.n_live[b];
-  }
+  int32_t x0, n_live;
+  att_live(g, seq_lens, table, b, x0, n_live);
   if (n_live == 1) return;  // the sequence was one segment: its block has written the row
-  const float sv = scales ? scales[g.n_kv_heads + h] : 1.0f;
   const int64_t hq = row % g.n_q_heads;
   const float *pp = part + (hq * ((int64_t)g.n_run + g.n_seqs) + x0 + b) * (2 + D);
-  float M = -INFINITY, L = 0.0f, A = 0.0f;
-  for (int base = 0; base < n_live; base += 64) {
-    const int cnt = min(64, n_live - base);
-    const float *p0 = pp + (int64_t)base * (2 + D);
-    const float ms = lane < cnt ? p0[lane * (2 + D)] : -INFINITY;
-    const float ls = lane < cnt ? p0[lane * (2 + D) + 1] : 0.0f;
-    float v[CB_U];
-#pragma unroll
-    for (int u = 0; u < CB_U; ++u) v[u] = p0[min(u, cnt - 1) * (2 + D) + 2 + d];
-    const float Mn = fmaxf(M, xrow_max(row16_max(ms)));
-    const float alpha = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M - Mn);
-    const float w = Mn == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ms - Mn);
-    M = Mn;
-    L = L * alpha + rows_sum(group_sum<16>(w * ls));
-    A *= alpha;
-    for (int s = 0; s < cnt; s += CB_U) {
-      float nx[CB_U];
-      if (s + CB_U < cnt) {
-#pragma unroll
-        for (int u = 0; u < CB_U; ++u) nx[u] = p0[min(s + CB_U + u, cnt - 1) * (2 + D) + 2 + d];
-      }
-#pragma unroll
-      for (int u = 0; u < CB_U; ++u)
-        if (s + u < cnt)
-          A += __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), s + u)) * v[u];
-#pragma unroll
-      for (int u = 0; u < CB_U; ++u) v[u] = nx[u];
-    }
-  }
-  // a sequence without positions (L = 0) gives zeros
-  const float o = L == 0.0f ? 0.0f : A / L * sv;
-  out[row * D + d] = (uint16_t)(pack_bf16(o, 0.0f) & 0xFFFFu);
+  out[row * D + threadIdx.x] = att_combine_row(pp, 2 + D, n_live, threadIdx.x, scales ? scales[g.n_kv_heads + h] : 1.0f);
 }
 
 int att_make_table(const AttnGeom &g, const int32_t *seq_lens, void *table, hipStream_t st) {
