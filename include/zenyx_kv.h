@@ -489,8 +489,10 @@ int zx_rope(const void *x, int dtype, int64_t n_rows, int32_t n_heads, int32_t h
  * ZX_APPEND_SATURATE, ZX_ROPE_INTERLEAVED.  A token at or beyond n_pos is not stored and sets
  * ZX_KERR_POS_RANGE; dynamic scales are taken over the tokens that have a position (rows
  * outside [cu_seqlens[0], cu_seqlens[n_seqs]) have none).  workspace:
- * zx_kv_rope_append_workspace_bytes() device bytes, 16-byte aligned. */
-size_t zx_kv_rope_append_workspace_bytes(int32_t n_layers, int64_t n_tok, int32_t n_heads, int32_t head_dim);
+ * zx_kv_rope_append_workspace_bytes() device bytes (0 for a small call with static scales),
+ * 16-byte aligned. */
+size_t zx_kv_rope_append_workspace_bytes(int32_t n_layers, int64_t n_tok, int32_t n_heads, int32_t head_dim,
+                                         int32_t flags);
 int zx_kv_rope_append(const uint16_t *x, int64_t x_layer_stride, int32_t n_layers, int64_t n_tok, int32_t n_heads,
                       int32_t head_dim, const float *table, int64_t n_pos, int32_t rot_dim,
                       const int32_t *cu_seqlens, const int32_t *start_pos, int32_t n_seqs,
@@ -510,8 +512,8 @@ int zx_kv_rope_append(const uint16_t *x, int64_t x_layer_stride, int32_t n_layer
 /* Paged append of x[L][n_tok][2][H][D] bf16 (arguments as zx_kv_quant_append); with a table
  * (may be NULL) the keys are rotated first, as zx_rope does.  flags: ZX_ROPE_INTERLEAVED.
  * Tokens at bad pages or positions are not stored and set their bits in *err.  workspace:
- * zx_kv4_append_workspace_bytes() device bytes, 16-byte aligned. */
-size_t zx_kv4_append_workspace_bytes(int64_t n_tok);
+ * zx_kv4_append_workspace_bytes() device bytes (0 for a small call), 16-byte aligned. */
+size_t zx_kv4_append_workspace_bytes(int32_t n_layers, int64_t n_tok, int32_t n_heads);
 int zx_kv4_append(const uint16_t *x, int64_t x_layer_stride, int32_t n_layers, int64_t n_tok, int32_t n_heads,
                   int32_t head_dim, const float *table, int64_t n_pos, int32_t rot_dim, const int32_t *cu_seqlens,
                   const int32_t *start_pos, int32_t n_seqs, const int32_t *block_tables, int32_t max_blocks,

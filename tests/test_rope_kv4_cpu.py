@@ -59,7 +59,8 @@ def append_args(four, **kw):
     (dict(page=0), N.ZX_ERR_INVALID), (dict(n_pages=0), N.ZX_ERR_INVALID), (dict(n_pages=1 << 31), N.ZX_ERR_INVALID),
     (dict(H=0), N.ZX_ERR_INVALID), (dict(L=0), N.ZX_ERR_INVALID), (dict(L=2, xl=8), N.ZX_ERR_INVALID),
     (dict(L=2, pl=16), N.ZX_ERR_INVALID), (dict(rot=40), N.ZX_ERR_UNSUPPORTED), (dict(rot=128), N.ZX_ERR_INVALID),
-    (dict(n_pos=0), N.ZX_ERR_INVALID), (dict(ws=None), N.ZX_ERR_WORKSPACE), (dict(wsb=8), N.ZX_ERR_WORKSPACE)])
+    (dict(n_pos=0), N.ZX_ERR_INVALID), (dict(ws=P + 8), N.ZX_ERR_INVALID),
+    (dict(T=50000, xl=1 << 30, ws=None), N.ZX_ERR_WORKSPACE), (dict(T=50000, xl=1 << 30, wsb=8), N.ZX_ERR_WORKSPACE)])
 def test_append_refusals(lib, four, kw, rc):
     f = lib.zx_kv4_append if four else lib.zx_kv_rope_append
     assert f(*append_args(four, **kw)) == rc
@@ -131,8 +132,12 @@ def test_gather_refusals(lib):
 
 
 def test_workspace_queries(lib):
-    assert lib.zx_kv4_append_workspace_bytes(0) == 0 and lib.zx_kv4_append_workspace_bytes(33) >= 33 * 8
-    assert lib.zx_kv_rope_append_workspace_bytes(1, -5, 8, 128) == 0
+    assert lib.zx_kv4_append_workspace_bytes(1, 0, 8) == 0 and lib.zx_kv4_append_workspace_bytes(1, 33, 8) == 0
+    assert lib.zx_kv4_append_workspace_bytes(4, 50000, 8) >= 50000 * 8
+    assert lib.zx_kv_rope_append_workspace_bytes(1, -5, 8, 128, 0) == 0
+    assert lib.zx_kv_rope_append_workspace_bytes(1, 64, 8, 128, 1) == 0  # static scales, few tokens: none
+    assert lib.zx_kv_rope_append_workspace_bytes(1, 64, 8, 128, 0) >= 16 * 4
+    assert lib.zx_kv_rope_append_workspace_bytes(1, 50000, 8, 128, 1) >= 50000 * 8
     assert lib.zx_paged_attention4_decode_workspace_bytes(4, 32, 8, 96, 10, 16) == 0
     assert lib.zx_paged_attention4_decode_workspace_bytes(4, 32, 8, 128, 10, 24) == 0
     assert lib.zx_paged_attention4_prefill_workspace_bytes(32, 8, 128, 16, 1024, 1, 4) > 0

@@ -88,10 +88,10 @@ SIGNATURES = {
     "zx_ring_shard_bounds": (_INT, [_P, _I32, _I32, _I32, _P, _P, _P]),
     "zx_rope_table": (_INT, [_P, _I32, _I64, ctypes.c_double, _P, _P]),
     "zx_rope": (_INT, [_P, _INT, _I64, _I32, _I32, _I64, _I64, _P, _I64, _I32, _P, _I32, _P, _I64, _I64, _P, _P]),
-    "zx_kv_rope_append_workspace_bytes": (_SZ, [_I32, _I64, _I32, _I32]),
+    "zx_kv_rope_append_workspace_bytes": (_SZ, [_I32, _I64, _I32, _I32, _I32]),
     "zx_kv_rope_append": (_INT, [_P, _I64, _I32, _I64, _I32, _I32, _P, _I64, _I32, _P, _P, _I32, _P, _I32, _I32, _P,
                                  _I64, _I64, _P, _I32, _P, _P, _SZ, _P]),
-    "zx_kv4_append_workspace_bytes": (_SZ, [_I64]),
+    "zx_kv4_append_workspace_bytes": (_SZ, [_I32, _I64, _I32]),
     "zx_kv4_append": (_INT, [_P, _I64, _I32, _I64, _I32, _I32, _P, _I64, _I32, _P, _P, _I32, _P, _I32, _I32, _P,
                              _I64, _I64, _I32, _P, _P, _SZ, _P]),
     "zx_kv4_gather_dequant": (_INT, [_P, _I64, _I32, _I32, _I32, _P, _I32, _P, _I32, _I32, _P, _P, _P, _P]),

@@ -223,8 +223,13 @@ constexpr int64_t K4_LOCATE_WPC = 16;
 
 using namespace zx;
 
-extern "C" size_t zx_kv4_append_workspace_bytes(int64_t n_tok) {
-  return n_tok > 0 ? align256((size_t)n_tok * sizeof(K4Place)) : 0;
+static bool kv4_locates(int32_t n_layers, int64_t n_tok, int32_t n_heads) {
+  return ceil_div(n_tok, 16) * 2 * n_heads * n_layers <= K4_LOCATE_WPC * num_cus();
+}
+
+extern "C" size_t zx_kv4_append_workspace_bytes(int32_t n_layers, int64_t n_tok, int32_t n_heads) {
+  if (n_layers <= 0 || n_tok <= 0 || n_heads <= 0 || kv4_locates(n_layers, n_tok, n_heads)) return 0;
+  return align256((size_t)n_tok * sizeof(K4Place));
 }
 
 template <int D>
@@ -267,8 +272,9 @@ extern "C" int zx_kv4_append(const uint16_t *x, int64_t x_layer_stride, int32_t 
   ZX_REQUIRE(n_layers == 1 || pool_layer_stride >= n_pages * page_bytes,
              "kv4_append: pool layer stride smaller than a layer's pages");
   if (n_tok == 0) return ZX_OK;
-  const size_t need = zx_kv4_append_workspace_bytes(n_tok);
-  if (!workspace || workspace_bytes < need)
+  const size_t need = zx_kv4_append_workspace_bytes(n_layers, n_tok, n_heads);
+  ZX_REQUIRE(aligned16(workspace), "kv4_append: workspace must be 16-byte aligned");
+  if (need && (!workspace || workspace_bytes < need))
     return fail(ZX_ERR_WORKSPACE, "kv4_append: workspace %zu < %zu bytes", workspace_bytes, need);
   K4Append a;
   a.x = x;
@@ -287,7 +293,7 @@ extern "C" int zx_kv4_append(const uint16_t *x, int64_t x_layer_stride, int32_t 
   const int64_t blocks = ceil_div(a.n_grp, K4_WAVES);
   if (blocks >= (1LL << 31)) return fail(ZX_ERR_UNSUPPORTED, "kv4_append: too many rows");
   const hipStream_t st = as_stream(stream);
-  const bool locate = a.n_grp * n_layers <= K4_LOCATE_WPC * num_cus();
+  const bool locate = kv4_locates(n_layers, n_tok, n_heads);
   if (!locate) {
     kv4_places_kernel<<<(unsigned)ceil_div(n_tok, 256), 256, 0, st>>>(a.tg, a.limit, n_tok,
                                                                       static_cast<K4Place *>(workspace), err);

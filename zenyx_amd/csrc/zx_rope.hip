@@ -382,12 +382,21 @@ extern "C" int zx_rope(const void *x, int dtype, int64_t n_rows, int32_t n_heads
   return check_launch("rope");
 }
 
-extern "C" size_t zx_kv_rope_append_workspace_bytes(int32_t n_layers, int64_t n_tok, int32_t n_heads,
-                                                    int32_t head_dim) {
-  (void)head_dim;
-  if (n_layers <= 0 || n_tok <= 0 || n_heads <= 0) return 0;
+// Rows that a block of the append takes at a time.
+static int32_t ra_rows_per_block(int32_t n_heads, int32_t head_dim) {
+  const int32_t units = n_heads * head_dim / 8;
+  return units >= 256 ? 1 : 256 / units;
+}
+static bool ra_locates(int32_t n_layers, int64_t n_tok, int32_t n_heads, int32_t head_dim) {
+  return ceil_div(n_tok, (int64_t)RA_U * ra_rows_per_block(n_heads, head_dim)) * n_layers <= RA_LOCATE_BPC * num_cus();
+}
+
+extern "C" size_t zx_kv_rope_append_workspace_bytes(int32_t n_layers, int64_t n_tok, int32_t n_heads, int32_t head_dim,
+                                                    int32_t flags) {
+  if (n_layers <= 0 || n_tok <= 0 || n_heads <= 0 || head_dim < 8) return 0;
   const int64_t gx = std::max<int64_t>(1, ceil_div((int64_t)num_cus() * RA_BPC, n_layers));
-  return align256((size_t)n_tok * sizeof(TokPlace)) + align256((size_t)gx * n_layers * 2 * n_heads * sizeof(uint32_t));
+  return (ra_locates(n_layers, n_tok, n_heads, head_dim) ? 0 : align256((size_t)n_tok * sizeof(TokPlace))) +
+         (flags & ZX_APPEND_STATIC_SCALES ? 0 : align256((size_t)gx * n_layers * 2 * n_heads * sizeof(uint32_t)));
 }
 
 extern "C" int zx_kv_rope_append(const uint16_t *x, int64_t x_layer_stride, int32_t n_layers, int64_t n_tok,
@@ -423,12 +432,13 @@ extern "C" int zx_kv_rope_append(const uint16_t *x, int64_t x_layer_stride, int3
   const hipStream_t st = as_stream(stream);
   if (n_tok == 0)  // no token: the scales of an empty batch
     return dynamic ? zx_kv_scales(x, 0, n_layers, 0, n_heads, head_dim, scales, stream) : ZX_OK;
-  const size_t need = zx_kv_rope_append_workspace_bytes(n_layers, n_tok, n_heads, head_dim);
-  if (!workspace || workspace_bytes < need)
+  const size_t need = zx_kv_rope_append_workspace_bytes(n_layers, n_tok, n_heads, head_dim, flags);
+  ZX_REQUIRE(aligned16(workspace), "kv_rope_append: workspace must be 16-byte aligned");
+  if (need && (!workspace || workspace_bytes < need))
     return fail(ZX_ERR_WORKSPACE, "kv_rope_append: workspace %zu < %zu bytes", workspace_bytes, need);
   RaGeom g;
   g.n_unit = (int32_t)(row / 16);
-  g.rpb = g.n_unit >= 256 ? 1 : 256 / g.n_unit;
+  g.rpb = ra_rows_per_block(n_heads, head_dim);
   g.upd = head_dim / 16;
   g.n_slabs = 2 * n_heads;
   g.head_dim = head_dim;
@@ -439,9 +449,10 @@ extern "C" int zx_kv_rope_append(const uint16_t *x, int64_t x_layer_stride, int3
   const TokGeom tg = {cu_seqlens, start_pos, block_tables, n_seqs, max_blocks, page_size, head_dim, n_pages, page_bytes};
   const int64_t limit = std::min((int64_t)max_blocks * page_size, n_pos);
   const int64_t tiles = ceil_div(n_tok, (int64_t)RA_U * g.rpb);
-  const bool locate = tiles * n_layers <= RA_LOCATE_BPC * num_cus();
+  const bool locate = ra_locates(n_layers, n_tok, n_heads, head_dim);
   TokPlace *places = static_cast<TokPlace *>(workspace);
-  uint32_t *part = reinterpret_cast<uint32_t *>(static_cast<char *>(workspace) + align256((size_t)n_tok * sizeof(TokPlace)));
+  uint32_t *part = reinterpret_cast<uint32_t *>(static_cast<char *>(workspace) +
+                                                (locate ? 0 : align256((size_t)n_tok * sizeof(TokPlace))));
   if (!locate) {
     ra_places_kernel<<<(unsigned)ceil_div(n_tok, 256), 256, 0, st>>>(tg, limit, n_tok, places, err);
     if ((rc = check_launch("ra_places"))) return rc;

@@ -15,6 +15,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 
 import torch
 
@@ -851,17 +852,33 @@ def tier_copy_runs(dst: torch.Tensor, src: torch.Tensor, dst_offs, src_offs, run
 _same_device = contextlib.nullcontext()
 
 
-def _on(device: torch.device):
-    """Makes ``device`` current for a launch (nothing to do where it already is)."""
-    return _same_device if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+def _on(index: int):
+    """Makes device ``index`` current for a launch (nothing to do where it already is)."""
+    return _same_device if torch._C._cuda_getDevice() == index else torch.cuda.device(index)
 
 
-def _all_on(device: torch.device, **tensors) -> None:
+def _fits(t: torch.Tensor, index: int) -> bool:
+    return t.get_device() == index and t.is_contiguous() and not t.data_ptr() & 15
+
+
+def _all_on(index: int, **tensors) -> None:
+    """Raises for a tensor that is not contiguous, 16-byte aligned and on device ``index``."""
     for name, t in tensors.items():
-        if t is not None:
+        if t is not None and not _fits(t, index):
             N.require_device(t, name)
-            if t.device != device:
-                raise ValueError(f"{name} must be on {device}, got {t.device}")
+            raise ValueError(f"{name} must be on cuda:{index}, got {t.device}")
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(query: str, index: int, *sizes) -> int:
+    """A workspace query's answer for these sizes (the same for a device whenever it is asked)."""
+    return getattr(N.load(), query)(*sizes)
+
+
+def _workspace_for(query: str, index: int, *sizes):
+    """Workspace (None where the call needs none) and its bytes."""
+    nb = _workspace_bytes(query, index, *sizes)
+    return (torch.empty(nb, dtype=torch.uint8, device=torch.device("cuda", index)), nb) if nb else (None, 0)
 
 
 def _rope_table_of(table: torch.Tensor, D: int) -> tuple[int, int]:
@@ -882,18 +899,21 @@ def rope_table(inv_freq: torch.Tensor, n_pos: int, scale: float = 1.0) -> torch.
         raise ValueError("inv_freq must be float64 [rot_dim / 2]")
     N.require_device(inv_freq, "inv_freq")
     out = torch.empty((int(n_pos), 2 * inv_freq.numel()), dtype=torch.float32, device=inv_freq.device)
-    with _on(out.device):
+    with _on(out.get_device()):
         N.check(N.load().zx_rope_table(N.ptr(inv_freq), out.shape[1], out.shape[0], float(scale), N.ptr(out),
                                        N.stream_ptr(out.device)), "rope_table")
     return out
 
 
-def _rows_of(t: torch.Tensor, name: str) -> None:
+def _rows_of(t: torch.Tensor, name: str) -> tuple[int, int]:
+    """The row and head strides of ``[n, H, D]`` rows that the kernel can take."""
     vec = 16 // t.element_size()
+    row, head, channel = t.stride()
     if not t.is_cuda:
         raise ValueError(f"{name} must be a HIP device tensor, got {t.device}")
-    if t.stride(2) != 1 or t.stride(0) % vec or t.stride(1) % vec or t.data_ptr() % 16:
+    if channel != 1 or row % vec or head % vec or t.data_ptr() & 15:
         raise ValueError(f"{name}: channels must be contiguous and every head's row 16-byte aligned")
+    return row, head
 
 
 def rope(x: torch.Tensor, table: torch.Tensor, positions: torch.Tensor, interleaved: bool = False,
@@ -913,15 +933,18 @@ def rope(x: torch.Tensor, table: torch.Tensor, positions: torch.Tensor, interlea
         raise ValueError(f"positions must be int32 [{n}]")
     if H == 0 or D == 0:
         raise ValueError("x has no heads or no channels")
-    _rows_of(x, "x")
-    _all_on(x.device, table=table, positions=positions)
+    index = x.get_device()
+    x_row, x_head = _rows_of(x, "x")
+    if not (_fits(table, index) and _fits(positions, index)):
+        _all_on(index, table=table, positions=positions)
     if out is None:
         out = torch.empty((n, H, D), dtype=x.dtype, device=x.device)
+        o_row, o_head = H * D, D
     else:
         if out.shape != x.shape or out.dtype != x.dtype or out.device != x.device:
             raise ValueError("out must be like x")
-        _rows_of(out, "out")
-        if n > 1 and out.stride(0) < D or H > 1 and out.stride(1) < D:
+        o_row, o_head = _rows_of(out, "out")
+        if n > 1 and o_row < D or H > 1 and o_head < D:
             raise ValueError("out: rows must not overlap")
         if n and not (out.data_ptr() == x.data_ptr() and out.stride() == x.stride()):
             (a, z), (b, y) = ((t.data_ptr(), t.data_ptr() + t.element_size() * (
@@ -930,10 +953,10 @@ def rope(x: torch.Tensor, table: torch.Tensor, positions: torch.Tensor, interlea
                 raise ValueError("out must be x itself or not overlap it")
     err = _err_word_if(check, x.device)
     flags = (N.ZX_ROPE_INTERLEAVED if interleaved else 0) | (N.ZX_ROPE_TRANSPOSE if transpose else 0)
-    with _on(x.device):
-        N.check(N.load().zx_rope(N.ptr(x), _DT[x.dtype], n, H, D, x.stride(0), x.stride(1), N.ptr(table), n_pos, rot,
-                                 N.ptr(positions), flags, N.ptr(out), out.stride(0), out.stride(1), N.ptr(err),
-                                 N.stream_ptr(x.device)), "rope")
+    with _on(index):
+        N.check(N.load().zx_rope(x.data_ptr(), _DT[x.dtype], n, H, D, x_row, x_head, table.data_ptr(), n_pos, rot,
+                                 positions.data_ptr(), flags, out.data_ptr(), o_row, o_head, N.ptr(err),
+                                 torch._C._cuda_getCurrentRawStream(index)), "rope")
     if check:
         _raise_kernel_error(err, "rope")
     return out
@@ -979,19 +1002,19 @@ def kv_rope_append(x: torch.Tensor, table: torch.Tensor, cu_seqlens: torch.Tenso
         raise ValueError(f"scales must be float32 [{L}, 2, {H}]")
     if saturate and not static_scales:
         raise ValueError("saturate applies to static scales (dynamic scales never overflow)")
-    _all_on(x.device, x=x, table=table, cu_seqlens=cu_seqlens, block_tables=block_tables, pool=pool, scales=scales,
+    index = x.get_device()
+    _all_on(index, x=x, table=table, cu_seqlens=cu_seqlens, block_tables=block_tables, pool=pool, scales=scales,
             start_pos=start_pos)
-    lib = N.load()
     flags = (N.ZX_APPEND_STATIC_SCALES if static_scales else 0) | (N.ZX_APPEND_SATURATE if saturate else 0) | \
         (N.ZX_ROPE_INTERLEAVED if interleaved else 0)
-    with _on(x.device):
-        ws = _workspace(lib.zx_kv_rope_append_workspace_bytes(L, T, H, D), x.device)
+    with _on(index):
+        ws, nb = _workspace_for("zx_kv_rope_append_workspace_bytes", index, L, T, H, D, flags)
         err = _err_word_if(check, x.device) if err is None else err
-        N.check(lib.zx_kv_rope_append(N.ptr(x), T * 2 * H * D, L, T, H, D, N.ptr(table), n_pos, rot, N.ptr(cu_seqlens),
-                                      N.ptr(start_pos), block_tables.shape[0], N.ptr(block_tables),
-                                      block_tables.shape[1], P, N.ptr(pool), pool[0].numel(), n_pages, N.ptr(scales),
-                                      flags, N.ptr(err), N.ptr(ws), ws.numel(), N.stream_ptr(x.device)),
-                "kv_rope_append")
+        N.check(N.load().zx_kv_rope_append(
+            x.data_ptr(), T * 2 * H * D, L, T, H, D, table.data_ptr(), n_pos, rot, cu_seqlens.data_ptr(),
+            N.ptr(start_pos), block_tables.shape[0], block_tables.data_ptr(), block_tables.shape[1], P,
+            pool.data_ptr(), n_pages * 2 * H * P * D, n_pages, scales.data_ptr(), flags, N.ptr(err), N.ptr(ws), nb,
+            torch._C._cuda_getCurrentRawStream(index)), "kv_rope_append")
     if check:
         _raise_kernel_error(err, "kv_rope_append")
     return scales
@@ -1041,17 +1064,17 @@ def kv4_append(x: torch.Tensor, cu_seqlens: torch.Tensor, block_tables: torch.Te
         raise ValueError("interleaved needs a table")
     n_pos, rot = _rope_table_of(table, D) if table is not None else (0, 0)
     _append_args(x, cu_seqlens, block_tables, start_pos, err)
-    _all_on(x.device, x=x, table=table, cu_seqlens=cu_seqlens, block_tables=block_tables, pool=pool,
-            start_pos=start_pos)
-    lib = N.load()
-    with _on(x.device):
-        ws = _workspace(lib.zx_kv4_append_workspace_bytes(T), x.device)
+    index = x.get_device()
+    _all_on(index, x=x, table=table, cu_seqlens=cu_seqlens, block_tables=block_tables, pool=pool, start_pos=start_pos)
+    with _on(index):
+        ws, nb = _workspace_for("zx_kv4_append_workspace_bytes", index, L, T, H)
         err = _err_word_if(check, x.device) if err is None else err
-        N.check(lib.zx_kv4_append(N.ptr(x), T * 2 * H * D, L, T, H, D, N.ptr(table), n_pos, rot, N.ptr(cu_seqlens),
-                                  N.ptr(start_pos), block_tables.shape[0], N.ptr(block_tables), block_tables.shape[1],
-                                  P, N.ptr(pool), pool[0].numel(), n_pages,
-                                  N.ZX_ROPE_INTERLEAVED if interleaved else 0, N.ptr(err), N.ptr(ws), ws.numel(),
-                                  N.stream_ptr(x.device)), "kv4_append")
+        N.check(N.load().zx_kv4_append(
+            x.data_ptr(), T * 2 * H * D, L, T, H, D, N.ptr(table), n_pos, rot, cu_seqlens.data_ptr(),
+            N.ptr(start_pos), block_tables.shape[0], block_tables.data_ptr(), block_tables.shape[1], P,
+            pool.data_ptr(), n_pages * 2 * H * (P // 16) * (17 * D // 2), n_pages,
+            N.ZX_ROPE_INTERLEAVED if interleaved else 0, N.ptr(err), N.ptr(ws), nb,
+            torch._C._cuda_getCurrentRawStream(index)), "kv4_append")
     if check:
         _raise_kernel_error(err, "kv4_append")
 
@@ -1071,8 +1094,8 @@ def kv4_gather_dequant(pool_layer: torch.Tensor, block_tables: torch.Tensor, seq
         raise ValueError("seq_lens must have one entry per block-table row")
     if out_len is None:
         out_len = block_tables.shape[1] * P
-    dev = pool_layer.device
-    _all_on(dev, pool_layer=pool_layer, block_tables=block_tables, seq_lens=seq_lens)
+    dev, index = pool_layer.device, pool_layer.get_device()
+    _all_on(index, pool_layer=pool_layer, block_tables=block_tables, seq_lens=seq_lens)
     if out is None:
         k = torch.empty((B, H, out_len, D), dtype=torch.bfloat16, device=dev)
         v = torch.empty_like(k)
@@ -1081,12 +1104,13 @@ def kv4_gather_dequant(pool_layer: torch.Tensor, block_tables: torch.Tensor, seq
         for t in (k, v):
             if t.shape != (B, H, out_len, D) or t.dtype != torch.bfloat16:
                 raise ValueError(f"out tensors must be bf16 {(B, H, out_len, D)}")
-        _all_on(dev, out_k=k, out_v=v)
-    with _on(dev):
+        _all_on(index, out_k=k, out_v=v)
+    with _on(index):
         err = _err_word_if(check, dev)
-        N.check(N.load().zx_kv4_gather_dequant(N.ptr(pool_layer), n_pages, H, D, P, N.ptr(block_tables),
-                                               block_tables.shape[1], N.ptr(seq_lens), B, out_len, N.ptr(k), N.ptr(v),
-                                               N.ptr(err), N.stream_ptr(dev)), "kv4_gather_dequant")
+        N.check(N.load().zx_kv4_gather_dequant(
+            pool_layer.data_ptr(), n_pages, H, D, P, block_tables.data_ptr(), block_tables.shape[1],
+            seq_lens.data_ptr(), B, out_len, k.data_ptr(), v.data_ptr(), N.ptr(err),
+            torch._C._cuda_getCurrentRawStream(index)), "kv4_gather_dequant")
     if check:
         _raise_kernel_error(err, "kv4_gather_dequant")
     return k, v
@@ -1115,18 +1139,19 @@ def paged_attention4_decode(q: torch.Tensor, pool_layer: torch.Tensor, block_tab
     B, Hq, _ = q.shape
     if block_tables.shape[0] != B or seq_lens.numel() != B or seq_lens.dtype != torch.int32:
         raise ValueError("block_tables and seq_lens (int32) need one row per sequence")
-    q = q.contiguous()
+    q, index = q.contiguous(), q.get_device()
     out = torch.empty((B, Hq, D), dtype=torch.bfloat16, device=q.device) if out is None else out
-    _all_on(q.device, q=q, pool_layer=pool_layer, block_tables=block_tables, seq_lens=seq_lens, out=out)
-    lib = N.load()
+    if not (_fits(q, index) and _fits(pool_layer, index) and _fits(block_tables, index) and _fits(seq_lens, index) and
+            _fits(out, index)):
+        _all_on(index, q=q, pool_layer=pool_layer, block_tables=block_tables, seq_lens=seq_lens, out=out)
     mb = block_tables.shape[1]
-    with _on(q.device):
-        ws = _workspace(lib.zx_paged_attention4_decode_workspace_bytes(B, Hq, Hkv, D, mb, P), q.device)
+    with _on(index):
+        ws, nb = _workspace_for("zx_paged_attention4_decode_workspace_bytes", index, B, Hq, Hkv, D, mb, P)
         err = _err_word_if(check, q.device)
-        N.check(lib.zx_paged_attention4_decode(
-            N.ptr(q), Hq, N.ptr(pool_layer), n_pages, Hkv, D, P, N.ptr(block_tables), mb, N.ptr(seq_lens), B,
-            float(D ** -0.5 if sm_scale is None else sm_scale), N.ptr(out), N.ptr(err), N.ptr(ws), ws.numel(),
-            N.stream_ptr(q.device)), "paged_attention4_decode")
+        N.check(N.load().zx_paged_attention4_decode(
+            q.data_ptr(), Hq, pool_layer.data_ptr(), n_pages, Hkv, D, P, block_tables.data_ptr(), mb,
+            seq_lens.data_ptr(), B, D ** -0.5 if sm_scale is None else float(sm_scale), out.data_ptr(), N.ptr(err),
+            N.ptr(ws), nb, torch._C._cuda_getCurrentRawStream(index)), "paged_attention4_decode")
     if check:
         _raise_kernel_error(err, "paged_attention4_decode")
     return out
@@ -1161,22 +1186,22 @@ def paged_attention4_prefill(q: torch.Tensor, cu_q: torch.Tensor, q_pos0: torch.
     if err is not None and (err.dtype != torch.int32 or err.numel() < 1 or err.device != q.device):
         raise ValueError("err must be an int32 tensor on q's device")
     out = torch.empty_like(q) if out is None else out
-    _all_on(q.device, q=q, cu_q=cu_q, q_pos0=q_pos0, pool_layer=pool_layer, block_tables=block_tables, kv_len=kv_len,
+    index = q.get_device()
+    _all_on(index, q=q, cu_q=cu_q, q_pos0=q_pos0, pool_layer=pool_layer, block_tables=block_tables, kv_len=kv_len,
             out=out)
     if max_q_per_seq is None:
         max_q_per_seq = int((cu_q[1:] - cu_q[:-1]).max().item()) if B else 0
     mq = max(0, min(int(max_q_per_seq), n_q))
-    lib = N.load()
     mb = block_tables.shape[1]
-    with _on(q.device):
-        nb = lib.zx_paged_attention4_prefill_workspace_bytes(Hq, Hkv, D, P, mb, B, mq)
-        ws = _workspace(nb, q.device) if nb else None
+    with _on(index):
+        ws, nb = _workspace_for("zx_paged_attention4_prefill_workspace_bytes", index, Hq, Hkv, D, P, mb, B, mq)
         err = _err_word_if(check, q.device) if err is None else err
-        N.check(lib.zx_paged_attention4_prefill(
-            N.ptr(q), n_q, N.ptr(cu_q), N.ptr(q_pos0), Hq, N.ptr(pool_layer), n_pages, Hkv, D, P, N.ptr(block_tables),
-            mb, N.ptr(kv_len), B, mq, int(bool(causal)), float(D ** -0.5 if sm_scale is None else sm_scale),
-            N.ZX_PREFILL_EXACT_P if precision == "exact" else 0, N.ptr(out), N.ptr(err), N.ptr(ws), nb,
-            N.stream_ptr(q.device)), "paged_attention4_prefill")
+        N.check(N.load().zx_paged_attention4_prefill(
+            q.data_ptr(), n_q, cu_q.data_ptr(), q_pos0.data_ptr(), Hq, pool_layer.data_ptr(), n_pages, Hkv, D, P,
+            block_tables.data_ptr(), mb, kv_len.data_ptr(), B, mq, int(bool(causal)),
+            D ** -0.5 if sm_scale is None else float(sm_scale), N.ZX_PREFILL_EXACT_P if precision == "exact" else 0,
+            out.data_ptr(), N.ptr(err), N.ptr(ws), nb, torch._C._cuda_getCurrentRawStream(index)),
+            "paged_attention4_prefill")
     if check:
         _raise_kernel_error(err, "paged_attention4_prefill")
     return out
