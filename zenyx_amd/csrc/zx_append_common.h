@@ -59,9 +59,11 @@ struct TokGeom {
 // (-1: in no sequence, negative, or at or beyond `limit` <= max_blocks * page_size); *e collects
 // the error bits.  The U searches (last b with cu_seqlens[b] <= t) take their steps together,
 // so that a step waits for one load.
+// cu, start: g.cu_seqlens and g.start_pos (may be NULL), or copies of them in LDS.
 template <int U>
-__device__ __forceinline__ void token_places(const TokGeom &g, int64_t limit, const int64_t (&t)[U], int64_t n_tok,
-                                             int64_t (&page)[U], int64_t (&pos)[U], int32_t &e) {
+__device__ __forceinline__ void token_places(const TokGeom &g, const int32_t *cu, const int32_t *start, int64_t limit,
+                                             const int64_t (&t)[U], int64_t n_tok, int64_t (&page)[U],
+                                             int64_t (&pos)[U], int32_t &e) {
   int lo[U], hi[U];
 #pragma unroll
   for (int k = 0; k < U; ++k) lo[k] = 0, hi[k] = g.n_seqs - 1;
@@ -69,7 +71,7 @@ __device__ __forceinline__ void token_places(const TokGeom &g, int64_t limit, co
 #pragma unroll
     for (int k = 0; k < U; ++k) {
       const int mid = (lo[k] + hi[k] + 1) >> 1;
-      const bool up = g.cu_seqlens[mid] <= t[k];
+      const bool up = cu[mid] <= t[k];
       if (lo[k] < hi[k]) {
         if (up) lo[k] = mid;
         else hi[k] = mid - 1;
@@ -79,9 +81,9 @@ __device__ __forceinline__ void token_places(const TokGeom &g, int64_t limit, co
   int32_t c0[U], c1[U], p0[U];
 #pragma unroll
   for (int k = 0; k < U; ++k) {
-    c0[k] = g.cu_seqlens[lo[k]];
-    c1[k] = g.cu_seqlens[lo[k] + 1];
-    p0[k] = g.start_pos ? g.start_pos[lo[k]] : 0;
+    c0[k] = cu[lo[k]];
+    c1[k] = cu[lo[k] + 1];
+    p0[k] = start ? start[lo[k]] : 0;
   }
 #pragma unroll
   for (int k = 0; k < U; ++k) {
@@ -99,12 +101,33 @@ __device__ __forceinline__ void token_places(const TokGeom &g, int64_t limit, co
   }
 }
 
+// The search's tables in LDS, for up to TOK_STAGED sequences: one load of the whole table instead
+// of a chain of loads per token.  Every thread of the block calls token_stage (it has a barrier).
+constexpr int TOK_STAGED = 256;
+struct TokStage {
+  int32_t cu[TOK_STAGED + 1], start[TOK_STAGED];
+};
+__device__ __forceinline__ void token_stage(const TokGeom &g, TokStage &s) {
+  if (g.n_seqs > TOK_STAGED) return;
+  for (int i = threadIdx.x; i <= g.n_seqs; i += blockDim.x) {
+    s.cu[i] = g.cu_seqlens[i];
+    if (i < g.n_seqs) s.start[i] = g.start_pos ? g.start_pos[i] : 0;
+  }
+  __syncthreads();
+}
+template <int U>
+__device__ __forceinline__ void token_places(const TokGeom &g, const TokStage &s, int64_t limit, const int64_t (&t)[U],
+                                             int64_t n_tok, int64_t (&page)[U], int64_t (&pos)[U], int32_t &e) {
+  if (g.n_seqs <= TOK_STAGED) token_places<U>(g, s.cu, s.start, limit, t, n_tok, page, pos, e);
+  else token_places<U>(g, g.cu_seqlens, g.start_pos, limit, t, n_tok, page, pos, e);
+}
+
 // Pool offsets (bytes within one layer of FP8 pages) of U tokens' (page, row) bases, or -1.
 template <int U>
 __device__ __forceinline__ void token_offsets(const TokGeom &g, const int64_t (&t)[U], int64_t n_tok,
                                               int64_t (&off)[U], int32_t &e) {
   int64_t page[U], pos[U];
-  token_places<U>(g, (int64_t)g.max_blocks * g.page_size, t, n_tok, page, pos, e);
+  token_places<U>(g, g.cu_seqlens, g.start_pos, (int64_t)g.max_blocks * g.page_size, t, n_tok, page, pos, e);
 #pragma unroll
   for (int k = 0; k < U; ++k)
     off[k] = page[k] < 0 ? -1

@@ -21,7 +21,7 @@ kv4_places_kernel(TokGeom g, int64_t limit, int64_t n_tok, K4Place *places, int3
   if (t[0] >= n_tok) return;
   int64_t page[1], pos[1];
   int32_t e = 0;
-  token_places<1>(g, limit, t, n_tok, page, pos, e);
+  token_places<1>(g, g.cu_seqlens, g.start_pos, limit, t, n_tok, page, pos, e);
   if (e && err) atomicOr(err, e);
   places[t[0]] = K4Place{(int32_t)page[0], (int32_t)pos[0]};
 }
@@ -55,7 +55,7 @@ __global__ void __launch_bounds__(64 * K4_WAVES) kv4_append_kernel(K4Append a) {
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t grp = (int64_t)blockIdx.x * K4_WAVES + wave;
-  if (grp >= a.n_grp) return;  // (no barrier follows)
+  const bool live = grp < a.n_grp;  // uniform
   const int slabs = 2 * a.n_heads;
   const int64_t tg16 = grp / slabs;
   const int slab = (int)(grp - tg16 * slabs);  // neighbours take neighbouring heads of the same tokens
@@ -64,8 +64,8 @@ __global__ void __launch_bounds__(64 * K4_WAVES) kv4_append_kernel(K4Append a) {
   const char *src = reinterpret_cast<const char *>(a.x + (int64_t)layer * a.x_layer_stride) + t0 * a.row_bytes +
                     2LL * slab * D;
   // past the last token the loads return zeros
-  const int64_t left = (a.n_tok - t0) * a.row_bytes - 2LL * slab * D;
-  const __amdgpu_buffer_rsrc_t rs = q_rsrc(src, left);
+  const int64_t left = live ? (a.n_tok - t0) * a.row_bytes - 2LL * slab * D : 0;
+  const __amdgpu_buffer_rsrc_t rs = q_rsrc(live ? src : reinterpret_cast<const char *>(a.x), left);
   q_v4u v[NL];
 #pragma unroll
   for (int i = 0; i < NL; ++i) {
@@ -74,10 +74,13 @@ __global__ void __launch_bounds__(64 * K4_WAVES) kv4_append_kernel(K4Append a) {
   }
   const int n = lane & 15;
   int64_t page[1], pos[1];
+  __shared__ TokStage stage;
+  if constexpr (LOCATE) token_stage(a.tg, stage);
+  if (!live) return;  // (no barrier follows)
   if constexpr (LOCATE) {
     const int64_t t[1] = {t0 + n};
     int32_t e = 0;
-    token_places<1>(a.tg, a.limit, t, a.n_tok, page, pos, e);
+    token_places<1>(a.tg, stage, a.limit, t, a.n_tok, page, pos, e);
     if (e && a.err && layer == 0 && slab == 0 && lane < 16) atomicOr(a.err, e);
   } else {
     const K4Place p = t0 + n < a.n_tok ? a.places[t0 + n] : K4Place{-1, -1};

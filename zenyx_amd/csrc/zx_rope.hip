@@ -170,16 +170,17 @@ ra_places_kernel(TokGeom g, int64_t limit, int64_t n_tok, TokPlace *places, int3
   if (t[0] >= n_tok) return;
   int64_t page[1], pos[1];
   int32_t e = 0;
-  token_places<1>(g, limit, t, n_tok, page, pos, e);
+  token_places<1>(g, g.cu_seqlens, g.start_pos, limit, t, n_tok, page, pos, e);
   if (e && err) atomicOr(err, e);
   places[t[0]] = TokPlace{(int32_t)page[0], (int32_t)pos[0]};
 }
 
 template <int U, bool LOCATE>
-__device__ __forceinline__ void ra_find(const TokGeom &tg, int64_t limit, const TokPlace *places, const int64_t (&row)[U],
-                                        int64_t n_tok, int64_t (&page)[U], int64_t (&pos)[U], int32_t &e) {
+__device__ __forceinline__ void ra_find(const TokGeom &tg, const TokStage &stage, int64_t limit, const TokPlace *places,
+                                        const int64_t (&row)[U], int64_t n_tok, int64_t (&page)[U], int64_t (&pos)[U],
+                                        int32_t &e) {
   if constexpr (LOCATE) {
-    token_places<U>(tg, limit, row, n_tok, page, pos, e);
+    token_places<U>(tg, stage, limit, row, n_tok, page, pos, e);
   } else {
 #pragma unroll
     for (int k = 0; k < U; ++k) {
@@ -204,6 +205,8 @@ rope_append_amax_kernel(const uint16_t *x, RaGeom g, RopeTable r, TokGeom tg, in
   const int64_t step = (int64_t)gridDim.x * U * g.rpb;
   uint32_t m = 0;  // two packed 16-bit maxima
   int32_t e = 0;
+  __shared__ TokStage stage;
+  if constexpr (LOCATE) token_stage(tg, stage);
   for (int64_t r0 = (int64_t)blockIdx.x * U * g.rpb; r0 < g.n_tok; r0 += step) {
     const __amdgpu_buffer_rsrc_t rsrc = q_rsrc(xl + r0 * g.row_bytes, (g.n_tok - r0) * g.row_bytes);
     uint4 a[U], b[U];
@@ -217,7 +220,7 @@ rope_append_amax_kernel(const uint16_t *x, RaGeom g, RopeTable r, TokGeom tg, in
       b[k] = make_uint4(w.x, w.y, w.z, w.w);
       row[k] = r0 + k * g.rpb + rs;
     }
-    ra_find<U, LOCATE>(tg, limit, places, row, g.n_tok, page, pos, e);
+    ra_find<U, LOCATE>(tg, stage, limit, places, row, g.n_tok, page, pos, e);
 #pragma unroll
     for (int k = 0; k < U; ++k) {
       if (n.turns) {
@@ -269,7 +272,9 @@ rope_append_rows_kernel(const uint16_t *x, RaGeom g, RopeTable r, TokGeom tg, in
     row[k] = r0 + k * g.rpb + rs;
   }
   int32_t e = 0;
-  ra_find<U, LOCATE>(tg, limit, places, row, g.n_tok, page, pos, e);
+  __shared__ TokStage stage;
+  if constexpr (LOCATE) token_stage(tg, stage);
+  ra_find<U, LOCATE>(tg, stage, limit, places, row, g.n_tok, page, pos, e);
   if (LOCATE && e && err && layer == 0 && n.slab == 0 && n.p == 0) atomicOr(err, e);
 #pragma unroll
   for (int k = 0; k < U; ++k) {
@@ -448,7 +453,6 @@ extern "C" int zx_kv_rope_append(const uint16_t *x, int64_t x_layer_stride, int3
   const RopeTable r = {table, n_pos, rot_dim};
   const TokGeom tg = {cu_seqlens, start_pos, block_tables, n_seqs, max_blocks, page_size, head_dim, n_pages, page_bytes};
   const int64_t limit = std::min((int64_t)max_blocks * page_size, n_pos);
-  const int64_t tiles = ceil_div(n_tok, (int64_t)RA_U * g.rpb);
   const bool locate = ra_locates(n_layers, n_tok, n_heads, head_dim);
   TokPlace *places = static_cast<TokPlace *>(workspace);
   uint32_t *part = reinterpret_cast<uint32_t *>(static_cast<char *>(workspace) +
@@ -462,25 +466,25 @@ extern "C" int zx_kv_rope_append(const uint16_t *x, int64_t x_layer_stride, int3
   if (dynamic) {
     const unsigned gx = (unsigned)ra_amax_grid_x(n_tok, g.rpb, n_layers);
     const dim3 grid(gx, n_layers);
-#define ZX_RA_AMAX(loc, il) \
-  rope_append_amax_kernel<RA_U, loc, il><<<grid, threads, 0, st>>>(x, g, r, tg, limit, places, part)
-    if (locate && inter) ZX_RA_AMAX(true, true);
-    else if (locate) ZX_RA_AMAX(true, false);
-    else if (inter) ZX_RA_AMAX(false, true);
-    else ZX_RA_AMAX(false, false);
+#define ZX_RA_AMAX(u, loc, il) \
+  rope_append_amax_kernel<u, loc, il><<<grid, threads, 0, st>>>(x, g, r, tg, limit, places, part)
+    if (locate && inter) ZX_RA_AMAX(1, true, true);
+    else if (locate) ZX_RA_AMAX(1, true, false);
+    else if (inter) ZX_RA_AMAX(RA_U, false, true);
+    else ZX_RA_AMAX(RA_U, false, false);
 #undef ZX_RA_AMAX
     if ((rc = check_launch("rope_append_amax"))) return rc;
     if ((rc = finalize_partials(part, (int32_t)gx, g.n_slabs, n_layers, scales, st))) return rc;
   }
-  const dim3 grid((unsigned)tiles, n_layers);
-#define ZX_RA_ROWS2(mode, loc, il) \
-  rope_append_rows_kernel<RA_U, mode, loc, il><<<grid, threads, 0, st>>>(x, g, r, tg, limit, places, scales, pool, \
-                                                                        pool_layer_stride, err)
-#define ZX_RA_ROWS(mode)                                   \
-  if (locate && inter) ZX_RA_ROWS2(mode, true, true);      \
-  else if (locate) ZX_RA_ROWS2(mode, true, false);         \
-  else if (inter) ZX_RA_ROWS2(mode, false, true);          \
-  else ZX_RA_ROWS2(mode, false, false);
+  const dim3 grid((unsigned)ceil_div(n_tok, (int64_t)(locate ? 1 : RA_U) * g.rpb), n_layers);
+#define ZX_RA_ROWS2(mode, u, loc, il)                                                                                  \
+  rope_append_rows_kernel<u, mode, loc, il><<<grid, threads, 0, st>>>(x, g, r, tg, limit, places, scales, pool,        \
+                                                                     pool_layer_stride, err)
+#define ZX_RA_ROWS(mode)                                 \
+  if (locate && inter) ZX_RA_ROWS2(mode, 1, true, true); \
+  else if (locate) ZX_RA_ROWS2(mode, 1, true, false);    \
+  else if (inter) ZX_RA_ROWS2(mode, RA_U, false, true);  \
+  else ZX_RA_ROWS2(mode, RA_U, false, false);
   if (dynamic) {
     ZX_RA_ROWS(0)
   } else if (flags & ZX_APPEND_SATURATE) {
