@@ -485,8 +485,8 @@ int zx_rope(const void *x, int dtype, int64_t n_rows, int32_t n_heads, int32_t h
 
 /* zx_kv_quant_append with the keys rotated by their positions on the way (rounded to bf16 as
  * zx_rope rounds them, then quantised): the codes and scales of zx_rope followed by
- * zx_kv_quant_append, without the rotated copy.  flags: ZX_APPEND_STATIC_SCALES,
- * ZX_APPEND_SATURATE, ZX_ROPE_INTERLEAVED.  A token at or beyond n_pos is not stored and sets
+ * zx_kv_quant_append, without the rotated copy.  flags: zx_kv_quant_append's and
+ * ZX_ROPE_INTERLEAVED (the single pass only where a CU's share of a slab fits its registers).  A token at or beyond n_pos is not stored and sets
  * ZX_KERR_POS_RANGE; dynamic scales are taken over the tokens that have a position (rows
  * outside [cu_seqlens[0], cu_seqlens[n_seqs]) have none).  workspace:
  * zx_kv_rope_append_workspace_bytes() device bytes (0 for a small call with static scales),

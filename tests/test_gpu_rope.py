@@ -250,7 +250,7 @@ CASES = [  # lens, old, L, H, D, P, rot, padded rows
 
 
 @pytest.mark.parametrize("interleaved", [False, True])
-@pytest.mark.parametrize("mode", ["dynamic", "static", "saturate"])
+@pytest.mark.parametrize("mode", ["dynamic", "single", "two", "static", "saturate"])
 @pytest.mark.parametrize("case", range(len(CASES)))
 def test_append_equals_rotation_then_append(dev, interleaved, mode, case):
     lens, old, L, H, D, P, rot, pad = CASES[case]
@@ -269,16 +269,35 @@ def test_append_equals_rotation_then_append(dev, interleaved, mode, case):
     pool = torch.randint(0, 256, (L, n_pages, 2, H, P, D), generator=g, device=dev, dtype=torch.uint8)
     want_pool = pool.clone()
     scales = None
-    if mode != "dynamic":
+    dynamic = mode in ("dynamic", "single", "two")
+    if not dynamic:
         scales = torch.rand((L, 2, H), generator=g, device=dev) * 0.02 + 0.01
         scales[0, 0, 0] = -0.03
     want_err, err = torch.zeros(1, dtype=torch.int32, device=dev), torch.zeros(1, dtype=torch.int32, device=dev)
-    kw = dict(start_pos=start, static_scales=mode != "dynamic", saturate=mode == "saturate")
+    kw = dict(start_pos=start, static_scales=not dynamic, saturate=mode == "saturate")
     want = kv.kv_quant_append(turned, cu, bt, want_pool, scales=None if scales is None else scales.clone(), err=want_err,
                               **kw)
-    got = kv.kv_rope_append(x, table, cu, bt, pool, scales=scales, interleaved=interleaved, err=err, **kw)
+    got = kv.kv_rope_append(x, table, cu, bt, pool, scales=scales, interleaved=interleaved, err=err,
+                            single_pass=mode == "single", two_pass=mode == "two", **kw)
     assert same_bits(got, want) and torch.equal(pool, want_pool)
     assert err.item() == want_err.item()
+
+
+def test_append_that_the_rule_sends_through_one_pass(dev):
+    """A batch large enough that the call takes the cooperative pass by itself, in several parts:
+    many sequences, rows behind them, a share that nearly fills the registers."""
+    L, H, D, P, rot = 2, 8, 128, 16, 128
+    rng = np.random.default_rng(3)
+    lens = rng.integers(100, 1900, 70).tolist()
+    bt, cu, start, n_pages = paged(lens, [0] * 70, P, 2, dev, 7)
+    T = sum(lens)
+    x = torch.randn((L, T + 50, 2, H, D), device=dev).to(torch.bfloat16)
+    x[:, T:] = 1e4
+    table = table64(2000, rot, dev)
+    a, b = (torch.zeros((L, n_pages, 2, H, P, D), dtype=torch.uint8, device=dev) for _ in range(2))
+    sa = kv.kv_rope_append(x, table, cu, bt, a, check=True)
+    sb = kv.kv_rope_append(x, table, cu, bt, b, check=True, two_pass=True)
+    assert same_bits(sa, sb) and torch.equal(a, b)
 
 
 def test_append_bad_pages_and_positions(dev):
@@ -308,13 +327,13 @@ def test_append_non_finite(dev):
     H, D, P = 2, 64, 16
     bt, cu, start, n_pages = paged([20], [0], P, 0, dev, 0)
     table = table64(20, D, dev)
-    for bad in (float("nan"), float("inf")):
+    for bad, one in ((float("nan"), False), (float("inf"), False), (float("nan"), True), (float("inf"), True)):
         x = torch.randn((1, 20, 2, H, D), device=dev).to(torch.bfloat16)
         x[0, 3, 0, 1, 5] = bad
         turned = x.clone()
         turned[0, :, 0] = kv.rope(x[0, :, 0].contiguous(), table, torch.arange(20, dtype=torch.int32, device=dev))
         a, b = (torch.zeros((1, n_pages, 2, H, P, D), dtype=torch.uint8, device=dev) for _ in range(2))
-        sa, sb = kv.kv_rope_append(x, table, cu, bt, a), kv.kv_quant_append(turned, cu, bt, b)
+        sa, sb = kv.kv_rope_append(x, table, cu, bt, a, single_pass=one), kv.kv_quant_append(turned, cu, bt, b)
         assert torch.equal(sa.isnan(), sb.isnan()) and torch.equal(a, b)
 
 

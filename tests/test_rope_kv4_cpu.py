@@ -69,6 +69,7 @@ def test_append_refusals(lib, four, kw, rc):
 
 def test_append_refusals_of_one_kind(lib):
     assert lib.zx_kv_rope_append(*append_args(False, flags=4)) == N.ZX_ERR_INVALID  # saturate, dynamic scales
+    assert lib.zx_kv_rope_append(*append_args(False, flags=2 | 8)) == N.ZX_ERR_INVALID  # one pass and two
     assert lib.zx_kv_rope_append(*append_args(False, table=None)) == N.ZX_ERR_INVALID
     assert lib.zx_kv_rope_append(*append_args(False, H=40, D=128)) == N.ZX_ERR_UNSUPPORTED
     assert lib.zx_kv4_append(*append_args(True, flags=1)) == N.ZX_ERR_INVALID  # no scales to be static

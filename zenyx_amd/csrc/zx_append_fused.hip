@@ -25,9 +25,16 @@
 // registers hold are re-read from memory (both for the max and for the encode).
 // Every wait is bounded in wall time; a timeout raises a global abort flag that
 // releases every other waiter, so all waves always exit.
+//
+// ROPE: the keys are rotated as they arrive (zx_rope_common.h).  A thread's vectors sit at the same
+// tokens and channels in every slab, so the workgroup's rows of the rotary table are copied to
+// LDS once, laid out so that the 16-byte reads of neighbouring lanes are contiguous; a pair's
+// other half comes from the lane that holds it (ds_bpermute).  4 layers x 59,548 tokens, 8 heads,
+// D = 128: 465 us in two passes, 352 us so (4.2 TB/s).
 #include <type_traits>
 
 #include "zx_internal.h"
+#include "zx_rope_common.h"
 
 namespace zx {
 
@@ -52,6 +59,9 @@ struct FusedArgs {
   uint32_t *abort_flag;
   int32_t *err;
   uint64_t spin_ticks;  // bound of one wait in s_memrealtime ticks (100 MHz)
+  const float *table;   // ROPE: [n_pos][rot], and every token's position (-1: none)
+  const int32_t *tok_pos;
+  int32_t rot;
 };
 
 struct FusedShared {
@@ -205,6 +215,100 @@ __device__ __forceinline__ void encode_share(const FusedArgs &a, const ThreadMap
   }
 }
 
+// ROPE: what a thread needs to rotate its vectors.
+constexpr int FA_ROPE_NONE = 0, FA_ROPE_HALF = 1, FA_ROPE_PAIRS = 2;
+struct FusedRope {
+  int cs;            // of vector 0 in LDS (FA_ROPE_HALF: 4 planes of rot / 4, else cosines and sines)
+  int plane, step;   // floats between the planes; between the vectors of a thread
+  int partner;       // byte address of the lane with the pairs' other halves
+  uint32_t flip;     // sign of the sines for this half
+  bool turns;        // the thread's channels are rotated in a key
+  uint32_t live;     // bit k: vector k's token has a position
+};
+__device__ __forceinline__ int rope_lds_floats(const FusedArgs &a, int k) {
+  return k * (FA_DATA_THREADS >> a.vpt_log2) * a.rot;
+}
+
+// The table rows of the workgroup's tokens into LDS (zeros where there is none).
+template <int K, int ROPE>
+__device__ __forceinline__ void rope_stage(const FusedArgs &a, int64_t t_lo, int n_own, float *lds) {
+  const int q4 = a.rot / 4, half = a.rot / 2;
+  const int n_tok = K * (FA_DATA_THREADS >> a.vpt_log2);
+  for (int i = threadIdx.x; i < n_tok * q4; i += FA_THREADS) {
+    const int tok = i / q4, e = 4 * (i - tok * q4), sine = e >= half, pair = e - sine * half;
+    const int32_t pos = tok < n_own ? a.tok_pos[t_lo + tok] : -1;
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (pos >= 0) v = *reinterpret_cast<const float4 *>(a.table + (int64_t)pos * a.rot + e);
+    const int at = ROPE == FA_ROPE_HALF ? (2 * sine + (pair >> 2 & 1)) * q4 + (pair >> 3) * 4 : sine * half + pair;
+    *reinterpret_cast<float4 *>(lds + tok * a.rot + at) = v;
+  }
+}
+
+template <int K, int ROPE>
+__device__ __forceinline__ FusedRope rope_map(const FusedArgs &a, int64_t t_lo, int nreg) {
+  FusedRope f;
+  const int lane = threadIdx.x & 63, c = threadIdx.x & ((1 << a.vpt_log2) - 1), h = a.rot / 16;
+  const bool first = c < h;
+  f.turns = 8 * c < a.rot;
+  f.plane = ROPE == FA_ROPE_HALF ? a.rot / 4 : a.rot / 2;
+  f.step = rope_lds_floats(a, 1);
+  const int own = ROPE == FA_ROPE_HALF ? (first ? c : c - h) : c;
+  f.cs = (threadIdx.x >> a.vpt_log2) * a.rot + 4 * (f.turns ? own : 0);
+  f.partner = 4 * (f.turns ? (first ? lane + h : lane - h) : lane);
+  f.flip = first ? 0x80000000u : 0u;
+  f.live = 0;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int v = k * FA_DATA_THREADS + threadIdx.x;
+    if (v < nreg && a.tok_pos[t_lo + (v >> a.vpt_log2)] >= 0) f.live |= 1u << k;
+  }
+  return f;
+}
+
+// Rotates the share of a key's slab in its registers; vectors of tokens without a position become
+// zeros (they count for no scale and are not stored).
+template <int K, int ROPE>
+__device__ __forceinline__ void rope_share(const FusedRope &f, const float *lds, bool key, uint4 (&r)[K]) {
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    __builtin_amdgcn_sched_barrier(0);  // one vector's operands at a time: the slabs fill the registers
+    if (key) {  // uniform
+      int at = f.cs;
+      asm volatile("" : "+v"(at));  // (addresses made here, not kept in registers over the slabs)
+      const float *cs = lds + (at + k * f.step);
+      uint4 w;
+      uint32_t(&rw)[4] = reinterpret_cast<uint32_t(&)[4]>(r[k]), (&ww)[4] = reinterpret_cast<uint32_t(&)[4]>(w);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {  // four channels
+        const float x[4] = {bf_lo(rw[2 * i]), bf_hi(rw[2 * i]), bf_lo(rw[2 * i + 1]), bf_hi(rw[2 * i + 1])};
+        float y[4];
+        if constexpr (ROPE == FA_ROPE_HALF) {
+          const float4 c = *reinterpret_cast<const float4 *>(cs + i * f.plane);
+          const float4 s = *reinterpret_cast<const float4 *>(cs + (2 + i) * f.plane);
+          const uint32_t o0 = __builtin_amdgcn_ds_bpermute(f.partner, rw[2 * i]);
+          const uint32_t o1 = __builtin_amdgcn_ds_bpermute(f.partner, rw[2 * i + 1]);
+          const float z[4] = {bf_lo(o0), bf_hi(o0), bf_lo(o1), bf_hi(o1)};
+          const float cc[4] = {c.x, c.y, c.z, c.w}, ss[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j)  // first half: x c - z s (z (-s) is -(z s), exactly)
+            y[j] = x[j] * cc[j] + z[j] * __uint_as_float(__float_as_uint(ss[j]) ^ f.flip);
+        } else {
+          const float2 c = *reinterpret_cast<const float2 *>(cs + 2 * i);
+          const float2 s = *reinterpret_cast<const float2 *>(cs + f.plane + 2 * i);
+          y[0] = x[0] * c.x - x[1] * s.x;
+          y[1] = x[1] * c.x + x[0] * s.x;
+          y[2] = x[2] * c.y - x[3] * s.y;
+          y[3] = x[3] * c.y + x[2] * s.y;
+        }
+        ww[2 * i] = pack_bf16(y[0], y[1]);
+        ww[2 * i + 1] = pack_bf16(y[2], y[3]);
+      }
+      if (f.turns) r[k] = w;
+    }
+    if (!(f.live >> k & 1u)) r[k] = make_uint4(0, 0, 0, 0);
+  }
+}
+
 // Data wave: fold its max into the workgroup's LDS slot for slab s.
 __device__ __forceinline__ void contribute(FusedShared &sh, int s, uint32_t mx, bool real) {
   mx = group_max(mx, 64);
@@ -299,9 +403,10 @@ __device__ __forceinline__ bool control_loop(const FusedArgs &a, FusedShared &sh
 // K: 16-byte vectors per data thread per slab kept in registers; NB: register buffers
 // (the data waves run NB - 1 slabs ahead of the oldest unresolved one).
 // SPILL: some share holds more vectors than the registers (extra loops re-read them);
-// without it the data path is straight-line code between waits.
-template <int K, int NB, bool SPILL, bool WIDE>
+// without it the data path is straight-line code between waits.  ROPE without SPILL only.
+template <int K, int NB, bool SPILL, bool WIDE, int ROPE = FA_ROPE_NONE>
 __global__ void __launch_bounds__(FA_THREADS, 1) kv_append_fused_kernel(FusedArgs a) {
+  static_assert(ROPE == FA_ROPE_NONE || !SPILL, "rotated shares live in registers");
   static_assert(NB + 1 <= FA_SLOTS, "slot ring too small");
   __shared__ FusedShared sh;
   const uint32_t G = gridDim.x;
@@ -315,6 +420,8 @@ __global__ void __launch_bounds__(FA_THREADS, 1) kv_append_fused_kernel(FusedArg
     sh.ready[threadIdx.x] = 0;
   }
   if (threadIdx.x == 0) sh.abort = 0;
+  extern __shared__ __attribute__((aligned(16))) float rope_lds[];
+  if constexpr (ROPE != FA_ROPE_NONE) rope_stage<K, ROPE>(a, t_lo, (int)(t_hi - t_lo), rope_lds);
   __syncthreads();
 
   const int S_pad = (int)ceil_div(S, NB) * NB;
@@ -356,11 +463,20 @@ __global__ void __launch_bounds__(FA_THREADS, 1) kv_append_fused_kernel(FusedArg
   // Slabs past the end are clamped to the last one: the loads stay unconditional (and
   // valid) and their maxes are simply not contributed.
   auto slab = [&](int q) { return phys_slab(a, q < S ? q : S - 1); };
+  FusedRope rope;
+  if constexpr (ROPE != FA_ROPE_NONE) rope = rope_map<K, ROPE>(a, t_lo, m.nreg);
+  const int two_h = 2 * a.n_heads;
+  auto turn = [&](int s, uint4 (&r)[K]) {
+    if constexpr (ROPE != FA_ROPE_NONE) rope_share<K, ROPE>(rope, rope_lds, s % two_h < a.n_heads, r);
+  };
   uint4 buf[NB][K];
 #pragma unroll
   for (int i = 0; i < NB; ++i) load_share<K, WIDE>(a, m, slab(i), t_base, buf[i]);
 #pragma unroll
-  for (int i = 0; i + 1 < NB; ++i) contribute(sh, i, share_max<K, SPILL, WIDE>(a, m, slab(i), t_lo, nv, buf[i]), i < S);
+  for (int i = 0; i + 1 < NB; ++i) {
+    turn(slab(i), buf[i]);
+    contribute(sh, i, share_max<K, SPILL, WIDE>(a, m, slab(i), t_lo, nv, buf[i]), i < S);
+  }
 
   // step q (buffer i = q % NB): reduce q + NB - 1 (loaded during step q - 1), wait for
   // slab q's scale, encode q, refill the buffer with q + NB.  Reducing first hands the
@@ -375,6 +491,7 @@ __global__ void __launch_bounds__(FA_THREADS, 1) kv_append_fused_kernel(FusedArg
       const int q = q0 + i;
       const int j = (i + NB - 1) % NB;  // constant after unrolling
       const int r = q + NB - 1;
+      turn(slab(r), buf[j]);
       contribute(sh, r, share_max<K, SPILL, WIDE>(a, m, slab(r), t_lo, nv, buf[j]), r < S);
       float sc;
       if (!wait_ready(sh, q, sc)) return;
@@ -395,28 +512,50 @@ __global__ void __launch_bounds__(FA_THREADS, 1) kv_append_fused_kernel(FusedArg
 // 3.12 ms per call.
 constexpr int FA_K = FA_K_CHOICE;
 #define FA_KERNEL(spill, wide) kv_append_fused_kernel<FA_K, ((spill) || (wide)) ? 4 : 5, spill, wide>
+#define FA_ROPE_KERNEL(wide, rope) kv_append_fused_kernel<FA_K, 4, false, wide, rope>
 
-static int fused_supported() {
-  static int cached[64] = {0};
+// LDS for the table rows of the tokens that a workgroup's registers hold.
+static size_t fused_rope_lds(int32_t head_dim, int32_t rot) {
+  return (size_t)FA_K * (FA_DATA_THREADS / (head_dim / 8)) * rot * sizeof(float);
+}
+static const void *fused_fn(bool spill, bool wide, int rope) {
+  if (rope == FA_ROPE_HALF)
+    return wide ? reinterpret_cast<const void *>(FA_ROPE_KERNEL(true, FA_ROPE_HALF))
+                : reinterpret_cast<const void *>(FA_ROPE_KERNEL(false, FA_ROPE_HALF));
+  if (rope == FA_ROPE_PAIRS)
+    return wide ? reinterpret_cast<const void *>(FA_ROPE_KERNEL(true, FA_ROPE_PAIRS))
+                : reinterpret_cast<const void *>(FA_ROPE_KERNEL(false, FA_ROPE_PAIRS));
+  return spill ? (wide ? reinterpret_cast<const void *>(FA_KERNEL(true, true))
+                       : reinterpret_cast<const void *>(FA_KERNEL(true, false)))
+               : (wide ? reinterpret_cast<const void *>(FA_KERNEL(false, true))
+                       : reinterpret_cast<const void *>(FA_KERNEL(false, false)));
+}
+
+// rope: whether the kernels that rotate are meant (their LDS has to fit too).
+static int fused_supported(bool rope) {
+  static int cached[2][64] = {{0}};
   int dev = 0;
   ZX_TRY_HIP(hipGetDevice(&dev));
   if (dev < 0 || dev >= 64) return fail(ZX_ERR_UNSUPPORTED, "device index out of range");
-  if (!cached[dev]) {
+  if (!cached[rope][dev]) {
     int coop = 0, fits = 1;
     ZX_TRY_HIP(hipDeviceGetAttribute(&coop, hipDeviceAttributeCooperativeLaunch, dev));
-    const void *fns[4] = {reinterpret_cast<const void *>(FA_KERNEL(false, false)),
-                          reinterpret_cast<const void *>(FA_KERNEL(true, false)),
-                          reinterpret_cast<const void *>(FA_KERNEL(false, true)),
-                          reinterpret_cast<const void *>(FA_KERNEL(true, true))};
-    for (const void *fn : fns) {
+    const size_t lds = rope ? fused_rope_lds(128, 128) : 0;  // (the same for every full head)
+    for (int i = 0; i < 4; ++i) {
+      const void *fn = rope ? fused_fn(false, i & 1, i & 2 ? FA_ROPE_HALF : FA_ROPE_PAIRS) : fused_fn(i & 1, i & 2, 0);
+      if (rope) ZX_TRY_HIP(hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
       int per_cu = 0;
-      ZX_TRY_HIP(hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, fn, FA_THREADS, 0));
+      ZX_TRY_HIP(hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, fn, FA_THREADS, lds));
       fits = fits && per_cu >= 1;
     }
-    cached[dev] = (coop && fits) ? 1 : -1;
+    cached[rope][dev] = (coop && fits) ? 1 : -1;
   }
-  if (cached[dev] < 0) return fail(ZX_ERR_UNSUPPORTED, "device cannot co-schedule the single-pass append");
+  if (cached[rope][dev] < 0) return fail(ZX_ERR_UNSUPPORTED, "device cannot co-schedule the single-pass append");
   return ZX_OK;
+}
+
+bool append_fused_holds(int64_t n_tok, int32_t head_dim) {
+  return ceil_div(n_tok, num_cus()) * (head_dim / 8) <= (int64_t)FA_K * FA_DATA_THREADS;
 }
 
 // The single pass pays a device-wide exchange per slab (~3.6 us on MI355X whatever the
@@ -441,9 +580,11 @@ size_t append_fused_workspace_bytes(int32_t n_layers, int32_t n_heads) {
 
 int append_fused(const uint16_t *x, int64_t x_layer_stride, int32_t n_layers, int64_t n_tok, int32_t n_heads,
                  int32_t head_dim, const int64_t *tok_off, uint8_t *pool, int64_t pool_layer_stride,
-                 int32_t page_size, float *scales, int32_t *err, void *ws, hipStream_t st) {
-  int rc = fused_supported();
+                 int32_t page_size, float *scales, int32_t *err, void *ws, hipStream_t st, const AppendRope *rope) {
+  int rc = fused_supported(rope != nullptr);
   if (rc) return rc;
+  if (rope && !append_fused_holds(n_tok, head_dim))
+    return fail(ZX_ERR_UNSUPPORTED, "fused append: a rotated share must fit the registers");
   const int G = num_cus();
   if (ceil_div(n_tok, G) * (head_dim / 8) >= (1LL << 30))
     return fail(ZX_ERR_UNSUPPORTED, "fused append: share too large");
@@ -468,6 +609,9 @@ int append_fused(const uint16_t *x, int64_t x_layer_stride, int32_t n_layers, in
   a.abort_flag = reinterpret_cast<uint32_t *>(w);
   a.slots = reinterpret_cast<uint32_t *>(w + 256);
   a.err = err;
+  a.table = rope ? rope->table : nullptr;
+  a.tok_pos = rope ? rope->tok_pos : nullptr;
+  a.rot = rope ? rope->rot : 0;
   a.spin_ticks = wait_bound_ticks();  // default 2 s without progress (zx_set_wait_bound_us)
   // the abort flag and every slot start at zero: one fill kernel (not a memset, so the
   // sequence stays valid inside a captured graph) over the header and the slots
@@ -475,11 +619,9 @@ int append_fused(const uint16_t *x, int64_t x_layer_stride, int32_t n_layers, in
   void *args[] = {&a};
   const bool spill = ceil_div(n_tok, G) * (head_dim / 8) > (int64_t)FA_K * FA_DATA_THREADS;
   const bool wide = pool_layer_stride > FA_RANGE;  // pool offsets beyond 32-bit buffer offsets
-  const void *fn = spill ? (wide ? reinterpret_cast<const void *>(FA_KERNEL(true, true))
-                                 : reinterpret_cast<const void *>(FA_KERNEL(true, false)))
-                         : (wide ? reinterpret_cast<const void *>(FA_KERNEL(false, true))
-                                 : reinterpret_cast<const void *>(FA_KERNEL(false, false)));
-  ZX_TRY_HIP(hipLaunchCooperativeKernel(fn, dim3(G), dim3(FA_THREADS), args, 0, st));
+  const void *fn = fused_fn(spill, wide, rope ? (rope->inter ? FA_ROPE_PAIRS : FA_ROPE_HALF) : FA_ROPE_NONE);
+  const unsigned lds = rope ? (unsigned)fused_rope_lds(head_dim, rope->rot) : 0;
+  ZX_TRY_HIP(hipLaunchCooperativeKernel(fn, dim3(G), dim3(FA_THREADS), args, lds, st));
   return check_launch("kv_append_fused");
 }
 

@@ -175,6 +175,21 @@ ra_places_kernel(TokGeom g, int64_t limit, int64_t n_tok, TokPlace *places, int3
   places[t[0]] = TokPlace{(int32_t)page[0], (int32_t)pos[0]};
 }
 
+// The same as the single pass takes it: byte offsets into a layer's pool (-1: none) and positions.
+__global__ void __launch_bounds__(256)
+ra_offsets_kernel(TokGeom g, int64_t limit, int64_t n_tok, int64_t *tok_off, int32_t *tok_pos, int32_t *err) {
+  const int64_t t[1] = {(int64_t)blockIdx.x * 256 + threadIdx.x};
+  if (t[0] >= n_tok) return;
+  int64_t page[1], pos[1];
+  int32_t e = 0;
+  token_places<1>(g, g.cu_seqlens, g.start_pos, limit, t, n_tok, page, pos, e);
+  if (e && err) atomicOr(err, e);
+  tok_off[t[0]] = page[0] < 0 ? -1
+                              : page[0] * g.page_bytes +
+                                    (int64_t)((uint32_t)pos[0] % (uint32_t)g.page_size) * g.head_dim;
+  tok_pos[t[0]] = (int32_t)pos[0];
+}
+
 template <int U, bool LOCATE>
 __device__ __forceinline__ void ra_find(const TokGeom &tg, const TokStage &stage, int64_t limit, const TokPlace *places,
                                         const int64_t (&row)[U], int64_t n_tok, int64_t (&page)[U], int64_t (&pos)[U],
@@ -396,12 +411,27 @@ static bool ra_locates(int32_t n_layers, int64_t n_tok, int32_t n_heads, int32_t
   return ceil_div(n_tok, (int64_t)RA_U * ra_rows_per_block(n_heads, head_dim)) * n_layers <= RA_LOCATE_BPC * num_cus();
 }
 
+// Dynamic scales in one cooperative pass (zx_append_fused.hip)?  By the rule of the append that
+// does not rotate, if a share fits the registers.  Whole calls, 8 heads, D = 128, one / two
+// passes: 76,000 tokens x 2 layers 228 / 298 us, x 16 1485 / 2276; 37,000 (just under half the
+// registers) x 2 172 / 149, x 16 1074 / 1098; 19,000 x 16 1033 / 570.
+static bool ra_single_pass(int32_t n_layers, int64_t n_tok, int32_t n_heads, int32_t head_dim, int32_t flags) {
+  return !(flags & (ZX_APPEND_STATIC_SCALES | ZX_APPEND_TWO_PASS)) && append_fused_holds(n_tok, head_dim) &&
+         ((flags & ZX_APPEND_SINGLE_PASS) || append_fused_preferred(n_tok, head_dim, (int64_t)n_layers * 2 * n_heads));
+}
+static size_t ra_offsets_bytes(int64_t n_tok) {
+  return align256((size_t)n_tok * sizeof(int64_t)) + align256((size_t)n_tok * sizeof(int32_t));
+}
+
 extern "C" size_t zx_kv_rope_append_workspace_bytes(int32_t n_layers, int64_t n_tok, int32_t n_heads, int32_t head_dim,
                                                     int32_t flags) {
   if (n_layers <= 0 || n_tok <= 0 || n_heads <= 0 || head_dim < 8) return 0;
   const int64_t gx = std::max<int64_t>(1, ceil_div((int64_t)num_cus() * RA_BPC, n_layers));
-  return (ra_locates(n_layers, n_tok, n_heads, head_dim) ? 0 : align256((size_t)n_tok * sizeof(TokPlace))) +
-         (flags & ZX_APPEND_STATIC_SCALES ? 0 : align256((size_t)gx * n_layers * 2 * n_heads * sizeof(uint32_t)));
+  const size_t two = (ra_locates(n_layers, n_tok, n_heads, head_dim) ? 0 : align256((size_t)n_tok * sizeof(TokPlace))) +
+                     (flags & ZX_APPEND_STATIC_SCALES ? 0 : align256((size_t)gx * n_layers * 2 * n_heads * sizeof(uint32_t)));
+  return ra_single_pass(n_layers, n_tok, n_heads, head_dim, flags)
+             ? std::max(two, ra_offsets_bytes(n_tok) + append_fused_workspace_bytes(n_layers, n_heads))
+             : two;
 }
 
 extern "C" int zx_kv_rope_append(const uint16_t *x, int64_t x_layer_stride, int32_t n_layers, int64_t n_tok,
@@ -411,8 +441,11 @@ extern "C" int zx_kv_rope_append(const uint16_t *x, int64_t x_layer_stride, int3
                                  int64_t pool_layer_stride, int64_t n_pages, float *scales, int32_t flags, int32_t *err,
                                  void *workspace, size_t workspace_bytes, zx_stream_t stream) {
   clear_error();
-  ZX_REQUIRE(!(flags & ~(ZX_APPEND_STATIC_SCALES | ZX_APPEND_SATURATE | ZX_ROPE_INTERLEAVED)),
+  ZX_REQUIRE(!(flags & ~(ZX_APPEND_STATIC_SCALES | ZX_APPEND_SATURATE | ZX_APPEND_TWO_PASS | ZX_APPEND_SINGLE_PASS |
+                         ZX_ROPE_INTERLEAVED)),
              "kv_rope_append: unknown flag bits 0x%x", (unsigned)flags);
+  ZX_REQUIRE((flags & (ZX_APPEND_TWO_PASS | ZX_APPEND_SINGLE_PASS)) != (ZX_APPEND_TWO_PASS | ZX_APPEND_SINGLE_PASS),
+             "kv_rope_append: ZX_APPEND_TWO_PASS and ZX_APPEND_SINGLE_PASS together");
   const bool dynamic = !(flags & ZX_APPEND_STATIC_SCALES);
   ZX_REQUIRE(!(dynamic && (flags & ZX_APPEND_SATURATE)), "kv_rope_append: ZX_APPEND_SATURATE needs static scales");
   ZX_REQUIRE(scales && cu_seqlens && block_tables && pool && (x || n_tok == 0), "kv_rope_append: null pointer");
@@ -454,6 +487,18 @@ extern "C" int zx_kv_rope_append(const uint16_t *x, int64_t x_layer_stride, int3
   const TokGeom tg = {cu_seqlens, start_pos, block_tables, n_seqs, max_blocks, page_size, head_dim, n_pages, page_bytes};
   const int64_t limit = std::min((int64_t)max_blocks * page_size, n_pos);
   const bool locate = ra_locates(n_layers, n_tok, n_heads, head_dim);
+  const bool inter = flags & ZX_ROPE_INTERLEAVED;
+  if (ra_single_pass(n_layers, n_tok, n_heads, head_dim, flags)) {
+    int64_t *tok_off = static_cast<int64_t *>(workspace);
+    int32_t *tok_pos = reinterpret_cast<int32_t *>(static_cast<char *>(workspace) + align256((size_t)n_tok * sizeof(int64_t)));
+    ra_offsets_kernel<<<(unsigned)ceil_div(n_tok, 256), 256, 0, st>>>(tg, limit, n_tok, tok_off, tok_pos, err);
+    if ((rc = check_launch("ra_offsets"))) return rc;
+    const AppendRope ar = {table, rot_dim, inter, tok_pos};
+    rc = append_fused(x, x_layer_stride, n_layers, n_tok, n_heads, head_dim, tok_off, pool, pool_layer_stride, page_size,
+                      scales, err, static_cast<char *>(workspace) + ra_offsets_bytes(n_tok), st, &ar);
+    if (rc != ZX_ERR_UNSUPPORTED) return rc;
+    clear_error();  // this device cannot run the single-pass kernel: two passes below
+  }
   TokPlace *places = static_cast<TokPlace *>(workspace);
   uint32_t *part = reinterpret_cast<uint32_t *>(static_cast<char *>(workspace) +
                                                 (locate ? 0 : align256((size_t)n_tok * sizeof(TokPlace))));
@@ -461,7 +506,6 @@ extern "C" int zx_kv_rope_append(const uint16_t *x, int64_t x_layer_stride, int3
     ra_places_kernel<<<(unsigned)ceil_div(n_tok, 256), 256, 0, st>>>(tg, limit, n_tok, places, err);
     if ((rc = check_launch("ra_places"))) return rc;
   }
-  const bool inter = flags & ZX_ROPE_INTERLEAVED;
   const int threads = g.n_unit * g.rpb;
   if (dynamic) {
     const unsigned gx = (unsigned)ra_amax_grid_x(n_tok, g.rpb, n_layers);

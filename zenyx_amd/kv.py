@@ -977,7 +977,8 @@ def _append_args(x, cu_seqlens, block_tables, start_pos, err):
 def kv_rope_append(x: torch.Tensor, table: torch.Tensor, cu_seqlens: torch.Tensor, block_tables: torch.Tensor,
                    pool: torch.Tensor, scales: torch.Tensor | None = None, start_pos: torch.Tensor | None = None,
                    interleaved: bool = False, static_scales: bool = False, saturate: bool = False,
-                   check: bool = False, err: torch.Tensor | None = None) -> torch.Tensor:
+                   check: bool = False, err: torch.Tensor | None = None, two_pass: bool = False,
+                   single_pass: bool = False) -> torch.Tensor:
     """``kv_quant_append`` with the keys of ``x [L, n_tok, 2, H, D]`` rotated by their positions
     on the way: the codes and scales of ``rope`` on the keys followed by ``kv_quant_append``.
     ``table``: ``rope_table``; a token at a position it does not have is not stored (and
@@ -1002,11 +1003,14 @@ def kv_rope_append(x: torch.Tensor, table: torch.Tensor, cu_seqlens: torch.Tenso
         raise ValueError(f"scales must be float32 [{L}, 2, {H}]")
     if saturate and not static_scales:
         raise ValueError("saturate applies to static scales (dynamic scales never overflow)")
+    if two_pass and single_pass:
+        raise ValueError("kv_rope_append: two_pass and single_pass are exclusive")
     index = x.get_device()
     _all_on(index, x=x, table=table, cu_seqlens=cu_seqlens, block_tables=block_tables, pool=pool, scales=scales,
             start_pos=start_pos)
     flags = (N.ZX_APPEND_STATIC_SCALES if static_scales else 0) | (N.ZX_APPEND_SATURATE if saturate else 0) | \
-        (N.ZX_ROPE_INTERLEAVED if interleaved else 0)
+        (N.ZX_ROPE_INTERLEAVED if interleaved else 0) | (N.ZX_APPEND_TWO_PASS if two_pass else 0) | \
+        (N.ZX_APPEND_SINGLE_PASS if single_pass else 0)
     with _on(index):
         ws, nb = _workspace_for("zx_kv_rope_append_workspace_bytes", index, L, T, H, D, flags)
         err = _err_word_if(check, x.device) if err is None else err

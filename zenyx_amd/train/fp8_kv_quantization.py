@@ -120,7 +120,8 @@ class PagedFP8KVCache:
         saturate = (not dyn) and self.overflow == "saturate"
         if self.rope is not None:
             kv.kv_rope_append(x, self.rope.table, cu, tables, self.pool, scales=self.scales, start_pos=start_pos,
-                              interleaved=self.rope.interleaved, static_scales=not dyn, saturate=saturate, err=word)
+                              interleaved=self.rope.interleaved, static_scales=not dyn, saturate=saturate, err=word,
+                              single_pass=single_pass and dyn)
         else:
             kv.kv_quant_append(x, cu, tables, self.pool, scales=self.scales, start_pos=start_pos,
                                static_scales=not dyn, saturate=saturate, err=word, single_pass=single_pass and dyn)
@@ -266,8 +267,6 @@ class PagedFP8KVCache:
             self.check_errors()  # earlier appends first, so the word read below is this call's own
         start = [self.lengths.get(s, 0) for s in seq_ids]
         if self.rope is not None:
-            if single_pass:
-                raise ValueError("single_pass is for appends that do not rotate their keys")
             if any(st + n > self.rope.max_positions for st, n in zip(start, lengths)):
                 raise ValueError(f"a sequence would pass the {self.rope.max_positions} positions of the cache's rope")
         word = self._err[self._n_err:self._n_err + 1]
