@@ -400,11 +400,113 @@ def test_prefill_nan_reaches_only_rows_that_see_it(dev):
         pool = clean.copy()
         pool[bt[0, 1], kv_, 0, 0, 8 * D + 16 * 3 + 9] = 255  # block 3 (channels 96..128) of position 25
         got = run(pool)
-        assert torch.isnan(got[25:]).any(-1).all()
-        if kv_ == 0:
-            assert torch.equal(got[:25], want[:25])
-        else:  # weights of 0 times NaN may reach earlier rows of the same 32 keys, in its channels only
-            assert torch.equal(got[..., :96], want[..., :96]) and not torch.isnan(got[..., :96]).any()
+        assert torch.isnan(got[25:]).any(-1).all() and torch.equal(got[:25], want[:25])
+        if kv_:  # in its channels only
+            assert torch.equal(got[..., :96], want[..., :96]) and torch.isnan(got[25:, :, 96:]).all()
+
+
+@pytest.mark.parametrize("precision", ["bf16", "exact"])
+@pytest.mark.parametrize("rows, old, Hq, H, D", [([70], [9], 4, 2, 128), ([130], [40], 2, 2, 64), ([50], [3], 1, 1, 256),
+                                                 ([3, 2], [40, 17], 6, 2, 128), ([20], [0], 8, 4, 64)])
+def test_prefill_nan_values(dev, rows, old, Hq, H, D, precision):
+    """NaN blocks in every tenth position's values: NaN in the rows that see them, in their
+    channels, and the oracle's numbers everywhere else."""
+    P = 16
+    lens = [a + b for a, b in zip(rows, old)]
+    bt, n_pages = tables(lens, P, 0, D)
+    pool = random_pool(n_pages, H, P, D, D)
+    rng = np.random.default_rng(D)
+    for b, n in enumerate(lens):
+        for pos in range(n - min(rows[b], 40), n, 7):
+            pool[bt[b, pos // P], 1, rng.integers(H), 0, 8 * D + 16 * rng.integers(D // 32) + pos % 16] = 255
+    q = torch.randn((sum(rows), Hq, D), device=dev).to(torch.bfloat16)
+    cu = i32(np.concatenate([[0], np.cumsum(rows)]), dev)
+    got = kv.paged_attention4_prefill(q, cu, i32(old, dev), torch.from_numpy(pool).to(dev), i32(bt, dev), i32(lens, dev),
+                                      precision=precision).double().cpu().numpy()
+    qn, at = q.double().cpu().numpy(), 0
+    for b, n in enumerate(lens):
+        k, v = R.load(pool, bt[b], n, 0)[0], R.load(pool, bt[b], n, 1)[0]
+        for r in range(rows[b]):
+            see = old[b] + r + 1
+            for hq in range(Hq):
+                vh = v[hq * H // Hq][:see]
+                bad = np.isnan(vh).any(0)
+                assert np.array_equal(np.isnan(got[at + r, hq]), bad), (b, r, hq)
+                want, qk, vm = R.attend(qn[at + r:at + r + 1, hq], k[hq * H // Hq][:see], np.nan_to_num(vh),
+                                        np.ones((1, see), bool), D ** -0.5)
+                ok = ~bad
+                check_rows(got[at + r:at + r + 1, hq][:, ok], want[:, ok], qk, vm[ok], see, D, D ** -0.5,
+                           2.0 ** -16 if precision == "exact" else 2.0 ** -8)
+        at += rows[b]
+
+
+def test_prefill_of_many_short_sequences(dev):
+    """More than 64 sequences of 0 to 6 rows: dealt by a table, in runs and whole."""
+    H, Hq, D, P = 2, 8, 128, 16
+    rng = np.random.default_rng(2)
+    for n_seqs, longest in ((70, 900), (65, 60)):
+        rows = rng.integers(0, 7, n_seqs).tolist()
+        old = rng.integers(0, longest, n_seqs).tolist()
+        lens = [a + b for a, b in zip(rows, old)]
+        bt, n_pages = tables(lens, P, 0, 1)
+        pool = random_pool(n_pages, H, P, D, 1)
+        q = torch.randn((sum(rows) + 1, Hq, D), device=dev).to(torch.bfloat16)
+        out = torch.full_like(q, 5.0)
+        cu = i32(np.concatenate([[0], np.cumsum(rows)]), dev)
+        kv.paged_attention4_prefill(q, cu, i32(old, dev), torch.from_numpy(pool).to(dev), i32(bt, dev), i32(lens, dev),
+                                    precision="exact", out=out, check=True)
+        assert torch.all(out[-1] == 5)
+        check_attention(out, q, pool, bt, lens, D ** -0.5, 2.0 ** -16, rows, old, True)
+
+
+@pytest.mark.parametrize("sm", [0.0, -0.3, 1e-6, 4.0])
+def test_prefill_scales(dev, sm):
+    for rows, old, Hq, H, D in (([3, 1], [90, 20], 4, 2, 128), ([60], [10], 4, 4, 64)):
+        lens = [a + b for a, b in zip(rows, old)]
+        bt, n_pages = tables(lens, 16, 0, 3)
+        pool = random_pool(n_pages, H, 16, D, 3)
+        q = torch.randn((sum(rows), Hq, D), device=dev).to(torch.bfloat16)
+        cu = i32(np.concatenate([[0], np.cumsum(rows)]), dev)
+        got = kv.paged_attention4_prefill(q, cu, i32(old, dev), torch.from_numpy(pool).to(dev), i32(bt, dev),
+                                          i32(lens, dev), sm_scale=sm, precision="exact", check=True)
+        check_attention(got, q, pool, bt, lens, sm, 2.0 ** -16, rows, old, True)
+
+
+@pytest.mark.parametrize("n, most, Hq, H", [(70, 50, 4, 4), (70, 70, 4, 1), (6, 4, 8, 2)])
+def test_prefill_computes_no_other_rows(dev, n, most, Hq, H):
+    """Rows beyond max_q_per_seq, and rows that cu_q claims and q does not have."""
+    D, P = 128, 16
+    bt, n_pages = tables([n + 30], P, 0, 6)
+    pool = random_pool(n_pages, H, P, D, 6)
+    back = torch.randn((n + 40, Hq, D), device=dev).to(torch.bfloat16)
+    for claimed in (n, n + 30):
+        out = torch.full_like(back, 5.0)
+        err = torch.zeros(1, dtype=torch.int32, device=dev)
+        kv.paged_attention4_prefill(back[:n], i32([0, claimed], dev), i32([20], dev), torch.from_numpy(pool).to(dev),
+                                    i32(bt, dev), i32([n + 20], dev), max_q_per_seq=most, out=out[:n], err=err)
+        assert torch.all(out[most:] == 5) and err.item() == (N.ZX_KERR_POS_RANGE if claimed > most else 0)
+        check_attention(out[:most], back, pool, bt, [n + 20], D ** -0.5, 2.0 ** -8, [most], [20], True)
+
+
+def test_two_calls_at_once(dev):
+    """Calls on two streams, workspaces and all, do not meet."""
+    Hq, H, D, P = 32, 8, 128, 16
+    made = []
+    for seed in range(2):
+        lens = [3000 + 500 * seed, 100]
+        bt, n_pages = tables(lens, P, 0, seed)
+        pool = random_pool(n_pages, H, P, D, seed)
+        q = torch.randn((2, Hq, D), device=dev).to(torch.bfloat16)
+        made.append((q, torch.from_numpy(pool).to(dev), i32(bt, dev), i32(lens, dev)))
+    want = [kv.paged_attention4_decode(*a) for a in made]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in made], [[], []]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(kv.paged_attention4_decode(*made[i]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, w) for w, many in zip(want, got) for g in many)
 
 
 def test_refusals(dev):

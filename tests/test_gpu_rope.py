@@ -357,21 +357,23 @@ def test_append_of_nothing_and_refusals(dev):
             bad()
 
 
-def test_append_in_a_graph(dev):
+@pytest.mark.parametrize("single", [False, True])
+def test_append_in_a_graph(dev, single):
     """Captured appends (two graphs, each with its own workspace) replay to the eager bits."""
     H, D, P, L = 4, 128, 16, 2
     lens, old = [40, 3], [0, 20]
     bt, cu, start, n_pages = paged(lens, old, P, 0, dev, 1)
     table = table64(64, D, dev)
     x = torch.randn((L, 43, 2, H, D), device=dev).to(torch.bfloat16)
-    kv.kv_rope_append(x, table, cu, bt, torch.zeros((L, n_pages, 2, H, P, D), dtype=torch.uint8, device=dev), start_pos=start)
+    kv.kv_rope_append(x, table, cu, bt, torch.zeros((L, n_pages, 2, H, P, D), dtype=torch.uint8, device=dev), start_pos=start,
+                      single_pass=single)
     pools = [torch.zeros((L, n_pages, 2, H, P, D), dtype=torch.uint8, device=dev) for _ in range(2)]
     scales = [torch.zeros((L, 2, H), device=dev) for _ in range(2)]
     graphs = []
     for pool, sc in zip(pools, scales):
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g):
-            kv.kv_rope_append(x, table, cu, bt, pool, scales=sc, start_pos=start)
+            kv.kv_rope_append(x, table, cu, bt, pool, scales=sc, start_pos=start, single_pass=single)
         graphs.append(g)
     for i in range(3):
         x.copy_(torch.randn(x.shape, device=dev))

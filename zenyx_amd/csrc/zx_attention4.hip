@@ -211,8 +211,30 @@ template <int D, int CT, bool EXACT> struct A4Wave {
     }
   }
 
+  // A weight of 0 times a NaN is one, so on a step that some column does not see to its end the
+  // values' NaN blocks go into the products as zeros, and are put into the accumulators of the
+  // columns that see them here.  bad: lanes (n, kg) whose block i of token t + n is NaN.
+  __device__ __forceinline__ void nan_values(uint64_t bad, int i, uint32_t t) {
+    constexpr int GROUPS = D == 64 ? 2 : 4;
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      const uint32_t seen = (1u << (lim[ct] > t ? min(lim[ct] - t, (uint32_t)K4_TOK) : 0u)) - 1u;
+#pragma unroll
+      for (int j = 0; j < GROUPS; ++j) {
+        const uint32_t tokens = (uint32_t)(bad >> (D == 64 ? 32 * j : 16 * j)) & 0xFFFFu;
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int jt = 2 * ((D == 256 && i ? 4 : 0) + j) + half;
+            if (tokens & seen) o[ct][jt][k] = __uint_as_float(0x7FC00000u);
+          }
+      }
+    }
+  }
+
   // V rows into LDS; tokens past the last one as zeros (what a page holds there may be NaN).
-  __device__ __forceinline__ void store_v(const A4Tile<D> (&v)[2], const int (&rows)[2]) {
+  __device__ __forceinline__ void store_v(uint32_t t0, const A4Tile<D> (&v)[2], const int (&rows)[2]) {
 #pragma unroll
     for (int T = 0; T < 2; ++T) {
       A4Tile<D> t = v[T];
@@ -221,6 +243,16 @@ template <int D, int CT, bool EXACT> struct A4Wave {
         for (int w = 0; w < A4Tile<D>::CW; ++w) t.c[w] = n < rows[T] ? t.c[w] : 0u;
 #pragma unroll
         for (int i = 0; i < A4Tile<D>::NB; ++i) t.p[i] = n < rows[T] ? t.p[i] : 127u;
+      }
+      if (t0 + A4_STEP > lim_all) {  // uniform
+#pragma unroll
+        for (int i = 0; i < A4Tile<D>::NB; ++i) {
+          const uint64_t bad = __builtin_amdgcn_ballot_w64(t.p[i] == K4_NAN);
+          if (bad) {
+            nan_values(bad, i, t0 + K4_TOK * T);
+            t.p[i] = t.p[i] == K4_NAN ? 127u : t.p[i];
+          }
+        }
       }
 #pragma unroll
       for (int w = 0; w < A4Tile<D>::CW; ++w)
@@ -365,7 +397,7 @@ template <int D, int CT, bool EXACT> struct A4Wave {
     }
     if constexpr (AHEAD) {
       auto compute = [&](const Step &x) {
-        store_v(x.v, x.rows);
+        store_v(t0, x.v, x.rows);
         scores(x.k, s);
         mask(t0, x.rows, s);
         raise(s);
@@ -390,7 +422,7 @@ template <int D, int CT, bool EXACT> struct A4Wave {
       while (t0 < t_end) {
         scores(now.k, s);
         __builtin_amdgcn_sched_barrier(0);
-        store_v(now.v, now.rows);
+        store_v(t0, now.v, now.rows);
         mask(t0, now.rows, s);
         __builtin_amdgcn_sched_barrier(0);
         t0 += stride;
@@ -453,7 +485,14 @@ struct A4Rows {
   const int32_t *cu_q, *q_pos0;
   int32_t most;    // rows of a sequence that are computed
   int32_t causal;
+  int64_t n_q;     // rows that there are
 };
+
+// Rows [lo, hi) of a sequence that are computed: at most `most`, and none outside [0, n_q).
+__device__ __forceinline__ int32_t a4_rows(int64_t lo, int64_t hi, int64_t n_q, int64_t most, int32_t &e) {
+  if (lo < 0 || hi > n_q || hi - lo > most) e |= ZX_KERR_POS_RANGE;
+  return lo < 0 ? 0 : (int32_t)max((int64_t)0, min(min(hi, n_q) - lo, most));
+}
 
 // Sequences dealt in equal runs (att_locate).  Up to 16 CT columns: the (query row, head) pairs of
 // one sequence and KV head's group.  g.group heads per block at most; the last group of a KV
@@ -488,9 +527,7 @@ paged_decode4_kernel(const uint16_t *__restrict__ q, AttnGeom g, A4Rows qr, cons
     row0 = b;
     if constexpr (!ROWS) return 1;
     row0 = qr.cu_q[b];
-    const int64_t n = (int64_t)qr.cu_q[b + 1] - row0;
-    if (n > qr.most) w.e |= ZX_KERR_POS_RANGE;
-    return (int)max((int64_t)0, min(n, (int64_t)qr.most));
+    return a4_rows(row0, qr.cu_q[b + 1], qr.n_q, qr.most, w.e);
   };
   auto zero_rows = [&](int b) {  // an empty sequence
     int64_t row0;
@@ -568,10 +605,10 @@ decode4_rows_combine_kernel(const float *__restrict__ part, AttnGeom g, A4Rows q
   const uint32_t row_all = blockIdx.x / (uint32_t)g.n_q_heads;
   const int hq = (int)(blockIdx.x - row_all * (uint32_t)g.n_q_heads);
   const int b = a4_seq_of(qr.cu_q, g.n_seqs, (int32_t)row_all);
-  const int64_t r = (int64_t)row_all - qr.cu_q[b];
-  int32_t x0, n_live;
+  int32_t x0, n_live, e = 0;
+  const int64_t lo = qr.cu_q[b], r = (int64_t)row_all - lo;
   att_live(g, seq_lens, table, b, x0, n_live);
-  if (r < 0 || r >= qr.most || (int32_t)row_all >= qr.cu_q[b + 1] || n_live == 1) return;
+  if (r < 0 || r >= a4_rows(lo, qr.cu_q[b + 1], qr.n_q, qr.most, e) || n_live == 1) return;
   const float *pp = part + ((r * g.n_q_heads + hq) * ((int64_t)g.n_run + g.n_seqs) + x0 + b) * (2 + D);
   out[(int64_t)blockIdx.x * D + threadIdx.x] = att_combine_row(pp, 2 + D, n_live, threadIdx.x, 1.0f);
 }
@@ -599,7 +636,7 @@ struct Prefill4Args {
   int32_t rows;            // query rows per tile: 16 CT / group
   int32_t n_rt, n_split;   // row tiles per sequence, the most blocks per tile
   uint32_t n_items;        // tiles: n_rt * n_group * n_seqs
-  int64_t max_rows;        // n_rt * rows
+  int64_t max_q, n_q;      // rows of a sequence that are computed at most; rows of q
   uint32_t p_magic;
   int32_t p_shift;
   float sm_log2e;
@@ -631,10 +668,11 @@ __global__ void __launch_bounds__(ATT_THREADS, a4_per_cu(D, CT)) paged_prefill4_
   const int G = min(a.group, grp - first), hq0 = h * grp + first;
   const int32_t lo = a.cu_q[b], hi = a.cu_q[b + 1], kv_len = a.kv_len[b];
   const int64_t pos0 = a.q_pos0[b];
-  int32_t e = rt_rev == 0 && (int64_t)hi - lo > a.max_rows ? ZX_KERR_POS_RANGE : 0;
+  int32_t e = 0;
+  const int32_t rows = a4_rows(lo, hi, a.n_q, a.max_q, e);
   if (kv_len > (int64_t)a.max_blocks * a.page_size) e |= ZX_KERR_POS_RANGE;
   const int64_t row0 = ((int64_t)a.n_rt - 1 - rt_rev) * a.rows;
-  const int n_rows = (int)max((int64_t)0, min((int64_t)a.rows, (int64_t)hi - lo - row0));
+  const int n_rows = (int)max((int64_t)0, min((int64_t)a.rows, rows - row0));
   const uint32_t end = p4_keys(a, kv_len, pos0, row0 + n_rows);
   const int parts = p4_parts(a, end);
   if (n_rows == 0 || split >= parts) {  // block-uniform
@@ -706,8 +744,10 @@ __global__ void __launch_bounds__(D) prefill4_combine_kernel(Prefill4Args a, int
   const uint32_t row_all = blockIdx.x / (uint32_t)a.n_q_heads;
   const int hq = (int)(blockIdx.x - row_all * (uint32_t)a.n_q_heads);
   const int b = a4_seq_of(a.cu_q, a.n_seqs, (int32_t)row_all);
-  const int64_t q_lo = a.cu_q[b], rows = a.cu_q[b + 1] - q_lo, row = (int64_t)row_all - q_lo;
-  if (row < 0 || row >= rows || row >= a.max_rows) return;  // in no sequence, or not computed
+  int32_t e = 0;
+  const int64_t q_lo = a.cu_q[b], row = (int64_t)row_all - q_lo;
+  const int64_t rows = a4_rows(q_lo, a.cu_q[b + 1], a.n_q, a.max_q, e);
+  if (row < 0 || row >= rows) return;  // in no sequence, or not computed
   const int grp = a.n_q_heads / a.n_kv_heads, per_kv = a.n_group / a.n_kv_heads;
   const int h = hq / grp, sub = (hq - h * grp) / a.group, first = sub * a.group;
   const int G = min(a.group, grp - first);
@@ -792,7 +832,7 @@ extern "C" int zx_paged_attention4_decode(const uint16_t *q, int32_t n_q_heads, 
   g.group = (int32_t)ceil_div(grp, a4_groups(grp));
   g.n_group = n_kv_heads * a4_groups(grp);
   ZX_REQUIRE(p.n_blk * g.n_group < (1LL << 31), "paged_attention4_decode: too many sequences or heads");
-  const A4Rows qr = {nullptr, nullptr, 1, 0};
+  const A4Rows qr = {nullptr, nullptr, 1, 0, n_seqs};
   const hipStream_t st = as_stream(stream);
   switch (head_dim) {
     case 64: return a4_launch_runs<64, 1, true, false>(p, g, qr, n_seqs, q, pool, block_tables, seq_lens, out, err, workspace, st);
@@ -889,7 +929,7 @@ extern "C" int zx_paged_attention4_prefill(const uint16_t *q, int64_t n_q, const
     AttnGeom g = att_geom(p.deal, n_seqs, n_q_heads, n_kv_heads, head_dim, max_blocks, page_size, n_pages, sm_scale);
     g.group = p.group;
     g.n_group = p.n_group;
-    const A4Rows qr = {cu_q, q_pos0, max_q_per_seq, causal ? 1 : 0};
+    const A4Rows qr = {cu_q, q_pos0, max_q_per_seq, causal ? 1 : 0, n_q};
 #define ZX_A4_RUNS(D, CT, EX) \
   a4_launch_runs<D, CT, EX, true>(p.deal, g, qr, n_q, q, pool, block_tables, kv_len, out, err, workspace, st)
     switch (head_dim) {
@@ -926,7 +966,8 @@ extern "C" int zx_paged_attention4_prefill(const uint16_t *q, int64_t n_q, const
   a.n_group = p.n_group;
   a.rows = p.rows;
   a.n_rt = (int32_t)p.n_rt;
-  a.max_rows = p.n_rt * p.rows;
+  a.max_q = max_q_per_seq;
+  a.n_q = n_q;
   a.sm_log2e = sm_scale * ATT_LOG2E;
   a.n_split = room && !p.runs ? (int32_t)p.n_split : 1;
   {
