@@ -758,9 +758,12 @@ static AttnPlan att_plan(int32_t n_seqs, int32_t n_q_heads, int32_t n_kv_heads, 
   // More runs than resident blocks leave a second, partly filled round: 16 x 1k-8k 37 against
   // 31 us at three per CU.
   const int64_t resident = ((p.mfma ? head_dim == 64 : p.group == 1 && head_dim < 256) ? 3LL : 2LL) * num_cus();
-  static_cast<AttnRuns &>(p) = att_runs(n_seqs, n_q_heads / p.group, resident,
-                                        ATT_WAVES * (p.mfma ? AM_STEP : ATT_U * 64 / (head_dim / 16)), max_blocks,
-                                        page_size);
+  // Whole sequences, in a graph, Hq 32 / Hkv 8, D = 128, tables of 32k positions: 512 x 100-500
+  // 139 us in runs, 90 whole; 4 x 100-500 10.9 in runs, 16.3 whole; 64 x 512-4k 59 in runs, 73
+  // whole.
+  const int32_t unit = ATT_WAVES * (p.mfma ? AM_STEP : ATT_U * 64 / (head_dim / 16));
+  const AttnSlack slack = {8, 2, 1, std::max<uint32_t>(1, 1024u / unit), 0};
+  static_cast<AttnRuns &>(p) = att_runs(n_seqs, n_q_heads / p.group, resident, unit, max_blocks, page_size, slack);
   return p;
 }
 

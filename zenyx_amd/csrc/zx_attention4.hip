@@ -597,20 +597,23 @@ paged_decode4_kernel(const uint16_t *__restrict__ q, AttnGeom g, A4Rows qr, cons
   if (w.e && err) atomicOr(err, w.e);
 }
 
-// Pass 2 of a call with several rows per sequence: a block of D threads per (row, head).
+// Pass 2 of a call with several rows per sequence: a block per (sequence, head), D threads per row.
 template <int D>
-__global__ void __launch_bounds__(D)
+__global__ void __launch_bounds__(1024)
 decode4_rows_combine_kernel(const float *__restrict__ part, AttnGeom g, A4Rows qr, const int32_t *__restrict__ seq_lens,
                             uint16_t *__restrict__ out, void *table) {
-  const uint32_t row_all = blockIdx.x / (uint32_t)g.n_q_heads;
-  const int hq = (int)(blockIdx.x - row_all * (uint32_t)g.n_q_heads);
-  const int b = a4_seq_of(qr.cu_q, g.n_seqs, (int32_t)row_all);
+  const int b = (int)(blockIdx.x / (uint32_t)g.n_q_heads);
+  const int hq = (int)(blockIdx.x - (uint32_t)b * (uint32_t)g.n_q_heads);
   int32_t x0, n_live, e = 0;
-  const int64_t lo = qr.cu_q[b], r = (int64_t)row_all - lo;
   att_live(g, seq_lens, table, b, x0, n_live);
-  if (r < 0 || r >= a4_rows(lo, qr.cu_q[b + 1], qr.n_q, qr.most, e) || n_live == 1) return;
-  const float *pp = part + ((r * g.n_q_heads + hq) * ((int64_t)g.n_run + g.n_seqs) + x0 + b) * (2 + D);
-  out[(int64_t)blockIdx.x * D + threadIdx.x] = att_combine_row(pp, 2 + D, n_live, threadIdx.x, 1.0f);
+  if (n_live == 1) return;
+  const int64_t lo = qr.cu_q[b];
+  const int32_t rows = a4_rows(lo, qr.cu_q[b + 1], qr.n_q, qr.most, e);
+  const int d = threadIdx.x % D;
+  for (int r = threadIdx.x / D; r < rows; r += blockDim.x / D) {
+    const float *pp = part + (((int64_t)r * g.n_q_heads + hq) * ((int64_t)g.n_run + g.n_seqs) + x0 + b) * (2 + D);
+    out[((lo + r) * g.n_q_heads + hq) * D + d] = att_combine_row(pp, 2 + D, n_live, d, 1.0f);
+  }
 }
 
 // Blocks of queries.  A block takes a tile of the (query row, head) columns of one sequence and KV
@@ -770,11 +773,22 @@ using namespace zx;
 // Query heads per block: as few groups of at most 16 as there can be, of equal size but the last.
 static int32_t a4_groups(int32_t grp) { return (int32_t)ceil_div(grp, A4_HEADS); }
 
+// When sequences are dealt whole.  In a graph, Hq 32 / Hkv 8, D = 128, in runs / whole: 64 x 100-600
+// keys 17.9 / 15.1 us, 64 x 1,000-1,200 26 / 22, 128 x 1,000-1,200 44 / 38; the other way 16 x
+// 1,000-1,200 14.9 / 17, 64 x 200-4k 36 / 46, 64 x 100-16k 102 / 158, 256 x 100-16k 410 / 447.
+// Several rows per sequence, whose start costs more (4 rows, 64 x 200-4k 53 / 50, 128 x 200-4k
+// 85 / 78; the other way 64 x 100-16k 133 / 150).  As many sequences as runs or more and none
+// above 8 units: whole whatever their lengths, without the launches for the other way of
+// dealing (128 x 100-600, 12 heads, D = 64, tables of 600: 22.5 us, without them 16.0).
+constexpr AttnSlack A4_SLACK = {20, 2, 5, 8, 8}, A4_SLACK_ROWS = {20, 2, 12, 8, 32};
 // Sequences in equal runs: one row each (columns <= 16), or as many rows as a block's columns hold.
 static AttnRuns a4_plan(int32_t n_seqs, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim, int32_t max_blocks,
-                        int32_t page_size, int ct) {
+                        int32_t page_size, int ct, const AttnSlack &slack) {
   const int64_t groups = (int64_t)n_kv_heads * a4_groups(n_q_heads / n_kv_heads);
-  return att_runs(n_seqs, groups, std::min(a4_per_cu(head_dim, ct), head_dim == 64 ? 4 : 3) * (int64_t)num_cus(), P4_UNIT, max_blocks, page_size);
+  // at D = 128 three blocks per CU though four fit: 1 x 32k positions 20.4 us against 23.6, 4 x
+  // 100-16k 19.2 against 21.7, 32 x 32k 199 against 197
+  const int64_t resident = std::min(a4_per_cu(head_dim, ct), head_dim == 64 ? 4 : 3) * (int64_t)num_cus();
+  return att_runs(n_seqs, groups, resident, P4_UNIT, max_blocks, page_size, slack);
 }
 
 static bool a4_dims_ok(int32_t n_seqs, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim, int32_t max_blocks,
@@ -786,13 +800,13 @@ static bool a4_dims_ok(int32_t n_seqs, int32_t n_q_heads, int32_t n_kv_heads, in
 extern "C" size_t zx_paged_attention4_decode_workspace_bytes(int32_t n_seqs, int32_t n_q_heads, int32_t n_kv_heads,
                                                              int32_t head_dim, int32_t max_blocks, int32_t page_size) {
   if (!a4_dims_ok(n_seqs, n_q_heads, n_kv_heads, head_dim, max_blocks, page_size)) return 0;
-  return att_workspace_bytes(a4_plan(n_seqs, n_q_heads, n_kv_heads, head_dim, max_blocks, page_size, 1), n_seqs,
+  return att_workspace_bytes(a4_plan(n_seqs, n_q_heads, n_kv_heads, head_dim, max_blocks, page_size, 1, A4_SLACK), n_seqs,
                              n_q_heads, head_dim);
 }
 
 // Launches the runs of a plan; part and table lie in the workspace.
 template <int D, int CT, bool EXACT, bool ROWS>
-static int a4_launch_runs(const AttnRuns &p, const AttnGeom &g, const A4Rows &qr, int64_t n_q, const uint16_t *q,
+static int a4_launch_runs(const AttnRuns &p, const AttnGeom &g, const A4Rows &qr, const uint16_t *q,
                           const uint8_t *pool, const int32_t *bt, const int32_t *lens, uint16_t *out, int32_t *err,
                           void *workspace, hipStream_t st) {
   float *part = static_cast<float *>(workspace);
@@ -804,7 +818,8 @@ static int a4_launch_runs(const AttnRuns &p, const AttnGeom &g, const A4Rows &qr
   if ((rc = check_launch("paged_decode4"))) return rc;
   if (!ROWS) return att_combine(part, g, nullptr, lens, out, table, st);
   if (g.whole) return ZX_OK;
-  decode4_rows_combine_kernel<D><<<(unsigned)(n_q * g.n_q_heads), D, 0, st>>>(part, g, qr, lens, out, table);
+  decode4_rows_combine_kernel<D><<<(unsigned)(g.n_seqs * g.n_q_heads), D * std::min(1024 / D, qr.most), 0, st>>>(
+      part, g, qr, lens, out, table);
   return check_launch("decode4_rows_combine");
 }
 
@@ -826,7 +841,7 @@ extern "C" int zx_paged_attention4_decode(const uint16_t *q, int32_t n_q_heads, 
       zx_paged_attention4_decode_workspace_bytes(n_seqs, n_q_heads, n_kv_heads, head_dim, max_blocks, page_size);
   if (!workspace || workspace_bytes < need)
     return fail(ZX_ERR_WORKSPACE, "paged_attention4_decode: workspace %zu < %zu bytes", workspace_bytes, need);
-  const AttnRuns p = a4_plan(n_seqs, n_q_heads, n_kv_heads, head_dim, max_blocks, page_size, 1);
+  const AttnRuns p = a4_plan(n_seqs, n_q_heads, n_kv_heads, head_dim, max_blocks, page_size, 1, A4_SLACK);
   AttnGeom g = att_geom(p, n_seqs, n_q_heads, n_kv_heads, head_dim, max_blocks, page_size, n_pages, sm_scale);
   const int32_t grp = n_q_heads / n_kv_heads;
   g.group = (int32_t)ceil_div(grp, a4_groups(grp));
@@ -835,9 +850,9 @@ extern "C" int zx_paged_attention4_decode(const uint16_t *q, int32_t n_q_heads, 
   const A4Rows qr = {nullptr, nullptr, 1, 0, n_seqs};
   const hipStream_t st = as_stream(stream);
   switch (head_dim) {
-    case 64: return a4_launch_runs<64, 1, true, false>(p, g, qr, n_seqs, q, pool, block_tables, seq_lens, out, err, workspace, st);
-    case 128: return a4_launch_runs<128, 1, true, false>(p, g, qr, n_seqs, q, pool, block_tables, seq_lens, out, err, workspace, st);
-    default: return a4_launch_runs<256, 1, true, false>(p, g, qr, n_seqs, q, pool, block_tables, seq_lens, out, err, workspace, st);
+    case 64: return a4_launch_runs<64, 1, true, false>(p, g, qr, q, pool, block_tables, seq_lens, out, err, workspace, st);
+    case 128: return a4_launch_runs<128, 1, true, false>(p, g, qr, q, pool, block_tables, seq_lens, out, err, workspace, st);
+    default: return a4_launch_runs<256, 1, true, false>(p, g, qr, q, pool, block_tables, seq_lens, out, err, workspace, st);
   }
 }
 
@@ -861,11 +876,11 @@ static Prefill4Plan p4_plan(int32_t n_q_heads, int32_t n_kv_heads, int32_t head_
   p.rows = 16 * p.ct / p.group;
   p.n_rt = ceil_div(max_q, p.rows);
   p.items = p.n_rt * p.n_group * n_seqs;
-  p.runs = p.n_rt == 1 && n_seqs <= 65535;
-  p.deal = a4_plan(n_seqs, n_q_heads, n_kv_heads, head_dim, max_blocks, page_size, p.ct);
+  p.deal = a4_plan(n_seqs, n_q_heads, n_kv_heads, head_dim, max_blocks, page_size, p.ct, A4_SLACK_ROWS);
   // parts of a tile where the tiles do not fill the chip
   const int64_t units = ceil_div((int64_t)max_blocks * page_size, P4_UNIT);
   const int64_t resident = (int64_t)a4_per_cu(head_dim, p.ct) * num_cus();
+  p.runs = p.n_rt == 1 && p.items < 4 * resident;
   p.n_split = std::max<int64_t>(1, std::min<int64_t>({units / 2, resident / p.items, 64}));
   return p;
 }
@@ -931,7 +946,7 @@ extern "C" int zx_paged_attention4_prefill(const uint16_t *q, int64_t n_q, const
     g.n_group = p.n_group;
     const A4Rows qr = {cu_q, q_pos0, max_q_per_seq, causal ? 1 : 0, n_q};
 #define ZX_A4_RUNS(D, CT, EX) \
-  a4_launch_runs<D, CT, EX, true>(p.deal, g, qr, n_q, q, pool, block_tables, kv_len, out, err, workspace, st)
+  a4_launch_runs<D, CT, EX, true>(p.deal, g, qr, q, pool, block_tables, kv_len, out, err, workspace, st)
     switch (head_dim) {
       case 64:
         return p.ct == 1   ? ZX_A4_RUNS(64, 1, true)

@@ -16,7 +16,7 @@ struct AttnGeom {
   int32_t n_q_heads, n_kv_heads, head_dim, page_size, max_blocks, n_seqs;
   int32_t n_run;        // equal runs, one block per head group each
   uint32_t unit, cap;   // positions per unit (a power of two); positions a block table holds
-  uint32_t tail;        // see att_take_whole
+  uint32_t tail, part, more;  // see att_take_whole
   int32_t whole;        // every sequence is taken whole: known to the host
   int32_t group, n_group;       // query heads per block; groups of them
   uint32_t p_magic;  // t / page_size = (t * p_magic) >> (31 + p_shift) for t < 2^31
@@ -48,16 +48,12 @@ template <typename T> struct AttnDeal {
 
 // Whole sequences instead of equal runs?  A run starts anew in every sequence that it touches
 // (q, the first page ids, K and V one after the other: about as long as four units) and its
-// parts are merged; whole sequences leave blocks idle while the longest one ends.  With as many
-// sequences as runs or more, where most runs would start anew anyway: if the longest one has
-// at most ATT_TAIL_MANY positions and an eighth of an equal share.  Else if it exceeds a share
-// by at most ATT_TAIL_ONE units.  (g.tail: that slack in units; a call whose longest sequence
-// is within it needs no sums.)  In a graph, Hq 32 / Hkv 8, D = 128, tables of 32k positions:
-// 512 x 100-500 139 us in runs, 90 whole; 4 x 100-500 10.9 in runs, 16.3 whole; 64 x 512-4k
-// 59 in runs, 73 whole.
-constexpr uint32_t ATT_TAIL_ONE = 2, ATT_TAIL_MANY = 1024;
+// parts are merged; whole sequences leave blocks idle while the longest one ends.  So: if the
+// longest one has at most tail units beyond the lesser of part / 8 of an equal share and a share
+// and `more` (a call whose longest sequence is within the tail needs no sums).  The figures are
+// the kernels' (AttnSlack).
 __device__ __forceinline__ bool att_take_whole(const AttnGeom &g, uint64_t most, uint64_t share) {
-  return most <= g.tail + (g.n_seqs < g.n_run ? share : share / 8);
+  return most <= g.tail + min(share * g.part / 8, share + g.more);
 }
 
 // Inclusive sum over the lanes below n (n <= 64, uniform).
@@ -274,15 +270,20 @@ __device__ __forceinline__ uint16_t att_combine_row(const float *pp, int64_t ste
 struct AttnRuns {
   bool whole;
   int32_t unit;
-  uint32_t tail;
+  uint32_t tail, part, more;
   int64_t n_run, n_blk;
+};
+// When a kernel takes whole sequences (att_take_whole): with fewer sequences than runs, and with
+// as many or more, where most runs would start anew anyway.
+struct AttnSlack {
+  uint32_t part_few, tail_few, part_many, tail_many, more;
 };
 // resident: blocks that the chip holds at once, one equal run each.  A number of groups that
 // leaves a part of the CUs without a run takes up to four rounds of shorter ones where those
 // fill the chip by 5% more (152 groups: 3 runs on 456 of 512, or 10 in three rounds: 16 x
 // 1k-8k, 19 heads per kv head, D = 128 371 -> 311 us, D = 64 221 -> 164).
 inline AttnRuns att_runs(int32_t n_seqs, int64_t groups, int64_t resident, int32_t unit, int32_t max_blocks,
-                         int32_t page_size) {
+                         int32_t page_size, const AttnSlack &slack) {
   AttnRuns p;
   p.unit = unit;
   // units of the longest sequence there can be (lengths are int32)
@@ -297,7 +298,9 @@ inline AttnRuns att_runs(int32_t n_seqs, int64_t groups, int64_t resident, int32
     }
   }
   p.n_run = std::min(seq_units * n_seqs, slots);
-  p.tail = n_seqs >= p.n_run ? std::max<uint32_t>(1, ATT_TAIL_MANY / p.unit) : ATT_TAIL_ONE;
+  p.tail = n_seqs >= p.n_run ? slack.tail_many : slack.tail_few;
+  p.part = n_seqs >= p.n_run ? slack.part_many : slack.part_few;
+  p.more = slack.more;
   // Whole sequences whatever their lengths, without the merge's launch: one unit each, or at
   // most 512 positions where they fill half the chip (32 x 100-500: 10.2 us, in runs 17), or
   // so short that att_take_whole() says so anyway (128 x 100-600, 12 heads, D = 64: 26 -> 19).
@@ -325,6 +328,8 @@ inline AttnGeom att_geom(const AttnRuns &p, int32_t n_seqs, int32_t n_q_heads, i
   g.n_seqs = n_seqs;
   g.n_run = (int32_t)p.n_run;
   g.tail = p.tail;
+  g.part = p.part;
+  g.more = p.more;
   g.unit = (uint32_t)p.unit;
   g.cap = (uint32_t)std::min((int64_t)max_blocks * page_size, (int64_t)INT32_MAX);
   g.whole = p.whole ? 1 : 0;
