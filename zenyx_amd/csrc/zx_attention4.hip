@@ -636,6 +636,7 @@ struct Prefill4Args {
   int64_t n_pages;
   int32_t n_q_heads, n_kv_heads, page_size, max_blocks, n_seqs, causal;
   int32_t group, n_group;  // heads per block, groups of them
+  int32_t by_length;       // tiles of the longest sequence first (one part per tile, 2 to 64 sequences)
   int32_t rows;            // query rows per tile: 16 CT / group
   int32_t n_rt, n_split;   // row tiles per sequence, the most blocks per tile
   uint32_t n_items;        // tiles: n_rt * n_group * n_seqs
@@ -656,16 +657,29 @@ __device__ __forceinline__ int p4_parts(const Prefill4Args &a, uint32_t keys) {
   return max(1, min(a.n_split, (int)((keys + P4_UNIT - 1) / P4_UNIT / 2)));
 }
 
+// The s-th longest of up to 64 sequences (of equal ones the first).
+__device__ __forceinline__ int p4_nth_longest(const Prefill4Args &a, int s) {
+  const int lane = threadIdx.x & 63;
+  const int32_t len = lane < a.n_seqs ? a.kv_len[lane] : 0;
+  int before = 0;
+  for (int i = 0; i < a.n_seqs; ++i) {
+    const int32_t other = __builtin_amdgcn_readlane(len, i);
+    before += other > len || (other == len && i < lane);
+  }
+  return __ffsll((long long)__ballot(lane < a.n_seqs && before == s)) - 1;
+}
+
 template <int D, int CT, bool EXACT>
 __global__ void __launch_bounds__(ATT_THREADS, a4_per_cu(D, CT)) paged_prefill4_kernel(Prefill4Args a) {
-  // row tiles slowest and last ones first: under a causal mask they see the most keys; a tile's
-  // parts next to each other
+  // the sequence with the most keys first, its last row tiles first (under a causal mask they
+  // see the most): the chip is left with short tiles at the end; a tile's parts next to each other
   const uint32_t item = blockIdx.x / (uint32_t)a.n_split;
   const int split = (int)(blockIdx.x - item * (uint32_t)a.n_split);
-  const uint32_t per_rt = (uint32_t)a.n_group * (uint32_t)a.n_seqs;
-  const uint32_t rt_rev = item / per_rt, rem = item - rt_rev * per_rt;
-  const int b = (int)(rem / (uint32_t)a.n_group);
-  const int y = (int)(rem - (uint32_t)b * (uint32_t)a.n_group);
+  const uint32_t per_seq = (uint32_t)a.n_group * (uint32_t)a.n_rt;
+  const uint32_t s = item / per_seq, rem = item - s * per_seq;
+  const int b = a.by_length ? p4_nth_longest(a, (int)s) : (int)s;
+  const uint32_t rt_rev = rem / (uint32_t)a.n_group;
+  const int y = (int)(rem - rt_rev * (uint32_t)a.n_group);
   const int grp = a.n_q_heads / a.n_kv_heads, per_kv = a.n_group / a.n_kv_heads;
   const int h = y / per_kv, first = (y - h * per_kv) * a.group;
   const int G = min(a.group, grp - first), hq0 = h * grp + first;
@@ -728,7 +742,7 @@ __global__ void __launch_bounds__(ATT_THREADS, a4_per_cu(D, CT)) paged_prefill4_
         const float v = sum == 0.0f ? 0.0f : acc / sum;
         a.out[((lo + row0 + r) * a.n_q_heads + hq0 + (c - r * G)) * (int64_t)D + d] = (uint16_t)(pack_bf16(v, 0.0f) & 0xFFFFu);
       } else {
-        float *pp = a.part + (((int64_t)item * a.n_split + split) * (16 * CT) + c) * (int64_t)(2 + D);
+        float *pp = a.part + (((int64_t)item * a.n_split + split) * (16 * CT) + c) * (int64_t)(2 + D);  // (s is b)
         pp[2 + d] = acc;
         if (d == 0) {
           pp[0] = M;
@@ -757,7 +771,7 @@ __global__ void __launch_bounds__(D) prefill4_combine_kernel(Prefill4Args a, int
   const int64_t rt = row / a.rows, row_end = min(rows, (rt + 1) * a.rows);
   const int parts = p4_parts(a, p4_keys(a, a.kv_len[b], a.q_pos0[b], row_end));
   if (parts == 1) return;  // its block has written the row
-  const int64_t item = ((a.n_rt - 1 - rt) * a.n_seqs + b) * a.n_group + h * per_kv + sub;
+  const int64_t item = ((int64_t)b * a.n_rt + a.n_rt - 1 - rt) * a.n_group + h * per_kv + sub;
   const int c = (int)(row - rt * a.rows) * G + (hq - h * grp - first);
   const float *pp = a.part + (item * a.n_split * columns + c) * (int64_t)(2 + D);
   a.out[(int64_t)blockIdx.x * D + threadIdx.x] = att_combine_row(pp, (int64_t)columns * (2 + D), parts, threadIdx.x, 1.0f);
@@ -985,6 +999,7 @@ extern "C" int zx_paged_attention4_prefill(const uint16_t *q, int64_t n_q, const
   a.n_q = n_q;
   a.sm_log2e = sm_scale * ATT_LOG2E;
   a.n_split = room && !p.runs ? (int32_t)p.n_split : 1;
+  a.by_length = a.n_split == 1 && n_seqs > 1 && n_seqs <= 64;
   {
     int sh = 0;
     while ((1LL << sh) < page_size) ++sh;
