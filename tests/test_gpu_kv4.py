@@ -317,6 +317,27 @@ def test_decode_nan_and_bad_pages(dev):
     assert torch.isnan(got).all()
 
 
+@pytest.mark.parametrize("Hq, H, D", [(17, 1, 64), (8, 2, 128), (16, 2, 256)])
+def test_attention_repeats_to_the_bit(dev, Hq, H, D):
+    """Every call gives the same bits, decode and prefill (a product's result read before it is
+    complete would now and then change a running maximum, and with it the last bits)."""
+    lens, rows, P = [2000, 3, 700], [40, 3, 5], 16
+    bt, n_pages = tables(lens, P, 0, 5)
+    pool = torch.from_numpy(random_pool(n_pages, H, P, D, 5)).to(dev)
+    btd, ld = i32(bt, dev), i32(lens, dev)
+    q = torch.randn((sum(rows), Hq, D), device=dev).mul(2).to(torch.bfloat16)
+    cu, pos0 = i32(np.concatenate([[0], np.cumsum(rows)]), dev), i32([n - r for n, r in zip(lens, rows)], dev)
+
+    def both(precision):
+        return (kv.paged_attention4_decode(q[:3], pool, btd, ld),
+                kv.paged_attention4_prefill(q, cu, pos0, pool, btd, ld, max_q_per_seq=40, precision=precision),
+                kv.paged_attention4_prefill(q[:2], i32([0, 2, 2, 2], dev), pos0, pool, btd, ld, max_q_per_seq=2))
+    for precision in ("bf16", "exact"):
+        want = both(precision)
+        for _ in range(30):
+            assert all(torch.equal(a, b) for a, b in zip(both(precision), want))
+
+
 PREFILL = [  # rows, tokens before, Hq, Hkv, D, P, causal
     ([1], [0], 1, 1, 64, 16, True), ([3, 0, 5], [10, 4, 0], 4, 2, 128, 16, True), ([4, 1, 2], [500, 1000, 31], 32, 8, 128, 16, True),
     ([40, 17], [0, 90], 4, 1, 128, 32, True), ([130], [60], 8, 8, 64, 16, True), ([33, 64], [100, 0], 6, 2, 256, 16, True),

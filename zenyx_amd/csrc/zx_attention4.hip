@@ -90,12 +90,11 @@ constexpr float A4_NONE = -3.402823466e38f;
 constexpr float A4_LAZY = 8.0f;
 
 
-// The largest of 8 scores (NaN ignored).  v_max3_f32 by hand: from fmaxf the compiler makes an
-// instruction more for every operand, to quiet signalling NaN.
+// The largest of 8 scores, NaN if one is (then the column's row is NaN whatever its maximum): from
+// fmaxf the compiler makes an instruction more for every operand, to quiet signalling NaN.  (Not
+// by hand in assembly: no wait would be put between a matrix product and its reader.)
 __device__ __forceinline__ float a4_max3(float a, float b, float c) {
-  float r;
-  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
-  return r;
+  return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c);
 }
 __device__ __forceinline__ float a4_max8(const float (&s)[8]) {
   const float x = a4_max3(s[0], s[1], s[2]);
