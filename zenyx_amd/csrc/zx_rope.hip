@@ -75,62 +75,54 @@ struct RopeArgs {
   uint32_t n_rows;
   int32_t n_heads, head_dim;
   uint32_t units;    // of a head: rot / 16 that turn 8 pairs, then (copy) 8 channels each
-  uint32_t n_share;  // threads that share a row's unit; a thread takes every n_share-th head
   int32_t transpose, copy;  // copy: out is another tensor (the channels past rot are written too)
 };
 
-// Unit u of a row for the heads h0, h0 + n_share, ...: the cosines and sines are loaded once for
-// all of them.  Neighbouring threads take neighbouring units, then heads: whole cache lines.
+// A thread: one unit of a head.  Neighbouring threads take neighbouring units, then heads, then
+// rows: whole cache lines, and the table's row comes from the cache (four heads per thread, so
+// that it is read once for them, gained nothing: 4,096 x 32 x 128 bf16 12.6 us either way).
 template <int DT, bool INTER> __global__ void __launch_bounds__(256) rope_kernel(RopeArgs a) {
   using Io = RopeIo<DT>;
   using T = typename Io::T;
-  const uint32_t per_row = a.units * a.n_share;
+  const uint32_t per_row = a.units * (uint32_t)a.n_heads;
   const uint32_t at = blockIdx.x * 256u + threadIdx.x;
   const uint32_t row = at / per_row;
   if (row >= a.n_rows) return;
   const uint32_t rest = at - row * per_row;
-  const uint32_t h0 = rest / a.units, u = rest - h0 * a.units;
+  const uint32_t h = rest / a.units, u = rest - h * a.units;
   const int32_t pos = a.positions[row];
-  const bool live = pos >= 0 && pos < a.r.n_pos;
-  if (!live && rest == 0 && a.err) atomicOr(a.err, ZX_KERR_POS_RANGE);
-  const T *x = static_cast<const T *>(a.x) + row * a.x_row;
-  T *out = static_cast<T *>(a.out) + row * a.o_row;
+  const T *x = static_cast<const T *>(a.x) + row * a.x_row + h * a.x_head;
+  T *out = static_cast<T *>(a.out) + row * a.o_row + h * a.o_head;
   const uint32_t turning = (uint32_t)a.r.rot / 16;
+  float f[8], g[8];
   if (u >= turning) {  // 8 channels past rot
     const int c0 = a.r.rot + 8 * (int)(u - turning);
-    for (int h = h0; h < a.n_heads; h += a.n_share) {
-      float f[8];
-      Io::load(x + h * a.x_head + c0, f);
-      Io::store(out + h * a.o_head + c0, f);
-    }
+    Io::load(x + c0, f);
+    Io::store(out + c0, f);
     return;
   }
   const int ca = INTER ? 16 * u : 8 * u, cb = INTER ? ca + 8 : ca + a.r.rot / 2;
-  if (!live) {  // no row of the table: as it is
-    if (a.copy)
-      for (int h = h0; h < a.n_heads; h += a.n_share) {
-        float f[8], g[8];
-        Io::load(x + h * a.x_head + ca, f);
-        Io::load(x + h * a.x_head + cb, g);
-        Io::store(out + h * a.o_head + ca, f);
-        Io::store(out + h * a.o_head + cb, g);
-      }
+  if (pos < 0 || pos >= a.r.n_pos) {  // no row of the table: as it is
+    if (rest == 0 && a.err) atomicOr(a.err, ZX_KERR_POS_RANGE);
+    if (a.copy) {
+      Io::load(x + ca, f);
+      Io::load(x + cb, g);
+      Io::store(out + ca, f);
+      Io::store(out + cb, g);
+    }
     return;
   }
   float c[8], s[8];
   rope_row(a.r, pos, u, c, s);
+  Io::load(x + ca, f);
+  Io::load(x + cb, g);
   if (a.transpose) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) s[i] = -s[i];
   }
-  for (int h = h0; h < a.n_heads; h += a.n_share) {
-    float f[8], g[8];
-    Io::load(x + h * a.x_head + ca, f);
-    Io::load(x + h * a.x_head + cb, g);
-    rope_turn<INTER>(f, g, c, s);
-    Io::store(out + h * a.o_head + ca, f);
-    Io::store(out + h * a.o_head + cb, g);
-  }
+  rope_turn<INTER>(f, g, c, s);
+  Io::store(out + ca, f);
+  Io::store(out + cb, g);
 }
 
 // ------------------------------------------------------------------ FP8 append with rotation
@@ -190,24 +182,33 @@ ra_offsets_kernel(TokGeom g, int64_t limit, int64_t n_tok, int64_t *tok_off, int
   tok_pos[t[0]] = (int32_t)pos[0];
 }
 
-template <int U, bool LOCATE>
+template <bool LOCATE>
 __device__ __forceinline__ void ra_find(const TokGeom &tg, const TokStage &stage, int64_t limit, const TokPlace *places,
-                                        const int64_t (&row)[U], int64_t n_tok, int64_t (&page)[U], int64_t (&pos)[U],
-                                        int32_t &e) {
+                                        int64_t row, int64_t n_tok, int64_t &page, int64_t &pos, int32_t &e) {
   if constexpr (LOCATE) {
-    token_places<U>(tg, stage, limit, row, n_tok, page, pos, e);
+    const int64_t t[1] = {row};
+    int64_t pg[1], ps[1];
+    token_places<1>(tg, stage, limit, t, n_tok, pg, ps, e);
+    page = pg[0];
+    pos = ps[0];
   } else {
-#pragma unroll
-    for (int k = 0; k < U; ++k) {
-      const TokPlace p = row[k] < n_tok ? places[row[k]] : TokPlace{-1, -1};
-      page[k] = p.page;
-      pos[k] = p.pos;
-    }
+    const TokPlace p = row < n_tok ? places[row] : TokPlace{-1, -1};
+    page = p.page;
+    pos = p.pos;
   }
+}
+// Both columns of a unit; rows past the last one are zeros.
+__device__ __forceinline__ void ra_load(__amdgpu_buffer_rsrc_t rsrc, int off, const RaUnit &n, bool last, uint4 &a, uint4 &b) {
+  const q_v4u v = last ? __builtin_amdgcn_raw_buffer_load_b128(rsrc, off + 2 * n.ca, 0, 2 /* nontemporal */)
+                       : __builtin_amdgcn_raw_buffer_load_b128(rsrc, off + 2 * n.ca, 0, 0);
+  const q_v4u w = last ? __builtin_amdgcn_raw_buffer_load_b128(rsrc, off + 2 * n.cb, 0, 2)
+                       : __builtin_amdgcn_raw_buffer_load_b128(rsrc, off + 2 * n.cb, 0, 0);
+  a = make_uint4(v.x, v.y, v.z, v.w);
+  b = make_uint4(w.x, w.y, w.z, w.w);
 }
 
 // Pass 1 (dynamic scales): maxima of |rotated K| and |V| of the tokens that have a position.
-template <int U, bool LOCATE, bool INTER>
+template <bool LOCATE, bool INTER>
 __global__ void __launch_bounds__(512)
 rope_append_amax_kernel(const uint16_t *x, RaGeom g, RopeTable r, TokGeom tg, int64_t limit, const TokPlace *places,
                         uint32_t *part /* [L][gridDim.x][2H] */) {
@@ -216,35 +217,23 @@ rope_append_amax_kernel(const uint16_t *x, RaGeom g, RopeTable r, TokGeom tg, in
   const RaUnit n = ra_unit<INTER>(g, r.rot, t - rs * g.n_unit);
   const int layer = blockIdx.y;
   const char *xl = reinterpret_cast<const char *>(x + (int64_t)layer * g.x_layer_stride);
-  const int col = 2 * n.slab * g.head_dim;
-  const int64_t step = (int64_t)gridDim.x * U * g.rpb;
+  const int64_t step = (int64_t)gridDim.x * g.rpb;
   uint32_t m = 0;  // two packed 16-bit maxima
   int32_t e = 0;
   __shared__ TokStage stage;
   if constexpr (LOCATE) token_stage(tg, stage);
-  for (int64_t r0 = (int64_t)blockIdx.x * U * g.rpb; r0 < g.n_tok; r0 += step) {
-    const __amdgpu_buffer_rsrc_t rsrc = q_rsrc(xl + r0 * g.row_bytes, (g.n_tok - r0) * g.row_bytes);
-    uint4 a[U], b[U];
-    int64_t row[U], page[U], pos[U];
-#pragma unroll
-    for (int k = 0; k < U; ++k) {
-      const int off = (int)((k * g.rpb + rs) * g.row_bytes) + col;
-      const q_v4u v = __builtin_amdgcn_raw_buffer_load_b128(rsrc, off + 2 * n.ca, 0, 0);
-      const q_v4u w = __builtin_amdgcn_raw_buffer_load_b128(rsrc, off + 2 * n.cb, 0, 0);
-      a[k] = make_uint4(v.x, v.y, v.z, v.w);
-      b[k] = make_uint4(w.x, w.y, w.z, w.w);
-      row[k] = r0 + k * g.rpb + rs;
+  for (int64_t r0 = (int64_t)blockIdx.x * g.rpb; r0 < g.n_tok; r0 += step) {
+    uint4 a, b;
+    int64_t page, pos;
+    ra_load(q_rsrc(xl + r0 * g.row_bytes, (g.n_tok - r0) * g.row_bytes),
+            (int)(rs * g.row_bytes) + 2 * n.slab * g.head_dim, n, false, a, b);
+    ra_find<LOCATE>(tg, stage, limit, places, r0 + rs, g.n_tok, page, pos, e);
+    if (n.turns) {
+      float c[8], s[8];
+      rope_row(r, pos < 0 ? 0 : pos, n.p, c, s);
+      rope_turn_bf16<INTER>(a, b, c, s);
     }
-    ra_find<U, LOCATE>(tg, stage, limit, places, row, g.n_tok, page, pos, e);
-#pragma unroll
-    for (int k = 0; k < U; ++k) {
-      if (n.turns) {
-        float c[8], s[8];
-        rope_row(r, pos[k] < 0 ? 0 : pos[k], n.p, c, s);
-        rope_turn_bf16<INTER>(a[k], b[k], c, s);
-      }
-      if (pos[k] >= 0) m = absmax_acc(absmax_acc(m, a[k]), b[k]);
-    }
+    if (pos >= 0) m = absmax_acc(absmax_acc(m, a), b);
   }
   const uint32_t mx = group_max(fold16(m), g.upd);
   __shared__ uint32_t red[512];
@@ -257,10 +246,10 @@ rope_append_amax_kernel(const uint16_t *x, RaGeom g, RopeTable r, TokGeom tg, in
   }
 }
 
-// Pass 2: rotate, encode, scatter (tiles from the end of the batch first, where the first
+// Pass 2: rotate, encode, scatter (rows from the end of the batch first, where the first
 // pass has left the caches).  MODE as kv_quant_rows_kernel's: 0 dynamic scales, 1 static, 2 static and
 // saturating.
-template <int U, int MODE, bool LOCATE, bool INTER>
+template <int MODE, bool LOCATE, bool INTER>
 __global__ void __launch_bounds__(512)
 rope_append_rows_kernel(const uint16_t *x, RaGeom g, RopeTable r, TokGeom tg, int64_t limit, const TokPlace *places,
                         const float *scales, uint8_t *pool, int64_t pool_layer_stride, int32_t *err) {
@@ -271,53 +260,48 @@ rope_append_rows_kernel(const uint16_t *x, RaGeom g, RopeTable r, TokGeom tg, in
   const float sc = scales[(int64_t)layer * g.n_slabs + n.slab];
   const QuantScale q = quant_scale(sc);
   const uint32_t s_sign = (__float_as_uint(sc) >> 24) & 0x80u;
-  const int64_t r0 = ((int64_t)gridDim.x - 1 - blockIdx.x) * U * g.rpb;
+  const int64_t r0 = ((int64_t)gridDim.x - 1 - blockIdx.x) * g.rpb;
   const char *xl = reinterpret_cast<const char *>(x + (int64_t)layer * g.x_layer_stride);
-  const __amdgpu_buffer_rsrc_t rsrc = q_rsrc(xl + r0 * g.row_bytes, (g.n_tok - r0) * g.row_bytes);
   uint8_t *pl = pool + (int64_t)layer * pool_layer_stride + (int64_t)n.slab * tg.page_size * tg.head_dim;
-  uint4 a[U], b[U];
-  int64_t row[U], page[U], pos[U];
-#pragma unroll
-  for (int k = 0; k < U; ++k) {
-    const int off = (int)((k * g.rpb + rs) * g.row_bytes) + 2 * n.slab * g.head_dim;
-    const q_v4u v = __builtin_amdgcn_raw_buffer_load_b128(rsrc, off + 2 * n.ca, 0, 2 /* nontemporal: last read */);
-    const q_v4u w = __builtin_amdgcn_raw_buffer_load_b128(rsrc, off + 2 * n.cb, 0, 2);
-    a[k] = make_uint4(v.x, v.y, v.z, v.w);
-    b[k] = make_uint4(w.x, w.y, w.z, w.w);
-    row[k] = r0 + k * g.rpb + rs;
-  }
+  uint4 a, b;
+  int64_t page, pos;
+  ra_load(q_rsrc(xl + r0 * g.row_bytes, (g.n_tok - r0) * g.row_bytes),
+          (int)(rs * g.row_bytes) + 2 * n.slab * g.head_dim, n, true, a, b);
   int32_t e = 0;
   __shared__ TokStage stage;
   if constexpr (LOCATE) token_stage(tg, stage);
-  ra_find<U, LOCATE>(tg, stage, limit, places, row, g.n_tok, page, pos, e);
+  ra_find<LOCATE>(tg, stage, limit, places, r0 + rs, g.n_tok, page, pos, e);
   if (LOCATE && e && err && layer == 0 && n.slab == 0 && n.p == 0) atomicOr(err, e);
-#pragma unroll
-  for (int k = 0; k < U; ++k) {
-    if (page[k] < 0) continue;
-    if (n.turns) {
-      float c[8], s[8];
-      rope_row(r, pos[k], n.p, c, s);
-      rope_turn_bf16<INTER>(a[k], b[k], c, s);
-    }
-    uint2 ea = quant8(a[k], q), eb = quant8(b[k], q);
-    if (MODE != 0 && q.nan_fix == 0) {
-      ea = static_overflow<MODE>(a[k], ea, s_sign, err);
-      eb = static_overflow<MODE>(b[k], eb, s_sign, err);
-    }
-    uint8_t *dst = pl + page[k] * tg.page_bytes + (int64_t)((uint32_t)pos[k] % (uint32_t)tg.page_size) * tg.head_dim;
-    typedef unsigned int v2u __attribute__((ext_vector_type(2)));
-    const v2u wa = {ea.x, ea.y}, wb = {eb.x, eb.y};
-    __builtin_nontemporal_store(wa, reinterpret_cast<v2u *>(dst + n.ca));
-    __builtin_nontemporal_store(wb, reinterpret_cast<v2u *>(dst + n.cb));
+  if (page < 0) return;
+  if (n.turns) {
+    float c[8], s[8];
+    rope_row(r, pos, n.p, c, s);
+    rope_turn_bf16<INTER>(a, b, c, s);
   }
+  uint2 ea = quant8(a, q), eb = quant8(b, q);
+  if (MODE != 0 && q.nan_fix == 0) {
+    ea = static_overflow<MODE>(a, ea, s_sign, err);
+    eb = static_overflow<MODE>(b, eb, s_sign, err);
+  }
+  uint8_t *dst = pl + page * tg.page_bytes + (int64_t)((uint32_t)pos % (uint32_t)tg.page_size) * tg.head_dim;
+  typedef unsigned int v2u __attribute__((ext_vector_type(2)));
+  const v2u wa = {ea.x, ea.y}, wb = {eb.x, eb.y};
+  __builtin_nontemporal_store(wa, reinterpret_cast<v2u *>(dst + n.ca));
+  __builtin_nontemporal_store(wb, reinterpret_cast<v2u *>(dst + n.cb));
 }
 
-constexpr int RA_U = 4;        // rows per thread and step, both passes
-constexpr int RA_BPC = 4;      // blocks per CU of the first pass
-constexpr int64_t RA_LOCATE_BPC = 4;  // up to this many blocks per CU find the places themselves
+// A thread takes one row: two and four in flight were slower throughout (static scales, 8 heads, D
+// = 128, in a graph: 2 layers x 16,000 tokens 40.4 / 41.9 / 44.7 us, 4 x 4,000 22.7 / 24.2 / 25.6),
+// and so were 2 and 8 blocks per CU in the first pass (2 x 16,000, both passes: 78 and 72, with 4
+// 70 us).
+constexpr int RA_BPC = 4;
+// Up to this many blocks per CU find the places themselves, without a launch for it before (32 layers
+// x 16 tokens 4.5 us against 8.0, x 64 5.9 / 8.7, x 128 8.8 / 9.9; x 256, where too many look for
+// the same few, 15.7 / 14.5).
+constexpr int64_t RA_LOCATE_BPC = 8;
 
 static int64_t ra_amax_grid_x(int64_t n_tok, int32_t rpb, int32_t n_layers) {
-  const int64_t tiles = ceil_div(n_tok, (int64_t)RA_U * rpb);
+  const int64_t tiles = ceil_div(n_tok, rpb);
   const int64_t want = std::max<int64_t>(1, ceil_div((int64_t)num_cus() * RA_BPC, n_layers));
   return std::max<int64_t>(1, std::min(tiles, want));
 }
@@ -375,13 +359,7 @@ extern "C" int zx_rope(const void *x, int dtype, int64_t n_rows, int32_t n_heads
   a.copy = x != out;
   a.transpose = (flags & ZX_ROPE_TRANSPOSE) != 0;
   a.units = (uint32_t)(rot_dim / 16 + (a.copy ? (head_dim - rot_dim) / 8 : 0));
-  // as many heads per thread as leave eight blocks per CU, at most 4
-  int64_t share = n_heads;
-  while (share > 1 && ceil_div(n_heads, share) < 4 &&
-         n_rows * ceil_div(share, 2) * a.units >= 8LL * 256 * num_cus())
-    share = ceil_div(share, 2);
-  a.n_share = (uint32_t)share;
-  const int64_t threads = n_rows * share * a.units;
+  const int64_t threads = n_rows * n_heads * a.units;
   if (threads >= (1LL << 32) - 256) return fail(ZX_ERR_UNSUPPORTED, "rope: too many rows");
   const unsigned blocks = (unsigned)ceil_div(threads, 256);
   const hipStream_t st = as_stream(stream);
@@ -408,7 +386,7 @@ static int32_t ra_rows_per_block(int32_t n_heads, int32_t head_dim) {
   return units >= 256 ? 1 : 256 / units;
 }
 static bool ra_locates(int32_t n_layers, int64_t n_tok, int32_t n_heads, int32_t head_dim) {
-  return ceil_div(n_tok, (int64_t)RA_U * ra_rows_per_block(n_heads, head_dim)) * n_layers <= RA_LOCATE_BPC * num_cus();
+  return ceil_div(n_tok, ra_rows_per_block(n_heads, head_dim)) * n_layers <= RA_LOCATE_BPC * num_cus();
 }
 
 // Dynamic scales in one cooperative pass (zx_append_fused.hip)?  By the rule of the append that
@@ -510,25 +488,25 @@ extern "C" int zx_kv_rope_append(const uint16_t *x, int64_t x_layer_stride, int3
   if (dynamic) {
     const unsigned gx = (unsigned)ra_amax_grid_x(n_tok, g.rpb, n_layers);
     const dim3 grid(gx, n_layers);
-#define ZX_RA_AMAX(u, loc, il) \
-  rope_append_amax_kernel<u, loc, il><<<grid, threads, 0, st>>>(x, g, r, tg, limit, places, part)
-    if (locate && inter) ZX_RA_AMAX(1, true, true);
-    else if (locate) ZX_RA_AMAX(1, true, false);
-    else if (inter) ZX_RA_AMAX(RA_U, false, true);
-    else ZX_RA_AMAX(RA_U, false, false);
+#define ZX_RA_AMAX(loc, il) \
+  rope_append_amax_kernel<loc, il><<<grid, threads, 0, st>>>(x, g, r, tg, limit, places, part)
+    if (locate && inter) ZX_RA_AMAX(true, true);
+    else if (locate) ZX_RA_AMAX(true, false);
+    else if (inter) ZX_RA_AMAX(false, true);
+    else ZX_RA_AMAX(false, false);
 #undef ZX_RA_AMAX
     if ((rc = check_launch("rope_append_amax"))) return rc;
     if ((rc = finalize_partials(part, (int32_t)gx, g.n_slabs, n_layers, scales, st))) return rc;
   }
-  const dim3 grid((unsigned)ceil_div(n_tok, (int64_t)(locate ? 1 : RA_U) * g.rpb), n_layers);
-#define ZX_RA_ROWS2(mode, u, loc, il)                                                                                  \
-  rope_append_rows_kernel<u, mode, loc, il><<<grid, threads, 0, st>>>(x, g, r, tg, limit, places, scales, pool,        \
-                                                                     pool_layer_stride, err)
-#define ZX_RA_ROWS(mode)                                 \
-  if (locate && inter) ZX_RA_ROWS2(mode, 1, true, true); \
-  else if (locate) ZX_RA_ROWS2(mode, 1, true, false);    \
-  else if (inter) ZX_RA_ROWS2(mode, RA_U, false, true);  \
-  else ZX_RA_ROWS2(mode, RA_U, false, false);
+  const dim3 grid((unsigned)ceil_div(n_tok, g.rpb), n_layers);
+#define ZX_RA_ROWS2(mode, loc, il)                                                                                     \
+  rope_append_rows_kernel<mode, loc, il><<<grid, threads, 0, st>>>(x, g, r, tg, limit, places, scales, pool,           \
+                                                                  pool_layer_stride, err)
+#define ZX_RA_ROWS(mode)                              \
+  if (locate && inter) ZX_RA_ROWS2(mode, true, true); \
+  else if (locate) ZX_RA_ROWS2(mode, true, false);    \
+  else if (inter) ZX_RA_ROWS2(mode, false, true);     \
+  else ZX_RA_ROWS2(mode, false, false);
   if (dynamic) {
     ZX_RA_ROWS(0)
   } else if (flags & ZX_APPEND_SATURATE) {
