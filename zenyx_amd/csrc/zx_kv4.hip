@@ -221,8 +221,8 @@ kv4_gather_kernel(const uint8_t *__restrict__ pool, K4Gather g, const int32_t *_
 
 // Up to this many waves per CU find the pages themselves, without a launch for it before (8 heads,
 // D = 128, in a graph: 32 layers x 16 tokens 5.2 us against 6.8, x 64 7.6 / 9.0, x 256 23.8 / 26.6;
-// at twice as many, 4 layers x 4,000, 39.7 / 40.4).
-constexpr int64_t K4_LOCATE_WPC = 64;
+// at twice as many, 4 layers x 4,000, 39.7 / 40.4: no difference).
+constexpr int64_t K4_LOCATE_WPC = 32;
 
 }  // namespace zx
 
