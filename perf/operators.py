@@ -322,7 +322,7 @@ def _own(s):
         return {"codes": s["pool"].view(torch.float8_e4m3fn), "scales": scales}
     if kind == "append4":
         kv.kv4_append(s["x"], s["cu"], s["bt"], s["pool"], start_pos=s["old"], table=s.get("table"),
-                      interleaved=s["interleaved"])
+                      interleaved=s["interleaved"] and "table" in s)
         k, v = kv.kv4_gather_dequant(s["pool"][0], s["bt"], s["lens"], s["most"])
         return {"k": k, "v": v}
     if kind == "decode4":
