@@ -119,6 +119,7 @@ __device__ __forceinline__ int a4_seq_of(const int32_t *cu_q, int32_t n_seqs, in
 template <int D> struct A4Lds {
   static constexpr int VROW = 2 * D + 32;
   static constexpr int WAVE = A4_STEP * VROW;
+  static constexpr int AROW = D + 4;  // floats of a column of accumulators (eight on distinct banks)
 };
 
 // Where word w of lane (n, kg) goes: token 16 T + n.
@@ -440,7 +441,7 @@ template <int D, int CT, bool EXACT> struct A4Wave {
   // Tile ct's accumulators into the wave's LDS (in the place of V), [column][channel], and its
   // columns' maxima and sums; the first `live` columns.
   __device__ __forceinline__ void spill(int ct, int live, float *sm_m, float *sm_l) {
-    static_assert(A4_HEADS * D * 4 <= Lds::WAVE, "a tile of O fits where V was");
+    static_assert(A4_HEADS * Lds::AROW * 4 <= Lds::WAVE, "a tile of O fits where V was");
     float *acc = reinterpret_cast<float *>(vt);
     float sum = ol[ct][0];
     if constexpr (EXACT) {
@@ -451,7 +452,7 @@ template <int D, int CT, bool EXACT> struct A4Wave {
     }
     if (n >= live) return;
 #pragma unroll
-    for (int jt = 0; jt < NT; ++jt) *reinterpret_cast<att_f32x4 *>(acc + n * D + 16 * jt + 4 * kg) = o[ct][jt];
+    for (int jt = 0; jt < NT; ++jt) *reinterpret_cast<att_f32x4 *>(acc + n * Lds::AROW + 16 * jt + 4 * kg) = o[ct][jt];
     if (kg == 0) {
       sm_m[n] = m[ct];
       sm_l[n] = sum;
@@ -459,22 +460,58 @@ template <int D, int CT, bool EXACT> struct A4Wave {
   }
 };
 
-// Column j's channel d over the block's four waves: the maximum, the sum and the accumulator.
-template <int D>
-__device__ __forceinline__ void a4_merge(const float (&sm_m)[ATT_WAVES][A4_HEADS], const float (&sm_l)[ATT_WAVES][A4_HEADS],
-                                         const uint8_t (&lds)[ATT_WAVES][A4Lds<D>::WAVE], int j, int d, float &M,
-                                         float &sum, float &acc) {
-  M = sm_m[0][j];
+// The end of a tile of columns: thread t has column t / 16, E channels from (t % 16) E on.  (A
+// channel per thread and pass, with its column's maxima, divisions and a 2-byte store each,
+// took 13 us per tile: 2 x 857 rows, 32 heads, D = 128, on one key 49 us, 26 so; on 1,024
+// keys 77, 54 so.)
+template <int D> struct A4End {
+  static constexpr int E = D / 16;
+  static_assert(A4_HEADS * 16 == ATT_THREADS, "a thread per sixteenth of a column");
+  float M, sum, acc[E];
+  static __device__ __forceinline__ int column() { return threadIdx.x >> 4; }
+  static __device__ __forceinline__ int channel() { return (threadIdx.x & 15) * E; }
+  // Over the block's four waves: the maximum, the sum and the accumulators.
+  __device__ __forceinline__ A4End(const float (&sm_m)[ATT_WAVES][A4_HEADS], const float (&sm_l)[ATT_WAVES][A4_HEADS],
+                                   const uint8_t (&lds)[ATT_WAVES][A4Lds<D>::WAVE]) {
+    const int j = column();
+    M = sm_m[0][j];
 #pragma unroll
-  for (int w = 1; w < ATT_WAVES; ++w) M = fmaxf(M, sm_m[w][j]);
-  acc = sum = 0.0f;
+    for (int w = 1; w < ATT_WAVES; ++w) M = fmaxf(M, sm_m[w][j]);
+    sum = 0.0f;
 #pragma unroll
-  for (int w = 0; w < ATT_WAVES; ++w) {
-    const float f = __builtin_amdgcn_exp2f(sm_m[w][j] - M);  // (maxima are finite)
-    acc += f * reinterpret_cast<const float *>(lds[w])[j * D + d];
-    sum += f * sm_l[w][j];
+    for (int i = 0; i < E; ++i) acc[i] = 0.0f;
+#pragma unroll
+    for (int w = 0; w < ATT_WAVES; ++w) {
+      const float f = __builtin_amdgcn_exp2f(sm_m[w][j] - M);  // (maxima are finite)
+      sum += f * sm_l[w][j];
+      const att_f32x4 *row =
+          reinterpret_cast<const att_f32x4 *>(reinterpret_cast<const float *>(lds[w]) + j * A4Lds<D>::AROW + channel());
+#pragma unroll
+      for (int i = 0; i < E; ++i) acc[i] += f * row[i / 4][i % 4];
+    }
   }
-}
+  // The finished row (of D channels at `row`), zeros when no key counted.
+  __device__ __forceinline__ void store(uint16_t *row) const {
+    uint32_t w[E / 2];
+#pragma unroll
+    for (int i = 0; i < E / 2; ++i)
+      w[i] = sum == 0.0f ? 0u : pack_bf16(acc[2 * i] / sum, acc[2 * i + 1] / sum);
+    if constexpr (E == 4) {
+      *reinterpret_cast<uint2 *>(row + channel()) = make_uint2(w[0], w[1]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < E / 8; ++i)
+        reinterpret_cast<uint4 *>(row + channel())[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+    }
+  }
+  // A part of it: maximum, sum, accumulators (8-byte aligned).
+  __device__ __forceinline__ void store_part(float *pp) const {
+#pragma unroll
+    for (int i = 0; i < E / 2; ++i)
+      reinterpret_cast<float2 *>(pp + 2 + channel())[i] = make_float2(acc[2 * i], acc[2 * i + 1]);
+    if (channel() == 0) *reinterpret_cast<float2 *>(pp) = make_float2(M, sum);
+  }
+};
 
 // Blocks per CU (waves per SIMD) by the registers of CT tiles of columns.
 __host__ __device__ constexpr int a4_per_cu(int D, int CT) { return D * CT > 128 ? 2 : CT > 1 ? 3 : 4; }
@@ -568,23 +605,12 @@ paged_decode4_kernel(const uint16_t *__restrict__ q, AttnGeom g, A4Rows qr, cons
         if (16 * ct >= cols) break;  // block-uniform
         w.spill(ct, cols - 16 * ct, sm_m[wave], sm_l[wave]);
         __syncthreads();
-        for (int i = threadIdx.x; i < 16 * D; i += ATT_THREADS) {
-          const int j = i / D, d = i % D, c = 16 * ct + j;
-          if (c >= cols) break;
-          float M, sum, acc;
-          a4_merge<D>(sm_m, sm_l, lds, j, d, M, sum, acc);
+        const int c = 16 * ct + A4End<D>::column();
+        if (c < cols) {
+          const A4End<D> end(sm_m, sm_l, lds);
           const int r = ROWS ? c / G : 0, hq = hq0 + (c - r * G);
-          if (whole_seq) {
-            const float v = sum == 0.0f ? 0.0f : acc / sum;
-            out[((row0 + r) * g.n_q_heads + hq) * D + d] = (uint16_t)(pack_bf16(v, 0.0f) & 0xFFFFu);
-          } else {
-            float *pp = part + ((int64_t)(r * g.n_q_heads + hq) * ((int64_t)g.n_run + g.n_seqs) + run.x + b) * (2 + D);
-            pp[2 + d] = acc;
-            if (d == 0) {
-              pp[0] = M;
-              pp[1] = sum;
-            }
-          }
+          if (whole_seq) end.store(out + ((row0 + r) * g.n_q_heads + hq) * D);
+          else end.store_part(part + ((int64_t)(r * g.n_q_heads + hq) * ((int64_t)g.n_run + g.n_seqs) + run.x + b) * (2 + D));
         }
         __syncthreads();
       }
@@ -731,23 +757,12 @@ __global__ void __launch_bounds__(ATT_THREADS, a4_per_cu(D, CT)) paged_prefill4_
     if (16 * ct >= cols) break;      // block-uniform
     w.spill(ct, cols - 16 * ct, sm_m[wave], sm_l[wave]);
     __syncthreads();
-    for (int i = threadIdx.x; i < 16 * D; i += ATT_THREADS) {
-      const int j = i / D, d = i % D, c = 16 * ct + j;
-      if (c >= cols) break;
-      float M, sum, acc;
-      a4_merge<D>(sm_m, sm_l, lds, j, d, M, sum, acc);
-      if (parts == 1) {
-        const int r = c / G;
-        const float v = sum == 0.0f ? 0.0f : acc / sum;
-        a.out[((lo + row0 + r) * a.n_q_heads + hq0 + (c - r * G)) * (int64_t)D + d] = (uint16_t)(pack_bf16(v, 0.0f) & 0xFFFFu);
-      } else {
-        float *pp = a.part + (((int64_t)item * a.n_split + split) * (16 * CT) + c) * (int64_t)(2 + D);  // (s is b)
-        pp[2 + d] = acc;
-        if (d == 0) {
-          pp[0] = M;
-          pp[1] = sum;
-        }
-      }
+    const int c = 16 * ct + A4End<D>::column();
+    if (c < cols) {
+      const A4End<D> end(sm_m, sm_l, lds);
+      const int r = c / G;
+      if (parts == 1) end.store(a.out + ((lo + row0 + r) * a.n_q_heads + hq0 + (c - r * G)) * (int64_t)D);
+      else end.store_part(a.part + (((int64_t)item * a.n_split + split) * (16 * CT) + c) * (int64_t)(2 + D));  // (s is b)
     }
     __syncthreads();
   }
