@@ -16,7 +16,8 @@
 //     standing for key 16 T + 4 kg + i, as bf16 hi + lo (2^-17 of a weight);
 //   * V: bf16 rows in LDS, read back transposed (ds_read_b64_tr_b16).
 // Up to 16 query heads of a KV head share a block; the columns without a head cost nothing that
-// counts (a step's products take a quarter of the time its bytes take).
+// counts (matrix cores are busy 27% of a long call's time, vector units 48%).  64 x 32k
+// positions, 2.3 GB of pages: 380 us, 6.0 TB/s; 16 x 1k-8k, 85 MB: 24 us.
 #include <algorithm>
 
 #include "zx_attn_deal.h"
@@ -646,9 +647,9 @@ decode4_rows_combine_kernel(const float *__restrict__ part, AttnGeom g, A4Rows q
 // its own, merged at the end.  So no wave waits for another within the loop, K goes from memory
 // to the operand without LDS, every conversion serves CT products, and a K/V byte read serves
 // 16 CT columns: what a block reads is small, the pages have 4 bits.  Bound by the issue of the
-// matrix products, the conversions and the exponentials together (2 x 2,048 rows on 4k-14k
-// positions: matrix cores 32% and vector units 44% of the time, and no faster when every
-// sequence's pages are the same four).
+// matrix products, the conversions and the exponentials together: 2 x 2,048 rows on 4k and 14k
+// positions, 32/8 heads, D = 128, 714 us or 937 TFLOP/s, matrix cores busy 41% and vector units
+// 52% of the time; a library product of 8,192^3 reaches 1,109.
 // With few tiles a tile's keys are shared by up to n_split blocks, whose parts
 // prefill4_combine_kernel merges.
 struct Prefill4Args {
@@ -677,9 +678,13 @@ __device__ __forceinline__ uint32_t p4_keys(const Prefill4Args &a, int32_t kv_le
   const int64_t len = max((int64_t)0, min((int64_t)kv_len, (int64_t)a.max_blocks * a.page_size));
   return (uint32_t)(a.causal ? min(len, max((int64_t)0, qpos0 + row_end)) : len);  // below 2^31
 }
-// Parts of a tile with so many keys: at least two units each, at most n_split.
+// Parts of a tile with so many keys: at least P4_PART units each, at most n_split.  A part starts
+// anew and is merged (2 x 128 rows on 2,000 and 500 positions, 32/8 heads, D = 128: two units 35
+// us, four 29; 200 rows on 2,000, 12 heads, D = 64 19.9 / 16.9; the other way 64 rows on 1,000
+// 16.6 / 18.8).
+constexpr int P4_PART = 4;
 __device__ __forceinline__ int p4_parts(const Prefill4Args &a, uint32_t keys) {
-  return max(1, min(a.n_split, (int)((keys + P4_UNIT - 1) / P4_UNIT / 2)));
+  return max(1, min(a.n_split, (int)((keys + P4_UNIT - 1) / P4_UNIT / P4_PART)));
 }
 
 // The s-th longest of up to 64 sequences (of equal ones the first).
@@ -791,7 +796,9 @@ __global__ void __launch_bounds__(D) prefill4_combine_kernel(Prefill4Args a, int
   a.out[(int64_t)blockIdx.x * D + threadIdx.x] = att_combine_row(pp, (int64_t)columns * (2 + D), parts, threadIdx.x, 1.0f);
 }
 
-// Tiles of 16 columns that a block can hold: what leaves two waves per SIMD.
+// Tiles of 16 columns that a block can hold: what leaves two waves per SIMD.  (With two at most, D
+// = 128: 2 x 2,048 rows on 8,000 positions 806 us against 703, 8,192 rows from nothing 735 / 601;
+// D = 64, 2 x 2,048 rows on 4k and 14k 472 / 439.)
 constexpr int a4_most_tiles(int D) { return D == 64 ? 4 : D == 128 ? 3 : 1; }
 
 }  // namespace zx
@@ -909,7 +916,7 @@ static Prefill4Plan p4_plan(int32_t n_q_heads, int32_t n_kv_heads, int32_t head_
   const int64_t units = ceil_div((int64_t)max_blocks * page_size, P4_UNIT);
   const int64_t resident = (int64_t)a4_per_cu(head_dim, p.ct) * num_cus();
   p.runs = p.n_rt == 1 && p.items < 4 * resident;
-  p.n_split = std::max<int64_t>(1, std::min<int64_t>({units / 2, resident / p.items, 64}));
+  p.n_split = std::max<int64_t>(1, std::min<int64_t>({units / P4_PART, resident / p.items, 64}));
   return p;
 }
 static size_t p4_bytes(const Prefill4Plan &p, int32_t n_seqs, int32_t n_q_heads, int32_t head_dim, int32_t max_q) {
