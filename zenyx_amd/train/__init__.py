@@ -3,4 +3,5 @@
 (the three-tier HBM / DRAM / NVMe hierarchy with Belady at both levels),
 ``dynamic_ring_curriculum`` (ring degree per training step and the page traces it
 implies) and ``fp8_kv_quantization`` (per-head FP8 KV quantisation, a paged FP8 KV
-cache and ring attention reading it)."""
+cache, a paged 4-bit one and ring attention reading them); beside them ``rotary`` (rotary
+positions, which those caches can apply to their keys)."""
