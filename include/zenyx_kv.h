@@ -486,8 +486,8 @@ int zx_rope(const void *x, int dtype, int64_t n_rows, int32_t n_heads, int32_t h
 /* zx_kv_quant_append with the keys rotated by their positions on the way (rounded to bf16 as
  * zx_rope rounds them, then quantised): the codes and scales of zx_rope followed by
  * zx_kv_quant_append, without the rotated copy.  flags: zx_kv_quant_append's and
- * ZX_ROPE_INTERLEAVED (the single pass only where a CU's share of a slab fits its registers).  A token at or beyond n_pos is not stored and sets
- * ZX_KERR_POS_RANGE; dynamic scales are taken over the tokens that have a position (rows
+ * ZX_ROPE_INTERLEAVED (the single pass only where a CU's share of a slab fits its registers).
+ * A token at or beyond n_pos is not stored and sets ZX_KERR_POS_RANGE; dynamic scales are taken over the tokens that have a position (rows
  * outside [cu_seqlens[0], cu_seqlens[n_seqs]) have none).  workspace:
  * zx_kv_rope_append_workspace_bytes() device bytes (0 for a small call with static scales),
  * 16-byte aligned. */
@@ -537,8 +537,8 @@ int zx_paged_attention4_decode(const uint16_t *q, int32_t n_q_heads, const uint8
 /* Blocks of queries over 4-bit pages: rows [cu_q[b], cu_q[b + 1]) of q [n_q][n_q_heads]
  * [head_dim], row i of sequence b at position q_pos0[b] + i, attend to keys [0, kv_len[b]), when
  * `causal` those up to their own position.  A row without a key gives zeros; rows beyond
- * max_q_per_seq (host) or in no sequence are left unwritten (the former set
- * ZX_KERR_POS_RANGE); kv_len beyond max_blocks * page_size is clipped and sets it too; keys on
+ * max_q_per_seq (host) or in no sequence are left unwritten, rows that cu_q claims beyond n_q do
+ * not exist (either sets ZX_KERR_POS_RANGE); a NaN value reaches the rows that see it; kv_len beyond max_blocks * page_size is clipped and sets it too; keys on
  * a page outside [0, n_pages) are left out and set ZX_KERR_PAGE_RANGE.  Softmax weights are
  * rounded once to bf16 (the row sums use the same): |error| <= one bf16 ulp + 2^-7 max|V|; with
  * ZX_PREFILL_EXACT_P they are carried as bf16 hi + lo: one ulp + 2^-15 max|V|.  workspace:

@@ -509,6 +509,35 @@ def test_prefill_computes_no_other_rows(dev, n, most, Hq, H):
         check_attention(out[:most], back, pool, bt, [n + 20], D ** -0.5, 2.0 ** -8, [most], [20], True)
 
 
+def test_a_pool_beyond_2_gib(dev):
+    """Pages whose offsets pass 31 and 32 bits: append, gather and both attentions."""
+    H, Hq, D, P, n = 8, 8, 128, 16, 90
+    n_pages = 260_000  # 17 KiB each
+    ids = [n_pages - 1, 0, 123_361, 123_362, 246_723, 246_724]
+    x = torch.randn((1, n, 2, H, D), device=dev).to(torch.bfloat16)
+    q = torch.randn((n, Hq, D), device=dev).to(torch.bfloat16)
+    cu, lens, zero = i32([0, n], dev), i32([n], dev), i32([0], dev)
+
+    def run(pool, bt):
+        kv.kv4_append(x, cu, bt, pool, check=True)
+        return (*kv.kv4_gather_dequant(pool[0], bt, lens, n, check=True),
+                kv.paged_attention4_decode(q[:1], pool[0], bt, lens, check=True),
+                kv.paged_attention4_prefill(q, cu, zero, pool[0], bt, lens, max_q_per_seq=n, check=True),
+                kv.paged_attention4_prefill(q[:2], i32([0, 2], dev), i32([n - 2], dev), pool[0], bt, lens, max_q_per_seq=2))
+    want = run(kv.kv4_pool(1, 6, H, P, D), i32([list(range(6))], dev))
+    got = run(torch.empty((1, n_pages, 2, H, 1, 17 * D // 2), dtype=torch.uint8, device=dev), i32([ids], dev))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_append_of_nothing(dev):
+    pool = kv.kv4_pool(1, 2, 2, 16, 64)
+    x = torch.zeros((1, 0, 2, 2, 64), dtype=torch.bfloat16, device=dev)
+    kv.kv4_append(x, i32([0, 0], dev), i32([[0, 1]], dev), pool, check=True)
+    assert not pool.any()
+    k, v = kv.kv4_gather_dequant(pool[0], i32([[0, 1]], dev), i32([0], dev), 0)
+    assert k.shape == v.shape == (1, 2, 0, 64)
+
+
 def test_two_calls_at_once(dev):
     """Calls on two streams, workspaces and all, do not meet."""
     Hq, H, D, P = 32, 8, 128, 16

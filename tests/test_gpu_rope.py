@@ -195,6 +195,31 @@ def test_gradient(dev, interleaved, scaling):
             assert abs(d - x.grad[at]) <= 32 * 2.0 ** -24 * big  # 4 changed values, 4 roundings each, both sides
 
 
+def test_gradient_of_the_gradient(dev):
+    """Second derivatives of sum(sin(R x)) along v: -R^T (sin(R x) * R v).  R x and R v are off by 3
+    roundings of their largest sum, the sine by as much and 4 steps of 2^-24, product and R^T by
+    four more."""
+    rope = RotaryPositions(32, 50)
+    x = torch.randn((5, 2, 32), device=dev, requires_grad=True)
+    v = torch.randn((5, 2, 32), device=dev)
+    p = torch.randint(0, 50, (5,), dtype=torch.int32, device=dev)
+    first, = torch.autograd.grad(rope(x, p).sin().sum(), x, create_graph=True)
+    got, = torch.autograd.grad((first * v).sum(), x)
+    c, s = (t[:, None] for t in rope.table.double()[p.long()].split(16, -1))
+
+    def turn(a, sign):
+        a1, a2 = a.detach().double().split(16, -1)
+        return torch.cat([a1 * c - sign * a2 * s, a2 * c + sign * a1 * s], -1)
+    want = -turn(turn(x, 1).sin() * turn(v, 1), -1)
+    mx, mv = 2 * x.abs().max(), 2 * v.abs().max()
+    assert torch.all((got.double() - want).abs() <= 2 * mv * (3 * mx + 12) * 2.0 ** -24)
+    # a second use of the same keys adds up
+    x.grad = None
+    (rope(x, p).sum() + rope(x, p).sum()).backward()
+    once, = torch.autograd.grad(rope(x, p).sum(), x)
+    assert torch.equal(x.grad, 2 * once)
+
+
 def test_rotations_compose_and_keep_distances(dev):
     """Scores depend on distances only: q at m against k at n as q at m + s against k at n + s."""
     rope = RotaryPositions(128, 131072)
@@ -298,6 +323,42 @@ def test_append_that_the_rule_sends_through_one_pass(dev):
     sa = kv.kv_rope_append(x, table, cu, bt, a, check=True)
     sb = kv.kv_rope_append(x, table, cu, bt, b, check=True, two_pass=True)
     assert same_bits(sa, sb) and torch.equal(a, b)
+
+
+def test_append_into_a_pool_beyond_2_gib(dev):
+    """Pages whose offsets pass 31 bits, both passes and one, static scales."""
+    H, D, P = 8, 128, 16
+    n_pages = 140_000  # 32 KiB each
+    table = table64(300, D, dev)
+    bt = torch.tensor([[n_pages - 1, 3, 70_000, 65_535, 65_536]], dtype=torch.int32, device=dev)
+    cu = torch.tensor([0, 70], dtype=torch.int32, device=dev)
+    x = torch.randn((1, 70, 2, H, D), device=dev).to(torch.bfloat16)
+    small = torch.zeros((1, 5, 2, H, P, D), dtype=torch.uint8, device=dev)
+    want = kv.kv_rope_append(x, table, cu, torch.arange(5, dtype=torch.int32, device=dev)[None], small)
+    pool = torch.empty((1, n_pages, 2, H, P, D), dtype=torch.uint8, device=dev)
+    for kw in (dict(two_pass=True), dict(single_pass=True), dict(static_scales=True, scales=want)):
+        pool[0, bt[0].long()] = 0
+        got = kv.kv_rope_append(x, table, cu, bt, pool, check=True, **kw)
+        assert same_bits(got, want) and torch.equal(pool[0, bt[0].long()], small[0]), kw
+
+
+def test_append_gives_up_waiting_then_recovers(dev):
+    """A bound of zero makes the single pass's first wait without progress take the release path:
+    every wave exits, the call is flagged, and with the bound restored the bits are right."""
+    H, D, P = 8, 128, 16
+    bt, cu, start, n_pages = paged([700, 333, 1201], [0, 0, 0], P, 1, dev, 2)
+    table = table64(1300, D, dev)
+    x = torch.randn((2, 2234, 2, H, D), device=dev).to(torch.bfloat16)
+    pools = [torch.zeros((2, n_pages, 2, H, P, D), dtype=torch.uint8, device=dev) for _ in range(2)]
+    kv.set_wait_bound_us(0)
+    try:
+        with pytest.raises(ValueError, match="wait"):
+            kv.kv_rope_append(x, table, cu, bt, pools[0], check=True, single_pass=True)
+    finally:
+        kv.set_wait_bound_us(None)
+    a = kv.kv_rope_append(x, table, cu, bt, pools[0], check=True, single_pass=True)
+    b = kv.kv_rope_append(x, table, cu, bt, pools[1], check=True, two_pass=True)
+    assert same_bits(a, b) and torch.equal(*pools)
 
 
 def test_append_bad_pages_and_positions(dev):

@@ -62,16 +62,18 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: dict | N
 
 
 class _Rotate(torch.autograd.Function):
+    """A linear map: its gradient is the transposed one, which is differentiable in its turn."""
+
     @staticmethod
-    def forward(ctx, x, table, positions, interleaved):
+    def forward(ctx, x, table, positions, interleaved, transpose):
         ctx.save_for_backward(table, positions)
-        ctx.interleaved = interleaved
-        return kv.rope(x, table, positions, interleaved=interleaved)
+        ctx.interleaved, ctx.transpose = interleaved, transpose
+        return kv.rope(x, table, positions, interleaved=interleaved, transpose=transpose)
 
     @staticmethod
     def backward(ctx, grad):
         table, positions = ctx.saved_tensors
-        return kv.rope(grad.contiguous(), table, positions, interleaved=ctx.interleaved, transpose=True), None, None, None
+        return _Rotate.apply(grad.contiguous(), table, positions, ctx.interleaved, not ctx.transpose), None, None, None, None
 
 
 class RotaryPositions:
@@ -98,7 +100,7 @@ class RotaryPositions:
         if x.shape[-1] != self.head_dim:
             raise ValueError(f"x must have heads of {self.head_dim}")
         if torch.is_grad_enabled() and x.requires_grad:
-            return _Rotate.apply(x, self.table, positions, self.interleaved)
+            return _Rotate.apply(x, self.table, positions, self.interleaved, False)
         return kv.rope(x, self.table, positions, interleaved=self.interleaved)
 
 
