@@ -461,6 +461,40 @@ def test_prefill_nan_values(dev, rows, old, Hq, H, D, precision):
         at += rows[b]
 
 
+@pytest.mark.parametrize("precision", ["bf16", "exact"])
+@pytest.mark.parametrize("Hq, H, D, P", [(16, 16, 64, 16), (30, 15, 128, 32), (8, 8, 256, 16)])
+def test_prefill_of_many_tiles_with_few_keys(dev, Hq, H, D, P, precision):
+    """So many tiles of so few steps (at most 4) that every wave takes one by itself; with NaN
+    values in one sequence, rows without keys, and rows behind the last."""
+    rng = np.random.default_rng(D)
+    rows = rng.integers(50, 90, 24).tolist()
+    rows[5], rows[9] = 0, 1
+    old = [int(rng.integers(0, 120 - r)) for r in rows]
+    old[3] = -7  # its first rows see nothing
+    lens = [a + b for a, b in zip(rows, old)]
+    lens[7] = 0
+    bt, n_pages = tables(lens, P, 1, 4)
+    pool = random_pool(n_pages, H, P, D, 4)
+    b, pos = 11, lens[11] - 20
+    pool[bt[b, pos // P], 1, 2, pos % P // 16, 8 * D + pos % 16] = 255  # block 0 of kv head 2
+    q = torch.randn((sum(rows) + 2, Hq, D), device=dev).to(torch.bfloat16)
+    out = torch.full_like(q, 5.0)
+    cu = np.concatenate([[0], np.cumsum(rows)])
+    kv.paged_attention4_prefill(q, i32(cu, dev), i32(old, dev), torch.from_numpy(pool).to(dev), i32(bt, dev),
+                                i32(lens, dev), precision=precision, out=out, check=True)
+    assert torch.all(out[sum(rows):] == 5) and not out[cu[7]:cu[8]].any() and not out[cu[3]:cu[3] + 7].any()
+    weight = 2.0 ** -16 if precision == "exact" else 2.0 ** -8
+    hit = out[cu[b]:cu[b + 1]]
+    grp = Hq // H
+    seen = torch.isnan(hit)
+    first = pos - old[b]
+    assert seen[first:, 2 * grp:3 * grp, :32].all() and seen.sum() == (rows[b] - first) * grp * 32
+    check = [i for i in range(24) if i != b]
+    keep = torch.cat([torch.arange(cu[i], cu[i + 1]) for i in check]).to(dev)
+    check_attention(out[keep], q[keep], pool, bt[check], [lens[i] for i in check], D ** -0.5, weight,
+                    [rows[i] for i in check], [old[i] for i in check], True)
+
+
 def test_prefill_of_many_short_sequences(dev):
     """More than 64 sequences of 0 to 6 rows: dealt by a table, in runs and whole."""
     H, Hq, D, P = 2, 8, 128, 16

@@ -347,14 +347,12 @@ template <int D, int CT, bool EXACT> struct A4Wave {
     }
   }
 
-  // Keys [t0, t_end) in steps of 32, every fourth (the block's waves take them in turn), t0 <
-  // t_end.  Branch-free: a page id is read for a position clamped into the range, a tile past
+  // Keys [t0, t_end) in steps of 32, `stride` apart, t0 < t_end.  Branch-free: a page id is read for a position clamped into the range, a tile past
   // the end or on a bad page loads through an empty resource.  Page ids are read a step before
   // the loads that they are for.  With one tile of columns the loads go out a step ahead, into a
   // second set of registers (16 x 1k-8k positions 26.7 -> 24.9 us, 128 x 100-600 17.5 -> 15.8);
   // with more, where the set would cost a wave per SIMD, once the step's codes are converted.
-  __device__ __forceinline__ void run(const A4Pages &pg, uint32_t t0, uint32_t t_end) {
-    constexpr uint32_t stride = ATT_WAVES * A4_STEP;
+  __device__ __forceinline__ void run(const A4Pages &pg, uint32_t t0, uint32_t t_end, uint32_t stride) {
     constexpr bool AHEAD = D * CT <= 64;
     const uint32_t t_last = t_end - 1;
     struct Step {
@@ -439,18 +437,29 @@ template <int D, int CT, bool EXACT> struct A4Wave {
     }
   }
 
+  // The sum of column 16 ct + n's weights.
+  __device__ __forceinline__ float row_sum(int ct) const {
+    if constexpr (!EXACT) return ol[ct][0];
+    float x, y;
+    xrow_pair32(l[ct], x, y);
+    xrow_pair16(x + y, x, y);
+    return x + y;
+  }
+  // Column 16 ct + n's finished row (`row`: its D channels) from the wave's own keys alone.
+  __device__ __forceinline__ void store_row(int ct, float sum, uint16_t *row) const {
+    const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+    for (int jt = 0; jt < NT; ++jt)
+      *reinterpret_cast<uint2 *>(row + 16 * jt + 4 * kg) =
+          sum == 0.0f ? make_uint2(0u, 0u)
+                      : make_uint2(pack_bf16(o[ct][jt][0] * f, o[ct][jt][1] * f), pack_bf16(o[ct][jt][2] * f, o[ct][jt][3] * f));
+  }
   // Tile ct's accumulators into the wave's LDS (in the place of V), [column][channel], and its
   // columns' maxima and sums; the first `live` columns.
   __device__ __forceinline__ void spill(int ct, int live, float *sm_m, float *sm_l) {
     static_assert(A4_HEADS * Lds::AROW * 4 <= Lds::WAVE, "a tile of O fits where V was");
     float *acc = reinterpret_cast<float *>(vt);
-    float sum = ol[ct][0];
-    if constexpr (EXACT) {
-      float x, y;
-      xrow_pair32(l[ct], x, y);
-      xrow_pair16(x + y, x, y);
-      sum = x + y;
-    }
+    const float sum = row_sum(ct);
     if (n >= live) return;
 #pragma unroll
     for (int jt = 0; jt < NT; ++jt) *reinterpret_cast<att_f32x4 *>(acc + n * Lds::AROW + 16 * jt + 4 * kg) = o[ct][jt];
@@ -600,7 +609,7 @@ paged_decode4_kernel(const uint16_t *__restrict__ q, AttnGeom g, A4Rows qr, cons
       }
       w.clear();
       const uint32_t t0 = t_begin + (uint32_t)wave * A4_STEP;
-      if (t0 < t_end) w.run(pg, t0, t_end);
+      if (t0 < t_end) w.run(pg, t0, t_end, ATT_WAVES * A4_STEP);
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) {
         if (16 * ct >= cols) break;  // block-uniform
@@ -648,7 +657,7 @@ decode4_rows_combine_kernel(const float *__restrict__ part, AttnGeom g, A4Rows q
 // to the operand without LDS, every conversion serves CT products, and a K/V byte read serves
 // 16 CT columns: what a block reads is small, the pages have 4 bits.  Bound by the issue of the
 // matrix products, the conversions and the exponentials together: 2 x 2,048 rows on 4k and 14k
-// positions, 32/8 heads, D = 128, 714 us or 937 TFLOP/s, matrix cores busy 41% and vector units
+// positions, 32/8 heads, D = 128, 724 us or 925 TFLOP/s, matrix cores busy 41% and vector units
 // 52% of the time; a library product of 8,192^3 reaches 1,109.
 // With few tiles a tile's keys are shared by up to n_split blocks, whose parts
 // prefill4_combine_kernel merges.
@@ -662,7 +671,8 @@ struct Prefill4Args {
   int64_t n_pages;
   int32_t n_q_heads, n_kv_heads, page_size, max_blocks, n_seqs, causal;
   int32_t group, n_group;  // heads per block, groups of them
-  int32_t by_length;       // tiles of the longest sequence first (one part per tile, 2 to 64 sequences)
+  int32_t order;           // P4Order (one part per tile, up to 64 sequences)
+  uint32_t slots;          // blocks that the chip holds
   int32_t rows;            // query rows per tile: 16 CT / group
   int32_t n_rt, n_split;   // row tiles per sequence, the most blocks per tile
   uint32_t n_items;        // tiles: n_rt * n_group * n_seqs
@@ -687,34 +697,79 @@ __device__ __forceinline__ int p4_parts(const Prefill4Args &a, uint32_t keys) {
   return max(1, min(a.n_split, (int)((keys + P4_UNIT - 1) / P4_UNIT / P4_PART)));
 }
 
-// The s-th longest of up to 64 sequences (of equal ones the first).
-__device__ __forceinline__ int p4_nth_longest(const Prefill4Args &a, int s) {
-  const int lane = threadIdx.x & 63;
-  const int32_t len = lane < a.n_seqs ? a.kv_len[lane] : 0;
-  int before = 0;
-  for (int i = 0; i < a.n_seqs; ++i) {
-    const int32_t other = __builtin_amdgcn_readlane(len, i);
-    before += other > len || (other == len && i < lane);
+// Up to 64 sequences, lane b holding sequence b: which come first, and whether a wave takes a tile
+// by itself.  A tile that four waves share costs about 6 us of a block's time besides its steps
+// (four starts, the merge), one of a wave's own 4 us of a wave's, but the launch then ends with
+// whole tiles: a step is 1.8 us of a wave's time.  So by themselves if the tiles are many for
+// their length: 7 times the tiles per block slot exceed the longest one's steps.  4 x 2,048 new
+// rows, 32/8 heads, D = 128, shared 218 us, alone 193; 9 x 227-455 rows, 32/8 heads, D = 64 40 / 28;
+// 8 x 768 rows on 1,024 keys 160 / 129.  2 x 2,048 rows on 4k and 14k stay shared.
+struct P4Order {
+  int32_t lo, hi, len, pos0;
+  int before;  // sequences before this lane's
+  bool alone;
+  __device__ __forceinline__ explicit P4Order(const Prefill4Args &a) : lo(0), hi(0), len(0), pos0(0), before(0) {
+    const int lane = threadIdx.x & 63;
+    if (lane < a.n_seqs) {
+      lo = a.cu_q[lane];
+      hi = a.cu_q[lane + 1];
+      len = a.kv_len[lane];
+      pos0 = a.q_pos0[lane];
+    }
+    int32_t e = 0;
+    const int32_t rows = a4_rows(lo, hi, a.n_q, a.max_q, e);
+    const uint32_t tiles = (uint32_t)((rows + a.rows - 1) / a.rows) * (uint32_t)a.n_group;
+    const uint32_t steps = rows > 0 ? (p4_keys(a, len, pos0, rows) + A4_STEP - 1) / A4_STEP : 0u;
+    uint64_t all = 0;
+    uint32_t most = 0;
+    for (int i = 0; i < a.n_seqs; ++i) {
+      const int32_t other = __builtin_amdgcn_readlane(len, i);
+      before += other > len || (other == len && i < lane);
+      all += (uint32_t)__builtin_amdgcn_readlane((int)tiles, i);
+      most = max(most, (uint32_t)__builtin_amdgcn_readlane((int)steps, i));
+    }
+    alone = 7 * all > (uint64_t)a.slots * most;
   }
-  return __ffsll((long long)__ballot(lane < a.n_seqs && before == s)) - 1;
-}
+};
 
 template <int D, int CT, bool EXACT>
 __global__ void __launch_bounds__(ATT_THREADS, a4_per_cu(D, CT)) paged_prefill4_kernel(Prefill4Args a) {
   // the sequence with the most keys first, its last row tiles first (under a causal mask they
   // see the most): the chip is left with short tiles at the end; a tile's parts next to each other
-  const uint32_t item = blockIdx.x / (uint32_t)a.n_split;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  uint32_t item = blockIdx.x / (uint32_t)a.n_split;
   const int split = (int)(blockIdx.x - item * (uint32_t)a.n_split);
+  bool alone = false;  // every wave has a tile
   const uint32_t per_seq = (uint32_t)a.n_group * (uint32_t)a.n_rt;
-  const uint32_t s = item / per_seq, rem = item - s * per_seq;
-  const int b = a.by_length ? p4_nth_longest(a, (int)s) : (int)s;
+  uint32_t s = item / per_seq;
+  int b = (int)s;
+  int32_t lo, hi, kv_len;
+  int64_t pos0;
+  if (a.order) {
+    const P4Order o(a);
+    alone = o.alone;
+    if (alone) {
+      item = blockIdx.x * ATT_WAVES + wave;
+      s = item / per_seq;
+    }
+    if (item >= a.n_items) return;
+    b = __ffsll((long long)__ballot((int)(threadIdx.x & 63) < a.n_seqs && o.before == (int)s)) - 1;
+    lo = __builtin_amdgcn_readlane(o.lo, b);
+    hi = __builtin_amdgcn_readlane(o.hi, b);
+    kv_len = __builtin_amdgcn_readlane(o.len, b);
+    pos0 = __builtin_amdgcn_readlane(o.pos0, b);
+  } else {
+    lo = a.cu_q[b];
+    hi = a.cu_q[b + 1];
+    kv_len = a.kv_len[b];
+    pos0 = a.q_pos0[b];
+  }
+  const uint32_t rem = item - s * per_seq;
   const uint32_t rt_rev = rem / (uint32_t)a.n_group;
   const int y = (int)(rem - rt_rev * (uint32_t)a.n_group);
   const int grp = a.n_q_heads / a.n_kv_heads, per_kv = a.n_group / a.n_kv_heads;
   const int h = y / per_kv, first = (y - h * per_kv) * a.group;
   const int G = min(a.group, grp - first), hq0 = h * grp + first;
-  const int32_t lo = a.cu_q[b], hi = a.cu_q[b + 1], kv_len = a.kv_len[b];
-  const int64_t pos0 = a.q_pos0[b];
   int32_t e = 0;
   const int32_t rows = a4_rows(lo, hi, a.n_q, a.max_q, e);
   if (kv_len > (int64_t)a.max_blocks * a.page_size) e |= ZX_KERR_POS_RANGE;
@@ -729,7 +784,6 @@ __global__ void __launch_bounds__(ATT_THREADS, a4_per_cu(D, CT)) paged_prefill4_
   const uint32_t units = (end + P4_UNIT - 1) / P4_UNIT;  // below 2^24, and at most 64 parts
   const uint32_t t_begin = units * (uint32_t)split / (uint32_t)parts * P4_UNIT;
   const uint32_t t_end = min(end, units * (uint32_t)(split + 1) / (uint32_t)parts * P4_UNIT);
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t head_bytes = (int64_t)(a.page_size / K4_TOK) * k4_tile_bytes(D);
   A4Pages pg;
   pg.pool = a.pool;
@@ -755,8 +809,21 @@ __global__ void __launch_bounds__(ATT_THREADS, a4_per_cu(D, CT)) paged_prefill4_
   }
   w.lim_all = a.causal ? (uint32_t)max((int64_t)0, min((int64_t)end, pos0 + row0 + 1)) : end;
   w.clear();
-  const uint32_t t0 = t_begin + (uint32_t)wave * A4_STEP;
-  if (t0 < t_end) w.run(pg, t0, t_end);
+  const uint32_t t0 = t_begin + (alone ? 0u : (uint32_t)wave * A4_STEP);
+  // (readfirstlane: one loop for both strides.  Where it sees two, the compiler loses the products
+  // with V and everything after them)
+  const int stride = __builtin_amdgcn_readfirstlane(alone ? A4_STEP : ATT_WAVES * A4_STEP);
+  if (t0 < t_end) w.run(pg, t0, t_end, (uint32_t)stride);
+  if (alone) {
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      const int c = 16 * ct + w.n, r = c / G;
+      const float sum = w.row_sum(ct);
+      if (c < cols) w.store_row(ct, sum, a.out + ((lo + row0 + r) * a.n_q_heads + hq0 + (c - r * G)) * (int64_t)D);
+    }
+    if (w.e && a.err) atomicOr(a.err, w.e);
+    return;
+  }
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {  // one tile of columns after the other
     if (16 * ct >= cols) break;      // block-uniform
@@ -1020,7 +1087,8 @@ extern "C" int zx_paged_attention4_prefill(const uint16_t *q, int64_t n_q, const
   a.n_q = n_q;
   a.sm_log2e = sm_scale * ATT_LOG2E;
   a.n_split = room && !p.runs ? (int32_t)p.n_split : 1;
-  a.by_length = a.n_split == 1 && n_seqs > 1 && n_seqs <= 64;
+  a.order = a.n_split == 1 && n_seqs <= 64;
+  a.slots = (uint32_t)(a4_per_cu(head_dim, p.ct) * num_cus());
   {
     int sh = 0;
     while ((1LL << sh) < page_size) ++sh;
