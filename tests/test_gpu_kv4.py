@@ -495,6 +495,22 @@ def test_prefill_of_many_tiles_with_few_keys(dev, Hq, H, D, P, precision):
                     [rows[i] for i in check], [old[i] for i in check], True)
 
 
+def test_prefill_flags_of_sequences_without_rows(dev):
+    """A sequence that computes no row but claims more keys than its table holds is flagged
+    wherever its tiles fall (one tile per sequence and head, a wave each)."""
+    H, D, P = 1, 64, 16
+    pool = kv.kv4_pool(1, 64, H, P, D)
+    bt = torch.arange(64, dtype=torch.int32, device=dev)[:, None].contiguous()
+    for rows_of, bad in ((70, 1), (70, 2), (70, 3), (70, 62)):
+        rows = [0 if b == bad else rows_of for b in range(63)]
+        q = torch.zeros((sum(rows), 1, D), dtype=torch.bfloat16, device=dev)
+        lens = [17 if b == bad else 16 for b in range(63)]
+        err = torch.zeros(1, dtype=torch.int32, device=dev)
+        kv.paged_attention4_prefill(q, i32(np.concatenate([[0], np.cumsum(rows)]), dev), i32([0] * 63, dev), pool[0],
+                                    bt[:63], i32(lens, dev), max_q_per_seq=rows_of, err=err)
+        assert err.item() == N.ZX_KERR_POS_RANGE, bad
+
+
 def test_prefill_of_many_short_sequences(dev):
     """More than 64 sequences of 0 to 6 rows: dealt by a table, in runs and whole."""
     H, Hq, D, P = 2, 8, 128, 16

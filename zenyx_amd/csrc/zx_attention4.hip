@@ -777,8 +777,8 @@ __global__ void __launch_bounds__(ATT_THREADS, a4_per_cu(D, CT)) paged_prefill4_
   const int n_rows = (int)max((int64_t)0, min((int64_t)a.rows, rows - row0));
   const uint32_t end = p4_keys(a, kv_len, pos0, row0 + n_rows);
   const int parts = p4_parts(a, end);
-  if (n_rows == 0 || split >= parts) {  // block-uniform
-    if (e && a.err && threadIdx.x == 0) atomicOr(a.err, e);
+  if (n_rows == 0 || split >= parts) {  // block-uniform, or the wave's own
+    if (e && a.err && (threadIdx.x & 63) == 0) atomicOr(a.err, e);
     return;
   }
   const uint32_t units = (end + P4_UNIT - 1) / P4_UNIT;  // below 2^24, and at most 64 parts
