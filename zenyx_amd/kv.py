@@ -938,7 +938,7 @@ def rope(x: torch.Tensor, table: torch.Tensor, positions: torch.Tensor, interlea
     if not (_fits(table, index) and _fits(positions, index)):
         _all_on(index, table=table, positions=positions)
     if out is None:
-        out = torch.empty((n, H, D), dtype=x.dtype, device=x.device)
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
         o_row, o_head = H * D, D
     else:
         if out.shape != x.shape or out.dtype != x.dtype or out.device != x.device:
@@ -1006,8 +1006,10 @@ def kv_rope_append(x: torch.Tensor, table: torch.Tensor, cu_seqlens: torch.Tenso
     if two_pass and single_pass:
         raise ValueError("kv_rope_append: two_pass and single_pass are exclusive")
     index = x.get_device()
-    _all_on(index, x=x, table=table, cu_seqlens=cu_seqlens, block_tables=block_tables, pool=pool, scales=scales,
-            start_pos=start_pos)
+    if not (_fits(x, index) and _fits(table, index) and _fits(cu_seqlens, index) and _fits(block_tables, index) and
+            _fits(pool, index) and _fits(scales, index) and (start_pos is None or _fits(start_pos, index))):
+        _all_on(index, x=x, table=table, cu_seqlens=cu_seqlens, block_tables=block_tables, pool=pool, scales=scales,
+                start_pos=start_pos)
     flags = (N.ZX_APPEND_STATIC_SCALES if static_scales else 0) | (N.ZX_APPEND_SATURATE if saturate else 0) | \
         (N.ZX_ROPE_INTERLEAVED if interleaved else 0) | (N.ZX_APPEND_TWO_PASS if two_pass else 0) | \
         (N.ZX_APPEND_SINGLE_PASS if single_pass else 0)
@@ -1069,7 +1071,10 @@ def kv4_append(x: torch.Tensor, cu_seqlens: torch.Tensor, block_tables: torch.Te
     n_pos, rot = _rope_table_of(table, D) if table is not None else (0, 0)
     _append_args(x, cu_seqlens, block_tables, start_pos, err)
     index = x.get_device()
-    _all_on(index, x=x, table=table, cu_seqlens=cu_seqlens, block_tables=block_tables, pool=pool, start_pos=start_pos)
+    if not (_fits(x, index) and _fits(cu_seqlens, index) and _fits(block_tables, index) and _fits(pool, index) and
+            (table is None or _fits(table, index)) and (start_pos is None or _fits(start_pos, index))):
+        _all_on(index, x=x, table=table, cu_seqlens=cu_seqlens, block_tables=block_tables, pool=pool,
+                start_pos=start_pos)
     with _on(index):
         ws, nb = _workspace_for("zx_kv4_append_workspace_bytes", index, L, T, H)
         err = _err_word_if(check, x.device) if err is None else err
@@ -1099,7 +1104,8 @@ def kv4_gather_dequant(pool_layer: torch.Tensor, block_tables: torch.Tensor, seq
     if out_len is None:
         out_len = block_tables.shape[1] * P
     dev, index = pool_layer.device, pool_layer.get_device()
-    _all_on(index, pool_layer=pool_layer, block_tables=block_tables, seq_lens=seq_lens)
+    if not (_fits(pool_layer, index) and _fits(block_tables, index) and _fits(seq_lens, index)):
+        _all_on(index, pool_layer=pool_layer, block_tables=block_tables, seq_lens=seq_lens)
     if out is None:
         k = torch.empty((B, H, out_len, D), dtype=torch.bfloat16, device=dev)
         v = torch.empty_like(k)
@@ -1144,7 +1150,7 @@ def paged_attention4_decode(q: torch.Tensor, pool_layer: torch.Tensor, block_tab
     if block_tables.shape[0] != B or seq_lens.numel() != B or seq_lens.dtype != torch.int32:
         raise ValueError("block_tables and seq_lens (int32) need one row per sequence")
     q, index = q.contiguous(), q.get_device()
-    out = torch.empty((B, Hq, D), dtype=torch.bfloat16, device=q.device) if out is None else out
+    out = torch.empty_like(q) if out is None else out
     if not (_fits(q, index) and _fits(pool_layer, index) and _fits(block_tables, index) and _fits(seq_lens, index) and
             _fits(out, index)):
         _all_on(index, q=q, pool_layer=pool_layer, block_tables=block_tables, seq_lens=seq_lens, out=out)
