@@ -530,6 +530,26 @@ def test_prefill_of_many_short_sequences(dev):
         check_attention(out, q, pool, bt, lens, D ** -0.5, 2.0 ** -16, rows, old, True)
 
 
+@pytest.mark.parametrize("n_seqs, most, Hq, H, D", [(66, 60, 2, 2, 128), (66, 90, 2, 1, 64), (260, 2, 16, 16, 128),
+                                                    (70, 20, 1, 1, 256), (130, 3, 32, 32, 64)])
+def test_prefill_of_more_than_64_sequences_in_tiles(dev, n_seqs, most, Hq, H, D):
+    """Several tiles per sequence, or so many of one that they are not dealt in runs."""
+    rng = np.random.default_rng(n_seqs + D)
+    rows = rng.integers(0, most + 1, n_seqs).tolist()
+    rows[1] = most
+    old = rng.integers(0, 40, n_seqs).tolist()
+    lens = [a + b for a, b in zip(rows, old)]
+    bt, n_pages = tables(lens, 16, 0, 1)
+    pool = random_pool(n_pages, H, 16, D, 1)
+    q = torch.randn((sum(rows) + 1, Hq, D), device=dev).to(torch.bfloat16)
+    out = torch.full_like(q, 5.0)
+    cu = i32(np.concatenate([[0], np.cumsum(rows)]), dev)
+    kv.paged_attention4_prefill(q, cu, i32(old, dev), torch.from_numpy(pool).to(dev), i32(bt, dev), i32(lens, dev),
+                                precision="exact", out=out, max_q_per_seq=most, check=True)
+    assert torch.all(out[-1] == 5)
+    check_attention(out, q, pool, bt, lens, D ** -0.5, 2.0 ** -16, rows, old, True)
+
+
 @pytest.mark.parametrize("sm", [0.0, -0.3, 1e-6, 4.0])
 def test_prefill_scales(dev, sm):
     for rows, old, Hq, H, D in (([3, 1], [90, 20], 4, 2, 128), ([60], [10], 4, 4, 64)):
