@@ -857,6 +857,14 @@ def _on(index: int):
     return _same_device if torch._C._cuda_getDevice() == index else torch.cuda.device(index)
 
 
+def _index(t: torch.Tensor, name: str) -> int:
+    """The device of a call's first tensor; the others are held to it (host tensors, all of which
+    have index -1, would otherwise agree with each other)."""
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a HIP device tensor, got {t.device}")
+    return t.get_device()
+
+
 def _fits(t: torch.Tensor, index: int) -> bool:
     return t.get_device() == index and t.is_contiguous() and not t.data_ptr() & 15
 
@@ -909,8 +917,6 @@ def _rows_of(t: torch.Tensor, name: str) -> tuple[int, int]:
     """The row and head strides of ``[n, H, D]`` rows that the kernel can take."""
     vec = 16 // t.element_size()
     row, head, channel = t.stride()
-    if not t.is_cuda:
-        raise ValueError(f"{name} must be a HIP device tensor, got {t.device}")
     if channel != 1 or row % vec or head % vec or t.data_ptr() & 15:
         raise ValueError(f"{name}: channels must be contiguous and every head's row 16-byte aligned")
     return row, head
@@ -933,7 +939,7 @@ def rope(x: torch.Tensor, table: torch.Tensor, positions: torch.Tensor, interlea
         raise ValueError(f"positions must be int32 [{n}]")
     if H == 0 or D == 0:
         raise ValueError("x has no heads or no channels")
-    index = x.get_device()
+    index = _index(x, "x")
     x_row, x_head = _rows_of(x, "x")
     if not (_fits(table, index) and _fits(positions, index)):
         _all_on(index, table=table, positions=positions)
@@ -1005,7 +1011,7 @@ def kv_rope_append(x: torch.Tensor, table: torch.Tensor, cu_seqlens: torch.Tenso
         raise ValueError("saturate applies to static scales (dynamic scales never overflow)")
     if two_pass and single_pass:
         raise ValueError("kv_rope_append: two_pass and single_pass are exclusive")
-    index = x.get_device()
+    index = _index(x, "x")
     if not (_fits(x, index) and _fits(table, index) and _fits(cu_seqlens, index) and _fits(block_tables, index) and
             _fits(pool, index) and _fits(scales, index) and (start_pos is None or _fits(start_pos, index))):
         _all_on(index, x=x, table=table, cu_seqlens=cu_seqlens, block_tables=block_tables, pool=pool, scales=scales,
@@ -1070,7 +1076,7 @@ def kv4_append(x: torch.Tensor, cu_seqlens: torch.Tensor, block_tables: torch.Te
         raise ValueError("interleaved needs a table")
     n_pos, rot = _rope_table_of(table, D) if table is not None else (0, 0)
     _append_args(x, cu_seqlens, block_tables, start_pos, err)
-    index = x.get_device()
+    index = _index(x, "x")
     if not (_fits(x, index) and _fits(cu_seqlens, index) and _fits(block_tables, index) and _fits(pool, index) and
             (table is None or _fits(table, index)) and (start_pos is None or _fits(start_pos, index))):
         _all_on(index, x=x, table=table, cu_seqlens=cu_seqlens, block_tables=block_tables, pool=pool,
@@ -1103,7 +1109,7 @@ def kv4_gather_dequant(pool_layer: torch.Tensor, block_tables: torch.Tensor, seq
         raise ValueError("seq_lens must have one entry per block-table row")
     if out_len is None:
         out_len = block_tables.shape[1] * P
-    dev, index = pool_layer.device, pool_layer.get_device()
+    dev, index = pool_layer.device, _index(pool_layer, "pool_layer")
     if not (_fits(pool_layer, index) and _fits(block_tables, index) and _fits(seq_lens, index)):
         _all_on(index, pool_layer=pool_layer, block_tables=block_tables, seq_lens=seq_lens)
     if out is None:
@@ -1149,7 +1155,7 @@ def paged_attention4_decode(q: torch.Tensor, pool_layer: torch.Tensor, block_tab
     B, Hq, _ = q.shape
     if block_tables.shape[0] != B or seq_lens.numel() != B or seq_lens.dtype != torch.int32:
         raise ValueError("block_tables and seq_lens (int32) need one row per sequence")
-    q, index = q.contiguous(), q.get_device()
+    q, index = q.contiguous(), _index(q, "q")
     out = torch.empty_like(q) if out is None else out
     if not (_fits(q, index) and _fits(pool_layer, index) and _fits(block_tables, index) and _fits(seq_lens, index) and
             _fits(out, index)):
@@ -1195,8 +1201,8 @@ def paged_attention4_prefill(q: torch.Tensor, cu_q: torch.Tensor, q_pos0: torch.
             raise ValueError(f"{name} must be int32 [{n}]")
     if err is not None and (err.dtype != torch.int32 or err.numel() < 1 or err.device != q.device):
         raise ValueError("err must be an int32 tensor on q's device")
+    index = _index(q, "q")
     out = torch.empty_like(q) if out is None else out
-    index = q.get_device()
     _all_on(index, q=q, cu_q=cu_q, q_pos0=q_pos0, pool_layer=pool_layer, block_tables=block_tables, kv_len=kv_len,
             out=out)
     if max_q_per_seq is None:
