@@ -475,9 +475,9 @@ int zx_rope_table(const double *inv_freq, int32_t rot_dim, int64_t n_pos, double
                   zx_stream_t stream);
 /* Rows x[n_rows][n_heads][head_dim] of `dtype`, strides in elements (channels contiguous, rows
  * of a head 16-byte aligned), row i at positions[i] (device int32).  Channels from rot_dim on
- * are copied.  out may be x (then with its strides) and must not overlap it otherwise.  A row
- * whose position is outside [0, n_pos) is copied and sets ZX_KERR_POS_RANGE in *err (may be
- * NULL).  head_dim is a multiple of 8. */
+ * are copied.  out may be x (then with its strides) and must not overlap it otherwise;
+ * no two of its rows may overlap.  A row whose position is outside [0, n_pos) is copied and sets
+ * ZX_KERR_POS_RANGE in *err (may be NULL).  head_dim is a multiple of 8. */
 int zx_rope(const void *x, int dtype, int64_t n_rows, int32_t n_heads, int32_t head_dim, int64_t x_row_stride,
             int64_t x_head_stride, const float *table, int64_t n_pos, int32_t rot_dim, const int32_t *positions,
             int32_t flags, void *out, int64_t out_row_stride, int64_t out_head_stride, int32_t *err,

@@ -445,3 +445,28 @@ def test_append_in_a_graph(dev, single):
         torch.cuda.synchronize()
         for pool, sc in zip(pools, scales):
             assert torch.equal(pool, want) and same_bits(sc, s)
+
+
+@pytest.mark.parametrize("n, H, D, row, head", [
+    (2, 3, 16, 64, 48), (3, 2, 16, 16, 64), (2, 3, 16, 16, 32), (1, 4, 16, 0, 16), (4, 1, 16, 16, 0), (7, 5, 32, 32, 7 * 32),
+    (2, 2, 32, 36, 72), (3, 3, 16, 116, 40)])
+def test_an_out_whose_rows_lie_between_each_other(dev, n, H, D, row, head):
+    """Any strides whose rows do not overlap are written, and nothing between the rows is."""
+    x = torch.randn((n, H, D), device=dev)
+    table, p = table64(9, 16, dev), torch.randint(0, 9, (n,), dtype=torch.int32, device=dev)
+    room = torch.full(((n - 1) * row + (H - 1) * head + D + 4,), 7.0, device=dev)
+    out = room.as_strided((n, H, D), (row, head, 1))
+    want = torch.full_like(room, 7.0)
+    want.as_strided((n, H, D), (row, head, 1)).copy_(kv.rope(x, table, p))
+    assert kv.rope(x, table, p, out=out) is out
+    assert same_bits(room, want)
+
+
+def test_an_out_whose_rows_overlap_is_refused(dev):
+    x = torch.randn((4, 2, 64), device=dev)
+    table, p = table64(9, 64, dev), torch.zeros(4, dtype=torch.int32, device=dev)
+    room = torch.zeros(1000, device=dev)
+    for row, head in ((64, 64), (72, 64), (64, 72), (64, 128)):
+        with pytest.raises(ValueError, match="overlap"):
+            kv.rope(x, table, p, out=room.as_strided((4, 2, 64), (row, head, 1)))
+    assert not room.any()

@@ -183,3 +183,17 @@ def test_ctypes_signatures_cover_the_new_entry_points():
     for name in ("zx_rope", "zx_rope_table", "zx_kv_rope_append", "zx_kv4_append", "zx_kv4_gather_dequant",
                  "zx_paged_attention4_decode", "zx_paged_attention4_prefill"):
         assert name in N.SIGNATURES and isinstance(getattr(N.load(), name), ctypes._CFuncPtr)
+
+
+@pytest.mark.parametrize("n, H, D, row, head", [
+    (4, 2, 64, 64, 64),    # row 1 of head 0 is row 0 of head 1
+    (2, 2, 64, 72, 64),    # half-way into it
+    (2, 2, 64, 64, 72), (3, 5, 64, 256, 64), (2, 3, 64, 144, 128), (2, 8, 64, 192 + 56, 64),
+    (1000, 3, 64, 64, 64 * 999), (2, 2, 64, 0, 64), (2, 2, 64, 128, 0), (5, 4, 64, 72, 96)])
+def test_rope_refuses_an_out_whose_rows_overlap(lib, n, H, D, row, head):
+    cells = [(i * row + j * head) for i in range(n) for j in range(H)]
+    cells.sort()
+    assert min(b - a for a, b in zip(cells, cells[1:])) < D  # they do
+    assert lib.zx_rope(*rope_args(n=n, H=H, D=D, xr=H * D, xh=D, outr=row, outh=head)) == N.ZX_ERR_INVALID
+    assert b"overlap" in lib.zx_last_error()
+    assert lib.zx_rope(*rope_args(n=n, H=H, D=D, xr=row, xh=head, outr=row, outh=head, out=P)) == N.ZX_ERR_INVALID

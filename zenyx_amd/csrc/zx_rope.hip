@@ -324,6 +324,24 @@ extern "C" int zx_rope_table(const double *inv_freq, int32_t rot_dim, int64_t n_
   return check_launch("rope_table");
 }
 
+// Whether two of n x heads rows of d elements, `row` and `head` elements apart, share one: is some
+// (i, j) != (0, 0), |i| < n, |j| < heads, with |i row + j head| < d?  (128 bits: a stride is anything.)
+static bool rope_rows_overlap(int64_t n, int64_t heads, int64_t row, int64_t head, int64_t d) {
+  if ((n > 1 && row < d) || (heads > 1 && head < d)) return true;
+  if (n == 1 || heads == 1) return false;
+  typedef __int128 wide;
+  const bool by_head = head <= row;
+  const wide small = by_head ? head : row, n_small = by_head ? heads : n, large = by_head ? row : head;
+  const int64_t n_large = by_head ? n : heads;
+  const wide last = (n_small - 1) * small;  // where the last of the near ones begins
+  for (int64_t k = 1; k < n_large && k * large < last + d; ++k) {  // (the usual layouts: no step)
+    const wide at = k * large, below = at / small;
+    if (at - std::min(below, n_small - 1) * small < d) return true;
+    if (below + 1 < n_small && (below + 1) * small - at < d) return true;
+  }
+  return false;
+}
+
 extern "C" int zx_rope(const void *x, int dtype, int64_t n_rows, int32_t n_heads, int32_t head_dim, int64_t x_row_stride,
                        int64_t x_head_stride, const float *table, int64_t n_pos, int32_t rot_dim,
                        const int32_t *positions, int32_t flags, void *out, int64_t out_row_stride,
@@ -363,6 +381,8 @@ extern "C" int zx_rope(const void *x, int dtype, int64_t n_rows, int32_t n_heads
   a.units = (uint32_t)(rot_dim / 16 + (a.copy ? (head_dim - rot_dim) / 8 : 0));
   const int64_t threads = n_rows * n_heads * a.units;
   if (threads >= (1LL << 32) - 256) return fail(ZX_ERR_UNSUPPORTED, "rope: too many rows");
+  ZX_REQUIRE(!rope_rows_overlap(n_rows, n_heads, out_row_stride, out_head_stride, head_dim),
+             "rope: rows of out must not overlap");
   const unsigned blocks = (unsigned)ceil_div(threads, 256);
   const hipStream_t st = as_stream(stream);
   const bool inter = flags & ZX_ROPE_INTERLEAVED;

@@ -928,8 +928,9 @@ def rope(x: torch.Tensor, table: torch.Tensor, positions: torch.Tensor, interlea
     be given, e.g. the queries of a fused projection) at ``positions`` (int32 ``[n]``) of
     ``table`` (``rope_table``).  Pair i of the first rot_dim channels is (i, i + rot_dim / 2),
     or (2 i, 2 i + 1) when ``interleaved``; later channels are copied.  ``transpose`` applies
-    the transposed rotation, which takes a gradient back.  ``out`` may be ``x`` itself.  A row
-    at a position the table does not have is copied (``check`` synchronises and raises)."""
+    the transposed rotation, which takes a gradient back.  ``out`` may be ``x`` itself; no two of
+    its rows may overlap.  A row at a position the table does not have is copied (``check``
+    synchronises and raises)."""
     N.need_gpu()
     if x.dim() != 3 or x.dtype not in _DT:
         raise ValueError("x must be [n, n_heads, head_dim] in bf16, f16 or f32")
@@ -950,8 +951,6 @@ def rope(x: torch.Tensor, table: torch.Tensor, positions: torch.Tensor, interlea
         if out.shape != x.shape or out.dtype != x.dtype or out.device != x.device:
             raise ValueError("out must be like x")
         o_row, o_head = _rows_of(out, "out")
-        if n > 1 and o_row < D or H > 1 and o_head < D:
-            raise ValueError("out: rows must not overlap")
         if n and not (out.data_ptr() == x.data_ptr() and out.stride() == x.stride()):
             (a, z), (b, y) = ((t.data_ptr(), t.data_ptr() + t.element_size() * (
                 (n - 1) * t.stride(0) + (H - 1) * t.stride(1) + D)) for t in (x, out))
