@@ -470,3 +470,22 @@ def test_an_out_whose_rows_overlap_is_refused(dev):
         with pytest.raises(ValueError, match="overlap"):
             kv.rope(x, table, p, out=room.as_strided((4, 2, 64), (row, head, 1)))
     assert not room.any()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_gradient_at_any_alignment(dev, dtype):
+    """A gradient arrives as autograd lays it out: at an odd offset, expanded, with other strides."""
+    rope = RotaryPositions(32, 20, rotary_dim=16)
+    x = torch.randn((5, 2, 32), device=dev).to(dtype).requires_grad_()
+    p = torch.randint(0, 20, (5,), dtype=torch.int32, device=dev)
+    g = torch.randn(320 + 7, device=dev).to(dtype)
+
+    def back(t):
+        return kv.rope(t.contiguous().clone(), rope.table, p, transpose=True)
+    for lead in (0, 1, 3, 7):
+        got, = torch.autograd.grad(torch.cat([g[:lead], rope(x, p).flatten()]), x, g[:320 + lead])
+        assert same_bits(got, back(g[lead:320 + lead].view(5, 2, 32))), lead
+    got, = torch.autograd.grad(rope(x, p).sum(), x)
+    assert same_bits(got, back(torch.ones((5, 2, 32), device=dev, dtype=dtype)))
+    got, = torch.autograd.grad(rope(x, p).transpose(0, 2).contiguous(), x, g[:320].view(32, 2, 5))
+    assert same_bits(got, back(g[:320].view(32, 2, 5).transpose(0, 2)))

@@ -5,6 +5,7 @@ import torch
 
 from zenyx_amd import _native as N
 from zenyx_amd import kv
+from zenyx_amd.train.rotary import RotaryPositions
 
 
 class Recorder:
@@ -69,3 +70,47 @@ def test_calls_with_host_tensors_alone_are_refused(lib, name):
     with pytest.raises(ValueError, match="HIP device tensor"):
         host_calls()[name]()
     assert not [c for c, _ in lib.calls if not c.endswith("workspace_bytes")]
+
+
+# ------------------------------------------------------------------ RotaryPositions as an operation
+
+def plain_rope(x, table, positions, interleaved=False, transpose=False, out=None, check=False):
+    """kv.rope by torch operations that autograd does not see (as it does not see the kernel), with
+    its demand on alignment."""
+    if x.data_ptr() % 16:
+        raise ValueError("every head's row must be 16-byte aligned")
+    y = torch.tensor(x.tolist(), dtype=x.dtype).view(x.shape)
+    n = table.shape[1] // 2
+    c, s = (t[:, None] for t in table[positions.long()].split(n, 1))
+    s = -s if transpose else s
+    first, second = (slice(0, 2 * n, 2), slice(1, 2 * n, 2)) if interleaved else (slice(0, n), slice(n, 2 * n))
+    a, b = y[..., first].clone(), y[..., second].clone()
+    y[..., first], y[..., second] = a * c - b * s, b * c + a * s
+    return y
+
+
+@pytest.fixture(params=[False, True])
+def rotary(monkeypatch, request):
+    monkeypatch.setattr(kv, "rope", plain_rope)
+    f = torch.arange(8, dtype=torch.float64)
+    angle = torch.arange(20, dtype=torch.float64)[:, None] * 100.0 ** (-f / 8)
+    monkeypatch.setattr(kv, "rope_table", lambda *a: torch.cat([angle.cos(), angle.sin()], 1).float())
+    return RotaryPositions(24, 20, rotary_dim=16, interleaved=request.param, device=torch.device("cpu"))
+
+
+def test_gradients_at_any_alignment(rotary):
+    """The gradient of a slice of a concatenation begins wherever the slice does."""
+    p = torch.tensor([3, 0, 19], dtype=torch.int32)
+    x = torch.randn((3, 2, 24), requires_grad=True)
+    g = torch.randn(144 + 5)
+    for lead in (0, 1, 2, 3, 5):
+        y = torch.cat([torch.zeros(lead), rotary(x, p).flatten()])
+        got, = torch.autograd.grad((y * g[:144 + lead]).sum(), x)
+        want = plain_rope(g[lead:144 + lead].clone().view(3, 2, 24), rotary.table, p, rotary.interleaved, True)
+        assert torch.equal(got, want), lead
+    # an expanded gradient, and one that is not contiguous
+    got, = torch.autograd.grad(rotary(x, p).sum(), x)
+    assert torch.equal(got, plain_rope(torch.ones(3, 2, 24), rotary.table, p, rotary.interleaved, True))
+    got, = torch.autograd.grad((rotary(x, p).transpose(0, 2).contiguous() * g[:144].view(24, 2, 3)).sum(), x)
+    want = plain_rope(g[:144].view(24, 2, 3).transpose(0, 2).contiguous(), rotary.table, p, rotary.interleaved, True)
+    assert torch.equal(got, want)

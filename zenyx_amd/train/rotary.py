@@ -61,6 +61,13 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: dict | N
     return freq * (1 - ramp) + freq / factor * ramp, 0.1 * math.log(factor) + 1 if mult is None else float(mult)
 
 
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """``t`` as the kernel takes it: the caller has no say in how autograd lays a gradient out (one of a
+    slice of a concatenation is a view that begins anywhere)."""
+    t = t.contiguous()
+    return t.clone() if t.data_ptr() % 16 else t
+
+
 class _Rotate(torch.autograd.Function):
     """A linear map: its gradient is the transposed one, which is differentiable in its turn."""
 
@@ -73,7 +80,8 @@ class _Rotate(torch.autograd.Function):
     @staticmethod
     def backward(ctx, grad):
         table, positions = ctx.saved_tensors
-        return _Rotate.apply(grad.contiguous(), table, positions, ctx.interleaved, not ctx.transpose), None, None, None, None
+        return (_Rotate.apply(_rows(grad), table, positions, ctx.interleaved, not ctx.transpose),
+                None, None, None, None)
 
 
 class RotaryPositions:
