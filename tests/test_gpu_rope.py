@@ -7,9 +7,12 @@ exactly, and with float64 within what those roundings allow: 3 roundings of 2^-2
 products' magnitudes, and half a step (2^-8 bf16, 2^-11 fp16, 2^-24 fp32) of the result (fp16:
 2^-25 absolute below its normal range).  The append is compared to the bit with the rotation
 followed by the append that takes rotated keys."""
+import warnings
+
 import numpy as np
 import pytest
 import torch
+import torch.autograd.forward_ad as fwAD
 
 from oracle import kv4 as R
 from zenyx_amd import _native as N
@@ -489,3 +492,34 @@ def test_gradient_at_any_alignment(dev, dtype):
     assert same_bits(got, back(torch.ones((5, 2, 32), device=dev, dtype=dtype)))
     got, = torch.autograd.grad(rope(x, p).transpose(0, 2).contiguous(), x, g[:320].view(32, 2, 5))
     assert same_bits(got, back(g[:320].view(32, 2, 5).transpose(0, 2)))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_forward_mode_derivative(dev, dtype):
+    """The tangent turns with the values, to the bit, alone and where a gradient is asked for too; a
+    trace holds the kernel."""
+    rope = RotaryPositions(64, 50, rotary_dim=32, interleaved=True)
+    p = torch.randint(0, 50, (9,), dtype=torch.int32, device=dev)
+    x, v = torch.randn((2, 9, 4, 64), device=dev).to(dtype)
+    for primal in (x, x.clone().requires_grad_()):
+        with fwAD.dual_level():
+            out = fwAD.unpack_dual(rope(fwAD.make_dual(primal, v), p))
+            assert same_bits(out.primal.detach(), rope(x, p)) and same_bits(out.tangent.detach(), rope(v, p))
+    leaf, u = x.clone().requires_grad_(), torch.randn(x.shape, device=dev).to(dtype)
+    with fwAD.dual_level():  # the gradient's own tangent: d/de <u, (R (x + e v))^2> = R^T (2 u R v)
+        g, = torch.autograd.grad((rope(fwAD.make_dual(leaf, v), p).square() * u).sum(), leaf)
+        got = fwAD.unpack_dual(g).tangent
+    rv = rope(v, p).double()
+    want, near = 2 * u.double() * rv, 2 * u.double().abs() * rv.abs()
+    c, s = (t[:, None] for t in rope.table.double()[p.long()].split(16, 1))
+    a, b = want[..., 0:32:2].clone(), want[..., 1:32:2].clone()
+    want[..., 0:32:2], want[..., 1:32:2] = a * c + b * s, b * c - a * s
+    a, b = near[..., 0:32:2].clone(), near[..., 1:32:2].clone()
+    near[..., 0:32:2], near[..., 1:32:2] = a + b, a + b
+    # six roundings to the type on the way at most: the square's derivative (2), its tangent (2), their
+    # sum with u, the rotation
+    assert torch.all((got.double() - want).abs() <= 6 * HALF_STEP[dtype] * 1.05 * near + 1e-30)
+    with warnings.catch_warnings():
+        warnings.simplefilter("ignore")
+        traced = torch.jit.trace(lambda t: rope(t, p), (x,))
+    assert same_bits(traced(v), rope(v, p))

@@ -1,7 +1,10 @@
 """What the wrappers of rotary positions and 4-bit pages do before the library is called, without a
 GPU: the library is replaced by one that records its calls and launches nothing."""
+import warnings
+
 import pytest
 import torch
+import torch.autograd.forward_ad as fwAD
 
 from zenyx_amd import _native as N
 from zenyx_amd import kv
@@ -114,3 +117,49 @@ def test_gradients_at_any_alignment(rotary):
     got, = torch.autograd.grad((rotary(x, p).transpose(0, 2).contiguous() * g[:144].view(24, 2, 3)).sum(), x)
     want = plain_rope(g[:144].view(24, 2, 3).transpose(0, 2).contiguous(), rotary.table, p, rotary.interleaved, True)
     assert torch.equal(got, want)
+
+
+def test_forward_mode_derivatives(rotary):
+    """The rotation is linear: a tangent turns as the values do, with or without a gradient asked for,
+    at any alignment, and the two modes mix in either order."""
+    p = torch.tensor([3, 0, 19], dtype=torch.int32)
+    x, v = torch.randn((3, 2, 24)), torch.randn(145)[1:].view(3, 2, 24)
+    turned = plain_rope(v.clone(), rotary.table, p, rotary.interleaved)
+    for primal in (x, x.clone().requires_grad_()):
+        with fwAD.dual_level():
+            out = fwAD.unpack_dual(rotary(fwAD.make_dual(primal, v), p))
+            assert torch.equal(out.primal, rotary(x, p)) and out.tangent is not None
+            assert torch.equal(out.tangent, turned)
+            with torch.no_grad():  # (ends reverse mode alone)
+                assert torch.equal(fwAD.unpack_dual(rotary(fwAD.make_dual(primal, v), p)).tangent, turned)
+            assert fwAD.unpack_dual(rotary(primal, p)).tangent is None
+    # the tangent of a gradient: d/de of R^T sin(R (x + e v)) is R^T (cos(R x) * R v)
+    leaf = x.clone().requires_grad_()
+    rx, rv = (plain_rope(t.clone(), rotary.table, p, rotary.interleaved) for t in (x, v))
+    want = plain_rope(rx.cos() * rv, rotary.table, p, rotary.interleaved, True)
+    with fwAD.dual_level():
+        y = rotary(fwAD.make_dual(leaf, v), p)
+        grad, = torch.autograd.grad(-y.cos().sum(), leaf)
+        torch.testing.assert_close(fwAD.unpack_dual(grad).tangent, want)
+    # the gradient of a tangent, in x: <u, cos(R x) * R v> gives R^T (-sin(R x) * R v * u)
+    u = torch.randn((3, 2, 24))
+    with fwAD.dual_level():
+        t = fwAD.unpack_dual(rotary(fwAD.make_dual(leaf, v), p).sin()).tangent
+        grad, = torch.autograd.grad((t * u).sum(), leaf)
+    torch.testing.assert_close(grad, plain_rope(-rx.sin() * rv * u, rotary.table, p, rotary.interleaved, True))
+    # ... and in the tangent itself
+    w = v.clone().requires_grad_()
+    with fwAD.dual_level():
+        t = fwAD.unpack_dual(rotary(fwAD.make_dual(x, w), p)).tangent
+        grad, = torch.autograd.grad((t * u).sum(), w)
+    assert torch.equal(grad, plain_rope(u, rotary.table, p, rotary.interleaved, True))
+
+
+def test_a_trace_holds_the_rotation(rotary):
+    """torch.jit.trace records the operation, not the allocation of its output alone."""
+    p = torch.tensor([3, 0, 19], dtype=torch.int32)
+    with warnings.catch_warnings():
+        warnings.simplefilter("ignore")  # (the check of the heads' width is a Python branch)
+        traced = torch.jit.trace(lambda t: rotary(t, p), (torch.randn((3, 2, 24)),))
+    x = torch.randn((3, 2, 24))
+    assert torch.equal(traced(x), rotary(x, p))

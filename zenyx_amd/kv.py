@@ -930,7 +930,8 @@ def rope(x: torch.Tensor, table: torch.Tensor, positions: torch.Tensor, interlea
     or (2 i, 2 i + 1) when ``interleaved``; later channels are copied.  ``transpose`` applies
     the transposed rotation, which takes a gradient back.  ``out`` may be ``x`` itself; no two of
     its rows may overlap.  A row at a position the table does not have is copied (``check``
-    synchronises and raises)."""
+    synchronises and raises).  autograd does not see this call, in either mode:
+    ``train.rotary.RotaryPositions`` is the differentiable form."""
     N.need_gpu()
     if x.dim() != 3 or x.dtype not in _DT:
         raise ValueError("x must be [n, n_heads, head_dim] in bf16, f16 or f32")

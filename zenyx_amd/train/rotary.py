@@ -8,6 +8,7 @@ from __future__ import annotations
 import math
 
 import torch
+import torch.autograd.forward_ad as fwAD
 
 from .. import kv
 from .._native import ensure_gpu
@@ -69,11 +70,13 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
 
 
 class _Rotate(torch.autograd.Function):
-    """A linear map: its gradient is the transposed one, which is differentiable in its turn."""
+    """A linear map: its gradient is the transposed one, its derivative along a tangent the map itself,
+    both differentiable in their turn."""
 
     @staticmethod
     def forward(ctx, x, table, positions, interleaved, transpose):
         ctx.save_for_backward(table, positions)
+        ctx.save_for_forward(table, positions)
         ctx.interleaved, ctx.transpose = interleaved, transpose
         return kv.rope(x, table, positions, interleaved=interleaved, transpose=transpose)
 
@@ -82,6 +85,11 @@ class _Rotate(torch.autograd.Function):
         table, positions = ctx.saved_tensors
         return (_Rotate.apply(_rows(grad), table, positions, ctx.interleaved, not ctx.transpose),
                 None, None, None, None)
+
+    @staticmethod
+    def jvp(ctx, tangent, *_):
+        table, positions = ctx.saved_tensors
+        return _Rotate.apply(_rows(tangent), table, positions, ctx.interleaved, ctx.transpose)
 
 
 class RotaryPositions:
@@ -104,10 +112,13 @@ class RotaryPositions:
 
     def __call__(self, x: torch.Tensor, positions: torch.Tensor) -> torch.Tensor:
         """``x [n, H, head_dim]`` (bf16, f16, f32) at ``positions`` (int32 ``[n]``); differentiable
-        in x (the gradient is rotated back)."""
+        in x, in reverse mode (the gradient is rotated back) and in forward mode.  ``kv.rope``
+        itself is not: autograd does not see it."""
         if x.shape[-1] != self.head_dim:
             raise ValueError(f"x must have heads of {self.head_dim}")
-        if torch.is_grad_enabled() and x.requires_grad:
+        # (an autograd function costs a call 5 us of the host's time: only where one is needed)
+        if torch.is_grad_enabled() and x.requires_grad or fwAD.unpack_dual(x).tangent is not None or \
+                torch.jit.is_tracing():
             return _Rotate.apply(x, self.table, positions, self.interleaved, False)
         return kv.rope(x, self.table, positions, interleaved=self.interleaved)
 
