@@ -759,3 +759,21 @@ def test_4_bit_attention_against_float64_end_to_end(dev):
     assert one.shape == (2, Hq, D) and torch.isfinite(one).all()
     with pytest.raises(ValueError):
         cache.append(x, [0], [10])
+
+
+def test_prefill_keeps_its_weights_unless_told(dev):
+    """The default, and what QuantizedRingAttention's precisions become: "f16" and "exact" the weights to
+    2^-17, "bf16" those of one rounding."""
+    H, Hq, D, n = 2, 8, 128, 90
+    cache = PagedFP4KVCache(1, H, D, 20)
+    cache.append(torch.randn((1, n, 2, H, D), device=dev).to(torch.bfloat16), [0], [n], check=True)
+    q = torch.randn((n, Hq, D), device=dev).mul(3).to(torch.bfloat16)
+    pool, bt, lens = cache.pool[0], cache._tables([0]), cache._lengths([0])
+    args = (q, i32([0, n], dev), i32([0], dev), pool, bt, lens)
+    exact, one = (kv.paged_attention4_prefill(*args, max_q_per_seq=n, precision=p) for p in ("exact", "bf16"))
+    assert not torch.equal(exact, one)
+    check_attention(exact, q, pool.cpu().numpy(), bt.cpu().numpy(), [n], D ** -0.5, 2.0 ** -16, [n], [0], True)
+    assert torch.equal(kv.paged_attention4_prefill(*args, max_q_per_seq=n), exact)
+    for precision, want in (("f16", exact), ("exact", exact), ("bf16", one)):
+        assert torch.equal(QuantizedRingAttention(cache, precision=precision)(q, 0, [0], [n]), want), precision
+    assert torch.equal(QuantizedRingAttention(cache)(q, 0, [0], [n]), exact)

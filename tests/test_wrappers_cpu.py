@@ -8,6 +8,7 @@ import torch.autograd.forward_ad as fwAD
 
 from zenyx_amd import _native as N
 from zenyx_amd import kv
+from zenyx_amd.train.fp8_kv_quantization import PagedFP4KVCache, QuantizedRingAttention
 from zenyx_amd.train.rotary import RotaryPositions
 
 
@@ -163,3 +164,32 @@ def test_a_trace_holds_the_rotation(rotary):
         traced = torch.jit.trace(lambda t: rotary(t, p), (torch.randn((3, 2, 24)),))
     x = torch.randn((3, 2, 24))
     assert torch.equal(traced(x), rotary(x, p))
+
+
+# ------------------------------------------------------------------ precision over 4-bit pages
+
+@pytest.mark.parametrize("asked, given", [(None, "exact"), ("f16", "exact"), ("exact", "exact"), ("bf16", "bf16")])
+def test_attention_over_4_bit_pages_keeps_the_bits_asked_for(monkeypatch, asked, given):
+    """The 4-bit kernels have no fp16 weights: who asks for them (the default) gets more bits, not fewer."""
+    seen = []
+
+    def prefill(q, *args, precision="nothing passed", **kw):
+        seen.append(precision)
+        return q
+    monkeypatch.setattr(kv, "paged_attention4_prefill", prefill)
+    cache = PagedFP4KVCache(1, 2, 64, 4, device=torch.device("cpu"))
+    cache.lengths, cache.pages = {0: 5}, {0: [1]}
+    att = QuantizedRingAttention(cache, **({} if asked is None else {"precision": asked}), check=False)
+    att(torch.zeros((5, 4, 64), dtype=torch.bfloat16), 0, [0], [5])
+    assert seen == [given]
+
+
+def test_4_bit_prefill_does_not_drop_bits_by_itself(lib, monkeypatch):
+    """Weights rounded to bf16 are the caller's choice."""
+    monkeypatch.setattr(kv, "_index", lambda t, name: -1)
+    q, cu, lens = aligned(1, 4, 64, dtype=torch.bfloat16), aligned(2, dtype=torch.int32), aligned(1, dtype=torch.int32)
+    bt, pool = aligned(1, 2, dtype=torch.int32), aligned(3, 2, 2, 1, 544)
+    for kw, flag in (({}, N.ZX_PREFILL_EXACT_P), ({"precision": "exact"}, N.ZX_PREFILL_EXACT_P), ({"precision": "bf16"}, 0)):
+        kv.paged_attention4_prefill(q, cu, lens, pool, bt, lens, max_q_per_seq=1, **kw)
+        name, args = lib.calls[-1]
+        assert name == "zx_paged_attention4_prefill" and args[17] == flag

@@ -1173,20 +1173,26 @@ def paged_attention4_decode(q: torch.Tensor, pool_layer: torch.Tensor, block_tab
     return out
 
 
-PRECISIONS4 = ("bf16", "exact")
+# How 4-bit prefill carries the softmax weights (error bound beside one bf16 ulp of the value):
+#   "exact" (default) bf16 hi + lo, 2^-17 of a weight: 2^-15 max|V|;
+#   "bf16"  rounded once to bf16, the row sums with them: 2^-7 max|V|.  2 x 2,048 rows on 4k and 14k
+#           positions, 32/8 heads, D = 128: 735 us against 960, D = 64 460 / 610; few rows 30 / 32;
+#           the same as "exact" for D = 256 and for sequences of 16 columns (row x head) at most.
+# There is no fp16 form as over 8-bit pages: a block's power may be beyond fp16's.
+PRECISIONS4 = ("exact", "bf16")
 
 
 def paged_attention4_prefill(q: torch.Tensor, cu_q: torch.Tensor, q_pos0: torch.Tensor, pool_layer: torch.Tensor,
                              block_tables: torch.Tensor, kv_len: torch.Tensor, causal: bool = True,
                              sm_scale: float | None = None, max_q_per_seq: int | None = None,
-                             precision: str = "bf16", out: torch.Tensor | None = None, check: bool = False,
+                             precision: str = "exact", out: torch.Tensor | None = None, check: bool = False,
                              err: torch.Tensor | None = None) -> torch.Tensor:
     """Blocks of queries over 4-bit pages: ``q [n_q, Hq, D]`` bf16 rows of all sequences
     (``cu_q`` int32 ``[B + 1]`` offsets, ``q_pos0`` int32 ``[B]`` position of each sequence's
     first row) attend to keys ``[0, kv_len[b])``, when ``causal`` those up to their own
-    position.  ``precision``: the softmax weights rounded once to bf16 (error within one ulp +
-    2^-7 max|V|), or ``"exact"``, carried to 2^-17 (one ulp + 2^-15 max|V|).  ``max_q_per_seq``
-    bounds every sequence's rows (read back from ``cu_q`` without it, which waits for the
+    position.  ``precision``: the softmax weights carried to 2^-17 (``"exact"``: error within one
+    ulp + 2^-15 max|V|), or rounded once to bf16 (``"bf16"``, faster: one ulp + 2^-7 max|V|); see
+    PRECISIONS4.  ``max_q_per_seq`` bounds every sequence's rows (read back from ``cu_q`` without it, which waits for the
     device); rows beyond it, and rows in no sequence, are left as they are in ``out``.
     ``err`` (device int32 ``[1]``) collects the kernels' error bits; ``check`` reads them and
     raises."""

@@ -367,7 +367,7 @@ class PagedFP4KVCache(PagedFP8KVCache):
     def _attend(self, q, layer: int, tables, cu, q_pos0, lens, att, max_q: int) -> torch.Tensor:
         return kv.paged_attention4_prefill(q, cu, q_pos0, self.pool[layer], tables, lens, causal=att.causal,
                                            sm_scale=att.sm_scale, max_q_per_seq=max_q, check=att.check,
-                                           precision="exact" if att.precision == "exact" else "bf16")
+                                           precision="bf16" if att.precision == "bf16" else "exact")
 
     def _attend_step(self, q, layer: int, tables, lens, att) -> torch.Tensor:
         return kv.paged_attention4_decode(q, self.pool[layer], tables, lens, sm_scale=att.sm_scale, check=att.check)
@@ -387,8 +387,8 @@ class QuantizedRingAttention:
     in sequence.  ``decode`` is the one-token case (split-K decode kernel).
 
     With a ``PagedFP4KVCache`` one launch takes all keys, whatever ``ring_degree`` (the union
-    of a ring's shards), and ``precision`` is "exact" or, for the others, weights rounded once
-    to bf16.  A cache with ``rope`` has rotated its keys: the queries are rotated here, by the
+    of a ring's shards), and ``precision`` "f16" is given as "exact": the 4-bit kernels have no
+    fp16 weights, and "bf16" has fewer bits.  A cache with ``rope`` has rotated its keys: the queries are rotated here, by the
     positions of the tokens they stand for."""
 
     def __init__(self, cache: PagedFP8KVCache, ring_degree: int = 8, causal: bool = True,
