@@ -777,3 +777,32 @@ def test_prefill_keeps_its_weights_unless_told(dev):
     for precision, want in (("f16", exact), ("exact", exact), ("bf16", one)):
         assert torch.equal(QuantizedRingAttention(cache, precision=precision)(q, 0, [0], [n]), want), precision
     assert torch.equal(QuantizedRingAttention(cache)(q, 0, [0], [n]), exact)
+
+
+@pytest.mark.parametrize("other", [40, 1000])  # the other sequence's keys: sequences are taken whole, or in runs
+@pytest.mark.parametrize("n_seqs", [2, 70])
+@pytest.mark.parametrize("claim", [2, 3, 9])
+def test_flags_of_sequences_without_keys(dev, other, n_seqs, claim):
+    """A few rows per sequence, dealt in runs: a sequence without keys that claims rows beyond
+    max_q_per_seq (2), or rows that q does not have, is flagged as any other, and its two rows are zeros."""
+    H, Hq, D, P = 2, 4, 64, 16
+    bt, n_pages = tables([1024] * 2 + [16] * (n_seqs - 2), P, 0, 1)
+    bt[1, other // P + 1:] = -1
+    pool = torch.from_numpy(random_pool(n_pages, H, P, D, 1)).to(dev)
+    for empty, length in ((0, 0), (1, -3), (n_seqs - 1, 0)):
+        lens = [other] + [16] * (n_seqs - 1)
+        lens[empty] = length
+        rows = [2] * n_seqs
+        rows[empty] = claim
+        cu = np.concatenate([[0], np.cumsum(rows)])
+        n_q = int(cu[-1])
+        missing = claim == 9 and empty == n_seqs - 1  # rows that q does not have
+        q = torch.randn((n_q - 7 if missing else n_q, Hq, D), device=dev).to(torch.bfloat16)
+        out = torch.full_like(q, 5.0)
+        err = torch.zeros(1, dtype=torch.int32, device=dev)
+        kv.paged_attention4_prefill(q, i32(cu, dev), i32([2000] * n_seqs, dev), pool, i32(bt, dev), i32(lens, dev),
+                                    max_q_per_seq=2, out=out, err=err)
+        assert err.item() == (N.ZX_KERR_POS_RANGE if claim > 2 else 0), (empty, length)
+        at = int(cu[empty])
+        assert not out[at:at + 2].any() and torch.all(out[at + 2:int(cu[empty + 1])] == 5)
+        assert torch.isfinite(out).all() and not (out[:2] == 5).any()

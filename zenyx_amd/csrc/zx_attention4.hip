@@ -636,7 +636,7 @@ paged_decode4_kernel(const uint16_t *__restrict__ q, AttnGeom g, A4Rows qr, cons
 template <int D>
 __global__ void __launch_bounds__(1024)
 decode4_rows_combine_kernel(const float *__restrict__ part, AttnGeom g, A4Rows qr, const int32_t *__restrict__ seq_lens,
-                            uint16_t *__restrict__ out, void *table) {
+                            uint16_t *__restrict__ out, int32_t *err, void *table) {
   const int b = (int)(blockIdx.x / (uint32_t)g.n_q_heads);
   const int hq = (int)(blockIdx.x - (uint32_t)b * (uint32_t)g.n_q_heads);
   int32_t x0, n_live, e = 0;
@@ -644,6 +644,8 @@ decode4_rows_combine_kernel(const float *__restrict__ part, AttnGeom g, A4Rows q
   if (n_live == 1) return;
   const int64_t lo = qr.cu_q[b];
   const int32_t rows = a4_rows(lo, qr.cu_q[b + 1], qr.n_q, qr.most, e);
+  // (a sequence without keys is met here alone)
+  if (e && err && n_live == 0 && hq == 0 && threadIdx.x == 0) atomicOr(err, e);
   const int d = threadIdx.x % D;
   for (int r = threadIdx.x / D; r < rows; r += blockDim.x / D) {
     const float *pp = part + (((int64_t)r * g.n_q_heads + hq) * ((int64_t)g.n_run + g.n_seqs) + x0 + b) * (2 + D);
@@ -921,7 +923,7 @@ static int a4_launch_runs(const AttnRuns &p, const AttnGeom &g, const A4Rows &qr
   if (!ROWS) return att_combine(part, g, nullptr, lens, out, table, st);
   if (g.whole) return ZX_OK;
   decode4_rows_combine_kernel<D><<<(unsigned)(g.n_seqs * g.n_q_heads), D * std::min(1024 / D, qr.most), 0, st>>>(
-      part, g, qr, lens, out, table);
+      part, g, qr, lens, out, err, table);
   return check_launch("decode4_rows_combine");
 }
 
