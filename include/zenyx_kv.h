@@ -525,7 +525,8 @@ int zx_kv4_gather_dequant(const uint8_t *pool, int64_t n_pages, int32_t n_heads,
                           const int32_t *block_tables, int32_t max_blocks, const int32_t *seq_lens, int32_t n_seqs,
                           int32_t out_len, uint16_t *k_out, uint16_t *v_out, int32_t *err, zx_stream_t stream);
 /* Decode attention from 4-bit pages: as zx_paged_attention_decode (softmax weights carried to
- * 2^-17, sums in fp32, rounded once to bf16), any n_q_heads / n_kv_heads. */
+ * 2^-17, sums in fp32, rounded once to bf16), any n_q_heads / n_kv_heads.  workspace:
+ * zx_paged_attention4_decode_workspace_bytes() device bytes, 16-byte aligned. */
 size_t zx_paged_attention4_decode_workspace_bytes(int32_t n_seqs, int32_t n_q_heads, int32_t n_kv_heads,
                                                   int32_t head_dim, int32_t max_blocks, int32_t page_size);
 int zx_paged_attention4_decode(const uint16_t *q, int32_t n_q_heads, const uint8_t *pool, int64_t n_pages,

@@ -197,3 +197,11 @@ def test_rope_refuses_an_out_whose_rows_overlap(lib, n, H, D, row, head):
     assert lib.zx_rope(*rope_args(n=n, H=H, D=D, xr=H * D, xh=D, outr=row, outh=head)) == N.ZX_ERR_INVALID
     assert b"overlap" in lib.zx_last_error()
     assert lib.zx_rope(*rope_args(n=n, H=H, D=D, xr=row, xh=head, outr=row, outh=head, out=P)) == N.ZX_ERR_INVALID
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_decode_refuses_a_workspace_off_16_bytes(lib, D):
+    """Its parts and tables are read by 8 bytes, as prefill's, which refuses it too."""
+    for off in (4, 8):
+        assert lib.zx_paged_attention4_decode(*decode_args(ws=P + off, D=D)) == N.ZX_ERR_INVALID
+        assert b"workspace" in lib.zx_last_error()

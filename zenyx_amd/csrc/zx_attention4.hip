@@ -941,6 +941,7 @@ extern "C" int zx_paged_attention4_decode(const uint16_t *q, int32_t n_q_heads, 
   ZX_REQUIRE(n_q_heads > 0 && max_blocks > 0 && n_seqs > 0, "paged_attention4_decode: sizes must be positive");
   ZX_REQUIRE(n_q_heads % n_kv_heads == 0, "paged_attention4_decode: n_q_heads must be a multiple of n_kv_heads");
   if (n_seqs > 65535) return fail(ZX_ERR_UNSUPPORTED, "paged_attention4_decode: more than 65535 sequences");
+  ZX_REQUIRE(!workspace || aligned16(workspace), "paged_attention4_decode: workspace must be 16-byte aligned");
   const size_t need =
       zx_paged_attention4_decode_workspace_bytes(n_seqs, n_q_heads, n_kv_heads, head_dim, max_blocks, page_size);
   if (!workspace || workspace_bytes < need)
