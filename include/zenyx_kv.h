@@ -487,8 +487,8 @@ int zx_rope(const void *x, int dtype, int64_t n_rows, int32_t n_heads, int32_t h
  * zx_rope rounds them, then quantised): the codes and scales of zx_rope followed by
  * zx_kv_quant_append, without the rotated copy.  flags: zx_kv_quant_append's and
  * ZX_ROPE_INTERLEAVED (the single pass only where a CU's share of a slab fits its registers).
- * A token at or beyond n_pos is not stored and sets ZX_KERR_POS_RANGE; dynamic scales are taken over the tokens that have a position (rows
- * outside [cu_seqlens[0], cu_seqlens[n_seqs]) have none).  workspace:
+ * A token at or beyond n_pos is not stored and sets ZX_KERR_POS_RANGE; dynamic scales are taken
+ * over the tokens that have a position (rows outside [cu_seqlens[0], cu_seqlens[n_seqs]) have none).  workspace:
  * zx_kv_rope_append_workspace_bytes() device bytes (0 for a small call with static scales),
  * 16-byte aligned. */
 size_t zx_kv_rope_append_workspace_bytes(int32_t n_layers, int64_t n_tok, int32_t n_heads, int32_t head_dim,
@@ -539,12 +539,15 @@ int zx_paged_attention4_decode(const uint16_t *q, int32_t n_q_heads, const uint8
  * [head_dim], row i of sequence b at position q_pos0[b] + i, attend to keys [0, kv_len[b]), when
  * `causal` those up to their own position.  A row without a key gives zeros; rows beyond
  * max_q_per_seq (host) or in no sequence are left unwritten, rows that cu_q claims beyond n_q do
- * not exist (either sets ZX_KERR_POS_RANGE); a NaN value reaches the rows that see it; kv_len beyond max_blocks * page_size is clipped and sets it too; keys on
- * a page outside [0, n_pages) are left out and set ZX_KERR_PAGE_RANGE.  Softmax weights are
- * rounded once to bf16 (the row sums use the same): |error| <= one bf16 ulp + 2^-7 max|V|; with
+ * not exist (either sets ZX_KERR_POS_RANGE); a NaN value reaches the rows that see it; kv_len
+ * beyond max_blocks * page_size is clipped and sets ZX_KERR_POS_RANGE too; keys on a page outside
+ * [0, n_pages) are left out and set ZX_KERR_PAGE_RANGE.  Softmax weights are rounded once to bf16 (the row sums use the same): |error| <= one bf16 ulp + 2^-7 max|V|; with
  * ZX_PREFILL_EXACT_P they are carried as bf16 hi + lo: one ulp + 2^-15 max|V|.  workspace:
- * zx_paged_attention4_prefill_workspace_bytes() device bytes let several blocks share a row's
- * keys where the rows do not fill the chip; a smaller or NULL one runs the call uncut. */
+ * zx_paged_attention4_prefill_workspace_bytes() device bytes, 16-byte aligned, let several blocks
+ * share a row's keys where the rows do not fill the chip; a smaller or NULL one runs the call
+ * uncut.  The call plans for min(max_q_per_seq, n_q) rows per sequence: that is what the query is
+ * to be asked for (a loose bound's answer may be less).  A call with n_q or max_q_per_seq 0 does
+ * nothing and flags nothing. */
 size_t zx_paged_attention4_prefill_workspace_bytes(int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim,
                                                    int32_t page_size, int32_t max_blocks, int32_t n_seqs,
                                                    int32_t max_q_per_seq);
