@@ -806,3 +806,20 @@ def test_flags_of_sequences_without_keys(dev, other, n_seqs, claim):
         at = int(cu[empty])
         assert not out[at:at + 2].any() and torch.all(out[at + 2:int(cu[empty + 1])] == 5)
         assert torch.isfinite(out).all() and not (out[:2] == 5).any()
+
+
+@pytest.mark.parametrize("sm", [-0.3, 0.0, 0.7, -1e-6])
+@pytest.mark.parametrize("case", range(len(DECODE)))
+def test_decode_scales_into_the_callers_buffer(dev, case, sm):
+    """Every shape's values under scales of either sign and zero (then each sequence's mean), in a buffer
+    that held something else."""
+    lens, Hq, H, D, P, spare = DECODE[case]
+    bt, n_pages = tables(lens, P, 2, case)
+    bt = np.concatenate([bt, np.full((len(lens), spare), -1, np.int32)], 1)
+    pool = random_pool(n_pages, H, P, D, case + 100)
+    q = torch.randn((len(lens), Hq, D), device=dev).mul(1.5).to(torch.bfloat16)
+    out = torch.full_like(q, 3.0)
+    got = kv.paged_attention4_decode(q, torch.from_numpy(pool).to(dev), i32(bt, dev), i32(lens, dev), sm_scale=sm,
+                                     out=out, check=True)
+    assert got is out
+    check_attention(out, q, pool, bt, lens, sm, 2.0 ** -16)
