@@ -170,6 +170,14 @@ struct A4Pages {
   }
 };
 
+// Tokens below `end` of the tile at t: 0 to 16.  Without a difference that wraps where it is not
+// chosen: of `t < end ? min(16, end - t) : 0` the compiler's constraint elimination takes the
+// difference for one that never does, concludes that t never reaches end, and may drop a loop's
+// exit and everything behind it (it did where prefill's loop saw two strides).
+__device__ __forceinline__ uint32_t a4_tile_live(uint32_t end, uint32_t t) {
+  return min((uint32_t)K4_TOK, end - min(t, end));
+}
+
 // The attention of one wave: CT tiles of 16 columns (a column is a query row and head), its
 // steps of 32 keys, their softmax and accumulators.  Everything lives in registers; vt is the
 // wave's LDS.  EXACT: weights as bf16 hi + lo (2^-17), otherwise rounded once to bf16.
@@ -219,7 +227,7 @@ template <int D, int CT, bool EXACT> struct A4Wave {
     constexpr int GROUPS = D == 64 ? 2 : 4;
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
-      const uint32_t seen = (1u << (lim[ct] > t ? min(lim[ct] - t, (uint32_t)K4_TOK) : 0u)) - 1u;
+      const uint32_t seen = (1u << a4_tile_live(lim[ct], t)) - 1u;
 #pragma unroll
       for (int j = 0; j < GROUPS; ++j) {
         const uint32_t tokens = (uint32_t)(bad >> (D == 64 ? 32 * j : 16 * j)) & 0xFFFFu;
@@ -365,7 +373,8 @@ template <int D, int CT, bool EXACT> struct A4Wave {
       page[1] = pg.bt[pg.page_of(min(ts + K4_TOK, t_last))];
     };
     auto load_tile = [&](uint32_t tp, int32_t id, A4Tile<D> &k, A4Tile<D> &v, int &r) {
-      const int live = tp < t_end ? (int)min((uint32_t)K4_TOK, t_end - tp) : 0;
+      // (readfirstlane: uniform, but taken for a vector operand, and the loads then for a loop over lanes)
+      const int live = __builtin_amdgcn_readfirstlane((int)a4_tile_live(t_end, tp));
       const uint32_t tc = min(tp, t_last);
       const uint32_t in_page = tc - pg.page_of(tc) * pg.page_size;
       const bool ok = id >= 0 && id < pg.n_pages;
@@ -812,10 +821,7 @@ __global__ void __launch_bounds__(ATT_THREADS, a4_per_cu(D, CT)) paged_prefill4_
   w.lim_all = a.causal ? (uint32_t)max((int64_t)0, min((int64_t)end, pos0 + row0 + 1)) : end;
   w.clear();
   const uint32_t t0 = t_begin + (alone ? 0u : (uint32_t)wave * A4_STEP);
-  // (readfirstlane: one loop for both strides.  Where it sees two, the compiler loses the products
-  // with V and everything after them)
-  const int stride = __builtin_amdgcn_readfirstlane(alone ? A4_STEP : ATT_WAVES * A4_STEP);
-  if (t0 < t_end) w.run(pg, t0, t_end, (uint32_t)stride);
+  if (t0 < t_end) w.run(pg, t0, t_end, alone ? A4_STEP : ATT_WAVES * A4_STEP);
   if (alone) {
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
