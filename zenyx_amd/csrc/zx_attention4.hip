@@ -355,11 +355,13 @@ template <int D, int CT, bool EXACT> struct A4Wave {
     }
   }
 
-  // Keys [t0, t_end) in steps of 32, `stride` apart, t0 < t_end.  Branch-free: a page id is read for a position clamped into the range, a tile past
-  // the end or on a bad page loads through an empty resource.  Page ids are read a step before
-  // the loads that they are for.  With one tile of columns the loads go out a step ahead, into a
-  // second set of registers (16 x 1k-8k positions 26.7 -> 24.9 us, 128 x 100-600 17.5 -> 15.8);
-  // with more, where the set would cost a wave per SIMD, once the step's codes are converted.
+  // Keys [t0, t_end) in steps of 32, `stride` apart, t0 < t_end.  Branch-free: a page id is read
+  // for a position clamped into the range, a tile past the end or on a bad page loads through an
+  // empty resource.  Page ids are read a step before the loads that they are for.  At D = 64 with
+  // one tile of columns the loads go out a step ahead, into a second set of registers (in a graph,
+  // 128 x 100-600, 12 heads 16.8 -> 16.5 us, 16 x 1k-8k, 32/8 heads 20.0 -> 19.5, 64 x 8,000 67.2
+  // -> 65.8); with more columns or channels, where the set would cost a wave per SIMD, once the
+  // step's codes are converted.
   __device__ __forceinline__ void run(const A4Pages &pg, uint32_t t0, uint32_t t_end, uint32_t stride) {
     constexpr bool AHEAD = D * CT <= 64;
     const uint32_t t_last = t_end - 1;
@@ -668,8 +670,9 @@ decode4_rows_combine_kernel(const float *__restrict__ part, AttnGeom g, A4Rows q
 // to the operand without LDS, every conversion serves CT products, and a K/V byte read serves
 // 16 CT columns: what a block reads is small, the pages have 4 bits.  Bound by the issue of the
 // matrix products, the conversions and the exponentials together: 2 x 2,048 rows on 4k and 14k
-// positions, 32/8 heads, D = 128, 724 us or 925 TFLOP/s, matrix cores busy 41% and vector units
-// 52% of the time; a library product of 8,192^3 reaches 1,109.
+// positions, 32/8 heads, D = 128, weights rounded to bf16, 724 us or 925 TFLOP/s, matrix cores busy
+// 41% and vector units 52% of the time; with a second product for the weights' low halves 930 us.
+// A library product of 8,192^3 reaches 1,109.
 // With few tiles a tile's keys are shared by up to n_split blocks, whose parts
 // prefill4_combine_kernel merges.
 struct Prefill4Args {
@@ -712,9 +715,10 @@ __device__ __forceinline__ int p4_parts(const Prefill4Args &a, uint32_t keys) {
 // by itself.  A tile that four waves share costs about 6 us of a block's time besides its steps
 // (four starts, the merge), one of a wave's own 4 us of a wave's, but the launch then ends with
 // whole tiles: a step is 1.8 us of a wave's time.  So by themselves if the tiles are many for
-// their length: 7 times the tiles per block slot exceed the longest one's steps.  4 x 2,048 new
-// rows, 32/8 heads, D = 128, shared 218 us, alone 193; 9 x 227-455 rows, 32/8 heads, D = 64 40 / 28;
-// 8 x 768 rows on 1,024 keys 160 / 129.  2 x 2,048 rows on 4k and 14k stay shared.
+// their length: 7 times the tiles per block slot exceed the longest one's steps.  Weights of one
+// rounding / carried to 2^-17: 4 x 2,048 new rows, 32/8 heads, D = 128, shared 231 / 264 us, alone
+// 206 / 243; 9 x 227-455 rows, 32/8 heads, D = 64 35 / 39 and 24 / 28; 8 x 768 rows on 1,024 keys 139
+// / 155 and 117 / 142; the other way 2 x 2,048 rows on 4k and 14k 719 / 922 and 773 / 989.
 struct P4Order {
   int32_t lo, hi, len, pos0;
   int before;  // sequences before this lane's
@@ -872,8 +876,8 @@ __global__ void __launch_bounds__(D) prefill4_combine_kernel(Prefill4Args a, int
 }
 
 // Tiles of 16 columns that a block can hold: what leaves two waves per SIMD.  (With two at most, D
-// = 128: 2 x 2,048 rows on 8,000 positions 806 us against 703, 8,192 rows from nothing 735 / 601;
-// D = 64, 2 x 2,048 rows on 4k and 14k 472 / 439.)
+// = 128, weights rounded to bf16: 2 x 2,048 rows on 8,000 positions 806 us against 703, 8,192 rows
+// from nothing 735 / 601; D = 64, 2 x 2,048 rows on 4k and 14k 472 / 439.)
 constexpr int a4_most_tiles(int D) { return D == 64 ? 4 : D == 128 ? 3 : 1; }
 
 }  // namespace zx
@@ -1013,7 +1017,9 @@ extern "C" size_t zx_paged_attention4_prefill_workspace_bytes(int32_t n_q_heads,
 template <int D, int CT>
 static int p4_launch(const Prefill4Args &a, bool exact, unsigned rows, hipStream_t st) {
   const unsigned grid = a.n_items * (unsigned)a.n_split;
-  if (CT == 1 || exact)  // (one tile of columns: bound by the reads, the second product is free)
+  // (one tile of columns: at D = 64 and 128 a sequence of at most 16, bound by the reads, where the
+  // second product is free; at D = 256 every call: it has no form with one)
+  if (CT == 1 || exact)
     paged_prefill4_kernel<D, CT, true><<<grid, ATT_THREADS, 0, st>>>(a);
   else if constexpr (CT > 1)
     paged_prefill4_kernel<D, CT, false><<<grid, ATT_THREADS, 0, st>>>(a);
