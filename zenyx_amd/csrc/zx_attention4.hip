@@ -671,8 +671,8 @@ decode4_rows_combine_kernel(const float *__restrict__ part, AttnGeom g, A4Rows q
 // 16 CT columns: what a block reads is small, the pages have 4 bits.  Bound by the issue of the
 // matrix products, the conversions and the exponentials together: 2 x 2,048 rows on 4k and 14k
 // positions, 32/8 heads, D = 128, weights rounded to bf16, 724 us or 925 TFLOP/s, matrix cores busy
-// 41% and vector units 52% of the time; with a second product for the weights' low halves 930 us.
-// A library product of 8,192^3 reaches 1,109.
+// 41% and vector units 52% of the time; with a second product for the weights' low halves 924 us,
+// 46% and 60%.  A library product of 8,192^3 reaches 1,109.
 // With few tiles a tile's keys are shared by up to n_split blocks, whose parts
 // prefill4_combine_kernel merges.
 struct Prefill4Args {

@@ -1176,7 +1176,7 @@ def paged_attention4_decode(q: torch.Tensor, pool_layer: torch.Tensor, block_tab
 # How 4-bit prefill carries the softmax weights (error bound beside one bf16 ulp of the value):
 #   "exact" (default) bf16 hi + lo, 2^-17 of a weight: 2^-15 max|V|;
 #   "bf16"  rounded once to bf16, the row sums with them: 2^-7 max|V|.  2 x 2,048 rows on 4k and 14k
-#           positions, 32/8 heads, D = 128: 735 us against 960, D = 64 460 / 610; few rows 30 / 32;
+#           positions, 32/8 heads, D = 128: 720 us against 924, D = 64 462 / 615; few rows 28 / 30;
 #           the same as "exact" for D = 256 and for sequences of 16 columns (row x head) at most.
 # There is no fp16 form as over 8-bit pages: a block's power may be beyond fp16's.
 PRECISIONS4 = ("exact", "bf16")
