@@ -823,3 +823,63 @@ def test_decode_scales_into_the_callers_buffer(dev, case, sm):
                                      out=out, check=True)
     assert got is out
     check_attention(out, q, pool, bt, lens, sm, 2.0 ** -16)
+
+
+@pytest.mark.parametrize("n_seqs", [255, 256, 257, 258, 700])
+@pytest.mark.parametrize("longest", [1, 40])
+def test_append_of_many_sequences(dev, n_seqs, longest):
+    """Either side of the 256 sequences whose table fits the kernels' LDS, few tokens (found in the append
+    itself) and more (found by a launch before it), empty sequences among them, rotating."""
+    L, H, D, P, rot = 2, 2, 64, 16, 32
+    rng = np.random.default_rng(n_seqs + longest)
+    lens = rng.integers(0, longest + 1, n_seqs)
+    lens[[0, -1]] = 0, longest
+    old = rng.integers(0, 30, n_seqs)
+    T = int(lens.sum())
+    bt, n_pages = tables(lens + old, P, 2, 1)
+    x = torch.randn((L, T + 1, 2, H, D), device=dev).to(torch.bfloat16)
+    table = kv.rope_table(rotary_frequencies(rot)[0].to(dev), int((lens + old).max()) + 1)
+    pos = i32(np.concatenate([np.arange(a, a + n) for a, n in zip(old, lens)]), dev)
+    turned = x.clone()
+    for layer in range(L):
+        turned[layer, :T, 0] = kv.rope(x[layer, :T, 0].contiguous(), table, pos)
+    cu, start = i32(np.concatenate([[0], np.cumsum(lens)]), dev), i32(old, dev)
+    pool = torch.randint(0, 256, tuple(kv.kv4_pool(L, n_pages, H, P, D).shape), device=dev, dtype=torch.uint8)
+    want = pool.cpu().numpy()
+    oracle_append(turned, bt, lens, old, want)
+    kv.kv4_append(x, cu, i32(bt, dev), pool, start_pos=start, table=table, check=True)
+    assert np.array_equal(pool.cpu().numpy(), want)
+    # the FP8 append that rotates, against the one that takes rotated keys
+    a, b = (torch.zeros((L, n_pages, 2, H, P, D), dtype=torch.uint8, device=dev) for _ in range(2))
+    got = kv.kv_rope_append(x, table, cu, i32(bt, dev), a, start_pos=start, check=True)
+    assert torch.equal(got, kv.kv_quant_append(turned[:, :T].contiguous(), cu, i32(bt, dev), b, start_pos=start, check=True))
+    assert torch.equal(a, b)
+
+
+def test_append_and_gather_in_a_graph(dev):
+    """Captured appends and gathers, small and large ones (with a workspace each), replay to the eager bits."""
+    H, D, P = 2, 128, 16
+    for lens, old in (([3, 1], [5, 40]), ([6000, 11000], [0, 9])):
+        total = [a + b for a, b in zip(lens, old)]
+        bt, n_pages = tables(total, P, 0, 2)
+        btd, cu, start, ld = i32(bt, dev), i32([0, lens[0], sum(lens)], dev), i32(old, dev), i32(total, dev)
+        table = kv.rope_table(rotary_frequencies(D)[0].to(dev), max(total))
+        x = torch.randn((1, sum(lens), 2, H, D), device=dev).to(torch.bfloat16)
+        graphs, outs = [], []
+        kv.kv4_append(x, cu, btd, kv.kv4_pool(1, n_pages, H, P, D), start_pos=start, table=table)
+        for _ in range(2):
+            pool, g = kv.kv4_pool(1, n_pages, H, P, D), torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g):
+                kv.kv4_append(x, cu, btd, pool, start_pos=start, table=table)
+                outs.append((pool, *kv.kv4_gather_dequant(pool[0], btd, ld, max(total))))
+            graphs.append(g)
+        for _ in range(3):
+            x.copy_(torch.randn(x.shape, device=dev))
+            for g in graphs:
+                g.replay()
+            want = kv.kv4_pool(1, n_pages, H, P, D)
+            kv.kv4_append(x, cu, btd, want, start_pos=start, table=table)
+            k, v = kv.kv4_gather_dequant(want[0], btd, ld, max(total))
+            torch.cuda.synchronize()
+            for o in outs:
+                assert all(torch.equal(a, b) for a, b in zip(o, (want, k, v)))
