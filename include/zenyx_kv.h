@@ -558,6 +558,42 @@ int zx_paged_attention4_prefill(const uint16_t *q, int64_t n_q, const int32_t *c
                                 float sm_scale, int32_t flags, uint16_t *out, int32_t *err, void *workspace,
                                 size_t workspace_bytes, zx_stream_t stream);
 
+/* ---------------------------------------------------------------------------
+ * Attention for a batch whose sequences share pages (ABI version 10).  Sequences [cu_group[g],
+ * cu_group[g + 1]) (device int32 [n_groups + 1], ascending) have their first shared_lens[g] positions
+ * on the same pages: those of the group's first sequence's block table, which are read and
+ * multiplied once for all the group's rows.  Positions from shared_lens[g] (rounded down to a
+ * multiple of 16) on are read through each sequence's own table; a sequence in no group has
+ * only those.  Rows [cu_q[b], cu_q[b + 1]) of q [n_q][n_q_heads][head_dim] bf16 are sequence b's
+ * newest (cu_q NULL: a row each, n_q == n_seqs): row i of n is at position seq_lens[b] - n + i and
+ * sees, when `causal`, the keys up to it, otherwise all seq_lens[b].  out is that of attention over
+ * every sequence's own table, whatever the sequences of a group have in common beyond it.
+ * n_groups may be 0.  A row without a key gives zeros; rows beyond max_q_per_seq (host) or in no
+ * sequence are left unwritten, rows that cu_q claims beyond n_q do not exist (either sets
+ * ZX_KERR_POS_RANGE, as lengths beyond max_blocks * page_size, which are clipped, and groups that
+ * are out of order do); keys on a page outside [0, n_pages) are left out and set
+ * ZX_KERR_PAGE_RANGE.  head_dim 64, 128 or 256, page_size a multiple of 16; scores and sums in fp32.
+ * FP8: scales [2][n_kv_heads]; softmax weights rounded once to fp16 (times 2^7; the row sums use
+ * the same): |error| <= one bf16 ulp + 2^-10 max|V|.  4 bits: weights as bf16 hi + lo, one ulp +
+ * 2^-15 max|V|.  A NaN value reaches the rows that see it.  workspace: the query's device bytes,
+ * 16-byte aligned; it holds nothing between calls. */
+size_t zx_paged_attention_shared_workspace_bytes(int64_t n_q, int32_t n_seqs, int32_t n_groups, int32_t n_q_heads,
+                                                 int32_t n_kv_heads, int32_t head_dim, int32_t max_q_per_seq);
+int zx_paged_attention_shared(const uint16_t *q, int64_t n_q, const int32_t *cu_q, int32_t n_q_heads,
+                              const uint8_t *pool, int64_t n_pages, int32_t n_kv_heads, int32_t head_dim,
+                              int32_t page_size, const float *scales, const int32_t *block_tables, int32_t max_blocks,
+                              const int32_t *seq_lens, int32_t n_seqs, const int32_t *cu_group,
+                              const int32_t *shared_lens, int32_t n_groups, int32_t max_q_per_seq, int32_t causal,
+                              float sm_scale, uint16_t *out, int32_t *err, void *workspace, size_t workspace_bytes,
+                              zx_stream_t stream);
+int zx_paged_attention4_shared(const uint16_t *q, int64_t n_q, const int32_t *cu_q, int32_t n_q_heads,
+                               const uint8_t *pool, int64_t n_pages, int32_t n_kv_heads, int32_t head_dim,
+                               int32_t page_size, const int32_t *block_tables, int32_t max_blocks,
+                               const int32_t *seq_lens, int32_t n_seqs, const int32_t *cu_group,
+                               const int32_t *shared_lens, int32_t n_groups, int32_t max_q_per_seq, int32_t causal,
+                               float sm_scale, uint16_t *out, int32_t *err, void *workspace, size_t workspace_bytes,
+                               zx_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

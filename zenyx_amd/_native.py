@@ -34,7 +34,7 @@ ZX_HEADS_TWO_PASS = 1
 ZX_HEADS_SINGLE_PASS = 2
 ZX_NEVER = 0x7FFFFFFF
 ZX_ROPE_INTERLEAVED, ZX_ROPE_TRANSPOSE = 16, 32
-ABI_VERSION = 9
+ABI_VERSION = 10
 
 _P = ctypes.c_void_p
 _I64, _I32, _SZ, _INT = ctypes.c_int64, ctypes.c_int32, ctypes.c_size_t, ctypes.c_int
@@ -101,6 +101,11 @@ SIGNATURES = {
     "zx_paged_attention4_prefill_workspace_bytes": (_SZ, [_I32, _I32, _I32, _I32, _I32, _I32, _I32]),
     "zx_paged_attention4_prefill": (_INT, [_P, _I64, _P, _P, _I32, _P, _I64, _I32, _I32, _I32, _P, _I32, _P, _I32,
                                            _I32, _I32, ctypes.c_float, _I32, _P, _P, _P, _SZ, _P]),
+    "zx_paged_attention_shared_workspace_bytes": (_SZ, [_I64, _I32, _I32, _I32, _I32, _I32, _I32]),
+    "zx_paged_attention_shared": (_INT, [_P, _I64, _P, _I32, _P, _I64, _I32, _I32, _I32, _P, _P, _I32, _P, _I32, _P, _P,
+                                         _I32, _I32, _I32, ctypes.c_float, _P, _P, _P, _SZ, _P]),
+    "zx_paged_attention4_shared": (_INT, [_P, _I64, _P, _I32, _P, _I64, _I32, _I32, _I32, _P, _I32, _P, _I32, _P, _P,
+                                          _I32, _I32, _I32, ctypes.c_float, _P, _P, _P, _SZ, _P]),
 }
 
 _lib = None

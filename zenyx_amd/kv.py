@@ -46,7 +46,7 @@ def kernel_error_text(e: int) -> str:
         parts.append("block table entry outside [0, n_pages)")
     if e & N.ZX_KERR_POS_RANGE:
         parts.append("token position beyond max_blocks * page_size (attention: or a query row beyond "
-                     "max_q_per_seq)")
+                     "max_q_per_seq, or groups out of order)")
     if e & N.ZX_KERR_SPIN:
         parts.append("bounded wait ran out")
     if e & N.ZX_KERR_OVERFLOW:
@@ -1227,3 +1227,101 @@ def paged_attention4_prefill(q: torch.Tensor, cu_q: torch.Tensor, q_pos0: torch.
     if check:
         _raise_kernel_error(err, "paged_attention4_prefill")
     return out
+
+
+# ------------------------------------------------------------------ pages that sequences share
+
+def _attention_shared(what, q, pool_layer, scales_layer, block_tables, seq_lens, cu_group, shared_lens, cu_q,
+                      max_q_per_seq, causal, sm_scale, out, check, err):
+    N.need_gpu()
+    if scales_layer is None:
+        n_pages, Hkv, P, D = _pool4(pool_layer)
+    else:
+        if pool_layer.dim() != 5 or pool_layer.dtype != torch.uint8 or pool_layer.shape[1] != 2:
+            raise ValueError("pool_layer must be uint8 [n_pages, 2, Hkv, P, D]")
+        n_pages, _, Hkv, P, D = pool_layer.shape
+        if scales_layer.shape != (2, Hkv) or scales_layer.dtype != torch.float32:
+            raise ValueError(f"scales_layer must be float32 [2, {Hkv}]")
+        scales_layer = _aligned_scales(scales_layer)
+    if q.dim() != 3 or q.dtype != torch.bfloat16 or q.shape[2] != D:
+        raise ValueError(f"q must be bf16 [rows, Hq, {D}]")
+    n_q, Hq, _ = q.shape
+    if Hq == 0 or Hkv == 0 or Hq % Hkv:
+        raise ValueError("the number of query heads must be a multiple of the number of kv heads")
+    if block_tables.dtype != torch.int32 or block_tables.dim() != 2:
+        raise ValueError("block_tables must be int32 [B, max_blocks]")
+    B, mb = block_tables.shape
+    if shared_lens.dim() != 1:
+        raise ValueError("shared_lens must be int32 [n_groups]")
+    n_groups = shared_lens.shape[0]
+    for name, t, n in (("seq_lens", seq_lens, B), ("cu_group", cu_group, n_groups + 1),
+                       ("shared_lens", shared_lens, n_groups)) + ((("cu_q", cu_q, B + 1),) if cu_q is not None else ()):
+        if t.dtype != torch.int32 or t.shape != (n,):
+            raise ValueError(f"{name} must be int32 [{n}]")
+    if cu_q is None and n_q != B:
+        raise ValueError("without cu_q q must have one row per sequence")
+    if err is not None and (err.dtype != torch.int32 or err.numel() < 1 or err.device != q.device):
+        raise ValueError("err must be an int32 tensor on q's device")
+    if out is not None and (out.shape != q.shape or out.dtype != torch.bfloat16):
+        raise ValueError(f"out must be bf16 {tuple(q.shape)}")
+    q, index = q.contiguous(), _index(q, "q")
+    out = torch.empty_like(q) if out is None else out
+    _all_on(index, q=q, pool_layer=pool_layer, scales_layer=scales_layer, block_tables=block_tables, seq_lens=seq_lens,
+            cu_group=cu_group, shared_lens=shared_lens, cu_q=cu_q, out=out)
+    if cu_q is None:
+        mq = 1
+    elif max_q_per_seq is None:
+        mq = int((cu_q[1:] - cu_q[:-1]).max().item()) if B else 0
+    else:
+        mq = int(max_q_per_seq)
+    mq = max(0, min(mq, n_q))
+    with _on(index):
+        ws, nb = _workspace_for("zx_paged_attention_shared_workspace_bytes", index, n_q, B, n_groups, Hq, Hkv, D, mq)
+        err = _err_word_if(check, q.device) if err is None else err
+        entry = N.load().zx_paged_attention4_shared if scales_layer is None else N.load().zx_paged_attention_shared
+        N.check(entry(
+            q.data_ptr(), n_q, N.ptr(cu_q), Hq, pool_layer.data_ptr(), n_pages, Hkv, D, P,
+            *(() if scales_layer is None else (scales_layer.data_ptr(),)), block_tables.data_ptr(), mb,
+            seq_lens.data_ptr(), B, cu_group.data_ptr(), shared_lens.data_ptr(), n_groups, mq, int(bool(causal)),
+            D ** -0.5 if sm_scale is None else float(sm_scale), out.data_ptr(), N.ptr(err), N.ptr(ws), nb,
+            torch._C._cuda_getCurrentRawStream(index)), what)
+    if check:
+        _raise_kernel_error(err, what)
+    return out
+
+
+def paged_attention_shared(q: torch.Tensor, pool_layer: torch.Tensor, scales_layer: torch.Tensor,
+                           block_tables: torch.Tensor, seq_lens: torch.Tensor, cu_group: torch.Tensor,
+                           shared_lens: torch.Tensor, cu_q: torch.Tensor | None = None,
+                           max_q_per_seq: int | None = None, causal: bool = True, sm_scale: float | None = None,
+                           out: torch.Tensor | None = None, check: bool = False,
+                           err: torch.Tensor | None = None) -> torch.Tensor:
+    """``paged_attention_decode`` for a batch whose sequences share pages, the shared keys read and
+    multiplied once for all of them: sequences ``cu_group[g]`` to ``cu_group[g + 1]`` (int32
+    ``[n_groups + 1]``, ascending) have the same pages for their first ``shared_lens[g]`` (int32
+    ``[n_groups]``) positions.  ``block_tables`` ``[B, max_blocks]`` and ``seq_lens`` ``[B]`` are
+    those of whole sequences; the shared pages are read through the first sequence's row of a group
+    (a ``shared_lens`` that is no multiple of 16 is rounded down).  A sequence may be in no group.
+
+    q ``[B, Hq, D]`` bf16, one row per sequence; or with ``cu_q`` (int32 ``[B + 1]``) the newest rows
+    of every sequence, row i of n at position ``seq_lens[b] - n + i``, which sees the keys up to it
+    (all of them when not ``causal``).  ``max_q_per_seq`` bounds a sequence's rows (read back from
+    ``cu_q`` without it, which waits for the device); rows beyond it, and rows in no sequence, are
+    left as they are in ``out``.  Pages of a multiple of 16 tokens, head_dim 64, 128 or 256.
+    Softmax weights are rounded to fp16: error within one bf16 ulp + 2^-10 max|V|.  ``err``
+    (device int32 ``[1]``) collects the kernels' error bits; ``check`` reads them and raises."""
+    if scales_layer is None:
+        raise ValueError("scales_layer must be float32 [2, Hkv]")
+    return _attention_shared("paged_attention_shared", q, pool_layer, scales_layer, block_tables, seq_lens, cu_group,
+                             shared_lens, cu_q, max_q_per_seq, causal, sm_scale, out, check, err)
+
+
+def paged_attention4_shared(q: torch.Tensor, pool_layer: torch.Tensor, block_tables: torch.Tensor,
+                            seq_lens: torch.Tensor, cu_group: torch.Tensor, shared_lens: torch.Tensor,
+                            cu_q: torch.Tensor | None = None, max_q_per_seq: int | None = None, causal: bool = True,
+                            sm_scale: float | None = None, out: torch.Tensor | None = None, check: bool = False,
+                            err: torch.Tensor | None = None) -> torch.Tensor:
+    """``paged_attention_shared`` over a ``kv4_pool`` layer (which has no scales); softmax weights are
+    carried to 2^-17: error within one bf16 ulp + 2^-15 max|V|."""
+    return _attention_shared("paged_attention4_shared", q, pool_layer, None, block_tables, seq_lens, cu_group,
+                             shared_lens, cu_q, max_q_per_seq, causal, sm_scale, out, check, err)
