@@ -220,6 +220,12 @@ struct AttnPages {
   __device__ __forceinline__ uint32_t page_of(uint32_t t) const {
     return (uint32_t)(((uint64_t)t * p_magic) >> (31 + p_shift));
   }
+  // The page of position t (uniform), by the scalar cache: a vector load of it would be waited for
+  // together with the loads of K and V before it (shared pages, 128 x 32k positions 187 -> 105 us).
+  __device__ __forceinline__ int32_t page_id(uint32_t t) const {
+    typedef const __attribute__((address_space(4))) int32_t *scalar;
+    return reinterpret_cast<scalar>(reinterpret_cast<uintptr_t>(bt))[page_of(t)];
+  }
 };
 
 // Tokens below `end` of the tile at t: 0 to 16.  Without a difference that wraps where it is not
@@ -233,8 +239,9 @@ __device__ __forceinline__ uint32_t aw_tile_live(uint32_t end, uint32_t t) {
 // The attention of one wave: CT tiles of 16 columns (a column is a query row and head), its
 // steps of 32 keys, their softmax and accumulators.  Everything lives in registers; vt is the
 // wave's LDS.  EXACT: weights as bf16 hi + lo (2^-17), otherwise rounded once to F's 16-bit type.
-// POLICY: of the loads of K and V.
-template <class F, int CT, bool EXACT, int POLICY = AW_STREAM> struct AttnWave {
+// POLICY: of the loads of K and V.  MASK: columns may end before others (lim); without it all see
+// every key of a run.
+template <class F, int CT, bool EXACT, int POLICY = AW_STREAM, bool MASK = true> struct AttnWave {
   static constexpr int D = F::DIM;
   using Tile = typename F::Tile;
   static constexpr int NC = D / 32;  // products per tile of S^T
@@ -339,7 +346,7 @@ template <class F, int CT, bool EXACT, int POLICY = AW_STREAM> struct AttnWave {
   __device__ __forceinline__ void store_v(uint32_t t0, const Tile (&v)[2], const int (&rows)[2]) {
     uint32_t drop = 0;  // FP8: all ones where NaN codes are to go into the products as zeros
     if constexpr (F::BITS == 8) {
-      if (t0 + AW_STEP > lim_all) {  // uniform
+      if (MASK && t0 + AW_STEP > lim_all) {  // uniform
         uint32_t any = 0;
 #pragma unroll
         for (int T = 0; T < 2; ++T)
@@ -361,7 +368,7 @@ template <class F, int CT, bool EXACT, int POLICY = AW_STREAM> struct AttnWave {
 #pragma unroll
           for (int i = 0; i < F::NB; ++i) t.p[i] = n < rows[T] ? t.p[i] : 127u;
         }
-        if (t0 + AW_STEP > lim_all) {  // uniform
+        if (MASK && t0 + AW_STEP > lim_all) {  // uniform
 #pragma unroll
           for (int i = 0; i < F::NB; ++i) {
             const uint64_t bad = __builtin_amdgcn_ballot_w64(t.p[i] == K4_NAN);
@@ -402,7 +409,7 @@ template <class F, int CT, bool EXACT, int POLICY = AW_STREAM> struct AttnWave {
     }
   }
   __device__ __forceinline__ void mask(uint32_t t0, const int (&rows)[2], float (&s)[CT][8]) {
-    if (rows[0] < K4_TOK || rows[1] < K4_TOK || t0 + AW_STEP > lim_all) {  // uniform
+    if (rows[0] < K4_TOK || rows[1] < K4_TOK || (MASK && t0 + AW_STEP > lim_all)) {  // uniform
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
@@ -410,7 +417,7 @@ template <class F, int CT, bool EXACT, int POLICY = AW_STREAM> struct AttnWave {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int j = 4 * kg + i;
-            if (j >= rows[T] || t0 + 16 * T + j >= lim[ct]) s[ct][4 * T + i] = -INFINITY;
+            if (j >= rows[T] || (MASK && t0 + 16 * T + j >= lim[ct])) s[ct][4 * T + i] = -INFINITY;
           }
     }
   }
@@ -486,8 +493,8 @@ template <class F, int CT, bool EXACT, int POLICY = AW_STREAM> struct AttnWave {
     };
     int32_t page[2];
     auto pages_of_step = [&](uint32_t ts) {
-      page[0] = pg.bt[pg.page_of(min(ts, t_last))];
-      page[1] = pg.bt[pg.page_of(min(ts + K4_TOK, t_last))];
+      page[0] = pg.page_id(min(ts, t_last));
+      page[1] = pg.page_id(min(ts + K4_TOK, t_last));
     };
     auto load_tile = [&](uint32_t tp, int32_t id, Tile &k, Tile &v, int &r) {
       // (readfirstlane: uniform, but taken for a vector operand, and the loads then for a loop over lanes)

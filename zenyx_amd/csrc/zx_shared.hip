@@ -50,30 +50,31 @@ struct SharedArgs {
   float sm_scale;
 };
 
-// What the merge needs to know: written once per call by a block of its own.
+// What the merge needs to know of a sequence: written once per call by a block of its own.
 struct SharedSeq {
-  uint64_t first;   // the sequence's first own unit
+  uint32_t first;   // its first own unit
   uint32_t units;   // own units of each of its row tiles
-  int32_t g;        // its group, -1: none
-};
-struct SharedGroup {
-  uint64_t slot;    // of part 0 of its first row
-  int64_t row0, rows;
-  int64_t parts;    // 0: no shared keys
+  uint32_t parts;   // parts of its shared keys
+  uint32_t pad;
+  int64_t slot;     // of part 0 of its shared keys, for row 0 of q: row r's is slot + r
+  int64_t step;     // slots from one part to the next
 };
 struct SharedTable {
-  uint64_t *head;  // [2]: q, r of the deal
+  uint32_t *head;  // [2]: q, r of the deal
   SharedSeq *seq;
-  SharedGroup *grp;
-  __host__ __device__ SharedTable(void *at, int64_t n_seqs) {
-    head = static_cast<uint64_t *>(at);
-    seq = reinterpret_cast<SharedSeq *>(head + 2);
-    grp = reinterpret_cast<SharedGroup *>(seq + n_seqs);
+  __host__ __device__ explicit SharedTable(void *at) {
+    head = static_cast<uint32_t *>(at);
+    seq = reinterpret_cast<SharedSeq *>(head + 4);
   }
-  static size_t bytes(int64_t n_seqs, int64_t n_groups) {
-    return 2 * sizeof(uint64_t) + (size_t)n_seqs * sizeof(SharedSeq) + (size_t)n_groups * sizeof(SharedGroup);
-  }
+  static size_t bytes(int64_t n_seqs) { return 4 * sizeof(uint32_t) + (size_t)n_seqs * sizeof(SharedSeq); }
 };
+
+// A value that is the same in all lanes, as a scalar.
+__device__ __forceinline__ int32_t sh_uni(int32_t v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ uint32_t sh_uni(uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
+__device__ __forceinline__ int64_t sh_uni(int64_t v) {
+  return (int64_t)(((uint64_t)sh_uni((uint32_t)((uint64_t)v >> 32)) << 32) | sh_uni((uint32_t)v));
+}
 
 __device__ __forceinline__ int64_t sh_row(const SharedArgs &a, int32_t b) {
   return a.cu_q ? max((int64_t)0, min((int64_t)a.cu_q[b], a.n_q)) : b;
@@ -133,125 +134,151 @@ __device__ __forceinline__ ShSeq sh_seq(const SharedArgs &a, int32_t b, int32_t 
   return s;
 }
 
-// Sums over the block's threads (every thread gets them); lds: of 4 words per value.
-template <int N> __device__ __forceinline__ void sh_sums(uint64_t (&v)[N], uint64_t (*lds)[N]) {
-#pragma unroll
-  for (int i = 0; i < N; ++i)
-#pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) v[i] += __shfl_xor(v[i], off, 64);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0)
-#pragma unroll
-    for (int i = 0; i < N; ++i) lds[threadIdx.x >> 6][i] = v[i];
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = lds[0][i] + lds[1][i] + lds[2][i] + lds[3][i];
+template <int CTRL, int ROWS> __device__ __forceinline__ uint32_t sh_dpp(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false);
+}
+// Inclusive sum over the wave's lanes.
+__device__ __forceinline__ uint32_t sh_wave_scan(uint32_t v) {
+  v += sh_dpp<0x111, 0xF>(v);  // row_shr 1, 2, 4, 8
+  v += sh_dpp<0x112, 0xF>(v);
+  v += sh_dpp<0x114, 0xF>(v);
+  v += sh_dpp<0x118, 0xF>(v);
+  v += sh_dpp<0x142, 0xA>(v);  // row_bcast 15 into rows 1 and 3, 31 into rows 2 and 3
+  v += sh_dpp<0x143, 0xC>(v);
+  return v;
 }
 
 // How a call is dealt.
 constexpr int SH_CAND = 8;
+constexpr int SH_STAGE = 512;  // sequences (and groups) whose lengths are kept in LDS
 struct ShPlan {
-  uint32_t n_pre;     // blocks (per group of heads) for the groups' tiles
-  uint64_t n_seg;     // pieces of them
-  uint32_t piece;     // their units at most
-  uint64_t q, r;      // own units per block, and how many blocks have one more
+  uint32_t n_pre;  // blocks (per group of heads) for the groups' tiles
+  uint32_t n_seg;  // pieces of them
+  uint32_t piece;  // their units at most
+  uint32_t q, r;   // own units per block, and how many blocks have one more
 };
 struct ShLds {
-  uint64_t sums[ATT_WAVES][SH_CAND];
-  uint64_t base, slot;
+  uint32_t sums[ATT_WAVES][SH_CAND];
+  uint32_t base, slot;
   int32_t found;
-  // sequences [win, win + 256): what their runs need
-  int64_t row0[ATT_THREADS];
-  int32_t rows[ATT_THREADS];
-  uint32_t keys[ATT_THREADS], from[ATT_THREADS];
+  int32_t lens[SH_STAGE], shared[SH_STAGE], cu_q[SH_STAGE + 1], cu_group[SH_STAGE + 1];
 };
+
+// Sums over the block's threads, as scalars.
+template <int N> __device__ __forceinline__ void sh_sums(uint32_t (&v)[N], ShLds &lds) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = sh_wave_scan(v[i]);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 63)
+#pragma unroll
+    for (int i = 0; i < N; ++i) lds.sums[threadIdx.x >> 6][i] = v[i];
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = sh_uni(lds.sums[0][i] + lds.sums[1][i] + lds.sums[2][i] + lds.sums[3][i]);
+}
+// Inclusive sum over the block's threads of v, and the sum of all.
+__device__ __forceinline__ uint32_t sh_scan(uint32_t v, uint32_t &all, ShLds &lds, int at) {
+  const int wave = threadIdx.x >> 6;
+  v = sh_wave_scan(v);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 63) lds.sums[wave][at] = v;
+  __syncthreads();
+  all = 0;
+#pragma unroll
+  for (int w = 0; w < ATT_WAVES; ++w) {
+    const uint32_t n = lds.sums[w][at];
+    if (w < wave) v += n;
+    all += n;
+  }
+  all = sh_uni(all);
+  return v;
+}
+
+// The lengths into LDS, all loads at once, where they fit: the searches below then cost no trip
+// to memory each.
+__device__ __forceinline__ void sh_stage(SharedArgs &a, ShLds &lds) {
+  if (a.n_seqs > SH_STAGE) return;
+  for (int i = threadIdx.x; i <= a.n_seqs; i += ATT_THREADS) {
+    if (i < a.n_seqs) lds.lens[i] = a.seq_lens[i];
+    if (a.cu_q) lds.cu_q[i] = a.cu_q[i];
+    if (i < a.n_groups) lds.shared[i] = a.shared_lens[i];
+    if (a.n_groups && i <= a.n_groups) lds.cu_group[i] = a.cu_group[i];
+  }
+  __syncthreads();
+  a.seq_lens = lds.lens;
+  if (a.cu_q) a.cu_q = lds.cu_q;
+  a.shared_lens = lds.shared;
+  a.cu_group = lds.cu_group;
+}
 
 __device__ __forceinline__ ShPlan sh_plan(const SharedArgs &a, ShLds &lds, int32_t &e) {
   ShPlan p;
-  uint64_t pq[2] = {0, 0};
+  uint32_t pq[2] = {0, 0};  // (sums below 2^31: the host has seen to it)
   for (int32_t g = threadIdx.x; g < a.n_groups; g += ATT_THREADS) {
     const ShGroup s(a, g);
-    pq[0] += (uint64_t)s.units * s.tiles;
+    pq[0] += s.units * s.tiles;
   }
   for (int32_t b = threadIdx.x; b < a.n_seqs; b += ATT_THREADS) {
     const ShSeq s = sh_seq(a, b, e);
-    pq[1] += (uint64_t)s.units() * s.tiles(a);
+    pq[1] += s.units() * s.tiles(a);
   }
-  sh_sums<2>(pq, reinterpret_cast<uint64_t(*)[2]>(lds.sums));
-  const uint64_t P = pq[0], Q = pq[1], n = (uint64_t)a.n_run;
+  sh_sums<2>(pq, lds);
+  const uint32_t P = pq[0], Q = pq[1], n = (uint32_t)a.n_run;
   // blocks in the proportion of the work
-  const float share = (float)P * (float)a.cost_p / ((float)P * (float)a.cost_p + 4.0f * (float)Q);
-  p.n_pre = P == 0 ? 0u : Q == 0 ? (uint32_t)n : (uint32_t)max(1, min((int)n - 1, (int)((float)n * share + 0.5f)));
+  const float wp = (float)P * (float)a.cost_p, share = wp / (wp + 4.0f * (float)Q);
+  p.n_pre = P == 0 ? 0u : Q == 0 ? n : (uint32_t)max(1, min((int)n - 1, (int)((float)n * share + 0.5f)));
+  p.n_pre = sh_uni(p.n_pre);
   p.piece = 1;
   p.n_seg = 0;
   if (p.n_pre) {
     // A piece of L units at most costs L and about 3 more (its start, its part of the merge); of a
     // few lengths the one with which the last block ends first.
-    const uint64_t ideal = (P + p.n_pre - 1) / p.n_pre;
-    uint32_t len[SH_CAND];
-    uint64_t segs[SH_CAND];
+    const uint32_t ideal = (P + p.n_pre - 1) / p.n_pre;
+    uint32_t len[SH_CAND], segs[SH_CAND];
 #pragma unroll
     for (int k = 0; k < SH_CAND; ++k) {
       constexpr int EIGHTHS[SH_CAND] = {4, 8, 9, 10, 12, 16, 24, 32};
-      len[k] = (uint32_t)min((uint64_t)0x40000000u, (ideal * EIGHTHS[k] + 7) / 8);
+      len[k] = (uint32_t)(((uint64_t)ideal * EIGHTHS[k] + 7) / 8);
       segs[k] = 0;
     }
     for (int32_t g = threadIdx.x; g < a.n_groups; g += ATT_THREADS) {
       const ShGroup s(a, g);
 #pragma unroll
-      for (int k = 0; k < SH_CAND; ++k) segs[k] += (uint64_t)((s.units + len[k] - 1) / len[k]) * s.tiles;
+      for (int k = 0; k < SH_CAND; ++k) segs[k] += (s.units + len[k] - 1) / len[k] * s.tiles;
     }
-    sh_sums<SH_CAND>(segs, lds.sums);
+    sh_sums<SH_CAND>(segs, lds);
     uint64_t best = ~0ull;
 #pragma unroll
     for (int k = 0; k < SH_CAND; ++k) {
-      const uint64_t t = (segs[k] + p.n_pre - 1) / p.n_pre * (len[k] + 3);
+      const uint64_t t = (uint64_t)((segs[k] + p.n_pre - 1) / p.n_pre) * (len[k] + 3);
       if (t <= best) best = t, p.piece = len[k], p.n_seg = segs[k];
     }
-    if (Q == 0) p.n_pre = (uint32_t)n;
-    else if (p.n_seg < p.n_pre) p.n_pre = (uint32_t)p.n_seg;  // (the others take own units)
+    p.piece = sh_uni(p.piece);
+    p.n_seg = sh_uni(p.n_seg);
+    if (Q && p.n_seg < p.n_pre) p.n_pre = p.n_seg;  // (the others take own units)
   }
-  const uint64_t rest = n - p.n_pre;
-  p.q = rest ? Q / rest : 0;
-  p.r = rest ? Q % rest : 0;
+  const uint32_t rest = n - p.n_pre;
+  p.q = sh_uni(rest ? Q / rest : 0u);
+  p.r = sh_uni(rest ? Q - p.q * rest : 0u);
   return p;
 }
 
-// Inclusive sum over the block's threads of v, and the sum of all; every thread calls it.
-__device__ __forceinline__ uint64_t sh_scan(uint64_t v, uint64_t &all, ShLds &lds, int at) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const uint64_t y = __shfl_up(v, off, 64);
-    if (lane >= off) v += y;
-  }
-  __syncthreads();
-  if (lane == 63) lds.sums[wave][at] = v;
-  __syncthreads();
-  all = 0;
-#pragma unroll
-  for (int w = 0; w < ATT_WAVES; ++w) {
-    if (w < wave) v += lds.sums[w][at];
-    all += lds.sums[w][at];
-  }
-  return v;
-}
-
-// The group of piece `seg`: its number, its first piece and its first slot (found: -1 none).
-__device__ __forceinline__ void sh_find_group(const SharedArgs &a, uint32_t piece, uint64_t seg, ShLds &lds) {
-  uint64_t segs = 0, slots = 0;
+// The group of piece `seg`: its number (-1: none), its first piece and its first slot.
+__device__ __forceinline__ int32_t sh_find_group(const SharedArgs &a, uint32_t piece, uint32_t seg, uint32_t &base,
+                                                 uint32_t &slot, ShLds &lds) {
+  uint32_t segs = 0, slots = 0;
   __syncthreads();
   if (threadIdx.x == 0) lds.found = -1;
   for (int32_t g0 = 0; g0 < a.n_groups; g0 += ATT_THREADS) {  // uniform
     const int32_t g = g0 + threadIdx.x;
-    uint64_t n = 0, rows = 0, all_n, all_rows;
+    uint32_t n = 0, rows = 0, all_n, all_rows;
     if (g < a.n_groups) {
       const ShGroup s(a, g);
-      const uint64_t parts = (s.units + piece - 1) / piece;
+      const uint32_t parts = (s.units + piece - 1) / piece;
       n = parts * s.tiles;
-      rows = parts * (uint64_t)s.rows;
+      rows = parts * (uint32_t)s.rows;
     }
-    const uint64_t in = sh_scan(n, all_n, lds, 0), ir = sh_scan(rows, all_rows, lds, 1);
+    const uint32_t in = sh_scan(n, all_n, lds, 0), ir = sh_scan(rows, all_rows, lds, 1);
     if (segs + in > seg && segs + in - n <= seg) {
       lds.found = g;
       lds.base = segs + in - n;
@@ -262,104 +289,105 @@ __device__ __forceinline__ void sh_find_group(const SharedArgs &a, uint32_t piec
     if (segs > seg) break;  // uniform
   }
   __syncthreads();
+  base = sh_uni(lds.base);
+  slot = sh_uni(lds.slot);
+  return sh_uni(lds.found);
 }
 
-// Sequences [win, win + 256) into LDS.
-__device__ __forceinline__ uint64_t sh_window(const SharedArgs &a, int32_t win, ShLds &lds) {
-  const int32_t b = win + (int32_t)threadIdx.x;
-  int32_t e = 0;
-  ShSeq s = {};
-  if (b < a.n_seqs) s = sh_seq(a, b, e);
+// The sequence of own unit u, and its first unit.
+__device__ __forceinline__ int32_t sh_find_seq(const SharedArgs &a, uint32_t u, uint32_t &base, ShLds &lds) {
+  uint32_t before = 0;
   __syncthreads();
-  lds.row0[threadIdx.x] = s.row0;
-  lds.rows[threadIdx.x] = s.rows;
-  lds.keys[threadIdx.x] = s.keys;
-  lds.from[threadIdx.x] = s.from;
-  __syncthreads();
-  return b < a.n_seqs ? (uint64_t)s.units() * s.tiles(a) : 0;
-}
-// The sequence of own unit u: its number and first unit, with its window in LDS; returns the window's first.
-__device__ __forceinline__ int32_t sh_find_seq(const SharedArgs &a, uint64_t u, ShLds &lds) {
-  uint64_t before = 0;
-  int32_t win = 0;
-  for (;; win += ATT_THREADS) {  // uniform; u is below the sum of all
-    const uint64_t n = sh_window(a, win, lds);
-    uint64_t all;
-    const uint64_t in = sh_scan(n, all, lds, 0);
+  if (threadIdx.x == 0) lds.found = a.n_seqs;
+  for (int32_t b0 = 0; b0 < a.n_seqs; b0 += ATT_THREADS) {  // uniform
+    const int32_t b = b0 + (int32_t)threadIdx.x;
+    int32_t e = 0;
+    uint32_t n = 0, all;
+    if (b < a.n_seqs) {
+      const ShSeq s = sh_seq(a, b, e);
+      n = s.units() * s.tiles(a);
+    }
+    const uint32_t in = sh_scan(n, all, lds, 0);
     if (before + in > u && before + in - n <= u) {
-      lds.found = win + (int32_t)threadIdx.x;
+      lds.found = b;
       lds.base = before + in - n;
     }
     before += all;
-    if (before > u || win + ATT_THREADS >= a.n_seqs) break;
+    if (before > u) break;
   }
   __syncthreads();
-  return win;
+  base = sh_uni(lds.base);
+  return sh_uni(lds.found);
 }
 
 // The block of its own: the table.
 __device__ __forceinline__ void sh_write_table(const SharedArgs &a, const ShPlan &p, ShLds &lds, int32_t &e) {
-  const SharedTable t(a.table, a.n_seqs);
+  const SharedTable t(a.table);
   if (threadIdx.x == 0) {
     t.head[0] = p.q;
     t.head[1] = p.r;
   }
-  uint64_t before = 0;
+  uint32_t before = 0;
   for (int32_t b0 = 0; b0 < a.n_seqs; b0 += ATT_THREADS) {  // uniform
-    const int32_t b = b0 + threadIdx.x;
+    const int32_t b = b0 + (int32_t)threadIdx.x;
     ShSeq s = {};
     if (b < a.n_seqs) s = sh_seq(a, b, e);
-    const uint32_t units = b < a.n_seqs ? s.units() : 0u;
-    const uint64_t n = (uint64_t)units * s.tiles(a);
-    uint64_t all;
-    const uint64_t in = sh_scan(n, all, lds, 0);
-    if (b < a.n_seqs) t.seq[b] = SharedSeq{before + in - n, units, s.g};
+    const uint32_t units = b < a.n_seqs ? s.units() : 0u, n = units * s.tiles(a);
+    uint32_t all;
+    const uint32_t in = sh_scan(n, all, lds, 0);
+    if (b < a.n_seqs) t.seq[b] = SharedSeq{before + in - n, units, 0u, 0u, 0, 0};
     before += all;
   }
-  uint64_t slots = 0;
+  uint32_t slots = 0;
   for (int32_t g0 = 0; g0 < a.n_groups; g0 += ATT_THREADS) {  // uniform
-    const int32_t g = g0 + threadIdx.x;
-    uint64_t rows = 0, parts = 0, all;
+    const int32_t g = g0 + (int32_t)threadIdx.x;
+    uint32_t rows = 0, parts = 0, all;
     int64_t row0 = 0, n_rows = 0;
+    int32_t first = 0, last = 0;
     if (g < a.n_groups) {
       const ShGroup s(a, g);
       // groups are in order, and none reaches beyond the sequences
       if (a.cu_group[g] < 0 || a.cu_group[g + 1] < a.cu_group[g] || a.cu_group[g + 1] > a.n_seqs) e |= ZX_KERR_POS_RANGE;
       if (s.first < s.last && a.shared_lens[g] > 0 && (uint32_t)a.shared_lens[g] > a.cap) e |= ZX_KERR_POS_RANGE;
-      parts = s.tiles ? (s.units + p.piece - 1) / p.piece : 0;
-      rows = parts * (uint64_t)s.rows;
+      parts = s.tiles ? (s.units + p.piece - 1) / p.piece : 0u;
+      rows = parts * (uint32_t)s.rows;
       row0 = s.row0;
       n_rows = s.rows;
+      first = s.first;
+      last = s.last;
     }
-    const uint64_t ir = sh_scan(rows, all, lds, 0);
-    if (g < a.n_groups) t.grp[g] = SharedGroup{slots + ir - rows, row0, n_rows, (int64_t)parts};
+    const uint32_t ir = sh_scan(rows, all, lds, 0);  // (and behind its barriers the entries above are written)
+    const uint32_t slot = slots + ir - rows;
+    if (parts && (int64_t)slot + rows <= a.pre_slots)
+      for (int32_t b = first; b < last; ++b) {
+        t.seq[b].parts = parts;
+        t.seq[b].slot = (int64_t)slot - row0;
+        t.seq[b].step = n_rows;
+      }
     slots += all;
   }
 }
 
-// Up to 16 CT columns of a head group on keys [t_begin, t_end): rows row0 .. row0 + n_rows of q; lim(r):
-// keys below it count for row r; part(r): where row r's parts are (of its first head).
-template <class F, int CT, bool EXACT, int POLICY, class Lim, class Part>
+// Up to 16 CT columns of a head group on keys [t_begin, t_end): columns c0 .. c0 + cols of those of
+// rows row0 on; lim(r) (MASK): keys below it count for row r; part(r): where row r's parts are (of
+// its first head).
+template <class F, int CT, bool EXACT, int POLICY, bool MASK, class Lim, class Part>
 __device__ __forceinline__ void sh_segment(const SharedArgs &a, const AttnPages &pg, float scale, int G, int hq0,
-                                           int64_t row0, int n_rows, uint32_t t_begin, uint32_t t_end,
+                                           int64_t row0, int c0, int cols, uint32_t t_begin, uint32_t t_end,
                                            uint8_t (&lds)[ATT_WAVES][AttnLds<F::DIM>::WAVE],
                                            float (&sm_m)[ATT_WAVES][AW_COLS], float (&sm_l)[ATT_WAVES][AW_COLS],
                                            int32_t &e, Lim lim, Part part) {
   constexpr int D = F::DIM;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  AttnWave<F, CT, EXACT, POLICY> w(scale, lds[wave]);
-  const int cols = n_rows * G;
-  bool all = true;
+  AttnWave<F, CT, EXACT, POLICY, MASK> w(scale, lds[wave]);
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
-    const int c = 16 * ct + w.n, r = c / G;
-    const bool live = c < cols;
-    w.lim[ct] = live ? min(t_end, lim(r)) : t_end;
-    all &= w.lim[ct] == t_end;
+    const int c = c0 + 16 * ct + w.n, r = c / G;
+    const bool live = 16 * ct + w.n < cols;
+    if constexpr (MASK) w.lim[ct] = live ? min(t_end, lim(r)) : t_end;
     w.load_q(ct, a.q + ((row0 + (live ? r : 0)) * a.n_q_heads + hq0 + (live ? c - r * G : 0)) * D, live);
   }
-  // (0: every step is masked)
-  w.lim_all = __builtin_amdgcn_ballot_w64(!all) ? 0u : t_end;
+  if constexpr (MASK) w.lim_all = 0;  // every step is masked
   w.clear();
   const uint32_t t0 = t_begin + (uint32_t)wave * AW_STEP;
   if (t0 < t_end) w.run(pg, t0, t_end, ATT_WAVES * AW_STEP);
@@ -369,25 +397,28 @@ __device__ __forceinline__ void sh_segment(const SharedArgs &a, const AttnPages 
     if (16 * ct >= cols) break;  // block-uniform
     w.spill(ct, cols - 16 * ct, sm_m[wave], sm_l[wave]);
     __syncthreads();
-    const int c = 16 * ct + AttnEnd<D>::column();
-    if (c < cols) {
+    const int i = 16 * ct + AttnEnd<D>::column();
+    if (i < cols) {
       const AttnEnd<D> end(sm_m, sm_l, lds);
-      const int r = c / G;
-      end.store_part(part(r) + (int64_t)(hq0 + (c - r * G)) * (2 + D));
+      const int r = (c0 + i) / G;
+      end.store_part(part(r) + (int64_t)(hq0 + (c0 + i - r * G)) * (2 + D));
     }
     __syncthreads();
   }
 }
 
-__host__ __device__ constexpr int sh_per_cu(int D, int CT) { return D * CT > 128 ? 2 : CT > 1 ? 3 : 4; }
+// Blocks per CU by the registers of CT tiles of columns, and (D = 128) by LDS.
+__host__ __device__ constexpr int sh_per_cu(int D, int CT) { return D * CT > 128 ? 2 : CT > 1 || D == 128 ? 3 : 4; }
 
-template <class F, int CT, int CTO, bool EXACT>
+// CTO: column tiles of a sequence's own keys.  ROWS: several rows per sequence.
+template <class F, int CT, int CTO, bool EXACT, bool ROWS>
 __global__ void __launch_bounds__(ATT_THREADS, sh_per_cu(F::DIM, CT)) paged_shared_kernel(SharedArgs a) {
   constexpr int D = F::DIM;
   __shared__ __attribute__((aligned(16))) uint8_t lds[ATT_WAVES][AttnLds<D>::WAVE];
   __shared__ float sm_m[ATT_WAVES][AW_COLS], sm_l[ATT_WAVES][AW_COLS];
   __shared__ ShLds sh;
   int32_t e = 0;
+  sh_stage(a, sh);
   const ShPlan p = sh_plan(a, sh, e);
   const uint32_t x = blockIdx.x / (uint32_t)a.n_group;
   if (x >= (uint32_t)a.n_run) {
@@ -414,80 +445,88 @@ __global__ void __launch_bounds__(ATT_THREADS, sh_per_cu(F::DIM, CT)) paged_shar
   const int64_t row_part = (int64_t)a.n_q_heads * (2 + D);
 
   if (x < p.n_pre) {
-    for (uint64_t seg = x; seg < p.n_seg; seg += p.n_pre) {
-      sh_find_group(a, p.piece, seg, sh);
-      const int32_t g = sh.found;
+    for (uint32_t seg = x; seg < p.n_seg; seg += p.n_pre) {
+      uint32_t base, slot;
+      const int32_t g = sh_find_group(a, p.piece, seg, base, slot, sh);
       if (g < 0) break;
       const ShGroup s(a, g);
-      const uint32_t parts = (s.units + p.piece - 1) / p.piece;
-      const uint32_t local = (uint32_t)(seg - sh.base), n = local / s.tiles, tile = local - n * s.tiles;
-      const uint32_t t_begin = (uint32_t)((uint64_t)s.units * n / parts) * SH_UNIT;
-      const uint32_t t_end = min(s.len, (uint32_t)((uint64_t)s.units * (n + 1) / parts) * SH_UNIT);
-      const int64_t r0 = (int64_t)tile * a.rows_p;
-      const int n_rows = (int)min((int64_t)a.rows_p, s.rows - r0);
-      const uint64_t slot = sh.slot + (uint64_t)n * (uint64_t)s.rows + (uint64_t)r0;
+      const uint32_t units = sh_uni(s.units), tiles = sh_uni(s.tiles), len = sh_uni(s.len);
+      const int32_t b0 = sh_uni(s.first), b1 = sh_uni(s.last);
+      const uint32_t parts = (units + p.piece - 1) / p.piece;
+      const uint32_t n = (seg - base) / tiles, tile = (seg - base) - n * tiles;
+      const uint32_t t_begin = (uint32_t)((uint64_t)units * n / parts) * SH_UNIT;
+      const uint32_t t_end = min(len, (uint32_t)((uint64_t)units * (n + 1) / parts) * SH_UNIT);
+      const uint32_t r0 = tile * (uint32_t)a.rows_p, all_rows = sh_uni((uint32_t)s.rows);
+      const int n_rows = (int)min((uint32_t)a.rows_p, all_rows - r0);
+      const int64_t row0 = sh_uni(s.row0) + r0;
+      slot += n * all_rows + r0;
       // (more only where groups overlap)
-      if (slot + n_rows > (uint64_t)a.pre_slots) continue;
-      pg.bt = a.bt + (int64_t)s.first * a.max_blocks;
+      if ((int64_t)slot + n_rows > a.pre_slots) continue;
+      pg.bt = a.bt + (int64_t)b0 * a.max_blocks;
       auto lim = [&](int r) -> uint32_t {  // the row's own sequence may be shorter than what its group shares
-        const int64_t row = s.row0 + r0 + r;
+        const int64_t row = row0 + r;
         int32_t b = (int32_t)row;
         int64_t behind = 0;  // rows of the sequence after this one
-        if (a.cu_q) {
-          b = s.first;
-          int32_t hi = s.last - 1;
+        if (ROWS && a.cu_q) {
+          b = b0;
+          int32_t hi = b1 - 1;
           while (b < hi) {
             const int32_t mid = (b + hi + 1) >> 1;
             if (a.cu_q[mid] <= row) b = mid;
             else hi = mid - 1;
           }
           behind = a.causal ? (int64_t)a.cu_q[b + 1] - 1 - row : 0;
+        } else if (a.cu_q) {  // one row each at most: sequences without one between them
+          b = aw_seq_of(a.cu_q, a.n_seqs, (int32_t)row);
         }
         return (uint32_t)min(max((int64_t)a.seq_lens[b] - behind, (int64_t)0), (int64_t)a.cap);
       };
-      sh_segment<F, CT, EXACT, 0>(a, pg, scale, G, hq0, s.row0 + r0, n_rows, t_begin, t_end, lds, sm_m, sm_l, e, lim,
-                                  [&](int r) { return a.pre + (int64_t)(slot + r) * row_part; });
+      auto part = [&](int r) { return a.pre + (int64_t)(slot + r) * row_part; };
+      const int cols = n_rows * G;
+      // every row sees all of the piece?  (Otherwise a tile of columns at a time.)
+      bool all = true;
+      for (int r = threadIdx.x & 63; r < n_rows; r += 64) all &= lim(r) >= t_end;
+      if (!__builtin_amdgcn_ballot_w64(!all)) {
+        sh_segment<F, CT, EXACT, 0, false>(a, pg, scale, G, hq0, row0, 0, cols, t_begin, t_end, lds, sm_m, sm_l, e, lim,
+                                           part);
+      } else {
+        for (int c0 = 0; c0 < cols; c0 += AW_COLS)
+          sh_segment<F, 1, EXACT, 0, true>(a, pg, scale, G, hq0, row0, c0, min(AW_COLS, cols - c0), t_begin, t_end, lds,
+                                           sm_m, sm_l, e, lim, part);
+      }
     }
   } else {
-    const uint64_t xo = x - p.n_pre;
-    uint64_t u = xo * p.q + min(xo, p.r);
-    const uint64_t u_end = u + p.q + (xo < p.r ? 1 : 0);
+    const uint32_t xo = x - p.n_pre;
+    uint32_t u = xo * p.q + min(xo, p.r);
+    const uint32_t u_end = u + p.q + (xo < p.r ? 1 : 0);
     if (u < u_end) {
-      int32_t win = sh_find_seq(a, u, sh);
-      int32_t b = sh.found;
-      uint64_t base = sh.base;
-      while (u < u_end) {
-        if (b >= a.n_seqs) break;
-        if (b - win >= ATT_THREADS) {
-          win = b;
-          sh_window(a, win, sh);
-        }
-        ShSeq s;
-        s.row0 = sh.row0[b - win];
-        s.rows = sh.rows[b - win];
-        s.keys = sh.keys[b - win];
-        s.from = sh.from[b - win];
-        const uint32_t units = s.units(), tiles = units ? s.tiles(a) : 0u;
-        const uint64_t n = (uint64_t)units * tiles;
-        if (u >= base + n) {
-          base += n;
+      uint32_t base;
+      int32_t b = sh_find_seq(a, u, base, sh);
+      while (u < u_end && b < a.n_seqs) {
+        int32_t unused = 0;
+        const ShSeq s = sh_seq(a, b, unused);
+        const uint32_t units = sh_uni(s.units()), tiles = sh_uni(s.tiles(a));
+        if (u >= base + units * tiles) {
+          base += units * tiles;
           ++b;
           continue;
         }
-        const uint64_t local = u - base;
-        const uint32_t rt = (uint32_t)(local / units), u0 = (uint32_t)(local - (uint64_t)rt * units);
-        const uint32_t u1 = (uint32_t)min((uint64_t)units, u0 + (u_end - u));
-        const int r0 = (int)rt * a.rows_o, n_rows = min(a.rows_o, s.rows - r0);
+        const uint32_t keys = sh_uni(s.keys), from = sh_uni(s.from);
+        const int rows = sh_uni(s.rows);
+        const uint32_t rt = (u - base) / units, u0 = (u - base) - rt * units;
+        const uint32_t u1 = min(units, u0 + (u_end - u));
+        const int r0 = (int)rt * a.rows_o, n_rows = min(a.rows_o, rows - r0);
         // keys that row r of the tile sees
         auto lim = [&](int r) -> uint32_t {
-          return a.causal ? (uint32_t)max((int64_t)s.keys - (s.rows - 1 - r0 - r), (int64_t)0) : s.keys;
+          return ROWS && a.causal ? (uint32_t)max((int64_t)keys - (rows - 1 - r0 - r), (int64_t)0) : keys;
         };
-        const uint32_t t_begin = s.from + u0 * SH_UNIT;
-        const uint32_t t_end = min(min(s.keys, s.from + u1 * SH_UNIT), lim(n_rows - 1));
-        const uint64_t slot = (xo + (uint64_t)b * (uint64_t)a.n_rt + rt) * (uint64_t)a.rows_o;
+        const uint32_t t_begin = from + u0 * SH_UNIT;
+        const uint32_t t_end = min(min(keys, from + u1 * SH_UNIT), lim(n_rows - 1));
+        const int64_t slot = ((int64_t)xo + (int64_t)b * a.n_rt + rt) * a.rows_o;
         pg.bt = a.bt + (int64_t)b * a.max_blocks;
-        sh_segment<F, CTO, EXACT, AW_STREAM>(a, pg, scale, G, hq0, s.row0 + r0, n_rows, t_begin, t_end, lds, sm_m, sm_l,
-                                             e, lim, [&](int r) { return a.own + (int64_t)(slot + r) * row_part; });
+        sh_segment<F, CTO, EXACT, AW_STREAM, ROWS>(a, pg, scale, G, hq0, sh_uni(s.row0) + r0, 0, n_rows * G, t_begin,
+                                                   t_end, lds, sm_m, sm_l, e, lim,
+                                                   [&](int r) { return a.own + (slot + r) * row_part; });
         u += u1 - u0;
       }
     }
@@ -537,7 +576,7 @@ template <int D> __global__ void __launch_bounds__(256) shared_combine_kernel(Sh
   const int64_t row = at / a.n_q_heads;
   if (row >= a.n_q) return;
   const int hq = (int)(at - row * a.n_q_heads), d = threadIdx.x % D;
-  const SharedTable t(a.table, a.n_seqs);
+  const SharedTable t(a.table);
   int32_t b = (int32_t)row, i = 0;
   if (a.cu_q) {
     b = aw_seq_of(a.cu_q, a.n_seqs, (int32_t)row);
@@ -546,22 +585,17 @@ template <int D> __global__ void __launch_bounds__(256) shared_combine_kernel(Sh
     if (lo < 0 || row < lo || row >= hi || row - lo >= a.most) return;
     i = (int32_t)(row - lo);
   }
+  const AttnDeal<uint32_t> deal(t.head[0], t.head[1]);
   const SharedSeq s = t.seq[b];
-  const int64_t row_part = (int64_t)a.n_q_heads * (2 + D);
+  const int64_t row_part = (int64_t)a.n_q_heads * (2 + D), at_head = (int64_t)hq * (2 + D);
   ShCombine c;
-  if (s.g >= 0) {
-    const SharedGroup g = t.grp[s.g];
-    const uint64_t slot = g.slot + (uint64_t)(row - g.row0);
-    if (g.parts && slot + (uint64_t)((g.parts - 1) * g.rows) < (uint64_t)a.pre_slots)
-      c.add(a.pre + (int64_t)slot * row_part + (int64_t)hq * (2 + D), g.rows * row_part, (int)g.parts, d);
-  }
+  if (s.parts) c.add(a.pre + (s.slot + row) * row_part + at_head, s.step * row_part, (int)s.parts, d);
   if (s.units) {
-    const AttnDeal<uint64_t> deal(t.head[0], t.head[1]);
     const int32_t rt = i / a.rows_o;
-    const uint64_t u = s.first + (uint64_t)rt * s.units;
-    const uint64_t xa = deal.run_of(u), xz = deal.run_of(u + s.units - 1);
-    const int64_t slot = (int64_t)(xa + (uint64_t)b * (uint64_t)a.n_rt + (uint64_t)rt) * a.rows_o + (i - rt * a.rows_o);
-    c.add(a.own + slot * row_part + (int64_t)hq * (2 + D), a.rows_o * row_part, (int)(xz - xa + 1), d);
+    const uint32_t u = s.first + (uint32_t)rt * s.units;
+    const uint32_t xa = deal.run_of(u), xz = deal.run_of(u + s.units - 1);
+    const int64_t slot = ((int64_t)xa + (int64_t)b * a.n_rt + rt) * a.rows_o + (i - rt * a.rows_o);
+    c.add(a.own + slot * row_part + at_head, a.rows_o * row_part, (int)(xz - xa + 1), d);
   }
   const float sv = a.scales ? a.scales[a.n_kv_heads + hq / (a.n_q_heads / a.n_kv_heads)] : 1.0f;
   a.out[(row * a.n_q_heads + hq) * D + d] = (uint16_t)(pack_bf16(c.L == 0.0f ? 0.0f : c.A / c.L * sv, 0.0f) & 0xFFFFu);
@@ -591,8 +625,8 @@ static SharedHost sh_host(int64_t n_q, int32_t n_seqs, int32_t n_groups, int32_t
   const int64_t cols = ceil_div(n_q, std::max(n_groups, 1)) * p.group;
   p.ct = n_groups == 0 || cols <= 16 || tiles == 1 ? 1 : cols <= 32 ? 2 : tiles;
   const int64_t own = (int64_t)most * p.group;
-  if (own > 16 && p.ct == 1 && tiles > 1) p.ct = own <= 32 ? 2 : tiles;
-  p.ct_own = own <= 16 ? 1 : p.ct;
+  if (own > 16 && p.ct == 1 && tiles > 1) p.ct = 2;
+  p.ct_own = most == 1 || p.ct == 1 ? 1 : 2;
   p.rows_p = 16 * p.ct / p.group;
   p.rows_o = (int32_t)std::min<int64_t>(most, 16 * p.ct_own / p.group);
   p.n_rt = (int32_t)ceil_div(most, p.rows_o);
@@ -600,7 +634,7 @@ static SharedHost sh_host(int64_t n_q, int32_t n_seqs, int32_t n_groups, int32_t
   p.pre_slots = n_groups ? n_q + 2 * (p.n_run + 1) * p.rows_p : 0;
   p.own_slots = (p.n_run + (int64_t)n_seqs * p.n_rt) * p.rows_o;
   p.part_bytes = (size_t)((p.pre_slots + p.own_slots) * n_q_heads * (2 + head_dim)) * sizeof(float);
-  p.bytes = p.part_bytes + SharedTable::bytes(n_seqs, n_groups);
+  p.bytes = p.part_bytes + SharedTable::bytes(n_seqs);
   return p;
 }
 static bool sh_dims_ok(int64_t n_q, int32_t n_seqs, int32_t n_groups, int32_t n_q_heads, int32_t n_kv_heads,
@@ -616,8 +650,8 @@ extern "C" size_t zx_paged_attention_shared_workspace_bytes(int64_t n_q, int32_t
   return sh_host(n_q, n_seqs, n_groups, n_q_heads, n_kv_heads, head_dim, max_q_per_seq).bytes;
 }
 
-template <class F, int CT, int CTO, bool EXACT> static int sh_launch(const SharedArgs &a, hipStream_t st) {
-  paged_shared_kernel<F, CT, CTO, EXACT><<<(unsigned)(a.n_run * a.n_group + 1), ATT_THREADS, 0, st>>>(a);
+template <class F, int CT, int CTO, bool EXACT, bool ROWS> static int sh_launch(const SharedArgs &a, hipStream_t st) {
+  paged_shared_kernel<F, CT, CTO, EXACT, ROWS><<<(unsigned)(a.n_run * a.n_group + 1), ATT_THREADS, 0, st>>>(a);
   const int rc = check_launch("paged_shared");
   if (rc) return rc;
   shared_combine_kernel<F::DIM><<<(unsigned)ceil_div(a.n_q * a.n_q_heads, 256 / F::DIM), 256, 0, st>>>(a);
@@ -645,6 +679,11 @@ static int sh_call(const char *what, SharedArgs a, int32_t head_dim, int32_t max
   const SharedHost p = sh_host(a.n_q, a.n_seqs, a.n_groups, a.n_q_heads, a.n_kv_heads, head_dim, a.most);
   if (a.n_q * a.n_q_heads >= (1LL << 31) || (int64_t)a.n_seqs * p.n_rt >= (1LL << 31))
     return fail(ZX_ERR_UNSUPPORTED, "%s: too many rows", what);
+  // units are counted in 32 bits
+  const int64_t most_units = ceil_div((int64_t)a.max_blocks * a.page_size, SH_UNIT);
+  if ((int64_t)a.n_seqs * p.n_rt * most_units >= (1LL << 31) ||
+      (ceil_div(a.n_q, p.rows_p) + a.n_groups) * most_units >= (1LL << 31) || p.pre_slots >= (1LL << 31))
+    return fail(ZX_ERR_UNSUPPORTED, "%s: too many rows for block tables of so many positions", what);
   if (!workspace || workspace_bytes < p.bytes)
     return fail(ZX_ERR_WORKSPACE, "%s: workspace %zu < %zu bytes", what, workspace_bytes, p.bytes);
   a.pre = static_cast<float *>(workspace);
@@ -666,16 +705,10 @@ static int sh_call(const char *what, SharedArgs a, int32_t head_dim, int32_t max
     a.p_magic = (uint32_t)(((1ULL << (31 + sh)) + (uint64_t)a.page_size - 1) / (uint64_t)a.page_size);
   }
   const hipStream_t st = as_stream(stream);
-#define ZX_SH(D, CT, CTO) sh_launch<Page<D>, CT, CTO, EXACT>(a, st)
+#define ZX_SH(D, CT, CTO) (a.most > 1 ? sh_launch<Page<D>, CT, CTO, EXACT, true>(a, st) : sh_launch<Page<D>, CT, 1, EXACT, false>(a, st))
   switch (head_dim) {
-    case 64:
-      return p.ct == 1   ? ZX_SH(64, 1, 1)
-             : p.ct == 2 ? (p.ct_own == 1 ? ZX_SH(64, 2, 1) : ZX_SH(64, 2, 2))
-                         : (p.ct_own == 1 ? ZX_SH(64, 4, 1) : ZX_SH(64, 4, 4));
-    case 128:
-      return p.ct == 1   ? ZX_SH(128, 1, 1)
-             : p.ct == 2 ? (p.ct_own == 1 ? ZX_SH(128, 2, 1) : ZX_SH(128, 2, 2))
-                         : (p.ct_own == 1 ? ZX_SH(128, 3, 1) : ZX_SH(128, 3, 3));
+    case 64: return p.ct == 1 ? ZX_SH(64, 1, 1) : p.ct == 2 ? ZX_SH(64, 2, 2) : ZX_SH(64, 4, 2);
+    case 128: return p.ct == 1 ? ZX_SH(128, 1, 1) : p.ct == 2 ? ZX_SH(128, 2, 2) : ZX_SH(128, 3, 2);
     default: return ZX_SH(256, 1, 1);
   }
 #undef ZX_SH
