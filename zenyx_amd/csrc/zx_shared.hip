@@ -44,7 +44,6 @@ struct SharedArgs {
   int32_t n_rt;            // row tiles of a sequence at most
   int32_t n_run;           // blocks per group of heads
   uint32_t cap;            // positions that a block table holds
-  uint32_t cost_p;         // of a group's unit, in quarters of an own unit
   uint32_t p_magic;
   int32_t p_shift;
   float sm_scale;
@@ -224,8 +223,11 @@ __device__ __forceinline__ ShPlan sh_plan(const SharedArgs &a, ShLds &lds, int32
   }
   sh_sums<2>(pq, lds);
   const uint32_t P = pq[0], Q = pq[1], n = (uint32_t)a.n_run;
-  // blocks in the proportion of the work
-  const float wp = (float)P * (float)a.cost_p, share = wp / (wp + 4.0f * (float)Q);
+  // Blocks in the proportion of the units: a group's unit is bound by its products and an own one
+  // by its reads, and they take about as long as each other (a group's counted for 2 / 1.25 / 1 / 0.75
+  // own ones: 64 sequences on 2,048 shared positions and 100-2,000 each 54 / 51 / 52 / 51 us, 50 rows
+  // of 4-bit pages in 4 groups on 4k-16k shared ones 112 / 79 / 79 / 79).
+  const float share = (float)P / ((float)P + (float)Q);
   p.n_pre = P == 0 ? 0u : Q == 0 ? n : (uint32_t)max(1, min((int)n - 1, (int)((float)n * share + 0.5f)));
   p.n_pre = sh_uni(p.n_pre);
   p.piece = 1;
@@ -534,41 +536,44 @@ __global__ void __launch_bounds__(ATT_THREADS, sh_per_cu(F::DIM, CT)) paged_shar
   if (e && a.err) atomicOr(a.err, e);
 }
 
-// A channel of a row over its parts: att_combine_row's state, for lists one after the other.
-struct ShCombine {
-  float M = -INFINITY, L = 0.0f, A = 0.0f;
-  __device__ __forceinline__ void add(const float *pp, int64_t step, int n, int d) {
-    const int lane = threadIdx.x & 63;
-    for (int base = 0; base < n; base += 64) {
-      const int cnt = min(64, n - base);
-      const float *p0 = pp + (int64_t)base * step;
-      const float ms = lane < cnt ? p0[lane * step] : -INFINITY;
-      const float ls = lane < cnt ? p0[lane * step + 1] : 0.0f;
-      float v[CB_U];
-#pragma unroll
-      for (int u = 0; u < CB_U; ++u) v[u] = p0[min(u, cnt - 1) * step + 2 + d];
-      const float Mn = fmaxf(M, xrow_max(row16_max(ms)));
-      const float alpha = __builtin_amdgcn_exp2f(M - Mn);  // (parts' maxima are finite: Mn is, after the first)
-      const float w = __builtin_amdgcn_exp2f(ms - Mn);
-      M = Mn;
-      L = L * alpha + att_xrow_sum(group_sum<16>(w * ls));
-      A *= alpha;
-      for (int s = 0; s < cnt; s += CB_U) {
-        float nx[CB_U];
-        if (s + CB_U < cnt) {
-#pragma unroll
-          for (int u = 0; u < CB_U; ++u) nx[u] = p0[min(s + CB_U + u, cnt - 1) * step + 2 + d];
-        }
-#pragma unroll
-        for (int u = 0; u < CB_U; ++u)
-          if (s + u < cnt)
-            A += __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), s + u)) * v[u];
-#pragma unroll
-        for (int u = 0; u < CB_U; ++u) v[u] = nx[u];
-      }
-    }
+// A channel of a row over its parts: as att_combine_row merges them, from two lists.
+struct ShParts {
+  const float *p[2];  // part 0 of each list
+  int64_t step[2];
+  int n[2];
+  __device__ __forceinline__ const float *at(int i) const {
+    return i < n[0] ? p[0] + i * step[0] : p[1] + (i - n[0]) * step[1];
   }
 };
+__device__ __forceinline__ float sh_combine(const ShParts &parts, int d) {
+  const int lane = threadIdx.x & 63, n = parts.n[0] + parts.n[1];
+  float M = -INFINITY, L = 0.0f, A = 0.0f;
+  for (int base = 0; base < n; base += 64) {
+    const int cnt = min(64, n - base);
+    const float2 ml = lane < cnt ? *reinterpret_cast<const float2 *>(parts.at(base + lane)) : make_float2(-INFINITY, 0.0f);
+    float v[CB_U];
+#pragma unroll
+    for (int u = 0; u < CB_U; ++u) v[u] = parts.at(base + min(u, cnt - 1))[2 + d];
+    const float Mn = fmaxf(M, xrow_max(row16_max(ml.x)));  // (parts' maxima are finite)
+    const float alpha = __builtin_amdgcn_exp2f(M - Mn), w = __builtin_amdgcn_exp2f(ml.x - Mn);
+    M = Mn;
+    L = L * alpha + att_xrow_sum(group_sum<16>(w * ml.y));
+    A *= alpha;
+    for (int s = 0; s < cnt; s += CB_U) {
+      float nx[CB_U];
+      if (s + CB_U < cnt) {
+#pragma unroll
+        for (int u = 0; u < CB_U; ++u) nx[u] = parts.at(base + min(s + CB_U + u, cnt - 1))[2 + d];
+      }
+#pragma unroll
+      for (int u = 0; u < CB_U; ++u)
+        if (s + u < cnt) A += __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), s + u)) * v[u];
+#pragma unroll
+      for (int u = 0; u < CB_U; ++u) v[u] = nx[u];
+    }
+  }
+  return L == 0.0f ? 0.0f : A / L;
+}
 
 // The rows: D threads per (row, head).
 template <int D> __global__ void __launch_bounds__(256) shared_combine_kernel(SharedArgs a) {
@@ -588,17 +593,23 @@ template <int D> __global__ void __launch_bounds__(256) shared_combine_kernel(Sh
   const AttnDeal<uint32_t> deal(t.head[0], t.head[1]);
   const SharedSeq s = t.seq[b];
   const int64_t row_part = (int64_t)a.n_q_heads * (2 + D), at_head = (int64_t)hq * (2 + D);
-  ShCombine c;
-  if (s.parts) c.add(a.pre + (s.slot + row) * row_part + at_head, s.step * row_part, (int)s.parts, d);
+  ShParts c = {};
+  if (s.parts) {
+    c.p[0] = a.pre + (s.slot + row) * row_part + at_head;
+    c.step[0] = s.step * row_part;
+    c.n[0] = (int)s.parts;
+  }
   if (s.units) {
     const int32_t rt = i / a.rows_o;
     const uint32_t u = s.first + (uint32_t)rt * s.units;
     const uint32_t xa = deal.run_of(u), xz = deal.run_of(u + s.units - 1);
     const int64_t slot = ((int64_t)xa + (int64_t)b * a.n_rt + rt) * a.rows_o + (i - rt * a.rows_o);
-    c.add(a.own + slot * row_part + at_head, a.rows_o * row_part, (int)(xz - xa + 1), d);
+    c.p[1] = a.own + slot * row_part + at_head;
+    c.step[1] = a.rows_o * row_part;
+    c.n[1] = (int)(xz - xa + 1);
   }
   const float sv = a.scales ? a.scales[a.n_kv_heads + hq / (a.n_q_heads / a.n_kv_heads)] : 1.0f;
-  a.out[(row * a.n_q_heads + hq) * D + d] = (uint16_t)(pack_bf16(c.L == 0.0f ? 0.0f : c.A / c.L * sv, 0.0f) & 0xFFFFu);
+  a.out[(row * a.n_q_heads + hq) * D + d] = (uint16_t)(pack_bf16(sh_combine(c, d) * sv, 0.0f) & 0xFFFFu);
 }
 
 }  // namespace zx
@@ -697,7 +708,6 @@ static int sh_call(const char *what, SharedArgs a, int32_t head_dim, int32_t max
   a.n_rt = p.n_rt;
   a.n_run = (int32_t)p.n_run;
   a.cap = (uint32_t)((int64_t)a.max_blocks * a.page_size);
-  a.cost_p = p.ct == 1 ? 4 : p.ct == 2 ? 5 : 8;
   {  // magic division by the page size for positions below 2^31
     int sh = 0;
     while ((1LL << sh) < a.page_size) ++sh;
