@@ -594,6 +594,44 @@ int zx_paged_attention4_shared(const uint16_t *q, int64_t n_q, const int32_t *cu
                                float sm_scale, uint16_t *out, int32_t *err, void *workspace, size_t workspace_bytes,
                                zx_stream_t stream);
 
+/* ---------------------------------------------------------------------------
+ * Attention of packed query rows to packed states of other lengths, with its gradients (cross
+ * attention to an encoder's states; ABI version 10).  dtype ZX_BF16 or ZX_F16.  q [n_q][n_q_heads]
+ * [head_dim], k and v [n_k][n_kv_heads][head_dim] with strides in elements (channels contiguous, every row of
+ * a head 16-byte aligned): rows [cu_q[b], cu_q[b + 1]) attend to all of the keys [cu_k[b], cu_k[b + 1]),
+ * with k_lens (device int32, may be NULL) to the first k_lens[b] of them (what the others hold does not
+ * count, and their gradients are zeros).  Query head i reads KV head i / (n_q_heads / n_kv_heads).
+ * out [n_q][n_q_heads][head_dim] contiguous; lse2 (may be NULL) [n_q_heads][n_q] fp32, log2 of a row's sum
+ * of exponentials.  A row without a key gives zeros and -inf.  Scores and sums in fp32, softmax
+ * weights rounded once to dtype (fp16: times 2^7): |error| <= half an ulp + 2^-8 max|v| (fp16: 2^-11).
+ * Rows beyond max_q_per_seq and keys beyond max_k_per_seq (both host) are not computed or seen, nor
+ * do rows that cu_q or cu_k claim beyond n_q or n_k exist (either sets ZX_KERR_POS_RANGE).  Rows in no
+ * sequence are left unwritten, with ZX_CROSS_ZERO_REST zeros.  head_dim 64 or 128.  workspace: the
+ * query's device bytes (0: NULL will do), 16-byte aligned; it holds nothing between calls. */
+enum zx_cross_flags { ZX_CROSS_ZERO_REST = 1 };
+size_t zx_cross_attention_workspace_bytes(int64_t n_q, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim,
+                                          int32_t n_seqs, int32_t max_q_per_seq, int32_t max_k_per_seq);
+int zx_cross_attention(int dtype, const void *q, int64_t n_q, int64_t q_row_stride, int64_t q_head_stride,
+                       int32_t n_q_heads, const void *k, int64_t k_row_stride, int64_t k_head_stride, const void *v,
+                       int64_t v_row_stride, int64_t v_head_stride, int64_t n_k, int32_t n_kv_heads, int32_t head_dim,
+                       const int32_t *cu_q, const int32_t *cu_k, const int32_t *k_lens, int32_t n_seqs,
+                       int32_t max_q_per_seq, int32_t max_k_per_seq, float sm_scale, int32_t flags, void *out,
+                       float *lse2, int32_t *err, void *workspace, size_t workspace_bytes, zx_stream_t stream);
+/* Its gradients, from the output's (strided as q), out and lse2 as zx_cross_attention left them: dq, dk,
+ * dv contiguous, of rows in no sequence zeros.  The score's gradients are rounded once to dtype
+ * (fp16: they have to be below 65504), every sum is in fp32 and in a fixed order. */
+size_t zx_cross_attention_backward_workspace_bytes(int64_t n_q, int64_t n_k, int32_t n_q_heads, int32_t n_kv_heads,
+                                                   int32_t head_dim, int32_t n_seqs, int32_t max_q_per_seq,
+                                                   int32_t max_k_per_seq);
+int zx_cross_attention_backward(int dtype, const void *grad, int64_t g_row_stride, int64_t g_head_stride,
+                                const void *q, int64_t n_q, int64_t q_row_stride, int64_t q_head_stride,
+                                int32_t n_q_heads, const void *k, int64_t k_row_stride, int64_t k_head_stride,
+                                const void *v, int64_t v_row_stride, int64_t v_head_stride, int64_t n_k,
+                                int32_t n_kv_heads, int32_t head_dim, const void *out, const float *lse2,
+                                const int32_t *cu_q, const int32_t *cu_k, const int32_t *k_lens, int32_t n_seqs,
+                                int32_t max_q_per_seq, int32_t max_k_per_seq, float sm_scale, void *dq, void *dk,
+                                void *dv, int32_t *err, void *workspace, size_t workspace_bytes, zx_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -34,6 +34,7 @@ ZX_HEADS_TWO_PASS = 1
 ZX_HEADS_SINGLE_PASS = 2
 ZX_NEVER = 0x7FFFFFFF
 ZX_ROPE_INTERLEAVED, ZX_ROPE_TRANSPOSE = 16, 32
+ZX_CROSS_ZERO_REST = 1
 ABI_VERSION = 10
 
 _P = ctypes.c_void_p
@@ -106,6 +107,13 @@ SIGNATURES = {
                                          _I32, _I32, _I32, ctypes.c_float, _P, _P, _P, _SZ, _P]),
     "zx_paged_attention4_shared": (_INT, [_P, _I64, _P, _I32, _P, _I64, _I32, _I32, _I32, _P, _I32, _P, _I32, _P, _P,
                                           _I32, _I32, _I32, ctypes.c_float, _P, _P, _P, _SZ, _P]),
+    "zx_cross_attention_workspace_bytes": (_SZ, [_I64, _I32, _I32, _I32, _I32, _I32, _I32]),
+    "zx_cross_attention": (_INT, [_INT, _P, _I64, _I64, _I64, _I32, _P, _I64, _I64, _P, _I64, _I64, _I64, _I32, _I32, _P,
+                                  _P, _P, _I32, _I32, _I32, ctypes.c_float, _I32, _P, _P, _P, _P, _SZ, _P]),
+    "zx_cross_attention_backward_workspace_bytes": (_SZ, [_I64, _I64, _I32, _I32, _I32, _I32, _I32, _I32]),
+    "zx_cross_attention_backward": (_INT, [_INT, _P, _I64, _I64, _P, _I64, _I64, _I64, _I32, _P, _I64, _I64, _P, _I64, _I64,
+                                           _I64, _I32, _I32, _P, _P, _P, _P, _P, _I32, _I32, _I32, ctypes.c_float, _P, _P,
+                                           _P, _P, _P, _SZ, _P]),
 }
 
 _lib = None

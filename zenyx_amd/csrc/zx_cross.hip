@@ -1,0 +1,1030 @@
+// zx_cross.hip -- attention of packed query rows to packed states of other lengths (cross attention
+// to an encoder's states), and its gradients.  bf16 and fp16.
+//
+//   s_rt = sm_scale q_r . k_t,  p = softmax over the sequence's keys,  o_r = sum_t p_rt v_t,
+//   lse_r = log2 sum_t 2^(s_rt log2 e);
+//   with D_r = sum_d dO_rd o_rd:  p = 2^(s log2 e - lse),  dS = p (dO . v - D),
+//   dq = sm_scale dS k,  dk = sm_scale dS^T q,  dv = p^T dO  (dk, dv over the KV head's query heads).
+//
+// All on v_mfma_f32_32x32x16, transposed so that the products' outputs are the next ones' operands:
+// a score tile's lanes hold a column each (32 of them, two lanes with 16 rows of the tile each), and
+// 8 of a lane's values are one B operand of the next product if that product's other operand
+// takes the 16 rows in the order 16 c + 8 a + 4 half + b.  It is read transposed from LDS
+// (ds_read_b64_tr_b16) in that order.
+//   forward, dq:  columns are (query row, head of the KV head's group); K and V tiles of 64 keys in
+//                 LDS; S^T = K Q^T, dP^T = V dO^T, O^T += V^T P^T, dQ^T += K^T dS^T
+//   dk, dv:       columns are keys, whose K and V stay in registers; Q and dO tiles of 64 (row, head)
+//                 in LDS; S = Q K^T, dP = dO V^T, dV^T += dO^T P, dK^T += Q^T dS
+// Every sum has a fixed order: gradients do not change from call to call (dq has a kernel of its
+// own, two of seven products more than atomics would need).  Bound by the matrix products and
+// the LDS reads that feed them; a call of few rows by the reads of K and V, its keys cut among
+// blocks and the parts merged.
+#include <algorithm>
+
+#include "zx_attn_common.h"
+#include "zx_internal.h"
+
+namespace zx {
+
+typedef float cr_f32x16 __attribute__((ext_vector_type(16)));
+typedef short cr_i16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 cr_f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 cr_f16x2 __attribute__((ext_vector_type(2)));
+
+constexpr int CR_THREADS = 256, CR_WAVES = 4;
+constexpr int CR_TILE = 64;  // rows of a tile in LDS
+constexpr float CR_NONE = -3.402823466e38f;
+constexpr float CR_LAZY = 8.0f;  // a maximum is raised when a score exceeds it by more (log2)
+
+struct CrBf16 {
+  static constexpr float BIAS = 0.0f;
+  static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack_bf16(a, b); }
+  static __device__ __forceinline__ float lo(uint32_t w) { return bf_lo(w); }
+  static __device__ __forceinline__ float hi(uint32_t w) { return bf_hi(w); }
+  static __device__ __forceinline__ cr_f32x16 mfma(att_u32x4 a, att_u32x4 b, cr_f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(att_bf16x8, a), __builtin_bit_cast(att_bf16x8, b), c,
+                                                   0, 0, 0);
+  }
+};
+// Weights times 2^BIAS: fp16 loses bits of what is below 2^-14.
+struct CrF16 {
+  static constexpr float BIAS = 7.0f;
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    return __builtin_bit_cast(uint32_t, cr_f16x2{(_Float16)a, (_Float16)b});
+  }
+  static __device__ __forceinline__ float lo(uint32_t w) { return (float)__builtin_bit_cast(cr_f16x2, w)[0]; }
+  static __device__ __forceinline__ float hi(uint32_t w) { return (float)__builtin_bit_cast(cr_f16x2, w)[1]; }
+  static __device__ __forceinline__ cr_f32x16 mfma(att_u32x4 a, att_u32x4 b, cr_f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(cr_f16x8, a), __builtin_bit_cast(cr_f16x8, b), c, 0, 0,
+                                                  0);
+  }
+};
+
+// Rows [n][heads][D], strides in elements.
+struct CrIn {
+  const uint16_t *p;
+  int64_t row, head;
+};
+struct CrossArgs {
+  CrIn q, k, v, o, g;       // g: the output's gradient
+  const int32_t *cu_q, *cu_k, *k_lens;
+  uint16_t *out;            // forward: out; dq
+  uint16_t *dk, *dv;
+  float *lse, *delta;       // [n_q_heads][n_q]
+  float *part;              // forward: [split][n_q][n_q_heads][2 + D]; gradients: [split][rows][heads][D] each
+  int32_t *err;
+  int64_t n_q, n_k;
+  int32_t n_q_heads, n_kv_heads, n_seqs, group;
+  int32_t max_q, max_k;
+  int32_t n_tile, n_split;  // tiles of a sequence and KV head at most, parts of each
+  int32_t zero_rest;
+  float sm_scale;
+};
+
+// Rows [lo, hi) of the packed n that sequence b has, none outside and at most `most`.
+struct CrSpan {
+  int64_t lo;
+  int32_t n;
+};
+__device__ __forceinline__ CrSpan cr_span(const int32_t *cu, int32_t b, int64_t n, int32_t most, int32_t &e) {
+  const int64_t lo = cu[b], hi = cu[b + 1];
+  if (lo < 0 || hi > n || hi - lo > most || hi < lo) e |= ZX_KERR_POS_RANGE;
+  return CrSpan{lo < 0 ? 0 : lo, lo < 0 ? 0 : (int32_t)max((int64_t)0, min(min(hi, n) - lo, (int64_t)most))};
+}
+__device__ __forceinline__ int32_t cr_keys(const CrossArgs &a, int32_t b, int32_t n) {
+  return a.k_lens ? max(0, min(a.k_lens[b], n)) : n;
+}
+
+// What a block does: tiles of one sequence and KV head on the same XCD (block ids go round the
+// eight), so that what they read in common is in its L2.
+struct CrItem {
+  int32_t b, h, tile, split;
+  bool any;
+};
+__device__ __forceinline__ CrItem cr_item(const CrossArgs &a) {
+  const uint32_t xcd = blockIdx.x & 7u, i = blockIdx.x >> 3, per = (uint32_t)(a.n_tile * a.n_split);
+  const uint32_t pair = (i / per) * 8 + xcd, rem = i - (i / per) * per;
+  CrItem it;
+  it.any = pair < (uint32_t)(a.n_seqs * a.n_kv_heads);
+  it.b = (int32_t)(pair / (uint32_t)a.n_kv_heads);
+  it.h = (int32_t)(pair - (uint32_t)it.b * (uint32_t)a.n_kv_heads);
+  it.tile = (int32_t)(rem / (uint32_t)a.n_split);
+  it.split = (int32_t)(rem - (uint32_t)it.tile * (uint32_t)a.n_split);
+  return it;
+}
+static unsigned cr_grid(const CrossArgs &a) {
+  return (unsigned)(8 * ceil_div((int64_t)a.n_seqs * a.n_kv_heads, 8) * a.n_tile * a.n_split);
+}
+
+// A tile of 64 rows in LDS: rows of D 16-bit values, 32 bytes apart (mod 128) and the 16-byte
+// chunks of rows 4-7 of 8 swapped in pairs: the 8 lanes of a 16-byte read (8 rows) and the 16
+// of a transposing one (4 rows of 32 bytes) touch distinct banks, and a store writes a row's chunks in a run.
+template <int D> struct CrLds {
+  static constexpr int ROW = 2 * D + 32;
+  static constexpr int BYTES = CR_TILE * ROW;
+  static constexpr int LOADS = CR_TILE * D / 8 / CR_THREADS;  // 16 bytes each, per thread
+  static constexpr int CHUNKS = D / 8;
+};
+template <int D> __device__ __forceinline__ uint8_t *cr_at(uint8_t *t, int row, int byte) {
+  return t + row * CrLds<D>::ROW + (byte ^ (16 * ((row >> 2) & 1)));
+}
+// Row 32 kt + (lane & 31), channels 16 kc + 8 half ..+8: an operand whose rows (or columns) are the tile's.
+template <int D> __device__ __forceinline__ att_u32x4 cr_rows(uint8_t *t, int kt, int kc, int lane) {
+  return *reinterpret_cast<const att_u32x4 *>(cr_at<D>(t, 32 * kt + (lane & 31), 32 * kc + 16 * (lane >> 5)));
+}
+// Channel 32 dt + (lane & 31) of rows 16 c + 8 a + 4 half + b (a = 0, 1; b = 0 .. 3): a transposed operand.
+template <int D> __device__ __forceinline__ att_u32x4 cr_cols(uint8_t *t, int c, int dt, int lane) {
+  const int row = 16 * c + 4 * (lane >> 5) + ((lane & 15) >> 2);
+  const uint8_t *p = cr_at<D>(t, row, 64 * dt + 32 * ((lane >> 4) & 1) + 8 * (lane & 3));
+  typedef __attribute__((address_space(3))) cr_i16x4 *lds_ptr;
+  const uint2 x = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p)));
+  const uint2 y = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p + 8 * CrLds<D>::ROW)));
+  return att_u32x4{x.x, x.y, y.x, y.y};
+}
+// 16 values of a product's column as the two operands of the next product.
+template <class T> __device__ __forceinline__ void cr_operands(const float (&x)[16], att_u32x4 (&o)[2]) {
+#pragma unroll
+  for (int c = 0; c < 2; ++c)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[c][i] = T::pack(x[8 * c + 2 * i], x[8 * c + 2 * i + 1]);
+}
+
+// The tile's loads, in registers until the LDS buffer is free.  Rows from n on are zeros (and not read).
+template <int D> struct CrStage {
+  uint4 x[CrLds<D>::LOADS];
+  static __device__ __forceinline__ int row(int j) {
+    return (int)threadIdx.x / CrLds<D>::CHUNKS + j * (CR_THREADS / CrLds<D>::CHUNKS);
+  }
+  static __device__ __forceinline__ int chunk() { return (int)threadIdx.x % CrLds<D>::CHUNKS; }
+  // n >= 1 rows of `step` elements from p on
+  __device__ __forceinline__ void load(const uint16_t *p, int64_t step, int n) {
+#pragma unroll
+    for (int j = 0; j < CrLds<D>::LOADS; ++j)
+      x[j] = *reinterpret_cast<const uint4 *>(p + min(row(j), n - 1) * step + 8 * chunk());
+  }
+  // (row, head) pairs c0 .. of a group: pair c is row c / G, head c % G
+  __device__ __forceinline__ void load_pairs(const uint16_t *p, int64_t step, int64_t head, int c0, int n, int G) {
+#pragma unroll
+    for (int j = 0; j < CrLds<D>::LOADS; ++j) {
+      const uint32_t c = (uint32_t)(c0 + min(row(j), n - 1)), r = c / (uint32_t)G;
+      x[j] = *reinterpret_cast<const uint4 *>(p + (int64_t)r * step + (int64_t)(c - r * (uint32_t)G) * head + 8 * chunk());
+    }
+  }
+  __device__ __forceinline__ void store(uint8_t *t, int n) const {
+#pragma unroll
+    for (int j = 0; j < CrLds<D>::LOADS; ++j) {
+      const uint4 z = row(j) < n ? x[j] : make_uint4(0u, 0u, 0u, 0u);
+      *reinterpret_cast<uint4 *>(cr_at<D>(t, row(j), 16 * chunk())) = z;
+    }
+  }
+};
+
+__device__ __forceinline__ float cr_halves_sum(float v) {
+  float x, y;
+  xrow_pair32(v, x, y);
+  return x + y;
+}
+__device__ __forceinline__ float cr_halves_max(float v) {
+  float x, y;
+  xrow_pair32(v, x, y);
+  return fmaxf(x, y);
+}
+__device__ __forceinline__ cr_f32x16 cr_zero() {
+  cr_f32x16 z;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) z[i] = 0.0f;
+  return z;
+}
+// Row of value i of a product's column.
+__device__ __forceinline__ int cr_row(int i, int lane) { return 8 * (i >> 2) + 4 * (lane >> 5) + (i & 3); }
+
+// Columns of a wave: 32 CT of the block's 128 CT.
+template <int D, int CT> struct CrCols {
+  int64_t off[CT];  // rows' element offset (row, head) in q's layout: row number, head
+  int32_t row[CT], head[CT];
+  bool live[CT];
+  __device__ __forceinline__ CrCols(const CrossArgs &a, int c0, int n_cols, int h, int64_t lo) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      const int c = c0 + 32 * (CT * wave + ct) + (lane & 31);
+      live[ct] = c < n_cols;
+      const uint32_t cc = (uint32_t)min(c, n_cols - 1), r = cc / (uint32_t)a.group;
+      row[ct] = (int32_t)(lo + r);
+      head[ct] = h * a.group + (int32_t)(cc - r * (uint32_t)a.group);
+    }
+  }
+  // Their D channels as B operands (columns that are not there as zeros).
+  __device__ __forceinline__ void load(const CrIn &x, att_u32x4 (&f)[CT][D / 16]) const {
+    const int half = (threadIdx.x & 63) >> 5;
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      const uint16_t *p = x.p + row[ct] * x.row + head[ct] * x.head + 8 * half;
+#pragma unroll
+      for (int kc = 0; kc < D / 16; ++kc) {
+        const att_u32x4 w = *reinterpret_cast<const att_u32x4 *>(p + 16 * kc);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[ct][kc][i] = live[ct] ? w[i] : 0u;
+      }
+    }
+  }
+};
+
+// Rows in no sequence: zeros, where they are asked for (a block of its own for each tensor).
+__device__ __forceinline__ void cr_zero_rest(uint16_t *out, const int32_t *cu, int32_t n_seqs, int64_t n, int64_t width) {
+  const int64_t lo = max((int64_t)0, min((int64_t)cu[0], n)), hi = max(lo, min((int64_t)cu[n_seqs], n));
+  uint4 *p = reinterpret_cast<uint4 *>(out);
+  const int64_t w = width / 8;
+  for (int64_t i = threadIdx.x; i < lo * w; i += blockDim.x) p[i] = make_uint4(0u, 0u, 0u, 0u);
+  for (int64_t i = hi * w + threadIdx.x; i < n * w; i += blockDim.x) p[i] = make_uint4(0u, 0u, 0u, 0u);
+}
+
+// ------------------------------------------------------------------ forward
+
+template <class T, int D, int CT>
+__global__ void __launch_bounds__(CR_THREADS, D *CT > 128 ? 1 : 2) cross_forward_kernel(CrossArgs a) {
+  constexpr int KC = D / 16, DT = D / 32;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[2][2][CrLds<D>::BYTES];
+  if (blockIdx.x + 1 == gridDim.x) {
+    if (a.zero_rest) cr_zero_rest(a.out, a.cu_q, a.n_seqs, a.n_q, (int64_t)a.n_q_heads * D);
+    return;
+  }
+  const CrItem it = cr_item(a);
+  if (!it.any) return;
+  int32_t e = 0;
+  const CrSpan qs = cr_span(a.cu_q, it.b, a.n_q, a.max_q, e), ks = cr_span(a.cu_k, it.b, a.n_k, a.max_k, e);
+  if (e && a.err && threadIdx.x == 0) atomicOr(a.err, e);
+  const int n_cols = qs.n * a.group, c0 = it.tile * 32 * CT * CR_WAVES;
+  if (c0 >= n_cols) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int keys = cr_keys(a, it.b, ks.n), units = (keys + CR_TILE - 1) / CR_TILE;
+  const int t_begin = (int)((int64_t)units * it.split / a.n_split) * CR_TILE;
+  const int t_end = min(keys, (int)((int64_t)units * (it.split + 1) / a.n_split) * CR_TILE);
+  const CrCols<D, CT> cols(a, c0, n_cols, it.h, qs.lo);
+  const bool work = c0 + 32 * CT * wave < n_cols;  // uniform in the wave
+  att_u32x4 q[CT][KC];
+  cols.load(a.q, q);
+  cr_f32x16 o[CT][DT];
+  float m[CT], top[CT], l[CT];
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) o[ct][dt] = cr_zero();
+    m[ct] = top[ct] = CR_NONE;
+    l[ct] = 0.0f;
+  }
+  // the scores' factor as a positive number: a negative one turns q's signs, 0 makes q zero
+  const float scale = a.sm_scale * ATT_LOG2E, f = scale == 0.0f ? 1.0f : fabsf(scale);
+  if (scale <= 0.0f) {
+    const uint32_t flip = scale < 0.0f ? 0x80008000u : 0u, keep = scale < 0.0f ? 0xFFFFFFFFu : 0u;
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+      for (int kc = 0; kc < KC; ++kc)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) q[ct][kc][i] = (q[ct][kc][i] ^ flip) & keep;
+  }
+  const uint16_t *kp = a.k.p + ks.lo * a.k.row + it.h * a.k.head, *vp = a.v.p + ks.lo * a.v.row + it.h * a.v.head;
+  CrStage<D> sk, sv;
+  if (t_begin < t_end) {
+    const int n = min(CR_TILE, t_end - t_begin);
+    sk.load(kp + t_begin * a.k.row, a.k.row, n);
+    sv.load(vp + t_begin * a.v.row, a.v.row, n);
+    sk.store(lds[0][0], n);
+    sv.store(lds[0][1], n);
+  }
+  __syncthreads();
+  int buf = 0;
+  for (int t = t_begin; t < t_end; t += CR_TILE, buf ^= 1) {
+    const int next = t + CR_TILE, n_next = min(CR_TILE, t_end - next);
+    if (next < t_end) {
+      sk.load(kp + next * a.k.row, a.k.row, n_next);
+      sv.load(vp + next * a.v.row, a.v.row, n_next);
+    }
+    if (work) {
+      uint8_t *lk = lds[buf][0], *lv = lds[buf][1];
+      cr_f32x16 s[CT][2];
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt) {
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) s[ct][kt] = cr_zero();
+#pragma unroll
+        for (int kc = 0; kc < KC; ++kc) {
+          const att_u32x4 k = cr_rows<D>(lk, kt, kc, lane);
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct) s[ct][kt] = T::mfma(k, q[ct][kc], s[ct][kt]);
+        }
+      }
+      if (t + CR_TILE > t_end) {  // uniform
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+          for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              if (t + 32 * kt + cr_row(i, lane) >= t_end) s[ct][kt][i] = -INFINITY;
+      }
+      float mx[CT];
+      bool grew = false;
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
+        mx[ct] = s[ct][0][0];
+#pragma unroll
+        for (int i = 1; i < 32; ++i) mx[ct] = __builtin_elementwise_maximum(mx[ct], s[ct][i / 16][i % 16]);
+        grew |= mx[ct] > top[ct];
+      }
+      if (__builtin_amdgcn_ballot_w64(grew)) {
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) {
+          const float m_new = fmaxf(m[ct], cr_halves_max(mx[ct]) * f - T::BIAS);
+          const float alpha = __builtin_amdgcn_exp2f(m[ct] - m_new);
+          m[ct] = m_new;
+          top[ct] = (m_new + (CR_LAZY + T::BIAS)) / f;
+          l[ct] *= alpha;
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[ct][dt][i] *= alpha;
+        }
+      }
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt) {
+        att_u32x4 p[CT][2];
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) {
+          float x[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[ct][kt][i], f, -m[ct]));
+            l[ct] += x[i];
+          }
+          cr_operands<T>(x, p[ct]);
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt) {
+            const att_u32x4 v = cr_cols<D>(lv, 2 * kt + c, dt, lane);
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) o[ct][dt] = T::mfma(v, p[ct][c], o[ct][dt]);
+          }
+      }
+    }
+    if (next < t_end) {
+      sk.store(lds[buf ^ 1][0], n_next);
+      sv.store(lds[buf ^ 1][1], n_next);
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    if (!cols.live[ct]) continue;
+    const float sum = cr_halves_sum(l[ct]);
+    const int64_t at = (int64_t)cols.row[ct] * a.n_q_heads + cols.head[ct];
+    if (a.n_split == 1) {
+      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+      uint16_t *row = a.out + at * D + 4 * (lane >> 5);
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4)
+          *reinterpret_cast<uint2 *>(row + 32 * dt + 2 * i) =
+              sum == 0.0f ? make_uint2(0u, 0u)
+                          : make_uint2(T::pack(o[ct][dt][i] * inv, o[ct][dt][i + 1] * inv),
+                                       T::pack(o[ct][dt][i + 2] * inv, o[ct][dt][i + 3] * inv));
+      if (a.lse && lane < 32)
+        a.lse[(int64_t)cols.head[ct] * a.n_q + cols.row[ct]] = sum == 0.0f ? -INFINITY : m[ct] + __builtin_amdgcn_logf(sum);
+    } else {
+      float *pp = a.part + ((int64_t)it.split * a.n_q * a.n_q_heads + at) * (2 + D);
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int i = 0; i < 16; i += 2)
+          *reinterpret_cast<float2 *>(pp + 2 + 32 * dt + cr_row(i, lane)) = make_float2(o[ct][dt][i], o[ct][dt][i + 1]);
+      if (lane < 32) *reinterpret_cast<float2 *>(pp) = make_float2(m[ct], sum);
+    }
+  }
+}
+
+// The sequence of a packed row, or -1.
+__device__ __forceinline__ int32_t cr_seq_of(const int32_t *cu, int32_t n_seqs, int64_t row) {
+  int32_t lo = 0, hi = n_seqs - 1;
+  while (lo < hi) {
+    const int32_t mid = (lo + hi + 1) >> 1;
+    if (cu[mid] <= row) lo = mid;
+    else hi = mid - 1;
+  }
+  return row >= cu[lo] && row < cu[lo + 1] ? lo : -1;
+}
+
+// Rows whose keys were cut: D threads per (row, head).
+template <class T, int D> __global__ void __launch_bounds__(256) cross_merge_kernel(CrossArgs a) {
+  const int64_t at = (int64_t)blockIdx.x * (256 / D) + threadIdx.x / D, row = at / a.n_q_heads;
+  if (row >= a.n_q) return;
+  const int32_t b = cr_seq_of(a.cu_q, a.n_seqs, row);
+  if (b < 0 || row - a.cu_q[b] >= a.max_q) return;
+  const int d = threadIdx.x % D;
+  const int64_t step = a.n_q * a.n_q_heads * (2 + D);
+  const float *pp = a.part + at * (2 + D);
+  float M = CR_NONE, L = 0.0f, A = 0.0f;
+  for (int s0 = 0; s0 < a.n_split; s0 += 8) {
+    float2 ml[8];
+    float v[8];
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+      const float *p = pp + min(s0 + s, a.n_split - 1) * step;
+      ml[s] = *reinterpret_cast<const float2 *>(p);
+      v[s] = p[2 + d];
+    }
+    float Mn = M;
+#pragma unroll
+    for (int s = 0; s < 8; ++s) Mn = fmaxf(Mn, ml[s].x);
+    const float alpha = __builtin_amdgcn_exp2f(M - Mn);
+    L *= alpha;
+    A *= alpha;
+    M = Mn;
+#pragma unroll
+    for (int s = 0; s < 8; ++s)
+      if (s0 + s < a.n_split) {
+        const float w = __builtin_amdgcn_exp2f(ml[s].x - M);
+        L += w * ml[s].y;
+        A += w * v[s];
+      }
+  }
+  a.out[at * D + d] = (uint16_t)(T::pack(L == 0.0f ? 0.0f : A / L, 0.0f) & 0xFFFFu);
+  if (a.lse && d == 0)
+    a.lse[(at - row * a.n_q_heads) * a.n_q + row] = L == 0.0f ? -INFINITY : M + __builtin_amdgcn_logf(L);
+}
+
+// ------------------------------------------------------------------ gradients
+
+// dq, and on the way D_r for the other kernel.
+template <class T, int D, int CT>
+__global__ void __launch_bounds__(CR_THREADS, D *CT > 64 ? 1 : 2) cross_dq_kernel(CrossArgs a) {
+  constexpr int KC = D / 16, DT = D / 32;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[2][2][CrLds<D>::BYTES];
+  if (blockIdx.x + 1 == gridDim.x) {
+    cr_zero_rest(a.out, a.cu_q, a.n_seqs, a.n_q, (int64_t)a.n_q_heads * D);
+    return;
+  }
+  const CrItem it = cr_item(a);
+  if (!it.any) return;
+  int32_t e = 0;
+  const CrSpan qs = cr_span(a.cu_q, it.b, a.n_q, a.max_q, e), ks = cr_span(a.cu_k, it.b, a.n_k, a.max_k, e);
+  if (e && a.err && threadIdx.x == 0) atomicOr(a.err, e);
+  const int n_cols = qs.n * a.group, c0 = it.tile * 32 * CT * CR_WAVES;
+  if (c0 >= n_cols) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int keys = cr_keys(a, it.b, ks.n), units = (keys + CR_TILE - 1) / CR_TILE;
+  const int t_begin = (int)((int64_t)units * it.split / a.n_split) * CR_TILE;
+  const int t_end = min(keys, (int)((int64_t)units * (it.split + 1) / a.n_split) * CR_TILE);
+  const CrCols<D, CT> cols(a, c0, n_cols, it.h, qs.lo);
+  const bool work = c0 + 32 * CT * wave < n_cols;
+  att_u32x4 q[CT][KC], g[CT][KC];
+  cols.load(a.q, q);
+  cols.load(a.g, g);
+  float lse[CT], delta[CT];
+  cr_f32x16 dq[CT][DT];
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    const uint16_t *p = a.o.p + cols.row[ct] * a.o.row + cols.head[ct] * a.o.head + 8 * (lane >> 5);
+    float sum = 0.0f;
+#pragma unroll
+    for (int kc = 0; kc < KC; ++kc) {
+      const att_u32x4 w = *reinterpret_cast<const att_u32x4 *>(p + 16 * kc);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        sum = __builtin_fmaf(T::lo(w[i]), T::lo(g[ct][kc][i]), sum);
+        sum = __builtin_fmaf(T::hi(w[i]), T::hi(g[ct][kc][i]), sum);
+      }
+    }
+    delta[ct] = cr_halves_sum(sum);
+    const int64_t at = (int64_t)cols.head[ct] * a.n_q + cols.row[ct];
+    lse[ct] = a.lse[at];
+    if (it.split == 0 && cols.live[ct] && lane < 32) a.delta[at] = delta[ct];
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) dq[ct][dt] = cr_zero();
+  }
+  const float scale = a.sm_scale * ATT_LOG2E;
+  const uint16_t *kp = a.k.p + ks.lo * a.k.row + it.h * a.k.head, *vp = a.v.p + ks.lo * a.v.row + it.h * a.v.head;
+  CrStage<D> sk, sv;
+  if (t_begin < t_end) {
+    const int n = min(CR_TILE, t_end - t_begin);
+    sk.load(kp + t_begin * a.k.row, a.k.row, n);
+    sv.load(vp + t_begin * a.v.row, a.v.row, n);
+    sk.store(lds[0][0], n);
+    sv.store(lds[0][1], n);
+  }
+  __syncthreads();
+  int buf = 0;
+  for (int t = t_begin; t < t_end; t += CR_TILE, buf ^= 1) {
+    const int next = t + CR_TILE, n_next = min(CR_TILE, t_end - next);
+    if (next < t_end) {
+      sk.load(kp + next * a.k.row, a.k.row, n_next);
+      sv.load(vp + next * a.v.row, a.v.row, n_next);
+    }
+    if (work) {
+      uint8_t *lk = lds[buf][0], *lv = lds[buf][1];
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt) {
+        cr_f32x16 s[CT], dp[CT];
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) s[ct] = dp[ct] = cr_zero();
+#pragma unroll
+        for (int kc = 0; kc < KC; ++kc) {
+          const att_u32x4 k = cr_rows<D>(lk, kt, kc, lane), v = cr_rows<D>(lv, kt, kc, lane);
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct) {
+            s[ct] = T::mfma(k, q[ct][kc], s[ct]);
+            dp[ct] = T::mfma(v, g[ct][kc], dp[ct]);
+          }
+        }
+        att_u32x4 ds[CT][2];
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) {
+          float x[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[ct][i], scale, -lse[ct])) * (dp[ct][i] - delta[ct]);
+          if (t + CR_TILE > t_end) {  // uniform
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              if (t + 32 * kt + cr_row(i, lane) >= t_end) x[i] = 0.0f;
+          }
+          cr_operands<T>(x, ds[ct]);
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt) {
+            const att_u32x4 k = cr_cols<D>(lk, 2 * kt + c, dt, lane);
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) dq[ct][dt] = T::mfma(k, ds[ct][c], dq[ct][dt]);
+          }
+      }
+    }
+    if (next < t_end) {
+      sk.store(lds[buf ^ 1][0], n_next);
+      sv.store(lds[buf ^ 1][1], n_next);
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    if (!cols.live[ct]) continue;
+    const int64_t at = ((int64_t)cols.row[ct] * a.n_q_heads + cols.head[ct]) * D + 4 * (lane >> 5);
+    if (a.n_split == 1) {
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4)
+          *reinterpret_cast<uint2 *>(a.out + at + 32 * dt + 2 * i) =
+              make_uint2(T::pack(dq[ct][dt][i] * a.sm_scale, dq[ct][dt][i + 1] * a.sm_scale),
+                         T::pack(dq[ct][dt][i + 2] * a.sm_scale, dq[ct][dt][i + 3] * a.sm_scale));
+    } else {
+      float *pp = a.part + (int64_t)it.split * a.n_q * a.n_q_heads * D + at;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4)
+          *reinterpret_cast<float4 *>(pp + 32 * dt + 2 * i) =
+              make_float4(dq[ct][dt][i] * a.sm_scale, dq[ct][dt][i + 1] * a.sm_scale, dq[ct][dt][i + 2] * a.sm_scale,
+                          dq[ct][dt][i + 3] * a.sm_scale);
+    }
+  }
+}
+
+// dk and dv of 128 KT keys, a wave 32 KT of them.
+template <class T, int D, int KT>
+__global__ void __launch_bounds__(CR_THREADS, D *KT > 64 ? 1 : 2) cross_dkv_kernel(CrossArgs a) {
+  constexpr int KC = D / 16, DT = D / 32;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[2][2][CrLds<D>::BYTES];
+  __shared__ __attribute__((aligned(16))) float sm_lse[2][CR_TILE], sm_delta[2][CR_TILE];
+  if (blockIdx.x + 1 == gridDim.x) {
+    cr_zero_rest(a.dk, a.cu_k, a.n_seqs, a.n_k, (int64_t)a.n_kv_heads * D);
+    cr_zero_rest(a.dv, a.cu_k, a.n_seqs, a.n_k, (int64_t)a.n_kv_heads * D);
+    return;
+  }
+  const CrItem it = cr_item(a);
+  if (!it.any) return;
+  int32_t e = 0;  // (reported with dq)
+  const CrSpan qs = cr_span(a.cu_q, it.b, a.n_q, a.max_q, e), ks = cr_span(a.cu_k, it.b, a.n_k, a.max_k, e);
+  const int key0 = it.tile * 32 * KT * CR_WAVES;
+  if (key0 >= ks.n) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int keys = cr_keys(a, it.b, ks.n);
+  const int n_cols = key0 < keys ? qs.n * a.group : 0, units = (n_cols + CR_TILE - 1) / CR_TILE;
+  const int t_begin = (int)((int64_t)units * it.split / a.n_split) * CR_TILE;
+  const int t_end = min(n_cols, (int)((int64_t)units * (it.split + 1) / a.n_split) * CR_TILE);
+  const int wk = key0 + 32 * KT * wave;  // the wave's first key
+  const bool work = wk < keys;
+  att_u32x4 k[KT][KC], v[KT][KC];
+  cr_f32x16 dk[KT][DT], dv[KT][DT];
+#pragma unroll
+  for (int kt = 0; kt < KT; ++kt) {
+    const int key = wk + 32 * kt + (lane & 31);
+    const int64_t row = ks.lo + max(0, min(key, keys - 1));
+    const uint16_t *kp = a.k.p + row * a.k.row + it.h * a.k.head + 8 * (lane >> 5);
+    const uint16_t *vp = a.v.p + row * a.v.row + it.h * a.v.head + 8 * (lane >> 5);
+#pragma unroll
+    for (int kc = 0; kc < KC; ++kc) {
+      k[kt][kc] = *reinterpret_cast<const att_u32x4 *>(kp + 16 * kc);
+      v[kt][kc] = *reinterpret_cast<const att_u32x4 *>(vp + 16 * kc);
+    }
+    // keys that are not there: zeros (what memory holds in their place may be NaN)
+#pragma unroll
+    for (int kc = 0; kc < KC; ++kc)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        k[kt][kc][i] = key < keys ? k[kt][kc][i] : 0u;
+        v[kt][kc][i] = key < keys ? v[kt][kc][i] : 0u;
+      }
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) dk[kt][dt] = dv[kt][dt] = cr_zero();
+  }
+  const float scale = a.sm_scale * ATT_LOG2E;
+  const uint16_t *qp = a.q.p + qs.lo * a.q.row + (int64_t)it.h * a.group * a.q.head;
+  const uint16_t *gp = a.g.p + qs.lo * a.g.row + (int64_t)it.h * a.group * a.g.head;
+  CrStage<D> sq, sg;
+  float my_lse = 0.0f, my_delta = 0.0f;
+  auto load = [&](int c0, int n) {
+    sq.load_pairs(qp, a.q.row, a.q.head, c0, n, a.group);
+    sg.load_pairs(gp, a.g.row, a.g.head, c0, n, a.group);
+    if (threadIdx.x < CR_TILE) {
+      const uint32_t c = (uint32_t)(c0 + min((int)threadIdx.x, n - 1)), r = c / (uint32_t)a.group;
+      const int64_t at = (int64_t)(it.h * a.group + (int32_t)(c - r * (uint32_t)a.group)) * a.n_q + qs.lo + r;
+      my_lse = a.lse[at];
+      my_delta = a.delta[at];
+    }
+  };
+  auto store = [&](int buf, int n) {
+    sq.store(lds[buf][0], n);
+    sg.store(lds[buf][1], n);
+    if (threadIdx.x < CR_TILE) {  // (a row that is not there: weights of 0)
+      sm_lse[buf][threadIdx.x] = (int)threadIdx.x < n ? my_lse - T::BIAS : INFINITY;
+      sm_delta[buf][threadIdx.x] = (int)threadIdx.x < n ? my_delta : 0.0f;
+    }
+  };
+  if (t_begin < t_end) {
+    const int n = min(CR_TILE, t_end - t_begin);
+    load(t_begin, n);
+    store(0, n);
+  }
+  __syncthreads();
+  const float unbias = __builtin_amdgcn_exp2f(-T::BIAS);
+  int buf = 0;
+  for (int t = t_begin; t < t_end; t += CR_TILE, buf ^= 1) {
+    const int next = t + CR_TILE, n_next = min(CR_TILE, t_end - next);
+    if (next < t_end) load(next, n_next);
+    if (work) {
+      uint8_t *lq = lds[buf][0], *lg = lds[buf][1];
+#pragma unroll
+      for (int rt = 0; rt < 2; ++rt) {
+        cr_f32x16 s[KT], dp[KT];
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt) s[kt] = dp[kt] = cr_zero();
+#pragma unroll
+        for (int kc = 0; kc < KC; ++kc) {
+          const att_u32x4 q = cr_rows<D>(lq, rt, kc, lane), g = cr_rows<D>(lg, rt, kc, lane);
+#pragma unroll
+          for (int kt = 0; kt < KT; ++kt) {
+            s[kt] = T::mfma(q, k[kt][kc], s[kt]);
+            dp[kt] = T::mfma(g, v[kt][kc], dp[kt]);
+          }
+        }
+        att_u32x4 p[KT][2], ds[KT][2];
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt) {
+          const bool live = wk + 32 * kt + (lane & 31) < keys;
+          float x[16], y[16];
+#pragma unroll
+          for (int i4 = 0; i4 < 4; ++i4) {
+            const int row = 32 * rt + 8 * i4 + 4 * (lane >> 5);
+            const att_f32x4 lse = *reinterpret_cast<const att_f32x4 *>(&sm_lse[buf][row]);
+            const att_f32x4 delta = *reinterpret_cast<const att_f32x4 *>(&sm_delta[buf][row]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int i = 4 * i4 + j;
+              const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][i], scale, -lse[j]));
+              x[i] = live ? w : 0.0f;
+              y[i] = x[i] * unbias * (dp[kt][i] - delta[j]);
+            }
+          }
+          cr_operands<T>(x, p[kt]);
+          cr_operands<T>(y, ds[kt]);
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt) {
+            const att_u32x4 g = cr_cols<D>(lg, 2 * rt + c, dt, lane), q = cr_cols<D>(lq, 2 * rt + c, dt, lane);
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt) {
+              dv[kt][dt] = T::mfma(g, p[kt][c], dv[kt][dt]);
+              dk[kt][dt] = T::mfma(q, ds[kt][c], dk[kt][dt]);
+            }
+          }
+      }
+    }
+    if (next < t_end) store(buf ^ 1, n_next);
+    __syncthreads();
+  }
+#pragma unroll
+  for (int kt = 0; kt < KT; ++kt) {
+    const int key = wk + 32 * kt + (lane & 31);
+    if (key >= ks.n) continue;
+    const int64_t at = ((ks.lo + key) * a.n_kv_heads + it.h) * D + 4 * (lane >> 5);
+    const int64_t all = a.n_k * a.n_kv_heads * D;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int i = 0; i < 16; i += 4) {
+        float x[4], y[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          x[j] = dk[kt][dt][i + j] * a.sm_scale;
+          y[j] = dv[kt][dt][i + j] * unbias;
+        }
+        const int64_t w = at + 32 * dt + 2 * i;
+        if (a.n_split == 1) {
+          *reinterpret_cast<uint2 *>(a.dk + w) = make_uint2(T::pack(x[0], x[1]), T::pack(x[2], x[3]));
+          *reinterpret_cast<uint2 *>(a.dv + w) = make_uint2(T::pack(y[0], y[1]), T::pack(y[2], y[3]));
+        } else {
+          float *pp = a.part + 2 * (int64_t)it.split * all + w;
+          *reinterpret_cast<float4 *>(pp) = make_float4(x[0], x[1], x[2], x[3]);
+          *reinterpret_cast<float4 *>(pp + all) = make_float4(y[0], y[1], y[2], y[3]);
+        }
+      }
+  }
+}
+
+// Sums of the parts of a gradient, in order: [n_split] parts `step` floats apart, 8 values per thread.
+template <class T>
+__global__ void __launch_bounds__(256) cross_sum_kernel(const float *part, int64_t step, int32_t n_split, uint16_t *out,
+                                                        const int32_t *cu, int32_t n_seqs, int64_t n, int64_t width,
+                                                        int32_t most) {
+  const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
+  if (at >= n * width) return;
+  const int64_t row = at / width;
+  const int32_t b = cr_seq_of(cu, n_seqs, row);
+  if (b < 0 || row - cu[b] >= most) return;  // zeros already, or not computed
+  float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  for (int s = 0; s < n_split; ++s) {
+    const att_f32x4 *p = reinterpret_cast<const att_f32x4 *>(part + s * step + at);
+    const att_f32x4 u = p[0], v = p[1];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[i] += u[i];
+      x[4 + i] += v[i];
+    }
+  }
+  *reinterpret_cast<uint4 *>(out + at) =
+      make_uint4(T::pack(x[0], x[1]), T::pack(x[2], x[3]), T::pack(x[4], x[5]), T::pack(x[6], x[7]));
+}
+
+}  // namespace zx
+
+using namespace zx;
+
+// How a kernel is cut: column (or key) tiles per wave, tiles of a pair of sequence and KV head,
+// parts of a tile where the tiles do not fill the chip.
+struct CrossPlan {
+  int ct;
+  int64_t n_tile, n_split;
+};
+static CrossPlan cr_plan(int64_t pairs, int64_t columns, int64_t length, int ct, int64_t per_cu, int64_t units_least) {
+  CrossPlan p;
+  p.ct = ct;
+  p.n_tile = std::max<int64_t>(1, ceil_div(columns, 32 * ct * CR_WAVES));
+  const int64_t blocks = pairs * p.n_tile, slots = per_cu * num_cus();
+  const int64_t units = ceil_div(length, CR_TILE);
+  p.n_split = std::max<int64_t>(1, std::min<int64_t>({slots / std::max<int64_t>(1, blocks), units / units_least, 64}));
+  return p;
+}
+static CrossPlan cr_forward_plan(int32_t n_seqs, int32_t n_kv_heads, int32_t group, int32_t D, int32_t max_q, int32_t max_k) {
+  const int64_t columns = (int64_t)max_q * group;
+  const int ct = columns >= 512 ? 2 : 1;
+  return cr_plan((int64_t)n_seqs * n_kv_heads, columns, max_k, ct, D * ct > 128 ? 1 : D == 64 ? 4 : 2, 2);
+}
+static CrossPlan cr_dq_plan(int32_t n_seqs, int32_t n_kv_heads, int32_t group, int32_t D, int32_t max_q, int32_t max_k) {
+  const int64_t columns = (int64_t)max_q * group;
+  const int ct = columns >= 512 ? 2 : 1;
+  return cr_plan((int64_t)n_seqs * n_kv_heads, columns, max_k, ct, D * ct > 64 ? 1 : 2, 4);
+}
+static CrossPlan cr_dkv_plan(int32_t n_seqs, int32_t n_kv_heads, int32_t group, int32_t D, int32_t max_q, int32_t max_k) {
+  const int kt = D == 64 && max_k >= 512 ? 2 : 1;
+  return cr_plan((int64_t)n_seqs * n_kv_heads, max_k, (int64_t)max_q * group, kt, D * kt > 64 ? 1 : 2, 4);
+}
+static bool cr_dims_ok(int64_t n_q, int64_t n_k, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim, int32_t n_seqs,
+                       int32_t max_q, int32_t max_k) {
+  return n_q >= 0 && n_k >= 0 && n_q_heads > 0 && n_kv_heads > 0 && n_q_heads % n_kv_heads == 0 &&
+         (head_dim == 64 || head_dim == 128) && n_seqs > 0 && max_q >= 0 && max_k >= 0;
+}
+
+static size_t cr_forward_bytes(const CrossPlan &p, int64_t n_q, int32_t n_q_heads, int32_t D) {
+  return p.n_split > 1 ? (size_t)(p.n_split * n_q * n_q_heads * (2 + D)) * sizeof(float) : 0;
+}
+extern "C" size_t zx_cross_attention_workspace_bytes(int64_t n_q, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim,
+                                                     int32_t n_seqs, int32_t max_q_per_seq, int32_t max_k_per_seq) {
+  if (!cr_dims_ok(n_q, 0, n_q_heads, n_kv_heads, head_dim, n_seqs, max_q_per_seq, max_k_per_seq)) return 0;
+  return cr_forward_bytes(cr_forward_plan(n_seqs, n_kv_heads, n_q_heads / n_kv_heads, head_dim,
+                                          (int32_t)std::min<int64_t>(max_q_per_seq, n_q), max_k_per_seq),
+                          n_q, n_q_heads, head_dim);
+}
+
+struct CrossGradBytes {
+  size_t delta, part;
+};
+static CrossGradBytes cr_grad_bytes(const CrossPlan &dq, const CrossPlan &dkv, int64_t n_q, int64_t n_k, int32_t n_q_heads,
+                                    int32_t n_kv_heads, int32_t D) {
+  const size_t a = dq.n_split > 1 ? (size_t)(dq.n_split * n_q * n_q_heads * D) * sizeof(float) : 0;
+  const size_t b = dkv.n_split > 1 ? (size_t)(2 * dkv.n_split * n_k * n_kv_heads * D) * sizeof(float) : 0;
+  return CrossGradBytes{align256((size_t)(n_q * n_q_heads) * sizeof(float)), std::max(a, b)};
+}
+extern "C" size_t zx_cross_attention_backward_workspace_bytes(int64_t n_q, int64_t n_k, int32_t n_q_heads,
+                                                              int32_t n_kv_heads, int32_t head_dim, int32_t n_seqs,
+                                                              int32_t max_q_per_seq, int32_t max_k_per_seq) {
+  if (!cr_dims_ok(n_q, n_k, n_q_heads, n_kv_heads, head_dim, n_seqs, max_q_per_seq, max_k_per_seq)) return 0;
+  const int32_t group = n_q_heads / n_kv_heads, mq = (int32_t)std::min<int64_t>(max_q_per_seq, n_q);
+  const int32_t mk = (int32_t)std::min<int64_t>(max_k_per_seq, n_k);
+  const CrossGradBytes b = cr_grad_bytes(cr_dq_plan(n_seqs, n_kv_heads, group, head_dim, mq, mk),
+                                         cr_dkv_plan(n_seqs, n_kv_heads, group, head_dim, mq, mk), n_q, n_k, n_q_heads,
+                                         n_kv_heads, head_dim);
+  return b.delta + b.part;
+}
+
+static int cr_check(const char *what, int dtype, const CrossArgs &a, int32_t head_dim) {
+  ZX_REQUIRE(dtype == ZX_BF16 || dtype == ZX_F16, "%s: dtype must be bf16 or f16", what);
+  ZX_REQUIRE(a.n_q >= 0 && a.n_k >= 0 && a.n_q_heads > 0 && a.n_kv_heads > 0 && a.n_seqs > 0 && a.max_q >= 0 && a.max_k >= 0,
+             "%s: sizes must be positive", what);
+  ZX_REQUIRE(a.n_q_heads % a.n_kv_heads == 0, "%s: n_q_heads must be a multiple of n_kv_heads", what);
+  if (head_dim != 64 && head_dim != 128)
+    return fail(ZX_ERR_UNSUPPORTED, "%s: head_dim %d not in {64, 128}", what, head_dim);
+  if (a.n_q >= (1LL << 31) || a.n_k >= (1LL << 31) || a.n_q * a.n_q_heads >= (1LL << 31) || a.n_k * a.n_kv_heads >= (1LL << 31))
+    return fail(ZX_ERR_UNSUPPORTED, "%s: too many rows", what);
+  return ZX_OK;
+}
+// Strided rows: channels contiguous, every head's row 16-byte aligned.
+static int cr_check_rows(const char *what, const char *name, const CrIn &x) {
+  ZX_REQUIRE(x.p, "%s: null pointer", what);
+  ZX_REQUIRE(aligned16(x.p) && x.row % 8 == 0 && x.head % 8 == 0 && x.row >= 0 && x.head >= 0,
+             "%s: every row of a head of %s must be 16-byte aligned, with strides that are not negative", what, name);
+  return ZX_OK;
+}
+
+template <class T, int D> static int cr_forward(CrossArgs a, const CrossPlan &p, hipStream_t st) {
+  const unsigned grid = cr_grid(a) + 1;
+  if (p.ct == 2) cross_forward_kernel<T, D, 2><<<grid, CR_THREADS, 0, st>>>(a);
+  else cross_forward_kernel<T, D, 1><<<grid, CR_THREADS, 0, st>>>(a);
+  const int rc = check_launch("cross_forward");
+  if (rc || a.n_split == 1) return rc;
+  cross_merge_kernel<T, D><<<(unsigned)ceil_div(a.n_q * a.n_q_heads, 256 / D), 256, 0, st>>>(a);
+  return check_launch("cross_merge");
+}
+
+extern "C" int zx_cross_attention(int dtype, const void *q, int64_t n_q, int64_t q_row, int64_t q_head, int32_t n_q_heads,
+                                  const void *k, int64_t k_row, int64_t k_head, const void *v, int64_t v_row, int64_t v_head,
+                                  int64_t n_k, int32_t n_kv_heads, int32_t head_dim, const int32_t *cu_q,
+                                  const int32_t *cu_k, const int32_t *k_lens, int32_t n_seqs, int32_t max_q_per_seq,
+                                  int32_t max_k_per_seq, float sm_scale, int32_t flags, void *out, float *lse2, int32_t *err,
+                                  void *workspace, size_t workspace_bytes, zx_stream_t stream) {
+  clear_error();
+  ZX_REQUIRE(!(flags & ~ZX_CROSS_ZERO_REST), "cross_attention: unknown flag bits 0x%x", (unsigned)flags);
+  CrossArgs a = {};
+  a.q = {static_cast<const uint16_t *>(q), q_row, q_head};
+  a.k = {static_cast<const uint16_t *>(k), k_row, k_head};
+  a.v = {static_cast<const uint16_t *>(v), v_row, v_head};
+  a.cu_q = cu_q;
+  a.cu_k = cu_k;
+  a.k_lens = k_lens;
+  a.out = static_cast<uint16_t *>(out);
+  a.lse = lse2;
+  a.part = static_cast<float *>(workspace);
+  a.err = err;
+  a.n_q = n_q;
+  a.n_k = n_k;
+  a.n_q_heads = n_q_heads;
+  a.n_kv_heads = n_kv_heads;
+  a.n_seqs = n_seqs;
+  a.max_q = max_q_per_seq;
+  a.max_k = max_k_per_seq;
+  a.zero_rest = flags & ZX_CROSS_ZERO_REST ? 1 : 0;
+  a.sm_scale = sm_scale;
+  int rc = cr_check("cross_attention", dtype, a, head_dim);
+  if (rc) return rc;
+  if (n_q == 0) return ZX_OK;
+  a.max_q = (int32_t)std::min<int64_t>(max_q_per_seq, n_q);
+  a.group = n_q_heads / n_kv_heads;
+  ZX_REQUIRE(cu_q && cu_k && out, "cross_attention: null pointer");
+  if ((rc = cr_check_rows("cross_attention", "q", a.q))) return rc;
+  if (n_k && ((rc = cr_check_rows("cross_attention", "k", a.k)) || (rc = cr_check_rows("cross_attention", "v", a.v))))
+    return rc;
+  ZX_REQUIRE(aligned16(out) && aligned16(workspace), "cross_attention: out and workspace must be 16-byte aligned");
+  const CrossPlan p = cr_forward_plan(n_seqs, n_kv_heads, a.group, head_dim, a.max_q, max_k_per_seq);
+  if (workspace_bytes < cr_forward_bytes(p, n_q, n_q_heads, head_dim) || (!workspace && p.n_split > 1))
+    return fail(ZX_ERR_WORKSPACE, "cross_attention: workspace %zu < %zu bytes", workspace_bytes,
+                cr_forward_bytes(p, n_q, n_q_heads, head_dim));
+  a.n_tile = (int32_t)p.n_tile;
+  a.n_split = (int32_t)p.n_split;
+  if (8 * ceil_div((int64_t)n_seqs * n_kv_heads, 8) * p.n_tile * p.n_split >= (1LL << 31) - 1)
+    return fail(ZX_ERR_UNSUPPORTED, "cross_attention: too many sequences");
+  const hipStream_t st = as_stream(stream);
+  if (dtype == ZX_BF16) return head_dim == 64 ? cr_forward<CrBf16, 64>(a, p, st) : cr_forward<CrBf16, 128>(a, p, st);
+  return head_dim == 64 ? cr_forward<CrF16, 64>(a, p, st) : cr_forward<CrF16, 128>(a, p, st);
+}
+
+template <class T, int D>
+static int cr_backward(CrossArgs a, const CrossPlan &pq, const CrossPlan &pk, uint16_t *dq, hipStream_t st) {
+  int rc;
+  a.out = dq;
+  a.n_tile = (int32_t)pq.n_tile;
+  a.n_split = (int32_t)pq.n_split;
+  if (pq.ct == 2) cross_dq_kernel<T, D, 2><<<cr_grid(a) + 1, CR_THREADS, 0, st>>>(a);
+  else cross_dq_kernel<T, D, 1><<<cr_grid(a) + 1, CR_THREADS, 0, st>>>(a);
+  if ((rc = check_launch("cross_dq"))) return rc;
+  const int64_t wq = (int64_t)a.n_q_heads * D, wk = (int64_t)a.n_kv_heads * D;
+  if (pq.n_split > 1 && a.n_q) {
+    cross_sum_kernel<T><<<(unsigned)ceil_div(a.n_q * wq, 8 * 256), 256, 0, st>>>(a.part, a.n_q * wq, a.n_split, dq, a.cu_q,
+                                                                                a.n_seqs, a.n_q, wq, a.max_q);
+    if ((rc = check_launch("cross_sum"))) return rc;
+  }
+  if (a.n_k == 0) return ZX_OK;
+  a.n_tile = (int32_t)pk.n_tile;
+  a.n_split = (int32_t)pk.n_split;
+  if (pk.ct == 2) {
+    if constexpr (D == 64) cross_dkv_kernel<T, D, 2><<<cr_grid(a) + 1, CR_THREADS, 0, st>>>(a);
+  } else {
+    cross_dkv_kernel<T, D, 1><<<cr_grid(a) + 1, CR_THREADS, 0, st>>>(a);
+  }
+  if ((rc = check_launch("cross_dkv")) || pk.n_split == 1) return rc;
+  for (int i = 0; i < 2; ++i) {
+    cross_sum_kernel<T><<<(unsigned)ceil_div(a.n_k * wk, 8 * 256), 256, 0, st>>>(
+        a.part + i * a.n_k * wk, 2 * a.n_k * wk, a.n_split, i ? a.dv : a.dk, a.cu_k, a.n_seqs, a.n_k, wk, a.max_k);
+    if ((rc = check_launch("cross_sum"))) return rc;
+  }
+  return ZX_OK;
+}
+
+extern "C" int zx_cross_attention_backward(
+    int dtype, const void *grad, int64_t g_row, int64_t g_head, const void *q, int64_t n_q, int64_t q_row, int64_t q_head,
+    int32_t n_q_heads, const void *k, int64_t k_row, int64_t k_head, const void *v, int64_t v_row, int64_t v_head, int64_t n_k,
+    int32_t n_kv_heads, int32_t head_dim, const void *out, const float *lse2, const int32_t *cu_q, const int32_t *cu_k,
+    const int32_t *k_lens, int32_t n_seqs, int32_t max_q_per_seq, int32_t max_k_per_seq, float sm_scale, void *dq, void *dk,
+    void *dv, int32_t *err, void *workspace, size_t workspace_bytes, zx_stream_t stream) {
+  clear_error();
+  CrossArgs a = {};
+  a.q = {static_cast<const uint16_t *>(q), q_row, q_head};
+  a.k = {static_cast<const uint16_t *>(k), k_row, k_head};
+  a.v = {static_cast<const uint16_t *>(v), v_row, v_head};
+  a.g = {static_cast<const uint16_t *>(grad), g_row, g_head};
+  a.o = {static_cast<const uint16_t *>(out), (int64_t)n_q_heads * head_dim, head_dim};
+  a.cu_q = cu_q;
+  a.cu_k = cu_k;
+  a.k_lens = k_lens;
+  a.dk = static_cast<uint16_t *>(dk);
+  a.dv = static_cast<uint16_t *>(dv);
+  a.lse = const_cast<float *>(lse2);
+  a.err = err;
+  a.n_q = n_q;
+  a.n_k = n_k;
+  a.n_q_heads = n_q_heads;
+  a.n_kv_heads = n_kv_heads;
+  a.n_seqs = n_seqs;
+  a.max_q = max_q_per_seq;
+  a.max_k = max_k_per_seq;
+  a.zero_rest = 1;
+  a.sm_scale = sm_scale;
+  int rc = cr_check("cross_attention_backward", dtype, a, head_dim);
+  if (rc) return rc;
+  a.max_q = (int32_t)std::min<int64_t>(max_q_per_seq, n_q);
+  a.max_k = (int32_t)std::min<int64_t>(max_k_per_seq, n_k);
+  a.group = n_q_heads / n_kv_heads;
+  if (n_q == 0 && n_k == 0) return ZX_OK;
+  ZX_REQUIRE(cu_q && cu_k, "cross_attention_backward: null pointer");
+  if (n_q && ((rc = cr_check_rows("cross_attention_backward", "q", a.q)) ||
+              (rc = cr_check_rows("cross_attention_backward", "grad", a.g)) ||
+              (rc = cr_check_rows("cross_attention_backward", "out", a.o))))
+    return rc;
+  if (n_k && ((rc = cr_check_rows("cross_attention_backward", "k", a.k)) ||
+              (rc = cr_check_rows("cross_attention_backward", "v", a.v))))
+    return rc;
+  ZX_REQUIRE((!n_q || (dq && lse2)) && (!n_k || (dk && dv)), "cross_attention_backward: null pointer");
+  ZX_REQUIRE(aligned16(dq) && aligned16(dk) && aligned16(dv) && aligned16(workspace),
+             "cross_attention_backward: dq, dk, dv and workspace must be 16-byte aligned");
+  const CrossPlan pq = cr_dq_plan(n_seqs, n_kv_heads, a.group, head_dim, a.max_q, a.max_k);
+  const CrossPlan pk = cr_dkv_plan(n_seqs, n_kv_heads, a.group, head_dim, a.max_q, a.max_k);
+  const CrossGradBytes bytes = cr_grad_bytes(pq, pk, n_q, n_k, n_q_heads, n_kv_heads, head_dim);
+  if (workspace_bytes < bytes.delta + bytes.part || (!workspace && bytes.delta + bytes.part))
+    return fail(ZX_ERR_WORKSPACE, "cross_attention_backward: workspace %zu < %zu bytes", workspace_bytes,
+                bytes.delta + bytes.part);
+  a.delta = static_cast<float *>(workspace);
+  a.part = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + bytes.delta);
+  const int64_t pairs8 = 8 * ceil_div((int64_t)n_seqs * n_kv_heads, 8);
+  if (pairs8 * std::max(pq.n_tile * pq.n_split, pk.n_tile * pk.n_split) >= (1LL << 31) - 1)
+    return fail(ZX_ERR_UNSUPPORTED, "cross_attention_backward: too many sequences");
+  const hipStream_t st = as_stream(stream);
+  uint16_t *d = static_cast<uint16_t *>(dq);
+  if (dtype == ZX_BF16)
+    return head_dim == 64 ? cr_backward<CrBf16, 64>(a, pq, pk, d, st) : cr_backward<CrBf16, 128>(a, pq, pk, d, st);
+  return head_dim == 64 ? cr_backward<CrF16, 64>(a, pq, pk, d, st) : cr_backward<CrF16, 128>(a, pq, pk, d, st);
+}

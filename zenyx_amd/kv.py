@@ -1325,3 +1325,117 @@ def paged_attention4_shared(q: torch.Tensor, pool_layer: torch.Tensor, block_tab
     carried to 2^-17: error within one bf16 ulp + 2^-15 max|V|."""
     return _attention_shared("paged_attention4_shared", q, pool_layer, None, block_tables, seq_lens, cu_group,
                              shared_lens, cu_q, max_q_per_seq, causal, sm_scale, out, check, err)
+
+
+# ------------------------------------------------------------------ cross attention
+
+def _cross_args(q, k, v, cu_q, cu_k, k_lens, max_q_per_seq, max_k_per_seq, err):
+    """Checks, and (device index, sequences, bounds of a sequence's rows and keys)."""
+    if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
+        raise ValueError("q must be [n_q, Hq, D], k and v [n_k, Hkv, D]")
+    if q.dtype not in (torch.bfloat16, torch.float16) or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError("q, k and v must be bf16, or all f16")
+    n_q, Hq, D = q.shape
+    n_k, Hkv, Dk = k.shape
+    if v.shape != k.shape or Dk != D:
+        raise ValueError("k and v must be alike, with q's head_dim")
+    if D not in (64, 128):
+        raise ValueError(f"head_dim must be 64 or 128, got {D}")
+    if Hq == 0 or Hkv == 0 or Hq % Hkv:
+        raise ValueError("the number of query heads must be a multiple of the number of kv heads")
+    B = cu_q.numel() - 1
+    if B < 1:
+        raise ValueError("cu_q and cu_k must be int32 [B + 1]")
+    for name, t, n in (("cu_q", cu_q, B + 1), ("cu_k", cu_k, B + 1)) + ((("k_lens", k_lens, B),) if k_lens is not None
+                                                                      else ()):
+        if t.dtype != torch.int32 or t.shape != (n,):
+            raise ValueError(f"{name} must be int32 [{n}]")
+    if err is not None and (err.dtype != torch.int32 or err.numel() < 1 or err.device != q.device):
+        raise ValueError("err must be an int32 tensor on q's device")
+    index = _index(q, "q")
+    for name, t in (("k", k), ("v", v)):
+        if t.get_device() != index:
+            raise ValueError(f"{name} must be on cuda:{index}, got {t.device}")
+    _all_on(index, cu_q=cu_q, cu_k=cu_k, k_lens=k_lens)
+    mq = int((cu_q[1:] - cu_q[:-1]).max().item()) if max_q_per_seq is None else int(max_q_per_seq)
+    mk = int((cu_k[1:] - cu_k[:-1]).max().item()) if max_k_per_seq is None else int(max_k_per_seq)
+    return index, B, max(0, min(mq, n_q)), max(0, min(mk, n_k))
+
+
+def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor, cu_k: torch.Tensor,
+                    k_lens: torch.Tensor | None = None, sm_scale: float | None = None,
+                    max_q_per_seq: int | None = None, max_k_per_seq: int | None = None,
+                    out: torch.Tensor | None = None, return_lse: bool = False, zero_rest: bool = False,
+                    check: bool = False, err: torch.Tensor | None = None):
+    """Attention of packed query rows to packed states of other lengths, all of which a row sees:
+    ``q [n_q, Hq, D]`` rows ``cu_q[b]`` to ``cu_q[b + 1]`` (int32 ``[B + 1]``) attend to keys ``cu_k[b]``
+    to ``cu_k[b + 1]`` of ``k``, ``v`` ``[n_k, Hkv, D]``; with ``k_lens`` (int32 ``[B]``) to the first
+    ``k_lens[b]`` of them, as in a padded batch (what the others hold does not count).  bf16 or f16,
+    D 64 or 128; views with contiguous channels may be given, e.g. the halves of a fused
+    projection.  Query head i reads kv head i // (Hq / Hkv).  ``max_q_per_seq`` / ``max_k_per_seq``
+    bound a sequence's rows and keys (read back without them, which waits for the device); rows
+    and keys beyond them are not computed or seen.  Rows in no sequence are left as they are in
+    ``out``, or become zeros with ``zero_rest``; a row without a key is zeros.  ``return_lse``: also float32
+    ``[Hq, n_q]``, log2 of each row's sum of exponentials (what ``cross_attention_backward`` takes).
+    autograd does not see this call: ``train.cross_attention.CrossAttention`` is the
+    differentiable form."""
+    N.need_gpu()
+    index, B, mq, mk = _cross_args(q, k, v, cu_q, cu_k, k_lens, max_q_per_seq, max_k_per_seq, err)
+    n_q, Hq, D = q.shape
+    n_k, Hkv, _ = k.shape
+    (qr, qh), (kr, kh), (vr, vh) = (_rows_of(t, name) for t, name in ((q, "q"), (k, "k"), (v, "v")))
+    if out is None:
+        out = torch.empty((n_q, Hq, D), dtype=q.dtype, device=q.device)
+    else:
+        if out.shape != q.shape or out.dtype != q.dtype:
+            raise ValueError(f"out must be {q.dtype} {tuple(q.shape)}")
+        _all_on(index, out=out)
+    lse = torch.empty((Hq, n_q), dtype=torch.float32, device=q.device) if return_lse else None
+    with _on(index):
+        ws, nb = _workspace_for("zx_cross_attention_workspace_bytes", index, n_q, Hq, Hkv, D, B, mq, mk)
+        err = _err_word_if(check, q.device) if err is None else err
+        N.check(N.load().zx_cross_attention(
+            _DT[q.dtype], q.data_ptr(), n_q, qr, qh, Hq, k.data_ptr(), kr, kh, v.data_ptr(), vr, vh, n_k, Hkv, D,
+            cu_q.data_ptr(), cu_k.data_ptr(), N.ptr(k_lens), B, mq, mk, D ** -0.5 if sm_scale is None else float(sm_scale),
+            N.ZX_CROSS_ZERO_REST if zero_rest else 0, out.data_ptr(), N.ptr(lse), N.ptr(err), N.ptr(ws), nb,
+            torch._C._cuda_getCurrentRawStream(index)), "cross_attention")
+    if check:
+        _raise_kernel_error(err, "cross_attention")
+    return (out, lse) if return_lse else out
+
+
+def cross_attention_backward(grad: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor,
+                             lse: torch.Tensor, cu_q: torch.Tensor, cu_k: torch.Tensor,
+                             k_lens: torch.Tensor | None = None, sm_scale: float | None = None,
+                             max_q_per_seq: int | None = None, max_k_per_seq: int | None = None, check: bool = False,
+                             err: torch.Tensor | None = None):
+    """``(dq, dk, dv)`` of ``cross_attention`` for its output's gradient ``grad`` (like ``q``), from ``out`` and
+    ``lse`` as it returned them; the other arguments as it took them.  Each is contiguous and in
+    q's type; those of rows in no sequence and of keys beyond ``k_lens`` are zeros.  Sums are in
+    fp32 and in a fixed order (the same from call to call); the scores' gradients are rounded once to
+    q's type, in f16 they have to be below 65504."""
+    N.need_gpu()
+    index, B, mq, mk = _cross_args(q, k, v, cu_q, cu_k, k_lens, max_q_per_seq, max_k_per_seq, err)
+    n_q, Hq, D = q.shape
+    n_k, Hkv, _ = k.shape
+    if grad.shape != q.shape or grad.dtype != q.dtype or out.shape != q.shape or out.dtype != q.dtype:
+        raise ValueError(f"grad and out must be {q.dtype} {tuple(q.shape)}")
+    if lse.shape != (Hq, n_q) or lse.dtype != torch.float32:
+        raise ValueError(f"lse must be float32 [{Hq}, {n_q}]")
+    if grad.get_device() != index:
+        raise ValueError(f"grad must be on cuda:{index}, got {grad.device}")
+    _all_on(index, out=out, lse=lse)
+    (gr, gh), (qr, qh), (kr, kh), (vr, vh) = (_rows_of(t, name) for t, name in ((grad, "grad"), (q, "q"), (k, "k"),
+                                                                               (v, "v")))
+    dq, dk, dv = (torch.empty(t.shape, dtype=q.dtype, device=q.device) for t in (q, k, v))
+    with _on(index):
+        ws, nb = _workspace_for("zx_cross_attention_backward_workspace_bytes", index, n_q, n_k, Hq, Hkv, D, B, mq, mk)
+        err = _err_word_if(check, q.device) if err is None else err
+        N.check(N.load().zx_cross_attention_backward(
+            _DT[q.dtype], grad.data_ptr(), gr, gh, q.data_ptr(), n_q, qr, qh, Hq, k.data_ptr(), kr, kh, v.data_ptr(), vr, vh,
+            n_k, Hkv, D, out.data_ptr(), lse.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), N.ptr(k_lens), B, mq, mk,
+            D ** -0.5 if sm_scale is None else float(sm_scale), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), N.ptr(err),
+            N.ptr(ws), nb, torch._C._cuda_getCurrentRawStream(index)), "cross_attention_backward")
+    if check:
+        _raise_kernel_error(err, "cross_attention_backward")
+    return dq, dk, dv
