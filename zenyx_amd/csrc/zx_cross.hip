@@ -119,10 +119,10 @@ static unsigned cr_grid(const CrossArgs &a) {
 // A tile of 64 rows in LDS: rows of D 16-bit values, 32 bytes apart (mod 128) and the 16-byte
 // chunks of rows 4-7 of 8 swapped in pairs: the 8 lanes of a 16-byte read (8 rows) and the 16
 // of a transposing one (4 rows of 32 bytes) touch distinct banks, and a store writes a row's chunks in a run.
-template <int D> struct CrLds {
+template <int D, int R = CR_TILE> struct CrLds {
   static constexpr int ROW = 2 * D + 32;
-  static constexpr int BYTES = CR_TILE * ROW;
-  static constexpr int LOADS = CR_TILE * D / 8 / CR_THREADS;  // 16 bytes each, per thread
+  static constexpr int BYTES = R * ROW;
+  static constexpr int LOADS = R * D / 8 / CR_THREADS;  // 16 bytes each, per thread
   static constexpr int CHUNKS = D / 8;
 };
 template <int D> __device__ __forceinline__ uint8_t *cr_at(uint8_t *t, int row, int byte) {
@@ -150,8 +150,9 @@ template <class T> __device__ __forceinline__ void cr_operands(const float (&x)[
 }
 
 // The tile's loads, in registers until the LDS buffer is free.  Rows from n on are zeros (and not read).
-template <int D> struct CrStage {
-  uint4 x[CrLds<D>::LOADS];
+template <int D, int R = CR_TILE> struct CrStage {
+  static constexpr int LOADS = CrLds<D, R>::LOADS;
+  uint4 x[LOADS];
   static __device__ __forceinline__ int row(int j) {
     return (int)threadIdx.x / CrLds<D>::CHUNKS + j * (CR_THREADS / CrLds<D>::CHUNKS);
   }
@@ -159,20 +160,20 @@ template <int D> struct CrStage {
   // n >= 1 rows of `step` elements from p on
   __device__ __forceinline__ void load(const uint16_t *p, int64_t step, int n) {
 #pragma unroll
-    for (int j = 0; j < CrLds<D>::LOADS; ++j)
+    for (int j = 0; j < LOADS; ++j)
       x[j] = *reinterpret_cast<const uint4 *>(p + min(row(j), n - 1) * step + 8 * chunk());
   }
   // (row, head) pairs c0 .. of a group: pair c is row c / G, head c % G
   __device__ __forceinline__ void load_pairs(const uint16_t *p, int64_t step, int64_t head, int c0, int n, int G) {
 #pragma unroll
-    for (int j = 0; j < CrLds<D>::LOADS; ++j) {
+    for (int j = 0; j < LOADS; ++j) {
       const uint32_t c = (uint32_t)(c0 + min(row(j), n - 1)), r = c / (uint32_t)G;
       x[j] = *reinterpret_cast<const uint4 *>(p + (int64_t)r * step + (int64_t)(c - r * (uint32_t)G) * head + 8 * chunk());
     }
   }
   __device__ __forceinline__ void store(uint8_t *t, int n) const {
 #pragma unroll
-    for (int j = 0; j < CrLds<D>::LOADS; ++j) {
+    for (int j = 0; j < LOADS; ++j) {
       const uint4 z = row(j) < n ? x[j] : make_uint4(0u, 0u, 0u, 0u);
       *reinterpret_cast<uint4 *>(cr_at<D>(t, row(j), 16 * chunk())) = z;
     }
@@ -242,7 +243,7 @@ __device__ __forceinline__ void cr_zero_rest(uint16_t *out, const int32_t *cu, i
 // ------------------------------------------------------------------ forward
 
 template <class T, int D, int CT>
-__global__ void __launch_bounds__(CR_THREADS, D *CT > 128 ? 1 : 2) cross_forward_kernel(CrossArgs a) {
+__global__ void __launch_bounds__(CR_THREADS, 2) cross_forward_kernel(CrossArgs a) {
   constexpr int KC = D / 16, DT = D / 32;
   __shared__ __attribute__((aligned(16))) uint8_t lds[2][2][CrLds<D>::BYTES];
   if (blockIdx.x + 1 == gridDim.x) {
@@ -459,9 +460,9 @@ template <class T, int D> __global__ void __launch_bounds__(256) cross_merge_ker
 // ------------------------------------------------------------------ gradients
 
 // dq, and on the way D_r for the other kernel.
-template <class T, int D, int CT>
-__global__ void __launch_bounds__(CR_THREADS, D *CT > 64 ? 1 : 2) cross_dq_kernel(CrossArgs a) {
-  constexpr int KC = D / 16, DT = D / 32;
+template <class T, int D>
+__global__ void __launch_bounds__(CR_THREADS, 2) cross_dq_kernel(CrossArgs a) {
+  constexpr int CT = 1, KC = D / 16, DT = D / 32;
   __shared__ __attribute__((aligned(16))) uint8_t lds[2][2][CrLds<D>::BYTES];
   if (blockIdx.x + 1 == gridDim.x) {
     cr_zero_rest(a.out, a.cu_q, a.n_seqs, a.n_q, (int64_t)a.n_q_heads * D);
@@ -594,12 +595,15 @@ __global__ void __launch_bounds__(CR_THREADS, D *CT > 64 ? 1 : 2) cross_dq_kerne
   }
 }
 
-// dk and dv of 128 KT keys, a wave 32 KT of them.
-template <class T, int D, int KT>
-__global__ void __launch_bounds__(CR_THREADS, D *KT > 64 ? 1 : 2) cross_dkv_kernel(CrossArgs a) {
-  constexpr int KC = D / 16, DT = D / 32;
-  __shared__ __attribute__((aligned(16))) uint8_t lds[2][2][CrLds<D>::BYTES];
-  __shared__ __attribute__((aligned(16))) float sm_lse[2][CR_TILE], sm_delta[2][CR_TILE];
+// dk and dv of 128 keys, a wave 32 of them.
+template <class T, int D>
+__global__ void __launch_bounds__(CR_THREADS, 2) cross_dkv_kernel(CrossArgs a) {
+  constexpr int R = D == 128 ? 32 : 64;  // rows per tile
+  constexpr bool VL = D == 128;   // V's rows in LDS instead of registers
+  constexpr int KT = 1, KC = D / 16, DT = D / 32;
+  __shared__ __attribute__((aligned(16))) uint8_t lv[VL ? 2 * CrLds<D>::BYTES : 16];
+  __shared__ __attribute__((aligned(16))) uint8_t lds[2][2][CrLds<D, R>::BYTES];
+  __shared__ __attribute__((aligned(16))) float sm_lse[2][R], sm_delta[2][R];
   if (blockIdx.x + 1 == gridDim.x) {
     cr_zero_rest(a.dk, a.cu_k, a.n_seqs, a.n_k, (int64_t)a.n_kv_heads * D);
     cr_zero_rest(a.dv, a.cu_k, a.n_seqs, a.n_k, (int64_t)a.n_kv_heads * D);
@@ -613,12 +617,12 @@ __global__ void __launch_bounds__(CR_THREADS, D *KT > 64 ? 1 : 2) cross_dkv_kern
   if (key0 >= ks.n) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int keys = cr_keys(a, it.b, ks.n);
-  const int n_cols = key0 < keys ? qs.n * a.group : 0, units = (n_cols + CR_TILE - 1) / CR_TILE;
-  const int t_begin = (int)((int64_t)units * it.split / a.n_split) * CR_TILE;
-  const int t_end = min(n_cols, (int)((int64_t)units * (it.split + 1) / a.n_split) * CR_TILE);
+  const int n_cols = key0 < keys ? qs.n * a.group : 0, units = (n_cols + R - 1) / R;
+  const int t_begin = (int)((int64_t)units * it.split / a.n_split) * R;
+  const int t_end = min(n_cols, (int)((int64_t)units * (it.split + 1) / a.n_split) * R);
   const int wk = key0 + 32 * KT * wave;  // the wave's first key
   const bool work = wk < keys;
-  att_u32x4 k[KT][KC], v[KT][KC];
+  att_u32x4 k[KT][KC], v[KT][VL ? 1 : KC];
   cr_f32x16 dk[KT][DT], dv[KT][DT];
 #pragma unroll
   for (int kt = 0; kt < KT; ++kt) {
@@ -629,7 +633,7 @@ __global__ void __launch_bounds__(CR_THREADS, D *KT > 64 ? 1 : 2) cross_dkv_kern
 #pragma unroll
     for (int kc = 0; kc < KC; ++kc) {
       k[kt][kc] = *reinterpret_cast<const att_u32x4 *>(kp + 16 * kc);
-      v[kt][kc] = *reinterpret_cast<const att_u32x4 *>(vp + 16 * kc);
+      if constexpr (!VL) v[kt][kc] = *reinterpret_cast<const att_u32x4 *>(vp + 16 * kc);
     }
     // keys that are not there: zeros (what memory holds in their place may be NaN)
 #pragma unroll
@@ -637,20 +641,32 @@ __global__ void __launch_bounds__(CR_THREADS, D *KT > 64 ? 1 : 2) cross_dkv_kern
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         k[kt][kc][i] = key < keys ? k[kt][kc][i] : 0u;
-        v[kt][kc][i] = key < keys ? v[kt][kc][i] : 0u;
+        if constexpr (!VL) v[kt][kc][i] = key < keys ? v[kt][kc][i] : 0u;
       }
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) dk[kt][dt] = dv[kt][dt] = cr_zero();
   }
+  if constexpr (VL) {
+    const uint16_t *vp = a.v.p + ks.lo * a.v.row + it.h * a.v.head;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int at = key0 + 64 * i;
+      if (at < keys) {
+        CrStage<D> sv;
+        sv.load(vp + at * a.v.row, a.v.row, min(64, keys - at));
+        sv.store(lv + i * CrLds<D>::BYTES, min(64, keys - at));
+      }
+    }
+  }
   const float scale = a.sm_scale * ATT_LOG2E;
   const uint16_t *qp = a.q.p + qs.lo * a.q.row + (int64_t)it.h * a.group * a.q.head;
   const uint16_t *gp = a.g.p + qs.lo * a.g.row + (int64_t)it.h * a.group * a.g.head;
-  CrStage<D> sq, sg;
+  CrStage<D, R> sq, sg;
   float my_lse = 0.0f, my_delta = 0.0f;
   auto load = [&](int c0, int n) {
     sq.load_pairs(qp, a.q.row, a.q.head, c0, n, a.group);
     sg.load_pairs(gp, a.g.row, a.g.head, c0, n, a.group);
-    if (threadIdx.x < CR_TILE) {
+    if (threadIdx.x < R) {
       const uint32_t c = (uint32_t)(c0 + min((int)threadIdx.x, n - 1)), r = c / (uint32_t)a.group;
       const int64_t at = (int64_t)(it.h * a.group + (int32_t)(c - r * (uint32_t)a.group)) * a.n_q + qs.lo + r;
       my_lse = a.lse[at];
@@ -660,26 +676,26 @@ __global__ void __launch_bounds__(CR_THREADS, D *KT > 64 ? 1 : 2) cross_dkv_kern
   auto store = [&](int buf, int n) {
     sq.store(lds[buf][0], n);
     sg.store(lds[buf][1], n);
-    if (threadIdx.x < CR_TILE) {  // (a row that is not there: weights of 0)
+    if (threadIdx.x < R) {  // (a row that is not there: weights of 0)
       sm_lse[buf][threadIdx.x] = (int)threadIdx.x < n ? my_lse - T::BIAS : INFINITY;
       sm_delta[buf][threadIdx.x] = (int)threadIdx.x < n ? my_delta : 0.0f;
     }
   };
   if (t_begin < t_end) {
-    const int n = min(CR_TILE, t_end - t_begin);
+    const int n = min(R, t_end - t_begin);
     load(t_begin, n);
     store(0, n);
   }
   __syncthreads();
   const float unbias = __builtin_amdgcn_exp2f(-T::BIAS);
   int buf = 0;
-  for (int t = t_begin; t < t_end; t += CR_TILE, buf ^= 1) {
-    const int next = t + CR_TILE, n_next = min(CR_TILE, t_end - next);
+  for (int t = t_begin; t < t_end; t += R, buf ^= 1) {
+    const int next = t + R, n_next = min(R, t_end - next);
     if (next < t_end) load(next, n_next);
     if (work) {
       uint8_t *lq = lds[buf][0], *lg = lds[buf][1];
 #pragma unroll
-      for (int rt = 0; rt < 2; ++rt) {
+      for (int rt = 0; rt < R / 32; ++rt) {
         cr_f32x16 s[KT], dp[KT];
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt) s[kt] = dp[kt] = cr_zero();
@@ -689,7 +705,7 @@ __global__ void __launch_bounds__(CR_THREADS, D *KT > 64 ? 1 : 2) cross_dkv_kern
 #pragma unroll
           for (int kt = 0; kt < KT; ++kt) {
             s[kt] = T::mfma(q, k[kt][kc], s[kt]);
-            dp[kt] = T::mfma(g, v[kt][kc], dp[kt]);
+            dp[kt] = T::mfma(g, VL ? cr_rows<D>(lv + (wave / 2) * CrLds<D>::BYTES, wave & 1, kc, lane) : v[kt][VL ? 0 : kc], dp[kt]);
           }
         }
         att_u32x4 p[KT][2], ds[KT][2];
@@ -802,18 +818,19 @@ static CrossPlan cr_plan(int64_t pairs, int64_t columns, int64_t length, int ct,
   return p;
 }
 static CrossPlan cr_forward_plan(int32_t n_seqs, int32_t n_kv_heads, int32_t group, int32_t D, int32_t max_q, int32_t max_k) {
-  const int64_t columns = (int64_t)max_q * group;
-  const int ct = columns >= 512 ? 2 : 1;
-  return cr_plan((int64_t)n_seqs * n_kv_heads, columns, max_k, ct, D * ct > 128 ? 1 : D == 64 ? 4 : 2, 2);
+  const int64_t columns = (int64_t)max_q * group, pairs = (int64_t)n_seqs * n_kv_heads;
+  // Two column tiles per wave halve the LDS reads of K and V per product, where they leave two
+  // waves per SIMD (D = 64) and tiles enough: 4 x 2,048 rows x 4 heads on 4,096 keys 302 us against
+  // 340; 16 x 448 rows on 1,500 keys, 12 heads 106 against 57.  (D = 128, one wave per SIMD then: 4 x
+  // 2,048 rows, 32/8 heads, on 8,192 keys 1,364 against 1,202.)
+  const int ct = D == 64 && columns >= 1024 && pairs * ceil_div(columns, 256) >= 4 * num_cus() ? 2 : 1;
+  return cr_plan(pairs, columns, max_k, ct, D == 64 && ct == 1 ? 3 : 2, 2);
 }
 static CrossPlan cr_dq_plan(int32_t n_seqs, int32_t n_kv_heads, int32_t group, int32_t D, int32_t max_q, int32_t max_k) {
-  const int64_t columns = (int64_t)max_q * group;
-  const int ct = columns >= 512 ? 2 : 1;
-  return cr_plan((int64_t)n_seqs * n_kv_heads, columns, max_k, ct, D * ct > 64 ? 1 : 2, 4);
+  return cr_plan((int64_t)n_seqs * n_kv_heads, (int64_t)max_q * group, max_k, 1, D == 64 ? 3 : 2, 4);
 }
 static CrossPlan cr_dkv_plan(int32_t n_seqs, int32_t n_kv_heads, int32_t group, int32_t D, int32_t max_q, int32_t max_k) {
-  const int kt = D == 64 && max_k >= 512 ? 2 : 1;
-  return cr_plan((int64_t)n_seqs * n_kv_heads, max_k, (int64_t)max_q * group, kt, D * kt > 64 ? 1 : 2, 4);
+  return cr_plan((int64_t)n_seqs * n_kv_heads, max_k, (int64_t)max_q * group, 1, 2, 4);
 }
 static bool cr_dims_ok(int64_t n_q, int64_t n_k, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim, int32_t n_seqs,
                        int32_t max_q, int32_t max_k) {
@@ -874,7 +891,7 @@ static int cr_check_rows(const char *what, const char *name, const CrIn &x) {
 
 template <class T, int D> static int cr_forward(CrossArgs a, const CrossPlan &p, hipStream_t st) {
   const unsigned grid = cr_grid(a) + 1;
-  if (p.ct == 2) cross_forward_kernel<T, D, 2><<<grid, CR_THREADS, 0, st>>>(a);
+  if (D == 64 && p.ct == 2) cross_forward_kernel<T, 64, 2><<<grid, CR_THREADS, 0, st>>>(a);
   else cross_forward_kernel<T, D, 1><<<grid, CR_THREADS, 0, st>>>(a);
   const int rc = check_launch("cross_forward");
   if (rc || a.n_split == 1) return rc;
@@ -939,8 +956,7 @@ static int cr_backward(CrossArgs a, const CrossPlan &pq, const CrossPlan &pk, ui
   a.out = dq;
   a.n_tile = (int32_t)pq.n_tile;
   a.n_split = (int32_t)pq.n_split;
-  if (pq.ct == 2) cross_dq_kernel<T, D, 2><<<cr_grid(a) + 1, CR_THREADS, 0, st>>>(a);
-  else cross_dq_kernel<T, D, 1><<<cr_grid(a) + 1, CR_THREADS, 0, st>>>(a);
+  cross_dq_kernel<T, D><<<cr_grid(a) + 1, CR_THREADS, 0, st>>>(a);
   if ((rc = check_launch("cross_dq"))) return rc;
   const int64_t wq = (int64_t)a.n_q_heads * D, wk = (int64_t)a.n_kv_heads * D;
   if (pq.n_split > 1 && a.n_q) {
@@ -951,11 +967,7 @@ static int cr_backward(CrossArgs a, const CrossPlan &pq, const CrossPlan &pk, ui
   if (a.n_k == 0) return ZX_OK;
   a.n_tile = (int32_t)pk.n_tile;
   a.n_split = (int32_t)pk.n_split;
-  if (pk.ct == 2) {
-    if constexpr (D == 64) cross_dkv_kernel<T, D, 2><<<cr_grid(a) + 1, CR_THREADS, 0, st>>>(a);
-  } else {
-    cross_dkv_kernel<T, D, 1><<<cr_grid(a) + 1, CR_THREADS, 0, st>>>(a);
-  }
+  cross_dkv_kernel<T, D><<<cr_grid(a) + 1, CR_THREADS, 0, st>>>(a);
   if ((rc = check_launch("cross_dkv")) || pk.n_split == 1) return rc;
   for (int i = 0; i < 2; ++i) {
     cross_sum_kernel<T><<<(unsigned)ceil_div(a.n_k * wk, 8 * 256), 256, 0, st>>>(
