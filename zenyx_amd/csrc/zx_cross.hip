@@ -78,8 +78,18 @@ struct CrossArgs {
   int32_t max_q, max_k;
   int32_t n_tile, n_split;  // tiles of a sequence and KV head at most, parts of each
   int32_t zero_rest;
+  uint32_t g_magic;         // c / group = (c * g_magic) >> (31 + g_shift) for c < 2^31
+  int32_t g_shift;
+  int32_t order;            // the sequences with the most work first
   float sm_scale;
 };
+
+// The row and the head within its group of pair c.
+__device__ __forceinline__ uint32_t cr_pair(const CrossArgs &a, uint32_t c, uint32_t &head) {
+  const uint32_t r = (uint32_t)(((uint64_t)c * a.g_magic) >> (31 + a.g_shift));
+  head = c - r * (uint32_t)a.group;
+  return r;
+}
 
 // Rows [lo, hi) of the packed n that sequence b has, none outside and at most `most`.
 struct CrSpan {
@@ -96,7 +106,9 @@ __device__ __forceinline__ int32_t cr_keys(const CrossArgs &a, int32_t b, int32_
 }
 
 // What a block does: tiles of one sequence and KV head on the same XCD (block ids go round the
-// eight), so that what they read in common is in its L2.
+// eight), so that what they read in common is in its L2; where blocks are long (cr_order) the
+// sequences with the most work first: the chip is left with short ones at the end (1,000-2,048 rows on
+// 2,000-8,192 keys, 4 sequences, 32/8 heads, D = 128: 611 -> 569 us).
 struct CrItem {
   int32_t b, h, tile, split;
   bool any;
@@ -110,37 +122,61 @@ __device__ __forceinline__ CrItem cr_item(const CrossArgs &a) {
   it.h = (int32_t)(pair - (uint32_t)it.b * (uint32_t)a.n_kv_heads);
   it.tile = (int32_t)(rem / (uint32_t)a.n_split);
   it.split = (int32_t)(rem - (uint32_t)it.tile * (uint32_t)a.n_split);
+  if (a.order) {
+    const int lane = threadIdx.x & 63;
+    float w = -1.0f;
+    if (lane < a.n_seqs) {
+      const int32_t keys = a.cu_k[lane + 1] - a.cu_k[lane];
+      w = (float)(a.cu_q[lane + 1] - a.cu_q[lane]) * (float)(a.k_lens ? min(a.k_lens[lane], keys) : keys);
+    }
+    int before = lane < a.n_seqs ? 0 : 64;
+    for (int s = 0; s < a.n_seqs; ++s) {
+      const float other = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), s));
+      before += other > w || (other == w && s < lane);
+    }
+    it.b = __ffsll((long long)__ballot(before == it.b)) - 1;
+    it.any &= it.b >= 0;
+  }
   return it;
 }
 static unsigned cr_grid(const CrossArgs &a) {
   return (unsigned)(8 * ceil_div((int64_t)a.n_seqs * a.n_kv_heads, 8) * a.n_tile * a.n_split);
 }
 
-// A tile of 64 rows in LDS: rows of D 16-bit values, 32 bytes apart (mod 128) and the 16-byte
-// chunks of rows 4-7 of 8 swapped in pairs: the 8 lanes of a 16-byte read (8 rows) and the 16
-// of a transposing one (4 rows of 32 bytes) touch distinct banks, and a store writes a row's chunks in a run.
+// A tile of R rows of D 16-bit values in LDS: rows 64 bytes apart (mod 256), the 16-byte chunks of
+// every 64 bytes permuted by an XOR with two bits of the row.  So both ways of reading touch the 64
+// banks evenly: 16 lanes that take the same chunk of 16 rows, and 32 that take 64 bytes of 4 rows (rows
+// 32 bytes apart, free of conflicts on 32 banks only, made both take twice the cycles), and a
+// lane needs two addresses for either, the rest being constant offsets.
 template <int D, int R = CR_TILE> struct CrLds {
-  static constexpr int ROW = 2 * D + 32;
+  static constexpr int ROW = 2 * D + 64;
   static constexpr int BYTES = R * ROW;
   static constexpr int LOADS = R * D / 8 / CR_THREADS;  // 16 bytes each, per thread
   static constexpr int CHUNKS = D / 8;
 };
 template <int D> __device__ __forceinline__ uint8_t *cr_at(uint8_t *t, int row, int byte) {
-  return t + row * CrLds<D>::ROW + (byte ^ (16 * ((row >> 2) & 1)));
+  return t + row * CrLds<D>::ROW + (byte ^ (32 * ((row >> 2) & 1) + 16 * ((row >> 3) & 1)));
 }
 // Row 32 kt + (lane & 31), channels 16 kc + 8 half ..+8: an operand whose rows (or columns) are the tile's.
 template <int D> __device__ __forceinline__ att_u32x4 cr_rows(uint8_t *t, int kt, int kc, int lane) {
-  return *reinterpret_cast<const att_u32x4 *>(cr_at<D>(t, 32 * kt + (lane & 31), 32 * kc + 16 * (lane >> 5)));
+  const uint8_t *p = cr_at<D>(t, lane & 31, 32 * (kc & 1) + 16 * (lane >> 5));
+  return *reinterpret_cast<const att_u32x4 *>(p + 64 * (kc >> 1) + 32 * kt * CrLds<D>::ROW);
 }
 // Channel 32 dt + (lane & 31) of rows 16 c + 8 a + 4 half + b (a = 0, 1; b = 0 .. 3): a transposed operand.
 template <int D> __device__ __forceinline__ att_u32x4 cr_cols(uint8_t *t, int c, int dt, int lane) {
-  const int row = 16 * c + 4 * (lane >> 5) + ((lane & 15) >> 2);
-  const uint8_t *p = cr_at<D>(t, row, 64 * dt + 32 * ((lane >> 4) & 1) + 8 * (lane & 3));
+  const int row = 4 * (lane >> 5) + ((lane & 15) >> 2), byte = 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
+  const uint8_t *p = cr_at<D>(t, row, byte) + 64 * dt + 16 * c * CrLds<D>::ROW;
+  const uint8_t *p8 = cr_at<D>(t, row + 8, byte) + 64 * dt + 16 * c * CrLds<D>::ROW;
   typedef __attribute__((address_space(3))) cr_i16x4 *lds_ptr;
   const uint2 x = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p)));
-  const uint2 y = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p + 8 * CrLds<D>::ROW)));
+  const uint2 y = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p8)));
   return att_u32x4{x.x, x.y, y.x, y.y};
 }
+// A tile that is read by rows alone.
+template <int D> struct CrRowsOnly {
+  static constexpr int ROW = 2 * D + 16;
+  static __device__ __forceinline__ uint8_t *at(uint8_t *t, int row, int byte) { return t + row * ROW + byte; }
+};
 // 16 values of a product's column as the two operands of the next product.
 template <class T> __device__ __forceinline__ void cr_operands(const float (&x)[16], att_u32x4 (&o)[2]) {
 #pragma unroll
@@ -157,19 +193,11 @@ template <int D, int R = CR_TILE> struct CrStage {
     return (int)threadIdx.x / CrLds<D>::CHUNKS + j * (CR_THREADS / CrLds<D>::CHUNKS);
   }
   static __device__ __forceinline__ int chunk() { return (int)threadIdx.x % CrLds<D>::CHUNKS; }
-  // n >= 1 rows of `step` elements from p on
-  __device__ __forceinline__ void load(const uint16_t *p, int64_t step, int n) {
+  // n >= 1 rows of `step` elements from p on (uniform; a tile's offsets fit 32 bits: cr_check_rows)
+  __device__ __forceinline__ void load(const uint16_t *p, uint32_t step, int n) {
 #pragma unroll
     for (int j = 0; j < LOADS; ++j)
-      x[j] = *reinterpret_cast<const uint4 *>(p + min(row(j), n - 1) * step + 8 * chunk());
-  }
-  // (row, head) pairs c0 .. of a group: pair c is row c / G, head c % G
-  __device__ __forceinline__ void load_pairs(const uint16_t *p, int64_t step, int64_t head, int c0, int n, int G) {
-#pragma unroll
-    for (int j = 0; j < LOADS; ++j) {
-      const uint32_t c = (uint32_t)(c0 + min(row(j), n - 1)), r = c / (uint32_t)G;
-      x[j] = *reinterpret_cast<const uint4 *>(p + (int64_t)r * step + (int64_t)(c - r * (uint32_t)G) * head + 8 * chunk());
-    }
+      x[j] = *reinterpret_cast<const uint4 *>(p + ((uint32_t)min(row(j), n - 1) * step + 8u * (uint32_t)chunk()));
   }
   __device__ __forceinline__ void store(uint8_t *t, int n) const {
 #pragma unroll
@@ -179,6 +207,24 @@ template <int D, int R = CR_TILE> struct CrStage {
     }
   }
 };
+
+// Tiles [t_begin, t_end) in steps of `step` through two LDS buffers: load(t) issues a tile's loads,
+// store(buffer, t) writes them to LDS, compute(buffer, t) works on it.  (Loads two tiles ahead at
+// D = 64 took the same time, or 4% more where they cost registers.)
+template <class Load, class Store, class Compute>
+__device__ __forceinline__ void cr_pipeline(int t_begin, int t_end, int step, Load load, Store store, Compute compute) {
+  if (t_begin >= t_end) return;
+  load(t_begin);
+  store(0, t_begin);
+  __syncthreads();
+  int buf = 0;
+  for (int t = t_begin; t < t_end; t += step, buf ^= 1) {
+    if (t + step < t_end) load(t + step);
+    compute(buf, t);
+    if (t + step < t_end) store(buf ^ 1, t + step);
+    __syncthreads();
+  }
+}
 
 __device__ __forceinline__ float cr_halves_sum(float v) {
   float x, y;
@@ -210,9 +256,9 @@ template <int D, int CT> struct CrCols {
     for (int ct = 0; ct < CT; ++ct) {
       const int c = c0 + 32 * (CT * wave + ct) + (lane & 31);
       live[ct] = c < n_cols;
-      const uint32_t cc = (uint32_t)min(c, n_cols - 1), r = cc / (uint32_t)a.group;
-      row[ct] = (int32_t)(lo + r);
-      head[ct] = h * a.group + (int32_t)(cc - r * (uint32_t)a.group);
+      uint32_t hh;
+      row[ct] = (int32_t)(lo + cr_pair(a, (uint32_t)min(c, n_cols - 1), hh));
+      head[ct] = h * a.group + (int32_t)hh;
     }
   }
   // Their D channels as B operands (columns that are not there as zeros).
@@ -245,7 +291,7 @@ __device__ __forceinline__ void cr_zero_rest(uint16_t *out, const int32_t *cu, i
 template <class T, int D, int CT>
 __global__ void __launch_bounds__(CR_THREADS, 2) cross_forward_kernel(CrossArgs a) {
   constexpr int KC = D / 16, DT = D / 32;
-  __shared__ __attribute__((aligned(16))) uint8_t lds[2][2][CrLds<D>::BYTES];
+  __shared__ __attribute__((aligned(256))) uint8_t lds[2][2][CrLds<D>::BYTES];
   if (blockIdx.x + 1 == gridDim.x) {
     if (a.zero_rest) cr_zero_rest(a.out, a.cu_q, a.n_seqs, a.n_q, (int64_t)a.n_q_heads * D);
     return;
@@ -287,21 +333,15 @@ __global__ void __launch_bounds__(CR_THREADS, 2) cross_forward_kernel(CrossArgs 
   }
   const uint16_t *kp = a.k.p + ks.lo * a.k.row + it.h * a.k.head, *vp = a.v.p + ks.lo * a.v.row + it.h * a.v.head;
   CrStage<D> sk, sv;
-  if (t_begin < t_end) {
-    const int n = min(CR_TILE, t_end - t_begin);
-    sk.load(kp + t_begin * a.k.row, a.k.row, n);
-    sv.load(vp + t_begin * a.v.row, a.v.row, n);
-    sk.store(lds[0][0], n);
-    sv.store(lds[0][1], n);
-  }
-  __syncthreads();
-  int buf = 0;
-  for (int t = t_begin; t < t_end; t += CR_TILE, buf ^= 1) {
-    const int next = t + CR_TILE, n_next = min(CR_TILE, t_end - next);
-    if (next < t_end) {
-      sk.load(kp + next * a.k.row, a.k.row, n_next);
-      sv.load(vp + next * a.v.row, a.v.row, n_next);
-    }
+  auto load = [&](int t) {
+    sk.load(kp + t * a.k.row, (uint32_t)a.k.row, min(CR_TILE, t_end - t));
+    sv.load(vp + t * a.v.row, (uint32_t)a.v.row, min(CR_TILE, t_end - t));
+  };
+  auto store = [&](int buf, int t) {
+    sk.store(lds[buf][0], min(CR_TILE, t_end - t));
+    sv.store(lds[buf][1], min(CR_TILE, t_end - t));
+  };
+  auto compute = [&](int buf, int t) {
     if (work) {
       uint8_t *lk = lds[buf][0], *lv = lds[buf][1];
       cr_f32x16 s[CT][2];
@@ -371,12 +411,8 @@ __global__ void __launch_bounds__(CR_THREADS, 2) cross_forward_kernel(CrossArgs 
           }
       }
     }
-    if (next < t_end) {
-      sk.store(lds[buf ^ 1][0], n_next);
-      sv.store(lds[buf ^ 1][1], n_next);
-    }
-    __syncthreads();
-  }
+  };
+  cr_pipeline(t_begin, t_end, CR_TILE, load, store, compute);
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
     if (!cols.live[ct]) continue;
@@ -461,9 +497,9 @@ template <class T, int D> __global__ void __launch_bounds__(256) cross_merge_ker
 
 // dq, and on the way D_r for the other kernel.
 template <class T, int D>
-__global__ void __launch_bounds__(CR_THREADS, 2) cross_dq_kernel(CrossArgs a) {
+__global__ void __launch_bounds__(CR_THREADS, D == 64 ? 3 : 2) cross_dq_kernel(CrossArgs a) {
   constexpr int CT = 1, KC = D / 16, DT = D / 32;
-  __shared__ __attribute__((aligned(16))) uint8_t lds[2][2][CrLds<D>::BYTES];
+  __shared__ __attribute__((aligned(256))) uint8_t lds[2][2][CrLds<D>::BYTES];
   if (blockIdx.x + 1 == gridDim.x) {
     cr_zero_rest(a.out, a.cu_q, a.n_seqs, a.n_q, (int64_t)a.n_q_heads * D);
     return;
@@ -509,21 +545,15 @@ __global__ void __launch_bounds__(CR_THREADS, 2) cross_dq_kernel(CrossArgs a) {
   const float scale = a.sm_scale * ATT_LOG2E;
   const uint16_t *kp = a.k.p + ks.lo * a.k.row + it.h * a.k.head, *vp = a.v.p + ks.lo * a.v.row + it.h * a.v.head;
   CrStage<D> sk, sv;
-  if (t_begin < t_end) {
-    const int n = min(CR_TILE, t_end - t_begin);
-    sk.load(kp + t_begin * a.k.row, a.k.row, n);
-    sv.load(vp + t_begin * a.v.row, a.v.row, n);
-    sk.store(lds[0][0], n);
-    sv.store(lds[0][1], n);
-  }
-  __syncthreads();
-  int buf = 0;
-  for (int t = t_begin; t < t_end; t += CR_TILE, buf ^= 1) {
-    const int next = t + CR_TILE, n_next = min(CR_TILE, t_end - next);
-    if (next < t_end) {
-      sk.load(kp + next * a.k.row, a.k.row, n_next);
-      sv.load(vp + next * a.v.row, a.v.row, n_next);
-    }
+  auto load = [&](int t) {
+    sk.load(kp + t * a.k.row, (uint32_t)a.k.row, min(CR_TILE, t_end - t));
+    sv.load(vp + t * a.v.row, (uint32_t)a.v.row, min(CR_TILE, t_end - t));
+  };
+  auto store = [&](int buf, int t) {
+    sk.store(lds[buf][0], min(CR_TILE, t_end - t));
+    sv.store(lds[buf][1], min(CR_TILE, t_end - t));
+  };
+  auto compute = [&](int buf, int t) {
     if (work) {
       uint8_t *lk = lds[buf][0], *lv = lds[buf][1];
 #pragma unroll
@@ -564,12 +594,8 @@ __global__ void __launch_bounds__(CR_THREADS, 2) cross_dq_kernel(CrossArgs a) {
           }
       }
     }
-    if (next < t_end) {
-      sk.store(lds[buf ^ 1][0], n_next);
-      sv.store(lds[buf ^ 1][1], n_next);
-    }
-    __syncthreads();
-  }
+  };
+  cr_pipeline(t_begin, t_end, CR_TILE, load, store, compute);
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
     if (!cols.live[ct]) continue;
@@ -597,12 +623,12 @@ __global__ void __launch_bounds__(CR_THREADS, 2) cross_dq_kernel(CrossArgs a) {
 
 // dk and dv of 128 keys, a wave 32 of them.
 template <class T, int D>
-__global__ void __launch_bounds__(CR_THREADS, 2) cross_dkv_kernel(CrossArgs a) {
-  constexpr int R = D == 128 ? 32 : 64;  // rows per tile
-  constexpr bool VL = D == 128;   // V's rows in LDS instead of registers
-  constexpr int KT = 1, KC = D / 16, DT = D / 32;
-  __shared__ __attribute__((aligned(16))) uint8_t lv[VL ? 2 * CrLds<D>::BYTES : 16];
-  __shared__ __attribute__((aligned(16))) uint8_t lds[2][2][CrLds<D, R>::BYTES];
+__global__ void __launch_bounds__(CR_THREADS, D == 64 ? 3 : 2) cross_dkv_kernel(CrossArgs a) {
+  constexpr int R = 32;  // rows per tile
+  constexpr int KC = D / 16, DT = D / 32;
+  using VRows = CrRowsOnly<D>;
+  __shared__ __attribute__((aligned(256))) uint8_t lv[32 * CR_WAVES * VRows::ROW];  // V's rows
+  __shared__ __attribute__((aligned(256))) uint8_t lds[2][2][CrLds<D, R>::BYTES];
   __shared__ __attribute__((aligned(16))) float sm_lse[2][R], sm_delta[2][R];
   if (blockIdx.x + 1 == gridDim.x) {
     cr_zero_rest(a.dk, a.cu_k, a.n_seqs, a.n_k, (int64_t)a.n_kv_heads * D);
@@ -613,67 +639,64 @@ __global__ void __launch_bounds__(CR_THREADS, 2) cross_dkv_kernel(CrossArgs a) {
   if (!it.any) return;
   int32_t e = 0;  // (reported with dq)
   const CrSpan qs = cr_span(a.cu_q, it.b, a.n_q, a.max_q, e), ks = cr_span(a.cu_k, it.b, a.n_k, a.max_k, e);
-  const int key0 = it.tile * 32 * KT * CR_WAVES;
+  const int key0 = it.tile * 32 * CR_WAVES;
   if (key0 >= ks.n) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int keys = cr_keys(a, it.b, ks.n);
   const int n_cols = key0 < keys ? qs.n * a.group : 0, units = (n_cols + R - 1) / R;
   const int t_begin = (int)((int64_t)units * it.split / a.n_split) * R;
   const int t_end = min(n_cols, (int)((int64_t)units * (it.split + 1) / a.n_split) * R);
-  const int wk = key0 + 32 * KT * wave;  // the wave's first key
-  const bool work = wk < keys;
-  att_u32x4 k[KT][KC], v[KT][VL ? 1 : KC];
-  cr_f32x16 dk[KT][DT], dv[KT][DT];
-#pragma unroll
-  for (int kt = 0; kt < KT; ++kt) {
-    const int key = wk + 32 * kt + (lane & 31);
-    const int64_t row = ks.lo + max(0, min(key, keys - 1));
+  const int wk = key0 + 32 * wave;  // the wave's first key
+  const bool work = wk < keys, live = wk + (lane & 31) < keys;
+  att_u32x4 k[KC];
+  cr_f32x16 dk[DT], dv[DT];
+  {
+    const int64_t row = ks.lo + max(0, min(wk + (lane & 31), keys - 1));
     const uint16_t *kp = a.k.p + row * a.k.row + it.h * a.k.head + 8 * (lane >> 5);
-    const uint16_t *vp = a.v.p + row * a.v.row + it.h * a.v.head + 8 * (lane >> 5);
-#pragma unroll
-    for (int kc = 0; kc < KC; ++kc) {
-      k[kt][kc] = *reinterpret_cast<const att_u32x4 *>(kp + 16 * kc);
-      if constexpr (!VL) v[kt][kc] = *reinterpret_cast<const att_u32x4 *>(vp + 16 * kc);
-    }
     // keys that are not there: zeros (what memory holds in their place may be NaN)
 #pragma unroll
-    for (int kc = 0; kc < KC; ++kc)
+    for (int kc = 0; kc < KC; ++kc) {
+      const att_u32x4 w = *reinterpret_cast<const att_u32x4 *>(kp + 16 * kc);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        k[kt][kc][i] = key < keys ? k[kt][kc][i] : 0u;
-        if constexpr (!VL) v[kt][kc][i] = key < keys ? v[kt][kc][i] : 0u;
-      }
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) dk[kt][dt] = dv[kt][dt] = cr_zero();
-  }
-  if constexpr (VL) {
+      for (int i = 0; i < 4; ++i) k[kc][i] = live ? w[i] : 0u;
+    }
     const uint16_t *vp = a.v.p + ks.lo * a.v.row + it.h * a.v.head;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int at = key0 + 64 * i;
-      if (at < keys) {
-        CrStage<D> sv;
-        sv.load(vp + at * a.v.row, a.v.row, min(64, keys - at));
-        sv.store(lv + i * CrLds<D>::BYTES, min(64, keys - at));
-      }
+    for (int i = threadIdx.x; i < 32 * CR_WAVES * D / 8; i += CR_THREADS) {
+      const int r = i / (D / 8), c = i % (D / 8);
+      uint4 w = make_uint4(0u, 0u, 0u, 0u);
+      if (key0 + r < keys) w = *reinterpret_cast<const uint4 *>(vp + (key0 + r) * a.v.row + 8 * c);
+      *reinterpret_cast<uint4 *>(VRows::at(lv, r, 16 * c)) = w;
     }
   }
+  uint8_t *const my_v = VRows::at(lv, 32 * wave + (lane & 31), 16 * (lane >> 5));
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) dk[dt] = dv[dt] = cr_zero();
   const float scale = a.sm_scale * ATT_LOG2E;
   const uint16_t *qp = a.q.p + qs.lo * a.q.row + (int64_t)it.h * a.group * a.q.head;
   const uint16_t *gp = a.g.p + qs.lo * a.g.row + (int64_t)it.h * a.group * a.g.head;
   CrStage<D, R> sq, sg;
   float my_lse = 0.0f, my_delta = 0.0f;
-  auto load = [&](int c0, int n) {
-    sq.load_pairs(qp, a.q.row, a.q.head, c0, n, a.group);
-    sg.load_pairs(gp, a.g.row, a.g.head, c0, n, a.group);
+  auto load = [&](int t) {
+    const int n = min(R, t_end - t);
+    uint32_t hh;
+    const uint32_t r0 = cr_pair(a, (uint32_t)t, hh);  // uniform
+    const uint16_t *q = qp + (int64_t)r0 * a.q.row, *g = gp + (int64_t)r0 * a.g.row;
+#pragma unroll
+    for (int j = 0; j < CrStage<D, R>::LOADS; ++j) {
+      const uint32_t r = cr_pair(a, (uint32_t)(t + min(CrStage<D, R>::row(j), n - 1)), hh) - r0;
+      const uint32_t c = 8u * (uint32_t)CrStage<D, R>::chunk();
+      sq.x[j] = *reinterpret_cast<const uint4 *>(q + (r * (uint32_t)a.q.row + hh * (uint32_t)a.q.head + c));
+      sg.x[j] = *reinterpret_cast<const uint4 *>(g + (r * (uint32_t)a.g.row + hh * (uint32_t)a.g.head + c));
+    }
     if (threadIdx.x < R) {
-      const uint32_t c = (uint32_t)(c0 + min((int)threadIdx.x, n - 1)), r = c / (uint32_t)a.group;
-      const int64_t at = (int64_t)(it.h * a.group + (int32_t)(c - r * (uint32_t)a.group)) * a.n_q + qs.lo + r;
+      const uint32_t r = cr_pair(a, (uint32_t)(t + min((int)threadIdx.x, n - 1)), hh);
+      const int64_t at = (int64_t)(it.h * a.group + (int32_t)hh) * a.n_q + qs.lo + r;
       my_lse = a.lse[at];
       my_delta = a.delta[at];
     }
   };
-  auto store = [&](int buf, int n) {
+  auto store = [&](int buf, int t) {
+    const int n = min(R, t_end - t);
     sq.store(lds[buf][0], n);
     sg.store(lds[buf][1], n);
     if (threadIdx.x < R) {  // (a row that is not there: weights of 0)
@@ -681,97 +704,65 @@ __global__ void __launch_bounds__(CR_THREADS, 2) cross_dkv_kernel(CrossArgs a) {
       sm_delta[buf][threadIdx.x] = (int)threadIdx.x < n ? my_delta : 0.0f;
     }
   };
-  if (t_begin < t_end) {
-    const int n = min(R, t_end - t_begin);
-    load(t_begin, n);
-    store(0, n);
-  }
-  __syncthreads();
   const float unbias = __builtin_amdgcn_exp2f(-T::BIAS);
-  int buf = 0;
-  for (int t = t_begin; t < t_end; t += R, buf ^= 1) {
-    const int next = t + R, n_next = min(R, t_end - next);
-    if (next < t_end) load(next, n_next);
-    if (work) {
-      uint8_t *lq = lds[buf][0], *lg = lds[buf][1];
+  auto compute = [&](int buf, int) {
+    if (!work) return;
+    uint8_t *lq = lds[buf][0], *lg = lds[buf][1];
+    cr_f32x16 s = cr_zero(), dp = cr_zero();
 #pragma unroll
-      for (int rt = 0; rt < R / 32; ++rt) {
-        cr_f32x16 s[KT], dp[KT];
+    for (int kc = 0; kc < KC; ++kc) {
+      s = T::mfma(cr_rows<D>(lq, 0, kc, lane), k[kc], s);
+      dp = T::mfma(cr_rows<D>(lg, 0, kc, lane), *reinterpret_cast<const att_u32x4 *>(my_v + 32 * kc), dp);
+    }
+    att_u32x4 p[2], ds[2];
+    float x[16], y[16];
 #pragma unroll
-        for (int kt = 0; kt < KT; ++kt) s[kt] = dp[kt] = cr_zero();
+    for (int i4 = 0; i4 < 4; ++i4) {
+      const int row = 8 * i4 + 4 * (lane >> 5);
+      const att_f32x4 lse = *reinterpret_cast<const att_f32x4 *>(&sm_lse[buf][row]);
+      const att_f32x4 delta = *reinterpret_cast<const att_f32x4 *>(&sm_delta[buf][row]);
 #pragma unroll
-        for (int kc = 0; kc < KC; ++kc) {
-          const att_u32x4 q = cr_rows<D>(lq, rt, kc, lane), g = cr_rows<D>(lg, rt, kc, lane);
-#pragma unroll
-          for (int kt = 0; kt < KT; ++kt) {
-            s[kt] = T::mfma(q, k[kt][kc], s[kt]);
-            dp[kt] = T::mfma(g, VL ? cr_rows<D>(lv + (wave / 2) * CrLds<D>::BYTES, wave & 1, kc, lane) : v[kt][VL ? 0 : kc], dp[kt]);
-          }
-        }
-        att_u32x4 p[KT][2], ds[KT][2];
-#pragma unroll
-        for (int kt = 0; kt < KT; ++kt) {
-          const bool live = wk + 32 * kt + (lane & 31) < keys;
-          float x[16], y[16];
-#pragma unroll
-          for (int i4 = 0; i4 < 4; ++i4) {
-            const int row = 32 * rt + 8 * i4 + 4 * (lane >> 5);
-            const att_f32x4 lse = *reinterpret_cast<const att_f32x4 *>(&sm_lse[buf][row]);
-            const att_f32x4 delta = *reinterpret_cast<const att_f32x4 *>(&sm_delta[buf][row]);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const int i = 4 * i4 + j;
-              const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][i], scale, -lse[j]));
-              x[i] = live ? w : 0.0f;
-              y[i] = x[i] * unbias * (dp[kt][i] - delta[j]);
-            }
-          }
-          cr_operands<T>(x, p[kt]);
-          cr_operands<T>(y, ds[kt]);
-        }
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-          for (int dt = 0; dt < DT; ++dt) {
-            const att_u32x4 g = cr_cols<D>(lg, 2 * rt + c, dt, lane), q = cr_cols<D>(lq, 2 * rt + c, dt, lane);
-#pragma unroll
-            for (int kt = 0; kt < KT; ++kt) {
-              dv[kt][dt] = T::mfma(g, p[kt][c], dv[kt][dt]);
-              dk[kt][dt] = T::mfma(q, ds[kt][c], dk[kt][dt]);
-            }
-          }
+      for (int j = 0; j < 4; ++j) {
+        const int i = 4 * i4 + j;
+        const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], scale, -lse[j]));
+        x[i] = live ? w : 0.0f;
+        y[i] = x[i] * unbias * (dp[i] - delta[j]);
       }
     }
-    if (next < t_end) store(buf ^ 1, n_next);
-    __syncthreads();
-  }
+    cr_operands<T>(x, p);
+    cr_operands<T>(y, ds);
 #pragma unroll
-  for (int kt = 0; kt < KT; ++kt) {
-    const int key = wk + 32 * kt + (lane & 31);
-    if (key >= ks.n) continue;
-    const int64_t at = ((ks.lo + key) * a.n_kv_heads + it.h) * D + 4 * (lane >> 5);
-    const int64_t all = a.n_k * a.n_kv_heads * D;
+    for (int c = 0; c < 2; ++c)
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-      for (int i = 0; i < 16; i += 4) {
-        float x[4], y[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          x[j] = dk[kt][dt][i + j] * a.sm_scale;
-          y[j] = dv[kt][dt][i + j] * unbias;
-        }
-        const int64_t w = at + 32 * dt + 2 * i;
-        if (a.n_split == 1) {
-          *reinterpret_cast<uint2 *>(a.dk + w) = make_uint2(T::pack(x[0], x[1]), T::pack(x[2], x[3]));
-          *reinterpret_cast<uint2 *>(a.dv + w) = make_uint2(T::pack(y[0], y[1]), T::pack(y[2], y[3]));
-        } else {
-          float *pp = a.part + 2 * (int64_t)it.split * all + w;
-          *reinterpret_cast<float4 *>(pp) = make_float4(x[0], x[1], x[2], x[3]);
-          *reinterpret_cast<float4 *>(pp + all) = make_float4(y[0], y[1], y[2], y[3]);
-        }
+      for (int dt = 0; dt < DT; ++dt) {
+        dv[dt] = T::mfma(cr_cols<D>(lg, c, dt, lane), p[c], dv[dt]);
+        dk[dt] = T::mfma(cr_cols<D>(lq, c, dt, lane), ds[c], dk[dt]);
       }
-  }
+  };
+  cr_pipeline(t_begin, t_end, R, load, store, compute);
+  const int key = wk + (lane & 31);
+  if (key >= ks.n) return;
+  const int64_t at = ((ks.lo + key) * a.n_kv_heads + it.h) * D + 4 * (lane >> 5), all = a.n_k * a.n_kv_heads * D;
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+      float x[4], y[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        x[j] = dk[dt][i + j] * a.sm_scale;
+        y[j] = dv[dt][i + j] * unbias;
+      }
+      const int64_t w = at + 32 * dt + 2 * i;
+      if (a.n_split == 1) {
+        *reinterpret_cast<uint2 *>(a.dk + w) = make_uint2(T::pack(x[0], x[1]), T::pack(x[2], x[3]));
+        *reinterpret_cast<uint2 *>(a.dv + w) = make_uint2(T::pack(y[0], y[1]), T::pack(y[2], y[3]));
+      } else {
+        float *pp = a.part + 2 * (int64_t)it.split * all + w;
+        *reinterpret_cast<float4 *>(pp) = make_float4(x[0], x[1], x[2], x[3]);
+        *reinterpret_cast<float4 *>(pp + all) = make_float4(y[0], y[1], y[2], y[3]);
+      }
+    }
 }
 
 // Sums of the parts of a gradient, in order: [n_split] parts `step` floats apart, 8 values per thread.
@@ -808,6 +799,8 @@ struct CrossPlan {
   int ct;
   int64_t n_tile, n_split;
 };
+// Ranking the sequences costs every block about 1 us per 64 of them: for blocks of 16 tiles and more.
+static int32_t cr_order(int32_t n_seqs, int64_t length) { return n_seqs > 1 && n_seqs <= 64 && length >= 16 * CR_TILE; }
 static CrossPlan cr_plan(int64_t pairs, int64_t columns, int64_t length, int ct, int64_t per_cu, int64_t units_least) {
   CrossPlan p;
   p.ct = ct;
@@ -830,7 +823,7 @@ static CrossPlan cr_dq_plan(int32_t n_seqs, int32_t n_kv_heads, int32_t group, i
   return cr_plan((int64_t)n_seqs * n_kv_heads, (int64_t)max_q * group, max_k, 1, D == 64 ? 3 : 2, 4);
 }
 static CrossPlan cr_dkv_plan(int32_t n_seqs, int32_t n_kv_heads, int32_t group, int32_t D, int32_t max_q, int32_t max_k) {
-  return cr_plan((int64_t)n_seqs * n_kv_heads, max_k, (int64_t)max_q * group, 1, 2, 4);
+  return cr_plan((int64_t)n_seqs * n_kv_heads, max_k, (int64_t)max_q * group, 1, D == 64 ? 3 : 2, 4);
 }
 static bool cr_dims_ok(int64_t n_q, int64_t n_k, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim, int32_t n_seqs,
                        int32_t max_q, int32_t max_k) {
@@ -881,12 +874,22 @@ static int cr_check(const char *what, int dtype, const CrossArgs &a, int32_t hea
     return fail(ZX_ERR_UNSUPPORTED, "%s: too many rows", what);
   return ZX_OK;
 }
-// Strided rows: channels contiguous, every head's row 16-byte aligned.
-static int cr_check_rows(const char *what, const char *name, const CrIn &x) {
+// Strided rows: channels contiguous, every head's row 16-byte aligned, a tile's offsets below 2^31 bytes.
+static int cr_check_rows(const char *what, const char *name, const CrIn &x, int64_t group) {
   ZX_REQUIRE(x.p, "%s: null pointer", what);
   ZX_REQUIRE(aligned16(x.p) && x.row % 8 == 0 && x.head % 8 == 0 && x.row >= 0 && x.head >= 0,
              "%s: every row of a head of %s must be 16-byte aligned, with strides that are not negative", what, name);
+  if (x.row >= (1LL << 23) || (group > 1 && x.head >= (1LL << 29) / group))
+    return fail(ZX_ERR_UNSUPPORTED, "%s: strides of %s are too large", what, name);
   return ZX_OK;
+}
+
+static void cr_group(CrossArgs &a) {
+  a.group = a.n_q_heads / a.n_kv_heads;
+  int sh = 0;
+  while ((1LL << sh) < a.group) ++sh;
+  a.g_shift = sh;
+  a.g_magic = (uint32_t)(((1ULL << (31 + sh)) + (uint64_t)a.group - 1) / (uint64_t)a.group);
 }
 
 template <class T, int D> static int cr_forward(CrossArgs a, const CrossPlan &p, hipStream_t st) {
@@ -931,10 +934,10 @@ extern "C" int zx_cross_attention(int dtype, const void *q, int64_t n_q, int64_t
   if (rc) return rc;
   if (n_q == 0) return ZX_OK;
   a.max_q = (int32_t)std::min<int64_t>(max_q_per_seq, n_q);
-  a.group = n_q_heads / n_kv_heads;
+  cr_group(a);
   ZX_REQUIRE(cu_q && cu_k && out, "cross_attention: null pointer");
-  if ((rc = cr_check_rows("cross_attention", "q", a.q))) return rc;
-  if (n_k && ((rc = cr_check_rows("cross_attention", "k", a.k)) || (rc = cr_check_rows("cross_attention", "v", a.v))))
+  if ((rc = cr_check_rows("cross_attention", "q", a.q, a.group))) return rc;
+  if (n_k && ((rc = cr_check_rows("cross_attention", "k", a.k, 1)) || (rc = cr_check_rows("cross_attention", "v", a.v, 1))))
     return rc;
   ZX_REQUIRE(aligned16(out) && aligned16(workspace), "cross_attention: out and workspace must be 16-byte aligned");
   const CrossPlan p = cr_forward_plan(n_seqs, n_kv_heads, a.group, head_dim, a.max_q, max_k_per_seq);
@@ -943,6 +946,7 @@ extern "C" int zx_cross_attention(int dtype, const void *q, int64_t n_q, int64_t
                 cr_forward_bytes(p, n_q, n_q_heads, head_dim));
   a.n_tile = (int32_t)p.n_tile;
   a.n_split = (int32_t)p.n_split;
+  a.order = cr_order(n_seqs, a.max_k / p.n_split);
   if (8 * ceil_div((int64_t)n_seqs * n_kv_heads, 8) * p.n_tile * p.n_split >= (1LL << 31) - 1)
     return fail(ZX_ERR_UNSUPPORTED, "cross_attention: too many sequences");
   const hipStream_t st = as_stream(stream);
@@ -956,6 +960,7 @@ static int cr_backward(CrossArgs a, const CrossPlan &pq, const CrossPlan &pk, ui
   a.out = dq;
   a.n_tile = (int32_t)pq.n_tile;
   a.n_split = (int32_t)pq.n_split;
+  a.order = cr_order(a.n_seqs, a.max_k / pq.n_split);
   cross_dq_kernel<T, D><<<cr_grid(a) + 1, CR_THREADS, 0, st>>>(a);
   if ((rc = check_launch("cross_dq"))) return rc;
   const int64_t wq = (int64_t)a.n_q_heads * D, wk = (int64_t)a.n_kv_heads * D;
@@ -967,6 +972,7 @@ static int cr_backward(CrossArgs a, const CrossPlan &pq, const CrossPlan &pk, ui
   if (a.n_k == 0) return ZX_OK;
   a.n_tile = (int32_t)pk.n_tile;
   a.n_split = (int32_t)pk.n_split;
+  a.order = cr_order(a.n_seqs, (int64_t)a.max_q * a.group / pk.n_split);
   cross_dkv_kernel<T, D><<<cr_grid(a) + 1, CR_THREADS, 0, st>>>(a);
   if ((rc = check_launch("cross_dkv")) || pk.n_split == 1) return rc;
   for (int i = 0; i < 2; ++i) {
@@ -1010,15 +1016,15 @@ extern "C" int zx_cross_attention_backward(
   if (rc) return rc;
   a.max_q = (int32_t)std::min<int64_t>(max_q_per_seq, n_q);
   a.max_k = (int32_t)std::min<int64_t>(max_k_per_seq, n_k);
-  a.group = n_q_heads / n_kv_heads;
+  cr_group(a);
   if (n_q == 0 && n_k == 0) return ZX_OK;
   ZX_REQUIRE(cu_q && cu_k, "cross_attention_backward: null pointer");
-  if (n_q && ((rc = cr_check_rows("cross_attention_backward", "q", a.q)) ||
-              (rc = cr_check_rows("cross_attention_backward", "grad", a.g)) ||
-              (rc = cr_check_rows("cross_attention_backward", "out", a.o))))
+  if (n_q && ((rc = cr_check_rows("cross_attention_backward", "q", a.q, a.group)) ||
+              (rc = cr_check_rows("cross_attention_backward", "grad", a.g, a.group)) ||
+              (rc = cr_check_rows("cross_attention_backward", "out", a.o, a.group))))
     return rc;
-  if (n_k && ((rc = cr_check_rows("cross_attention_backward", "k", a.k)) ||
-              (rc = cr_check_rows("cross_attention_backward", "v", a.v))))
+  if (n_k && ((rc = cr_check_rows("cross_attention_backward", "k", a.k, 1)) ||
+              (rc = cr_check_rows("cross_attention_backward", "v", a.v, 1))))
     return rc;
   ZX_REQUIRE((!n_q || (dq && lse2)) && (!n_k || (dk && dv)), "cross_attention_backward: null pointer");
   ZX_REQUIRE(aligned16(dq) && aligned16(dk) && aligned16(dv) && aligned16(workspace),
