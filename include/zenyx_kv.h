@@ -576,9 +576,14 @@ int zx_paged_attention4_prefill(const uint16_t *q, int64_t n_q, const int32_t *c
  * FP8: scales [2][n_kv_heads]; softmax weights rounded once to fp16 (times 2^7; the row sums use
  * the same): |error| <= one bf16 ulp + 2^-10 max|V|.  4 bits: weights as bf16 hi + lo, one ulp +
  * 2^-15 max|V|.  A NaN value reaches the rows that see it.  workspace: the query's device bytes,
- * 16-byte aligned; it holds nothing between calls. */
+ * 16-byte aligned, for min(max_q_per_seq, n_q) rows per sequence (1 without cu_q); it holds nothing
+ * between calls. */
 size_t zx_paged_attention_shared_workspace_bytes(int64_t n_q, int32_t n_seqs, int32_t n_groups, int32_t n_q_heads,
-                                                 int32_t n_kv_heads, int32_t head_dim, int32_t max_q_per_seq);
+                                                 int32_t n_kv_heads, int32_t head_dim, int32_t page_size,
+                                                 int32_t max_blocks, int32_t max_q_per_seq);
+size_t zx_paged_attention4_shared_workspace_bytes(int64_t n_q, int32_t n_seqs, int32_t n_groups, int32_t n_q_heads,
+                                                  int32_t n_kv_heads, int32_t head_dim, int32_t page_size,
+                                                  int32_t max_blocks, int32_t max_q_per_seq);
 int zx_paged_attention_shared(const uint16_t *q, int64_t n_q, const int32_t *cu_q, int32_t n_q_heads,
                               const uint8_t *pool, int64_t n_pages, int32_t n_kv_heads, int32_t head_dim,
                               int32_t page_size, const float *scales, const int32_t *block_tables, int32_t max_blocks,

@@ -19,6 +19,7 @@
 // read a page while it is in the XCD's L2.
 #include <algorithm>
 
+#include "zx_attn_tile.h"
 #include "zx_attn_wave.h"
 #include "zx_internal.h"
 
@@ -44,6 +45,7 @@ struct SharedArgs {
   int32_t n_rt;            // row tiles of a sequence at most
   int32_t n_run;           // blocks per group of heads
   uint32_t cap;            // positions that a block table holds
+  float cost_p;            // of a group's unit, in own units
   uint32_t p_magic;
   int32_t p_shift;
   float sm_scale;
@@ -149,7 +151,7 @@ __device__ __forceinline__ uint32_t sh_wave_scan(uint32_t v) {
 
 // How a call is dealt.
 constexpr int SH_CAND = 8;
-constexpr int SH_STAGE = 512;  // sequences (and groups) whose lengths are kept in LDS
+constexpr int SH_STAGE = 256;  // sequences (and groups) whose lengths are kept in LDS
 struct ShPlan {
   uint32_t n_pre;  // blocks (per group of heads) for the groups' tiles
   uint32_t n_seg;  // pieces of them
@@ -223,11 +225,8 @@ __device__ __forceinline__ ShPlan sh_plan(const SharedArgs &a, ShLds &lds, int32
   }
   sh_sums<2>(pq, lds);
   const uint32_t P = pq[0], Q = pq[1], n = (uint32_t)a.n_run;
-  // Blocks in the proportion of the units: a group's unit is bound by its products and an own one
-  // by its reads, and they take about as long as each other (a group's counted for 2 / 1.25 / 1 / 0.75
-  // own ones: 64 sequences on 2,048 shared positions and 100-2,000 each 54 / 51 / 52 / 51 us, 50 rows
-  // of 4-bit pages in 4 groups on 4k-16k shared ones 112 / 79 / 79 / 79).
-  const float share = (float)P / ((float)P + (float)Q);
+  // blocks in the proportion of the work
+  const float wp = (float)P * a.cost_p, share = wp / (wp + (float)Q);
   p.n_pre = P == 0 ? 0u : Q == 0 ? n : (uint32_t)max(1, min((int)n - 1, (int)((float)n * share + 0.5f)));
   p.n_pre = sh_uni(p.n_pre);
   p.piece = 1;
@@ -409,15 +408,209 @@ __device__ __forceinline__ void sh_segment(const SharedArgs &a, const AttnPages 
   }
 }
 
-// Blocks per CU by the registers of CT tiles of columns, and (D = 128) by LDS.
-__host__ __device__ constexpr int sh_per_cu(int D, int CT) { return D * CT > 128 ? 2 : CT > 1 || D == 128 ? 3 : 4; }
+// A tile of 64 keys of a head in flight from FP8 pages to LDS: a thread has N pieces of 16 codes of K
+// rows and as many of V, converts them on the way, and has its rows' page ids a tile ahead.
+constexpr int SW_TILE = 64, SW_COLS = 32 * CR_WAVES;
+template <int D> struct ShStage {
+  static constexpr int PER_ROW = D / 16, N = SW_TILE * PER_ROW / CR_THREADS, STEP = CR_THREADS / PER_ROW;
+  static_assert(N * CR_THREADS == SW_TILE * PER_ROW, "pieces dealt evenly");
+  uint4 k[N], v[N];
+  int32_t id[N];
+  bool good[N];
+  static __device__ __forceinline__ int row(int i) { return (int)threadIdx.x / PER_ROW + i * STEP; }
+  static __device__ __forceinline__ int part() { return (int)threadIdx.x % PER_ROW; }
+  // The pages of the thread's rows in the tile at t (positions from t_end on: of the last one).
+  __device__ __forceinline__ void page(const AttnPages &pg, uint32_t t, uint32_t t_end) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) id[i] = pg.bt[pg.page_of(min(t + (uint32_t)row(i), t_end - 1))];
+  }
+  __device__ __forceinline__ void load(const AttnPages &pg, uint32_t t, uint32_t t_end) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const uint32_t at = min(t + (uint32_t)row(i), t_end - 1), in = at - pg.page_of(at) * pg.page_size;
+      good[i] = id[i] >= 0 && id[i] < pg.n_pages;
+      // (a bad page: the pool's first, whose codes are not used)
+      const uint8_t *p = pg.pool + (int64_t)(good[i] ? id[i] : 0) * pg.page_bytes + pg.head_off + in * D + 16 * part();
+      k[i] = *reinterpret_cast<const uint4 *>(p);
+      v[i] = *reinterpret_cast<const uint4 *>(p + pg.v_off);
+    }
+  }
+};
+template <bool F16> __device__ __forceinline__ void sh_codes(uint4 c, att_u32x4 &lo, att_u32x4 &hi) {
+  const uint32_t x[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+  for (int n = 0; n < 4; ++n) {
+    lo[n] = F16 ? aw_f16_of(x[n / 2], n & 1) : aw_bf16_of(x[n / 2], n & 1);
+    hi[n] = F16 ? aw_f16_of(x[2 + n / 2], n & 1) : aw_bf16_of(x[2 + n / 2], n & 1);
+  }
+}
+
+// Up to 128 columns on keys [t_begin, t_end) of FP8 pages, all of which every row sees.  A wave has 32
+// columns, and the four share tiles of 64 keys in LDS: a key is read and converted once per 128
+// columns, where AttnWave's waves, with 48 columns and keys of their own, convert it for each 48 (D =
+// 128, 64 sequences on 2,048 shared positions and 100-2,000 of their own 53 us, so 46; the other way
+// D = 64, 12 heads, 64 sequences on 16,384 28 us, so 36, and 4 bits, whose second product is twice as long,
+// 50 rows in 4 groups 74 us, so 92).
+struct ShWideLds {
+  static constexpr int D = 128;
+  uint8_t k[2][SW_TILE * CrRowsOnly<D>::ROW];
+  uint8_t v[2][CrLds<D, SW_TILE>::BYTES];
+  uint8_t ok[2][4];  // are the 16-token quarters of a tile on pages that exist?
+};
+template <class Part>
+__device__ __forceinline__ void sh_wide(const SharedArgs &a, const AttnPages &pg, float scale, int G, int hq0, int64_t row0,
+                                        int cols, uint32_t t_begin, uint32_t t_end, ShWideLds &lds, int32_t &e, Part part) {
+  constexpr int D = ShWideLds::D, KC = D / 16, DT = D / 32;
+  using KRows = CrRowsOnly<D>;
+  using T = CrF16;
+  static_assert(T::BIAS == Page8<D>::BIAS, "parts of both kinds of segment are merged");
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = 32 * wave + (lane & 31);
+  const bool work = 32 * wave < cols, live = col < cols;
+  const int r = live ? col / G : 0, hq = hq0 + (live ? col - r * G : 0);
+  AttnScale qs(scale);
+  att_u32x4 q[KC];
+  {
+    const uint16_t *p = a.q + ((row0 + r) * a.n_q_heads + hq) * D + 8 * (lane >> 5);
+#pragma unroll
+    for (int kc = 0; kc < KC; ++kc) {
+      q[kc] = *reinterpret_cast<const att_u32x4 *>(p + 16 * kc);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) q[kc][i] = live ? (q[kc][i] ^ qs.flip) & qs.keep : 0u;
+    }
+  }
+  cr_f32x16 o[DT];
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) o[dt] = cr_zero();
+  float m = CR_NONE, top = CR_NONE, l = 0.0f;
+  ShStage<D> st;
+  auto load = [&](uint32_t t) {
+    st.load(pg, t, t_end);
+    if (t + SW_TILE < t_end) st.page(pg, t + SW_TILE, t_end);
+  };
+  auto store = [&](int buf, uint32_t t) {
+#pragma unroll
+    for (int i = 0; i < ShStage<D>::N; ++i) {
+      const int row = ShStage<D>::row(i);
+      // rows past the end, and those on bad pages, as zeros
+      const bool there = st.good[i] && t + (uint32_t)row < t_end;
+      const uint4 z = make_uint4(0u, 0u, 0u, 0u);
+      att_u32x4 x, y;
+      sh_codes<false>(there ? st.k[i] : z, x, y);
+      uint8_t *k = KRows::at(lds.k[buf], row, 32 * ShStage<D>::part());
+      *reinterpret_cast<att_u32x4 *>(k) = x;
+      *reinterpret_cast<att_u32x4 *>(k + 16) = y;
+      sh_codes<true>(there ? st.v[i] : z, x, y);
+      *reinterpret_cast<att_u32x4 *>(cr_at<D>(lds.v[buf], row, 32 * ShStage<D>::part())) = x;
+      *reinterpret_cast<att_u32x4 *>(cr_at<D>(lds.v[buf], row, 32 * ShStage<D>::part() + 16)) = y;
+      if (ShStage<D>::part() == 0 && row % 16 == 0) {
+        lds.ok[buf][row / 16] = st.good[i];
+        if (!st.good[i] && t + (uint32_t)row < t_end) e |= ZX_KERR_PAGE_RANGE;
+      }
+    }
+  };
+  auto compute = [&](int buf, uint32_t t) {
+    if (!work) return;
+    const uint8_t *lk = KRows::at(lds.k[buf], lane & 31, 16 * (lane >> 5));
+    uint8_t *lv = lds.v[buf];
+    cr_f32x16 s[2];
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+      s[kt] = cr_zero();
+#pragma unroll
+      for (int kc = 0; kc < KC; ++kc)
+        s[kt] = CrBf16::mfma(*reinterpret_cast<const att_u32x4 *>(lk + 32 * kt * KRows::ROW + 32 * kc), q[kc], s[kt]);
+    }
+    const uint32_t ok = *reinterpret_cast<const uint32_t *>(lds.ok[buf]);
+    if (t + SW_TILE > t_end || __builtin_amdgcn_readfirstlane((int)ok) != 0x01010101) {  // uniform
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int row = 32 * kt + cr_row(i, lane);
+          if (t + row >= t_end || !((ok >> (8 * (row / 16))) & 1u)) s[kt][i] = -INFINITY;
+        }
+    }
+    float mx = s[0][0];
+#pragma unroll
+    for (int i = 1; i < 32; ++i) mx = __builtin_elementwise_maximum(mx, s[i / 16][i % 16]);
+    if (__builtin_amdgcn_ballot_w64(mx > top)) {
+      const float m_new = fmaxf(m, cr_halves_max(mx) * qs.f - T::BIAS), alpha = __builtin_amdgcn_exp2f(m - m_new);
+      m = m_new;
+      top = (m_new + (CR_LAZY + T::BIAS)) / qs.f;
+      l *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[dt][i] *= alpha;
+    }
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+      float x[16];
+      att_u32x4 p[2];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][i], qs.f, -m));
+        l += x[i];
+      }
+      cr_operands<T>(x, p);
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[dt] = T::mfma(cr_cols<D>(lv, 2 * kt + c, dt, lane), p[c], o[dt]);
+    }
+  };
+  if (t_begin < t_end) {
+    st.page(pg, t_begin, t_end);
+    load(t_begin);
+    store(0, t_begin);
+    __syncthreads();
+    int buf = 0;
+    for (uint32_t t = t_begin; t < t_end; t += SW_TILE, buf ^= 1) {
+      if (t + SW_TILE < t_end) load(t + SW_TILE);
+      compute(buf, t);
+      if (t + SW_TILE < t_end) store(buf ^ 1, t + SW_TILE);
+      __syncthreads();
+    }
+  }
+  const float sum = cr_halves_sum(l);
+  if (!live) return;
+  float *pp = part(r) + (int64_t)hq * (2 + D);
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int i = 0; i < 16; i += 2)
+      *reinterpret_cast<float2 *>(pp + 2 + 32 * dt + cr_row(i, lane)) = make_float2(o[dt][i], o[dt][i + 1]);
+  if (lane < 32) *reinterpret_cast<float2 *>(pp) = make_float2(m, sum);
+}
+
+// Tiles of 16 columns of a group that a block takes at most: by AttnWave what leaves two waves per
+// SIMD, of FP8 pages at D = 128 SH_WIDE (128 columns) by sh_wide instead.
+constexpr int SH_WIDE = SW_COLS / AW_COLS;
+__host__ __device__ constexpr int sh_most_tiles(int bits, int D) {
+  return D == 256 ? 1 : D == 64 ? 4 : bits == 8 ? SH_WIDE : 3;
+}
+// Blocks per CU by the registers, and (D = 128) by LDS.
+__host__ __device__ constexpr int sh_per_cu(int D, int CT) {
+  return D * CT > 128 ? 2 : CT > 1 || D == 128 ? 3 : 4;
+}
 
 // CTO: column tiles of a sequence's own keys.  ROWS: several rows per sequence.
 template <class F, int CT, int CTO, bool EXACT, bool ROWS>
 __global__ void __launch_bounds__(ATT_THREADS, sh_per_cu(F::DIM, CT)) paged_shared_kernel(SharedArgs a) {
   constexpr int D = F::DIM;
-  __shared__ __attribute__((aligned(16))) uint8_t lds[ATT_WAVES][AttnLds<D>::WAVE];
-  __shared__ float sm_m[ATT_WAVES][AW_COLS], sm_l[ATT_WAVES][AW_COLS];
+  struct Narrow {
+    uint8_t lds[ATT_WAVES][AttnLds<D>::WAVE];
+    float m[ATT_WAVES][AW_COLS], l[ATT_WAVES][AW_COLS];
+  };
+  union Lds {  // one segment after the other
+    Narrow n;
+    ShWideLds w;
+  };
+  __shared__ __attribute__((aligned(256))) uint8_t raw[CT == SH_WIDE ? sizeof(Lds) : sizeof(Narrow)];
+  Lds &u_lds = *reinterpret_cast<Lds *>(raw);
+  auto &lds = u_lds.n.lds;
+  auto &sm_m = u_lds.n.m, &sm_l = u_lds.n.l;
   __shared__ ShLds sh;
   int32_t e = 0;
   sh_stage(a, sh);
@@ -488,14 +681,20 @@ __global__ void __launch_bounds__(ATT_THREADS, sh_per_cu(F::DIM, CT)) paged_shar
       // every row sees all of the piece?  (Otherwise a tile of columns at a time.)
       bool all = true;
       for (int r = threadIdx.x & 63; r < n_rows; r += 64) all &= lim(r) >= t_end;
-      if (!__builtin_amdgcn_ballot_w64(!all)) {
+      const bool plain = !__builtin_amdgcn_ballot_w64(!all);
+      if constexpr (CT == SH_WIDE) {
+        if (plain) {
+          sh_wide(a, pg, scale, G, hq0, row0, cols, t_begin, t_end, u_lds.w, e, part);
+          continue;
+        }
+      } else if (plain) {
         sh_segment<F, CT, EXACT, 0, false>(a, pg, scale, G, hq0, row0, 0, cols, t_begin, t_end, lds, sm_m, sm_l, e, lim,
                                            part);
-      } else {
-        for (int c0 = 0; c0 < cols; c0 += AW_COLS)
-          sh_segment<F, 1, EXACT, 0, true>(a, pg, scale, G, hq0, row0, c0, min(AW_COLS, cols - c0), t_begin, t_end, lds,
-                                           sm_m, sm_l, e, lim, part);
+        continue;
       }
+      for (int c0 = 0; c0 < cols; c0 += AW_COLS)
+        sh_segment<F, 1, EXACT, 0, true>(a, pg, scale, G, hq0, row0, c0, min(AW_COLS, cols - c0), t_begin, t_end, lds, sm_m,
+                                         sm_l, e, lim, part);
     }
   } else {
     const uint32_t xo = x - p.n_pre;
@@ -616,32 +815,31 @@ template <int D> __global__ void __launch_bounds__(256) shared_combine_kernel(Sh
 
 using namespace zx;
 
-// Tiles of 16 columns that a block can hold.
-static int sh_most_tiles(int D) { return D == 64 ? 4 : D == 128 ? 3 : 1; }
-
 struct SharedHost {
   int ct, ct_own;
   int32_t group, n_group, rows_p, rows_o, n_rt;
   int64_t n_run, pre_slots, own_slots;
   size_t part_bytes, bytes;
 };
-static SharedHost sh_host(int64_t n_q, int32_t n_seqs, int32_t n_groups, int32_t n_q_heads, int32_t n_kv_heads,
-                          int32_t head_dim, int32_t most) {
+static SharedHost sh_host(int bits, int64_t n_q, int32_t n_seqs, int32_t n_groups, int32_t n_q_heads, int32_t n_kv_heads,
+                          int32_t head_dim, int32_t max_blocks, int32_t page_size, int32_t most) {
   SharedHost p;
   const int64_t grp = n_q_heads / n_kv_heads, subs = ceil_div(grp, AW_COLS);
   p.group = (int32_t)ceil_div(grp, subs);
   p.n_group = (int32_t)(n_kv_heads * subs);
-  // column tiles per block: by the columns of a group on average, of a sequence at most
-  const int tiles = sh_most_tiles(head_dim);
-  const int64_t cols = ceil_div(n_q, std::max(n_groups, 1)) * p.group;
-  p.ct = n_groups == 0 || cols <= 16 || tiles == 1 ? 1 : cols <= 32 ? 2 : tiles;
-  const int64_t own = (int64_t)most * p.group;
+  // columns per block: by those of a group on average, and of a sequence at most
+  const int64_t cols = n_groups ? ceil_div(n_q, n_groups) * p.group : 0, own = (int64_t)most * p.group;
+  const int tiles = sh_most_tiles(bits, head_dim);
+  p.ct = tiles == 1 || cols <= 16 ? 1 : cols <= 32 ? 2 : tiles;
   if (own > 16 && p.ct == 1 && tiles > 1) p.ct = 2;
   p.ct_own = most == 1 || p.ct == 1 ? 1 : 2;
   p.rows_p = 16 * p.ct / p.group;
   p.rows_o = (int32_t)std::min<int64_t>(most, 16 * p.ct_own / p.group);
   p.n_rt = (int32_t)ceil_div(most, p.rows_o);
-  p.n_run = std::max<int64_t>(2, (int64_t)sh_per_cu(head_dim, p.ct) * num_cus() / p.n_group);
+  // as many blocks as the chip holds, or as there can be units (768 blocks without one cost a call 4 us)
+  const int64_t units = ceil_div((int64_t)max_blocks * page_size, SH_UNIT);
+  const int64_t most_units = units * ((int64_t)n_seqs * p.n_rt + ceil_div(n_q, p.rows_p) + n_groups);
+  p.n_run = std::max<int64_t>(2, std::min<int64_t>(sh_per_cu(head_dim, p.ct) * num_cus() / p.n_group, most_units));
   p.pre_slots = n_groups ? n_q + 2 * (p.n_run + 1) * p.rows_p : 0;
   p.own_slots = (p.n_run + (int64_t)n_seqs * p.n_rt) * p.rows_o;
   p.part_bytes = (size_t)((p.pre_slots + p.own_slots) * n_q_heads * (2 + head_dim)) * sizeof(float);
@@ -654,11 +852,21 @@ static bool sh_dims_ok(int64_t n_q, int32_t n_seqs, int32_t n_groups, int32_t n_
          most > 0 && (head_dim == 64 || head_dim == 128 || head_dim == 256);
 }
 
+static size_t sh_bytes(int bits, int64_t n_q, int32_t n_seqs, int32_t n_groups, int32_t n_q_heads, int32_t n_kv_heads,
+                       int32_t head_dim, int32_t page_size, int32_t max_blocks, int32_t most) {
+  if (!sh_dims_ok(n_q, n_seqs, n_groups, n_q_heads, n_kv_heads, head_dim, most) || page_size <= 0 || max_blocks <= 0) return 0;
+  return sh_host(bits, n_q, n_seqs, n_groups, n_q_heads, n_kv_heads, head_dim, max_blocks, page_size, most).bytes;
+}
 extern "C" size_t zx_paged_attention_shared_workspace_bytes(int64_t n_q, int32_t n_seqs, int32_t n_groups,
                                                             int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim,
-                                                            int32_t max_q_per_seq) {
-  if (!sh_dims_ok(n_q, n_seqs, n_groups, n_q_heads, n_kv_heads, head_dim, max_q_per_seq)) return 0;
-  return sh_host(n_q, n_seqs, n_groups, n_q_heads, n_kv_heads, head_dim, max_q_per_seq).bytes;
+                                                            int32_t page_size, int32_t max_blocks, int32_t max_q_per_seq) {
+  return sh_bytes(8, n_q, n_seqs, n_groups, n_q_heads, n_kv_heads, head_dim, page_size, max_blocks, max_q_per_seq);
+}
+extern "C" size_t zx_paged_attention4_shared_workspace_bytes(int64_t n_q, int32_t n_seqs, int32_t n_groups,
+                                                             int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim,
+                                                             int32_t page_size, int32_t max_blocks,
+                                                             int32_t max_q_per_seq) {
+  return sh_bytes(4, n_q, n_seqs, n_groups, n_q_heads, n_kv_heads, head_dim, page_size, max_blocks, max_q_per_seq);
 }
 
 template <class F, int CT, int CTO, bool EXACT, bool ROWS> static int sh_launch(const SharedArgs &a, hipStream_t st) {
@@ -687,7 +895,9 @@ static int sh_call(const char *what, SharedArgs a, int32_t head_dim, int32_t max
   ZX_REQUIRE(aligned16(a.q) && aligned16(a.pool) && aligned16(a.out) && aligned16(workspace),
              "%s: q, pool, out and workspace must be 16-byte aligned", what);
   a.most = a.cu_q ? (int32_t)std::min<int64_t>(max_q_per_seq, a.n_q) : 1;
-  const SharedHost p = sh_host(a.n_q, a.n_seqs, a.n_groups, a.n_q_heads, a.n_kv_heads, head_dim, a.most);
+  constexpr int BITS = Page<64>::BITS;
+  const SharedHost p = sh_host(BITS, a.n_q, a.n_seqs, a.n_groups, a.n_q_heads, a.n_kv_heads, head_dim, a.max_blocks,
+                               a.page_size, a.most);
   if (a.n_q * a.n_q_heads >= (1LL << 31) || (int64_t)a.n_seqs * p.n_rt >= (1LL << 31))
     return fail(ZX_ERR_UNSUPPORTED, "%s: too many rows", what);
   // units are counted in 32 bits
@@ -707,6 +917,11 @@ static int sh_call(const char *what, SharedArgs a, int32_t head_dim, int32_t max
   a.rows_o = p.rows_o;
   a.n_rt = p.n_rt;
   a.n_run = (int32_t)p.n_run;
+  // A group's unit is bound by its products, an own one by its reads: up to 4 tiles of columns take about as
+  // long as an own unit (50 rows of 4-bit pages in 4 groups on 4k-16k shared positions, a group's unit
+  // counted for 2 / 1 / 0.75 own ones: 112 / 79 / 79 us), 128 columns three times that (128 sequences on
+  // 32k shared positions, counted for 2 / 3 / 4: 132 / 125 / 124 us).
+  a.cost_p = p.ct == SH_WIDE ? 3.0f : 1.0f;
   a.cap = (uint32_t)((int64_t)a.max_blocks * a.page_size);
   {  // magic division by the page size for positions below 2^31
     int sh = 0;
@@ -717,8 +932,8 @@ static int sh_call(const char *what, SharedArgs a, int32_t head_dim, int32_t max
   const hipStream_t st = as_stream(stream);
 #define ZX_SH(D, CT, CTO) (a.most > 1 ? sh_launch<Page<D>, CT, CTO, EXACT, true>(a, st) : sh_launch<Page<D>, CT, 1, EXACT, false>(a, st))
   switch (head_dim) {
-    case 64: return p.ct == 1 ? ZX_SH(64, 1, 1) : p.ct == 2 ? ZX_SH(64, 2, 2) : ZX_SH(64, 4, 2);
-    case 128: return p.ct == 1 ? ZX_SH(128, 1, 1) : p.ct == 2 ? ZX_SH(128, 2, 2) : ZX_SH(128, 3, 2);
+    case 64: return p.ct == 1 ? ZX_SH(64, 1, 1) : p.ct == 2 ? ZX_SH(64, 2, 2) : ZX_SH(64, sh_most_tiles(BITS, 64), 2);
+    case 128: return p.ct == 1 ? ZX_SH(128, 1, 1) : p.ct == 2 ? ZX_SH(128, 2, 2) : ZX_SH(128, sh_most_tiles(BITS, 128), 2);
     default: return ZX_SH(256, 1, 1);
   }
 #undef ZX_SH

@@ -1276,7 +1276,7 @@ def _attention_shared(what, q, pool_layer, scales_layer, block_tables, seq_lens,
         mq = int(max_q_per_seq)
     mq = max(0, min(mq, n_q))
     with _on(index):
-        ws, nb = _workspace_for("zx_paged_attention_shared_workspace_bytes", index, n_q, B, n_groups, Hq, Hkv, D, mq)
+        ws, nb = _workspace_for(f"zx_{what}_workspace_bytes", index, n_q, B, n_groups, Hq, Hkv, D, P, mb, mq)
         err = _err_word_if(check, q.device) if err is None else err
         entry = N.load().zx_paged_attention4_shared if scales_layer is None else N.load().zx_paged_attention_shared
         N.check(entry(
