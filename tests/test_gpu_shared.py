@@ -183,3 +183,211 @@ def test_against_float64(dev, bits, shape):
         t.check(t.call(cu_q=True, max_q_per_seq=1, check=True))
     else:
         t.check(t.call(causal=False, check=True), causal=False)
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("groups, loose, rows", [
+    ([(300, 64)], [], 1),                                # more sequences than the kernel keeps in LDS
+    ([(1, 16)] * 280 + [(30, 128)], [5] * 7, 1),         # and more groups
+    ([(150, 80), (120, 48)], [200, 0, 3], 2)])
+def test_many_sequences(dev, bits, groups, loose, rows):
+    n = sum(c for c, _ in groups)
+    own = [rows + i % 37 for i in range(n)]
+    r = [rows if i % 3 else 1 for i in range(n + len(loose))]
+    t = Batch(dev, bits, groups, own, r, 8, 2, 64, 16, seed=3, loose=loose)
+    t.check(t.call(check=True))
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("D, loose", [(128, [40, 0, 300]), (64, [1])])
+def test_sequences_in_no_group(dev, bits, D, loose):
+    t = Batch(dev, bits, [(3, 128)], [5, 60, 200], [1] * (3 + len(loose)), 8, 2, D, 16, loose=loose)
+    want = t.call(cu_q=False, check=True)
+    t.check(want)
+    # no groups at all: attention over each sequence's own table
+    t.cu_group, t.shared = i32([0], dev), i32([], dev)
+    t.check(t.call(cu_q=False, check=True))
+    # a group of which nothing is shared, one of each alone, and all that one has in common
+    for cu, s in (([0, 3], [0]), ([0, 1, 2, 3], [128, 128, 128]), ([0, 2, 3], [128, 0]), ([0, 3], [100]), ([0, 3], [15])):
+        t.cu_group, t.shared = i32(cu, dev), i32(s, dev)
+        t.check(t.call(cu_q=False, check=True))
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("sm", [-0.11, 0.0, 1.0])
+def test_other_scales(dev, bits, sm):
+    for rows in ([1] * 6, [2, 1, 5, 3, 1, 4]):
+        t = Batch(dev, bits, [(6, 192)], [9, 30, 5, 70, 6, 20], rows, 16, 4, 128, 16, seed=5)
+        t.check(t.call(sm_scale=sm, check=True), sm=sm)
+
+
+@pytest.mark.parametrize("n", [20, 6])
+def test_negative_fp8_scales(dev, n):
+    t = Batch(dev, 8, [(n, 160)], list(range(n)), [1] * n, 16, 4, 128, 16, seed=6)
+    t.scales[0, 1] *= -1
+    t.scales[1, 2] *= -1
+    t.check(t.call(cu_q=False, check=True))
+
+
+def nan_at(t, b, pos, head, ch, kv_):
+    """Makes channel ch (4 bits: its block) of position pos of sequence b a NaN."""
+    page = int(t.bt_np[b, pos // t.P])
+    if t.bits == 8:
+        t.pool[page, kv_, head, pos % t.P, ch] = 0xFF
+    else:
+        t.pool[page, kv_, head, (pos % t.P) // 16, 8 * t.D + 16 * (ch // 32) + pos % 16] = 255
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("D, n", [(64, 3), (128, 3), (128, 18)])
+def test_nan_values_reach_the_rows_that_see_them(dev, bits, D, n):
+    """Of the shared keys and of a sequence's own, at positions that some rows do not see; behind the last
+    position of a sequence they reach none."""
+    rows = [8, 3, 1] + [2] * (n - 3)
+    t = Batch(dev, bits, [(n, 96)], [8, 37, 5] + [10] * (n - 3), rows, 8, 2, D, 16, seed=9)
+    nan_at(t, 0, 40, 0, 5, 1)               # everyone's
+    nan_at(t, 0, 96 + 4, 1, 33, 1)          # seen by rows 4 .. of sequence 0
+    nan_at(t, 1, 96 + 36, 0, D - 1, 1)      # by the last row of sequence 1
+    for pos in range(96 + 5, 112):          # behind sequence 2's last position, on its page
+        nan_at(t, 2, pos, 1, 0, 1)
+        nan_at(t, 2, pos, 0, 3, 0)
+    t.check(t.call(check=True))
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("n", [2, 24])
+def test_nan_keys(dev, bits, n):
+    t = Batch(dev, bits, [(n, 64)], [20] * n, [1] * n, 8, 2, 128, 16, seed=10)
+    nan_at(t, 1, 64 + 3, 1, 7, 0)  # a key of sequence 1 alone: its rows of that KV head
+    got = t.call(cu_q=False, check=True)
+    bad = got.isnan().view(n, 2, 4, 128)
+    assert bad[1, 1].all() and not bad[1, 0].any() and not bad[0].any()
+    nan_at(t, 0, 9, 0, 7, 0)  # a shared one: every row of the other
+    bad = t.call(cu_q=False, check=True).isnan().view(n, 2, 4, 128)
+    assert bad[:, 0].all() and not bad[0, 1].any()
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("n", [2, 24])
+def test_bad_pages_are_left_out_and_flagged(dev, bits, n):
+    t = Batch(dev, bits, [(n, 128)], [40] * n, [1] * n, 8, 2, 128, 16, seed=11)
+    good = t.call(cu_q=False, check=True)
+    for b, col, bad in ((0, 3, -1), (0, 3, t.n_pages), (1, 8, -7), (1, 8, 1 << 30)):
+        keep = int(t.bt[b, col])
+        t.bt[b, col] = bad
+        err = torch.zeros(1, dtype=torch.int32, device=dev)
+        got = t.call(cu_q=False, err=err)
+        assert int(err) == N.ZX_KERR_PAGE_RANGE and torch.isfinite(got).all()
+        with pytest.raises(ValueError, match="block table"):
+            t.call(cu_q=False, check=True)
+        touched = (got != good).flatten(1).any(1)
+        assert touched.all() if b == 0 else touched.tolist() == [i == 1 for i in range(n)]
+        t.bt[b, col] = keep
+    assert torch.equal(t.call(cu_q=False, check=True), good)
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+def test_what_groups_and_lengths_flag(dev, bits):
+    t = Batch(dev, bits, [(4, 64), (3, 32)], [5] * 7, [1] * 7, 8, 2, 64, 16, seed=12)
+    for cu, lens in (([0, 5, 4], None), ([-1, 4, 7], None), ([0, 4, 9], None), ([0, 6, 2], None), ([3, 0, 7], None),
+                     ([0, 4, 7], 1 << 20)):
+        t.cu_group = i32(cu, dev)
+        s = t.seq_lens.clone()
+        if lens:
+            s[2] = lens
+        args = [t.q, t.pool] + ([t.scales] if bits == 8 else []) + [t.bt, s, t.cu_group, t.shared]
+        with pytest.raises(ValueError, match="position"):
+            (kv.paged_attention_shared if bits == 8 else kv.paged_attention4_shared)(*args, check=True)
+    # rows beyond max_q_per_seq: not computed, left as they are
+    t = Batch(dev, bits, [(3, 64)], [20] * 3, [2, 5, 1], 8, 2, 64, 16, seed=13)
+    out = torch.full_like(t.q, 7.0)
+    err = torch.zeros(1, dtype=torch.int32, device=dev)
+    t.call(max_q_per_seq=3, out=out, err=err)
+    assert int(err) == N.ZX_KERR_POS_RANGE
+    assert (out[5:7] == 7).all() and (out[:5] != 7).any(-1).any(-1).all() and (out[7] != 7).any()
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+def test_rows_in_no_sequence_are_left(dev, bits):
+    t = Batch(dev, bits, [(3, 64)], [20] * 3, [2, 0, 3], 8, 2, 64, 16, seed=14, behind=4)
+    out = torch.full_like(t.q, 7.0)
+    t.call(out=out, check=True)
+    t.check(out)
+    assert (out[5:] == 7).all()
+    empty = torch.empty((0, 8, 64), dtype=torch.bfloat16, device=dev)
+    t.q, t.cu_q = empty, i32([0, 0, 0, 0], dev)
+    assert t.call(check=True).shape == empty.shape
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("n, D", [(3, 64), (30, 128)])
+def test_captured_replays_follow_the_lengths(dev, bits, n, D):
+    """One captured call on other lengths, groups and pages, with eager work between the replays, and on
+    another stream; twice at once on streams of their own."""
+    t = Batch(dev, bits, [(n, 640)], [64] * n, [1] * n, 8, 2, D, 16, seed=15)
+    out = torch.empty_like(t.q)
+    t.call(cu_q=False, out=out)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        t.call(cu_q=False, out=out)
+    for k, (own, shared, cu) in enumerate(((64, 640, [0, n]), (3, 640, [0, n]), (50, 48, [0, n]), (64, 0, [0, n]),
+                                           (17, 320, [0, n - 1]), (64, 640, [0, n]))):
+        t.lens = [640 + own - i % 3 for i in range(n)]
+        t.seq_lens.copy_(i32(t.lens, dev))
+        t.shared.copy_(i32([shared], dev))
+        t.cu_group.copy_(i32(cu, dev))
+        t.q.mul_(-1.0)
+        out.zero_()
+        graph.replay()
+        t.check(out)
+        assert torch.equal(out, t.call(cu_q=False))  # the same launch: the same sums in the same order
+    streams = [torch.cuda.Stream(dev) for _ in range(2)]
+    want = out.clone()
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(4):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(t.call(cu_q=False))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want) for g in got)
+
+
+def test_pools_beyond_4_gib(dev):
+    """Pages whose bytes lie beyond 2^32, FP8 and 4 bits, of wide and narrow groups."""
+    for bits, D, n in ((8, 128, 20), (8, 64, 3), (4, 128, 3)):
+        t = Batch(dev, bits, [(n, 96)], [20] * n, [1] * n, 8, 2, D, 16, seed=16)
+        page = t.pool[0].numel()
+        far = torch.zeros((5 * 2 ** 30 // page, *t.pool.shape[1:]), dtype=torch.uint8, device=dev)
+        shift = far.shape[0] - t.n_pages
+        far[shift:] = t.pool
+        want = t.call(cu_q=False)
+        t.pool, t.bt = far, torch.where(t.bt >= 0, t.bt + shift, t.bt)
+        assert torch.equal(t.call(cu_q=False, check=True), want)
+        del far, t
+
+
+def test_wrappers_refuse(dev):
+    t = Batch(dev, 8, [(2, 32)], [5, 5], [1, 1], 8, 2, 128, 16)
+    f = Batch(dev, 4, [(2, 32)], [5, 5], [1, 1], 8, 2, 128, 16)
+    ok = [t.q, t.pool, t.scales, t.bt, t.seq_lens, t.cu_group, t.shared]
+    bad = {0: [t.q.float(), t.q[:1], t.q[..., :64].contiguous(), t.q[:, :3].contiguous(), t.q.cpu()],
+           1: [t.pool.int(), t.pool[:, :, :, :, :96].contiguous(), t.pool[0], f.pool],
+           2: [None, t.scales.half(), t.scales[:1]], 3: [t.bt.long(), t.bt[0], t.bt[:1].contiguous()],
+           4: [t.seq_lens.long(), t.seq_lens[:1]], 5: [t.cu_group.long(), t.cu_group[:1]],
+           6: [t.shared.long(), t.shared[None], torch.cat([t.shared] * 3)]}
+    for i, values in bad.items():
+        for v in values:
+            with pytest.raises(ValueError):
+                kv.paged_attention_shared(*(ok[:i] + [v] + ok[i + 1:]))
+    for kw in (dict(cu_q=t.cu_q.long()), dict(cu_q=t.cu_q[:2]), dict(out=t.q.float()), dict(out=t.q[:1]),
+               dict(err=torch.zeros(1, device=dev)), dict(err=torch.zeros(1, dtype=torch.int32))):
+        with pytest.raises(ValueError):
+            kv.paged_attention_shared(*ok, **kw)
+    with pytest.raises(ValueError):
+        kv.paged_attention4_shared(f.q, t.pool, f.bt, f.seq_lens, f.cu_group, f.shared)
+    # pages of other sizes belong to the usual decode
+    pool = torch.zeros((9, 2, 2, 8, 128), dtype=torch.uint8, device=dev)
+    with pytest.raises(ValueError, match="multiple of 16"):
+        kv.paged_attention_shared(t.q, pool, t.scales, t.bt, t.seq_lens, t.cu_group, t.shared)

@@ -10,7 +10,8 @@ its behaviour is defined here and in include/zenyx_kv.h).
 * ``PagedFP4KVCache`` -- the same cache with 4-bit pages (e2m1 codes, a power of two per 32
   channels): 17/32 byte per element, no scales to keep.
 * ``QuantizedRingAttention`` -- ring attention (and decode) over either cache, reading the
-  pages directly.
+  pages directly; where sequences of a batch share pages (``PagedFP8KVCache.fork``) those are read once for
+  all of them.
 A cache made with ``rope`` (train.rotary.RotaryPositions) takes unrotated keys, rotates them by
 their positions while it stores them, and the attention rotates the queries.
 All arithmetic runs in libzenyx_kv.so on the HIP device.
@@ -76,6 +77,11 @@ class PagedFP8KVCache:
     undoes its own faulty append (lengths, pages, scales) before raising."""
 
     _ERR_WORDS = 64
+    # Positions that reading shared pages once has to save a batch for the kernel that does it, which costs
+    # 5 us more to start (decode's / this one's time, 32/8 heads, D = 128: 16 sequences on 2,048 shared
+    # positions 20.2 / 20.2 us, on 4,096 28 / 23, 4 on 16,384 30 / 26, 64 on 16,384 244 / 50).
+    _LEAST_SAVED = 49152
+    _SHARED_PRECISIONS = ("f16",)  # of QuantizedRingAttention's, what that kernel computes
 
     def __init__(self, num_layers: int, num_kv_heads: int, head_dim: int, num_pages: int,
                  page_size: int = 16, device: torch.device | None = None, overflow: str = "raise", rope=None):
@@ -106,6 +112,11 @@ class PagedFP8KVCache:
         self._bt = torch.full((16, 64), -1, dtype=torch.int32, device=self.device)
         self._len = torch.zeros(16, dtype=torch.int32, device=self.device)
         self._rows_cache: tuple = ((), None)  # (seq_ids, device int64 rows) of the last call
+        # Pages that several sequences have: how many do (pages of one are not listed), and per
+        # sequence how many of its first pages it has in common with the others of a fork
+        self._users: dict = {}    # page id -> sequences, 2 or more
+        self._common: dict = {}   # seq id -> {fork: pages}
+        self._groups_cache: tuple = ((), None)  # (seq_ids, groups) of the last call
         self._ones_cache: dict = {}  # n -> device int32 ones [n] / arange [n + 1] (one-token steps)
 
     # ---------------------------------------------------------------- the pages' format
@@ -134,6 +145,11 @@ class PagedFP8KVCache:
     def _attend_step(self, q, layer: int, tables, lens, att) -> torch.Tensor:
         return kv.paged_attention_decode(q, self.pool[layer], self.scales[layer], tables, lens, sm_scale=att.sm_scale,
                                          check=att.check)
+
+    def _attend_shared(self, q, layer: int, tables, lens, groups, att, cu=None, max_q: int | None = None):
+        cu_group, shared = groups
+        return kv.paged_attention_shared(q, self.pool[layer], self.scales[layer], tables, lens, cu_group, shared, cu_q=cu,
+                                         max_q_per_seq=max_q, causal=att.causal, sm_scale=att.sm_scale, check=att.check)
 
     def _gather(self, layer: int, tables, lens, out_len: int):
         return kv.kv_gather_dequant(self.pool[layer], self.scales[layer], tables, lens, out_len)
@@ -235,6 +251,7 @@ class PagedFP8KVCache:
                 self._drop_row(seq_id)
 
     def _drop_row(self, seq_id) -> None:
+        self._groups_cache = ((), None)
         r = self._row.pop(seq_id, None)
         if r is None:
             return
@@ -334,10 +351,100 @@ class PagedFP8KVCache:
         return self._gather(layer, self._tables(seq_ids), self._lengths(seq_ids), out_len)
 
     def free(self, seq_id) -> None:
+        """Forget a sequence; pages that others share with it stay until the last one is freed."""
         for p in self.pages.pop(seq_id, []):
-            self._free.append(p)
+            n = self._users.get(p, 1)
+            if n == 1:
+                self._free.append(p)
+            elif n == 2:
+                del self._users[p]
+            else:
+                self._users[p] = n - 1
         self.lengths.pop(seq_id, None)
+        self._common.pop(seq_id, None)
         self._drop_row(seq_id)
+
+    # ---------------------------------------------------------------- sequences that share pages
+
+    def fork(self, seq_id, new_ids: list, length: int | None = None) -> None:
+        """New sequences that begin with the first ``length`` (default: all) tokens of ``seq_id``: a
+        system prompt or a document that many sequences go on from, several samples of one prompt, an
+        encoder's states that several rows attend to.  Whole pages are shared, not copied; a
+        page that ``length`` ends inside is copied for each new sequence.  Every sequence, ``seq_id``
+        too, goes on and is freed by itself.  ``QuantizedRingAttention`` reads the shared pages once
+        for a batch's neighbours that have them in common."""
+        if seq_id not in self.lengths:
+            raise KeyError(seq_id)
+        n = self.lengths[seq_id] if length is None else int(length)
+        if not 0 <= n <= self.lengths[seq_id]:
+            raise ValueError(f"length must lie in [0, {self.lengths[seq_id]}], the tokens of {seq_id!r}")
+        if len(set(new_ids)) != len(new_ids) or any(s in self.lengths or s in self.pages for s in new_ids):
+            raise ValueError("new_ids must be distinct and not in the cache")
+        if not new_ids:
+            return
+        whole, rest = divmod(n, self.P)
+        size = self.pool[0, 0].numel()
+        if rest and size % 16:
+            raise ValueError(f"pages of {size} bytes, no multiple of 16, cannot be copied")
+        if rest and len(self._free) < len(new_ids):
+            raise MemoryError("PagedFP8KVCache: out of pages")
+        src = self.pages.get(seq_id, [])
+        copies = [self._free.pop() for _ in new_ids] if rest else []
+        rows = [self._row_of(s) for s in new_ids]  # (may grow the tables)
+        self._rows_cache = ((), None)
+        at = torch.tensor(rows, dtype=torch.int64).to(self.device)
+        if whole:
+            self._bt[at, :whole] = self._bt[self._row[seq_id], :whole].clone()
+        self._len[at] = n
+        if rest:
+            self._write_entries([(r, whole, p) for r, p in zip(rows, copies)])
+            moves = [(layer * self.num_pages + p, layer * self.num_pages + src[whole])
+                     for layer in range(self.L) for p in copies]
+            dst, org = torch.tensor(moves, dtype=torch.int64).t().contiguous().to(self.device) * size
+            kv.tier_move_pages(self.pool, self.pool, dst, org, size,
+                               stream=torch.cuda.current_stream(self.device))
+        known = self._common.setdefault(seq_id, {})
+        if whole and whole not in known.values():
+            known[object()] = whole
+        for s, p in zip(new_ids, copies or [None] * len(new_ids)):
+            self.pages[s] = src[:whole] + ([] if p is None else [p])
+            self.lengths[s] = n
+            self._common[s] = {f: min(k, whole) for f, k in known.items()}
+        for p in src[:whole]:
+            self._users[p] = self._users.get(p, 1) + len(new_ids)
+
+    def _shared_pages(self, a, b) -> int:
+        """How many of their first pages two sequences are known to have in common."""
+        x, y = self._common.get(a), self._common.get(b)
+        return max((min(k, y[f]) for f, k in x.items() if f in y), default=0) if x and y else 0
+
+    def _groups(self, seq_ids):
+        """Device (int32 cu_group, int32 shared tokens) of a batch's neighbours that share pages, or None
+        where reading those once saves too little (or no kernel has the shape)."""
+        if not self._common or self.D not in (64, 128, 256) or self.P % 16:
+            return None
+        key = tuple(seq_ids)
+        if self._groups_cache[0] != key:
+            starts, shared = [], []
+            for i, s in enumerate(key):
+                c = self._shared_pages(key[starts[-1]], s) if i else 0
+                # (a neighbour that shares little of what the others do begins a group of its own)
+                if c and (shared[-1] is None or 2 * c >= shared[-1]):
+                    shared[-1] = c if shared[-1] is None else min(shared[-1], c)
+                else:
+                    starts.append(i)
+                    shared.append(None)
+            bounds = starts + [len(key)]
+            tokens = [0 if n is None else n * self.P for n in shared]
+            saved = sum((b - a - 1) * n for a, b, n in zip(bounds, bounds[1:], tokens))
+            groups = None
+            if saved >= self._LEAST_SAVED:
+                w = (len(bounds) + 3) // 4 * 4  # each row 16-byte aligned
+                t = torch.tensor([bounds + [0] * (w - len(bounds)), tokens + [0] * (w - len(tokens))],
+                                 dtype=torch.int32).to(self.device)
+                groups = t[0, :len(bounds)], t[1, :len(tokens)]
+            self._groups_cache = (key, groups)
+        return self._groups_cache[1]
 
 
 class PagedFP4KVCache(PagedFP8KVCache):
@@ -345,6 +452,8 @@ class PagedFP4KVCache(PagedFP8KVCache):
     codes times a power of two of their own, so tokens do not share scales: nothing overflows,
     and an append needs no earlier one.  A block of 32 that holds a NaN or an infinity is NaN.
     ``head_dim`` 64, 128 or 256, ``page_size`` a multiple of 16.  ``scales`` is None."""
+
+    _SHARED_PRECISIONS = ("f16", "exact")
 
     def __init__(self, num_layers: int, num_kv_heads: int, head_dim: int, num_pages: int, page_size: int = 16,
                  device: torch.device | None = None, rope=None):
@@ -372,6 +481,11 @@ class PagedFP4KVCache(PagedFP8KVCache):
     def _attend_step(self, q, layer: int, tables, lens, att) -> torch.Tensor:
         return kv.paged_attention4_decode(q, self.pool[layer], tables, lens, sm_scale=att.sm_scale, check=att.check)
 
+    def _attend_shared(self, q, layer: int, tables, lens, groups, att, cu=None, max_q: int | None = None):
+        cu_group, shared = groups
+        return kv.paged_attention4_shared(q, self.pool[layer], tables, lens, cu_group, shared, cu_q=cu,
+                                          max_q_per_seq=max_q, causal=att.causal, sm_scale=att.sm_scale, check=att.check)
+
     def _gather(self, layer: int, tables, lens, out_len: int):
         return kv.kv4_gather_dequant(self.pool[layer], tables, lens, out_len)
 
@@ -388,8 +502,12 @@ class QuantizedRingAttention:
 
     With a ``PagedFP4KVCache`` one launch takes all keys, whatever ``ring_degree`` (the union
     of a ring's shards), and ``precision`` "f16" is given as "exact": the 4-bit kernels have no
-    fp16 weights, and "bf16" has fewer bits.  A cache with ``rope`` has rotated its keys: the queries are rotated here, by the
+    fp16 weights, and "bf16" has fewer bits.  Neighbours of a batch that share pages
+    (``PagedFP8KVCache.fork``) attend to them together, in ``decode`` and in calls of few rows per
+    sequence: the shared keys are read and multiplied once for all of them.  A cache with ``rope`` has rotated its keys: the queries are rotated here, by the
     positions of the tokens they stand for."""
+
+    _FEW_ROWS = 8  # of a sequence, for which shared pages are attended to together
 
     def __init__(self, cache: PagedFP8KVCache, ring_degree: int = 8, causal: bool = True,
                  sm_scale: float | None = None, precision: str = "f16", check: bool = True):
@@ -422,7 +540,14 @@ class QuantizedRingAttention:
         if c.rope is not None:
             shift = torch.repeat_interleave(q_pos0 - cu[:-1], counts, output_size=q.shape[0])
             q = c.rope(q, shift + torch.arange(q.shape[0], dtype=torch.int32, device=q.device))
-        out = c._attend(q, layer, c._tables(seq_ids), cu, q_pos0, lens, self, max(q_lens, default=0))
+        most = max(q_lens, default=0)
+        # few rows per sequence (proposed tokens): bound by what they read of shared pages
+        few = 0 < most <= self._FEW_ROWS and self.precision in c._SHARED_PRECISIONS
+        groups = c._groups(seq_ids) if few else None
+        if groups is not None:
+            out = c._attend_shared(q, layer, c._tables(seq_ids), lens, groups, self, cu, most)
+        else:
+            out = c._attend(q, layer, c._tables(seq_ids), cu, q_pos0, lens, self, most)
         if self.check:
             c.check_errors()  # the appends behind these pages (the check above has synchronised)
         return out
@@ -433,7 +558,11 @@ class QuantizedRingAttention:
         q, lens = q.to(c.device).contiguous(), c._lengths(seq_ids)
         if c.rope is not None:
             q = c.rope(q, lens - 1)
-        out = c._attend_step(q, layer, c._tables(seq_ids), lens, self)
+        groups = c._groups(seq_ids)
+        if groups is not None:
+            out = c._attend_shared(q, layer, c._tables(seq_ids), lens, groups, self)
+        else:
+            out = c._attend_step(q, layer, c._tables(seq_ids), lens, self)
         if self.check:
             c.check_errors()
         return out
