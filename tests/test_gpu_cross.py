@@ -111,3 +111,331 @@ def test_against_float64(dev, case, kind):
     got = kv.cross_attention_backward(g, q, k, v, out, lse, cu_q, cu_k, check=True)
     for x, w, e, name in zip(got, want[1:], tol[1:], ("dq", "dk", "dv")):
         near(x, w, e, name)
+
+
+def inputs(dev, t, rows, keys, Hq, Hkv, D, seed=0, width=1):
+    """q, k, v, grad; width > 1: rows that lie in wider ones."""
+    gen = torch.Generator(device=dev).manual_seed(seed)
+
+    def make(n, H):
+        x = torch.randn((n, H, D * width), generator=gen, device=dev).to(t)
+        return x[..., D * (width - 1):]
+    return make(sum(rows), Hq), make(sum(keys), Hkv), make(sum(keys), Hkv), make(sum(rows), Hq)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("sm", [-0.07, 0.0, 0.5])
+@pytest.mark.parametrize("D, rows, keys", [(64, [70, 5], [90, 40]), (128, [4], [900])])
+def test_other_scales(dev, kind, sm, D, rows, keys):
+    t, h, tiny = TYPES[kind]
+    q, k, v, g = inputs(dev, t, rows, keys, 4, 2, D, 1)
+    cu_q, cu_k = starts(rows, dev), starts(keys, dev)
+    want, tol = exact(q, k, v, g, rows, keys, h, tiny, sm)
+    out, lse = kv.cross_attention(q, k, v, cu_q, cu_k, sm_scale=sm, return_lse=True, check=True)
+    near(out, want[0], tol[0], "out")
+    for x, w, e, name in zip(kv.cross_attention_backward(g, q, k, v, out, lse, cu_q, cu_k, sm_scale=sm), want[1:], tol[1:],
+                             ("dq", "dk", "dv")):
+        near(x, w, e, name)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("D, Hq, Hkv", [(64, 6, 2), (128, 4, 4)])
+def test_padded_states_and_rows_in_no_sequence(dev, kind, D, Hq, Hkv):
+    """k_lens over padding that holds NaN and infinities; rows and keys before the first sequence and behind
+    the last."""
+    t, h, tiny = TYPES[kind]
+    rows, lens, S = [9, 0, 200, 1, 33], [70, 12, 129, 0, 200], 200
+    q, k, v, g = inputs(dev, t, [7 + sum(rows) + 600], [3 + S * 5 + 70], Hq, Hkv, D, 2)
+    keep = torch.zeros(len(k), dtype=torch.bool, device=dev)
+    at = [3 + S * b for b in range(5)]
+    for a, n in zip(at, lens):
+        keep[a:a + n] = True
+    bad = torch.tensor([float("nan"), float("inf"), -float("inf")], device=dev, dtype=t)
+    k[~keep] = bad[torch.arange(int((~keep).sum()), device=dev) % 3][:, None, None]
+    v[~keep] = bad[0]
+    cu_q, cu_k, k_lens = starts(rows, dev, 7), i32([*at, 3 + S * 5], dev), i32(lens, dev)
+    clean = [torch.where(keep[:, None, None], x, torch.zeros_like(x)) for x in (k, v)]
+    mid = slice(7, 7 + sum(rows))
+    want, tol = exact(q[mid], *clean, g[mid], rows, lens, h, tiny, D ** -0.5, at)
+    out = torch.full_like(q, 5.0)
+    got, lse = kv.cross_attention(q, k, v, cu_q, cu_k, k_lens, out=out, return_lse=True, check=True)
+    assert got is out and (out[:7] == 5).all() and (out[7 + sum(rows):] == 5).all()
+    near(out[mid], want[0], tol[0], "out")
+    no_key = mid.start + sum(rows[:3])
+    assert (out[no_key] == 0).all() and (lse[:, no_key] == -torch.inf).all()
+    zero = kv.cross_attention(q, k, v, cu_q, cu_k, k_lens, zero_rest=True)
+    assert torch.equal(zero[mid], out[mid]) and (zero[:7] == 0).all() and (zero[mid.stop:] == 0).all()
+    # what rows in no sequence hold, and their gradients, reach nothing
+    for x in (q, g):
+        x[:7], x[mid.stop:] = float("nan"), float("inf")
+    grads = kv.cross_attention_backward(g, q, k, v, out, lse, cu_q, cu_k, k_lens, check=True)
+    assert (grads[0][:7] == 0).all() and (grads[0][mid.stop:] == 0).all()
+    near(grads[0][mid], want[1], tol[1], "dq")
+    for x, w, e, name in zip(grads[1:], want[2:], tol[2:], ("dk", "dv")):
+        near(x, w, e, name)
+        assert (x[~keep] == 0).all()
+    # gradients that overflowed do not reach the padding's either
+    g[mid] = float("inf")
+    for x in kv.cross_attention_backward(g, q, k, v, out, lse, cu_q, cu_k, k_lens)[1:]:
+        assert (x[~keep] == 0).all()
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+def test_lse_and_large_scores(dev, kind):
+    """Scores of some hundreds, falling and rising along the keys: log-sum-exp to fp32's accuracy."""
+    t = TYPES[kind][0]
+    for rows, keys, D in (([40], [500], 64), ([3], [2000], 128)):
+        q, k, v, _ = inputs(dev, t, rows, keys, 2, 1, D, 3)
+        k *= torch.linspace(-9, 9, keys[0], device=dev, dtype=t)[:, None, None]
+        q *= 4
+        out, lse = kv.cross_attention(q, k, v, starts(rows, dev), starts(keys, dev), sm_scale=0.25, return_lse=True)
+        s = torch.einsum("rhd,td->hrt", q.double(), k[:, 0].double()) * 0.25
+        want = torch.logsumexp(s, -1) / torch.log(torch.tensor(2.0, dtype=torch.float64))
+        size = torch.einsum("rhd,td->hrt", q.double().abs(), k[:, 0].double().abs()).amax(-1) * 0.25 * 1.4427
+        assert ((lse - want).abs() <= size * (D + 4) * 2.0 ** -24 + want.abs() * 2.0 ** -23 + 1e-5).all()
+        assert torch.isfinite(out).all()
+
+
+def test_strided_inputs(dev):
+    """The parts of fused projections, rows of wider ones, one KV head for all by a stride of 0, and rows so
+    far apart that their offsets pass 2^32 bytes."""
+    t, h, tiny = TYPES["bf16"]
+    rows, keys, D = [33, 4], [80, 130], 64
+    for Hq, Hkv, width in ((4, 4, 1), (8, 2, 3)):
+        q, k, v, g = inputs(dev, t, rows, keys, Hq, Hkv, D, 4, width)
+        flat = [x.contiguous() for x in (q, k, v, g)]
+        cu_q, cu_k = starts(rows, dev), starts(keys, dev)
+        want = kv.cross_attention(*flat[:3], cu_q, cu_k, return_lse=True)
+        grads = kv.cross_attention_backward(flat[3], *flat[:3], *want, cu_q, cu_k)
+
+        def same(q, k, v, g):
+            got = kv.cross_attention(q, k, v, cu_q, cu_k, return_lse=True, check=True)
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+            got = kv.cross_attention_backward(g, q, k, v, *got, cu_q, cu_k, check=True)
+            assert all(torch.equal(a, b) for a, b in zip(got, grads))
+        same(q, k, v, g)
+        head_major = [x.transpose(0, 1).contiguous().transpose(0, 1) for x in flat]
+        same(*head_major)
+        fused = torch.cat([flat[1], flat[2]], 1)
+        same(q, fused[:, :Hkv], fused[:, Hkv:], g)
+        fused = torch.empty((len(flat[1]), Hkv, 2 * D), dtype=t, device=dev)
+        fused[..., :D], fused[..., D:] = flat[1], flat[2]
+        same(q, fused[..., :D], fused[..., D:], g)
+    one = flat[1][:, :1].expand(-1, 2, -1)
+    got = kv.cross_attention(flat[0], one, one, cu_q, cu_k)
+    assert torch.equal(got, kv.cross_attention(flat[0], one.contiguous(), one.contiguous(), cu_q, cu_k))
+    far = torch.zeros((1100, 1 << 22), dtype=t, device=dev)  # 8.6 GiB
+    rows = keys = [500, 600]
+    q, k, v, g = inputs(dev, t, rows, keys, 2, 2, D, 5)
+    cu = starts(rows, dev)
+    out, lse = kv.cross_attention(q, k, v, cu, cu, return_lse=True)
+    grads = kv.cross_attention_backward(g, q, k, v, out, lse, cu, cu)
+    views = []
+    for i, x in enumerate((q, k, v, g)):
+        view = far[:, i * 2 * D:(i + 1) * 2 * D].unflatten(1, (2, D))
+        view.copy_(x)
+        views.append(view)
+    a, b = kv.cross_attention(*views[:3], cu, cu, return_lse=True)
+    assert torch.equal(a, out) and torch.equal(b, lse)
+    for x, w in zip(kv.cross_attention_backward(views[3], *views[:3], a, b, cu, cu), grads):
+        assert torch.equal(x, w)
+
+
+def test_bounds_are_flagged(dev):
+    t = torch.bfloat16
+    rows, keys = [5, 9], [70, 30]
+    q, k, v, g = inputs(dev, t, rows, keys, 4, 2, 64, 6)
+    cu_q, cu_k = starts(rows, dev), starts(keys, dev)
+    whole = kv.cross_attention(q, k, v, cu_q, cu_k)
+    out = torch.full_like(q, 3.0)
+    with pytest.raises(ValueError, match="position"):
+        kv.cross_attention(q, k, v, cu_q, cu_k, max_q_per_seq=6, out=out, check=True)
+    assert torch.equal(out[:11], whole[:11]) and (out[11:] == 3).all()
+    err = torch.zeros(1, dtype=torch.int32, device=dev)
+    got, lse = kv.cross_attention(q, k, v, cu_q, cu_k, max_k_per_seq=40, return_lse=True, err=err)
+    assert int(err) == N.ZX_KERR_POS_RANGE
+    assert torch.equal(got, kv.cross_attention(q, k, v, cu_q, cu_k, i32([40, 30], dev)))
+    for cq, ck in (([0, 5, 15], [0, 70, 100]), ([-1, 5, 14], [0, 70, 100]), ([0, 5, 14], [0, 70, 101]), ([0, 9, 5], [0, 70, 100]),
+                   ([0, 5, 14], [40, 20, 100]), ([0, 5, 14], [-9, 70, 100]), ([0, 1 << 30, 14], [0, 1 << 30, 100])):
+        for f in (lambda: kv.cross_attention(q, k, v, i32(cq, dev), i32(ck, dev), max_q_per_seq=14, max_k_per_seq=100,
+                                             check=True),
+                  lambda: kv.cross_attention_backward(g, q, k, v, got, lse, i32(cq, dev), i32(ck, dev), max_q_per_seq=14,
+                                                      max_k_per_seq=100, check=True)):
+            with pytest.raises(ValueError, match="position"):
+                f()
+    # k_lens beyond a sequence's keys and below 0: all of them, none
+    got = kv.cross_attention(q, k, v, cu_q, cu_k, i32([1 << 30, -4], dev), check=True)
+    assert torch.equal(got[:5], whole[:5]) and (got[5:] == 0).all()
+
+
+@pytest.mark.parametrize("D, rows, keys, Hq, Hkv", [(64, [300, 40], [500, 900], 4, 2), (128, [2, 3], [5000, 40], 4, 1),
+                                                    (128, [1500], [1100], 2, 2)])
+def test_captured_and_repeated(dev, D, rows, keys, Hq, Hkv):
+    """The same bits from call to call; a captured forward and backward on other inputs and lengths, with
+    eager work between the replays; two streams at once."""
+    q, k, v, g = inputs(dev, torch.bfloat16, rows, keys, Hq, Hkv, D, 7)
+    cu_q, cu_k, k_lens = starts(rows, dev), starts(keys, dev), i32(keys, dev)
+    mq, mk = max(rows), max(keys)
+
+    def step():
+        out, lse = kv.cross_attention(q, k, v, cu_q, cu_k, k_lens, max_q_per_seq=mq, max_k_per_seq=mk, return_lse=True,
+                                      zero_rest=True)
+        return (out, *kv.cross_attention_backward(g, q, k, v, out, lse, cu_q, cu_k, k_lens, max_q_per_seq=mq,
+                                                  max_k_per_seq=mk))
+    first = step()
+    for _ in range(3):
+        assert all(torch.equal(a, b) for a, b in zip(step(), first))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for i in range(4):
+        q.mul_(-1.0), g.mul_(0.5 if i % 2 else 2.0)
+        cut = [max(0, n - 37 * i) for n in keys]
+        k_lens.copy_(i32(cut, dev))
+        cu_q.copy_(starts([max(0, n - i) for n in rows], dev))
+        for x in held:
+            x.fill_(9.0)
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(held, step()))
+    torch.cuda.synchronize()
+    want, got = step(), []
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(dev) for _ in range(2)]
+    for _ in range(3):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(step())
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for x in got for a, b in zip(x, want))
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+def test_gradients_against_differences(dev, kind):
+    """<dq, x> and the like against the forward's own central difference along x.  The step e is exact in
+    the type for the direction's values of +-1 and inputs on a grid of 1/8 below 4; the forward is off by
+    tol per element at each end, the difference by 2 |g| tol / 2 e, its third-order term by
+    (e^2 / 6) |f'''|, which halving e would show: the bound takes a quarter of f(2e)'s difference from f(e)'s."""
+    t, h, tiny = TYPES[kind]
+    rows, keys, D = [6, 3], [20, 9], 64
+    gen = torch.Generator(device=dev).manual_seed(8)
+    q, k, v, g = (torch.randint(-8, 9, (n, H, D), generator=gen, device=dev).to(t) / 8
+                  for n, H in ((9, 4), (29, 2), (29, 2), (9, 4)))
+    cu_q, cu_k = starts(rows, dev), starts(keys, dev)
+
+    def f(q, k, v):
+        out = kv.cross_attention(q, k, v, cu_q, cu_k)
+        _, tol = exact(q, k, v, g, rows, keys, h, tiny, D ** -0.5)
+        return (out.double() * g.double()).sum(), (tol[0] * g.double().abs()).sum()
+    out, lse = kv.cross_attention(q, k, v, cu_q, cu_k, return_lse=True)
+    grads = kv.cross_attention_backward(g, q, k, v, out, lse, cu_q, cu_k)
+    _, tol = exact(q, k, v, g, rows, keys, h, tiny, D ** -0.5)
+    xs = [q, k, v]
+    for i in range(3):
+        for trial in range(3):
+            way = torch.randint(0, 2, xs[i].shape, generator=gen, device=dev).to(t) * 2 - 1
+            diff, noise = [], []
+            for e in (0.125, 0.25):
+                (hi, n1), (lo, n2) = (f(*[x + s * e * way if j == i else x for j, x in enumerate(xs)]) for s in (1, -1))
+                diff.append((hi - lo) / (2 * e))
+                noise.append((n1 + n2) / (2 * e))
+            got = (grads[i].double() * way.double()).sum()
+            bound = noise[0] + noise[1] + (tol[i + 1] * 1.0).sum() + (diff[1] - diff[0]).abs()
+            assert (got - diff[0]).abs() <= bound, (i, trial, float(got), float(diff[0]), float(bound))
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+def test_cross_attention_module(dev, kind):
+    """Through autograd: leaves that are views and broadcast, gradients as autograd lays them out, inputs
+    that need none, no grad, other bounds; and what it refuses."""
+    t, h, tiny = TYPES[kind]
+    rows, keys, D = [20, 1, 50], [64, 7, 300], 64
+    q, k, v, g = inputs(dev, t, rows, keys, 4, 2, D, 9)
+    cu_q, cu_k = starts(rows, dev), starts(keys, dev)
+    attend = CrossAttention()
+    out, lse = kv.cross_attention(q, k, v, cu_q, cu_k, return_lse=True)
+    want = kv.cross_attention_backward(g, q, k, v, out, lse, cu_q, cu_k)
+    fused = torch.stack([k, v], 1).requires_grad_()  # [n, 2, H, D]
+    ql = q.clone().requires_grad_()
+    y = attend(ql, fused[:, 0], fused[:, 1], cu_q, cu_k)
+    assert torch.equal(y, out)
+    y.backward(g)
+    assert torch.equal(ql.grad, want[0]) and torch.equal(fused.grad, torch.stack(want[1:], 1))
+    # gradients that are expanded, transposed or not aligned
+    for give in (torch.ones((), dtype=t, device=dev).expand(q.shape), g.transpose(0, 2).contiguous().transpose(0, 2),
+                 torch.empty(g.numel() + 1, dtype=t, device=dev)[1:].view(g.shape).copy_(g)):
+        ql.grad = None
+        attend(ql, k, v, cu_q, cu_k).backward(give)
+        assert torch.equal(ql.grad, kv.cross_attention_backward(give.contiguous().clone(), q, k, v, out, lse, cu_q, cu_k)[0])
+    # one head's states for both: their gradients come together, in the type
+    one = k[:, :1].clone().requires_grad_()
+    attend(q, one.expand(-1, 2, -1), v, cu_q, cu_k).backward(g)
+    both = one.detach().expand(-1, 2, -1).contiguous()
+    o1, l1 = kv.cross_attention(q, both, v, cu_q, cu_k, return_lse=True)
+    assert torch.equal(one.grad, kv.cross_attention_backward(g, q, both, v, o1, l1, cu_q, cu_k)[1].sum(1, keepdim=True))
+    with torch.no_grad():
+        z = attend(ql, k, v, cu_q, cu_k)
+    assert not z.requires_grad and torch.equal(z, out)
+    assert not attend(q, k, v, cu_q, cu_k).requires_grad
+    y = attend(ql, k, v, cu_q, cu_k, max_q_per_seq=71, max_k_per_seq=371)
+    (d,) = torch.autograd.grad(y, ql, g, create_graph=True)
+    with pytest.raises(RuntimeError):  # once, in reverse mode
+        torch.autograd.grad(d.float().sum(), ql)
+    with torch.autograd.forward_ad.dual_level():
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            attend(torch.autograd.forward_ad.make_dual(q, torch.ones_like(q)), k, v, cu_q, cu_k)
+    for bad in ((q.float(), k, v), (q, k[:, :, :32], v), (q[:, :3], k, v), (q, k[:5], v), (q, k.cpu(), v), (q, k, v.half().bfloat16() if
+                kind == "f16" else v.half()), (q[..., ::2], k, v), (q[0], k, v)):
+        with pytest.raises(ValueError):
+            attend(*bad, cu_q, cu_k)
+    for cq, ck, kl in ((cu_q.long(), cu_k, None), (cu_q, cu_k[:3], None), (cu_q, cu_k, cu_k), (cu_q[:1], cu_k[:1], None),
+                       (cu_q, cu_k, cu_k[:3].long()), (cu_q.cpu(), cu_k, None)):
+        with pytest.raises(ValueError):
+            attend(q, k, v, cq, ck, kl)
+    for kw in (dict(out=q.float()), dict(out=q[:3]), dict(out=q.transpose(0, 1)), dict(err=torch.zeros(1, device=dev))):
+        with pytest.raises(ValueError):
+            kv.cross_attention(q, k, v, cu_q, cu_k, **kw)
+    for i, x in ((0, g.float()), (0, g[:3]), (4, out.float()), (5, lse.double()), (5, lse[:1]), (0, g.cpu())):
+        args = [g, q, k, v, out, lse]
+        args[i] = x
+        with pytest.raises(ValueError):
+            kv.cross_attention_backward(*args, cu_q, cu_k)
+
+
+def test_captured_training_step(dev):
+    """Forward and backward through autograd in one graph, replayed with other inputs."""
+    rows, keys, D = [64, 30], [200, 77], 128
+    q, k, v, g = inputs(dev, torch.bfloat16, rows, keys, 4, 2, D, 10)
+    cu_q, cu_k = starts(rows, dev), starts(keys, dev)
+    for x in (q, k, v):
+        x.requires_grad_()
+    attend = CrossAttention()
+
+    def step():
+        out = attend(q, k, v, cu_q, cu_k, max_q_per_seq=64, max_k_per_seq=200)
+        return (out.detach(), *torch.autograd.grad(out, (q, k, v), g))
+    side = torch.cuda.Stream(dev)
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for i in range(3):
+        with torch.no_grad():
+            q.mul_(0.5 if i else -1.0), v.add_(1.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(held, step()))
+
+
+def test_no_rows_no_keys(dev):
+    for n, m in ((0, 5), (5, 0), (0, 0)):
+        q = torch.randn((n, 4, 64), device=dev).bfloat16().requires_grad_()
+        k = torch.randn((m, 2, 64), device=dev).bfloat16().requires_grad_()
+        y = CrossAttention()(q, k, k, i32([0, n], dev), i32([0, m], dev))
+        assert y.shape == q.shape and (y == 0).all()
+        y.backward(torch.ones_like(y))
+        assert (q.grad == 0).all() and (k.grad == 0).all()

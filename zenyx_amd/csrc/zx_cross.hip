@@ -10,8 +10,8 @@
 // (zx_attn_tile.h):
 //   forward, dq:  columns are (query row, head of the KV head's group); K and V tiles of 64 keys in
 //                 LDS; S^T = K Q^T, dP^T = V dO^T, O^T += V^T P^T, dQ^T += K^T dS^T
-//   dk, dv:       columns are keys, whose K and V stay in registers; Q and dO tiles of 64 (row, head)
-//                 in LDS; S = Q K^T, dP = dO V^T, dV^T += dO^T P, dK^T += Q^T dS
+//   dk, dv:       columns are keys, their K in registers and their V's rows in LDS; Q and dO tiles
+//                 of 32 (row, head) in LDS; S = Q K^T, dP = dO V^T, dV^T += dO^T P, dK^T += Q^T dS
 // Every sum has a fixed order: gradients do not change from call to call (dq has a kernel of its
 // own, two of seven products more than atomics would need).  Bound by the matrix products and
 // the LDS reads that feed them; a call of few rows by the reads of K and V, its keys cut among
@@ -40,7 +40,7 @@ struct CrossArgs {
   int32_t n_q_heads, n_kv_heads, n_seqs, group;
   int32_t max_q, max_k;
   int32_t n_tile, n_split;  // tiles of a sequence and KV head at most, parts of each
-  int32_t zero_rest;
+  int32_t n_rest;           // blocks behind the others that clear the rows in no sequence
   uint32_t g_magic;         // c / group = (c * g_magic) >> (31 + g_shift) for c < 2^31
   int32_t g_shift;
   int32_t order;            // the sequences with the most work first
@@ -103,7 +103,7 @@ __device__ __forceinline__ CrItem cr_item(const CrossArgs &a) {
   return it;
 }
 static unsigned cr_grid(const CrossArgs &a) {
-  return (unsigned)(8 * ceil_div((int64_t)a.n_seqs * a.n_kv_heads, 8) * a.n_tile * a.n_split);
+  return (unsigned)(8 * ceil_div((int64_t)a.n_seqs * a.n_kv_heads, 8) * a.n_tile * a.n_split) + (unsigned)a.n_rest;
 }
 
 // The tile's loads, in registers until the LDS buffer is free.  Rows from n on are zeros (and not read).
@@ -149,7 +149,6 @@ __device__ __forceinline__ void cr_pipeline(int t_begin, int t_end, int step, Lo
 
 // Columns of a wave: 32 CT of the block's 128 CT.
 template <int D, int CT> struct CrCols {
-  int64_t off[CT];  // rows' element offset (row, head) in q's layout: row number, head
   int32_t row[CT], head[CT];
   bool live[CT];
   __device__ __forceinline__ CrCols(const CrossArgs &a, int c0, int n_cols, int h, int64_t lo) {
@@ -179,13 +178,17 @@ template <int D, int CT> struct CrCols {
   }
 };
 
-// Rows in no sequence: zeros, where they are asked for (a block of its own for each tensor).
-__device__ __forceinline__ void cr_zero_rest(uint16_t *out, const int32_t *cu, int32_t n_seqs, int64_t n, int64_t width) {
-  const int64_t lo = max((int64_t)0, min((int64_t)cu[0], n)), hi = max(lo, min((int64_t)cu[n_seqs], n));
+// Rows in no sequence (before the first, behind the last): zeros.  How many there are only the device
+// knows: CR_REST blocks behind the others share them.
+constexpr unsigned CR_REST = 64;
+__device__ __forceinline__ bool cr_is_rest(const CrossArgs &a) { return blockIdx.x + (uint32_t)a.n_rest >= gridDim.x; }
+__device__ __forceinline__ void cr_zero_rest(const CrossArgs &a, uint16_t *out, const int32_t *cu, int64_t n, int64_t width) {
+  const int64_t lo = max((int64_t)0, min((int64_t)cu[0], n)), hi = max(lo, min((int64_t)cu[a.n_seqs], n));
   uint4 *p = reinterpret_cast<uint4 *>(out);
-  const int64_t w = width / 8;
-  for (int64_t i = threadIdx.x; i < lo * w; i += blockDim.x) p[i] = make_uint4(0u, 0u, 0u, 0u);
-  for (int64_t i = hi * w + threadIdx.x; i < n * w; i += blockDim.x) p[i] = make_uint4(0u, 0u, 0u, 0u);
+  const int64_t w = width / 8, step = (int64_t)a.n_rest * CR_THREADS;
+  const int64_t first = (int64_t)(gridDim.x - 1 - blockIdx.x) * CR_THREADS + threadIdx.x;
+  for (int64_t i = first; i < lo * w; i += step) p[i] = make_uint4(0u, 0u, 0u, 0u);
+  for (int64_t i = hi * w + first; i < n * w; i += step) p[i] = make_uint4(0u, 0u, 0u, 0u);
 }
 
 // ------------------------------------------------------------------ forward
@@ -194,8 +197,8 @@ template <class T, int D, int CT>
 __global__ void __launch_bounds__(CR_THREADS, 2) cross_forward_kernel(CrossArgs a) {
   constexpr int KC = D / 16, DT = D / 32;
   __shared__ __attribute__((aligned(256))) uint8_t lds[2][2][CrLds<D>::BYTES];
-  if (blockIdx.x + 1 == gridDim.x) {
-    if (a.zero_rest) cr_zero_rest(a.out, a.cu_q, a.n_seqs, a.n_q, (int64_t)a.n_q_heads * D);
+  if (cr_is_rest(a)) {
+    cr_zero_rest(a, a.out, a.cu_q, a.n_q, (int64_t)a.n_q_heads * D);
     return;
   }
   const CrItem it = cr_item(a);
@@ -402,8 +405,8 @@ template <class T, int D>
 __global__ void __launch_bounds__(CR_THREADS, D == 64 ? 3 : 2) cross_dq_kernel(CrossArgs a) {
   constexpr int CT = 1, KC = D / 16, DT = D / 32;
   __shared__ __attribute__((aligned(256))) uint8_t lds[2][2][CrLds<D>::BYTES];
-  if (blockIdx.x + 1 == gridDim.x) {
-    cr_zero_rest(a.out, a.cu_q, a.n_seqs, a.n_q, (int64_t)a.n_q_heads * D);
+  if (cr_is_rest(a)) {
+    cr_zero_rest(a, a.out, a.cu_q, a.n_q, (int64_t)a.n_q_heads * D);
     return;
   }
   const CrItem it = cr_item(a);
@@ -532,9 +535,9 @@ __global__ void __launch_bounds__(CR_THREADS, D == 64 ? 3 : 2) cross_dkv_kernel(
   __shared__ __attribute__((aligned(256))) uint8_t lv[32 * CR_WAVES * VRows::ROW];  // V's rows
   __shared__ __attribute__((aligned(256))) uint8_t lds[2][2][CrLds<D, R>::BYTES];
   __shared__ __attribute__((aligned(16))) float sm_lse[2][R], sm_delta[2][R];
-  if (blockIdx.x + 1 == gridDim.x) {
-    cr_zero_rest(a.dk, a.cu_k, a.n_seqs, a.n_k, (int64_t)a.n_kv_heads * D);
-    cr_zero_rest(a.dv, a.cu_k, a.n_seqs, a.n_k, (int64_t)a.n_kv_heads * D);
+  if (cr_is_rest(a)) {
+    cr_zero_rest(a, a.dk, a.cu_k, a.n_k, (int64_t)a.n_kv_heads * D);
+    cr_zero_rest(a, a.dv, a.cu_k, a.n_k, (int64_t)a.n_kv_heads * D);
     return;
   }
   const CrItem it = cr_item(a);
@@ -555,13 +558,9 @@ __global__ void __launch_bounds__(CR_THREADS, D == 64 ? 3 : 2) cross_dkv_kernel(
   {
     const int64_t row = ks.lo + max(0, min(wk + (lane & 31), keys - 1));
     const uint16_t *kp = a.k.p + row * a.k.row + it.h * a.k.head + 8 * (lane >> 5);
-    // keys that are not there: zeros (what memory holds in their place may be NaN)
+    // (keys that are not there are columns of their own: cleared where they are written)
 #pragma unroll
-    for (int kc = 0; kc < KC; ++kc) {
-      const att_u32x4 w = *reinterpret_cast<const att_u32x4 *>(kp + 16 * kc);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) k[kc][i] = live ? w[i] : 0u;
-    }
+    for (int kc = 0; kc < KC; ++kc) k[kc] = *reinterpret_cast<const att_u32x4 *>(kp + 16 * kc);
     const uint16_t *vp = a.v.p + ks.lo * a.v.row + it.h * a.v.head;
     for (int i = threadIdx.x; i < 32 * CR_WAVES * D / 8; i += CR_THREADS) {
       const int r = i / (D / 8), c = i % (D / 8);
@@ -626,8 +625,7 @@ __global__ void __launch_bounds__(CR_THREADS, D == 64 ? 3 : 2) cross_dkv_kernel(
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int i = 4 * i4 + j;
-        const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], scale, -lse[j]));
-        x[i] = live ? w : 0.0f;
+        x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], scale, -lse[j]));
         y[i] = x[i] * unbias * (dp[i] - delta[j]);
       }
     }
@@ -652,8 +650,8 @@ __global__ void __launch_bounds__(CR_THREADS, D == 64 ? 3 : 2) cross_dkv_kernel(
       float x[4], y[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        x[j] = dk[dt][i + j] * a.sm_scale;
-        y[j] = dv[dt][i + j] * unbias;
+        x[j] = live ? dk[dt][i + j] * a.sm_scale : 0.0f;
+        y[j] = live ? dv[dt][i + j] * unbias : 0.0f;
       }
       const int64_t w = at + 32 * dt + 2 * i;
       if (a.n_split == 1) {
@@ -772,7 +770,8 @@ static int cr_check(const char *what, int dtype, const CrossArgs &a, int32_t hea
   ZX_REQUIRE(a.n_q_heads % a.n_kv_heads == 0, "%s: n_q_heads must be a multiple of n_kv_heads", what);
   if (head_dim != 64 && head_dim != 128)
     return fail(ZX_ERR_UNSUPPORTED, "%s: head_dim %d not in {64, 128}", what, head_dim);
-  if (a.n_q >= (1LL << 31) || a.n_k >= (1LL << 31) || a.n_q * a.n_q_heads >= (1LL << 31) || a.n_k * a.n_kv_heads >= (1LL << 31))
+  constexpr int64_t MOST = (1LL << 31) - 4096;  // rounded up to tiles they fit 31 bits
+  if (a.n_q >= MOST || a.n_k >= MOST || a.n_q * a.n_q_heads >= MOST || a.n_k * a.n_kv_heads >= MOST)
     return fail(ZX_ERR_UNSUPPORTED, "%s: too many rows", what);
   return ZX_OK;
 }
@@ -795,7 +794,7 @@ static void cr_group(CrossArgs &a) {
 }
 
 template <class T, int D> static int cr_forward(CrossArgs a, const CrossPlan &p, hipStream_t st) {
-  const unsigned grid = cr_grid(a) + 1;
+  const unsigned grid = cr_grid(a);
   if (D == 64 && p.ct == 2) cross_forward_kernel<T, 64, 2><<<grid, CR_THREADS, 0, st>>>(a);
   else cross_forward_kernel<T, D, 1><<<grid, CR_THREADS, 0, st>>>(a);
   const int rc = check_launch("cross_forward");
@@ -830,7 +829,7 @@ extern "C" int zx_cross_attention(int dtype, const void *q, int64_t n_q, int64_t
   a.n_seqs = n_seqs;
   a.max_q = max_q_per_seq;
   a.max_k = max_k_per_seq;
-  a.zero_rest = flags & ZX_CROSS_ZERO_REST ? 1 : 0;
+  a.n_rest = flags & ZX_CROSS_ZERO_REST ? (int32_t)CR_REST : 0;
   a.sm_scale = sm_scale;
   int rc = cr_check("cross_attention", dtype, a, head_dim);
   if (rc) return rc;
@@ -849,7 +848,7 @@ extern "C" int zx_cross_attention(int dtype, const void *q, int64_t n_q, int64_t
   a.n_tile = (int32_t)p.n_tile;
   a.n_split = (int32_t)p.n_split;
   a.order = cr_order(n_seqs, a.max_k / p.n_split);
-  if (8 * ceil_div((int64_t)n_seqs * n_kv_heads, 8) * p.n_tile * p.n_split >= (1LL << 31) - 1)
+  if (8 * ceil_div((int64_t)n_seqs * n_kv_heads, 8) * p.n_tile * p.n_split >= (1LL << 31) - CR_REST)
     return fail(ZX_ERR_UNSUPPORTED, "cross_attention: too many sequences");
   const hipStream_t st = as_stream(stream);
   if (dtype == ZX_BF16) return head_dim == 64 ? cr_forward<CrBf16, 64>(a, p, st) : cr_forward<CrBf16, 128>(a, p, st);
@@ -863,7 +862,7 @@ static int cr_backward(CrossArgs a, const CrossPlan &pq, const CrossPlan &pk, ui
   a.n_tile = (int32_t)pq.n_tile;
   a.n_split = (int32_t)pq.n_split;
   a.order = cr_order(a.n_seqs, a.max_k / pq.n_split);
-  cross_dq_kernel<T, D><<<cr_grid(a) + 1, CR_THREADS, 0, st>>>(a);
+  cross_dq_kernel<T, D><<<cr_grid(a), CR_THREADS, 0, st>>>(a);
   if ((rc = check_launch("cross_dq"))) return rc;
   const int64_t wq = (int64_t)a.n_q_heads * D, wk = (int64_t)a.n_kv_heads * D;
   if (pq.n_split > 1 && a.n_q) {
@@ -875,7 +874,7 @@ static int cr_backward(CrossArgs a, const CrossPlan &pq, const CrossPlan &pk, ui
   a.n_tile = (int32_t)pk.n_tile;
   a.n_split = (int32_t)pk.n_split;
   a.order = cr_order(a.n_seqs, (int64_t)a.max_q * a.group / pk.n_split);
-  cross_dkv_kernel<T, D><<<cr_grid(a) + 1, CR_THREADS, 0, st>>>(a);
+  cross_dkv_kernel<T, D><<<cr_grid(a), CR_THREADS, 0, st>>>(a);
   if ((rc = check_launch("cross_dkv")) || pk.n_split == 1) return rc;
   for (int i = 0; i < 2; ++i) {
     cross_sum_kernel<T><<<(unsigned)ceil_div(a.n_k * wk, 8 * 256), 256, 0, st>>>(
@@ -912,7 +911,7 @@ extern "C" int zx_cross_attention_backward(
   a.n_seqs = n_seqs;
   a.max_q = max_q_per_seq;
   a.max_k = max_k_per_seq;
-  a.zero_rest = 1;
+  a.n_rest = (int32_t)CR_REST;
   a.sm_scale = sm_scale;
   int rc = cr_check("cross_attention_backward", dtype, a, head_dim);
   if (rc) return rc;
@@ -940,7 +939,7 @@ extern "C" int zx_cross_attention_backward(
   a.delta = static_cast<float *>(workspace);
   a.part = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + bytes.delta);
   const int64_t pairs8 = 8 * ceil_div((int64_t)n_seqs * n_kv_heads, 8);
-  if (pairs8 * std::max(pq.n_tile * pq.n_split, pk.n_tile * pk.n_split) >= (1LL << 31) - 1)
+  if (pairs8 * std::max(pq.n_tile * pq.n_split, pk.n_tile * pk.n_split) >= (1LL << 31) - CR_REST)
     return fail(ZX_ERR_UNSUPPORTED, "cross_attention_backward: too many sequences");
   const hipStream_t st = as_stream(stream);
   uint16_t *d = static_cast<uint16_t *>(dq);
