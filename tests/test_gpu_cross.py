@@ -439,3 +439,24 @@ def test_no_rows_no_keys(dev):
         assert y.shape == q.shape and (y == 0).all()
         y.backward(torch.ones_like(y))
         assert (q.grad == 0).all() and (k.grad == 0).all()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("rows, keys", [([40, 9], [1, 1]), ([3], [100])])
+def test_one_key_has_no_gradient(dev, D, rows, keys):
+    """Where all of a row's weight is on one key (the others, if any, at scores 40 below in log2), dS is
+    p (dP - p dP): p is 1 within 2^-20 (scores and log-sum-exp as the tolerances above), nothing else rounds."""
+    q, k, v, g = inputs(dev, torch.bfloat16, rows, keys, 2, 2, D, 11)
+    q, k = q.abs(), k.abs()
+    if keys[0] > 1:
+        k[1:] = 0
+        k[0] = 8
+        q = torch.ones_like(q) * 4
+    cu_q, cu_k = starts(rows, dev), starts(keys, dev)
+    out, lse = kv.cross_attention(q, k, v, cu_q, cu_k, return_lse=True)
+    dq, dk, _ = kv.cross_attention_backward(g, q, k, v, out, lse, cu_q, cu_k)
+    most = float((g.double().abs().sum(-1).max() * v.abs().max()))  # |dP|
+    size = float((q.double().abs().sum(-1).max() * k.abs().max())) * D ** -0.5
+    off = most * 2 * (2 * (D + 4) * 2.0 ** -24 * size + 2.0 ** -20)
+    assert dq.abs().max() <= off * float(k.abs().max()) * D ** -0.5 * sum(keys)
+    assert dk.abs().max() <= off * float(q.abs().max()) * D ** -0.5 * sum(rows)

@@ -427,8 +427,14 @@ __global__ void __launch_bounds__(CR_THREADS, D == 64 ? 3 : 2) cross_dq_kernel(C
   cols.load(a.g, g);
   float lse[CT], delta[CT];
   cr_f32x16 dq[CT][DT];
+  const bool few = a.n_split == 1 && keys <= 2 * CR_TILE;
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
+    const int64_t at = (int64_t)cols.head[ct] * a.n_q + cols.row[ct];
+    lse[ct] = a.lse[at];
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) dq[ct][dt] = cr_zero();
+    if (few) continue;
     const uint16_t *p = a.o.p + cols.row[ct] * a.o.row + cols.head[ct] * a.o.head + 8 * (lane >> 5);
     float sum = 0.0f;
 #pragma unroll
@@ -441,11 +447,7 @@ __global__ void __launch_bounds__(CR_THREADS, D == 64 ? 3 : 2) cross_dq_kernel(C
       }
     }
     delta[ct] = cr_halves_sum(sum);
-    const int64_t at = (int64_t)cols.head[ct] * a.n_q + cols.row[ct];
-    lse[ct] = a.lse[at];
     if (it.split == 0 && cols.live[ct] && lane < 32) a.delta[at] = delta[ct];
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) dq[ct][dt] = cr_zero();
   }
   const float scale = a.sm_scale * ATT_LOG2E;
   const uint16_t *kp = a.k.p + ks.lo * a.k.row + it.h * a.k.head, *vp = a.v.p + ks.lo * a.v.row + it.h * a.v.head;
@@ -458,23 +460,26 @@ __global__ void __launch_bounds__(CR_THREADS, D == 64 ? 3 : 2) cross_dq_kernel(C
     sk.store(lds[buf][0], min(CR_TILE, t_end - t));
     sv.store(lds[buf][1], min(CR_TILE, t_end - t));
   };
+  auto products = [&](int buf, int kt, cr_f32x16 (&s)[CT], cr_f32x16 (&dp)[CT]) {
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) s[ct] = dp[ct] = cr_zero();
+#pragma unroll
+    for (int kc = 0; kc < KC; ++kc) {
+      const att_u32x4 k = cr_rows<D>(lds[buf][0], kt, kc, lane), v = cr_rows<D>(lds[buf][1], kt, kc, lane);
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
+        s[ct] = T::mfma(k, q[ct][kc], s[ct]);
+        dp[ct] = T::mfma(v, g[ct][kc], dp[ct]);
+      }
+    }
+  };
   auto compute = [&](int buf, int t) {
     if (work) {
-      uint8_t *lk = lds[buf][0], *lv = lds[buf][1];
+      uint8_t *lk = lds[buf][0];
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt) {
         cr_f32x16 s[CT], dp[CT];
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct) s[ct] = dp[ct] = cr_zero();
-#pragma unroll
-        for (int kc = 0; kc < KC; ++kc) {
-          const att_u32x4 k = cr_rows<D>(lk, kt, kc, lane), v = cr_rows<D>(lv, kt, kc, lane);
-#pragma unroll
-          for (int ct = 0; ct < CT; ++ct) {
-            s[ct] = T::mfma(k, q[ct][kc], s[ct]);
-            dp[ct] = T::mfma(v, g[ct][kc], dp[ct]);
-          }
-        }
+        products(buf, kt, s, dp);
         att_u32x4 ds[CT][2];
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) {
@@ -500,7 +505,41 @@ __global__ void __launch_bounds__(CR_THREADS, D == 64 ? 3 : 2) cross_dq_kernel(C
       }
     }
   };
-  cr_pipeline(t_begin, t_end, CR_TILE, load, store, compute);
+  if (few) {
+    // All the keys fit the two buffers: D_r = sum_t p dP, which needs no rounded out.  (What out's last
+    // rounding adds to dS weighs the more the fewer the keys: of dq's error at 6 keys a third.)
+    for (int t = 0, buf = 0; t < t_end; t += CR_TILE, ++buf) {
+      load(t);
+      store(buf, t);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) delta[ct] = 0.0f;
+    if (work) {
+      for (int t = 0, buf = 0; t < t_end; t += CR_TILE, ++buf) {
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) {
+          cr_f32x16 s[CT], dp[CT];
+          products(buf, kt, s, dp);
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[ct][i], scale, -lse[ct])) * dp[ct][i];
+              delta[ct] += t + 32 * kt + cr_row(i, lane) < t_end ? x : 0.0f;
+            }
+        }
+      }
+    }
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      delta[ct] = cr_halves_sum(delta[ct]);
+      if (cols.live[ct] && lane < 32) a.delta[(int64_t)cols.head[ct] * a.n_q + cols.row[ct]] = delta[ct];
+    }
+    for (int t = 0, buf = 0; t < t_end; t += CR_TILE, ++buf) compute(buf, t);
+  } else {
+    cr_pipeline(t_begin, t_end, CR_TILE, load, store, compute);
+  }
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
     if (!cols.live[ct]) continue;
