@@ -391,3 +391,19 @@ def test_wrappers_refuse(dev):
     pool = torch.zeros((9, 2, 2, 8, 128), dtype=torch.uint8, device=dev)
     with pytest.raises(ValueError, match="multiple of 16"):
         kv.paged_attention_shared(t.q, pool, t.scales, t.bt, t.seq_lens, t.cu_group, t.shared)
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+def test_rows_out_of_order_are_flagged(dev, bits):
+    """cu_q or groups that go back: flagged, no access outside what there is (rows that lie before their
+    group's first take no part of it), and a good call afterwards is as before."""
+    t = Batch(dev, bits, [(6, 96)], [20] * 6, [2] * 6, 8, 2, 128, 16, seed=17)
+    want = t.call(check=True)
+    for cu in ([0, 10, 5, 12, 12, 12, 12], [0, 9, 1, 9, 1, 9, 12], [12, 10, 8, 6, 4, 2, 0]):
+        for groups, shared in (([0, 6], [96]), ([0, 1, 6], [0, 96]), ([0, 6, 2, 6], [96, 96, 96])):
+            cu_q, t.cu_q, t.cu_group, t.shared = t.cu_q, i32(cu, dev), i32(groups, dev), i32(shared, dev)
+            err = torch.zeros(1, dtype=torch.int32, device=dev)
+            t.call(max_q_per_seq=12, err=err)
+            assert int(err) & N.ZX_KERR_POS_RANGE
+            t.cu_q, t.cu_group, t.shared = cu_q, i32([0, 6], dev), i32([96], dev)
+    assert torch.equal(t.call(check=True), want)

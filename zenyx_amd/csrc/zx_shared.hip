@@ -10,8 +10,9 @@
 //
 // The group's keys: a tile is up to 16 CT columns (pairs of query row and head) of all the
 // group's rows, so that a key that is read and converted serves many sequences; bound by the matrix
-// products, conversions and exponentials of AttnWave once the columns are many, by the reads of
-// the pages where they are few.  A sequence's own keys: its own rows' columns, bound by the reads.
+// products, conversions and exponentials of AttnWave (of sh_wide: 128 columns, FP8 pages at D = 128) once
+// the columns are many, by the reads of the pages where they are few.  A sequence's own keys: its own
+// rows' columns, bound by the reads.
 // Both in one launch: blocks [0, n_pre) of a head take pieces of the groups' tiles, the others
 // equal runs of the sequences' own units; how many of each, and how long the pieces are, every
 // block finds from the lengths (on the device, so that a captured call may be replayed on
@@ -56,9 +57,9 @@ struct SharedSeq {
   uint32_t first;   // its first own unit
   uint32_t units;   // own units of each of its row tiles
   uint32_t parts;   // parts of its shared keys
-  uint32_t pad;
-  int64_t slot;     // of part 0 of its shared keys, for row 0 of q: row r's is slot + r
-  int64_t step;     // slots from one part to the next
+  int32_t row0;     // the group's first row of q
+  int64_t slot;     // of part 0 of its shared keys, for that row
+  int64_t step;     // slots from one part to the next: the group's rows
 };
 struct SharedTable {
   uint32_t *head;  // [2]: q, r of the deal
@@ -123,7 +124,7 @@ __device__ __forceinline__ ShSeq sh_seq(const SharedArgs &a, int32_t b, int32_t 
   s.rows = 1;
   if (a.cu_q) {
     const int64_t lo = a.cu_q[b], hi = a.cu_q[b + 1];
-    if (lo < 0 || hi > a.n_q || hi - lo > a.most) e |= ZX_KERR_POS_RANGE;
+    if (lo < 0 || hi < lo || hi > a.n_q || hi - lo > a.most) e |= ZX_KERR_POS_RANGE;
     s.row0 = lo;
     s.rows = lo < 0 ? 0 : (int32_t)max((int64_t)0, min(min(hi, a.n_q) - lo, (int64_t)a.most));
   }
@@ -336,7 +337,7 @@ __device__ __forceinline__ void sh_write_table(const SharedArgs &a, const ShPlan
     const uint32_t units = b < a.n_seqs ? s.units() : 0u, n = units * s.tiles(a);
     uint32_t all;
     const uint32_t in = sh_scan(n, all, lds, 0);
-    if (b < a.n_seqs) t.seq[b] = SharedSeq{before + in - n, units, 0u, 0u, 0, 0};
+    if (b < a.n_seqs) t.seq[b] = SharedSeq{before + in - n, units, 0u, 0, 0, 0};
     before += all;
   }
   uint32_t slots = 0;
@@ -359,10 +360,11 @@ __device__ __forceinline__ void sh_write_table(const SharedArgs &a, const ShPlan
     }
     const uint32_t ir = sh_scan(rows, all, lds, 0);  // (and behind its barriers the entries above are written)
     const uint32_t slot = slots + ir - rows;
-    if (parts && (int64_t)slot + rows <= a.pre_slots)
+    if (parts && (uint64_t)slot + (uint64_t)parts * (uint64_t)n_rows <= (uint64_t)a.pre_slots)
       for (int32_t b = first; b < last; ++b) {
         t.seq[b].parts = parts;
-        t.seq[b].slot = (int64_t)slot - row0;
+        t.seq[b].row0 = (int32_t)row0;
+        t.seq[b].slot = slot;
         t.seq[b].step = n_rows;
       }
     slots += all;
@@ -793,8 +795,9 @@ template <int D> __global__ void __launch_bounds__(256) shared_combine_kernel(Sh
   const SharedSeq s = t.seq[b];
   const int64_t row_part = (int64_t)a.n_q_heads * (2 + D), at_head = (int64_t)hq * (2 + D);
   ShParts c = {};
-  if (s.parts) {
-    c.p[0] = a.pre + (s.slot + row) * row_part + at_head;
+  // (a row outside its group's: cu_q out of order, which is flagged)
+  if (s.parts && row >= s.row0 && row - s.row0 < s.step) {
+    c.p[0] = a.pre + (s.slot + row - s.row0) * row_part + at_head;
     c.step[0] = s.step * row_part;
     c.n[0] = (int)s.parts;
   }
