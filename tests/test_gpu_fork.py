@@ -4,6 +4,7 @@ import pytest
 import torch
 
 from zenyx_amd import kv
+from zenyx_amd.train.cross_attention import CrossAttention
 from zenyx_amd.train.fp8_kv_quantization import PagedFP4KVCache, PagedFP8KVCache, QuantizedRingAttention
 from zenyx_amd.train.rotary import RotaryPositions
 
@@ -175,3 +176,87 @@ def test_cached_states_read_by_rows_of_several_sequences(dev):
                         k.abs().transpose(1, 2)).amax() * 128 ** -0.5 * 2.0 ** -8
     tol = 2.0 ** -8 * want.abs() + (2.0 ** -10 + 2.0 ** -8 + 2 * float(size)) * float(v.abs().max())
     assert ((out.double() - want).abs() <= tol).all()
+
+
+def test_precisions_of_forks(dev, monkeypatch):
+    """What attention to shared pages has the bits for takes it; "exact" over FP8 pages, with more, does not."""
+    monkeypatch.setattr(PagedFP8KVCache, "_LEAST_SAVED", 1)
+    calls = []
+    for name in ("paged_attention_shared", "paged_attention4_shared"):
+        f = getattr(kv, name)
+        monkeypatch.setattr(kv, name, lambda *a, f=f, **k: calls.append(1) or f(*a, **k))
+    q = torch.randn((3, 4, 128), device=dev, dtype=torch.bfloat16)
+    for C, takes in ((PagedFP8KVCache, {"f16": 2, "bf16": 2, "exact": 0}),
+                     (PagedFP4KVCache, {"f16": 2, "bf16": 2, "exact": 2})):
+        c = C(1, 2, 128, 60, 16)
+        c.append(tokens(100, 1, 2, 128, 0, dev), ["p"], [100])
+        c.fork("p", ["a", "b"])
+        for precision, n in takes.items():
+            del calls[:]
+            att = QuantizedRingAttention(c, precision=precision)
+            a, b = att.decode(q, 0, ["p", "a", "b"]), att(q, 0, ["p", "a", "b"], [1, 1, 1])
+            assert len(calls) == n
+            assert ((a.float() - b.float()).abs() <= 2 * (2.0 ** -7 * b.float().abs() + 2.0 ** -7 * float(
+                c.gather(0, ["p"])[1].abs().max()))).all()
+
+
+def test_ids_again_and_again(dev, monkeypatch):
+    """One sequence twice in a batch, ids freed and taken again by others, forks of forks whose source is
+    gone, and groups that shrink as the batch changes: always what each sequence's own table says."""
+    monkeypatch.setattr(PagedFP8KVCache, "_LEAST_SAVED", 1)
+    # (scales are those of the first tokens: others may saturate, in both alike)
+    c, w = (PagedFP8KVCache(1, 2, 64, 200, 16, overflow="saturate") for _ in range(2))
+    x, y = tokens(100, 1, 2, 64, 0, dev), tokens(50, 1, 2, 64, 1, dev)
+    c.append(x, ["p"], [100])
+    c.fork("p", ["a", "b"])
+    c.fork("a", ["c", "d"], length=70)
+    c.free("a"), c.free("p")
+    c.append(y, ["p"], [50])       # another sequence of that name
+    c.fork("c", ["a"])
+    w.append(x, ["b"], [100])
+    first = x[:, :70].contiguous()
+    for s in ("c", "d", "a"):
+        w.append(first, [s], [70])
+    w.append(y, ["p"], [50])
+    att, plain = (QuantizedRingAttention(k, check=True) for k in (c, w))
+    for batch in (["b", "c", "d", "a", "p"], ["a", "a", "p", "c"], ["d", "b"], ["p", "d", "p", "d"], ["c"]):
+        q = torch.randn((len(batch), 4, 64), device=dev, dtype=torch.bfloat16)
+        a, b = att.decode(q, 0, batch), plain.decode(q, 0, batch)
+        vmax = float(w.gather(0, batch)[1].abs().max())
+        assert ((a.float() - b.float()).abs() <= 2 * (2.0 ** -7 * b.float().abs() + 2.0 ** -10 * vmax)).all()
+    for s in ("b", "c", "d", "a", "p"):
+        c.free(s)
+    assert len(c._free) == 200 and not c._users and not c._common
+
+
+def test_training_and_serving_see_the_same(dev, monkeypatch):
+    """An encoder's states of two sources, projected; a step of training on them, and serving from 4-bit pages
+    that the rows' sequences are forks of.  What the pages hold is exact in bf16: cross attention to it and
+    attention to the shared pages are off by a bf16 step (2^-8 of the value) each, weights rounded to bf16
+    by another 2 x 2^-8 max|V| (numerator and sum), those of the pages 2^-15, fp32 sums 2^-15."""
+    monkeypatch.setattr(PagedFP8KVCache, "_LEAST_SAVED", 1)
+    D, H, Hq, lens = 128, 2, 8, [700, 1031]
+    g = torch.Generator(device=dev).manual_seed(0)
+    states = torch.randn((sum(lens), 64), generator=g, device=dev, dtype=torch.bfloat16)
+    w = (torch.randn((64, 2 * H * D), generator=g, device=dev, dtype=torch.bfloat16) / 8).requires_grad_()
+    wq = (torch.randn((64, Hq * D), generator=g, device=dev, dtype=torch.bfloat16) / 8).requires_grad_()
+    rows = [6, 9]  # decoder rows of each source
+    x = torch.randn((sum(rows), 64), generator=g, device=dev, dtype=torch.bfloat16)
+    cu_q, cu_k = (torch.tensor([0, n[0], sum(n)], dtype=torch.int32, device=dev) for n in (rows, lens))
+    q, kvs = (x @ wq).view(-1, Hq, D), (states @ w).view(-1, 2, H, D)
+    out = CrossAttention()(q, kvs[:, 0], kvs[:, 1], cu_q, cu_k, max_q_per_seq=9, max_k_per_seq=1031)
+    out.float().square().mean().backward()
+    assert all(torch.isfinite(p.grad).all() and p.grad.any() for p in (w, wq))
+    c = PagedFP4KVCache(1, H, D, 300, 16)
+    c.append(kvs.detach()[None].contiguous(), ["s0", "s1"], lens)
+    ids = [f"s{b}-{i}" for b in range(2) for i in range(rows[b])]
+    for b in range(2):
+        c.fork(f"s{b}", [s for s in ids if s.startswith(f"s{b}")])
+    q = q.detach()
+    served = QuantizedRingAttention(c, causal=False).decode(q, 0, ids)
+    k, v = c.gather(0, ["s0", "s1"])
+    held = [torch.cat([t[b, :, :n].transpose(0, 1) for b, n in enumerate(lens)]) for t in (k, v)]
+    want = kv.cross_attention(q, *held, cu_q, cu_k)
+    vmax = float(held[1].abs().max())
+    tol = 2 * 2.0 ** -8 * want.float().abs() * (1 + 2.0 ** -8) + (2 * 2.0 ** -8 + 2.0 ** -14) * vmax
+    assert ((served.float() - want.float()).abs() <= tol).all()

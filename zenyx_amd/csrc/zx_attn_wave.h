@@ -221,7 +221,7 @@ struct AttnPages {
     return (uint32_t)(((uint64_t)t * p_magic) >> (31 + p_shift));
   }
   // The page of position t (uniform), by the scalar cache: a vector load of it would be waited for
-  // together with the loads of K and V before it (shared pages, 128 x 32k positions 187 -> 105 us).
+  // together with the loads of K and V before it (shared pages, 128 x 32k positions 187 -> 135 us).
   __device__ __forceinline__ int32_t page_id(uint32_t t) const {
     typedef const __attribute__((address_space(4))) int32_t *scalar;
     return reinterpret_cast<scalar>(reinterpret_cast<uintptr_t>(bt))[page_of(t)];

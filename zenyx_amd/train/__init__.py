@@ -4,4 +4,5 @@
 ``dynamic_ring_curriculum`` (ring degree per training step and the page traces it
 implies) and ``fp8_kv_quantization`` (per-head FP8 KV quantisation, a paged FP8 KV
 cache, a paged 4-bit one and ring attention reading them); beside them ``rotary`` (rotary
-positions, which those caches can apply to their keys)."""
+positions, which those caches can apply to their keys) and ``cross_attention`` (attention to an
+encoder's states, with its gradients)."""

@@ -81,7 +81,7 @@ class PagedFP8KVCache:
     # 5 us more to start (decode's / this one's time, 32/8 heads, D = 128: 16 sequences on 2,048 shared
     # positions 20.2 / 20.2 us, on 4,096 28 / 23, 4 on 16,384 30 / 26, 64 on 16,384 244 / 50).
     _LEAST_SAVED = 49152
-    _SHARED_PRECISIONS = ("f16",)  # of QuantizedRingAttention's, what that kernel computes
+    _SHARED_PRECISIONS = ("f16", "bf16")  # of QuantizedRingAttention's, those that kernel has the bits for
 
     def __init__(self, num_layers: int, num_kv_heads: int, head_dim: int, num_pages: int,
                  page_size: int = 16, device: torch.device | None = None, overflow: str = "raise", rope=None):
@@ -453,7 +453,7 @@ class PagedFP4KVCache(PagedFP8KVCache):
     and an append needs no earlier one.  A block of 32 that holds a NaN or an infinity is NaN.
     ``head_dim`` 64, 128 or 256, ``page_size`` a multiple of 16.  ``scales`` is None."""
 
-    _SHARED_PRECISIONS = ("f16", "exact")
+    _SHARED_PRECISIONS = ("f16", "bf16", "exact")
 
     def __init__(self, num_layers: int, num_kv_heads: int, head_dim: int, num_pages: int, page_size: int = 16,
                  device: torch.device | None = None, rope=None):
@@ -504,8 +504,9 @@ class QuantizedRingAttention:
     of a ring's shards), and ``precision`` "f16" is given as "exact": the 4-bit kernels have no
     fp16 weights, and "bf16" has fewer bits.  Neighbours of a batch that share pages
     (``PagedFP8KVCache.fork``) attend to them together, in ``decode`` and in calls of few rows per
-    sequence: the shared keys are read and multiplied once for all of them.  A cache with ``rope`` has rotated its keys: the queries are rotated here, by the
-    positions of the tokens they stand for."""
+    sequence: the shared keys are read and multiplied once for all of them (over FP8 pages not with
+    "exact", whose weights have more bits).  A cache with ``rope`` has rotated its keys: the queries
+    are rotated here, by the positions of the tokens they stand for."""
 
     _FEW_ROWS = 8  # of a sequence, for which shared pages are attended to together
 
@@ -525,6 +526,9 @@ class QuantizedRingAttention:
         # and errors surface at the cache's next check_errors
         self.check = check
 
+    def _groups(self, seq_ids: list):
+        return self.cache._groups(seq_ids) if self.precision in self.cache._SHARED_PRECISIONS else None
+
     def __call__(self, q: torch.Tensor, layer: int, seq_ids: list, q_lens: list[int]) -> torch.Tensor:
         """q ``[n_q, Hq, D]`` bf16: the queries of ``seq_ids[i]`` packed in order, ``q_lens[i]``
         rows each, standing for that sequence's newest ``q_lens[i]`` cached tokens (the
@@ -542,8 +546,7 @@ class QuantizedRingAttention:
             q = c.rope(q, shift + torch.arange(q.shape[0], dtype=torch.int32, device=q.device))
         most = max(q_lens, default=0)
         # few rows per sequence (proposed tokens): bound by what they read of shared pages
-        few = 0 < most <= self._FEW_ROWS and self.precision in c._SHARED_PRECISIONS
-        groups = c._groups(seq_ids) if few else None
+        groups = self._groups(seq_ids) if 0 < most <= self._FEW_ROWS else None
         if groups is not None:
             out = c._attend_shared(q, layer, c._tables(seq_ids), lens, groups, self, cu, most)
         else:
@@ -558,7 +561,7 @@ class QuantizedRingAttention:
         q, lens = q.to(c.device).contiguous(), c._lengths(seq_ids)
         if c.rope is not None:
             q = c.rope(q, lens - 1)
-        groups = c._groups(seq_ids)
+        groups = self._groups(seq_ids)
         if groups is not None:
             out = c._attend_shared(q, layer, c._tables(seq_ids), lens, groups, self)
         else:
