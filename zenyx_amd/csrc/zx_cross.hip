@@ -28,6 +28,7 @@ struct CrIn {
   const uint16_t *p;
   int64_t row, head;
 };
+constexpr int32_t CR_BY_KEYS = 1, CR_BY_ROWS = 2;
 struct CrossArgs {
   CrIn q, k, v, o, g;       // g: the output's gradient
   const int32_t *cu_q, *cu_k, *k_lens;
@@ -43,7 +44,7 @@ struct CrossArgs {
   int32_t n_rest;           // blocks behind the others that clear the rows in no sequence
   uint32_t g_magic;         // c / group = (c * g_magic) >> (31 + g_shift) for c < 2^31
   int32_t g_shift;
-  int32_t order;            // the sequences with the most work first
+  int32_t order;            // CR_BY_KEYS, CR_BY_ROWS: the sequences with the longest blocks first; 0: as they come
   float sm_scale;
 };
 
@@ -70,8 +71,9 @@ __device__ __forceinline__ int32_t cr_keys(const CrossArgs &a, int32_t b, int32_
 
 // What a block does: tiles of one sequence and KV head on the same XCD (block ids go round the
 // eight), so that what they read in common is in its L2; where blocks are long (cr_order) the
-// sequences with the most work first: the chip is left with short ones at the end (1,000-2,048 rows on
-// 2,000-8,192 keys, 4 sequences, 32/8 heads, D = 128: 611 -> 569 us).
+// sequences with the longest blocks first: the chip is left with short ones at the end (8 x 200-1,000 rows
+// on 1,000-8,000 keys, 32/8 heads, D = 128: 350 -> 316 us, against those with the most pairs first; dk
+// and dv of 4 x 1,000-2,048 rows on 2,000-8,192 gain 30 of 1,200).
 struct CrItem {
   int32_t b, h, tile, split;
   bool any;
@@ -90,7 +92,7 @@ __device__ __forceinline__ CrItem cr_item(const CrossArgs &a) {
     float w = -1.0f;
     if (lane < a.n_seqs) {
       const int32_t keys = a.cu_k[lane + 1] - a.cu_k[lane];
-      w = (float)(a.cu_q[lane + 1] - a.cu_q[lane]) * (float)(a.k_lens ? min(a.k_lens[lane], keys) : keys);
+      w = (float)(a.order == CR_BY_ROWS ? a.cu_q[lane + 1] - a.cu_q[lane] : a.k_lens ? min(a.k_lens[lane], keys) : keys);
     }
     int before = lane < a.n_seqs ? 0 : 64;
     for (int s = 0; s < a.n_seqs; ++s) {
@@ -129,13 +131,13 @@ template <int D, int R = CR_TILE> struct CrStage {
   }
 };
 
-// Tiles [t_begin, t_end) in steps of `step` through two LDS buffers: load(t) issues a tile's loads,
-// store(buffer, t) writes them to LDS, compute(buffer, t) works on it.  (Loads two tiles ahead at
+// Tiles [t_begin, t_end) in steps of `step` through two LDS buffers: load(t) issues a tile's loads (the
+// first one's are under way, before the block reads its columns: 8 x 4,096 rows on 77 keys 29.6 -> 27.6
+// us), store(buffer, t) writes them to LDS, compute(buffer, t) works on it.  (Loads two tiles ahead at
 // D = 64 took the same time, or 4% more where they cost registers.)
 template <class Load, class Store, class Compute>
 __device__ __forceinline__ void cr_pipeline(int t_begin, int t_end, int step, Load load, Store store, Compute compute) {
   if (t_begin >= t_end) return;
-  load(t_begin);
   store(0, t_begin);
   __syncthreads();
   int buf = 0;
@@ -212,6 +214,13 @@ __global__ void __launch_bounds__(CR_THREADS, 2) cross_forward_kernel(CrossArgs 
   const int keys = cr_keys(a, it.b, ks.n), units = (keys + CR_TILE - 1) / CR_TILE;
   const int t_begin = (int)((int64_t)units * it.split / a.n_split) * CR_TILE;
   const int t_end = min(keys, (int)((int64_t)units * (it.split + 1) / a.n_split) * CR_TILE);
+  const uint16_t *kp = a.k.p + ks.lo * a.k.row + it.h * a.k.head, *vp = a.v.p + ks.lo * a.v.row + it.h * a.v.head;
+  CrStage<D> sk, sv;
+  auto load = [&](int t) {
+    sk.load(kp + t * a.k.row, (uint32_t)a.k.row, min(CR_TILE, t_end - t));
+    sv.load(vp + t * a.v.row, (uint32_t)a.v.row, min(CR_TILE, t_end - t));
+  };
+  if (t_begin < t_end) load(t_begin);
   const CrCols<D, CT> cols(a, c0, n_cols, it.h, qs.lo);
   const bool work = c0 + 32 * CT * wave < n_cols;  // uniform in the wave
   att_u32x4 q[CT][KC];
@@ -236,12 +245,6 @@ __global__ void __launch_bounds__(CR_THREADS, 2) cross_forward_kernel(CrossArgs 
 #pragma unroll
         for (int i = 0; i < 4; ++i) q[ct][kc][i] = (q[ct][kc][i] ^ flip) & keep;
   }
-  const uint16_t *kp = a.k.p + ks.lo * a.k.row + it.h * a.k.head, *vp = a.v.p + ks.lo * a.v.row + it.h * a.v.head;
-  CrStage<D> sk, sv;
-  auto load = [&](int t) {
-    sk.load(kp + t * a.k.row, (uint32_t)a.k.row, min(CR_TILE, t_end - t));
-    sv.load(vp + t * a.v.row, (uint32_t)a.v.row, min(CR_TILE, t_end - t));
-  };
   auto store = [&](int buf, int t) {
     sk.store(lds[buf][0], min(CR_TILE, t_end - t));
     sv.store(lds[buf][1], min(CR_TILE, t_end - t));
@@ -420,6 +423,14 @@ __global__ void __launch_bounds__(CR_THREADS, D == 64 ? 3 : 2) cross_dq_kernel(C
   const int keys = cr_keys(a, it.b, ks.n), units = (keys + CR_TILE - 1) / CR_TILE;
   const int t_begin = (int)((int64_t)units * it.split / a.n_split) * CR_TILE;
   const int t_end = min(keys, (int)((int64_t)units * (it.split + 1) / a.n_split) * CR_TILE);
+  const uint16_t *kp = a.k.p + ks.lo * a.k.row + it.h * a.k.head, *vp = a.v.p + ks.lo * a.v.row + it.h * a.v.head;
+  CrStage<D> sk, sv;
+  auto load = [&](int t) {
+    sk.load(kp + t * a.k.row, (uint32_t)a.k.row, min(CR_TILE, t_end - t));
+    sv.load(vp + t * a.v.row, (uint32_t)a.v.row, min(CR_TILE, t_end - t));
+  };
+  constexpr bool EARLY = D == 64;  // (at D = 128 ten registers would be spilled)
+  if (EARLY && t_begin < t_end) load(t_begin);
   const CrCols<D, CT> cols(a, c0, n_cols, it.h, qs.lo);
   const bool work = c0 + 32 * CT * wave < n_cols;
   att_u32x4 q[CT][KC], g[CT][KC];
@@ -450,12 +461,6 @@ __global__ void __launch_bounds__(CR_THREADS, D == 64 ? 3 : 2) cross_dq_kernel(C
     if (it.split == 0 && cols.live[ct] && lane < 32) a.delta[at] = delta[ct];
   }
   const float scale = a.sm_scale * ATT_LOG2E;
-  const uint16_t *kp = a.k.p + ks.lo * a.k.row + it.h * a.k.head, *vp = a.v.p + ks.lo * a.v.row + it.h * a.v.head;
-  CrStage<D> sk, sv;
-  auto load = [&](int t) {
-    sk.load(kp + t * a.k.row, (uint32_t)a.k.row, min(CR_TILE, t_end - t));
-    sv.load(vp + t * a.v.row, (uint32_t)a.v.row, min(CR_TILE, t_end - t));
-  };
   auto store = [&](int buf, int t) {
     sk.store(lds[buf][0], min(CR_TILE, t_end - t));
     sv.store(lds[buf][1], min(CR_TILE, t_end - t));
@@ -509,7 +514,7 @@ __global__ void __launch_bounds__(CR_THREADS, D == 64 ? 3 : 2) cross_dq_kernel(C
     // All the keys fit the two buffers: D_r = sum_t p dP, which needs no rounded out.  (What out's last
     // rounding adds to dS weighs the more the fewer the keys: of dq's error at 6 keys a third.)
     for (int t = 0, buf = 0; t < t_end; t += CR_TILE, ++buf) {
-      load(t);
+      if (!EARLY || t) load(t);
       store(buf, t);
     }
     __syncthreads();
@@ -538,6 +543,7 @@ __global__ void __launch_bounds__(CR_THREADS, D == 64 ? 3 : 2) cross_dq_kernel(C
     }
     for (int t = 0, buf = 0; t < t_end; t += CR_TILE, ++buf) compute(buf, t);
   } else {
+    if (!EARLY && t_begin < t_end) load(t_begin);
     cr_pipeline(t_begin, t_end, CR_TILE, load, store, compute);
   }
 #pragma unroll
@@ -600,13 +606,6 @@ __global__ void __launch_bounds__(CR_THREADS, D == 64 ? 3 : 2) cross_dkv_kernel(
     // (keys that are not there are columns of their own: cleared where they are written)
 #pragma unroll
     for (int kc = 0; kc < KC; ++kc) k[kc] = *reinterpret_cast<const att_u32x4 *>(kp + 16 * kc);
-    const uint16_t *vp = a.v.p + ks.lo * a.v.row + it.h * a.v.head;
-    for (int i = threadIdx.x; i < 32 * CR_WAVES * D / 8; i += CR_THREADS) {
-      const int r = i / (D / 8), c = i % (D / 8);
-      uint4 w = make_uint4(0u, 0u, 0u, 0u);
-      if (key0 + r < keys) w = *reinterpret_cast<const uint4 *>(vp + (key0 + r) * a.v.row + 8 * c);
-      *reinterpret_cast<uint4 *>(VRows::at(lv, r, 16 * c)) = w;
-    }
   }
   uint8_t *const my_v = VRows::at(lv, 32 * wave + (lane & 31), 16 * (lane >> 5));
 #pragma unroll
@@ -635,6 +634,16 @@ __global__ void __launch_bounds__(CR_THREADS, D == 64 ? 3 : 2) cross_dkv_kernel(
       my_delta = a.delta[at];
     }
   };
+  if (t_begin < t_end) load(t_begin);
+  {
+    const uint16_t *vp = a.v.p + ks.lo * a.v.row + it.h * a.v.head;
+    for (int i = threadIdx.x; i < 32 * CR_WAVES * D / 8; i += CR_THREADS) {
+      const int r = i / (D / 8), c = i % (D / 8);
+      uint4 w = make_uint4(0u, 0u, 0u, 0u);
+      if (key0 + r < keys) w = *reinterpret_cast<const uint4 *>(vp + (key0 + r) * a.v.row + 8 * c);
+      *reinterpret_cast<uint4 *>(VRows::at(lv, r, 16 * c)) = w;
+    }
+  }
   auto store = [&](int buf, int t) {
     const int n = min(R, t_end - t);
     sq.store(lds[buf][0], n);
@@ -704,17 +713,21 @@ __global__ void __launch_bounds__(CR_THREADS, D == 64 ? 3 : 2) cross_dkv_kernel(
     }
 }
 
-// Sums of the parts of a gradient, in order: [n_split] parts `step` floats apart, 8 values per thread.
+// Sums of the parts of a gradient, in order: [n_split] parts `step` floats apart, 8 values per thread;
+// blocks of y = 1: of a second one, whose parts lie behind the first one's.
 template <class T>
-__global__ void __launch_bounds__(256) cross_sum_kernel(const float *part, int64_t step, int32_t n_split, uint16_t *out,
-                                                        const int32_t *cu, int32_t n_seqs, int64_t n, int64_t width,
+__global__ void __launch_bounds__(256) cross_sum_kernel(const float *part, int64_t step, int32_t n_split, uint16_t *out0,
+                                                        uint16_t *out1, const int32_t *cu, int32_t n_seqs, int64_t n, int64_t width,
                                                         int32_t most) {
   const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
   if (at >= n * width) return;
   const int64_t row = at / width;
   const int32_t b = cr_seq_of(cu, n_seqs, row);
   if (b < 0 || row - cu[b] >= most) return;  // zeros already, or not computed
+  uint16_t *out = blockIdx.y ? out1 : out0;
+  if (blockIdx.y) part += n * width;
   float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll 4
   for (int s = 0; s < n_split; ++s) {
     const att_f32x4 *p = reinterpret_cast<const att_f32x4 *>(part + s * step + at);
     const att_f32x4 u = p[0], v = p[1];
@@ -739,7 +752,9 @@ struct CrossPlan {
   int64_t n_tile, n_split;
 };
 // Ranking the sequences costs every block about 1 us per 64 of them: for blocks of 16 tiles and more.
-static int32_t cr_order(int32_t n_seqs, int64_t length) { return n_seqs > 1 && n_seqs <= 64 && length >= 16 * CR_TILE; }
+static int32_t cr_order(int32_t n_seqs, int64_t length, int32_t by) {
+  return n_seqs > 1 && n_seqs <= 64 && length >= 16 * CR_TILE ? by : 0;
+}
 static CrossPlan cr_plan(int64_t pairs, int64_t columns, int64_t length, int ct, int64_t per_cu, int64_t units_least) {
   CrossPlan p;
   p.ct = ct;
@@ -886,7 +901,7 @@ extern "C" int zx_cross_attention(int dtype, const void *q, int64_t n_q, int64_t
                 cr_forward_bytes(p, n_q, n_q_heads, head_dim));
   a.n_tile = (int32_t)p.n_tile;
   a.n_split = (int32_t)p.n_split;
-  a.order = cr_order(n_seqs, a.max_k / p.n_split);
+  a.order = cr_order(n_seqs, a.max_k / p.n_split, CR_BY_KEYS);
   if (8 * ceil_div((int64_t)n_seqs * n_kv_heads, 8) * p.n_tile * p.n_split >= (1LL << 31) - CR_REST)
     return fail(ZX_ERR_UNSUPPORTED, "cross_attention: too many sequences");
   const hipStream_t st = as_stream(stream);
@@ -900,27 +915,24 @@ static int cr_backward(CrossArgs a, const CrossPlan &pq, const CrossPlan &pk, ui
   a.out = dq;
   a.n_tile = (int32_t)pq.n_tile;
   a.n_split = (int32_t)pq.n_split;
-  a.order = cr_order(a.n_seqs, a.max_k / pq.n_split);
+  a.order = cr_order(a.n_seqs, a.max_k / pq.n_split, CR_BY_KEYS);
   cross_dq_kernel<T, D><<<cr_grid(a), CR_THREADS, 0, st>>>(a);
   if ((rc = check_launch("cross_dq"))) return rc;
   const int64_t wq = (int64_t)a.n_q_heads * D, wk = (int64_t)a.n_kv_heads * D;
   if (pq.n_split > 1 && a.n_q) {
-    cross_sum_kernel<T><<<(unsigned)ceil_div(a.n_q * wq, 8 * 256), 256, 0, st>>>(a.part, a.n_q * wq, a.n_split, dq, a.cu_q,
-                                                                                a.n_seqs, a.n_q, wq, a.max_q);
+    cross_sum_kernel<T><<<(unsigned)ceil_div(a.n_q * wq, 8 * 256), 256, 0, st>>>(a.part, a.n_q * wq, a.n_split, dq, nullptr,
+                                                                                a.cu_q, a.n_seqs, a.n_q, wq, a.max_q);
     if ((rc = check_launch("cross_sum"))) return rc;
   }
   if (a.n_k == 0) return ZX_OK;
   a.n_tile = (int32_t)pk.n_tile;
   a.n_split = (int32_t)pk.n_split;
-  a.order = cr_order(a.n_seqs, (int64_t)a.max_q * a.group / pk.n_split);
+  a.order = cr_order(a.n_seqs, (int64_t)a.max_q * a.group / pk.n_split, CR_BY_ROWS);
   cross_dkv_kernel<T, D><<<cr_grid(a), CR_THREADS, 0, st>>>(a);
   if ((rc = check_launch("cross_dkv")) || pk.n_split == 1) return rc;
-  for (int i = 0; i < 2; ++i) {
-    cross_sum_kernel<T><<<(unsigned)ceil_div(a.n_k * wk, 8 * 256), 256, 0, st>>>(
-        a.part + i * a.n_k * wk, 2 * a.n_k * wk, a.n_split, i ? a.dv : a.dk, a.cu_k, a.n_seqs, a.n_k, wk, a.max_k);
-    if ((rc = check_launch("cross_sum"))) return rc;
-  }
-  return ZX_OK;
+  cross_sum_kernel<T><<<dim3((unsigned)ceil_div(a.n_k * wk, 8 * 256), 2), 256, 0, st>>>(
+      a.part, 2 * a.n_k * wk, a.n_split, a.dk, a.dv, a.cu_k, a.n_seqs, a.n_k, wk, a.max_k);
+  return check_launch("cross_sum");
 }
 
 extern "C" int zx_cross_attention_backward(
