@@ -460,3 +460,16 @@ def test_one_key_has_no_gradient(dev, D, rows, keys):
     off = most * 2 * (2 * (D + 4) * 2.0 ** -24 * size + 2.0 ** -20)
     assert dq.abs().max() <= off * float(k.abs().max()) * D ** -0.5 * sum(keys)
     assert dk.abs().max() <= off * float(q.abs().max()) * D ** -0.5 * sum(rows)
+
+
+def test_out_in_place(dev):
+    """out may be q itself (a block reads its rows before it writes them), but not lie in k or v."""
+    for rows, keys in (([300, 40], [500, 900]), ([2, 3], [5000, 40])):
+        q, k, v, _ = inputs(dev, torch.bfloat16, rows, keys, 4, 2, 64, 12)
+        cu_q, cu_k = starts(rows, dev), starts(keys, dev)
+        want = kv.cross_attention(q, k, v, cu_q, cu_k)
+        assert torch.equal(kv.cross_attention(q, k, v, cu_q, cu_k, out=q), want)
+    both = torch.zeros((2, 10, 2, 64), dtype=torch.bfloat16, device=dev)
+    cu = starts([10], dev)
+    with pytest.raises(ValueError, match="memory"):
+        kv.cross_attention(both[0].clone(), both[0], both[1], cu, cu, out=both[0])

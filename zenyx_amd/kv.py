@@ -1390,6 +1390,8 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: tor
         if out.shape != q.shape or out.dtype != q.dtype:
             raise ValueError(f"out must be {q.dtype} {tuple(q.shape)}")
         _all_on(index, out=out)
+        if any(t.untyped_storage().data_ptr() == out.untyped_storage().data_ptr() for t in (k, v) if t.numel()):
+            raise ValueError("out must not lie in k's or v's memory")
     lse = torch.empty((Hq, n_q), dtype=torch.float32, device=q.device) if return_lse else None
     with _on(index):
         ws, nb = _workspace_for("zx_cross_attention_workspace_bytes", index, n_q, Hq, Hkv, D, B, mq, mk)
