@@ -473,3 +473,38 @@ def test_out_in_place(dev):
     cu = starts([10], dev)
     with pytest.raises(ValueError, match="memory"):
         kv.cross_attention(both[0].clone(), both[0], both[1], cu, cu, out=both[0])
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("D, Hq, Hkv", [(64, 3, 1), (128, 2, 2)])
+def test_around_the_tiles_ends(dev, kind, D, Hq, Hkv):
+    """Keys around one and two tiles, by themselves and as the first ones of longer padded states; rows
+    around a wave's and a block's columns."""
+    t, h, tiny = TYPES[kind]
+    lens = [63, 64, 65, 127, 128, 129, 1, 0, 192]
+    rows = [31, 32, 33, 127, 128, 129, 2, 5, 1]
+    q, k, v, g = inputs(dev, t, rows, lens, Hq, Hkv, D, 13)
+    cu_q, cu_k = starts(rows, dev), starts(lens, dev)
+    want, tol = exact(q, k, v, g, rows, lens, h, tiny, D ** -0.5)
+    out, lse = kv.cross_attention(q, k, v, cu_q, cu_k, return_lse=True, check=True)
+    near(out, want[0], tol[0], "out")
+    grads = kv.cross_attention_backward(g, q, k, v, out, lse, cu_q, cu_k, check=True)
+    for x, w, e, name in zip(grads, want[1:], tol[1:], ("dq", "dk", "dv")):
+        near(x, w, e, name)
+    S = 200
+    pk, pv = (torch.full((S * len(lens), Hkv, D), float("nan"), dtype=t, device=dev) for _ in range(2))
+    at = 0
+    for b, n in enumerate(lens):
+        pk[b * S:b * S + n], pv[b * S:b * S + n] = k[at:at + n], v[at:at + n]
+        at += n
+    cu_p, k_lens = starts([S] * len(lens), dev), i32(lens, dev)
+    o, e = kv.cross_attention(q, pk, pv, cu_q, cu_p, k_lens, return_lse=True, check=True)
+    near(o, want[0], tol[0], "padded out")
+    dq, dk, dv = kv.cross_attention_backward(g, q, pk, pv, o, e, cu_q, cu_p, k_lens, check=True)
+    near(dq, want[1], tol[1], "padded dq")
+    at = 0
+    for b, n in enumerate(lens):
+        near(dk[b * S:b * S + n], want[2][at:at + n], tol[2][at:at + n], "padded dk") if n else None
+        near(dv[b * S:b * S + n], want[3][at:at + n], tol[3][at:at + n], "padded dv") if n else None
+        assert (dk[b * S + n:(b + 1) * S] == 0).all() and (dv[b * S + n:(b + 1) * S] == 0).all()
+        at += n
