@@ -565,9 +565,9 @@ int zx_paged_attention4_prefill(const uint16_t *q, int64_t n_q, const int32_t *c
  * multiplied once for all the group's rows.  Positions from shared_lens[g] (rounded down to a
  * multiple of 16) on are read through each sequence's own table; a sequence in no group has
  * only those.  Rows [cu_q[b], cu_q[b + 1]) of q [n_q][n_q_heads][head_dim] bf16 are sequence b's
- * newest (cu_q NULL: a row each, n_q == n_seqs): row i of n is at position seq_lens[b] - n + i and
- * sees, when `causal`, the keys up to it, otherwise all seq_lens[b].  out is that of attention over
- * every sequence's own table, whatever the sequences of a group have in common beyond it.
+ * newest (cu_q NULL: a row each, n_q == n_seqs): row i of n, n as cu_q has it whatever the call
+ * computes of them, is at position seq_lens[b] - n + i and sees, when `causal`, the keys up to it,
+ * otherwise all seq_lens[b].  out is that of attention over every sequence's own table, whatever the sequences of a group have in common beyond it.
  * n_groups may be 0.  A row without a key gives zeros; rows beyond max_q_per_seq (host) or in no
  * sequence are left unwritten, rows that cu_q claims beyond n_q do not exist (either sets
  * ZX_KERR_POS_RANGE, as lengths beyond max_blocks * page_size, which are clipped, and groups that

@@ -114,6 +114,7 @@ __device__ __forceinline__ int32_t sh_group_of(const SharedArgs &a, int32_t b) {
 struct ShSeq {
   int64_t row0;
   int32_t rows, g;
+  int32_t all;          // rows that cu_q gives it, computed or not: row i is at position keys - all + i
   uint32_t keys, from;  // keys there are, and the first that is not the group's
   __device__ __forceinline__ uint32_t units() const { return keys > from ? (keys - from + (SH_UNIT - 1)) / SH_UNIT : 0u; }
   __device__ __forceinline__ uint32_t tiles(const SharedArgs &a) const { return (uint32_t)((rows + a.rows_o - 1) / a.rows_o); }
@@ -121,12 +122,13 @@ struct ShSeq {
 __device__ __forceinline__ ShSeq sh_seq(const SharedArgs &a, int32_t b, int32_t &e) {
   ShSeq s;
   s.row0 = b;
-  s.rows = 1;
+  s.rows = s.all = 1;
   if (a.cu_q) {
     const int64_t lo = a.cu_q[b], hi = a.cu_q[b + 1];
     if (lo < 0 || hi < lo || hi > a.n_q || hi - lo > a.most) e |= ZX_KERR_POS_RANGE;
     s.row0 = lo;
     s.rows = lo < 0 ? 0 : (int32_t)max((int64_t)0, min(min(hi, a.n_q) - lo, (int64_t)a.most));
+    s.all = lo < 0 ? 0 : (int32_t)max((int64_t)0, hi - lo);
   }
   const int32_t len = a.seq_lens[b];
   if (len > 0 && (uint32_t)len > a.cap) e |= ZX_KERR_POS_RANGE;
@@ -664,19 +666,21 @@ __global__ void __launch_bounds__(ATT_THREADS, sh_per_cu(F::DIM, CT)) paged_shar
         const int64_t row = row0 + r;
         int32_t b = (int32_t)row;
         int64_t behind = 0;  // rows of the sequence after this one
-        if (ROWS && a.cu_q) {
-          b = b0;
-          int32_t hi = b1 - 1;
-          while (b < hi) {
-            const int32_t mid = (b + hi + 1) >> 1;
-            if (a.cu_q[mid] <= row) b = mid;
-            else hi = mid - 1;
+        if (a.cu_q) {
+          if (ROWS) {
+            b = b0;
+            int32_t hi = b1 - 1;
+            while (b < hi) {
+              const int32_t mid = (b + hi + 1) >> 1;
+              if (a.cu_q[mid] <= row) b = mid;
+              else hi = mid - 1;
+            }
+          } else {  // one row each is computed: sequences without one between them
+            b = aw_seq_of(a.cu_q, a.n_seqs, (int32_t)row);
           }
           behind = a.causal ? (int64_t)a.cu_q[b + 1] - 1 - row : 0;
-        } else if (a.cu_q) {  // one row each at most: sequences without one between them
-          b = aw_seq_of(a.cu_q, a.n_seqs, (int32_t)row);
         }
-        return (uint32_t)min(max((int64_t)a.seq_lens[b] - behind, (int64_t)0), (int64_t)a.cap);
+        return (uint32_t)max(min((int64_t)a.seq_lens[b], (int64_t)a.cap) - behind, (int64_t)0);
       };
       auto part = [&](int r) { return a.pre + (int64_t)(slot + r) * row_part; };
       const int cols = n_rows * G;
@@ -715,13 +719,13 @@ __global__ void __launch_bounds__(ATT_THREADS, sh_per_cu(F::DIM, CT)) paged_shar
           continue;
         }
         const uint32_t keys = sh_uni(s.keys), from = sh_uni(s.from);
-        const int rows = sh_uni(s.rows);
+        const int rows = sh_uni(s.rows), all = sh_uni(s.all);
         const uint32_t rt = (u - base) / units, u0 = (u - base) - rt * units;
         const uint32_t u1 = min(units, u0 + (u_end - u));
         const int r0 = (int)rt * a.rows_o, n_rows = min(a.rows_o, rows - r0);
-        // keys that row r of the tile sees
+        // keys that row r of the tile sees (one row: t_end below says it)
         auto lim = [&](int r) -> uint32_t {
-          return ROWS && a.causal ? (uint32_t)max((int64_t)keys - (rows - 1 - r0 - r), (int64_t)0) : keys;
+          return a.causal ? (uint32_t)max((int64_t)keys - (all - 1 - r0 - r), (int64_t)0) : keys;
         };
         const uint32_t t_begin = from + u0 * SH_UNIT;
         const uint32_t t_end = min(min(keys, from + u1 * SH_UNIT), lim(n_rows - 1));

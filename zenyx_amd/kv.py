@@ -1307,7 +1307,7 @@ def paged_attention_shared(q: torch.Tensor, pool_layer: torch.Tensor, scales_lay
     of every sequence, row i of n at position ``seq_lens[b] - n + i``, which sees the keys up to it
     (all of them when not ``causal``).  ``max_q_per_seq`` bounds a sequence's rows (read back from
     ``cu_q`` without it, which waits for the device); rows beyond it, and rows in no sequence, are
-    left as they are in ``out``.  Pages of a multiple of 16 tokens, head_dim 64, 128 or 256.
+    left as they are in ``out`` (and the others are at the positions that ``cu_q`` gives them).  Pages of a multiple of 16 tokens, head_dim 64, 128 or 256.
     Softmax weights are rounded to fp16: error within one bf16 ulp + 2^-10 max|V|.  ``err``
     (device int32 ``[1]``) collects the kernels' error bits; ``check`` reads them and raises."""
     if scales_layer is None:
