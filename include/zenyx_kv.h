@@ -610,9 +610,11 @@ int zx_paged_attention4_shared(const uint16_t *q, int64_t n_q, const int32_t *cu
  * of exponentials.  A row without a key gives zeros and -inf.  Scores and sums in fp32, softmax
  * weights rounded once to dtype (fp16: times 2^7): |error| <= half an ulp + 2^-8 max|v| (fp16: 2^-11).
  * Rows beyond max_q_per_seq and keys beyond max_k_per_seq (both host) are not computed or seen, nor
- * do rows that cu_q or cu_k claim beyond n_q or n_k exist (either sets ZX_KERR_POS_RANGE).  Rows in no
- * sequence are left unwritten, with ZX_CROSS_ZERO_REST zeros.  head_dim 64 or 128.  workspace: the
- * query's device bytes (0: NULL will do), 16-byte aligned; it holds nothing between calls. */
+ * do rows that cu_q or cu_k claim beyond n_q or n_k exist, nor are sequences computed that begin
+ * before row 0 (each sets ZX_KERR_POS_RANGE).  Rows that are not computed, those in no sequence among
+ * them, are left unwritten; with ZX_CROSS_ZERO_REST they are zeros in out (in lse2 left).  head_dim 64
+ * or 128.  workspace: the query's device bytes (0: NULL will do), 16-byte aligned; it holds nothing
+ * between calls. */
 enum zx_cross_flags { ZX_CROSS_ZERO_REST = 1 };
 size_t zx_cross_attention_workspace_bytes(int64_t n_q, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim,
                                           int32_t n_seqs, int32_t max_q_per_seq, int32_t max_k_per_seq);
@@ -623,8 +625,8 @@ int zx_cross_attention(int dtype, const void *q, int64_t n_q, int64_t q_row_stri
                        int32_t max_q_per_seq, int32_t max_k_per_seq, float sm_scale, int32_t flags, void *out,
                        float *lse2, int32_t *err, void *workspace, size_t workspace_bytes, zx_stream_t stream);
 /* Its gradients, from the output's (strided as q), out and lse2 as zx_cross_attention left them: dq, dk,
- * dv contiguous, of rows in no sequence zeros.  The score's gradients are rounded once to dtype
- * (fp16: they have to be below 65504), every sum is in fp32 and in a fixed order. */
+ * dv contiguous, zeros for rows and keys that are not computed or seen.  The score's gradients are
+ * rounded once to dtype (fp16: they have to be below 65504), every sum is in fp32 and in a fixed order. */
 size_t zx_cross_attention_backward_workspace_bytes(int64_t n_q, int64_t n_k, int32_t n_q_heads, int32_t n_kv_heads,
                                                    int32_t head_dim, int32_t n_seqs, int32_t max_q_per_seq,
                                                    int32_t max_k_per_seq);

@@ -55,15 +55,17 @@ __device__ __forceinline__ uint32_t cr_pair(const CrossArgs &a, uint32_t c, uint
   return r;
 }
 
-// Rows [lo, hi) of the packed n that sequence b has, none outside and at most `most`.
+// Rows of the packed n that sequence b has: [lo, end), none outside, of which [lo, lo + n) are computed (at
+// most `most`, and none of a sequence that begins before the first row).
 struct CrSpan {
-  int64_t lo;
+  int64_t lo, end;
   int32_t n;
 };
 __device__ __forceinline__ CrSpan cr_span(const int32_t *cu, int32_t b, int64_t n, int32_t most, int32_t &e) {
   const int64_t lo = cu[b], hi = cu[b + 1];
   if (lo < 0 || hi > n || hi - lo > most || hi < lo) e |= ZX_KERR_POS_RANGE;
-  return CrSpan{lo < 0 ? 0 : lo, lo < 0 ? 0 : (int32_t)max((int64_t)0, min(min(hi, n) - lo, (int64_t)most))};
+  const int64_t from = max(lo, (int64_t)0), end = max(from, min(hi, n));
+  return CrSpan{from, end, lo < 0 ? 0 : (int32_t)min(end - from, (int64_t)most)};
 }
 __device__ __forceinline__ int32_t cr_keys(const CrossArgs &a, int32_t b, int32_t n) {
   return a.k_lens ? max(0, min(a.k_lens[b], n)) : n;
@@ -193,6 +195,17 @@ __device__ __forceinline__ void cr_zero_rest(const CrossArgs &a, uint16_t *out, 
   for (int64_t i = hi * w + first; i < n * w; i += step) p[i] = make_uint4(0u, 0u, 0u, 0u);
 }
 
+// Rows of a sequence that are not computed: zeros, by the first block of the sequence and KV head (`at`: its first
+// element of a row, `width` elements).
+__device__ __forceinline__ void cr_zero_behind(const CrItem &it, const CrSpan &s, uint16_t *out, int64_t row, int64_t at,
+                                               int32_t width) {
+  if (it.tile != 0 || it.split != 0 || s.lo + s.n >= s.end) return;  // uniform
+  const int32_t w = width / 8;
+  out += (s.lo + s.n) * row + at;
+  for (int64_t i = threadIdx.x; i < (s.end - s.lo - s.n) * w; i += CR_THREADS)
+    *reinterpret_cast<uint4 *>(out + i / w * row + 8 * (i % w)) = make_uint4(0u, 0u, 0u, 0u);
+}
+
 // ------------------------------------------------------------------ forward
 
 template <class T, int D, int CT>
@@ -208,6 +221,7 @@ __global__ void __launch_bounds__(CR_THREADS, 2) cross_forward_kernel(CrossArgs 
   int32_t e = 0;
   const CrSpan qs = cr_span(a.cu_q, it.b, a.n_q, a.max_q, e), ks = cr_span(a.cu_k, it.b, a.n_k, a.max_k, e);
   if (e && a.err && threadIdx.x == 0) atomicOr(a.err, e);
+  if (a.n_rest) cr_zero_behind(it, qs, a.out, (int64_t)a.n_q_heads * D, (int64_t)it.h * a.group * D, a.group * D);
   const int n_cols = qs.n * a.group, c0 = it.tile * 32 * CT * CR_WAVES;
   if (c0 >= n_cols) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -351,23 +365,22 @@ __global__ void __launch_bounds__(CR_THREADS, 2) cross_forward_kernel(CrossArgs 
   }
 }
 
-// The sequence of a packed row, or -1.
-__device__ __forceinline__ int32_t cr_seq_of(const int32_t *cu, int32_t n_seqs, int64_t row) {
+// The sequence that computes a packed row, or -1: none, or the row is beyond what is computed of it (cr_span).
+__device__ __forceinline__ int32_t cr_seq_of(const int32_t *cu, int32_t n_seqs, int64_t row, int32_t most) {
   int32_t lo = 0, hi = n_seqs - 1;
   while (lo < hi) {
     const int32_t mid = (lo + hi + 1) >> 1;
     if (cu[mid] <= row) lo = mid;
     else hi = mid - 1;
   }
-  return row >= cu[lo] && row < cu[lo + 1] ? lo : -1;
+  return cu[lo] >= 0 && row >= cu[lo] && row < cu[lo + 1] && row - cu[lo] < most ? lo : -1;
 }
 
 // Rows whose keys were cut: D threads per (row, head).
 template <class T, int D> __global__ void __launch_bounds__(256) cross_merge_kernel(CrossArgs a) {
   const int64_t at = (int64_t)blockIdx.x * (256 / D) + threadIdx.x / D, row = at / a.n_q_heads;
   if (row >= a.n_q) return;
-  const int32_t b = cr_seq_of(a.cu_q, a.n_seqs, row);
-  if (b < 0 || row - a.cu_q[b] >= a.max_q) return;
+  if (cr_seq_of(a.cu_q, a.n_seqs, row, a.max_q) < 0) return;
   const int d = threadIdx.x % D;
   const int64_t step = a.n_q * a.n_q_heads * (2 + D);
   const float *pp = a.part + at * (2 + D);
@@ -417,6 +430,7 @@ __global__ void __launch_bounds__(CR_THREADS, D == 64 ? 3 : 2) cross_dq_kernel(C
   int32_t e = 0;
   const CrSpan qs = cr_span(a.cu_q, it.b, a.n_q, a.max_q, e), ks = cr_span(a.cu_k, it.b, a.n_k, a.max_k, e);
   if (e && a.err && threadIdx.x == 0) atomicOr(a.err, e);
+  cr_zero_behind(it, qs, a.out, (int64_t)a.n_q_heads * D, (int64_t)it.h * a.group * D, a.group * D);
   const int n_cols = qs.n * a.group, c0 = it.tile * 32 * CT * CR_WAVES;
   if (c0 >= n_cols) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -590,6 +604,8 @@ __global__ void __launch_bounds__(CR_THREADS, D == 64 ? 3 : 2) cross_dkv_kernel(
   int32_t e = 0;  // (reported with dq)
   const CrSpan qs = cr_span(a.cu_q, it.b, a.n_q, a.max_q, e), ks = cr_span(a.cu_k, it.b, a.n_k, a.max_k, e);
   const int key0 = it.tile * 32 * CR_WAVES;
+  cr_zero_behind(it, ks, a.dk, (int64_t)a.n_kv_heads * D, (int64_t)it.h * D, D);
+  cr_zero_behind(it, ks, a.dv, (int64_t)a.n_kv_heads * D, (int64_t)it.h * D, D);
   if (key0 >= ks.n) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int keys = cr_keys(a, it.b, ks.n);
@@ -722,8 +738,7 @@ __global__ void __launch_bounds__(256) cross_sum_kernel(const float *part, int64
   const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
   if (at >= n * width) return;
   const int64_t row = at / width;
-  const int32_t b = cr_seq_of(cu, n_seqs, row);
-  if (b < 0 || row - cu[b] >= most) return;  // zeros already, or not computed
+  if (cr_seq_of(cu, n_seqs, row, most) < 0) return;  // zeros already
   uint16_t *out = blockIdx.y ? out1 : out0;
   if (blockIdx.y) part += n * width;
   float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};

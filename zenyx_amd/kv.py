@@ -1374,9 +1374,11 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: tor
     D 64 or 128; views with contiguous channels may be given, e.g. the halves of a fused
     projection.  Query head i reads kv head i // (Hq / Hkv).  ``max_q_per_seq`` / ``max_k_per_seq``
     bound a sequence's rows and keys (read back without them, which waits for the device); rows
-    and keys beyond them are not computed or seen.  Rows in no sequence are left as they are in
-    ``out``, or become zeros with ``zero_rest``; a row without a key is zeros.  ``return_lse``: also float32
-    ``[Hq, n_q]``, log2 of each row's sum of exponentials (what ``cross_attention_backward`` takes).
+    and keys beyond them are not computed or seen.  Rows that are not computed, those in no sequence
+    among them, are left as they are in ``out``, or become zeros with ``zero_rest``; a row without a
+    key is zeros.  ``return_lse``: also float32
+    ``[Hq, n_q]``, log2 of each computed row's sum of exponentials (what ``cross_attention_backward``
+    takes).
     autograd does not see this call: ``train.cross_attention.CrossAttention`` is the
     differentiable form."""
     N.need_gpu()
@@ -1413,7 +1415,8 @@ def cross_attention_backward(grad: torch.Tensor, q: torch.Tensor, k: torch.Tenso
                              err: torch.Tensor | None = None):
     """``(dq, dk, dv)`` of ``cross_attention`` for its output's gradient ``grad`` (like ``q``), from ``out`` and
     ``lse`` as it returned them; the other arguments as it took them.  Each is contiguous and in
-    q's type; those of rows in no sequence and of keys beyond ``k_lens`` are zeros.  Sums are in
+    q's type; those of rows that were not computed (in no sequence, or beyond the bounds) and of keys that
+    no row saw (beyond ``k_lens`` or the bounds) are zeros.  Sums are in
     fp32 and in a fixed order (the same from call to call); the scores' gradients are rounded once to
     q's type, in f16 they have to be below 65504."""
     N.need_gpu()

@@ -48,8 +48,9 @@ class CrossAttention:
                  k_lens: torch.Tensor | None = None, max_q_per_seq: int | None = None,
                  max_k_per_seq: int | None = None) -> torch.Tensor:
         """``kv.cross_attention``, differentiable (once, in reverse mode) in q, k and v.  Rows in no
-        sequence give zeros and take no gradient.  Without ``max_q_per_seq`` and ``max_k_per_seq`` the
-        bounds are read back from ``cu_q`` and ``cu_k``, which waits for the device."""
+        sequence, and rows and keys beyond the bounds, give zeros and take no gradient.  Without
+        ``max_q_per_seq`` and ``max_k_per_seq`` the bounds are read back from ``cu_q`` and ``cu_k``,
+        which waits for the device."""
         if max_q_per_seq is None:
             max_q_per_seq = int((cu_q[1:] - cu_q[:-1]).max().item()) if cu_q.numel() > 1 else 0
         if max_k_per_seq is None:
