@@ -626,7 +626,8 @@ int zx_cross_attention(int dtype, const void *q, int64_t n_q, int64_t q_row_stri
                        float *lse2, int32_t *err, void *workspace, size_t workspace_bytes, zx_stream_t stream);
 /* Its gradients, from the output's (strided as q), out and lse2 as zx_cross_attention left them: dq, dk,
  * dv contiguous, zeros for rows and keys that are not computed or seen.  The score's gradients are
- * rounded once to dtype (fp16: they have to be below 65504), every sum is in fp32 and in a fixed order. */
+ * rounded once to dtype (fp16: times a power of two that each row of dq and key of dk has for itself, so
+ * that they may be of any size), every sum is in fp32 and in a fixed order. */
 size_t zx_cross_attention_backward_workspace_bytes(int64_t n_q, int64_t n_k, int32_t n_q_heads, int32_t n_kv_heads,
                                                    int32_t head_dim, int32_t n_seqs, int32_t max_q_per_seq,
                                                    int32_t max_k_per_seq);

@@ -31,7 +31,7 @@ struct CrBf16 {
                                                    0, 0, 0);
   }
 };
-// Weights times 2^BIAS: fp16 loses bits of what is below 2^-14.
+// Weights times 2^BIAS: fp16 loses bits of what is below 2^-14.  (bf16 has fp32's exponents.)
 struct CrF16 {
   static constexpr float BIAS = 7.0f;
   static __device__ __forceinline__ uint32_t pack(float a, float b) {

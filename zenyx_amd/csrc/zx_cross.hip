@@ -416,6 +416,41 @@ template <class T, int D> __global__ void __launch_bounds__(256) cross_merge_ker
 
 // ------------------------------------------------------------------ gradients
 
+// dS is one of the two 16-bit operands of dq's and dk's products, and in fp16 its size matters: on 1,500 keys,
+// with output gradients of 1e-4, it lies near 2^-21, where fp16 has 3 bits.  So in fp16 it is carried
+// times a power of two that every column (dq: a row, dk: a key) finds for itself and lowers when a value
+// exceeds 2^15, to where the largest is in [2^7, 2^8); what was summed before is rescaled, the sum divided at
+// the end.  So values keep fp16's 11 bits whatever the gradient's size, small ones are off by 2^-32 of the
+// largest so far at most, and none overflows.  (D = 64, 256 rows on 1,500 and 8,000 keys, gradients of 1e-4: dq
+// 1.9e-2 and 1.0e-1 off without it, 3.9e-3 and 9.3e-3 with it, which is its own last rounding; gradients of
+// 16 x 50-448 rows on 1,500 keys, 12 heads, 128 -> 133 us, of long ones at D = 128 1,973 -> 1,998.  bf16, with
+// fp32's exponents, needs none of it.)
+constexpr float CR_DS_FIRST = 0x1p64f;  // |dP| < 2^38 at D = 64 (128: 2^39): no overflow in fp32
+constexpr float CR_DS_MOST = 0x1p15f;
+template <class T> constexpr bool CR_SCALED = T::BIAS != 0.0f;
+
+// The factor by which a column whose largest of these values (over both of its lanes) is w goes down.
+__device__ __forceinline__ float cr_lower(float w) {
+  // (2^(e-1) <= w < 2^e; of an infinity e is 0)
+  return w > CR_DS_MOST ? __builtin_amdgcn_ldexpf(1.0f, min(8 - __builtin_amdgcn_frexp_expf(w), 0)) : 1.0f;
+}
+// Lowers a column's factor, with what x and `sums` have of it, where x needs that.
+template <int DT> __device__ __forceinline__ void cr_fit(float (&x)[16], float &up, cr_f32x16 (&sums)[DT]) {
+  float mx = fabsf(x[0]);
+#pragma unroll
+  for (int i = 1; i < 16; ++i) mx = __builtin_elementwise_maximum(mx, fabsf(x[i]));
+  if (__builtin_amdgcn_ballot_w64(mx > CR_DS_MOST)) {
+    const float a = cr_lower(cr_halves_max(mx));
+    up *= a;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] *= a;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sums[dt][i] *= a;
+  }
+}
+
 // dq, and on the way D_r for the other kernel.
 template <class T, int D>
 __global__ void __launch_bounds__(CR_THREADS, D == 64 ? 3 : 2) cross_dq_kernel(CrossArgs a) {
@@ -450,13 +485,14 @@ __global__ void __launch_bounds__(CR_THREADS, D == 64 ? 3 : 2) cross_dq_kernel(C
   att_u32x4 q[CT][KC], g[CT][KC];
   cols.load(a.q, q);
   cols.load(a.g, g);
-  float lse[CT], delta[CT];
+  float lse[CT], delta[CT], up[CT];
   cr_f32x16 dq[CT][DT];
   const bool few = a.n_split == 1 && keys <= 2 * CR_TILE;
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
     const int64_t at = (int64_t)cols.head[ct] * a.n_q + cols.row[ct];
     lse[ct] = a.lse[at];
+    up[ct] = CR_SCALED<T> ? CR_DS_FIRST : 1.0f;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) dq[ct][dt] = cr_zero();
     if (few) continue;
@@ -504,13 +540,16 @@ __global__ void __launch_bounds__(CR_THREADS, D == 64 ? 3 : 2) cross_dq_kernel(C
         for (int ct = 0; ct < CT; ++ct) {
           float x[16];
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[ct][i], scale, -lse[ct])) * (dp[ct][i] - delta[ct]);
+          for (int i = 0; i < 16; ++i) {
+            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[ct][i], scale, -lse[ct]));
+            x[i] = p * (CR_SCALED<T> ? __builtin_fmaf(dp[ct][i], up[ct], -delta[ct] * up[ct]) : dp[ct][i] - delta[ct]);
+          }
           if (t + CR_TILE > t_end) {  // uniform
 #pragma unroll
             for (int i = 0; i < 16; ++i)
               if (t + 32 * kt + cr_row(i, lane) >= t_end) x[i] = 0.0f;
           }
+          if constexpr (CR_SCALED<T>) cr_fit(x, up[ct], dq[ct]);
           cr_operands<T>(x, ds[ct]);
         }
 #pragma unroll
@@ -564,14 +603,15 @@ __global__ void __launch_bounds__(CR_THREADS, D == 64 ? 3 : 2) cross_dq_kernel(C
   for (int ct = 0; ct < CT; ++ct) {
     if (!cols.live[ct]) continue;
     const int64_t at = ((int64_t)cols.row[ct] * a.n_q_heads + cols.head[ct]) * D + 4 * (lane >> 5);
+    const float down = a.sm_scale / up[ct];
     if (a.n_split == 1) {
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
         for (int i = 0; i < 16; i += 4)
           *reinterpret_cast<uint2 *>(a.out + at + 32 * dt + 2 * i) =
-              make_uint2(T::pack(dq[ct][dt][i] * a.sm_scale, dq[ct][dt][i + 1] * a.sm_scale),
-                         T::pack(dq[ct][dt][i + 2] * a.sm_scale, dq[ct][dt][i + 3] * a.sm_scale));
+              make_uint2(T::pack(dq[ct][dt][i] * down, dq[ct][dt][i + 1] * down),
+                         T::pack(dq[ct][dt][i + 2] * down, dq[ct][dt][i + 3] * down));
     } else {
       float *pp = a.part + (int64_t)it.split * a.n_q * a.n_q_heads * D + at;
 #pragma unroll
@@ -579,8 +619,8 @@ __global__ void __launch_bounds__(CR_THREADS, D == 64 ? 3 : 2) cross_dq_kernel(C
 #pragma unroll
         for (int i = 0; i < 16; i += 4)
           *reinterpret_cast<float4 *>(pp + 32 * dt + 2 * i) =
-              make_float4(dq[ct][dt][i] * a.sm_scale, dq[ct][dt][i + 1] * a.sm_scale, dq[ct][dt][i + 2] * a.sm_scale,
-                          dq[ct][dt][i + 3] * a.sm_scale);
+              make_float4(dq[ct][dt][i] * down, dq[ct][dt][i + 1] * down, dq[ct][dt][i + 2] * down,
+                          dq[ct][dt][i + 3] * down);
     }
   }
 }
@@ -670,6 +710,7 @@ __global__ void __launch_bounds__(CR_THREADS, D == 64 ? 3 : 2) cross_dkv_kernel(
     }
   };
   const float unbias = __builtin_amdgcn_exp2f(-T::BIAS);
+  float up = CR_SCALED<T> ? CR_DS_FIRST * unbias : unbias;  // of dS, from the weights as they are carried
   auto compute = [&](int buf, int) {
     if (!work) return;
     uint8_t *lq = lds[buf][0], *lg = lds[buf][1];
@@ -690,9 +731,10 @@ __global__ void __launch_bounds__(CR_THREADS, D == 64 ? 3 : 2) cross_dkv_kernel(
       for (int j = 0; j < 4; ++j) {
         const int i = 4 * i4 + j;
         x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], scale, -lse[j]));
-        y[i] = x[i] * unbias * (dp[i] - delta[j]);
+        y[i] = x[i] * up * (dp[i] - delta[j]);
       }
     }
+    if constexpr (CR_SCALED<T>) cr_fit(y, up, dk);
     cr_operands<T>(x, p);
     cr_operands<T>(y, ds);
 #pragma unroll
@@ -704,6 +746,7 @@ __global__ void __launch_bounds__(CR_THREADS, D == 64 ? 3 : 2) cross_dkv_kernel(
       }
   };
   cr_pipeline(t_begin, t_end, R, load, store, compute);
+  const float down = a.sm_scale * (unbias / up);
   const int key = wk + (lane & 31);
   if (key >= ks.n) return;
   const int64_t at = ((ks.lo + key) * a.n_kv_heads + it.h) * D + 4 * (lane >> 5), all = a.n_k * a.n_kv_heads * D;
@@ -714,7 +757,7 @@ __global__ void __launch_bounds__(CR_THREADS, D == 64 ? 3 : 2) cross_dkv_kernel(
       float x[4], y[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        x[j] = live ? dk[dt][i + j] * a.sm_scale : 0.0f;
+        x[j] = live ? dk[dt][i + j] * down : 0.0f;
         y[j] = live ? dv[dt][i + j] * unbias : 0.0f;
       }
       const int64_t w = at + 32 * dt + 2 * i;

@@ -1416,9 +1416,9 @@ def cross_attention_backward(grad: torch.Tensor, q: torch.Tensor, k: torch.Tenso
     """``(dq, dk, dv)`` of ``cross_attention`` for its output's gradient ``grad`` (like ``q``), from ``out`` and
     ``lse`` as it returned them; the other arguments as it took them.  Each is contiguous and in
     q's type; those of rows that were not computed (in no sequence, or beyond the bounds) and of keys that
-    no row saw (beyond ``k_lens`` or the bounds) are zeros.  Sums are in
-    fp32 and in a fixed order (the same from call to call); the scores' gradients are rounded once to
-    q's type, in f16 they have to be below 65504."""
+    no row saw (beyond ``k_lens`` or the bounds) are zeros.  Sums are in fp32 and in a fixed order (the
+    same from call to call); the scores' gradients are rounded once to q's type, in f16 times a power of
+    two per row (dq) and per key (dk), so that small and large ones keep their bits."""
     N.need_gpu()
     index, B, mq, mk = _cross_args(q, k, v, cu_q, cu_k, k_lens, max_q_per_seq, max_k_per_seq, err)
     n_q, Hq, D = q.shape
