@@ -612,9 +612,10 @@ int zx_paged_attention4_shared(const uint16_t *q, int64_t n_q, const int32_t *cu
  * Rows beyond max_q_per_seq and keys beyond max_k_per_seq (both host) are not computed or seen, nor
  * do rows that cu_q or cu_k claim beyond n_q or n_k exist, nor are sequences computed that begin
  * before row 0 (each sets ZX_KERR_POS_RANGE).  Rows that are not computed, those in no sequence among
- * them, are left unwritten; with ZX_CROSS_ZERO_REST they are zeros in out (in lse2 left).  head_dim 64
- * or 128.  workspace: the query's device bytes (0: NULL will do), 16-byte aligned; it holds nothing
- * between calls. */
+ * them, are left unwritten; with ZX_CROSS_ZERO_REST they are zeros in out (in lse2 left).  out may be q
+ * itself (the same address and strides); what it writes must not lie otherwise between the first and the
+ * last element of q, k or v.  head_dim 64 or 128.  workspace: the query's device bytes (0: NULL will
+ * do), 16-byte aligned; it holds nothing between calls. */
 enum zx_cross_flags { ZX_CROSS_ZERO_REST = 1 };
 size_t zx_cross_attention_workspace_bytes(int64_t n_q, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim,
                                           int32_t n_seqs, int32_t max_q_per_seq, int32_t max_k_per_seq);
@@ -625,9 +626,9 @@ int zx_cross_attention(int dtype, const void *q, int64_t n_q, int64_t q_row_stri
                        int32_t max_q_per_seq, int32_t max_k_per_seq, float sm_scale, int32_t flags, void *out,
                        float *lse2, int32_t *err, void *workspace, size_t workspace_bytes, zx_stream_t stream);
 /* Its gradients, from the output's (strided as q), out and lse2 as zx_cross_attention left them: dq, dk,
- * dv contiguous, zeros for rows and keys that are not computed or seen.  The score's gradients are
- * rounded once to dtype (fp16: times a power of two that each row of dq and key of dk has for itself, so
- * that they may be of any size), every sum is in fp32 and in a fixed order. */
+ * dv contiguous, zeros for rows and keys that are not computed or seen, none in the memory of another or
+ * of an input.  The score's gradients are rounded once to dtype (fp16: times a power of two that each row
+ * of dq and key of dk has for itself, so that they may be of any size), every sum is in fp32 and in a fixed order. */
 size_t zx_cross_attention_backward_workspace_bytes(int64_t n_q, int64_t n_k, int32_t n_q_heads, int32_t n_kv_heads,
                                                    int32_t head_dim, int32_t n_seqs, int32_t max_q_per_seq,
                                                    int32_t max_k_per_seq);

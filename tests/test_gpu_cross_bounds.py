@@ -77,3 +77,26 @@ def test_sequences_out_of_order_leave_nothing_unwritten(dev, dirty, D, scale):
         lse = torch.where(lse.isnan(), 0.0, lse)
         for x in (out, *kv.cross_attention_backward(g, q, k, v, out, lse, cu_q, cu_k, **bounds)):
             assert torch.isfinite(x).all(), (cq, ck)
+
+
+def test_out_in_memory_that_inputs_have_parts_of(dev):
+    """Disjoint parts of one arena are as good as tensors of their own; what overlaps q is refused."""
+    q, k, v, _ = inputs(dev, torch.bfloat16, [40], [90], 2, 2, 64, 60)
+    cu_q, cu_k = starts([40], dev), starts([90], dev)
+    want = kv.cross_attention(q, k, v, cu_q, cu_k)
+    arena = torch.cat([x.flatten() for x in (q, k, v)] + [torch.zeros(2 * q.numel(), dtype=q.dtype, device=dev)])
+    at = [0, q.numel(), q.numel() + k.numel(), q.numel() + 2 * k.numel()]
+    parts = [arena[a:a + x.numel()].view(x.shape) for a, x in zip(at, (q, k, v))]
+    out = arena[at[3]:at[3] + q.numel()].view(q.shape)
+    assert torch.equal(kv.cross_attention(*parts, cu_q, cu_k, out=out), want)
+    assert torch.equal(parts[0], q)
+    for shift in (8, q.numel() - 8):  # over the last rows of q, and of v
+        with pytest.raises(ValueError, match="memory"):
+            kv.cross_attention(*parts, cu_q, cu_k, out=arena[at[3] - shift:][:q.numel()].view(q.shape))
+        with pytest.raises(ValueError, match="memory"):
+            kv.cross_attention(parts[0], k, v, cu_q, cu_k, out=arena[shift:][:q.numel()].view(q.shape))
+    # q's memory in another order
+    wide = torch.zeros((40, 4, 64), dtype=q.dtype, device=dev)
+    with pytest.raises(ValueError, match="memory"):
+        kv.cross_attention(wide[:, :2], k, v, cu_q, cu_k, out=wide.flatten()[:q.numel()].view(q.shape))
+    assert torch.equal(kv.cross_attention(parts[0], k, v, cu_q, cu_k, out=parts[0]), want)

@@ -897,6 +897,14 @@ static int cr_check_rows(const char *what, const char *name, const CrIn &x, int6
   return ZX_OK;
 }
 
+// Whether any of `bytes` from `out` on lies between the first and the last element of n x heads rows of x.
+static bool cr_meets(const void *out, int64_t bytes, const CrIn &x, int64_t n, int64_t heads, int64_t d) {
+  if (!out || !x.p || bytes <= 0 || n <= 0) return false;
+  typedef __int128 wide;  // (a stride is anything)
+  const wide at = (wide) reinterpret_cast<uintptr_t>(x.p), o = (wide) reinterpret_cast<uintptr_t>(out);
+  return o < at + 2 * ((n - 1) * (wide)x.row + (heads - 1) * (wide)x.head + d) && at < o + bytes;
+}
+
 static void cr_group(CrossArgs &a) {
   a.group = a.n_q_heads / a.n_kv_heads;
   int sh = 0;
@@ -962,6 +970,13 @@ extern "C" int zx_cross_attention(int dtype, const void *q, int64_t n_q, int64_t
   a.order = cr_order(n_seqs, a.max_k / p.n_split, CR_BY_KEYS);
   if (8 * ceil_div((int64_t)n_seqs * n_kv_heads, 8) * p.n_tile * p.n_split >= (1LL << 31) - CR_REST)
     return fail(ZX_ERR_UNSUPPORTED, "cross_attention: too many sequences");
+  // q itself is read by the blocks that write there, before they do
+  const int64_t width = (int64_t)n_q_heads * head_dim, bytes = 2 * n_q * width;
+  const bool in_place = out == q && (n_q == 1 || q_row == width) && (n_q_heads == 1 || q_head == head_dim);
+  ZX_REQUIRE(!cr_meets(out, bytes, a.k, n_k, n_kv_heads, head_dim) && !cr_meets(out, bytes, a.v, n_k, n_kv_heads, head_dim),
+             "cross_attention: out must not lie in k's or v's memory");
+  ZX_REQUIRE(in_place || !cr_meets(out, bytes, a.q, n_q, n_q_heads, head_dim),
+             "cross_attention: out must be q itself or not lie in its memory");
   const hipStream_t st = as_stream(stream);
   if (dtype == ZX_BF16) return head_dim == 64 ? cr_forward<CrBf16, 64>(a, p, st) : cr_forward<CrBf16, 128>(a, p, st);
   return head_dim == 64 ? cr_forward<CrF16, 64>(a, p, st) : cr_forward<CrF16, 128>(a, p, st);
@@ -1050,6 +1065,20 @@ extern "C" int zx_cross_attention_backward(
   const int64_t pairs8 = 8 * ceil_div((int64_t)n_seqs * n_kv_heads, 8);
   if (pairs8 * std::max(pq.n_tile * pq.n_split, pk.n_tile * pk.n_split) >= (1LL << 31) - CR_REST)
     return fail(ZX_ERR_UNSUPPORTED, "cross_attention_backward: too many sequences");
+  {
+    const int64_t wq = (int64_t)n_q_heads * head_dim, wk = (int64_t)n_kv_heads * head_dim;
+    struct Rows {
+      const CrIn x;
+      int64_t n, heads;
+    } const of[] = {{a.q, n_q, n_q_heads},  {a.g, n_q, n_q_heads},  {a.o, n_q, n_q_heads},
+                    {a.k, n_k, n_kv_heads}, {a.v, n_k, n_kv_heads}, {{a.dk, wk, head_dim}, n_k, n_kv_heads},
+                    {{a.dv, wk, head_dim}, n_k, n_kv_heads}};
+    bool meets = cr_meets(dk, 2 * n_k * wk, of[6].x, n_k, n_kv_heads, head_dim);
+    for (const Rows &r : of) meets = meets || cr_meets(dq, 2 * n_q * wq, r.x, r.n, r.heads, head_dim);
+    for (int i = 0; i < 5; ++i)
+      for (const void *d : {dk, dv}) meets = meets || cr_meets(d, 2 * n_k * wk, of[i].x, of[i].n, of[i].heads, head_dim);
+    ZX_REQUIRE(!meets, "cross_attention_backward: dq, dk and dv must not lie in each other's memory or the inputs'");
+  }
   const hipStream_t st = as_stream(stream);
   uint16_t *d = static_cast<uint16_t *>(dq);
   if (dtype == ZX_BF16)

@@ -1376,7 +1376,8 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: tor
     bound a sequence's rows and keys (read back without them, which waits for the device); rows
     and keys beyond them are not computed or seen.  Rows that are not computed, those in no sequence
     among them, are left as they are in ``out``, or become zeros with ``zero_rest``; a row without a
-    key is zeros.  ``return_lse``: also float32
+    key is zeros.  ``out`` may be ``q`` itself, and must not lie in the memory of its inputs otherwise
+    (from a tensor's first element to its last).  ``return_lse``: also float32
     ``[Hq, n_q]``, log2 of each computed row's sum of exponentials (what ``cross_attention_backward``
     takes).
     autograd does not see this call: ``train.cross_attention.CrossAttention`` is the
@@ -1392,8 +1393,6 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: tor
         if out.shape != q.shape or out.dtype != q.dtype:
             raise ValueError(f"out must be {q.dtype} {tuple(q.shape)}")
         _all_on(index, out=out)
-        if any(t.untyped_storage().data_ptr() == out.untyped_storage().data_ptr() for t in (k, v) if t.numel()):
-            raise ValueError("out must not lie in k's or v's memory")
     lse = torch.empty((Hq, n_q), dtype=torch.float32, device=q.device) if return_lse else None
     with _on(index):
         ws, nb = _workspace_for("zx_cross_attention_workspace_bytes", index, n_q, Hq, Hkv, D, B, mq, mk)
