@@ -1,0 +1,94 @@
+"""What a cache knows of its pages and rows around forks, without a GPU: the cache lies in host memory and
+nothing is launched."""
+import copy
+
+import pytest
+import torch
+
+from zenyx_amd import kv
+from zenyx_amd.train.fp8_kv_quantization import PagedFP4KVCache, PagedFP8KVCache
+
+HOST = torch.device("cpu")
+
+
+def held(c, ids, lengths):
+    """The cache with sequences of so many tokens, as appends would leave it."""
+    entries = []
+    for s, n in zip(ids, lengths):
+        c._reserve(s, n, [], entries)
+        c.lengths[s] = n
+        c._len[c._row_of(s)] = n
+    c._write_entries(entries)
+    return c
+
+
+def state(c):
+    """Free pages, pages, lengths, users of pages, what is known to be shared, and table rows by sequence."""
+    return (*copy.deepcopy((c._free, c.pages, c.lengths, c._users)), {s: sorted(k.values()) for s, k in c._common.items() if k},
+            [(s, c._bt[r].tolist(), int(c._len[r])) for s, r in c._row.items()])
+
+
+class Stop(Exception):
+    pass
+
+
+@pytest.fixture
+def streams(monkeypatch):
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda *a: None)
+
+
+def failing(name, calls):
+    """`name` of the module of kernels or of the cache, which raises at its call number `calls`."""
+    def make(monkeypatch, c):
+        where = kv if hasattr(kv, name) else c
+        real, left = getattr(where, name), [calls]
+
+        def f(*a, **k):
+            left[0] -= 1
+            if left[0] == 0:
+                raise Stop
+            return real(*a, **k)
+        monkeypatch.setattr(where, name, f)
+    return make
+
+
+@pytest.mark.parametrize("C", [PagedFP8KVCache, PagedFP4KVCache])
+@pytest.mark.parametrize("fault", [("tier_move_pages", 1), ("_write_entries", 1), ("_row_of", 1), ("_row_of", 3), ("_grow", 1)])
+def test_a_fork_that_fails_leaves_the_cache_as_it_was(monkeypatch, streams, C, fault):
+    """Pages, rows, tables and what is known of shared pages; the same fork then succeeds."""
+    c = held(C(2, 1, 64, 60, 16, device=HOST), ["p", "r"], [40, 100])
+    monkeypatch.setattr(kv, "tier_move_pages", lambda *a, **k: None)
+    c.fork("p", ["x", "y"], length=32)
+    ids = [f"n{i}" for i in range(14)]  # (more rows than the tables have at first)
+    c._tables(["n1"])  # a row that a question about a sequence left behind
+    before = state(c)
+    with monkeypatch.context() as m:
+        failing(*fault)(m, c)
+        with pytest.raises(Stop):
+            c.fork("p", ids)
+    # (an id that is not in the cache need not keep its row; a table that has grown stays wide)
+    after = state(c)
+    assert after[:5] == before[:5]
+    assert [x for x in after[5] if x[0] != "n1"] == [x for x in before[5] if x[0] != "n1"]
+    assert set(c._row) - {"n1"} == {"p", "r", "x", "y"}
+    assert sorted([*c._row.values(), *c._free_rows]) == list(range(len(c._row) + len(c._free_rows)))
+    for r in c._free_rows:
+        assert (c._bt[r] == -1).all() and c._len[r] == 0
+    c.fork("p", ids)
+    assert all(c.lengths[s] == 40 and c.pages[s][:2] == c.pages["p"][:2] for s in ids)
+    for s in ["p", "r", "x", "y", *ids]:
+        c.free(s)
+    assert sorted(c._free) == list(range(60)) and not c._users and not c._common
+
+
+def test_forks_share_whole_pages(monkeypatch, streams):
+    moved = []
+    monkeypatch.setattr(kv, "tier_move_pages", lambda dst, src, d, s, size, stream: moved.append((d.tolist(), s.tolist(), size)))
+    c = held(PagedFP8KVCache(2, 1, 64, 30, 16, device=HOST), ["p"], [40])
+    c.fork("p", ["a", "b"])
+    size = c.pool[0, 0].numel()
+    (d, s, n), = moved
+    assert n == size and s == [(layer * 30 + c.pages["p"][2]) * size for layer in range(2) for _ in "ab"]
+    assert d == [(layer * 30 + c.pages[x][2]) * size for layer in range(2) for x in "ab"]
+    assert c._tables(["p", "a", "b"])[:, :2].unique(dim=0).shape[0] == 1
+    assert c._lengths(["a", "b"]).tolist() == [40, 40]

@@ -390,19 +390,25 @@ class PagedFP8KVCache:
             raise MemoryError("PagedFP8KVCache: out of pages")
         src = self.pages.get(seq_id, [])
         copies = [self._free.pop() for _ in new_ids] if rest else []
-        rows = [self._row_of(s) for s in new_ids]  # (may grow the tables)
-        self._rows_cache = ((), None)
-        at = torch.tensor(rows, dtype=torch.int64).to(self.device)
-        if whole:
-            self._bt[at, :whole] = self._bt[self._row[seq_id], :whole].clone()
-        self._len[at] = n
-        if rest:
-            self._write_entries([(r, whole, p) for r, p in zip(rows, copies)])
-            moves = [(layer * self.num_pages + p, layer * self.num_pages + src[whole])
-                     for layer in range(self.L) for p in copies]
-            dst, org = torch.tensor(moves, dtype=torch.int64).t().contiguous().to(self.device) * size
-            kv.tier_move_pages(self.pool, self.pool, dst, org, size,
-                               stream=torch.cuda.current_stream(self.device))
+        try:
+            rows = [self._row_of(s) for s in new_ids]  # (may grow the tables)
+            self._rows_cache = ((), None)
+            at = torch.tensor(rows, dtype=torch.int64).to(self.device)
+            if whole:
+                self._bt[at, :whole] = self._bt[self._row[seq_id], :whole].clone()
+            self._len[at] = n
+            if rest:
+                self._write_entries([(r, whole, p) for r, p in zip(rows, copies)])
+                moves = [(layer * self.num_pages + p, layer * self.num_pages + src[whole])
+                         for layer in range(self.L) for p in copies]
+                dst, org = torch.tensor(moves, dtype=torch.int64).t().contiguous().to(self.device) * size
+                kv.tier_move_pages(self.pool, self.pool, dst, org, size,
+                                   stream=torch.cuda.current_stream(self.device))
+        except BaseException:
+            self._free.extend(reversed(copies))
+            for s in new_ids:
+                self._drop_row(s)
+            raise
         known = self._common.setdefault(seq_id, {})
         if whole and whole not in known.values():
             known[object()] = whole
