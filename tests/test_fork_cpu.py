@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from zenyx_amd import kv
-from zenyx_amd.train.fp8_kv_quantization import PagedFP4KVCache, PagedFP8KVCache
+from zenyx_amd.train.fp8_kv_quantization import PagedFP4KVCache, PagedFP8KVCache, QuantizedRingAttention
 
 HOST = torch.device("cpu")
 
@@ -92,3 +92,23 @@ def test_forks_share_whole_pages(monkeypatch, streams):
     assert d == [(layer * 30 + c.pages[x][2]) * size for layer in range(2) for x in "ab"]
     assert c._tables(["p", "a", "b"])[:, :2].unique(dim=0).shape[0] == 1
     assert c._lengths(["a", "b"]).tolist() == [40, 40]
+
+
+def test_batches_that_the_kernel_of_shared_pages_refuses_take_the_usual_one(monkeypatch, streams):
+    """More than 65,535 sequences, or more units of 128 positions than 32 bits count: prefill takes both."""
+    c = held(PagedFP8KVCache(1, 1, 64, 8, 16, device=HOST), ["p"], [32])
+    ids = list(range(65536))
+    c.fork("p", ids)
+    assert c._groups(ids[:-1]) is not None and c._groups(ids) is None
+    taken = []
+    monkeypatch.setattr(kv, "ring_attention_fp8", lambda q, *a, **k: taken.append("usual") or q)
+    monkeypatch.setattr(kv, "paged_attention_shared", lambda q, *a, **k: taken.append("shared") or q)
+    att = QuantizedRingAttention(c, check=False)
+    att(torch.zeros((len(ids), 1, 64), dtype=torch.bfloat16), 0, ids, [1] * len(ids))
+    assert taken == ["usual"]
+    c = held(PagedFP8KVCache(1, 1, 64, 40, 1024, device=HOST), ["p"], [1024])
+    ids = list(range(2000))
+    c.fork("p", ids)
+    assert c._groups(ids) is not None
+    c._grow(width=1 << 14)  # 16 M positions a table, 128 K units
+    assert c._groups(ids) is None

@@ -429,6 +429,11 @@ class PagedFP8KVCache:
         where reading those once saves too little (or no kernel has the shape)."""
         if not self._common or self.D not in (64, 128, 256) or self.P % 16:
             return None
+        # what that kernel takes: up to 65,535 sequences, and units of 128 positions (of at most 8 rows of each
+        # sequence, and of the groups) counted in 32 bits
+        n = len(seq_ids)
+        if n > 65535 or 9 * n * -(-self._bt.shape[1] * self.P // 128) >= 1 << 31:
+            return None
         key = tuple(seq_ids)
         if self._groups_cache[0] != key:
             starts, shared = [], []
