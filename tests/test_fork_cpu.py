@@ -112,3 +112,51 @@ def test_batches_that_the_kernel_of_shared_pages_refuses_take_the_usual_one(monk
     assert c._groups(ids) is not None
     c._grow(width=1 << 14)  # 16 M positions a table, 128 K units
     assert c._groups(ids) is None
+
+
+def shared_positions(C, Hkv, D, n, pages, P=16):
+    """n forks of a sequence of so many pages, and their ids."""
+    c = held(C(1, Hkv, D, pages + 2, P, device=HOST), ["p"], [pages * P])
+    ids = [f"f{i}" for i in range(n)]
+    c.fork("p", ids)
+    return c, ids
+
+
+@pytest.mark.parametrize("C, Hkv, D, n, pages, q_heads, rows, pays", [
+    # what reading once saves is counted in bytes: 96 MiB over FP8 pages of 8 x 128, ...
+    (PagedFP8KVCache, 8, 128, 25, 128, 32, 1, True), (PagedFP8KVCache, 8, 128, 24, 128, 32, 1, False),
+    # ... of fewer heads more positions, of more heads fewer
+    (PagedFP8KVCache, 2, 128, 25, 128, 8, 1, False), (PagedFP8KVCache, 2, 128, 97, 128, 8, 1, True),
+    (PagedFP8KVCache, 1, 64, 97, 256, 4, 1, False), (PagedFP8KVCache, 32, 128, 7, 128, 32, 1, True),
+    # 4 bits: 17/32 of the bytes
+    (PagedFP4KVCache, 8, 128, 25, 128, 32, 1, False), (PagedFP4KVCache, 8, 128, 47, 128, 32, 1, True),
+    # several rows, FP8: as one; heads that no other kernel takes
+    (PagedFP8KVCache, 8, 128, 25, 128, 32, 8, True), (PagedFP8KVCache, 8, 128, 24, 128, 32, 8, False),
+    (PagedFP8KVCache, 1, 64, 2, 1, 4, 2, True),
+    # 4 bits: in proportion to a sequence's columns, and not for very many of them
+    (PagedFP4KVCache, 8, 128, 25, 512, 32, 2, True), (PagedFP4KVCache, 8, 128, 25, 512, 32, 8, False),
+    (PagedFP4KVCache, 8, 128, 25, 2048, 32, 8, True), (PagedFP4KVCache, 8, 128, 97, 512, 32, 4, False),
+    (PagedFP4KVCache, 8, 128, 47, 256, 8, 4, True)])
+def test_sharing_is_taken_where_it_saves_bytes_enough(monkeypatch, streams, C, Hkv, D, n, pages, q_heads, rows, pays):
+    c, ids = shared_positions(C, Hkv, D, n, pages)
+    assert c._groups(ids) is not None  # (what is shared is known whether it pays or not)
+    taken = []
+    for name in ("ring_attention_fp8", "paged_attention4_prefill", "paged_attention_decode", "paged_attention4_decode"):
+        monkeypatch.setattr(kv, name, lambda q, *a, **k: taken.append(False) or q)
+    for name in ("paged_attention_shared", "paged_attention4_shared"):
+        monkeypatch.setattr(kv, name, lambda q, *a, **k: taken.append(True) or q)
+    att = QuantizedRingAttention(c, check=False)
+    q = torch.zeros((n * rows, q_heads, D), dtype=torch.bfloat16)
+    att.decode(q, 0, ids) if rows == 1 else att(q, 0, ids, [rows] * n)
+    assert taken == [pays]
+
+
+def test_what_is_known_of_a_batch_follows_it(monkeypatch, streams):
+    c, ids = shared_positions(PagedFP8KVCache, 8, 128, 30, 128)
+    assert c._sharing_pays(ids, 1, 32) and not c._sharing_pays(ids[:20], 1, 32) and c._sharing_pays(ids, 1, 32)
+    first = c._groups(ids)
+    assert c._groups(ids) is first and first[0].tolist() == [0, 30] and first[1].tolist() == [2048]
+    for s in ids[20:]:
+        c.free(s)
+    assert c._groups(ids)[0].tolist() == [0, 20, *range(21, 31)] and not c._sharing_pays(ids, 1, 32)
+    assert c._groups([ids[0]]) is None and not c._sharing_pays([], 1, 32)

@@ -77,9 +77,14 @@ class PagedFP8KVCache:
     undoes its own faulty append (lengths, pages, scales) before raising."""
 
     _ERR_WORDS = 64
-    # Positions that reading shared pages once has to save a batch for the kernel that does it, which costs
-    # 5 us more to start (decode's / this one's time, 32/8 heads, D = 128: 16 sequences on 2,048 shared
-    # positions 20.2 / 20.2 us, on 4,096 28 / 23, 4 on 16,384 30 / 26, 64 on 16,384 244 / 50).
+    # Positions of 2 KB (8 KV heads of 128 over FP8 pages) that reading shared pages once has to save a
+    # batch for the kernel that does it, which costs 5 us more to start: 96 MiB, whatever the heads and the
+    # format.  Decode's / that kernel's time where 100 MB are saved, for 4, 16 and 64 sequences: FP8 pages,
+    # 32/8 heads of 128 30 / 27, 25 / 23, 19 / 24 us (twice as much: 48 / 33, 35 / 30, 35 / 30), 32/32 of 128
+    # 23 / 21, 21 / 17, 21 / 30, 32/32 of 64 23 / 22, 21 / 16, 20 / 26, 8/2 of 128 32 / 45, 25 / 29, 25 / 23; 4
+    # bits, 32/8 of 128 30 / 29, 27 / 29, 26 / 26, 12/12 of 64 29 / 26, 26 / 18, 24 / 19.  Where 25 MB are, 8/2
+    # heads of 128 over FP8 pages: 20 / 27, 15 / 20, 16 / 19.  Several rows of each sequence, FP8 (prefill's
+    # time): 32/8 heads, 4 rows, 100 MB 80 / 37, 63 / 40, 58 / 45.
     _LEAST_SAVED = 49152
     _SHARED_PRECISIONS = ("f16", "bf16")  # of QuantizedRingAttention's, those that kernel has the bits for
 
@@ -116,7 +121,7 @@ class PagedFP8KVCache:
         # sequence how many of its first pages it has in common with the others of a fork
         self._users: dict = {}    # page id -> sequences, 2 or more
         self._common: dict = {}   # seq id -> {fork: pages}
-        self._groups_cache: tuple = ((), None)  # (seq_ids, groups) of the last call
+        self._groups_cache: tuple = (None, None, None)  # (seq_ids, _sharing, _groups) of the last call
         self._ones_cache: dict = {}  # n -> device int32 ones [n] / arange [n + 1] (one-token steps)
 
     # ---------------------------------------------------------------- the pages' format
@@ -251,7 +256,7 @@ class PagedFP8KVCache:
                 self._drop_row(seq_id)
 
     def _drop_row(self, seq_id) -> None:
-        self._groups_cache = ((), None)
+        self._groups_cache = (None, None, None)
         r = self._row.pop(seq_id, None)
         if r is None:
             return
@@ -424,38 +429,58 @@ class PagedFP8KVCache:
         x, y = self._common.get(a), self._common.get(b)
         return max((min(k, y[f]) for f, k in x.items() if f in y), default=0) if x and y else 0
 
-    def _groups(self, seq_ids):
-        """Device (int32 cu_group, int32 shared tokens) of a batch's neighbours that share pages, or None
-        where reading those once saves too little (or no kernel has the shape)."""
-        if not self._common or self.D not in (64, 128, 256) or self.P % 16:
-            return None
-        # what that kernel takes: up to 65,535 sequences, and units of 128 positions (of at most 8 rows of each
-        # sequence, and of the groups) counted in 32 bits
-        n = len(seq_ids)
-        if n > 65535 or 9 * n * -(-self._bt.shape[1] * self.P // 128) >= 1 << 31:
-            return None
-        key = tuple(seq_ids)
-        if self._groups_cache[0] != key:
+    def _sharing(self, seq_ids: tuple):
+        """(where groups begin and end, shared tokens of each, positions of 2 KB that reading those once
+        saves, sequences of the largest group) of a batch's neighbours that share pages; kept for a
+        repeated batch."""
+        if self._groups_cache[0] != seq_ids:
             starts, shared = [], []
-            for i, s in enumerate(key):
-                c = self._shared_pages(key[starts[-1]], s) if i else 0
+            for i, s in enumerate(seq_ids):
+                c = self._shared_pages(seq_ids[starts[-1]], s) if i else 0
                 # (a neighbour that shares little of what the others do begins a group of its own)
                 if c and (shared[-1] is None or 2 * c >= shared[-1]):
                     shared[-1] = c if shared[-1] is None else min(shared[-1], c)
                 else:
                     starts.append(i)
                     shared.append(None)
-            bounds = starts + [len(key)]
+            bounds = starts + [len(seq_ids)]
             tokens = [0 if n is None else n * self.P for n in shared]
-            saved = sum((b - a - 1) * n for a, b, n in zip(bounds, bounds[1:], tokens))
-            groups = None
-            if saved >= self._LEAST_SAVED:
-                w = (len(bounds) + 3) // 4 * 4  # each row 16-byte aligned
-                t = torch.tensor([bounds + [0] * (w - len(bounds)), tokens + [0] * (w - len(tokens))],
-                                 dtype=torch.int32).to(self.device)
-                groups = t[0, :len(bounds)], t[1, :len(tokens)]
-            self._groups_cache = (key, groups)
+            token = self.pool.stride(1) // self.P  # its bytes in a layer
+            saved = sum((b - a - 1) * n for a, b, n in zip(bounds, bounds[1:], tokens)) * token / 2048
+            most = max((b - a for a, b, n in zip(bounds, bounds[1:], tokens) if n), default=0)
+            self._groups_cache = (seq_ids, (bounds, tokens, saved, most), None)
         return self._groups_cache[1]
+
+    def _can_share(self, n: int) -> bool:
+        """Whether the kernel of shared pages takes n sequences of this cache: up to 65,535, and units of
+        128 positions (of at most 8 rows of each sequence, and of the groups) counted in 32 bits."""
+        return self.D in (64, 128, 256) and self.P % 16 == 0 and n <= 65535 and \
+            9 * n * -(-self._bt.shape[1] * self.P // 128) < 1 << 31
+
+    def _sharing_pays(self, seq_ids, rows: int, q_heads: int) -> bool:
+        """Whether that kernel is the faster one for up to ``rows`` rows of each sequence."""
+        if not self._common:
+            return False
+        _, _, saved, most = self._sharing(tuple(seq_ids))
+        return saved > 0 and self._saves_enough(saved, rows, q_heads // self.H, most) and self._can_share(len(seq_ids))
+
+    def _saves_enough(self, saved: float, rows: int, group: int, n: int) -> bool:
+        """``saved``: in positions of 2 KB; ``group``: query heads per KV head; n: sequences of the largest group."""
+        # (several rows: no other kernel takes FP8 pages of heads that are not of 128)
+        return saved >= self._LEAST_SAVED or (rows > 1 and self.D != 128)
+
+    def _groups(self, seq_ids):
+        """Device (int32 cu_group, int32 shared tokens) of a batch's neighbours that share pages, or None
+        where none do (or no kernel has the shape)."""
+        if not self._common or not self._can_share(len(seq_ids)):
+            return None
+        bounds, tokens, saved, _ = self._sharing(tuple(seq_ids))
+        if saved and self._groups_cache[2] is None:
+            w = (len(bounds) + 3) // 4 * 4  # each row 16-byte aligned
+            t = torch.tensor([bounds + [0] * (w - len(bounds)), tokens + [0] * (w - len(tokens))],
+                             dtype=torch.int32).to(self.device)
+            self._groups_cache = (*self._groups_cache[:2], (t[0, :len(bounds)], t[1, :len(tokens)]))
+        return self._groups_cache[2]
 
 
 class PagedFP4KVCache(PagedFP8KVCache):
@@ -465,6 +490,8 @@ class PagedFP4KVCache(PagedFP8KVCache):
     ``head_dim`` 64, 128 or 256, ``page_size`` a multiple of 16.  ``scales`` is None."""
 
     _SHARED_PRECISIONS = ("f16", "bf16", "exact")
+    # Columns (query rows and heads) of a group up to which the kernel of shared pages is taken for several rows
+    _MOST_COLUMNS = 1024
 
     def __init__(self, num_layers: int, num_kv_heads: int, head_dim: int, num_pages: int, page_size: int = 16,
                  device: torch.device | None = None, rope=None):
@@ -496,6 +523,17 @@ class PagedFP4KVCache(PagedFP8KVCache):
         cu_group, shared = groups
         return kv.paged_attention4_shared(q, self.pool[layer], tables, lens, cu_group, shared, cu_q=cu,
                                           max_q_per_seq=max_q, causal=att.causal, sm_scale=att.sm_scale, check=att.check)
+
+    def _saves_enough(self, saved: float, rows: int, group: int, n: int) -> bool:
+        # With several rows prefill has up to 48 columns for a key that it converts too: what sharing saves has
+        # to be more in proportion to a sequence's columns beyond 4.  (Prefill's / the other kernel's time, 32/8
+        # heads of 128, for 4, 8, 24 sequences: 2 rows, 214 MB saved 61 / 40, 47 / 42, 43 / 38 us; 4 rows, 428 MB
+        # 112 / 114, 95 / 75, 78 / 70, and 96 sequences, 1,536 columns, 72 / 136; 8 rows, 214 MB 76 / 80, 69 / 74, 68 /
+        # 82, 856 MB 279 / 243, 234 / 220, 225 / 227, and 96 sequences 197 / 603.)
+        if rows == 1:
+            return saved >= self._LEAST_SAVED
+        columns = rows * group
+        return saved >= self._LEAST_SAVED * max(1, columns / 4) and n * columns <= self._MOST_COLUMNS
 
     def _gather(self, layer: int, tables, lens, out_len: int):
         return kv.kv4_gather_dequant(self.pool[layer], tables, lens, out_len)
@@ -537,8 +575,11 @@ class QuantizedRingAttention:
         # and errors surface at the cache's next check_errors
         self.check = check
 
-    def _groups(self, seq_ids: list):
-        return self.cache._groups(seq_ids) if self.precision in self.cache._SHARED_PRECISIONS else None
+    def _groups(self, q: torch.Tensor, seq_ids: list, rows: int):
+        c = self.cache
+        if self.precision not in c._SHARED_PRECISIONS or not c._sharing_pays(seq_ids, rows, q.shape[1]):
+            return None
+        return c._groups(seq_ids)
 
     def __call__(self, q: torch.Tensor, layer: int, seq_ids: list, q_lens: list[int]) -> torch.Tensor:
         """q ``[n_q, Hq, D]`` bf16: the queries of ``seq_ids[i]`` packed in order, ``q_lens[i]``
@@ -557,7 +598,7 @@ class QuantizedRingAttention:
             q = c.rope(q, shift + torch.arange(q.shape[0], dtype=torch.int32, device=q.device))
         most = max(q_lens, default=0)
         # few rows per sequence (proposed tokens): bound by what they read of shared pages
-        groups = self._groups(seq_ids) if 0 < most <= self._FEW_ROWS else None
+        groups = self._groups(q, seq_ids, most) if 0 < most <= self._FEW_ROWS else None
         if groups is not None:
             out = c._attend_shared(q, layer, c._tables(seq_ids), lens, groups, self, cu, most)
         else:
@@ -572,7 +613,7 @@ class QuantizedRingAttention:
         q, lens = q.to(c.device).contiguous(), c._lengths(seq_ids)
         if c.rope is not None:
             q = c.rope(q, lens - 1)
-        groups = self._groups(seq_ids)
+        groups = self._groups(q, seq_ids, 1)
         if groups is not None:
             out = c._attend_shared(q, layer, c._tables(seq_ids), lens, groups, self)
         else:
