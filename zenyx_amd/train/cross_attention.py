@@ -10,13 +10,15 @@ import torch.autograd.forward_ad as fwAD
 from .. import kv
 
 
-def _strided(t: torch.Tensor) -> torch.Tensor:
-    """``t`` as the kernels take it: the caller has no say in how autograd lays a gradient out."""
+def _strided(t: torch.Tensor, group: int) -> torch.Tensor:
+    """``t`` as the kernels take it (``group`` heads per KV head): the caller has no say in how autograd lays a
+    gradient out."""
     vec = 16 // t.element_size()
-    if t.stride(-1) == 1 and not (t.stride(0) % vec or t.stride(1) % vec or t.data_ptr() % 16):
+    row, head, channel = t.stride()
+    if channel == 1 and not (row % vec or head % vec or t.data_ptr() % 16) and row < 1 << 23 and \
+            (group == 1 or head < (1 << 29) // group):
         return t
-    t = t.contiguous()
-    return t.clone() if t.data_ptr() % 16 else t
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 class _Cross(torch.autograd.Function):
@@ -32,8 +34,9 @@ class _Cross(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
         q, k, v, out, lse, cu_q, cu_k, k_lens = ctx.saved_tensors
-        dq, dk, dv = kv.cross_attention_backward(_strided(grad), q, k, v, out, lse, cu_q, cu_k, k_lens=k_lens,
-                                                 sm_scale=ctx.sm_scale, max_q_per_seq=ctx.max_q, max_k_per_seq=ctx.max_k)
+        grad = _strided(grad, q.shape[1] // k.shape[1])
+        dq, dk, dv = kv.cross_attention_backward(grad, q, k, v, out, lse, cu_q, cu_k, k_lens=k_lens, sm_scale=ctx.sm_scale,
+                                                 max_q_per_seq=ctx.max_q, max_k_per_seq=ctx.max_k)
         return dq, dk, dv, None, None, None, None, None, None
 
 
