@@ -26,3 +26,30 @@ def test_strides_of_single_rows_and_heads(shape, strides):
     got = ca._strided(t, 1)
     assert torch.equal(got.view(torch.int16), t.view(torch.int16))
     assert got.stride() == (shape[1] * 64, 64, 1) and got.data_ptr() % 16 == 0
+
+
+def test_errors_can_be_seen(monkeypatch):
+    """err reaches the forward pass and the gradients, check the forward pass, with and without autograd."""
+    seen = []
+
+    def forward(q, k, v, cu_q, cu_k, return_lse=False, **kw):
+        seen.append(("forward", kw["check"], kw["err"]))
+        return (torch.zeros_like(q), torch.zeros(q.shape[1], q.shape[0])) if return_lse else torch.zeros_like(q)
+
+    def backward(grad, q, k, v, out, lse, cu_q, cu_k, err=None, **kw):
+        seen.append(("backward", False, err))
+        return torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v)
+    monkeypatch.setattr(kv, "cross_attention", forward)
+    monkeypatch.setattr(kv, "cross_attention_backward", backward)
+    q, k = torch.zeros(3, 2, 64, dtype=torch.bfloat16), torch.zeros(5, 2, 64, dtype=torch.bfloat16)
+    cu_q, cu_k = (torch.tensor([0, n], dtype=torch.int32) for n in (3, 5))
+    err = torch.zeros(1, dtype=torch.int32)
+    attend = ca.CrossAttention()
+    for kw, want in (({}, (False, None)), (dict(check=True), (True, None)), (dict(err=err), (False, err)),
+                     (dict(err=err, check=True), (True, err))):
+        attend(q, k, k, cu_q, cu_k, **kw)
+        attend(q.clone().requires_grad_(), k, k, cu_q, cu_k, **kw).sum().backward()
+        (a, check, e), (b, check2, e2), (c, _, e3) = seen
+        assert (a, b, c) == ("forward", "forward", "backward") and check == check2 == want[0]
+        assert e is want[1] and e2 is want[1] and e3 is want[1]
+        del seen[:]

@@ -100,3 +100,24 @@ def test_out_in_memory_that_inputs_have_parts_of(dev):
     with pytest.raises(ValueError, match="memory"):
         kv.cross_attention(wide[:, :2], k, v, cu_q, cu_k, out=wide.flatten()[:q.numel()].view(q.shape))
     assert torch.equal(kv.cross_attention(parts[0], k, v, cu_q, cu_k, out=parts[0]), want)
+
+
+def test_cross_attention_module_reports_bounds(dev):
+    q, k, v, g = inputs(dev, torch.bfloat16, [5, 9], [70, 30], 4, 2, 64, 61)
+    cu_q, cu_k = starts([5, 9], dev), starts([70, 30], dev)
+    attend, leaf = CrossAttention(), q.clone().requires_grad_()
+    for x in (q, leaf):
+        assert attend(x, k, v, cu_q, cu_k, check=True).shape == q.shape
+        with pytest.raises(ValueError, match="position"):
+            attend(x, k, v, cu_q, cu_k, max_q_per_seq=6, max_k_per_seq=70, check=True)
+        with pytest.raises(ValueError, match="err"):
+            attend(x, k, v, cu_q, cu_k, err=torch.zeros(1, device=dev))
+    err = torch.zeros(1, dtype=torch.int32, device=dev)
+    y = attend(leaf, k, v, cu_q, cu_k, max_q_per_seq=9, max_k_per_seq=69, err=err)
+    assert int(err) == N.ZX_KERR_POS_RANGE
+    err.zero_()
+    y.backward(g)
+    assert int(err) == N.ZX_KERR_POS_RANGE
+    err.zero_()
+    attend(leaf, k, v, cu_q, cu_k, max_q_per_seq=9, max_k_per_seq=70, err=err).backward(g)
+    assert int(err) == 0
