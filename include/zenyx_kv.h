@@ -573,8 +573,8 @@ int zx_paged_attention4_prefill(const uint16_t *q, int64_t n_q, const int32_t *c
  * ZX_KERR_POS_RANGE, as lengths beyond max_blocks * page_size, which are clipped, and groups that
  * are out of order do); keys on a page outside [0, n_pages) are left out and set
  * ZX_KERR_PAGE_RANGE.  head_dim 64, 128 or 256, page_size a multiple of 16; scores and sums in fp32.
- * FP8: scales [2][n_kv_heads]; softmax weights rounded once to fp16 (times 2^7; the row sums use
- * the same): |error| <= one bf16 ulp + 2^-10 max|V|.  4 bits: weights as bf16 hi + lo, one ulp +
+ * FP8: scales [2][n_kv_heads]; softmax weights rounded once to fp16 (times 2^7; the row sums add the
+ * rounded ones or, over 128 columns of a group, the fp32 ones): |error| <= one bf16 ulp + 2^-10 max|V|.  4 bits: weights as bf16 hi + lo, one ulp +
  * 2^-15 max|V|.  A NaN value reaches the rows that see it.  workspace: the query's device bytes,
  * 16-byte aligned, for min(max_q_per_seq, n_q) rows per sequence (1 without cu_q); it holds nothing
  * between calls. */

@@ -449,7 +449,9 @@ template <bool F16> __device__ __forceinline__ void sh_codes(uint4 c, att_u32x4 
   }
 }
 
-// Up to 128 columns on keys [t_begin, t_end) of FP8 pages, all of which every row sees.  A wave has 32
+// Up to 128 columns on keys [t_begin, t_end) of FP8 pages, all of which every row sees.  The row sums add the
+// weights before they are rounded (AttnWave: after): the rounding then moves a row by 2^-11 max|V|, half of
+// what it does where both of the quotient's parts have it.  A wave has 32
 // columns, and the four share tiles of 64 keys in LDS: a key is read and converted once per 128
 // columns, where AttnWave's waves, with 48 columns and keys of their own, convert it for each 48 (D =
 // 128, 64 sequences on 2,048 shared positions and 100-2,000 of their own 53 us, so 46; the other way
@@ -594,9 +596,11 @@ constexpr int SH_WIDE = SW_COLS / AW_COLS;
 __host__ __device__ constexpr int sh_most_tiles(int bits, int D) {
   return D == 256 ? 1 : D == 64 ? 4 : bits == 8 ? SH_WIDE : 3;
 }
-// Blocks per CU by the registers, and (D = 128) by LDS.  (Four at D = 64 with one tile spilled 14 to 32
-// registers: 8 groups of 2 sequences on 8,000 shared positions, 12 heads, 34.2 against 28.7 us, of 8 on
-// 400 and up to 2,000 of their own 34.1 against 31.3, of 16 the other way, 47.6 against 52.1.)
+// Blocks per CU by the registers, and (D = 128) by LDS.  (Four at D = 64 with one tile.  FP8 pages, where they
+// spill 14 to 32 registers: 8 groups of 2 sequences on 8,000 shared positions, 12 heads, 34.2 against 28.7
+// us, of 8 on 400 and up to 2,000 of their own 34.1 against 31.3, of 16 the other way, 47.6 against 52.1.  4
+// bits, where none spill: of 2 on 8,000 30.0 against 28.1, of 8 on 400 and 1,000 of their own 30.5 against
+// 27.0, one of 16 on 16,000 24.1 against 20.9, 8 of 16 on 4,000 and 300 the other way, 34.9 against 36.5.)
 __host__ __device__ constexpr int sh_per_cu(int D, int CT) { return D * CT > 128 ? 2 : 3; }
 
 // CTO: column tiles of a sequence's own keys.  ROWS: several rows per sequence.

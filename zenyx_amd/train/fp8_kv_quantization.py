@@ -86,7 +86,9 @@ class PagedFP8KVCache:
     # heads of 128 over FP8 pages: 20 / 27, 15 / 20, 16 / 19.  Several rows of each sequence, FP8 (prefill's
     # time): 32/8 heads, 4 rows, 100 MB 80 / 37, 63 / 40, 58 / 45.
     _LEAST_SAVED = 49152
-    _SHARED_PRECISIONS = ("f16", "bf16")  # of QuantizedRingAttention's, those that kernel has the bits for
+    # Of QuantizedRingAttention's precisions those that kernel has the bits for; decode, which computes in
+    # fp32 whatever is asked for, gives some up with them
+    _SHARED_PRECISIONS = ("f16", "bf16")
 
     def __init__(self, num_layers: int, num_kv_heads: int, head_dim: int, num_pages: int,
                  page_size: int = 16, device: torch.device | None = None, overflow: str = "raise", rope=None):
@@ -553,8 +555,9 @@ class QuantizedRingAttention:
     of a ring's shards), and ``precision`` "f16" is given as "exact": the 4-bit kernels have no
     fp16 weights, and "bf16" has fewer bits.  Neighbours of a batch that share pages
     (``PagedFP8KVCache.fork``) attend to them together, in ``decode`` and in calls of few rows per
-    sequence: the shared keys are read and multiplied once for all of them (over FP8 pages not with
-    "exact", whose weights have more bits).  A cache with ``rope`` has rotated its keys: the queries
+    sequence, where that saves enough: the shared keys are read and multiplied once for all of them.
+    Over FP8 pages ``decode`` then rounds its softmax weights to fp16 (one bf16 ulp + 2^-10 max|V|), which
+    it does not for sequences by themselves; with "exact" every sequence is taken by itself.  A cache with ``rope`` has rotated its keys: the queries
     are rotated here, by the positions of the tokens they stand for."""
 
     _FEW_ROWS = 8  # of a sequence, for which shared pages are attended to together
