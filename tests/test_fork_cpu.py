@@ -160,3 +160,16 @@ def test_what_is_known_of_a_batch_follows_it(monkeypatch, streams):
         c.free(s)
     assert c._groups(ids)[0].tolist() == [0, 20, *range(21, 31)] and not c._sharing_pays(ids, 1, 32)
     assert c._groups([ids[0]]) is None and not c._sharing_pays([], 1, 32)
+
+
+def test_queries_of_any_shape_reach_the_kernels_wrapper(monkeypatch, streams):
+    """Which checks them: their shape is nobody else's business, with forks or without."""
+    c = held(PagedFP8KVCache(1, 1, 64, 8, 16, device=HOST), ["p"], [32])
+    seen = []
+    monkeypatch.setattr(kv, "paged_attention_decode", lambda q, *a, **k: seen.append(q.dim()) or q)
+    att = QuantizedRingAttention(c, check=False)
+    for ids in (["p"], ["p", "a"]):
+        for q in (torch.zeros(64), torch.zeros(1, 64), torch.zeros(1, 1, 1, 64)):
+            att.decode(q, 0, ids)
+        c.fork("p", ["a"]) if "a" not in c.lengths else None
+    assert seen == 2 * [1, 2, 4]

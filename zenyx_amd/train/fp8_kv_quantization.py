@@ -461,8 +461,6 @@ class PagedFP8KVCache:
 
     def _sharing_pays(self, seq_ids, rows: int, q_heads: int) -> bool:
         """Whether that kernel is the faster one for up to ``rows`` rows of each sequence."""
-        if not self._common:
-            return False
         _, _, saved, most = self._sharing(tuple(seq_ids))
         return saved > 0 and self._saves_enough(saved, rows, q_heads // self.H, most) and self._can_share(len(seq_ids))
 
@@ -580,7 +578,8 @@ class QuantizedRingAttention:
 
     def _groups(self, q: torch.Tensor, seq_ids: list, rows: int):
         c = self.cache
-        if self.precision not in c._SHARED_PRECISIONS or not c._sharing_pays(seq_ids, rows, q.shape[1]):
+        if not c._common or self.precision not in c._SHARED_PRECISIONS or q.dim() != 3 or \
+                not c._sharing_pays(seq_ids, rows, q.shape[1]):
             return None
         return c._groups(seq_ids)
 
