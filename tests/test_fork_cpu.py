@@ -173,3 +173,12 @@ def test_queries_of_any_shape_reach_the_kernels_wrapper(monkeypatch, streams):
             att.decode(q, 0, ids)
         c.fork("p", ["a"]) if "a" not in c.lengths else None
     assert seen == 2 * [1, 2, 4]
+
+
+def test_a_batch_asked_for_before_its_fork_was_made(monkeypatch, streams):
+    """An id that was not in the cache, and is a fork by the next call."""
+    c, ids = shared_positions(PagedFP8KVCache, 8, 128, 30, 128)
+    batch = [*ids, "later"]
+    assert c._groups(batch)[0].tolist() == [0, 30, 31]
+    c.fork("p", ["later"])
+    assert c._groups(batch)[0].tolist() == [0, 31]

@@ -399,6 +399,7 @@ class PagedFP8KVCache:
         copies = [self._free.pop() for _ in new_ids] if rest else []
         try:
             rows = [self._row_of(s) for s in new_ids]  # (may grow the tables)
+            self._groups_cache = (None, None, None)
             self._rows_cache = ((), None)
             at = torch.tensor(rows, dtype=torch.int64).to(self.device)
             if whole:
