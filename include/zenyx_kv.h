@@ -567,17 +567,18 @@ int zx_paged_attention4_prefill(const uint16_t *q, int64_t n_q, const int32_t *c
  * only those.  Rows [cu_q[b], cu_q[b + 1]) of q [n_q][n_q_heads][head_dim] bf16 are sequence b's
  * newest (cu_q NULL: a row each, n_q == n_seqs): row i of n, n as cu_q has it whatever the call
  * computes of them, is at position seq_lens[b] - n + i and sees, when `causal`, the keys up to it,
- * otherwise all seq_lens[b].  out is that of attention over every sequence's own table, whatever the sequences of a group have in common beyond it.
+ * otherwise all seq_lens[b].  out is that of attention over every sequence's own table, whatever the
+ * sequences of a group have in common beyond it.
  * n_groups may be 0.  A row without a key gives zeros; rows beyond max_q_per_seq (host) or in no
  * sequence are left unwritten, rows that cu_q claims beyond n_q do not exist (either sets
  * ZX_KERR_POS_RANGE, as lengths beyond max_blocks * page_size, which are clipped, and groups that
  * are out of order do); keys on a page outside [0, n_pages) are left out and set
  * ZX_KERR_PAGE_RANGE.  head_dim 64, 128 or 256, page_size a multiple of 16; scores and sums in fp32.
  * FP8: scales [2][n_kv_heads]; softmax weights rounded once to fp16 (times 2^7; the row sums add the
- * rounded ones or, over 128 columns of a group, the fp32 ones): |error| <= one bf16 ulp + 2^-10 max|V|.  4 bits: weights as bf16 hi + lo, one ulp +
- * 2^-15 max|V|.  A NaN value reaches the rows that see it.  workspace: the query's device bytes,
- * 16-byte aligned, for min(max_q_per_seq, n_q) rows per sequence (1 without cu_q); it holds nothing
- * between calls. */
+ * rounded ones or, over 128 columns of a group, the fp32 ones): |error| <= one bf16 ulp + 2^-10 max|V|.
+ * 4 bits: weights as bf16 hi + lo, one ulp + 2^-15 max|V|.  A NaN value reaches the rows that see it.
+ * workspace: the query's device bytes, 16-byte aligned, for min(max_q_per_seq, n_q) rows per sequence
+ * (1 without cu_q); it holds nothing between calls. */
 size_t zx_paged_attention_shared_workspace_bytes(int64_t n_q, int32_t n_seqs, int32_t n_groups, int32_t n_q_heads,
                                                  int32_t n_kv_heads, int32_t head_dim, int32_t page_size,
                                                  int32_t max_blocks, int32_t max_q_per_seq);
